@@ -1,0 +1,301 @@
+// Block tables and slot maps of a paged cache, built on the device from the lengths of a step's requests.
+//
+// The state is a row of block ids per slot (`tables`, of which the first `held` are the slot's) and a stack of free
+// blocks (`stack`, the first `count`).  A step's row i names slot s, which holds L tokens and brings n more:
+//
+//     need(x) = ceil(min(x, ring or x) / P)               blocks of P tokens that x tokens take up
+//     more_i  = max(0, need(L + n) - held[s])             taken from the top of the stack, rows in order
+//     pos     = L + j,  place = pos (% ring)              of its j-th new token
+//     row     = tables[s][place / P] * P + place % P      or -1 where pos / P + ring / P <= (L + n - 1) / P: the ring's
+//                                                         newest block has already taken that block's place
+//
+// A row with slot -1 is padding: its tokens get position and cache row -1, its length is 0.  All or nothing: where the
+// free blocks, a row of the tables or the outputs do not suffice, or a slot is wrong, the state stays as it is, every
+// output reads as padding (lengths and sums 0) and `status` says why.
+//
+// What bounds it is latency: a decode step of 64 rows reads and writes 2.6 KB.  One launch does all of it: every block of
+// threads of one cluster adds up all rows by itself (three short arrays out of the L2), which costs less than handing sums
+// around, the cluster's barrier then lets the state be written that all have read, and tokens and new table entries are
+// shared out.  A token's block is looked up in the stack where it is new, so nothing waits for the tables' new entries.
+#include "common.cuh"
+
+namespace {
+
+constexpr int THREADS = 1024;
+constexpr int MAX_ROWS = 4096;           // rows of a step: their sums lie in shared memory
+constexpr int MAX_SLOTS = 65536;         // a bit each: a slot named twice is found in shared memory
+
+enum : int { ST_OK = 0, ST_NO_BLOCKS = 1, ST_TABLE_WIDTH = 2, ST_TOO_MANY_TOKENS = 3, ST_BAD_ROW = 4 };
+
+struct ExtendArgs {
+    const int32_t *slots, *lengths, *fresh;        // of the step's rows
+    int32_t *tables, *held, *count;
+    const int32_t* stack;
+    int32_t *cu_q, *kv_len, *positions, *tok_seq, *cache_rows, *status;
+    int rows, n_slots, width, stack_size, block, ring, tokens;
+};
+
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;\n" ::: "memory");
+}
+
+__device__ __forceinline__ int blocks_for(long long n, int block, int ring) {
+    if (ring > 0 && n > ring) n = ring;
+    return (int)((n + block - 1) / block);
+}
+
+// Running sums of two numbers a thread over the block of threads; `total` gets both sums.  scratch: 2 x 33 long longs.
+__device__ __forceinline__ longlong2 scan2(long long a, long long b, long long (*scratch)[33], longlong2& total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const long long a0 = a, b0 = b;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long x = __shfl_up_sync(0xffffffffu, a, o), y = __shfl_up_sync(0xffffffffu, b, o);
+        if (lane >= o) { a += x; b += y; }
+    }
+    __syncthreads();
+    if (lane == 31) { scratch[0][warp] = a; scratch[1][warp] = b; }
+    __syncthreads();
+    if (warp == 0) {
+        long long x = scratch[0][lane], y = scratch[1][lane];
+        const long long x0 = x, y0 = y;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long u = __shfl_up_sync(0xffffffffu, x, o), v = __shfl_up_sync(0xffffffffu, y, o);
+            if (lane >= o) { x += u; y += v; }
+        }
+        scratch[0][lane] = x - x0;
+        scratch[1][lane] = y - y0;
+        if (lane == 31) { scratch[0][32] = x; scratch[1][32] = y; }
+    }
+    __syncthreads();
+    total = make_longlong2(scratch[0][32], scratch[1][32]);
+    return make_longlong2(scratch[0][warp] + a - a0, scratch[1][warp] + b - b0);
+}
+
+// The last i in [0, n) with at[i] <= x (at ascends, at[0] <= x).
+__device__ __forceinline__ int last_not_above(const int* at, int n, int x) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (at[mid] <= x) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+__global__ void __launch_bounds__(THREADS) blocks_extend_kernel(ExtendArgs a) {
+    extern __shared__ int rows_s[];
+    int* token0 = rows_s;                       // [rows + 1] tokens ahead of the row
+    int* block0 = token0 + a.rows + 1;          // [rows + 1] new blocks ahead of the row
+    int* slot_s = block0 + a.rows + 1;          // [rows]
+    int* held_s = slot_s + a.rows;              // [rows]
+    int* before = held_s + a.rows;              // [rows] length before the step, -1 for padding
+    unsigned* named = reinterpret_cast<unsigned*>(before + a.rows);      // a bit a slot
+    __shared__ long long scratch[2][33];
+    __shared__ int bad;
+    const int words = (a.n_slots + 31) / 32;
+    for (int i = threadIdx.x; i < words; i += THREADS) named[i] = 0u;
+    if (threadIdx.x == 0) bad = ST_OK;
+    pdl_trigger();
+    pdl_wait();
+    const int count = *a.count;
+    __syncthreads();
+    longlong2 sums = make_longlong2(0, 0);
+    for (int base = 0; base < a.rows; base += THREADS) {
+        const int i = base + threadIdx.x;
+        int more = 0, n = 0, wrong = ST_OK;
+        if (i < a.rows) {
+            const int s = a.slots[i], len = a.lengths[i];
+            n = a.fresh[i];
+            int have = 0, from = -1;
+            if (n < 0 || s < -1 || s >= a.n_slots || (s >= 0 && (len < 0 || (long long)len + n > 0x7fffffffll))) {
+                wrong = ST_BAD_ROW;
+                n = 0;
+            } else if (s >= 0) {
+                if (atomicOr(&named[s >> 5], 1u << (s & 31)) & (1u << (s & 31))) wrong = ST_BAD_ROW;
+                have = a.held[s];
+                if (have < 0 || have > a.width) {
+                    wrong = max(wrong, (int)ST_TABLE_WIDTH);
+                    have = 0;
+                }
+                from = len;
+                const int need = blocks_for((long long)len + n, a.block, a.ring);
+                if (need > a.width) wrong = max(wrong, (int)ST_TABLE_WIDTH);
+                more = max(0, need - have);
+            }
+            slot_s[i] = s;
+            held_s[i] = have;
+            before[i] = from;
+        }
+        if (wrong) atomicMax(&bad, wrong);
+        longlong2 total;
+        const longlong2 at = scan2(n, more, scratch, total);
+        if (i < a.rows) {                       // (where they pass 31 bits the step is refused below)
+            token0[i] = (int)(sums.x + at.x);
+            block0[i] = (int)(sums.y + at.y);
+        }
+        sums.x += total.x;
+        sums.y += total.y;
+    }
+    if (threadIdx.x == 0) {
+        token0[a.rows] = (int)sums.x;
+        block0[a.rows] = (int)sums.y;
+    }
+    cluster_barrier();                          // everyone has read the state (and every thread's shared stores are seen)
+    int status = bad;
+    if (sums.x > a.tokens) status = max(status, (int)ST_TOO_MANY_TOKENS);
+    if (sums.y > count || count > a.stack_size) status = max(status, (int)ST_NO_BLOCKS);
+    const bool ok = status == ST_OK;
+    const int rank = blockIdx.x, me = rank * THREADS + threadIdx.x, all = gridDim.x * THREADS;
+    const int n_new = ok ? (int)sums.y : 0, n_tok = ok ? (int)sums.x : 0;
+    if (me == 0) {
+        *a.status = status;
+        *a.count = count - n_new;
+        a.cu_q[a.rows] = n_tok;
+    }
+    for (int i = me; i < a.rows; i += all) {
+        const bool live = ok && before[i] >= 0;
+        a.cu_q[i] = ok ? token0[i] : 0;
+        a.kv_len[i] = live ? before[i] + token0[i + 1] - token0[i] : 0;
+        if (live && block0[i + 1] != block0[i]) a.held[slot_s[i]] = held_s[i] + block0[i + 1] - block0[i];
+    }
+    for (int k = me; k < n_new; k += all) {
+        const int i = last_not_above(block0, a.rows, k);
+        a.tables[(size_t)slot_s[i] * a.width + held_s[i] + k - block0[i]] = a.stack[count - 1 - k];
+    }
+    for (int t = me; t < a.tokens; t += all) {
+        int pos = -1, seq = 0, row = -1;
+        if (t < n_tok) {
+            seq = last_not_above(token0, a.rows, t);
+            if (before[seq] >= 0) {
+                pos = before[seq] + t - token0[seq];
+                const int last = before[seq] + token0[seq + 1] - token0[seq] - 1;
+                if (a.ring == 0 || pos / a.block + a.ring / a.block > last / a.block) {
+                    const int place = a.ring > 0 ? pos % a.ring : pos;
+                    const int e = place / a.block;
+                    const int id = e < held_s[seq] ? a.tables[(size_t)slot_s[seq] * a.width + e]
+                                                   : a.stack[count - 1 - (block0[seq] + e - held_s[seq])];
+                    row = id * a.block + place - e * a.block;
+                }
+            }
+        }
+        a.positions[t] = pos;
+        a.tok_seq[t] = seq;
+        a.cache_rows[t] = row;
+    }
+}
+
+// The blocks of the rows' slots go back to the stack, the last row's last block first: what one extend took, one release
+// of the same rows puts back in its old order.  Rows with slot -1 are left out; a wrong slot changes nothing.
+struct ReleaseArgs {
+    const int32_t *slots, *tables;
+    int32_t *held, *stack, *count, *status;
+    int rows, n_slots, width, stack_size;
+};
+
+__global__ void __launch_bounds__(THREADS) blocks_release_kernel(ReleaseArgs a) {
+    extern __shared__ int rows_s[];
+    int* block0 = rows_s;                       // [rows + 1] blocks given back ahead of the row (rows from the last to the first)
+    int* slot_s = block0 + a.rows + 1;
+    unsigned* named = reinterpret_cast<unsigned*>(slot_s + a.rows);
+    __shared__ long long scratch[2][33];
+    __shared__ int bad;
+    const int words = (a.n_slots + 31) / 32;
+    for (int i = threadIdx.x; i < words; i += THREADS) named[i] = 0u;
+    if (threadIdx.x == 0) bad = ST_OK;
+    pdl_trigger();
+    pdl_wait();
+    const int count = *a.count;
+    __syncthreads();
+    long long sum = 0;
+    for (int base = 0; base < a.rows; base += THREADS) {
+        const int k = base + threadIdx.x;       // in the order of giving back
+        int n = 0;
+        if (k < a.rows) {
+            const int s = a.slots[a.rows - 1 - k];
+            if (s < -1 || s >= a.n_slots) atomicMax(&bad, (int)ST_BAD_ROW);
+            else if (s >= 0) {
+                if (atomicOr(&named[s >> 5], 1u << (s & 31)) & (1u << (s & 31))) atomicMax(&bad, (int)ST_BAD_ROW);
+                n = a.held[s];
+                if (n < 0 || n > a.width) {
+                    atomicMax(&bad, (int)ST_TABLE_WIDTH);
+                    n = 0;
+                }
+            }
+            slot_s[k] = s;
+        }
+        longlong2 total;
+        const longlong2 at = scan2(n, 0, scratch, total);
+        if (k < a.rows) block0[k] = (int)(sum + at.x);
+        sum += total.x;
+    }
+    if (threadIdx.x == 0) block0[a.rows] = (int)sum;
+    cluster_barrier();
+    int status = bad;
+    if (count < 0 || count + sum > a.stack_size) status = max(status, (int)ST_NO_BLOCKS);
+    const int me = blockIdx.x * THREADS + threadIdx.x, all = gridDim.x * THREADS;
+    const int n_back = status == ST_OK ? (int)sum : 0;
+    if (me == 0) {
+        *a.status = status;
+        *a.count = count + n_back;
+    }
+    for (int b = me; b < n_back; b += all) {
+        const int k = last_not_above(block0, a.rows, b);
+        a.stack[count + b] = a.tables[(size_t)slot_s[k] * a.width + (block0[k + 1] - 1 - b)];
+    }
+    for (int k = me; status == ST_OK && k < a.rows; k += all)
+        if (slot_s[k] >= 0) a.held[slot_s[k]] = 0;
+}
+
+// One cluster of 1, 2, 4 or 8 blocks of threads: as many as give a thread a token, or an entry, of its own.
+template <typename Args>
+int launch_cluster(void (*kernel)(Args), const Args& a, long long work, size_t smem, OncePerDevice& raised, cudaStream_t stream) {
+    const int st = allow_shared_memory(kernel, 200 * 1024, raised);
+    if (st) return st;
+    int blocks = 1;
+    while (blocks < 8 && (long long)blocks * THREADS < work) blocks *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(blocks);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = blocks;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return (int)cudaLaunchKernelEx(&cfg, kernel, a);
+}
+
+}  // namespace
+
+BROLM_API int brolm_blocks_extend(const void* slots, const void* lengths, const void* fresh, void* tables, void* held,
+                                  const void* stack, void* count, void* cu_q, void* kv_len, void* positions, void* tok_seq,
+                                  void* cache_rows, void* status, int rows, int n_slots, int width, int stack_size, int block,
+                                  int ring, int tokens, cudaStream_t stream) {
+    if (rows < 0 || n_slots <= 0 || width <= 0 || stack_size < 0 || block <= 0 || tokens < 0) return BROLM_ERR_BAD_SIZE;
+    if (ring < 0 || ring % block) return BROLM_ERR_BAD_SIZE;
+    if (rows > MAX_ROWS || n_slots > MAX_SLOTS) return BROLM_ERR_TOO_LARGE;
+    if ((long long)stack_size * block > 0x7fffffffll) return BROLM_ERR_TOO_LARGE;          // (a cache row is 31 bits)
+    ExtendArgs a{(const int32_t*)slots, (const int32_t*)lengths, (const int32_t*)fresh, (int32_t*)tables, (int32_t*)held,
+                 (int32_t*)count, (const int32_t*)stack, (int32_t*)cu_q, (int32_t*)kv_len, (int32_t*)positions,
+                 (int32_t*)tok_seq, (int32_t*)cache_rows, (int32_t*)status, rows, n_slots, width, stack_size, block, ring, tokens};
+    static OncePerDevice raised;
+    const size_t smem = (size_t)(5 * rows + 2 + (n_slots + 31) / 32) * 4;
+    return launch_cluster(blocks_extend_kernel, a, tokens, smem, raised, stream);
+}
+
+BROLM_API int brolm_blocks_release(const void* slots, const void* tables, void* held, void* stack, void* count, void* status,
+                                   int rows, int n_slots, int width, int stack_size, cudaStream_t stream) {
+    if (rows < 0 || n_slots <= 0 || width <= 0 || stack_size < 0) return BROLM_ERR_BAD_SIZE;
+    if (rows > MAX_ROWS || n_slots > MAX_SLOTS) return BROLM_ERR_TOO_LARGE;
+    ReleaseArgs a{(const int32_t*)slots, (const int32_t*)tables, (int32_t*)held, (int32_t*)stack, (int32_t*)count,
+                  (int32_t*)status, rows, n_slots, width, stack_size};
+    static OncePerDevice raised;
+    const size_t smem = (size_t)(2 * rows + 1 + (n_slots + 31) / 32) * 4;
+    return launch_cluster(blocks_release_kernel, a, (long long)rows * 16, smem, raised, stream);
+}

@@ -55,8 +55,11 @@ LIBRARIES: dict[str, list[str]] = {
     "layernorm": ["layernorm.cu"],
     "delta_rule": ["delta_rule.cu"],
     "prompt_layer": ["prompt_layer.cu"],
+    "blocks": ["blocks.cu"],
+    "kv8": ["kv8.cu"],
+    "attn_kv8": ["attn_kv8.cu"],
 }
-HEADERS = ["common.cuh", "once_per_device.h", "attn_mma.cuh", "attn_decode_noalloc.h", "tcgen05.cuh"]
+HEADERS = ["common.cuh", "once_per_device.h", "attn_mma.cuh", "attn_decode_noalloc.h", "tcgen05.cuh", "kv8.cuh"]
 
 _loaded: dict[str, ctypes.CDLL] = {}
 _lock = threading.Lock()

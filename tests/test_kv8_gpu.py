@@ -1,0 +1,528 @@
+"""The 8-bit cache on the device against the plain restatement in 64 bits."""
+import math
+import random
+
+import pytest
+import torch
+
+from brolm_b200 import kernels
+from tests.plain import kv8_plain as plain
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+I32 = torch.int32
+NAN, INF = math.nan, math.inf
+
+
+def ints(v):
+    return torch.tensor(list(v), dtype=I32, device=DEV)
+
+
+def same(a, b):
+    """Equal numbers, NaN equal to NaN."""
+    return a.shape == b.shape and bool(((a == b) | (torch.isnan(a) & torch.isnan(b))).all())
+
+
+# --- tables ------------------------------------------------------------------------------------------------------------
+class Tables:
+    """The device's tables beside the plain ones; every step and every release is compared."""
+
+    def __init__(self, S, W, N, block, ring, seed):
+        self.block, self.ring = block, ring
+        self.order = list(range(N))
+        random.Random(seed).shuffle(self.order)
+        self.free, self.count = list(self.order), N
+        self.tables, self.held = [[0] * W for _ in range(S)], [0] * S
+        self.dev = dict(tables=torch.zeros((S, W), dtype=I32, device=DEV), held=ints([0] * S), free=ints(self.free),
+                        free_count=ints([N]))
+
+    def step(self, slots, lengths, new, tokens):
+        out = dict(cu_q=ints([7] * (len(slots) + 1)), kv_len=ints([7] * len(slots)), positions=ints([7] * tokens),
+                   tok_seq=ints([7] * tokens), cache_rows=ints([7] * tokens), status=ints([7]))
+        kernels.blocks_extend(ints(slots), ints(lengths), ints(new), *self.dev.values(), block=self.block, ring=self.ring, **out)
+        want = plain.extend(slots, lengths, new, self.tables, self.held, self.free, self.count, self.block, self.ring, tokens)
+        status, cu, kv_len, positions, seqs, rows, self.tables, self.held, self.count = want
+        assert out["status"].tolist() == [status]
+        for name, values in (("cu_q", cu), ("kv_len", kv_len), ("positions", positions), ("tok_seq", seqs), ("cache_rows", rows)):
+            assert out[name].tolist() == values, name
+        self.check()
+        return status
+
+    def release(self, slots):
+        status = ints([7])
+        kernels.blocks_release(ints(slots), *self.dev.values(), status=status)
+        live = [s for s in slots if s != -1]
+        bad = any(not 0 <= s < len(self.held) for s in live) or len(set(live)) != len(live)
+        if not bad:
+            for s in reversed(live):
+                while self.held[s]:
+                    self.held[s] -= 1
+                    self.free[self.count] = self.tables[s][self.held[s]]
+                    self.count += 1
+        assert status.tolist() == [4 if bad else 0]
+        self.check()
+
+    def check(self):
+        assert self.dev["tables"].tolist() == self.tables and self.dev["held"].tolist() == self.held
+        assert self.dev["free_count"].tolist() == [self.count] and self.dev["free"].tolist() == self.free
+
+
+@pytest.mark.parametrize("block,ring,S,W,N", [(32, 0, 5, 4, 17), (64, 192, 40, 3, 90), (128, 0, 200, 9, 900), (32, 32, 3, 1, 3)])
+def test_tables_over_many_steps(block, ring, S, W, N):
+    rng = random.Random(block + S)
+    t = Tables(S, W, N, block, ring, S)
+    lengths = [0] * S
+    seen = set()
+    for turn in range(25):
+        slots = rng.sample(range(S), rng.randint(1, S))
+        slots = [s if rng.random() < 0.9 else -1 for s in slots]
+        new = [rng.choice([0, 1, 1, 1, rng.randint(0, 3 * block)]) for _ in slots]
+        before = [lengths[s] if s >= 0 else rng.randint(-5, 5) for s in slots]
+        tokens = max(0, sum(new) + rng.choice([0, 0, 1, 40, -1]))
+        status = t.step(slots, before, new, tokens)
+        seen.add(status)
+        if status == 0:
+            for s, n in zip(slots, new):
+                if s >= 0:
+                    lengths[s] += n
+        if rng.random() < 0.4:
+            gone = rng.sample(range(S), rng.randint(1, S)) + [-1]
+            t.release(gone)
+            for s in gone[:-1]:
+                lengths[s] = 0
+    assert 0 in seen and len(seen) > 1
+
+
+def test_tables_of_many_rows_and_tokens():
+    n, S = 2500, 3000
+    rng = random.Random(1)
+    t = Tables(S, 4, 6000, 32, 128, 3)
+    slots = rng.sample(range(S), n)
+    new = [rng.choice([1, 2, 31, 32, 33, 64, 300]) for _ in slots]
+    free = list(t.free)
+    if t.step(slots, [0] * n, new, sum(new)) != 0:
+        new = [1] * n
+        assert t.step(slots, [0] * n, new, n) == 0
+    t.release(slots)
+    assert t.free == free                          # the stack is as it was
+
+
+@pytest.mark.parametrize("slots,lengths,new,tokens,status", [
+    ([0, 1, 0], [0, 0, 0], [1, 1, 1], 3, 4), ([0, 9], [0, 0], [1, 1], 2, 4), ([0, -2], [0, 0], [1, 1], 2, 4),
+    ([0, 1], [0, -1], [1, 1], 2, 4), ([0, 1], [0, 0], [1, -1], 2, 4), ([0, 1], [0, 0], [3, 4], 6, 3),
+    ([0], [0], [97], 200, 2), ([0, 1, 2], [0, 0, 0], [96, 64, 65], 300, 1), ([0], [2 ** 31 - 5], [20], 30, 4),
+    ([0, 1], [0, 0], [2 ** 31 - 1, 2 ** 31 - 1], 4, 3), ([0], [0], [0], 0, 0), ([], [], [], 5, 0)])
+def test_steps_that_do_not_fit_change_nothing(slots, lengths, new, tokens, status):
+    t = Tables(4, 3, 7, 32, 0, 0)
+    t.step([3], [0], [10], 10)
+    if max(new, default=0) > 2 ** 30 or max(lengths, default=0) > 2 ** 30:          # (too long for the plain lists)
+        out = dict(cu_q=ints([7] * (len(slots) + 1)), kv_len=ints([7] * len(slots)), positions=ints([7] * tokens),
+                   tok_seq=ints([7] * tokens), cache_rows=ints([7] * tokens), status=ints([7]))
+        kernels.blocks_extend(ints(slots), ints(lengths), ints(new), *t.dev.values(), block=32, **out)
+        t.check()
+        assert int(out["status"]) >= 2 and out["positions"].tolist() == [-1] * tokens and not out["cu_q"].any()
+    else:
+        assert t.step(slots, lengths, new, tokens) == status
+    t.release([0, 0])
+    t.release([4])
+    t.release([])
+
+
+def test_the_same_step_again_takes_no_more_blocks():
+    t = Tables(4, 8, 12, 32, 0, 0)
+    for _ in range(3):
+        assert t.step([2, 0], [33, 0], [40, 5], 50) == 0
+    assert t.count == 12 - 3 - 1
+
+
+# --- blocks ------------------------------------------------------------------------------------------------------------
+class Cached:
+    """Device blocks full of garbage beside plain ones, sequences with blocks in no order."""
+
+    def __init__(self, B, W, G, P, D, ring=0, seed=0, spare=2):
+        self.P, self.ring, self.G, self.D = P, ring, G, D
+        n = B * W + spare
+        g = torch.Generator().manual_seed(seed)
+        self.table = torch.randperm(n, generator=g)[:B * W].view(B, W)
+        self.pages = [torch.randint(-127, 128, (n, G, P, D), generator=g, dtype=torch.int8) for _ in range(2)]
+        self.scales = [torch.full((n, G), NAN) for _ in range(2)]                 # (blocks that nobody began)
+        self.dev = [p.to(DEV) for p in self.pages] + [s.to(DEV) for s in self.scales]
+        self.pages = [p.double() for p in self.pages]
+        self.scales = [s.double() for s in self.scales]
+        self.tables = self.table.to(I32).to(DEV)
+        self.lens = [0] * B
+
+    def places(self, i, n):
+        """Cache rows of the next n tokens of sequence i."""
+        first = plain.first_kept(self.lens[i] + n, self.P, self.ring)
+        out = []
+        for p in range(self.lens[i], self.lens[i] + n):
+            place = p % self.ring if self.ring else p
+            out.append(int(self.table[i, place // self.P]) * self.P + place % self.P if p >= first else -1)
+        return out
+
+    def write(self, rows, new, k, v, bound=None):
+        """k, v on the device; both sides."""
+        at = [self.places(i, n) if i >= 0 else [-1] * n for i, n in zip(rows, new)]
+        pos = [list(range(self.lens[i], self.lens[i] + n)) if i >= 0 else [-1] * n for i, n in zip(rows, new)]
+        cu = [0]
+        for n in new:
+            cu.append(cu[-1] + n)
+        kernels.kv8_write(k, v, ints(cu), ints(sum(pos, [])), ints(sum(at, [])), *self.dev, max_q_len=bound or max(new))
+        for i, n in zip(rows, new):
+            if i >= 0:
+                self.lens[i] += n
+        for x, pages, scales in zip((k, v), self.pages, self.scales):
+            plain.write(x.cpu(), sum(at, []), pages, scales)
+
+    def check(self):
+        for d, p in zip(self.dev[2:], self.scales):
+            assert same(d.cpu().double(), p)
+        for d, p, s in zip(self.dev[:2], self.pages, self.scales):
+            fine = ~torch.isnan(s)[:, :, None, None]
+            assert bool(((d.cpu().double() == p) | ~fine).all())
+
+    def values(self, which, i):
+        """(first position, [n, G, D]) of all that sequence i still holds."""
+        first = plain.first_kept(self.lens[i], self.P, self.ring)
+        return first, plain.read(self.pages[which], self.scales[which], self.table[i], range(first, self.lens[i]), self.ring)
+
+
+def rows_of(T, G, D, dtype, g, spread=2.0):
+    x = torch.randn((T, G, D), generator=g) * torch.exp2(spread * torch.randn((T, 1, 1), generator=g))
+    return x.to(dtype).to(DEV)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("G,P,D,ring", [(1, 32, 16, 0), (2, 64, 256, 0), (3, 128, 80, 0), (2, 32, 96, 96), (1, 256, 256, 0),
+                                        (5, 64, 48, 64)])
+def test_blocks_written_piece_by_piece(dtype, G, P, D, ring):
+    B, W = 4, (ring // P if ring else max(2, 640 // P))
+    c = Cached(B, W, G, P, D, ring, seed=D)
+    g = torch.Generator().manual_seed(P + D)
+    rng = random.Random(D)
+    for turn in range(14):
+        rows = rng.sample(range(B), rng.randint(1, B))
+        room = [(10 ** 6 if ring else W * P) - c.lens[i] for i in rows]
+        new = [min(r, rng.choice([0, 1, 1, 2, 7, P - 1, P, P + 1, 2 * P + 5])) for r in room]
+        if turn % 3 == 2:
+            new = [min(1, n) for n in new]
+        if sum(new) == 0:
+            continue
+        k, v = (rows_of(sum(new), G, D, dtype, g) for _ in range(2))
+        c.write(rows, new, k, v)
+        c.check()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_write_takes_rows_of_any_stride(dtype):
+    """Parts of a fused projection, heads apart from each other, rows that begin off 16 bytes."""
+    c = Cached(2, 3, 3, 32, 32, seed=1)
+    g = torch.Generator().manual_seed(3)
+    for cut in (0, 1, 5, 8):
+        wide = rows_of(30, 8, 70, dtype, g)
+        k, v = wide[:, 1:7:2, cut:cut + 32], wide[:, 2:8:2, 33:65]
+        c.write([0, 1], [29, 1], k, v)
+        c.write([1], [1], wide.reshape(30, -1)[3:4, 1:97].view(1, 3, 32), wide.reshape(30, -1)[5:6, 8:104].view(1, 3, 32))
+        c.check()
+        if c.lens[0] > 60:
+            break
+
+
+def test_write_at_the_ends_of_the_range():
+    """Zeros, the largest and the smallest numbers, the limits of a scale, and halves between two steps."""
+    rows = [0.0, 3.3895e38, 1e-45, 2.0 ** -127, 127 * 2.0 ** -126, 127.0, 127.00001, 254.0, 126.5, 0.5]
+    c = Cached(len(rows), 1, 1, 32, 16, seed=2)
+    for step in range(3):
+        x = torch.zeros((len(rows), 1, 16))
+        for i, r in enumerate(rows):
+            x[i, 0, :5] = torch.tensor([r, -r, r / 2, r / 254, -r / 508])
+            if step == 1:
+                x[i] *= 0.01
+        k = x.to(DEV)
+        c.write(list(range(len(rows))), [1] * len(rows), k, -k)
+        c.check()
+
+
+@pytest.mark.parametrize("value", [NAN, INF, -INF])
+def test_a_block_that_gets_a_number_that_is_not_finite(value):
+    c = Cached(2, 4, 2, 32, 32, seed=4)
+    g = torch.Generator().manual_seed(9)
+    for new, where in (([40, 3], None), ([1, 1], (0, 1, 7)), ([1, 1], None), ([30, 30], None), ([5, 5], (1, 0, 0))):
+        k, v = (rows_of(sum(new), 2, 32, torch.float32, g) for _ in range(2))
+        if where:
+            k[where] = value
+        c.write([0, 1], new, k, v)
+        c.check()
+    assert torch.isnan(c.dev[2]).sum() >= 2 + 2       # this block, and at least the two that nobody began
+    k, v = torch.empty((2, 75, 2, 32), device=DEV)
+    kernels.kv8_read(ints([0, 75]), ints([77]), ints([0]), c.tables, *c.dev, k, v, max_q_len=75)
+    want = c.values(0, 0)[1][2:]
+    assert same(k.cpu().double(), want) and torch.isnan(want).any() and not torch.isnan(want).all()
+    assert same(v.cpu().double(), c.values(1, 0)[1][2:])
+
+
+def test_write_of_padding_and_wrong_places_writes_nothing():
+    c = Cached(1, 2, 1, 32, 16)
+    before = [d.clone() for d in c.dev]
+    k = torch.ones((4, 1, 16), device=DEV)
+    n = c.pages[0].shape[0]
+    for bound in (1, 4):
+        for cu, pos, at in (([0, 1, 2, 3, 4], [-1] * 4, [-1] * 4), ([0, 1, 2, 3, 4], [0] * 4, [-1, n * 32, 2 ** 31 - 1, -7]),
+                            ([0, 0, 0, 0, 0], [0] * 4, [0] * 4)):
+            kernels.kv8_write(k, k, ints(cu), ints(pos), ints(at), *c.dev, max_q_len=bound)
+    assert all(same(a, b) for a, b in zip(before, c.dev))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("ring", [0, 96])
+def test_read_gives_back_what_is_held(dtype, ring):
+    c = Cached(3, 3 if ring else 9, 2, 32, 48, ring, seed=5)
+    g = torch.Generator().manual_seed(1)
+    for new in ([1, 70, 33], [200, 1, 64]):
+        c.write([0, 1, 2], new, rows_of(sum(new), 2, 48, dtype, g), rows_of(sum(new), 2, 48, dtype, g))
+    asked = [201, 0, 98]                                       # 201 and 97 are held: one more reads as zero
+    cu = ints([0, 201, 201, 299])
+    wide = torch.full((300, 4, 64), 5.0, dtype=dtype, device=DEV)
+    k, v = wide[:, ::2, :48], wide[:, 1::2, 16:]
+    kernels.kv8_read(cu, ints(c.lens), ints([0, 1, 2]), c.tables, *c.dev, k[:299], v[:299], ring=ring, max_q_len=201)
+    for which, got in ((0, k), (1, v)):
+        at = 0
+        for i, n in enumerate(asked):
+            first, held = c.values(which, i)
+            lead = torch.zeros((max(0, n - len(held)), 2, 48), dtype=torch.float64)
+            want = torch.cat([lead, held[max(0, len(held) - n):]]) if n else lead[:0]
+            assert same(got[at:at + n].cpu().double(), want.to(dtype).double())
+            at += n
+    assert bool((wide[299] == 5.0).all()) and bool((wide[:, ::2, 48:] == 5.0).all())
+
+
+# --- attention ---------------------------------------------------------------------------------------------------------
+def bound(dtype, ref, q, keys, values, scale):
+    """How far a row may be from 64 bits.  Scores: products and sums in 32 bits, D of them, and an exponential of relative
+    error below 2^-21, on scores of up to z = scale sum |q k|: 2^-21 (2 + z).  bfloat16 rounds the weights to 11 bits or
+    more (2^-11 of the largest value; they sum to one) and the result to 8 (2^-8 with a margin for a result at the edge)."""
+    z = scale * float((q.double().abs().amax() * keys.abs().sum(dim=2).amax())) if len(keys) else 0.0
+    most = float(values.abs().max()) if len(values) else 0.0
+    if dtype == torch.float32:
+        return most * 2.0 ** -21 * (2.0 + z) + 2.0 ** -22 * ref.abs()
+    return most * (2.0 ** -21 * (2.0 + z) + 2.0 ** -11) + 2.0 ** -8 * ref.abs()
+
+
+def compare(c, dtype, rows, new, group, scale, cap, window, seed=0, q_spread=1.0, max_kv_len=None, q=None):
+    """The newest tokens of the sequences ``rows`` (-1: a padding row) through the kernel and in 64 bits."""
+    H = c.G * group
+    g = torch.Generator().manual_seed(seed)
+    T = sum(new)
+    if q is None:
+        wide = (torch.randn((T, H * c.D + 64), generator=g) * q_spread).to(dtype).to(DEV)
+        q = wide[:, 32:32 + H * c.D]
+    out = torch.full((T, H * c.D + 32), 9.0, dtype=dtype, device=DEV)
+    cu = [0]
+    for n in new:
+        cu.append(cu[-1] + n)
+    lens = [c.lens[i] if i >= 0 else 0 for i in rows]
+    kernels.attention_kv8(q, out[:, :H * c.D], ints(cu), ints(lens), ints(rows), c.tables, *c.dev, n_kv=c.G, group=group,
+                          head_dim=c.D, scale=scale, cap=cap, window=window, ring=c.ring, batch=len(rows), max_q_len=max(new),
+                          max_kv_len=max_kv_len or max(1, max(lens)))
+    got = out[:, :H * c.D].cpu().double().view(T, H, c.D)
+    assert bool((out[:, H * c.D:] == 9.0).all())
+    qh = q.cpu().view(T, H, c.D)
+    for r, i in enumerate(rows):
+        first, keys = c.values(0, i) if i >= 0 else (0, torch.zeros((0, c.G, c.D), dtype=torch.float64))
+        _, values = c.values(1, i) if i >= 0 else (0, keys)
+        for j in range(new[r]):
+            t = cu[r] + j
+            ref = plain.attend(qh[t], keys, values, first, lens[r] - new[r] + j, scale, cap, window)
+            assert bool((torch.isnan(ref) == torch.isnan(got[t])).all()), (r, j)
+            fine = lambda x: torch.nan_to_num(x, nan=0.0)
+            off = fine(got[t] - ref).abs() - bound(dtype, fine(ref), fine(qh[t].double()), fine(keys), fine(values), scale)
+            assert float(off.max()) <= 0.0, (r, j, float(off.max()))
+    return got
+
+
+def filled(B, W, G, P, D, lens, ring=0, seed=0, dtype=torch.float32, spread=0.5):
+    c = Cached(B, W, G, P, D, ring, seed)
+    g = torch.Generator().manual_seed(seed + 1)
+    c.write(list(range(B)), lens, rows_of(sum(lens), G, D, dtype, g, spread), rows_of(sum(lens), G, D, dtype, g, spread))
+    return c
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D,G,group,P", [(16, 2, 2, 32), (32, 1, 6, 64), (64, 2, 1, 64), (80, 2, 3, 32), (96, 1, 8, 128), (128, 2, 4, 64),
+                                         (192, 1, 16, 32), (256, 4, 2, 64), (256, 1, 9, 256)])
+def test_attention_of_one_token(dtype, D, G, group, P):
+    lens = [1, 2, 31, 33, 64, 65, 200, 127]
+    c = filled(len(lens), -(-256 // P), G, P, D, lens, seed=D + group)
+    compare(c, dtype, [3, 0, -1, 6, 1, 2, 7, 4, 5], [1] * 9, group, D ** -0.5, 0.0, 0, q_spread=2.0)
+    compare(c, dtype, list(range(8)), [1] * 8, group, D ** -0.5, 20.0, 0, q_spread=4.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D,G,group,P", [(64, 2, 2, 64), (128, 1, 4, 32), (256, 2, 2, 64), (256, 1, 16, 64), (80, 1, 3, 32), (64, 1, 128, 32)])
+@pytest.mark.parametrize("window", [0, 1, 50])
+def test_attention_of_several_tokens(dtype, D, G, group, P, window):
+    lens = [3, 70, 140, 1, 257]
+    c = filled(len(lens), -(-288 // P), G, P, D, lens, seed=D + window)
+    for new in ([3, 1, 5, 1, 2], [3, 70, 40, 1, 131]):
+        compare(c, dtype, list(range(5)), new, group, D ** -0.5, 30.0 if window else 0.0, window, seed=sum(new))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("new", [1, 4, 67])
+def test_attention_over_a_ring(dtype, new):
+    P, window = 32, 41
+    ring = (window + new + P - 2 + P - 1) // P * P
+    c = filled(3, ring // P, 2, P, 64, [1, 33, 90], ring=ring, seed=new)
+    g = torch.Generator().manual_seed(8)
+    for _ in range(4):
+        c.write([0, 1, 2], [new] * 3, rows_of(3 * new, 2, 64, dtype, g), rows_of(3 * new, 2, 64, dtype, g))
+        compare(c, dtype, [2, 0, 1], [new] * 3, 2, 0.125, 0.0, window, seed=c.lens[0])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_attention_over_long_sequences_is_split_and_joined(dtype):
+    c = filled(3, 48, 1, 64, 64, [3000, 5, 1500], seed=11)
+    for bound_ in (3000, 3072, 100000):
+        compare(c, dtype, [0, 1, 2], [1, 1, 1], 2, 0.125, 0.0, 0, max_kv_len=bound_)
+    compare(c, dtype, [0], [1], 2, 0.125, 0.0, 0)
+    compare(c, dtype, [0, 2], [1, 1], 2, 0.125, 0.0, 900)
+    compare(c, dtype, [0, 2], [6, 3], 2, 0.125, 50.0, 0)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("new", [1, 3, 80])
+def test_blocks_that_a_token_does_not_see_change_nothing(dtype, new):
+    """A NaN block before the window, or behind the token, must not reach it; one that it sees makes it NaN."""
+    for value, at in ((NAN, 10), (INF, 140), (NAN, 295)):
+        c = Cached(2, 10, 2, 32, 64, seed=6)
+        g = torch.Generator().manual_seed(2)
+        k, v = (rows_of(600, 2, 64, torch.float32, g, 0.5) for _ in range(2))
+        k[at, 0, 3] = value
+        v[300 + at, 1, 5] = value
+        c.write([0, 1], [300, 300], k, v)
+        got = compare(c, dtype, [0, 1], [new, new], 2, 0.125, 0.0, 100)
+        assert not torch.isnan(got).all()
+        got = compare(c, dtype, [0, 1], [new, new], 2, 0.125, 25.0, 0)
+        assert torch.isnan(got).any() and not torch.isnan(got).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("new", [1, 40])
+def test_attention_where_numbers_are_of_all_sizes(dtype, new):
+    """Keys and values whose blocks differ by powers of ten, queries that are very large or small, scores that leave one
+    key all the weight."""
+    c = Cached(2, 6, 1, 32, 64, seed=7)
+    g = torch.Generator().manual_seed(3)
+    for step in range(6):
+        k, v = (rows_of(64, 1, 64, torch.float32, g, 0.5) for _ in range(2))
+        c.write([0, 1], [32, 32], k * 10.0 ** (step % 3 - 1), v * 10.0 ** (5 - 3 * step))
+    q = (torch.randn((2 * new, 128), generator=g)).to(dtype).to(DEV)
+    for size in (1.0, 30.0, 1e-30, 0.0):
+        compare(c, dtype, [0, 1], [new, new], 2, 0.125, 0.0, 0, q=q * size)
+    compare(c, dtype, [0, 1], [new, new], 2, 1e-20, 0.0, 0, q=q * 1e18)
+    compare(c, dtype, [0, 1], [new, new], 2, 0.125, 5.0, 0, q=q * 1e4)
+
+
+@pytest.mark.parametrize("new", [1, 5, 33])
+def test_a_query_that_is_not_a_number(new):
+    c = filled(2, 3, 2, 32, 32, [70, 50], seed=3)
+    g = torch.Generator().manual_seed(4)
+    for dtype in (torch.bfloat16, torch.float32):
+        q = torch.randn((2 * new, 4 * 32), generator=g).to(dtype).to(DEV)
+        q[0, 40] = NAN                                      # one head of one token
+        out = torch.empty_like(q)
+        kernels.attention_kv8(q, out, ints([0, new, 2 * new]), ints([70, 50]), ints([0, 1]), c.tables, *c.dev, n_kv=2, group=2,
+                              head_dim=32, scale=0.2, cap=0.0, window=0, ring=0, batch=2, max_q_len=new, max_kv_len=70)
+        bad = torch.isnan(out)
+        assert bool(bad[0, 32:64].all()) and int(bad.sum()) == 32
+
+
+@pytest.mark.parametrize("new", [1, 33])
+def test_cache_of_more_than_31_bits_of_bytes(new):
+    """Blocks whose bytes lie beyond 2^31, of a sequence and of its neighbours' heads."""
+    G, P, D = 16, 64, 256
+    N = (1 << 31) // (G * P * D) + 40
+    dev = [torch.empty((N, G, P, D), dtype=torch.int8, device=DEV) for _ in range(2)] + \
+          [torch.full((N, G), NAN, device=DEV) for _ in range(2)]
+    blocks = [N - 1, 3, N - 30, N - 2]
+    g = torch.Generator().manual_seed(5)
+    k, v = (rows_of(200, G, D, torch.bfloat16, g, 0.3) for _ in range(2))
+    at = [blocks[p // P] * P + p % P for p in range(200)]
+    kernels.kv8_write(k, v, ints([0, 200]), ints(range(200)), ints(at), *dev, max_q_len=200)
+    small = [torch.zeros((4, G, P, D), dtype=torch.float64) for _ in range(2)]
+    scales = [torch.zeros((4, G), dtype=torch.float64) for _ in range(2)]
+    for x, p, s in zip((k, v), small, scales):
+        plain.write(x.cpu(), list(range(200)), p, s)
+    tables = ints(blocks).view(1, 4)
+    ko, vo = torch.empty((2, 200, G, D), dtype=torch.bfloat16, device=DEV)
+    kernels.kv8_read(ints([0, 200]), ints([200]), ints([0]), tables, *dev, ko, vo, max_q_len=200)
+    keys, values = (plain.read(p, s, range(4), range(200)) for p, s in zip(small, scales))
+    assert same(ko.cpu().double(), keys) and same(vo.cpu().double(), values)
+    q = torch.randn((new, G * D), generator=g).bfloat16().to(DEV)
+    out = torch.empty_like(q)
+    kernels.attention_kv8(q, out, ints([0, new]), ints([200]), ints([0]), tables, *dev, n_kv=G, group=1, head_dim=D,
+                          scale=1 / 16, cap=0.0, window=0, ring=0, batch=1, max_q_len=new, max_kv_len=200)
+    for j in (0, new - 1):
+        qj = q[j].cpu().view(G, D)
+        ref = plain.attend(qj, keys, values, 0, 200 - new + j, 1 / 16, 0.0, 0)
+        off = (out[j].cpu().double().view(G, D) - ref).abs() - bound(torch.bfloat16, ref, qj, keys, values, 1 / 16)
+        assert float(off.max()) <= 0.0
+
+
+def test_everything_on_a_stream_of_its_own_and_twice_the_same_bits():
+    """A step's four calls one after the other on a stream that is not the default, without a wait between them."""
+    G, P, D, group, B = 2, 64, 128, 4, 3
+    g = torch.Generator().manual_seed(6)
+    lens, N = [500, 64, 129], 20
+    results = []
+    for _ in range(2):
+        side = torch.cuda.Stream()
+        g.manual_seed(6)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            state = dict(tables=torch.zeros((B, 9), dtype=I32, device=DEV), held=ints([0] * B), free=ints(range(N)), free_count=ints([N]))
+            cache = [torch.zeros((N, G, P, D), dtype=torch.int8, device=DEV) for _ in range(2)] + \
+                    [torch.zeros((N, G), device=DEV) for _ in range(2)]
+            out = []
+            for before, new in (([0] * B, lens), (lens, [1] * B), ([n + 1 for n in lens], [1, 20, 3])):
+                T = sum(new)
+                step = dict(cu_q=ints([0] * (B + 1)), kv_len=ints([0] * B), positions=ints([0] * T), tok_seq=ints([0] * T),
+                            cache_rows=ints([0] * T), status=ints([0]))
+                slots = ints([2, 0, 1])
+                kernels.blocks_extend(slots, ints(before), ints(new), *state.values(), block=P, **step)
+                x = torch.randn((T, (group + 2) * G * D), generator=g).bfloat16().to(DEV)
+                H = group * G * D
+                kernels.kv8_write(x[:, H:H + G * D].view(T, G, D), x[:, H + G * D:].view(T, G, D), step["cu_q"], step["positions"],
+                                  step["cache_rows"], *cache, max_q_len=max(new))
+                o = torch.empty((T, H), dtype=torch.bfloat16, device=DEV)
+                kernels.attention_kv8(x[:, :H], o, step["cu_q"], step["kv_len"], slots, state["tables"], *cache, n_kv=G, group=group,
+                                      head_dim=D, scale=D ** -0.5, cap=0.0, window=0, ring=0, batch=B, max_q_len=max(new), max_kv_len=520)
+                out.append(o)
+        side.synchronize()
+        results.append(out)
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    assert all(bool(torch.isfinite(o).all()) for o in results[0])
+
+
+def test_launchers_refuse_sizes():
+    c = Cached(1, 2, 1, 32, 16)
+    odd = [torch.zeros((3, 1, 32, 24), dtype=torch.int8, device=DEV)] * 2 + c.dev[2:]
+    k = torch.zeros((1, 1, 24), device=DEV)
+    for cache, x in ((odd, k),):
+        with pytest.raises(kernels.KernelError, match="size"):
+            kernels.kv8_write(x, x, ints([0, 1]), ints([0]), ints([0]), *[a[:3].contiguous() for a in cache], max_q_len=1)
+    block = [torch.zeros((3, 1, 48, 16), dtype=torch.int8, device=DEV)] * 2 + [d[:3].contiguous() for d in c.dev[2:]]
+    q = torch.zeros((1, 16), device=DEV)
+    with pytest.raises(kernels.KernelError, match="size"):
+        kernels.attention_kv8(q, q.clone(), ints([0, 1]), ints([1]), ints([0]), c.tables, *block, n_kv=1, group=1, head_dim=16, scale=1.0,
+                              cap=0.0, window=0, ring=0, batch=1, max_q_len=1, max_kv_len=1)
+    k = torch.zeros((2, 1, 16), device=DEV)
+    off = torch.zeros(40, device=DEV)[1:33].view(2, 1, 16)
+    with pytest.raises(kernels.KernelError, match="aligned"):
+        kernels.kv8_read(ints([0, 2]), ints([2]), ints([0]), c.tables, *c.dev, off, k, max_q_len=2)
+    with pytest.raises(kernels.KernelError, match="size"):
+        kernels.blocks_extend(ints([0]), ints([0]), ints([1]), c.tables, ints([0]), ints([0]), ints([1]), block=32, ring=40,
+                              cu_q=ints([0, 0]), kv_len=ints([0]), positions=ints([0]), tok_seq=ints([0]), cache_rows=ints([0]),
+                              status=ints([0]))
