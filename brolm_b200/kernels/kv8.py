@@ -21,7 +21,7 @@ from typing import Optional
 
 import torch
 
-from . import KernelError, _check, _code, _fn, _ptr, _stream
+from . import KernelError, _check, _code, _fn, _ptr, _stream, device_sms
 
 # what the tables' status word says
 BLOCKS_STATUS = {0: "ok", 1: "too few free blocks (or a stack that does not fit)", 2: "a row of the tables is too narrow",
@@ -141,6 +141,24 @@ def kv8_read(cu_q: torch.Tensor, kv_len: torch.Tensor, slots: torch.Tensor, tabl
              k_out.shape[0], rows, n_kv, dim, block, n_blocks, tables.shape[0], tables.shape[1], ring, _stream()), what)
 
 
+KV8_TILE, KV8_WARPS, KV8_CLUSTER = 32, 4, 8       # keys of a tile, warps of a block, blocks that join their results themselves
+
+
+def kv8_shares(batch: int, n_kv: int, row_tiles: int, keys: int, sms: Optional[int] = None) -> tuple[int, int]:
+    """How many blocks share the keys of one (sequence, kv head, tile of query rows): (blocks of a cluster, clusters).
+
+    Two blocks run on an SM; there are as many as give every SM its two, but none whose four warps would not have a tile
+    of keys each.  More than a cluster's eight are joined by a second launch: only where they shorten a long run."""
+    sms = sms or device_sms()
+    tiles = max(1, -(-keys // KV8_TILE))
+    want = min(2 * sms // max(1, batch * n_kv * row_tiles), -(-tiles // KV8_WARPS))
+    if want <= KV8_CLUSTER:
+        return max(1, want), 1
+    if tiles <= 8 * KV8_CLUSTER * KV8_WARPS:
+        return KV8_CLUSTER, 1
+    return KV8_CLUSTER, want // KV8_CLUSTER
+
+
 def attention_kv8(q: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, kv_len: torch.Tensor, slots: torch.Tensor,
                   tables: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale: torch.Tensor,
                   v_scale: torch.Tensor, *, n_kv: int, group: int, head_dim: int, scale: float, cap: float, window: int,
@@ -164,8 +182,17 @@ def attention_kv8(q: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, kv_len
         raise KernelError(f"{what}: a ring of {ring} does not keep what {max_q_len} new tokens see under a window of {window}: "
                           f"it takes window + tokens + {block} - 2")
     _ints(what, ("cu_q", cu_q, batch + 1), ("kv_len", kv_len, batch), ("slots", slots, batch), ("tables", tables, None))
+    rows = max_q_len * group
+    keys = min(max_kv_len, window + max_q_len) if window > 0 else max_kv_len
+    shares, spans = kv8_shares(batch, n_kv, -(-rows // (8 if rows <= 8 else 16)), keys)
+    part_o = part_ml = None
+    if spans > 1:
+        n = q.shape[0] * n_kv * group * spans
+        part_o = torch.empty(n * head_dim, dtype=torch.float32, device=q.device)
+        part_ml = torch.empty(n * 2, dtype=torch.float32, device=q.device)
     f = _fn("attn_kv8", "brolm_attn_kv8", [c_void_p, c_int, c_void_p, c_int, c_int] + [c_void_p] * 8 + [c_int] * 11 +
-            [c_float, c_float, c_int, c_int, c_void_p])
+            [c_float, c_float, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p])
     _check(f(_ptr(q), q.stride(0), _ptr(out), out.stride(0), _code(q), _ptr(cu_q), _ptr(kv_len), _ptr(slots), _ptr(tables),
              _ptr(k_pages), _ptr(v_pages), _ptr(k_scale), _ptr(v_scale), q.shape[0], batch, n_kv, group, head_dim, block, n_blocks,
-             tables.shape[0], tables.shape[1], ring, window, scale, cap, max_q_len, max_kv_len, _stream()), what)
+             tables.shape[0], tables.shape[1], ring, window, scale, cap, max_q_len, shares, spans, _ptr(part_o), _ptr(part_ml),
+             _stream()), what)
