@@ -35,6 +35,7 @@ using namespace kv8;
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int WARPS = 4, THREADS = 32 * WARPS;
+constexpr int MAX_SHARES = 8;             // blocks of a cluster
 constexpr int KT = 32;                    // keys of a tile: a divisor of every block size
 
 struct AttnArgs {
@@ -63,11 +64,6 @@ __device__ __forceinline__ float rcp(float x) {
 }
 __device__ __forceinline__ void cluster_barrier() {
     asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;\n" ::: "memory");
-}
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
 }
 __device__ __forceinline__ uint32_t of_rank(uint32_t addr, uint32_t rank) {
     uint32_t r;
@@ -136,9 +132,574 @@ __device__ __forceinline__ int value_offset(int row, int c) {
     }
 }
 
-template <typename T, int DP, int NT>
+__device__ __forceinline__ void add_part(float4& acc, float& sum, const float4& x, float l, float f) {
+    sum = fmaf(l, f, sum);
+    acc.x = fmaf(x.x, f, acc.x); acc.y = fmaf(x.y, f, acc.y); acc.z = fmaf(x.z, f, acc.z); acc.w = fmaf(x.w, f, acc.w);
+}
+// Four entries of a row: zeros where nothing was seen, NaN where something was not a number.
+template <typename T>
+__device__ __forceinline__ void store_row(const AttnArgs& a, int tok, int head, int d, const float4& acc, float sum) {
+    const float inv = sum > 0.0f ? 1.0f / sum : sum != 0.0f ? sum : acc.x != acc.x ? 1.0f : 0.0f;
+    T* dst = reinterpret_cast<T*>(a.out) + (size_t)tok * a.out_stride + head * a.dim + d;
+    dst[0] = from_float<T>(acc.x * inv);
+    dst[1] = from_float<T>(acc.y * inv);
+    dst[2] = from_float<T>(acc.z * inv);
+    dst[3] = from_float<T>(acc.w * inv);
+}
+
+__device__ __forceinline__ int ld_now(const int32_t* p) {
+    int v;
+    asm volatile("ld.global.b32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+    return v;
+}
+// Eight entries of a row, asked for now and looked at later; zeros where nothing was asked for.
+template <typename T>
+struct Eight {
+    static constexpr int PIECES = sizeof(T) / 2;               // of 16 bytes
+    uint4 raw[PIECES];
+    __device__ __forceinline__ Eight() {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) raw[i] = make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void fetch(const T* p, bool wide) {
+        if (wide) {
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i)
+                asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(raw[i].x), "=r"(raw[i].y), "=r"(raw[i].z), "=r"(raw[i].w)
+                             : "l"(reinterpret_cast<const uint4*>(p) + i) : "memory");
+        } else {
+            alignas(16) T v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = p[e];
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) raw[i] = reinterpret_cast<const uint4*>(v)[i];
+        }
+    }
+    __device__ __forceinline__ void numbers(float (&v)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 4 * PIECES; ++i) {
+            const uint32_t w = (&raw[i / 4].x)[i % 4];
+            if constexpr (PIECES == 2) v[i] = __uint_as_float(w);
+            else {
+                v[2 * i] = __uint_as_float(w << 16);
+                v[2 * i + 1] = __uint_as_float(w & 0xffff0000u);
+            }
+        }
+    }
+};
+
+// What a block works on: rows of one sequence and kv head, and the tiles [t_begin, t_end) of their keys.
+struct Item {
+    int share, span, g, first_tok, row0, n_rows, pos0, pos_lo, pos_hi, slot, t_begin, t_end;
+};
+// Three round trips to memory lie before the first product: what the sequence is; its row of the tables and the queries;
+// the tiles and their scales.  What one trip can fetch is asked for before anything of it is looked at.
+template <int ROWS>
+__device__ __forceinline__ Item find_item(const AttnArgs& a) {
+    Item it;
+    it.share = blockIdx.x % a.shares;
+    int rest = blockIdx.x / a.shares;
+    it.span = rest % a.spans;
+    rest /= a.spans;
+    const int b = rest / a.row_tiles;
+    it.row0 = (rest - b * a.row_tiles) * ROWS;
+    it.g = blockIdx.y;
+    it.first_tok = ld_now(a.cu_q + b);
+    const int end_tok = ld_now(a.cu_q + b + 1), kv_len = ld_now(a.kv_len + b);
+    it.slot = ld_now(a.slots + b);
+    const int n_tok = min(end_tok, a.tokens) - it.first_tok;
+    it.n_rows = it.first_tok < 0 ? 0 : (int)min((long long)ROWS, (long long)n_tok * a.group - it.row0);
+    it.pos0 = kv_len - n_tok;                                  // position of the sequence's first new token
+    it.pos_lo = it.pos0 + it.row0 / a.group;
+    it.pos_hi = it.pos0 + (it.row0 + it.n_rows - 1) / a.group;
+    it.t_begin = it.t_end = 0;
+    if (it.n_rows > 0 && it.pos_hi >= 0 && it.slot >= 0 && it.slot < a.n_slots) {
+        const int t_lo = a.window > 0 ? max(0, it.pos_lo - a.window + 1) / KT : 0, t_hi = it.pos_hi / KT;
+        const int parts = a.shares * a.spans, per = (t_hi - t_lo + parts) / parts;
+        it.t_begin = t_lo + (it.span * a.shares + it.share) * per;
+        it.t_end = min(t_hi + 1, it.t_begin + per);
+    }
+    return it;
+}
+
+// A warp's tiles of keys and values on their way into its part of shared memory.
+template <int DP, int SLOTS>
+struct TileRing {
+    static constexpr int UNIT = KT * DP;                       // a key or value tile
+    const AttnArgs& a;
+    const int32_t* table;
+    uint32_t base;
+    int g, lane, t0, n_tiles, n_units, unit_no;
+    long long place_l;                                         // of the 32 tiles that are being asked for, lane by lane: where they lie
+    float sk_l, sv_l, sk_c, sv_c;                              // .. their scales, and those of the tiles that are being multiplied
+
+    __device__ __forceinline__ TileRing(const AttnArgs& args, const Item& it, uint32_t smem, int warp, int lane_) : a(args) {
+        table = a.tables + (size_t)max(it.slot, 0) * a.width;
+        base = smem + warp * SLOTS * UNIT;
+        g = it.g;
+        lane = lane_;
+        t0 = it.t_begin + warp;                                // the block's warps take tiles in turn
+        n_tiles = t0 < it.t_end ? (it.t_end - t0 + WARPS - 1) / WARPS : 0;
+        n_units = 2 * n_tiles;
+        unit_no = 0;
+        sk_c = sv_c = 0.0f;
+    }
+    __device__ __forceinline__ void look_up(int n) {
+        place_l = 0;
+        sk_l = sv_l = 0.0f;
+        if (n + lane < n_tiles) {
+            const long long key = (long long)(t0 + (n + lane) * WARPS) * KT;
+            const int place = a.ring > 0 ? (int)(key % a.ring) : (int)key, e = place / a.block;
+            int id = e < a.width ? table[e] : 0;
+            if (id < 0 || id >= a.n_blocks) id = 0;            // (never followed out of the cache)
+            const size_t bh = (size_t)id * a.n_kv + g;
+            place_l = (long long)bh * a.block + (place - e * a.block);
+            sk_l = a.k_scale[bh];
+            sv_l = a.v_scale[bh];                              // (nothing waits for the scales before their first use)
+        }
+    }
+    __device__ __forceinline__ void load(int u) {              // key tile u / 2 or value tile u / 2 into slot u % SLOTS
+        const int n = u >> 1;
+        if (u > 0 && (u & 63) == 0) look_up(n);
+        const long long place = __shfl_sync(0xffffffffu, place_l, n & 31);
+        const int8_t* src = (u & 1 ? a.v_pages : a.k_pages) + place * a.dim;
+        const uint32_t dst = base + (u % SLOTS) * UNIT;
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+            const int piece = i * 32 + lane, row = piece / (DP / 16), c = piece % (DP / 16);
+            if (c * 16 < a.dim)
+                copy16(dst + (u & 1 ? value_offset<DP>(row, c) : key_offset<DP>(row, c)), src + row * a.dim + c * 16, true);
+        }
+    }
+    __device__ __forceinline__ void start() {
+        look_up(0);
+#pragma unroll
+        for (int u = 0; u < SLOTS - 1; ++u) {
+            if (u < n_units) load(u);
+            copy_commit();
+        }
+    }
+    __device__ __forceinline__ uint32_t next() {               // waits for the next unit and asks for one more; its address
+        copy_wait<SLOTS - 2>();
+        __syncwarp();                                          // it has landed for all lanes; all are done with the one before
+        if (unit_no + SLOTS - 1 < n_units) load(unit_no + SLOTS - 1);
+        copy_commit();
+        return base + (unit_no++ % SLOTS) * UNIT;
+    }
+    // (the scales of the next 32 tiles have been asked for when the first of them was, one or more tiles ago)
+    __device__ __forceinline__ float2 scales(int n) {
+        if ((n & 31) == 0) {
+            const bool bad = sk_l != sk_l || sv_l != sv_l;     // a NaN block: scores of zero, values of NaN
+            sk_c = bad ? 0.0f : sk_l;
+            sv_c = bad ? __int_as_float(0x7fc00000) : sv_l;
+        }
+        return make_float2(__shfl_sync(0xffffffffu, sk_c, n & 31), __shfl_sync(0xffffffffu, sv_c, n & 31));
+    }
+};
+
+// The queries of a block's rows, a warp a row, eight entries a lane.
+template <typename T, int ROWS>
+__device__ __forceinline__ void fetch_queries(const AttnArgs& a, const Item& it, int warp, int lane, Eight<T> (&raw)[(ROWS + WARPS - 1) / WARPS]) {
+#pragma unroll
+    for (int j = 0; j < (ROWS + WARPS - 1) / WARPS; ++j) {
+        const int r = warp + j * WARPS, row = it.row0 + r;
+        if (r < it.n_rows && lane * 8 < a.dim)
+            raw[j].fetch(reinterpret_cast<const T*>(a.q) + (size_t)(it.first_tok + row / a.group) * a.q_stride +
+                         (it.g * a.group + row % a.group) * a.dim + lane * 8, a.wide);
+    }
+}
+// The exponent that brings a row's largest number to [2^top, 2^(top + 1)), within what a float's exponent can say; a row
+// that is not finite gets zeros and the scale NaN.
+__device__ __forceinline__ int row_exponent(float (&v)[8], int top, bool& finite) {
+    float most = 0.0f;
+    finite = true;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        most = fmaxf(most, fabsf(v[e]));
+        finite = finite && fabsf(v[e]) < INFINITY;
+    }
+    most = warp_max(most);
+    finite = __all_sync(0xffffffffu, finite);
+    if (!finite) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+    }
+    return max(min(top + 127 - (int)(__float_as_uint(most) >> 23), 120), -126);
+}
+
+// What the warps have left in shared memory (wo [WARPS][ROWS][pitch] sums, wml [WARPS][ROWS][2] maxima in log2 units and
+// sums of weights) is joined over the block, then over the cluster; the result goes to the output, or, where several
+// clusters share the keys, to memory for the second launch.  co, cml: room for a block's own result.
+template <typename T, int ROWS, int PITCH>
+__device__ __forceinline__ void merge(const AttnArgs& a, const Item& it, const float* wo, const float* wml, float* co, float* cml,
+                                      const float* q_scale) {
+    const int d4 = a.dim >> 2;
+    for (int i = threadIdx.x; i < it.n_rows * d4; i += THREADS) {
+        const int r = i / d4, d = (i - r * d4) * 4;
+        float most = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) most = fmaxf(most, wml[(w * ROWS + r) * 2]);
+        float sum = 0.0f;
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            const float f = most > -INFINITY ? ex2(wml[(w * ROWS + r) * 2] - most) : 0.0f;
+            add_part(acc, sum, *reinterpret_cast<const float4*>(wo + (w * ROWS + r) * PITCH + d), wml[(w * ROWS + r) * 2 + 1], f);
+        }
+        *reinterpret_cast<float4*>(co + r * PITCH + d) = acc;
+        if (d == 0) {
+            cml[r * 2] = most;
+            cml[r * 2 + 1] = sum;
+        }
+    }
+    if (a.shares > 1) cluster_barrier();
+    else __syncthreads();
+    for (int i = it.share * THREADS + threadIdx.x; i < it.n_rows * d4; i += a.shares * THREADS) {
+        const int r = i / d4, d = (i - r * d4) * 4;
+        float most = -INFINITY, sum = 0.0f;
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (a.shares == 1) {
+            most = cml[r * 2];
+            sum = cml[r * 2 + 1];
+            acc = *reinterpret_cast<const float4*>(co + r * PITCH + d);
+        } else {
+            const uint32_t o_at = smem_addr(co + r * PITCH + d), ml_at = smem_addr(cml + r * 2);
+            float2 ml[MAX_SHARES];
+            float4 x[MAX_SHARES];
+#pragma unroll
+            for (int s = 0; s < MAX_SHARES; ++s)
+                if (s < a.shares) {
+                    ml[s] = ld_cluster2(of_rank(ml_at, s));
+                    x[s] = ld_cluster4(of_rank(o_at, s));
+                }
+#pragma unroll
+            for (int s = 0; s < MAX_SHARES; ++s)
+                if (s < a.shares) most = fmaxf(most, ml[s].x);
+#pragma unroll
+            for (int s = 0; s < MAX_SHARES; ++s)
+                if (s < a.shares) add_part(acc, sum, x[s], ml[s].y, most > -INFINITY ? ex2(ml[s].x - most) : 0.0f);
+        }
+        const int row = it.row0 + r, tok = it.first_tok + row / a.group, head = it.g * a.group + row % a.group;
+        if (q_scale[r] != q_scale[r]) acc.x = acc.y = acc.z = acc.w = it.pos0 + row / a.group >= 0 ? q_scale[r] : 0.0f;
+        if (a.spans > 1) {
+            const size_t at = ((size_t)tok * a.n_kv * a.group + head) * a.spans + it.span;
+            *reinterpret_cast<float4*>(a.part_o + at * a.dim + d) = acc;
+            if (d == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(most, sum);
+        } else {
+            store_row<T>(a, tok, head, d, acc, sum);
+        }
+    }
+    if (a.shares > 1) cluster_barrier();                       // nobody leaves while its results are being read
+}
+
+// --- up to eight rows: products of whole numbers -------------------------------------------------------------------------
+//
+// With few rows most of an instruction's columns would be empty and turning the cache's bytes into f16 is what a warp
+// spends its time on (1,380 instructions a tile of 32 keys of 256 entries, 2,870 cycles of a warp that has a scheduler to
+// itself).  Here the bytes are multiplied as they are (m16n8k32, whole sums), and what is multiplied with them is whole
+// numbers too, a digit of 8 bits a column:
+//
+//     q 2^s = sum_i d_i 256^(3 - i), four signed digits (30 bits of the row's largest number), two rows an instruction;
+//     p     = sum_i e_i 256^-i,      two unsigned digits (bfloat16: 16 bits of the tile's largest weight, four rows an
+//                                    instruction) or four (float32: 31 bits, two rows).
+//
+// A thread has two neighbouring digits' sums, joins them as whole numbers (below 2^31: 127 * 255 * 256 * 33 in both
+// products) and then in floats.  The keys are read as the instruction wants them; of the values, four keys' bytes of an
+// entry are gathered into a word by eight byte permutations for sixteen bytes.
+__device__ __forceinline__ void mma_s8(int (&d)[4], const uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_s8u8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                 : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0));
+}
+
+template <typename T, int DP, int ROWS>
+struct FewShape {
+    static constexpr int SEGS = DP / 64;
+    static constexpr int SLOTS = DP == 256 ? 3 : DP == 192 ? 4 : DP == 128 ? 6 : 8;
+    static constexpr int RING = WARPS * SLOTS * KT * DP;
+    static constexpr int QT = ROWS / 2;                                    // tiles of the first product: two rows each
+    static constexpr int PT = sizeof(T) == 4 ? QT : (QT + 1) / 2;          // .. of the second
+    static constexpr int Q_BYTES = QT * SEGS * 512;
+    static constexpr int PITCH = DP + 4;
+    static constexpr int MERGE = (WARPS * ROWS * PITCH + WARPS * ROWS * 2 + ROWS * PITCH + ROWS * 2) * 4;
+    static constexpr int SMEM = Q_BYTES + (RING > MERGE ? RING : MERGE);
+};
+
+template <typename T, int DP, int ROWS>
+__global__ void __launch_bounds__(THREADS, 2) attn_kv8_few_kernel(AttnArgs a) {
+    using SH = FewShape<T, DP, ROWS>;
+    constexpr int SEGS = SH::SEGS, QT = SH::QT, PT = SH::PT, PER_WARP = (ROWS + WARPS - 1) / WARPS;
+    constexpr bool EXACT = sizeof(T) == 4;
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ float q_scale[ROWS];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, t4 = lane & 3;
+    pdl_wait();
+    const Item it = find_item<ROWS>(a);
+    if (it.n_rows <= 0) return;                                // (the whole cluster)
+    Eight<T> raw[PER_WARP];
+    fetch_queries<T, ROWS>(a, it, warp, lane, raw);
+    TileRing<DP, SH::SLOTS> tiles(a, it, smem_addr(smem) + SH::Q_BYTES, warp, lane);
+    tiles.start();
+
+    // digit i of row r is column 4 (r % 2) + i of tile r / 2; a column's entries 16 t .. 16 t + 15 of a segment of 64 are
+    // read by thread t of the column's four
+#pragma unroll
+    for (int j = 0; j < PER_WARP; ++j) {
+        const int r = warp + j * WARPS;
+        if (r >= ROWS) break;
+        float v[8];
+        raw[j].numbers(v);
+        bool finite;
+        const int up = row_exponent(v, 29, finite);
+        const float f = power_of_two(up);
+        if (lane == 0) q_scale[r] = finite ? power_of_two(-up) : __int_as_float(0x7fc00000);
+        if (lane * 8 < DP) {
+            uint32_t dig[4][2] = {};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                int x = __float2int_rn(v[e] * f);
+#pragma unroll
+                for (int i = 3; i >= 0; --i) {
+                    const int low = (int)(int8_t)(x & 255);
+                    dig[i][e >> 2] |= (uint32_t)(low & 255) << (8 * (e & 3));
+                    x = (x - low) >> 8;
+                }
+            }
+            const int s = lane >> 3, t = (lane >> 1) & 3;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<uint2*>(smem + ((r >> 1) * SEGS + s) * 512 + ((4 * (r & 1) + i) * 4 + t) * 16 + (lane & 1) * 8) =
+                    make_uint2(dig[i][0], dig[i][1]);
+        }
+    }
+    __syncthreads();
+
+    // this thread's row of a tile: 2 q + t4 / 2 (and the two low digits of its scores where t4 is odd)
+    const float unit = a.cap > 0.0f ? (EXACT ? a.scale / a.cap : a.scale / a.cap * (2.0f * LOG2E)) : a.scale * LOG2E;
+    const float c1 = a.cap * LOG2E, c2 = 2.0f * a.cap * LOG2E;
+    const int window = a.window > 0 ? a.window : 0x3fffffff;
+    const float weight = t4 & 1 ? 1.0f : 65536.0f;
+    float qf[QT], m[QT], l[QT];
+    int pos[QT];
+#pragma unroll
+    for (int q = 0; q < QT; ++q) {
+        const int r = 2 * q + (t4 >> 1);
+        qf[q] = q_scale[r] * unit;
+        pos[q] = r < it.n_rows ? it.pos0 + (it.row0 + r) / a.group : -1;
+        m[q] = -INFINITY;
+        l[q] = 0.0f;
+    }
+    float o[SEGS][4][PT][2];
+#pragma unroll
+    for (int s = 0; s < SEGS; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int p = 0; p < PT; ++p) o[s][i][p][0] = o[s][i][p][1] = 0.0f;
+    const uint32_t q_frag = smem_addr(smem) + lane * 16;
+
+    for (int n = 0; n < tiles.n_tiles; ++n) {
+        const float2 sc = tiles.scales(n);
+        const int key0 = (tiles.t0 + n * WARPS) * KT;
+        uint32_t tile = tiles.next();
+
+        // S^T: keys 16 mt + g8 (+ 8) by digits 2 t4 (+ 1); two sums where there are few, so that one need not wait for the last
+        constexpr int SUMS = QT == 1 ? 2 : 1;
+        int zs[SUMS][2][QT][4];
+#pragma unroll
+        for (int c = 0; c < SUMS; ++c)
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                for (int q = 0; q < QT; ++q) zs[c][mt][q][0] = zs[c][mt][q][1] = zs[c][mt][q][2] = zs[c][mt][q][3] = 0;
+#pragma unroll
+        for (int s = 0; s < SEGS; ++s) {
+            uint4 qb[QT];
+#pragma unroll
+            for (int q = 0; q < QT; ++q) qb[q] = lds128(q_frag + (q * SEGS + s) * 512);
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt) {
+                const uint4 ka = lds128(tile + key_offset<DP>(16 * mt + g8, 4 * s + t4));
+                const uint4 kb = lds128(tile + key_offset<DP>(16 * mt + g8 + 8, 4 * s + t4));
+#pragma unroll
+                for (int q = 0; q < QT; ++q) {
+                    mma_s8(zs[0][mt][q], ka.x, kb.x, ka.y, kb.y, qb[q].x, qb[q].y);
+                    mma_s8(zs[SUMS - 1][mt][q], ka.z, kb.z, ka.w, kb.w, qb[q].z, qb[q].w);
+                }
+            }
+        }
+
+        // scores in log2 units, their maximum over the tile, weights relative to it
+        const bool edge = key0 + KT - 1 > it.pos_lo || key0 < it.pos_hi - window + 1;
+        float alpha[QT], coef[QT];
+        uint32_t digits[QT][2][2];                             // two digits of a weight, of keys 16 mt + 8 h + g8, at bits 0 and 16
+#pragma unroll
+        for (int q = 0; q < QT; ++q) {
+            const float to_z = qf[q] * sc.x;
+            float z[2][2], top = -INFINITY;
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    int hi = zs[0][mt][q][2 * h], lo = zs[0][mt][q][2 * h + 1];
+                    if constexpr (SUMS == 2) { hi += zs[1][mt][q][2 * h]; lo += zs[1][mt][q][2 * h + 1]; }
+                    float x = (float)(hi * 256 + lo) * weight;
+                    x += __shfl_xor_sync(0xffffffffu, x, 1);
+                    x *= to_z;
+                    if (a.cap > 0.0f) x = EXACT ? c1 * tanhf(x) : fmaf(-c2, rcp(1.0f + ex2(x)), c1);
+                    if (edge) {
+                        const int back = pos[q] - (key0 + 16 * mt + 8 * h + g8);
+                        if (back < 0 || back >= window) x = -INFINITY;
+                    }
+                    z[mt][h] = x;
+                    top = fmaxf(top, x);
+                }
+#pragma unroll
+            for (int w = 4; w < 32; w *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+            const bool seen = top > -INFINITY;
+            const float m_new = fmaxf(m[q], top), f = seen ? ex2(top - m_new) : 0.0f, from = seen ? top : 0.0f;
+            alpha[q] = m[q] == m_new ? 1.0f : ex2(m[q] - m_new);                 // (2^(-inf) = 0; both -inf: 1)
+            float sum = 0.0f;
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float p = ex2(z[mt][h] - from);
+                    sum += p;
+                    uint32_t two;                              // float32: digits 0, 1 or (t4 odd) 2, 3
+                    if constexpr (EXACT) {
+                        const uint32_t whole = __float2uint_rn(p * 2147483648.0f);
+                        two = t4 & 1 ? whole & 0xffffu : whole >> 16;
+                    } else {
+                        two = __float2uint_rn(p * 65535.0f);
+                    }
+                    digits[q][mt][h] = __byte_perm(two, 0, 0x4041);              // the high one first
+                }
+            m[q] = m_new;
+            l[q] = fmaf(l[q], alpha[q], f * sum);
+            coef[q] = seen ? sc.y * f * (EXACT ? weight * (1.0f / 2147483648.0f) : 1.0f / 65535.0f) : 0.0f;
+        }
+        // as the second product wants them: digit (column) g8 of keys 2 t4, 2 t4 + 1, 2 t4 + 8, 2 t4 + 9 in a word.  bfloat16:
+        // threads with even t4 give the rows of tile 2 p, those with odd t4 the rows of tile 2 p + 1
+        uint32_t pf[PT][2];
+        float pa[PT], pc[PT];
+#pragma unroll
+        for (int p = 0; p < PT; ++p) {
+            const int q0 = EXACT ? p : 2 * p, q1 = EXACT ? p : 2 * p + 1;
+            const bool other = !EXACT && (t4 & 1);
+            pa[p] = other ? (q1 < QT ? alpha[q1 < QT ? q1 : 0] : 1.0f) : alpha[q0];
+            pc[p] = other ? (q1 < QT ? coef[q1 < QT ? q1 : 0] : 0.0f) : coef[q0];
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt) {
+                uint32_t t[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    t[h] = transpose8x8(other ? (q1 < QT ? digits[q1 < QT ? q1 : 0][mt][h] : 0u) : digits[q0][mt][h]);
+                pf[p][mt] = __byte_perm(t[0], t[1], 0x6420);
+            }
+        }
+        bool still = true;
+#pragma unroll
+        for (int q = 0; q < QT; ++q) still = still && alpha[q] == 1.0f;
+        if (!__all_sync(0xffffffffu, still)) {
+#pragma unroll
+            for (int s = 0; s < SEGS; ++s)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int p = 0; p < PT; ++p) {
+                        o[s][i][p][0] *= pa[p];
+                        o[s][i][p][1] *= pa[p];
+                    }
+        }
+
+        // O^T: entries 64 s + 8 g8 + 2 i (+ 1) by digits 2 t4 (+ 1)
+        tile = tiles.next();
+#pragma unroll
+        for (int s = 0; s < SEGS; ++s) {
+            uint2 v[2][4];
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const int row = 16 * ks + 2 * t4 + (c & 1) + (c >> 1) * 8;
+                    v[ks][c] = lds64(tile + value_offset<DP>(row, 4 * s + (g8 >> 1)) + (g8 & 1) * 8);
+                }
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                uint32_t w[2][4];                              // entries 8 g8 + 4 half + 0 .. 3, four keys each
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks) {
+                    const uint32_t w0 = half ? v[ks][0].y : v[ks][0].x, w1 = half ? v[ks][1].y : v[ks][1].x;
+                    const uint32_t w2 = half ? v[ks][2].y : v[ks][2].x, w3 = half ? v[ks][3].y : v[ks][3].x;
+                    const uint32_t x0 = __byte_perm(w0, w1, 0x5140), x1 = __byte_perm(w0, w1, 0x7362);
+                    const uint32_t y0 = __byte_perm(w2, w3, 0x5140), y1 = __byte_perm(w2, w3, 0x7362);
+                    w[ks][0] = __byte_perm(x0, y0, 0x5410);
+                    w[ks][1] = __byte_perm(x0, y0, 0x7632);
+                    w[ks][2] = __byte_perm(x1, y1, 0x5410);
+                    w[ks][3] = __byte_perm(x1, y1, 0x7632);
+                }
+#pragma unroll
+                for (int i2 = 0; i2 < 2; ++i2) {
+                    const uint32_t af[4] = {w[0][2 * i2], w[0][2 * i2 + 1], w[1][2 * i2], w[1][2 * i2 + 1]};
+#pragma unroll
+                    for (int p = 0; p < PT; ++p) {
+                        int d[4];
+                        mma_s8u8(d, af, pf[p][0], pf[p][1]);
+                        float (&acc)[2] = o[s][2 * half + i2][p];
+                        acc[0] = fmaf((float)(d[0] * 256 + d[1]), pc[p], acc[0]);
+                        acc[1] = fmaf((float)(d[2] * 256 + d[3]), pc[p], acc[1]);
+                    }
+                }
+            }
+        }
+    }
+    copy_wait<0>();
+    pdl_trigger();
+    __syncthreads();
+
+    float* wo = reinterpret_cast<float*>(smem + SH::Q_BYTES);
+    float* wml = wo + WARPS * ROWS * SH::PITCH;
+    float* co = wml + WARPS * ROWS * 2;
+    float* cml = co + ROWS * SH::PITCH;
+#pragma unroll
+    for (int q = 0; q < QT; ++q) {
+        float sum = l[q];
+#pragma unroll
+        for (int w = 4; w < 32; w *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+        if (g8 == 0 && !(t4 & 1)) *reinterpret_cast<float2*>(wml + (warp * ROWS + 2 * q + (t4 >> 1)) * 2) = make_float2(m[q], sum);
+    }
+#pragma unroll
+    for (int p = 0; p < PT; ++p) {
+        const int r = EXACT ? 2 * p + (t4 >> 1) : 4 * p + (t4 >> 1) + 2 * (t4 & 1);
+        float* dst = wo + (warp * ROWS + r) * SH::PITCH + 8 * g8;
+#pragma unroll
+        for (int s = 0; s < SEGS; ++s) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x[e] = o[s][e >> 1][p][e & 1];
+                if constexpr (EXACT) x[e] += __shfl_xor_sync(0xffffffffu, x[e], 1);      // the low digits
+            }
+            if (r < it.n_rows && (!EXACT || !(t4 & 1))) {
+                *reinterpret_cast<float4*>(dst + 64 * s) = make_float4(x[0], x[1], x[2], x[3]);
+                *reinterpret_cast<float4*>(dst + 64 * s + 4) = make_float4(x[4], x[5], x[6], x[7]);
+            }
+        }
+    }
+    __syncthreads();
+    merge<T, ROWS, SH::PITCH>(a, it, wo, wml, co, cml, q_scale);
+}
+
+// --- more rows: f16 products, 16 rows a block ---------------------------------------------------------------------------
+
+template <typename T, int DP>
 struct Shape {
-    static constexpr int ROWS = 8 * NT;
+    static constexpr int NT = 2, ROWS = 8 * NT;
     static constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;
     static constexpr int SEGS = DP / 64;
     static constexpr int UNIT = KT * DP;                                   // a key or value tile
@@ -150,118 +711,40 @@ struct Shape {
     static constexpr int SMEM = Q_BYTES + (RING > MERGE ? RING : MERGE);
 };
 
-template <typename T, int DP, int NT>
+template <typename T, int DP>
 __global__ void __launch_bounds__(THREADS, 2) attn_kv8_kernel(AttnArgs a) {
-    using SH = Shape<T, DP, NT>;
-    constexpr int ROWS = SH::ROWS, PARTS = SH::PARTS, SEGS = SH::SEGS, UNIT = SH::UNIT, SLOTS = SH::SLOTS;
+    using SH = Shape<T, DP>;
+    constexpr int NT = SH::NT, ROWS = SH::ROWS, PARTS = SH::PARTS, SEGS = SH::SEGS;
     constexpr bool EXACT = sizeof(T) == 4;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ float q_scale[ROWS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, t4 = lane & 3;
-
-    const int share = blockIdx.x % a.shares;
-    int rest = blockIdx.x / a.shares;
-    const int span = rest % a.spans;
-    rest /= a.spans;
-    const int tile_of_rows = rest % a.row_tiles, b = rest / a.row_tiles;
-    const int g = blockIdx.y;
     pdl_wait();
-    const int first_tok = a.cu_q[b], n_tok = min(a.cu_q[b + 1], a.tokens) - first_tok;
-    const int row0 = tile_of_rows * ROWS, n_rows = min(ROWS, n_tok * a.group - row0);
-    if (n_rows <= 0) return;                                   // (the whole cluster)
-    const int kv_len = a.kv_len[b], slot = a.slots[b];
-    const int pos0 = kv_len - n_tok;                           // position of the sequence's first new token
-    const int pos_lo = pos0 + row0 / a.group, pos_hi = pos0 + (row0 + n_rows - 1) / a.group;
-    const int window = a.window > 0 ? a.window : 0x3fffffff;
+    const Item it = find_item<ROWS>(a);
+    if (it.n_rows <= 0) return;                                // (the whole cluster)
+    Eight<T> raw[ROWS / WARPS];
+    fetch_queries<T, ROWS>(a, it, warp, lane, raw);
+    TileRing<DP, SH::SLOTS> tiles(a, it, smem_addr(smem) + SH::Q_BYTES, warp, lane);
+    tiles.start();
 
-    // the tiles of this share: [t_begin, t_end), the warps in turn
-    int t_begin = 0, t_end = 0;
-    if (pos_hi >= 0 && slot >= 0 && slot < a.n_slots) {
-        const int t_lo = max(0, pos_lo - window + 1) / KT, t_hi = pos_hi / KT;
-        const int parts = a.shares * a.spans, per = (t_hi - t_lo + parts) / parts;
-        t_begin = t_lo + (span * a.shares + share) * per;
-        t_end = min(t_hi + 1, t_begin + per);
-    }
-    const int n_tiles = t_begin + warp < t_end ? (t_end - t_begin - warp + WARPS - 1) / WARPS : 0;
-    const int32_t* table = a.tables + (size_t)max(slot, 0) * a.width;
-
-    // of this warp's tiles n .. n + 31, lane by lane: where the numbers lie and their scales
-    auto look_up = [&](int n, long long& at, float& sk, float& sv) {
-        at = 0;
-        sk = sv = 0.0f;
-        if (n + lane < n_tiles) {
-            const long long key = (long long)(t_begin + warp + (n + lane) * WARPS) * KT;
-            const int place = a.ring > 0 ? (int)(key % a.ring) : (int)key, e = place / a.block;
-            int id = e < a.width ? table[e] : 0;
-            if (id < 0 || id >= a.n_blocks) id = 0;            // (never followed out of the cache)
-            const size_t bh = (size_t)id * a.n_kv + g;
-            at = (long long)bh * a.block + (place - e * a.block);
-            sk = a.k_scale[bh];
-            sv = a.v_scale[bh];
-            if (sk != sk || sv != sv) {                        // a NaN block: scores of zero, values of NaN
-                sk = 0.0f;
-                sv = __int_as_float(0x7fc00000);
-            }
-        }
-    };
-    long long at_l;                                            // of the tiles that are being asked for
-    float sk_l, sv_l, sk_c = 0.0f, sv_c = 0.0f;                // .. and the scales of those that are being multiplied
-    look_up(0, at_l, sk_l, sv_l);
-
-    const uint32_t ring = smem_addr(smem) + SH::Q_BYTES + warp * SLOTS * UNIT;
-    const int n_units = 2 * n_tiles;
-    auto load_unit = [&](int u) {                              // key tile u / 2 or value tile u / 2 into slot u % SLOTS
-        const int n = u >> 1;
-        if (u > 0 && (u & 63) == 0) look_up(n, at_l, sk_l, sv_l);
-        const long long at = __shfl_sync(0xffffffffu, at_l, n & 31);
-        const int8_t* src = (u & 1 ? a.v_pages : a.k_pages) + at * a.dim;
-        const uint32_t dst = ring + (u % SLOTS) * UNIT;
+    // the query rows, scaled to below 2^14 and laid out as the products read them (entry 16 t + e of a segment of 64 belongs
+    // to thread t of the row's four; eight entries are 16 bytes)
 #pragma unroll
-        for (int i = 0; i < DP / 16; ++i) {
-            const int piece = i * 32 + lane, row = piece / (DP / 16), c = piece % (DP / 16);
-            if (c * 16 < a.dim)
-                copy16(dst + (u & 1 ? value_offset<DP>(row, c) : key_offset<DP>(row, c)), src + row * a.dim + c * 16, true);
-        }
-    };
-#pragma unroll
-    for (int u = 0; u < SLOTS - 1; ++u) {
-        if (u < n_units) load_unit(u);
-        copy_commit();
-    }
-
-    // the query rows, a warp a row: scaled to below 2^14 and laid out as the products read them (entry 16 t + e of a
-    // segment of 64 belongs to thread t of the row's four; eight entries are 16 bytes)
-    for (int r = warp; r < ROWS; r += WARPS) {
-        float v[8] = {};
-        if (r < n_rows && lane * 8 < a.dim) {
-            const int row = row0 + r;
-            const T* src = reinterpret_cast<const T*>(a.q) + (size_t)(first_tok + row / a.group) * a.q_stride +
-                           (g * a.group + row % a.group) * a.dim + lane * 8;
-            if (a.wide) load8(src, v);
-            else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = to_float(src[e]);
-            }
-        }
-        float most = 0.0f;
-        bool finite = true;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            most = fmaxf(most, fabsf(v[e]));
-            finite = finite && fabsf(v[e]) < INFINITY;
-        }
-        most = warp_max(most);
-        finite = __all_sync(0xffffffffu, finite);
-        const int up = min(13 - ((int)(__float_as_uint(most) >> 23) - 127), 120);
-        const float f = finite ? power_of_two(max(up, -126)) : 0.0f;
-        if (lane == 0) q_scale[r] = finite ? power_of_two(-max(up, -126)) : __int_as_float(0x7fc00000);
+    for (int j = 0; j < ROWS / WARPS; ++j) {
+        const int r = warp + j * WARPS;
+        float v[8];
+        raw[j].numbers(v);
+        bool finite;
+        const int up = row_exponent(v, 13, finite);
+        const float f = power_of_two(up);
+        if (lane == 0) q_scale[r] = finite ? power_of_two(-up) : __int_as_float(0x7fc00000);
         if (lane * 8 < DP) {
             const int s = lane >> 3, t = (lane >> 1) & 3, half = lane & 1;
             uint8_t* dst = smem + ((((r >> 3) * SEGS + s) * 2 + half) * 32 + (r & 7) * 4 + t) * 16;
             uint32_t hi[4], lo[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float x = finite ? v[2 * e] * f : 0.0f, y = finite ? v[2 * e + 1] * f : 0.0f;
+                const float x = v[2 * e] * f, y = v[2 * e + 1] * f;
                 const __half2 h = __floats2half2_rn(x, y);
                 hi[e] = *reinterpret_cast<const uint32_t*>(&h);
                 if constexpr (PARTS == 2) lo[e] = pack_half(x - __low2float(h), y - __high2float(h));
@@ -283,7 +766,7 @@ __global__ void __launch_bounds__(THREADS, 2) attn_kv8_kernel(AttnArgs a) {
         for (int e = 0; e < 2; ++e) {
             const int r = nt * 8 + t4 * 2 + e;
             qf[nt][e] = q_scale[r] * unit;
-            pos[nt][e] = r < n_rows ? pos0 + (row0 + r) / a.group : -1;
+            pos[nt][e] = r < it.n_rows ? it.pos0 + (it.row0 + r) / a.group : -1;
             m[nt][e] = -INFINITY;
             l[nt][e] = 0.0f;
         }
@@ -295,22 +778,13 @@ __global__ void __launch_bounds__(THREADS, 2) attn_kv8_kernel(AttnArgs a) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) o[s][i][nt][0] = o[s][i][nt][1] = o[s][i][nt][2] = o[s][i][nt][3] = 0.0f;
 
-    int unit_no = 0;
-    auto next_unit = [&]() -> uint32_t {                       // waits for the next unit and asks for one more; its address
-        copy_wait<SLOTS - 2>();
-        __syncwarp();                                          // it has landed for all lanes; all are done with the one before
-        if (unit_no + SLOTS - 1 < n_units) load_unit(unit_no + SLOTS - 1);
-        copy_commit();
-        return ring + (unit_no++ % SLOTS) * UNIT;
-    };
+    const int window = a.window > 0 ? a.window : 0x3fffffff;
     const uint32_t q_frag = smem_addr(smem) + lane * 16;
 
-    for (int n = 0; n < n_tiles; ++n) {
-        // (the scales of the next 32 tiles have been asked for when the first of them was, one or more tiles ago)
-        if ((n & 31) == 0) { sk_c = sk_l; sv_c = sv_l; }
-        const float sk = __shfl_sync(0xffffffffu, sk_c, n & 31), sv = __shfl_sync(0xffffffffu, sv_c, n & 31);
-        const int key0 = (t_begin + warp + n * WARPS) * KT;
-        uint32_t tile = next_unit();
+    for (int n = 0; n < tiles.n_tiles; ++n) {
+        const float2 sc = tiles.scales(n);
+        const int key0 = (tiles.t0 + n * WARPS) * KT;
+        uint32_t tile = tiles.next();
 
         // S^T: keys 16 mt + g8 (+ 8) by query rows 2 t4 (+ 1)
         float z[2][NT][4];
@@ -347,7 +821,7 @@ __global__ void __launch_bounds__(THREADS, 2) attn_kv8_kernel(AttnArgs a) {
         }
 
         // scores in log2 units, their maximum over the tile, weights relative to it
-        const bool edge = key0 + KT - 1 > pos_lo || key0 < pos_hi - window + 1;
+        const bool edge = key0 + KT - 1 > it.pos_lo || key0 < it.pos_hi - window + 1;
         float alpha[NT][2], coef[NT][2];
         uint32_t pf[PARTS][2][NT][2];
 #pragma unroll
@@ -357,7 +831,7 @@ __global__ void __launch_bounds__(THREADS, 2) attn_kv8_kernel(AttnArgs a) {
             for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    float x = z[mt][nt][e] * (qf[nt][e & 1] * sk);
+                    float x = z[mt][nt][e] * (qf[nt][e & 1] * sc.x);
                     if (a.cap > 0.0f) x = EXACT ? c1 * tanhf(x) : fmaf(-c2, rcp(1.0f + ex2(x)), c1);
                     if (edge) {
                         const int back = pos[nt][e & 1] - (key0 + 16 * mt + g8 + (e & 2) * 4);
@@ -386,7 +860,7 @@ __global__ void __launch_bounds__(THREADS, 2) attn_kv8_kernel(AttnArgs a) {
                     }
                 m[nt][e] = m_new;
                 l[nt][e] = fmaf(l[nt][e], alpha[nt][e], f * sum);
-                coef[nt][e] = seen ? sv * f : 0.0f;
+                coef[nt][e] = seen ? sc.y * f : 0.0f;
             }
 #pragma unroll
             for (int mt = 0; mt < 2; ++mt)
@@ -413,7 +887,7 @@ __global__ void __launch_bounds__(THREADS, 2) attn_kv8_kernel(AttnArgs a) {
         }
 
         // O^T: entries 64 s + 8 g8 + 2 i (+ 1) by query rows 2 t4 (+ 1)
-        tile = next_unit();
+        tile = tiles.next();
 #pragma unroll
         for (int s = 0; s < SEGS; ++s) {
             uint2 v[2][4];
@@ -456,11 +930,10 @@ __global__ void __launch_bounds__(THREADS, 2) attn_kv8_kernel(AttnArgs a) {
     pdl_trigger();
     __syncthreads();
 
-    // the four warps' results, then the cluster's, then (spans > 1) the launch's second kernel
-    float* wo = reinterpret_cast<float*>(smem + SH::Q_BYTES);          // [WARPS][ROWS][PITCH]
-    float* wml = wo + WARPS * ROWS * SH::PITCH;                        // [WARPS][ROWS][2]
-    float* co = wml + WARPS * ROWS * 2;                                // [ROWS][PITCH]
-    float* cml = co + ROWS * SH::PITCH;                                // [ROWS][2]
+    float* wo = reinterpret_cast<float*>(smem + SH::Q_BYTES);
+    float* wml = wo + WARPS * ROWS * SH::PITCH;
+    float* co = wml + WARPS * ROWS * 2;
+    float* cml = co + ROWS * SH::PITCH;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -473,7 +946,7 @@ __global__ void __launch_bounds__(THREADS, 2) attn_kv8_kernel(AttnArgs a) {
                 wml[(warp * ROWS + r) * 2] = m[nt][e];
                 wml[(warp * ROWS + r) * 2 + 1] = sum;
             }
-            if (r < n_rows) {
+            if (r < it.n_rows) {
                 float* dst = wo + (warp * ROWS + r) * SH::PITCH + 8 * g8;
 #pragma unroll
                 for (int s = 0; s < SEGS; ++s) {
@@ -483,65 +956,7 @@ __global__ void __launch_bounds__(THREADS, 2) attn_kv8_kernel(AttnArgs a) {
             }
         }
     __syncthreads();
-    const int d4 = a.dim >> 2;
-    for (int it = threadIdx.x; it < n_rows * d4; it += THREADS) {
-        const int r = it / d4, d = (it - r * d4) * 4;
-        float most = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) most = fmaxf(most, wml[(w * ROWS + r) * 2]);
-        float sum = 0.0f;
-        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
-            const float f = most > -INFINITY ? ex2(wml[(w * ROWS + r) * 2] - most) : 0.0f;
-            const float4 x = *reinterpret_cast<const float4*>(wo + (w * ROWS + r) * SH::PITCH + d);
-            sum = fmaf(wml[(w * ROWS + r) * 2 + 1], f, sum);
-            acc.x = fmaf(x.x, f, acc.x); acc.y = fmaf(x.y, f, acc.y); acc.z = fmaf(x.z, f, acc.z); acc.w = fmaf(x.w, f, acc.w);
-        }
-        *reinterpret_cast<float4*>(co + r * SH::PITCH + d) = acc;
-        if (d == 0) {
-            cml[r * 2] = most;
-            cml[r * 2 + 1] = sum;
-        }
-    }
-    if (a.shares > 1) cluster_barrier();
-    else __syncthreads();
-    for (int it = share * THREADS + threadIdx.x; it < n_rows * d4; it += a.shares * THREADS) {
-        const int r = it / d4, d = (it - r * d4) * 4;
-        const uint32_t o_at = smem_addr(co + r * SH::PITCH + d), ml_at = smem_addr(cml + r * 2);
-        float most = -INFINITY, sum = 0.0f;
-        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (a.shares == 1) {
-            most = cml[r * 2];
-            sum = cml[r * 2 + 1];
-            acc = *reinterpret_cast<const float4*>(co + r * SH::PITCH + d);
-        } else {
-            for (int s = 0; s < a.shares; ++s) most = fmaxf(most, ld_cluster2(of_rank(ml_at, s)).x);
-#pragma unroll 4
-            for (int s = 0; s < a.shares; ++s) {
-                const float2 ml = ld_cluster2(of_rank(ml_at, s));
-                const float4 x = ld_cluster4(of_rank(o_at, s));
-                const float f = most > -INFINITY ? ex2(ml.x - most) : 0.0f;
-                sum = fmaf(ml.y, f, sum);
-                acc.x = fmaf(x.x, f, acc.x); acc.y = fmaf(x.y, f, acc.y); acc.z = fmaf(x.z, f, acc.z); acc.w = fmaf(x.w, f, acc.w);
-            }
-        }
-        const int row = row0 + r, tok = first_tok + row / a.group, head = g * a.group + row % a.group;
-        if (q_scale[r] != q_scale[r]) acc.x = acc.y = acc.z = acc.w = pos0 + row / a.group >= 0 ? q_scale[r] : 0.0f;
-        if (a.spans > 1) {
-            const size_t at = ((size_t)tok * a.n_kv * a.group + head) * a.spans + span;
-            *reinterpret_cast<float4*>(a.part_o + at * a.dim + d) = acc;
-            if (d == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(most, sum);
-        } else {
-            const float inv = sum > 0.0f ? 1.0f / sum : (acc.x != acc.x ? 1.0f : 0.0f);
-            T* dst = reinterpret_cast<T*>(a.out) + (size_t)tok * a.out_stride + head * a.dim + d;
-            dst[0] = from_float<T>(acc.x * inv);
-            dst[1] = from_float<T>(acc.y * inv);
-            dst[2] = from_float<T>(acc.z * inv);
-            dst[3] = from_float<T>(acc.w * inv);
-        }
-    }
-    if (a.shares > 1) cluster_barrier();                       // nobody leaves while its results are being read
+    merge<T, ROWS, SH::PITCH>(a, it, wo, wml, co, cml, q_scale);
 }
 
 // Rows whose keys were shared by several clusters: a block of threads for every (token, head).
@@ -552,37 +967,45 @@ __global__ void __launch_bounds__(64) attn_kv8_join_kernel(AttnArgs a) {
     const int tok = blockIdx.x, head = blockIdx.y;
     if (tok >= a.cu_q[a.rows]) return;
     const size_t at = ((size_t)tok * a.n_kv * a.group + head) * a.spans;
-    float most = -INFINITY, sum = 0.0f;
-    for (int s = 0; s < a.spans; ++s) most = fmaxf(most, a.part_ml[(at + s) * 2]);
     const int d = threadIdx.x * 4;
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (d >= a.dim) return;
-    for (int s = 0; s < a.spans; ++s) {
-        const float f = most > -INFINITY ? ex2(a.part_ml[(at + s) * 2] - most) : 0.0f;
-        const float4 x = *reinterpret_cast<const float4*>(a.part_o + (at + s) * a.dim + d);
-        sum = fmaf(a.part_ml[(at + s) * 2 + 1], f, sum);
-        acc.x = fmaf(x.x, f, acc.x); acc.y = fmaf(x.y, f, acc.y); acc.z = fmaf(x.z, f, acc.z); acc.w = fmaf(x.w, f, acc.w);
+    float most = -INFINITY, sum = 0.0f;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int s0 = 0; s0 < a.spans; s0 += 8) {                  // (eight parts are asked for at once)
+        float2 ml[8];
+        float4 x[8];
+        float top = most;
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+            ml[s] = make_float2(-INFINITY, 0.0f);
+            x[s] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (s0 + s < a.spans) {
+                ml[s] = *reinterpret_cast<const float2*>(a.part_ml + (at + s0 + s) * 2);
+                x[s] = *reinterpret_cast<const float4*>(a.part_o + (at + s0 + s) * a.dim + d);
+            }
+            top = fmaxf(top, ml[s].x);
+        }
+        const float keep = most > -INFINITY ? ex2(most - top) : 1.0f;
+        most = top;
+        sum *= keep;
+        acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+            if (s0 + s < a.spans) add_part(acc, sum, x[s], ml[s].y, top > -INFINITY ? ex2(ml[s].x - top) : 0.0f);
     }
-    const float inv = sum > 0.0f ? 1.0f / sum : (acc.x != acc.x ? 1.0f : 0.0f);
-    T* dst = reinterpret_cast<T*>(a.out) + (size_t)tok * a.out_stride + head * a.dim + d;
-    dst[0] = from_float<T>(acc.x * inv);
-    dst[1] = from_float<T>(acc.y * inv);
-    dst[2] = from_float<T>(acc.z * inv);
-    dst[3] = from_float<T>(acc.w * inv);
+    store_row<T>(a, tok, head, d, acc, sum);
 }
 
-template <typename T, int DP, int NT>
-int launch(const AttnArgs& a, cudaStream_t stream) {
-    using SH = Shape<T, DP, NT>;
-    static OncePerDevice raised;
-    const int st = allow_shared_memory(attn_kv8_kernel<T, DP, NT>, SH::SMEM, raised);
+template <typename T>
+int launch(void (*kernel)(AttnArgs), size_t smem, OncePerDevice& raised, const AttnArgs& a, cudaStream_t stream) {
+    const int st = allow_shared_memory(kernel, smem, raised);
     if (st) return st;
     cudaLaunchConfig_t cfg = {};
     const long long blocks = (long long)a.rows * a.row_tiles * a.spans * a.shares;
     if (blocks > 0x7fffffffll) return BROLM_ERR_TOO_LARGE;
     cfg.gridDim = dim3((unsigned)blocks, a.n_kv);
     cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = SH::SMEM;
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -592,43 +1015,58 @@ int launch(const AttnArgs& a, cudaStream_t stream) {
     attr[1].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    const int e = (int)cudaLaunchKernelEx(&cfg, attn_kv8_kernel<T, DP, NT>, a);
+    const int e = (int)cudaLaunchKernelEx(&cfg, kernel, a);
     if (e || a.spans == 1) return e;
     return launch_pdl(attn_kv8_join_kernel<T>, dim3(a.tokens, a.n_kv * a.group), dim3(64), 0, stream, a);
 }
 
-template <typename T, int NT>
-int launch_dim(const AttnArgs& a, cudaStream_t stream) {
-    if (a.dim <= 64) return launch<T, 64, NT>(a, stream);
-    if (a.dim <= 128) return launch<T, 128, NT>(a, stream);
-    if (a.dim <= 192) return launch<T, 192, NT>(a, stream);
-    return launch<T, 256, NT>(a, stream);
+template <typename T, int DP>
+int launch_rows(const AttnArgs& a, int rows, cudaStream_t stream) {
+    static OncePerDevice raised[4];
+    if (rows == 2) return launch<T>(attn_kv8_few_kernel<T, DP, 2>, FewShape<T, DP, 2>::SMEM, raised[0], a, stream);
+    if (rows == 4) return launch<T>(attn_kv8_few_kernel<T, DP, 4>, FewShape<T, DP, 4>::SMEM, raised[1], a, stream);
+    if (rows == 8) return launch<T>(attn_kv8_few_kernel<T, DP, 8>, FewShape<T, DP, 8>::SMEM, raised[2], a, stream);
+    return launch<T>(attn_kv8_kernel<T, DP>, Shape<T, DP>::SMEM, raised[3], a, stream);
+}
+
+template <typename T>
+int launch_dim(const AttnArgs& a, int rows, cudaStream_t stream) {
+    if (a.dim <= 64) return launch_rows<T, 64>(a, rows, stream);
+    if (a.dim <= 128) return launch_rows<T, 128>(a, rows, stream);
+    if (a.dim <= 192) return launch_rows<T, 192>(a, rows, stream);
+    return launch_rows<T, 256>(a, rows, stream);
 }
 
 }  // namespace
 
 // shares (1 .. 8): blocks of a cluster that share a row's keys; spans: clusters that do, joined by a second launch through
 // part_o [tokens * n_kv * group * spans * dim] and part_ml [.. * 2].
-BROLM_API int brolm_attn_kv8(const void* q, int q_stride, void* out, int out_stride, int dtype, const void* cu_q,
-                             const void* kv_len, const void* slots, const void* tables, const void* k_pages,
-                             const void* v_pages, const void* k_scale, const void* v_scale, int tokens, int rows, int n_kv,
-                             int group, int dim, int block, int n_blocks, int n_slots, int width, int ring, int window,
-                             float scale, float cap, int max_q_len, int shares, int spans, void* part_o, void* part_ml,
-                             cudaStream_t stream) {
-    if (dtype != BROLM_F32 && dtype != BROLM_BF16) return BROLM_ERR_BAD_DTYPE;
-    if (tokens < 0 || rows < 0 || n_kv <= 0 || group <= 0 || dim <= 0 || dim % 16 || block <= 0 || block % 32) return BROLM_ERR_BAD_SIZE;
-    if (n_blocks <= 0 || n_slots <= 0 || width <= 0 || ring < 0 || ring % block || window < 0 || max_q_len <= 0) return BROLM_ERR_BAD_SIZE;
-    if (shares < 1 || shares > 8 || spans < 1 || (spans > 1 && (!part_o || !part_ml))) return BROLM_ERR_BAD_SIZE;
-    if (dim > MAX_DIM || block > MAX_BLOCK || (long long)n_kv * group > 65535 || (long long)max_q_len * group > 0x3fffffff) return BROLM_ERR_TOO_LARGE;
-    if ((long long)n_blocks * block > 0x7fffffffll || tokens > 0x3fffffff) return BROLM_ERR_TOO_LARGE;
-    if (((uintptr_t)k_pages | (uintptr_t)v_pages) & 15) return BROLM_ERR_ALIGNMENT;
-    if (tokens == 0 || rows == 0) return BROLM_OK;
-    const int size = dtype == BROLM_F32 ? 4 : 2, most = max_q_len * group, per = most <= 8 ? 8 : 16;
-    const int wide = ((uintptr_t)q & 15) == 0 && (long long)q_stride * size % 16 == 0;
-    AttnArgs a{q, out, q_stride, out_stride, (const int32_t*)cu_q, (const int32_t*)kv_len, (const int32_t*)slots,
-               (const int32_t*)tables, (const int8_t*)k_pages, (const int8_t*)v_pages, (const float*)k_scale,
-               (const float*)v_scale, tokens, rows, n_kv, group, dim, block, n_blocks, n_slots, width, ring, window, scale, cap,
-               shares, spans, (most + per - 1) / per, wide, (float*)part_o, (float*)part_ml};
-    if (dtype == BROLM_F32) return per == 8 ? launch_dim<float, 1>(a, stream) : launch_dim<float, 2>(a, stream);
-    return per == 8 ? launch_dim<bf16, 1>(a, stream) : launch_dim<bf16, 2>(a, stream);
+struct AttnCall {
+    const void* q;
+    void* out;
+    const void *cu_q, *kv_len, *slots, *tables, *k_pages, *v_pages, *k_scale, *v_scale;
+    void *part_o, *part_ml;
+    cudaStream_t stream;
+    int q_stride, out_stride, dtype, tokens, rows, n_kv, group, dim, block, n_blocks, n_slots, width, ring, window, max_q_len, shares, spans;
+    float scale, cap;
+};
+
+BROLM_API int brolm_attn_kv8(const AttnCall* c) {
+    const int n_kv = c->n_kv, group = c->group, dim = c->dim, block = c->block;
+    if (c->dtype != BROLM_F32 && c->dtype != BROLM_BF16) return BROLM_ERR_BAD_DTYPE;
+    if (c->tokens < 0 || c->rows < 0 || n_kv <= 0 || group <= 0 || dim <= 0 || dim % 16 || block <= 0 || block % 32) return BROLM_ERR_BAD_SIZE;
+    if (c->n_blocks <= 0 || c->n_slots <= 0 || c->width <= 0 || c->ring < 0 || c->ring % block || c->window < 0 || c->max_q_len <= 0) return BROLM_ERR_BAD_SIZE;
+    if (c->shares < 1 || c->shares > MAX_SHARES || c->spans < 1 || (c->spans > 1 && (!c->part_o || !c->part_ml))) return BROLM_ERR_BAD_SIZE;
+    if (dim > MAX_DIM || block > MAX_BLOCK || (long long)n_kv * group > 65535 || (long long)c->max_q_len * group > 0x3fffffff) return BROLM_ERR_TOO_LARGE;
+    if ((long long)c->n_blocks * block > 0x7fffffffll || c->tokens > 0x3fffffff) return BROLM_ERR_TOO_LARGE;
+    if (((uintptr_t)c->k_pages | (uintptr_t)c->v_pages | (uintptr_t)c->part_o) & 15) return BROLM_ERR_ALIGNMENT;
+    if (c->tokens == 0 || c->rows == 0) return BROLM_OK;
+    const int size = c->dtype == BROLM_F32 ? 4 : 2, most = c->max_q_len * group, per = most <= 2 ? 2 : most <= 4 ? 4 : most <= 8 ? 8 : 16;
+    const int wide = ((uintptr_t)c->q & 15) == 0 && (long long)c->q_stride * size % 16 == 0;
+    AttnArgs a{c->q, c->out, c->q_stride, c->out_stride, (const int32_t*)c->cu_q, (const int32_t*)c->kv_len,
+               (const int32_t*)c->slots, (const int32_t*)c->tables, (const int8_t*)c->k_pages, (const int8_t*)c->v_pages,
+               (const float*)c->k_scale, (const float*)c->v_scale, c->tokens, c->rows, n_kv, group, dim, block, c->n_blocks,
+               c->n_slots, c->width, c->ring, c->window, c->scale, c->cap, c->shares, c->spans, (most + per - 1) / per, wide,
+               (float*)c->part_o, (float*)c->part_ml};
+    return c->dtype == BROLM_F32 ? launch_dim<float>(a, per, c->stream) : launch_dim<bf16>(a, per, c->stream);
 }
