@@ -273,29 +273,41 @@ int launch_cluster(void (*kernel)(Args), const Args& a, long long work, size_t s
 
 }  // namespace
 
-BROLM_API int brolm_blocks_extend(const void* slots, const void* lengths, const void* fresh, void* tables, void* held,
-                                  const void* stack, void* count, void* cu_q, void* kv_len, void* positions, void* tok_seq,
-                                  void* cache_rows, void* status, int rows, int n_slots, int width, int stack_size, int block,
-                                  int ring, int tokens, cudaStream_t stream) {
-    if (rows < 0 || n_slots <= 0 || width <= 0 || stack_size < 0 || block <= 0 || tokens < 0) return BROLM_ERR_BAD_SIZE;
-    if (ring < 0 || ring % block) return BROLM_ERR_BAD_SIZE;
-    if (rows > MAX_ROWS || n_slots > MAX_SLOTS) return BROLM_ERR_TOO_LARGE;
-    if ((long long)stack_size * block > 0x7fffffffll) return BROLM_ERR_TOO_LARGE;          // (a cache row is 31 bits)
-    ExtendArgs a{(const int32_t*)slots, (const int32_t*)lengths, (const int32_t*)fresh, (int32_t*)tables, (int32_t*)held,
-                 (int32_t*)count, (const int32_t*)stack, (int32_t*)cu_q, (int32_t*)kv_len, (int32_t*)positions,
-                 (int32_t*)tok_seq, (int32_t*)cache_rows, (int32_t*)status, rows, n_slots, width, stack_size, block, ring, tokens};
+struct ExtendCall {
+    const void *slots, *lengths, *fresh;
+    void *tables, *held;
+    const void* stack;
+    void *count, *cu_q, *kv_len, *positions, *tok_seq, *cache_rows, *status;
+    cudaStream_t stream;
+    int rows, n_slots, width, stack_size, block, ring, tokens;
+};
+struct ReleaseCall {
+    const void *slots, *tables;
+    void *held, *stack, *count, *status;
+    cudaStream_t stream;
+    int rows, n_slots, width, stack_size;
+};
+
+BROLM_API int brolm_blocks_extend(const ExtendCall* c) {
+    if (c->rows < 0 || c->n_slots <= 0 || c->width <= 0 || c->stack_size < 0 || c->block <= 0 || c->tokens < 0) return BROLM_ERR_BAD_SIZE;
+    if (c->ring < 0 || c->ring % c->block) return BROLM_ERR_BAD_SIZE;
+    if (c->rows > MAX_ROWS || c->n_slots > MAX_SLOTS) return BROLM_ERR_TOO_LARGE;
+    if ((long long)c->stack_size * c->block > 0x7fffffffll) return BROLM_ERR_TOO_LARGE;    // (a cache row is 31 bits)
+    ExtendArgs a{(const int32_t*)c->slots, (const int32_t*)c->lengths, (const int32_t*)c->fresh, (int32_t*)c->tables,
+                 (int32_t*)c->held, (int32_t*)c->count, (const int32_t*)c->stack, (int32_t*)c->cu_q, (int32_t*)c->kv_len,
+                 (int32_t*)c->positions, (int32_t*)c->tok_seq, (int32_t*)c->cache_rows, (int32_t*)c->status, c->rows, c->n_slots,
+                 c->width, c->stack_size, c->block, c->ring, c->tokens};
     static OncePerDevice raised;
-    const size_t smem = (size_t)(5 * rows + 2 + (n_slots + 31) / 32) * 4;
-    return launch_cluster(blocks_extend_kernel, a, tokens, smem, raised, stream);
+    const size_t smem = (size_t)(5 * c->rows + 2 + (c->n_slots + 31) / 32) * 4;
+    return launch_cluster(blocks_extend_kernel, a, c->tokens, smem, raised, c->stream);
 }
 
-BROLM_API int brolm_blocks_release(const void* slots, const void* tables, void* held, void* stack, void* count, void* status,
-                                   int rows, int n_slots, int width, int stack_size, cudaStream_t stream) {
-    if (rows < 0 || n_slots <= 0 || width <= 0 || stack_size < 0) return BROLM_ERR_BAD_SIZE;
-    if (rows > MAX_ROWS || n_slots > MAX_SLOTS) return BROLM_ERR_TOO_LARGE;
-    ReleaseArgs a{(const int32_t*)slots, (const int32_t*)tables, (int32_t*)held, (int32_t*)stack, (int32_t*)count,
-                  (int32_t*)status, rows, n_slots, width, stack_size};
+BROLM_API int brolm_blocks_release(const ReleaseCall* c) {
+    if (c->rows < 0 || c->n_slots <= 0 || c->width <= 0 || c->stack_size < 0) return BROLM_ERR_BAD_SIZE;
+    if (c->rows > MAX_ROWS || c->n_slots > MAX_SLOTS) return BROLM_ERR_TOO_LARGE;
+    ReleaseArgs a{(const int32_t*)c->slots, (const int32_t*)c->tables, (int32_t*)c->held, (int32_t*)c->stack, (int32_t*)c->count,
+                  (int32_t*)c->status, c->rows, c->n_slots, c->width, c->stack_size};
     static OncePerDevice raised;
-    const size_t smem = (size_t)(2 * rows + 1 + (n_slots + 31) / 32) * 4;
-    return launch_cluster(blocks_release_kernel, a, (long long)rows * 16, smem, raised, stream);
+    const size_t smem = (size_t)(2 * c->rows + 1 + (c->n_slots + 31) / 32) * 4;
+    return launch_cluster(blocks_release_kernel, a, (long long)c->rows * 16, smem, raised, c->stream);
 }

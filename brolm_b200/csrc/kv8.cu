@@ -223,42 +223,53 @@ int launch_write(const WriteArgs& a, dim3 grid, int threads, bool wide, cudaStre
 
 }  // namespace
 
-BROLM_API int brolm_kv8_write(const void* k, long long k_token, long long k_head, const void* v, long long v_token,
-                              long long v_head, int dtype, const void* cu_q, const void* positions, const void* cache_rows,
-                              void* k_pages, void* v_pages, void* k_scale, void* v_scale, int tokens, int rows, int n_kv, int dim,
-                              int block, int n_blocks, int max_q_len, cudaStream_t stream) {
-    if (dtype != BROLM_F32 && dtype != BROLM_BF16) return BROLM_ERR_BAD_DTYPE;
-    if (tokens < 0 || rows < 0) return BROLM_ERR_BAD_SIZE;
-    const int st = check_cache(k_pages, v_pages, n_kv, dim, block, n_blocks);
+struct WriteCall {
+    const void *k, *v, *cu_q, *positions, *cache_rows;
+    void *k_pages, *v_pages, *k_scale, *v_scale;
+    cudaStream_t stream;
+    long long k_token, v_token, k_head, v_head;
+    int dtype, tokens, rows, n_kv, dim, block, n_blocks, max_q_len;
+};
+struct ReadCall {
+    const void *cu_r, *kv_len, *slots, *tables, *k_pages, *v_pages, *k_scale, *v_scale;
+    void *k, *v;
+    cudaStream_t stream;
+    long long k_token, v_token, k_head, v_head;
+    int dtype, tokens, rows, n_kv, dim, block, n_blocks, n_slots, width, ring;
+};
+
+BROLM_API int brolm_kv8_write(const WriteCall* c) {
+    if (c->dtype != BROLM_F32 && c->dtype != BROLM_BF16) return BROLM_ERR_BAD_DTYPE;
+    if (c->tokens < 0 || c->rows < 0) return BROLM_ERR_BAD_SIZE;
+    const int st = check_cache(c->k_pages, c->v_pages, c->n_kv, c->dim, c->block, c->n_blocks);
     if (st) return st;
-    if (tokens == 0 || rows == 0) return BROLM_OK;
-    const long long places = max_q_len <= 1 ? rows : (long long)tokens / block + 2ll * rows;
+    if (c->tokens == 0 || c->rows == 0) return BROLM_OK;
+    const bool single = c->max_q_len <= 1;
+    const long long places = single ? c->rows : (long long)c->tokens / c->block + 2ll * c->rows;
     if (places > 0x7fffffffll) return BROLM_ERR_TOO_LARGE;
-    WriteArgs a{{k, v}, {k_token, v_token}, {k_head, v_head}, {(int8_t*)k_pages, (int8_t*)v_pages},
-                {(float*)k_scale, (float*)v_scale}, (const int32_t*)cu_q, (const int32_t*)positions, (const int32_t*)cache_rows,
-                tokens, rows, n_kv, dim, block, n_blocks, max_q_len <= 1};
-    const int size = dtype == BROLM_F32 ? 4 : 2;
-    const bool wide = aligned(k, k_token, k_head, size) && aligned(v, v_token, v_head, size);
-    const int threads = max_q_len <= 1 ? 128 : max(128, min(512, (block * dim / 64 + 31) / 32 * 32));
-    const dim3 grid((unsigned)places, n_kv, 2);
-    return dtype == BROLM_F32 ? launch_write<float>(a, grid, threads, wide, stream) : launch_write<bf16>(a, grid, threads, wide, stream);
+    WriteArgs a{{c->k, c->v}, {c->k_token, c->v_token}, {c->k_head, c->v_head}, {(int8_t*)c->k_pages, (int8_t*)c->v_pages},
+                {(float*)c->k_scale, (float*)c->v_scale}, (const int32_t*)c->cu_q, (const int32_t*)c->positions,
+                (const int32_t*)c->cache_rows, c->tokens, c->rows, c->n_kv, c->dim, c->block, c->n_blocks, single};
+    const int size = c->dtype == BROLM_F32 ? 4 : 2;
+    const bool wide = aligned(c->k, c->k_token, c->k_head, size) && aligned(c->v, c->v_token, c->v_head, size);
+    const int threads = single ? 128 : max(128, min(512, (c->block * c->dim / 64 + 31) / 32 * 32));
+    const dim3 grid((unsigned)places, c->n_kv, 2);
+    return c->dtype == BROLM_F32 ? launch_write<float>(a, grid, threads, wide, c->stream) : launch_write<bf16>(a, grid, threads, wide, c->stream);
 }
 
-BROLM_API int brolm_kv8_read(const void* cu_r, const void* kv_len, const void* slots, const void* tables, const void* k_pages,
-                             const void* v_pages, const void* k_scale, const void* v_scale, void* k, long long k_token,
-                             long long k_head, void* v, long long v_token, long long v_head, int dtype, int tokens, int rows,
-                             int n_kv, int dim, int block, int n_blocks, int n_slots, int width, int ring, cudaStream_t stream) {
-    if (dtype != BROLM_F32 && dtype != BROLM_BF16) return BROLM_ERR_BAD_DTYPE;
-    if (tokens < 0 || rows < 0 || n_slots <= 0 || width <= 0 || ring < 0 || (block > 0 && ring % block)) return BROLM_ERR_BAD_SIZE;
-    const int st = check_cache(k_pages, v_pages, n_kv, dim, block, n_blocks);
+BROLM_API int brolm_kv8_read(const ReadCall* c) {
+    if (c->dtype != BROLM_F32 && c->dtype != BROLM_BF16) return BROLM_ERR_BAD_DTYPE;
+    if (c->tokens < 0 || c->rows < 0 || c->n_slots <= 0 || c->width <= 0 || c->ring < 0 || (c->block > 0 && c->ring % c->block)) return BROLM_ERR_BAD_SIZE;
+    const int st = check_cache(c->k_pages, c->v_pages, c->n_kv, c->dim, c->block, c->n_blocks);
     if (st) return st;
-    const int size = dtype == BROLM_F32 ? 4 : 2;
-    if (!aligned(k, k_token, k_head, size) || !aligned(v, v_token, v_head, size)) return BROLM_ERR_ALIGNMENT;
-    if (tokens == 0 || rows == 0) return BROLM_OK;
-    ReadArgs a{{(const int8_t*)k_pages, (const int8_t*)v_pages}, {(const float*)k_scale, (const float*)v_scale}, {k, v},
-               {k_token, v_token}, {k_head, v_head}, (const int32_t*)cu_r, (const int32_t*)kv_len, (const int32_t*)slots,
-               (const int32_t*)tables, tokens, rows, n_kv, dim, block, n_blocks, n_slots, width, ring};
-    const dim3 grid((tokens + READ_TOKENS - 1) / READ_TOKENS, 2);
-    if (dtype == BROLM_F32) return launch_pdl(kv8_read_kernel<float>, grid, dim3(256), 0, stream, a);
-    return launch_pdl(kv8_read_kernel<bf16>, grid, dim3(256), 0, stream, a);
+    const int size = c->dtype == BROLM_F32 ? 4 : 2;
+    if (!aligned(c->k, c->k_token, c->k_head, size) || !aligned(c->v, c->v_token, c->v_head, size)) return BROLM_ERR_ALIGNMENT;
+    if (c->tokens == 0 || c->rows == 0) return BROLM_OK;
+    ReadArgs a{{(const int8_t*)c->k_pages, (const int8_t*)c->v_pages}, {(const float*)c->k_scale, (const float*)c->v_scale}, {c->k, c->v},
+               {c->k_token, c->v_token}, {c->k_head, c->v_head}, (const int32_t*)c->cu_r, (const int32_t*)c->kv_len,
+               (const int32_t*)c->slots, (const int32_t*)c->tables, c->tokens, c->rows, c->n_kv, c->dim, c->block, c->n_blocks,
+               c->n_slots, c->width, c->ring};
+    const dim3 grid((c->tokens + READ_TOKENS - 1) / READ_TOKENS, 2);
+    if (c->dtype == BROLM_F32) return launch_pdl(kv8_read_kernel<float>, grid, dim3(256), 0, c->stream, a);
+    return launch_pdl(kv8_read_kernel<bf16>, grid, dim3(256), 0, c->stream, a);
 }

@@ -4,7 +4,8 @@ A cache layer is four tensors: ``k_pages`` and ``v_pages``, int8 [blocks, kv hea
 ``k_scale`` and ``v_scale``, float32 [blocks, kv heads].  A number q of a block stands for ``q * scale``; the scale is the
 least power of two (2^-126 at least) under which nothing that the block of that head was given is beyond 127.  A scale
 never shrinks while its block fills; when it grows, the numbers that were there are rounded to it.  A block that gets a
-number that is not finite has the scale NaN, and all that sees it gets NaN, until it is begun anew.
+number that is not finite has the scale NaN, and all that sees it gets NaN, until it is begun anew.  Blocks hold 32, 64 or
+another multiple of 32 tokens, up to 256; heads have a multiple of 16 entries, up to 256.
 
 A sequence (a *slot*) holds a row of ``tables``, the ids of its blocks in the order of their places.  Position p lives at
 place p, or, with ``ring`` (a multiple of the block), at ``p % ring``: the newest ``ring / block`` blocks are then kept, the
@@ -17,23 +18,32 @@ come from the device (slots, block ids, cache rows) and lie outside the tensors 
 from __future__ import annotations
 
 import struct
-from ctypes import c_char_p, c_float, c_int, c_longlong, c_void_p
+from ctypes import c_char_p
 from typing import Optional
 
 import torch
 
-from . import KernelError, _check, _code, _fn, _ptr, _stream, device_sms
+from . import KernelError, _check, _fn, _stream, device_sms
 
 # what the tables' status word says
 BLOCKS_STATUS = {0: "ok", 1: "too few free blocks (or a stack that does not fit)", 2: "a row of the tables is too narrow",
                  3: "the step has more tokens than the outputs have places",
                  4: "a slot is out of range or named twice, or a length is negative"}
 
+_I8, _I32, _F32 = torch.int8, torch.int32, torch.float32
+_CODES = {torch.float32: 0, torch.bfloat16: 1}
 
-# The launchers of these libraries take one struct, packed here as C lays it out: converting a pointer and 35 numbers
-# one by one costs ctypes 3.4 us a call, packing them 0.4 and passing the one pointer 0.3.
+# A call of these operators is a few microseconds on the device, so what the host does for it counts.  Their launchers take
+# one struct, packed here as C lays it out (converting a pointer and 35 numbers one by one costs ctypes 3.4 us a call,
+# packing them 0.4 and passing the one pointer 0.3), and the checks of the arguments are one expression each; which of
+# them failed is found out only then.
+_EXTEND = struct.Struct("@14P7i")
+_RELEASE = struct.Struct("@7P4i")
+_WRITE = struct.Struct("@10P4q8i")
+_READ = struct.Struct("@11P4q10i")
 _ATTN = struct.Struct("@13P17i2f")
 _functions: dict = {}
+_NO_CPU = "brolm_b200 kernels run on CUDA tensors only; there is no CPU path"
 
 
 def _call(lib: str, name: str, packed: bytes, what: str) -> None:
@@ -43,18 +53,19 @@ def _call(lib: str, name: str, packed: bytes, what: str) -> None:
     _check(f(packed), what)
 
 
-def _ints(what: str, *named) -> None:
-    for name, t, n in named:
-        if t.dtype != torch.int32 or not t.is_contiguous():
+def _refuse_ints(what: str, **named) -> None:
+    """Raise for the first of ``name=(tensor, entries or None)`` that is not a contiguous int32 tensor on the device."""
+    for name, (t, n) in named.items():
+        if t.dtype != _I32 or not t.is_contiguous():
             raise KernelError(f"{what}: {name} must be a contiguous int32 tensor")
         if n is not None and t.numel() != n:
             raise KernelError(f"{what}: {name} has {t.numel()} entries, not {n}")
+        if not t.is_cuda:
+            raise KernelError(_NO_CPU)
 
 
-def _state(what: str, tables, held, free, free_count) -> None:
-    if tables.dim() != 2:
-        raise KernelError(f"{what}: tables must be [slots, width]")
-    _ints(what, ("tables", tables, None), ("held", held, tables.shape[0]), ("free", free, None), ("free_count", free_count, 1))
+def _odd_ints(t: torch.Tensor, n: int) -> bool:
+    return t.dtype is not _I32 or t.numel() != n or not t.is_contiguous() or not t.is_cuda
 
 
 def blocks_extend(slots: torch.Tensor, lengths: torch.Tensor, new: torch.Tensor, tables: torch.Tensor, held: torch.Tensor,
@@ -72,14 +83,21 @@ def blocks_extend(slots: torch.Tensor, lengths: torch.Tensor, new: torch.Tensor,
     A step that does not fit changes neither ``tables``, ``held`` nor the stack: its outputs read as padding and ``status``
     holds a key of ``BLOCKS_STATUS``.  The same step again takes no more blocks.  Up to 4,096 rows and 65,536 slots."""
     what = "blocks_extend"
-    _state(what, tables, held, free, free_count)
     n, T = slots.numel(), positions.numel()
-    _ints(what, ("slots", slots, None), ("lengths", lengths, n), ("new", new, n), ("cu_q", cu_q, n + 1), ("kv_len", kv_len, n),
-          ("positions", positions, None), ("tok_seq", tok_seq, T), ("cache_rows", cache_rows, T), ("status", status, 1))
-    f = _fn("blocks", "brolm_blocks_extend", [c_void_p] * 13 + [c_int] * 7 + [c_void_p])
-    _check(f(_ptr(slots), _ptr(lengths), _ptr(new), _ptr(tables), _ptr(held), _ptr(free), _ptr(free_count), _ptr(cu_q), _ptr(kv_len),
-             _ptr(positions), _ptr(tok_seq), _ptr(cache_rows), _ptr(status), n, tables.shape[0], tables.shape[1], free.numel(),
-             block, ring, T, _stream()), what)
+    if tables.dim() != 2:
+        raise KernelError(f"{what}: tables must be [slots, width]")
+    S, W = tables.shape
+    N = free.numel()
+    if _odd_ints(slots, n) or _odd_ints(lengths, n) or _odd_ints(new, n) or _odd_ints(tables, S * W) or _odd_ints(held, S) or \
+            _odd_ints(free, N) or _odd_ints(free_count, 1) or _odd_ints(cu_q, n + 1) or _odd_ints(kv_len, n) or \
+            _odd_ints(positions, T) or _odd_ints(tok_seq, T) or _odd_ints(cache_rows, T) or _odd_ints(status, 1):
+        _refuse_ints(what, slots=(slots, n), lengths=(lengths, n), new=(new, n), tables=(tables, None), held=(held, S), free=(free, N),
+                     free_count=(free_count, 1), cu_q=(cu_q, n + 1), kv_len=(kv_len, n), positions=(positions, T),
+                     tok_seq=(tok_seq, T), cache_rows=(cache_rows, T), status=(status, 1))
+    _call("blocks", "brolm_blocks_extend", _EXTEND.pack(
+        slots.data_ptr(), lengths.data_ptr(), new.data_ptr(), tables.data_ptr(), held.data_ptr(), free.data_ptr(),
+        free_count.data_ptr(), cu_q.data_ptr(), kv_len.data_ptr(), positions.data_ptr(), tok_seq.data_ptr(),
+        cache_rows.data_ptr(), status.data_ptr(), _stream(), n, S, W, N, block, ring, T), what)
 
 
 def blocks_release(slots: torch.Tensor, tables: torch.Tensor, held: torch.Tensor, free: torch.Tensor, free_count: torch.Tensor, *,
@@ -87,27 +105,43 @@ def blocks_release(slots: torch.Tensor, tables: torch.Tensor, held: torch.Tensor
     """Give the blocks of ``slots`` (-1: left out) back to the stack, the last row's last block first, so that releasing
     the rows of an extend restores the order it found.  ``status`` as in ``blocks_extend``; a wrong slot changes nothing."""
     what = "blocks_release"
-    _state(what, tables, held, free, free_count)
-    _ints(what, ("slots", slots, None), ("status", status, 1))
-    f = _fn("blocks", "brolm_blocks_release", [c_void_p] * 6 + [c_int] * 4 + [c_void_p])
-    _check(f(_ptr(slots), _ptr(tables), _ptr(held), _ptr(free), _ptr(free_count), _ptr(status), slots.numel(), tables.shape[0],
-             tables.shape[1], free.numel(), _stream()), what)
+    if tables.dim() != 2:
+        raise KernelError(f"{what}: tables must be [slots, width]")
+    S, W = tables.shape
+    n, N = slots.numel(), free.numel()
+    if _odd_ints(slots, n) or _odd_ints(tables, S * W) or _odd_ints(held, S) or _odd_ints(free, N) or _odd_ints(free_count, 1) or \
+            _odd_ints(status, 1):
+        _refuse_ints(what, slots=(slots, n), tables=(tables, None), held=(held, S), free=(free, N), free_count=(free_count, 1),
+                     status=(status, 1))
+    _call("blocks", "brolm_blocks_release", _RELEASE.pack(
+        slots.data_ptr(), tables.data_ptr(), held.data_ptr(), free.data_ptr(), free_count.data_ptr(), status.data_ptr(), _stream(),
+        n, S, W, N), what)
 
 
 def _cache(what: str, k_pages, v_pages, k_scale, v_scale) -> tuple:
-    if k_pages.dim() != 4 or k_pages.dtype != torch.int8 or v_pages.dtype != torch.int8:
+    shape = k_pages.shape
+    if len(shape) != 4 or k_pages.dtype is not _I8 or v_pages.dtype is not _I8:
         raise KernelError(f"{what}: the pages must be int8 [blocks, kv heads, block, head_dim]")
-    if v_pages.shape != k_pages.shape or not k_pages.is_contiguous() or not v_pages.is_contiguous():
+    if v_pages.shape != shape or not k_pages.is_contiguous() or not v_pages.is_contiguous():
         raise KernelError(f"{what}: key and value pages must be contiguous and of one shape")
-    for s in (k_scale, v_scale):
-        if s.dtype != torch.float32 or s.shape != k_pages.shape[:2] or not s.is_contiguous():
-            raise KernelError(f"{what}: the scales must be contiguous float32 [blocks, kv heads]")
-    return tuple(k_pages.shape)
+    n_blocks, n_kv, _, _ = shape
+    scales = (n_blocks, n_kv)
+    if k_scale.dtype is not _F32 or v_scale.dtype is not _F32 or k_scale.shape != scales or v_scale.shape != scales or \
+            not k_scale.is_contiguous() or not v_scale.is_contiguous():
+        raise KernelError(f"{what}: the scales must be contiguous float32 [blocks, kv heads]")
+    return shape
 
 
-def _rows3(what: str, name: str, x: torch.Tensor, n_kv: int, dim: int) -> None:
-    if x.dim() != 3 or x.shape[1:] != (n_kv, dim) or x.stride(2) != 1:
-        raise KernelError(f"{what}: {name} must be [tokens, {n_kv}, {dim}] with rows of consecutive entries")
+def _two(what: str, names: str, a: torch.Tensor, b: torch.Tensor, n_kv: int, dim: int) -> tuple:
+    """(tokens, element type code, strides of both) of two tensors [tokens, n_kv, dim] of one element type."""
+    dt = a.dtype
+    sa, sb = a.stride(), b.stride()
+    shape = a.shape
+    if len(shape) != 3 or b.shape != shape or shape[1] != n_kv or shape[2] != dim or sa[2] != 1 or sb[2] != 1:
+        raise KernelError(f"{what}: {names} must be [tokens, {n_kv}, {dim}], as many tokens both, with rows of consecutive entries")
+    if b.dtype is not dt or dt not in _CODES:
+        raise KernelError(f"{what}: {names} must both be float32 or both bfloat16, not {dt} and {b.dtype}")
+    return shape[0], _CODES[dt], sa[0], sa[1], sb[0], sb[1]
 
 
 def kv8_write(k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, positions: torch.Tensor, cache_rows: torch.Tensor,
@@ -119,18 +153,18 @@ def kv8_write(k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, positions: t
     that go to one block take its scale together; a block whose first place is among them is begun anew."""
     what = "kv8_write"
     n_blocks, n_kv, block, dim = _cache(what, k_pages, v_pages, k_scale, v_scale)
-    _rows3(what, "k", k, n_kv, dim)
-    _rows3(what, "v", v, n_kv, dim)
-    T = k.shape[0]
-    if v.shape[0] != T or v.dtype != k.dtype:
-        raise KernelError(f"{what}: k and v must have as many tokens and one element type")
-    if max_q_len < 1:
-        raise KernelError(f"{what}: max_q_len must be at least 1")
-    _ints(what, ("cu_q", cu_q, None), ("positions", positions, T), ("cache_rows", cache_rows, T))
-    f = _fn("kv8", "brolm_kv8_write", [c_void_p, c_longlong, c_longlong] * 2 + [c_int] + [c_void_p] * 7 + [c_int] * 7 + [c_void_p])
-    _check(f(_ptr(k), k.stride(0), k.stride(1), _ptr(v), v.stride(0), v.stride(1), _code(k), _ptr(cu_q), _ptr(positions),
-             _ptr(cache_rows), _ptr(k_pages), _ptr(v_pages), _ptr(k_scale), _ptr(v_scale), T, cu_q.numel() - 1, n_kv, dim, block,
-             n_blocks, max_q_len, _stream()), what)
+    T, code, k0, k1, v0, v1 = _two(what, "k and v", k, v, n_kv, dim)
+    rows = cu_q.numel() - 1
+    if max_q_len < 1 or rows < 0:
+        raise KernelError(f"{what}: max_q_len and the entries of cu_q must be at least 1")
+    if not (k.is_cuda and v.is_cuda and k_pages.is_cuda and v_pages.is_cuda and k_scale.is_cuda and v_scale.is_cuda):
+        raise KernelError(_NO_CPU)
+    if _odd_ints(cu_q, rows + 1) or _odd_ints(positions, T) or _odd_ints(cache_rows, T):
+        _refuse_ints(what, cu_q=(cu_q, None), positions=(positions, T), cache_rows=(cache_rows, T))
+    _call("kv8", "brolm_kv8_write", _WRITE.pack(
+        k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), positions.data_ptr(), cache_rows.data_ptr(), k_pages.data_ptr(),
+        v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), _stream(), k0, v0, k1, v1, code, T, rows, n_kv, dim, block,
+        n_blocks, max_q_len), what)
 
 
 def kv8_read(cu_q: torch.Tensor, kv_len: torch.Tensor, slots: torch.Tensor, tables: torch.Tensor, k_pages: torch.Tensor,
@@ -141,36 +175,51 @@ def kv8_read(cu_q: torch.Tensor, kv_len: torch.Tensor, slots: torch.Tensor, tabl
     or that the ring no longer holds, read as zero."""
     what = "kv8_read"
     n_blocks, n_kv, block, dim = _cache(what, k_pages, v_pages, k_scale, v_scale)
-    _rows3(what, "k_out", k_out, n_kv, dim)
-    _rows3(what, "v_out", v_out, n_kv, dim)
-    if v_out.shape[0] != k_out.shape[0] or v_out.dtype != k_out.dtype:
-        raise KernelError(f"{what}: k_out and v_out must have as many tokens and one element type")
+    T, code, k0, k1, v0, v1 = _two(what, "k_out and v_out", k_out, v_out, n_kv, dim)
     rows = cu_q.numel() - 1
-    if tables.dim() != 2 or max_q_len < 1:
-        raise KernelError(f"{what}: tables must be [slots, width] and max_q_len at least 1")
-    _ints(what, ("cu_q", cu_q, None), ("kv_len", kv_len, rows), ("slots", slots, rows), ("tables", tables, None))
-    f = _fn("kv8", "brolm_kv8_read", [c_void_p] * 8 + [c_void_p, c_longlong, c_longlong] * 2 + [c_int] * 10 + [c_void_p])
-    _check(f(_ptr(cu_q), _ptr(kv_len), _ptr(slots), _ptr(tables), _ptr(k_pages), _ptr(v_pages), _ptr(k_scale), _ptr(v_scale),
-             _ptr(k_out), k_out.stride(0), k_out.stride(1), _ptr(v_out), v_out.stride(0), v_out.stride(1), _code(k_out),
-             k_out.shape[0], rows, n_kv, dim, block, n_blocks, tables.shape[0], tables.shape[1], ring, _stream()), what)
+    if tables.dim() != 2 or max_q_len < 1 or rows < 0:
+        raise KernelError(f"{what}: tables must be [slots, width], max_q_len and the entries of cu_q at least 1")
+    S, W = tables.shape
+    if not (k_out.is_cuda and v_out.is_cuda and k_pages.is_cuda and v_pages.is_cuda and k_scale.is_cuda and v_scale.is_cuda):
+        raise KernelError(_NO_CPU)
+    if _odd_ints(cu_q, rows + 1) or _odd_ints(kv_len, rows) or _odd_ints(slots, rows) or _odd_ints(tables, S * W):
+        _refuse_ints(what, cu_q=(cu_q, None), kv_len=(kv_len, rows), slots=(slots, rows), tables=(tables, None))
+    _call("kv8", "brolm_kv8_read", _READ.pack(
+        cu_q.data_ptr(), kv_len.data_ptr(), slots.data_ptr(), tables.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+        k_scale.data_ptr(), v_scale.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), _stream(), k0, v0, k1, v1, code, T, rows, n_kv,
+        dim, block, n_blocks, S, W, ring), what)
 
 
 KV8_TILE, KV8_WARPS, KV8_CLUSTER = 32, 4, 8       # keys of a tile, warps of a block, blocks that join their results themselves
 
 
-def kv8_shares(batch: int, n_kv: int, row_tiles: int, keys: int, sms: Optional[int] = None) -> tuple[int, int]:
+def kv8_shares(batch: int, n_kv: int, row_tiles: int, keys: int, head_dim: int, sms: Optional[int] = None) -> tuple[int, int]:
     """How many blocks share the keys of one (sequence, kv head, tile of query rows): (blocks of a cluster, clusters).
 
-    Two blocks run on an SM; there are as many as give every SM its two, but none whose four warps would not have a tile
-    of keys each.  More than a cluster's eight are joined by a second launch: only where they shorten a long run."""
+    Two blocks run on an SM (three, of heads of up to 64 entries), and there are as many shares as give every SM its blocks,
+    but none whose four warps would not have a tile of keys each.  Up to eight join their results inside the launch; more
+    are joined by a second one, which pays from about 100 tiles on (1 sequence of 8,192 keys, 4 kv heads of 256: 18.3 us as
+    8 x 1, 11.1 as 8 x 8; 2 of 2,000: 8.6 as 8 x 1, 10.2 as 8 x 2).
+
+    Where the items give no more than two shares, the longest sequences' blocks would run alone at the end: such steps
+    are cut into rounds of blocks that the SMs take as they come free, if the shares stay long enough (24 tiles) and fill
+    their rounds (16 sequences of 129 to 6,145 keys under a window of 4,096, 8 kv heads: 36.9 us as 2 x 1, 32.1 as 1 x 4; of
+    equal ones 32 of 2,048, 4 kv heads: 28.3 as 2 x 1, 30.6 as 1 x 4, which is what it costs)."""
     sms = sms or device_sms()
+    places = (3 if head_dim <= 64 else 2) * sms
+    items = max(1, batch * n_kv * row_tiles)
     tiles = max(1, -(-keys // KV8_TILE))
-    want = min(2 * sms // max(1, batch * n_kv * row_tiles), -(-tiles // KV8_WARPS))
-    if want <= KV8_CLUSTER:
+    want = min(places // items, -(-tiles // KV8_WARPS))
+    if want <= 2:
+        if batch > 1 and items < 4 * places:
+            for k in (2, 3, 4):
+                rounds = k * items / places
+                if rounds > 1.5 and tiles >= 24 * k and rounds >= 0.8 * -(-k * items // places):
+                    return 1, k
         return max(1, want), 1
-    if tiles <= 8 * KV8_CLUSTER * KV8_WARPS:
-        return KV8_CLUSTER, 1
-    return KV8_CLUSTER, want // KV8_CLUSTER
+    if want <= KV8_CLUSTER:
+        return want, 1
+    return KV8_CLUSTER, (1 if tiles < 96 else want // KV8_CLUSTER)
 
 
 def attention_kv8(q: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, kv_len: torch.Tensor, slots: torch.Tensor,
@@ -183,29 +232,35 @@ def attention_kv8(q: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, kv_len
     that sees no key (padding) gets zeros.  ``max_q_len`` and ``max_kv_len`` bound the rows' new tokens and lengths."""
     what = "attention_kv8"
     n_blocks, G, block, dim = _cache(what, k_pages, v_pages, k_scale, v_scale)
-    if (G, dim) != (n_kv, head_dim):
+    if G != n_kv or dim != head_dim:
         raise KernelError(f"{what}: the pages hold {G} heads of {dim}, not {n_kv} of {head_dim}")
-    for name, x in (("q", q), ("out", out)):
-        if x.dim() != 2 or x.shape[1] != n_kv * group * head_dim or x.stride(1) != 1:
-            raise KernelError(f"{what}: {name} must be [tokens, {n_kv * group * head_dim}] with rows of consecutive entries")
-    if q.dtype != out.dtype or q.shape[0] != out.shape[0]:
-        raise KernelError(f"{what}: q and out must have as many tokens and one element type")
+    shape, dt = q.shape, q.dtype
+    q0, o0 = q.stride(), out.stride()
+    if len(shape) != 2 or shape[1] != n_kv * group * head_dim or out.shape != shape or q0[1] != 1 or o0[1] != 1:
+        raise KernelError(f"{what}: q and out must be [tokens, {n_kv * group * head_dim}] with rows of consecutive entries")
+    if out.dtype is not dt or dt not in _CODES:
+        raise KernelError(f"{what}: q and out must both be float32 or both bfloat16, not {dt} and {out.dtype}")
     if tables.dim() != 2 or max_q_len < 1:
         raise KernelError(f"{what}: tables must be [slots, width] and max_q_len at least 1")
     if ring and (window <= 0 or ring < window + max_q_len + block - 2):
         raise KernelError(f"{what}: a ring of {ring} does not keep what {max_q_len} new tokens see under a window of {window}: "
                           f"it takes window + tokens + {block} - 2")
-    _ints(what, ("cu_q", cu_q, batch + 1), ("kv_len", kv_len, batch), ("slots", slots, batch), ("tables", tables, None))
+    S, W = tables.shape
+    if not (q.is_cuda and out.is_cuda and k_pages.is_cuda and v_pages.is_cuda and k_scale.is_cuda and v_scale.is_cuda):
+        raise KernelError(_NO_CPU)
+    if _odd_ints(cu_q, batch + 1) or _odd_ints(kv_len, batch) or _odd_ints(slots, batch) or _odd_ints(tables, S * W):
+        _refuse_ints(what, cu_q=(cu_q, batch + 1), kv_len=(kv_len, batch), slots=(slots, batch), tables=(tables, None))
+    T = shape[0]
     rows = max_q_len * group
     keys = min(max_kv_len, window + max_q_len) if window > 0 else max_kv_len
-    shares, spans = kv8_shares(batch, n_kv, -(-rows // (8 if rows <= 8 else 16)), keys)
+    shares, spans = kv8_shares(batch, n_kv, 1 if rows <= 8 else -(-rows // 16), keys, head_dim)
     part_o = part_ml = 0
     if spans > 1:
-        n = q.shape[0] * n_kv * group * spans
-        parts = torch.empty(n * (head_dim + 2), dtype=torch.float32, device=q.device)
+        n = T * n_kv * group * spans
+        parts = torch.empty(n * (head_dim + 2), dtype=_F32, device=q.device)
         part_o = parts.data_ptr()
         part_ml = part_o + 4 * n * head_dim
     _call("attn_kv8", "brolm_attn_kv8", _ATTN.pack(
-        _ptr(q), _ptr(out), _ptr(cu_q), _ptr(kv_len), _ptr(slots), _ptr(tables), _ptr(k_pages), _ptr(v_pages), _ptr(k_scale),
-        _ptr(v_scale), part_o, part_ml, _stream(), q.stride(0), out.stride(0), _code(q), q.shape[0], batch, n_kv, group, head_dim,
-        block, n_blocks, tables.shape[0], tables.shape[1], ring, window, max_q_len, shares, spans, scale, cap), what)
+        q.data_ptr(), out.data_ptr(), cu_q.data_ptr(), kv_len.data_ptr(), slots.data_ptr(), tables.data_ptr(), k_pages.data_ptr(),
+        v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), part_o, part_ml, _stream(), q0[0], o0[0], _CODES[dt], T, batch,
+        n_kv, group, head_dim, block, n_blocks, S, W, ring, window, max_q_len, shares, spans, scale, cap), what)
