@@ -1,0 +1,756 @@
+// Attention of many new tokens over the cache in 8 bits (kv8.cuh) on the 5th-generation tensor cores (tcgen05), bfloat16,
+// sm_100a: pieces of prompts whose keys and values are in the cache already.
+//
+//     z = scale * q . k,   cap tanh(z / cap),   key j visible from position p iff 0 <= p - j < window,
+//     out = sum_j softmax_j(z) v_j,   zeros where a token sees no key.
+//
+// One block owns 128 rows of one (sequence, kv head); a row is a (token, query head of the group) pair.  The cache's
+// numbers become f16 in shared memory, exactly, and both products are f16 with float sums:
+//
+//   warps 0-7   softmax: two threads own each row, 64 of a tile's 128 scores each.  Scores come out of tensor memory, the
+//               weights go back over them as f16 pairs, and at the end the thread scales and stores its half of the row;
+//   warps 8-15  turn keys and values into f16 (1024 + 128 + q has the bits 0x6400 | (q + 128): one byte permutation makes
+//               two, one subtraction takes 1152 away) and store them as the tensor core reads them: keys in units of 64
+//               entries of a head, values in units of as many bytes, all in one ring of slots in the order of their use, four
+//               warps every other unit (with four warps for all of them a tile took 8,600 cycles: a unit is 260 of
+//               arithmetic and 500 of waiting for shared memory and barriers);
+//   warp 16     one thread issues tcgen05.mma: S = Q K^T (128 x 128) into one of two buffers in tensor memory, O += P V
+//               (128 x head size, P from tensor memory, the values as they lie, keys x entries);
+//   warp 17     looks up where the keys lie and what their scales are, 32 groups of 32 keys at a time, for all the others;
+//   warp 18, 19 issue the TMA loads of the units' bytes, of keys and of values, into a ring of their own.  (Loads into the
+//               converting threads' registers were as many, but what tells the tensor core of a thread's stores waits for its
+//               loads too: 6.4 us a tile of 128 keys and 256 entries.  One thread for all loads needs 1,000 cycles a unit.)
+//
+// Scales.  A key block's scale multiplies the scores.  A value block's scale 2^e goes into the weights: a weight is
+// 2^(z - m) 2^(e - e0), e0 the largest exponent of the keys this block of threads sees, and m the row's running maximum of
+// z + e - e0, so that what is rounded to f16 is at most 2^8 and exact to 11 bits for all that matters to the sum, however
+// the blocks' scales differ; the sum of 2^(z - m) is kept in 32 bits, without the values' scales.  (m is raised only when it
+// would be passed by more than 8: the accumulator in tensor memory is then scaled anew.)  A query row is scaled by a power
+// of two to below 2^14 and held in f16, exactly but for numbers 2^-38 of the row's largest.
+//
+// What bounds it: a tile of 128 keys and 256 entries takes the tensor core 2,770 cycles, the 3 x 16,384 exponentials and
+// reciprocals of a capped softmax 3,070 cycles of the special function units, and the instructions of softmax and of
+// turning bytes into f16 about 2,400 issue cycles of each scheduler.
+//
+// Every mbarrier wait is bounded; a wait that runs out records a code that brolm_attn_kv8_tc_status() returns, and the
+// launch ends without its results.
+#include "tcgen05.cuh"
+#include "kv8.cuh"
+
+#include <cuda_fp16.h>
+
+namespace {
+
+using namespace tc;
+using namespace kv8;
+
+constexpr int BM = 128, BN = 128;
+constexpr int SOFTMAX_WARPS = 8, CONVERT_WARPS = 4, CONVERT_GROUPS = 2;       // (warps of a group)
+constexpr int ISSUER = SOFTMAX_WARPS + CONVERT_GROUPS * CONVERT_WARPS, LOOKUP = ISSUER + 1, LOADER = LOOKUP + 1;
+constexpr int THREADS = 32 * (LOADER + 2);   // five groups of four warps
+// registers of a thread: 96 at launch, 61,440 in all, then 256 x 152 + 256 x 64 + 128 x 48 = 61,440
+constexpr int LAUNCH_REGS = 96, SOFTMAX_REGS = 152, CONVERT_REGS = 64, OTHER_REGS = 48;
+static_assert(THREADS * LAUNCH_REGS == 256 * SOFTMAX_REGS + 256 * CONVERT_REGS + 128 * OTHER_REGS, "registers of the block");
+constexpr int TMEM_COLS = 512;
+constexpr int UNIT = 16384;               // bytes of a slot: 128 keys x 64 entries, or the same number of values
+constexpr int RAW = UNIT / 2;             // .. as they come from the cache
+constexpr int CHUNK = 8;                  // tiles whose places and scales are looked up at a time (32 groups of 32 keys)
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float RESCALE_GAP = 8.0f;
+
+__device__ int g_attn_kv8_tc_error;
+
+struct TcArgs {
+    const bf16* q;
+    bf16* out;
+    int q_stride, out_stride;
+    const int32_t *cu_q, *kv_len, *slots, *tables;
+    const int8_t *k_pages, *v_pages;
+    const float *k_scale, *v_scale;
+    int tokens, rows, n_kv, group, block, n_blocks, n_slots, width, ring, window, row_tiles, wide;
+    float scale, cap;
+};
+
+template <int HD>
+struct Shape {
+    static constexpr int PARTS = HD / 64;                    // units of a key tile, and of a value tile
+    static constexpr int VK = BN / PARTS;                    // keys of a value unit
+    static constexpr int SLOTS = HD == 256 ? 5 : 8;
+    static constexpr int RAWS = HD == 256 ? 8 : 7;           // units on their way from the cache
+    static constexpr int Q_BYTES = BM * HD * 2;
+};
+
+// barriers
+enum : int { S_FULL = 0, P_FULL = 2, PV_DONE = 4, META_FULL = 6, META_EMPTY = 8, U_FULL = 10 };
+
+struct Meta {                             // of a group of 32 keys
+    int row;                              // the group's first row in the pages
+    float k_scale;
+    int v_exp;                            // exponent of the value scale less e0; BAD: a scale that is NaN
+};
+constexpr int BAD = 0x7fffffff;
+
+__device__ __forceinline__ uint32_t idesc_f16(int m, int n, int b_mn_major) {
+    return (1u << 4) | ((uint32_t)b_mn_major << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+__device__ __forceinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile int* give_up, int code) {
+    return mbar_wait(bar, parity, give_up, &g_attn_kv8_tc_error, code);
+}
+template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+// Waits that are mostly over when they begin: the limit and the flags are looked at only if they are not (which takes 190
+// cycles).  Only the softmax warps' waits, codes 8 and 9, can be stalled by brolm_attn_kv8_tc_wait_control at any time.
+__device__ __forceinline__ bool wait_one(uint32_t bar, uint32_t parity, volatile int* give_up, int code) {
+    return mbar_try(bar, parity) || wait_on(bar, parity, give_up, code);
+}
+__device__ __forceinline__ bool wait_soon(uint32_t bar, uint32_t parity, volatile int* give_up, int code) {
+    bool ok = mbar_try(bar, parity);
+    if (__all_sync(0xffffffffu, ok)) return true;
+    ok = wait_on(bar, parity, give_up, code);
+    return __all_sync(0xffffffffu, ok);
+}
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatile int* give_up, int code) {
+    const bool ok = wait_on(bar, parity, give_up, code);
+    return __all_sync(0xffffffffu, ok);
+}
+__device__ __forceinline__ void st_shared16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared16(uint32_t p) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(p) : "memory");
+    return v;
+}
+// Units in the order of their use: K(0); then K(j + 1), V(j) for every tile j but the last; V(last).
+template <int PARTS>
+struct UnitOrder {
+    int n_tiles, tile = 0, part = 0;
+    bool keys = true;
+    __device__ __forceinline__ explicit UnitOrder(int n) : n_tiles(n) {}
+    __device__ __forceinline__ void step() {
+        if (++part < PARTS) return;
+        part = 0;
+        if (keys) {
+            if (tile == 0 && n_tiles > 1) tile = 1;
+            else { keys = false; tile = max(0, tile - 1); }
+        } else if (tile + 2 < n_tiles) {
+            keys = true;
+            tile += 2;
+        } else {
+            ++tile;
+        }
+    }
+};
+// Two floats in one instruction, and the largest of three.
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    return v;
+}
+__device__ __forceinline__ float2 halves(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t v;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+__device__ __forceinline__ uint64_t mad2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+    return v;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float v;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(a), "f"(b), "f"(c));
+    return v;
+}
+
+// A barrier of 64 threads that tells whether all of them are well.
+__device__ __forceinline__ bool both_ok(int id, bool ok) {
+    uint32_t all;
+    asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 q, %2, 0;\nbarrier.cta.red.and.aligned.pred p, %1, 64, q;\nselp.u32 %0, 1, 0, p;\n}"
+                 : "=r"(all) : "r"(id), "r"((uint32_t)ok) : "memory");
+    return all != 0;
+}
+template <int SELECT>
+__device__ __forceinline__ uint32_t bytes_to_f16(uint32_t w) {
+    const uint32_t x = __byte_perm(w, 0x64646464u, SELECT);
+    const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0x6480)));
+    return *reinterpret_cast<const uint32_t*>(&y);
+}
+
+// 16 bytes of the cache as 16 f16 numbers: the pieces of 16 bytes `piece` and `piece ^ 1` of a 128-byte row.
+__device__ __forceinline__ void put_f16(uint32_t row_at, int piece, const uint4& raw) {
+    uint32_t h[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t w = (&raw.x)[i] ^ 0x80808080u;
+        h[2 * i] = bytes_to_f16<0x4140>(w);
+        h[2 * i + 1] = bytes_to_f16<0x4342>(w);
+    }
+    st_shared16(row_at + piece * 16, h[0], h[1], h[2], h[3]);
+    st_shared16(row_at + (piece ^ 1) * 16, h[4], h[5], h[6], h[7]);
+}
+
+template <int HD>
+__global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_constant__ CUtensorMap map_k,
+                                                                 const __grid_constant__ CUtensorMap map_v, TcArgs a) {
+    using SH = Shape<HD>;
+    constexpr int PARTS = SH::PARTS, VK = SH::VK, SLOTS = SH::SLOTS, RAWS = SH::RAWS;
+    constexpr uint32_t S_COL = 0, O_COL = 2 * BN;            // tensor-memory columns: two score buffers, then the output
+    static_assert(O_COL + HD <= TMEM_COLS, "tensor memory");
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    if ((smem_u32(smem_raw) & 1023u) != 0) {                 // never seen; refuse rather than compute wrongly
+        if (threadIdx.x == 0) atomicCAS(&g_attn_kv8_tc_error, 0, 13);
+        return;
+    }
+    const uint32_t q_s = smem_u32(smem_raw), ring = q_s + SH::Q_BYTES;
+    const uint32_t raw_s = ring + SLOTS * UNIT;
+    uint8_t* rest = smem_raw + SH::Q_BYTES + SLOTS * UNIT + RAWS * RAW;
+    Meta* meta = reinterpret_cast<Meta*>(rest);              // [2][CHUNK][4]
+    float* xch = reinterpret_cast<float*>(meta + 2 * CHUNK * 4);     // [2][2][BM]: maxima by tile parity and half; the sums reuse it
+    float* q_scale = xch + 4 * BM;                           // [BM]
+    uint64_t* bars = reinterpret_cast<uint64_t*>(q_scale + BM);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + U_FULL + 2 * SLOTS + 2 * RAWS);
+    volatile int* give_up = reinterpret_cast<volatile int*>(tmem_slot + 1);       // three
+    int* top_exp = reinterpret_cast<int*>(tmem_slot + 4);
+    const uint32_t bar0 = smem_u32(bars);
+    auto bar = [&](int i) { return bar0 + 8u * i; };
+    auto u_full = [&](int sl) { return bar0 + 8u * (U_FULL + sl); };
+    auto u_empty = [&](int sl) { return bar0 + 8u * (U_FULL + SLOTS + sl); };
+    auto r_full = [&](int sl) { return bar0 + 8u * (U_FULL + 2 * SLOTS + sl); };
+    auto r_empty = [&](int sl) { return bar0 + 8u * (U_FULL + 2 * SLOTS + RAWS + sl); };
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_wait();
+    // blocks start in the order of their index: the last rows, which see the most keys, of every sequence and head first
+    const int per = a.n_kv * a.rows;
+    const int xt = a.row_tiles - 1 - (int)(blockIdx.x / per), which = blockIdx.x % per;
+    const int b = which / a.n_kv, g = which - b * a.n_kv;
+    const int first_tok = a.cu_q[b], n_tok = min(a.cu_q[b + 1], a.tokens) - first_tok;
+    const int kv_len = a.kv_len[b], slot = a.slots[b];
+    const int row0 = xt * BM;
+    const int rows_here = first_tok < 0 ? 0 : (int)min((long long)BM, (long long)n_tok * a.group - row0);
+    if (rows_here <= 0) return;                              // (the whole block)
+    const int window = a.window > 0 ? a.window : 0x3fffffff;
+    const int pos0 = kv_len - n_tok, pos_lo = pos0 + row0 / a.group, pos_hi = pos0 + (row0 + rows_here - 1) / a.group;
+    int t_first = 0, n_tiles = 0;
+    if (pos_hi >= 0 && slot >= 0 && slot < a.n_slots) {
+        t_first = max(0, pos_lo - window + 1) / BN;
+        n_tiles = pos_hi / BN - t_first + 1;
+    }
+    const int32_t* table = a.tables + (size_t)max(slot, 0) * a.width;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(bar(S_FULL + s), 1);
+            mbar_init(bar(P_FULL + s), SOFTMAX_WARPS);
+            mbar_init(bar(PV_DONE + s), 1);
+            mbar_init(bar(META_FULL + s), 1);
+            mbar_init(bar(META_EMPTY + s), SOFTMAX_WARPS + 2);
+        }
+        for (int s = 0; s < SLOTS; ++s) {
+            mbar_init(u_full(s), CONVERT_WARPS);
+            mbar_init(u_empty(s), 1);
+        }
+        for (int s = 0; s < RAWS; ++s) {
+            mbar_init(r_full(s), 1);
+            mbar_init(r_empty(s), CONVERT_WARPS);
+        }
+        give_up[0] = 0;
+        give_up[1] = 0;
+        give_up[2] = tc::g_stall_code;
+        *top_exp = -126;
+        mbar_init_fence();
+    }
+    if (warp == ISSUER) tmem_alloc(smem_u32(tmem_slot), TMEM_COLS);
+    __syncthreads();
+    // where a key's block is, from its place in units of 32 (a block is a multiple of that)
+    const int block32 = a.block >> 5;
+    auto block_of = [&](int place32) -> int {
+        const int e = place32 / block32;
+        const int id = e < a.width ? table[e] : 0;
+        return id >= 0 && id < a.n_blocks ? id : 0;          // (never followed out of the cache)
+    };
+    if (n_tiles > 0) {
+        // e0: the largest exponent among the value scales of the keys that this block sees
+        const int first32 = t_first * (BN / 32), n32 = pos_hi / 32 - first32 + 1;
+        int top = -126;
+        for (int i = threadIdx.x; i * block32 < n32 + block32; i += THREADS) {
+            const int at = min(first32 + i * block32, pos_hi / 32);
+            const float s = a.v_scale[(size_t)block_of(a.ring > 0 ? at % (a.ring >> 5) : at) * a.n_kv + g];
+            if (s == s) top = max(top, (int)(__float_as_uint(s) >> 23 & 255u) - 127);
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+        if (lane == 0 && top > -126) atomicMax(top_exp, top);
+    }
+    // the queries: a warp a row, eight entries a lane, rows of 128 bytes per 64 entries, pieces of 16 bytes swizzled
+    for (int r = warp; r < BM; r += THREADS / 32) {
+        float v[8] = {};
+        if (r < rows_here && lane * 8 < HD) {
+            const int row = row0 + r;
+            const bf16* src = a.q + (size_t)(first_tok + row / a.group) * a.q_stride + (g * a.group + row % a.group) * HD + lane * 8;
+            if (a.wide) load8(src, v);
+            else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = to_float(src[e]);
+            }
+        }
+        float most = 0.0f;
+        bool finite = true;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            most = fmaxf(most, fabsf(v[e]));
+            finite = finite && fabsf(v[e]) < INFINITY;
+        }
+        most = warp_max(most);
+        finite = __all_sync(0xffffffffu, finite);
+        const int up = max(min(13 + 127 - (int)(__float_as_uint(most) >> 23), 120), -126);
+        const float f = power_of_two(up);
+        if (lane == 0) q_scale[r] = finite ? power_of_two(-up) : __int_as_float(0x7fc00000);
+        if (lane * 8 < HD) {
+            uint32_t h[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const __half2 t = __floats2half2_rn(finite ? v[2 * e] * f : 0.0f, finite ? v[2 * e + 1] * f : 0.0f);
+                h[e] = *reinterpret_cast<const uint32_t*>(&t);
+            }
+            st_shared16(q_s + (lane >> 3) * (BM * 128) + r * 128 + (((lane & 7) ^ (r & 7)) << 4), h[0], h[1], h[2], h[3]);
+        }
+    }
+    fence_proxy_async();
+    fence_before_sync();
+    __syncthreads();
+    fence_after_sync();
+    const uint32_t tmem = *tmem_slot;
+    const int e0 = *top_exp;
+
+    if (warp >= ISSUER) {
+        fewer_registers<OTHER_REGS>();
+        if (warp == LOOKUP) {
+            for (int m = 0; m * CHUNK < n_tiles; ++m) {
+                if (!wait_warp(bar(META_EMPTY + (m & 1)), ((m >> 1) & 1) ^ 1, give_up, 3)) break;
+                const int at32 = (t_first + m * CHUNK) * (BN / 32) + lane;
+                Meta x{0, 0.0f, 0};
+                if (at32 <= pos_hi / 32) {
+                    const int place32 = a.ring > 0 ? at32 % (a.ring >> 5) : at32;
+                    const size_t bh = (size_t)block_of(place32) * a.n_kv + g;
+                    x.row = (int)bh * a.block + (place32 % block32) * 32;
+                    x.k_scale = a.k_scale[bh];
+                    const float sv = a.v_scale[bh];
+                    x.v_exp = max((int)(__float_as_uint(sv) >> 23 & 255u) - 127, -126) - e0;
+                    if (x.k_scale != x.k_scale || sv != sv) {
+                        x.k_scale = 0.0f;
+                        x.v_exp = BAD;
+                    }
+                }
+                meta[(m & 1) * CHUNK * 4 + lane] = x;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(META_FULL + (m & 1)));
+            }
+        } else if (warp == ISSUER) {
+            if (lane == 0 && n_tiles > 0) {
+                const uint32_t id_qk = idesc_f16(BM, BN, 0), id_pv = idesc_f16(BM, HD, 1);
+                int u = 0;
+                // S(j) goes over the buffer that P(j-2) was read from: the product that read it was issued before
+                auto issue_qk = [&](int j) -> bool {
+                    const int s = j & 1;
+#pragma unroll
+                    for (int ku = 0; ku < PARTS; ++ku) {
+                        const int sl = u % SLOTS;
+                        if (!wait_one(u_full(sl), (u / SLOTS) & 1, give_up, 4)) return false;
+                        fence_after_sync();
+                        const uint64_t qa = desc_kmajor(q_s + ku * (BM * 128)), kb = desc_kmajor(ring + sl * UNIT);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) umma(tmem + S_COL + s * BN, qa + 2 * k, kb + 2 * k, id_qk, (ku | k) != 0);
+                        umma_commit(u_empty(sl));
+                        ++u;
+                    }
+                    umma_commit(bar(S_FULL + s));
+                    return true;
+                };
+                bool ok = issue_qk(0);
+                for (int j = 0; j < n_tiles && ok; ++j) {
+                    if (j + 1 < n_tiles) { ok = issue_qk(j + 1); if (!ok) break; }
+                    const int s = j & 1;
+                    ok = wait_one(bar(P_FULL + s), (j >> 1) & 1, give_up, 6);
+                    if (!ok) break;
+#pragma unroll
+                    for (int vu = 0; vu < PARTS; ++vu) {
+                        const int sl = u % SLOTS;
+                        ok = wait_one(u_full(sl), (u / SLOTS) & 1, give_up, 7);
+                        if (!ok) break;
+                        fence_after_sync();
+#pragma unroll
+                        for (int k = 0; k < VK / 16; ++k) {
+                            // sixteen keys further: eight columns of P, sixteen 128-byte rows down in V
+                            const uint64_t vb = desc_mnmajor(ring + sl * UNIT + k * (16 * 128), (VK * 128) >> 4, 1024 >> 4);
+                            umma_ts(tmem + O_COL, tmem + S_COL + s * BN + vu * (VK / 2) + k * 8, vb, id_pv, (j | vu | k) != 0);
+                        }
+                        umma_commit(u_empty(sl));
+                        ++u;
+                    }
+                    if (!ok) break;
+                    umma_commit(bar(PV_DONE + s));
+                }
+            }
+        } else {
+            // keys or values: a lane for each of a unit's boxes
+            const bool keys = warp == LOADER;
+            const int boxes = keys ? 4 : VK / 32;
+            const uint32_t box_bytes = keys ? RAW / 4 : 32 * HD;
+            int u = 0, tile = 0;
+            bool ok = true;
+            for (; tile < n_tiles && ok; ++tile) {
+                const int chunk = tile / CHUNK;
+                if (tile % CHUNK == 0) ok = wait_soon(bar(META_FULL + (chunk & 1)), (chunk >> 1) & 1, give_up, 2);
+                const Meta* m = meta + (chunk & 1) * CHUNK * 4 + (tile % CHUNK) * 4;
+                const int first = keys ? (tile == 0 ? 0 : 2 * tile - 1) * PARTS : min(2 * tile + 2, 2 * n_tiles - 1) * PARTS;
+#pragma unroll
+                for (int part = 0; part < PARTS; ++part) {
+                    if (!ok) break;
+                    u = first + part;
+                    const int sl = u % RAWS;
+                    ok = wait_soon(r_empty(sl), ((u / RAWS) & 1) ^ 1, give_up, 1);
+                    if (!ok) break;
+                    if (lane == 0) mbar_expect_tx(r_full(sl), RAW);
+                    __syncwarp();
+                    if (lane < boxes)
+                        tma_load_2d(raw_s + sl * RAW + lane * box_bytes, keys ? &map_k : &map_v, keys ? part * 64 : 0,
+                                    m[keys ? lane : part * (VK / 32) + lane].row, r_full(sl));
+                }
+                __syncwarp();
+                if (lane == 0 && tile % CHUNK == CHUNK - 1) mbar_arrive(bar(META_EMPTY + (chunk & 1)));
+            }
+            if (lane == 0) pdl_trigger();      // every tile is asked for: the next kernel may move in
+            if (*give_up) {                    // let the loads in flight land before the block goes away
+                // (this warp's last units, whichever of the ring's slots they went to; a slot that the other warp's load came
+                // to is drained by that warp)
+                for (int t = max(0, tile - 1 - RAWS); t < tile; ++t) {
+                    const int first = keys ? (t == 0 ? 0 : 2 * t - 1) * PARTS : min(2 * t + 2, 2 * n_tiles - 1) * PARTS;
+                    for (int part = 0; part < PARTS; ++part)
+                        if (first + part < u || (first + part == u && ok))
+                            mbar_wait(r_full((first + part) % RAWS), ((first + part) / RAWS) & 1, give_up, &g_attn_kv8_tc_error, 10, true);
+                }
+            }
+        }
+    } else if (warp >= SOFTMAX_WARPS) {
+        fewer_registers<CONVERT_REGS>();
+        // A thread has four pieces of 16 bytes of a unit: of keys [128][64], rows 32 i + t / 4; of values [VK][HD], rows
+        // VK / 4 further each.  Lanes are laid out so that eight of them store to all banks.
+        const int group = (warp - SOFTMAX_WARPS) / CONVERT_WARPS, t = threadIdx.x & (32 * CONVERT_WARPS - 1);
+        const int k_row = t >> 2, k_c = t & 3;
+        const int v_c = (t & 3) | (((t >> 3) % PARTS) << 2), v_row = ((t >> 2) & 1) + ((t >> 3) / PARTS) * 2;
+        const uint32_t k_src = k_row * 64 + k_c * 16, v_src = v_row * HD + v_c * 16;
+        const uint32_t k_dst = k_row * 128, v_dst = (v_c >> 2) * (VK * 128) + v_row * 128;
+        const int k_piece = (2 * k_c) ^ (k_row & 7), v_piece = (2 * (v_c & 3)) ^ (v_row & 7);
+        UnitOrder<PARTS> x(n_tiles);
+        const int units = 2 * PARTS * n_tiles;
+        if (group) x.step();
+        for (int u = group; u < units; u += CONVERT_GROUPS) {
+            const int sl = u % SLOTS, rs = u % RAWS;
+            if (!wait_soon(r_full(rs), (u / RAWS) & 1, give_up, 5)) break;
+            const uint32_t src = raw_s + rs * RAW + (x.keys ? k_src : v_src), far = x.keys ? 32 * 64 : VK / 4 * HD;
+            uint4 raw[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) raw[i] = ld_shared16(src + i * far);
+            if (!wait_soon(u_empty(sl), ((u / SLOTS) & 1) ^ 1, give_up, 14)) break;
+            const uint32_t at = ring + sl * UNIT + (x.keys ? k_dst : v_dst), stride = x.keys ? 32 * 128 : VK / 4 * 128;
+            const int piece = x.keys ? k_piece : v_piece;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) put_f16(at + i * stride, piece, raw[i]);
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(r_empty(rs));
+                mbar_arrive(u_full(sl));
+            }
+            x.step();
+            x.step();
+        }
+    } else {
+        more_registers<SOFTMAX_REGS>();
+        // Two warps share each quarter of the rows (a warp may only touch the 32 lanes of tensor memory of its quarter):
+        // warp w and warp w + 4 own the same 32 rows, the first takes score columns 0-63, the second 64-127.  They agree on
+        // the row's reference maximum through shared memory and a 64-thread barrier.
+        constexpr int W = BN / 2;
+        const int quarter = warp & 3, half = warp >> 2;
+        const int r = quarter * 32 + lane;
+        const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
+        const bool row_ok = r < rows_here;
+        const int pos = pos0 + (row0 + r) / a.group;
+        const float qs = q_scale[r];
+        const float unit = qs * (a.cap > 0.0f ? a.scale / a.cap : a.scale * LOG2E);
+        const float c1 = a.cap * LOG2E, c2 = 2.0f * a.cap * LOG2E;
+        const uint64_t t0 = pair_of(c1, c1), t1 = pair_of(c1 * (-1.0f / 3.0f), c1 * (-1.0f / 3.0f));
+        const uint64_t t2 = pair_of(c1 * (2.0f / 15.0f), c1 * (2.0f / 15.0f)), t3 = pair_of(c1 * (-17.0f / 315.0f), c1 * (-17.0f / 315.0f));
+        const uint64_t t4 = pair_of(c1 * (62.0f / 2835.0f), c1 * (62.0f / 2835.0f));
+        float m_ref = -INFINITY, l = 0.0f;                   // l: the sum over this thread's columns only
+        bool ok = true, sees_bad = false;
+        for (int j = 0; j < n_tiles; ++j) {
+            const int s = j & 1;
+            if (ok && j % CHUNK == 0) ok = wait_warp(bar(META_FULL + ((j / CHUNK) & 1)), (j / CHUNK >> 1) & 1, give_up, 9);
+            const Meta* m = meta + ((j / CHUNK) & 1) * CHUNK * 4 + (j % CHUNK) * 4 + 2 * half;
+            float f[2];
+            int ve[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                f[h] = m[h].k_scale * unit;
+                ve[h] = m[h].v_exp;
+            }
+            if (ok) ok = wait_warp(bar(S_FULL + s), (j >> 1) & 1, give_up, 8);
+            fence_after_sync();
+            const int key_base = (t_first + j) * BN, kp0 = key_base + half * W;
+            const bool edge = key_base + BN - 1 > pos_lo || key_base < pos_hi - window + 1;
+            // visible: lo <= c <= hi for column c of this thread
+            const int hi = row_ok ? pos - kp0 : -1, lo = pos - window + 1 - kp0;
+            uint64_t z[W / 2];                               // scores in log2 units, two by two
+            float top[2] = {-INFINITY, -INFINITY};
+            auto scores = [&](auto&& to_z) {
+                uint32_t sv[W];
+                uint32_t(&x0)[32] = *reinterpret_cast<uint32_t(*)[32]>(&sv[0]);
+                uint32_t(&x1)[32] = *reinterpret_cast<uint32_t(*)[32]>(&sv[32]);
+                tmem_ld32(tmem + lane_addr + S_COL + s * BN + half * W, x0);
+                tmem_ld32(tmem + lane_addr + S_COL + s * BN + half * W + 32, x1);
+                tmem_wait_ld();
+#pragma unroll
+                for (int c = 0; c < W / 2; ++c)
+                    z[c] = to_z(mul2(pair_of(__uint_as_float(sv[2 * c]), __uint_as_float(sv[2 * c + 1])), pair_of(f[c / 16], f[c / 16])));
+            };
+            if (a.cap > 0.0f) {
+                // cap log2e tanh(x).  Scores are mostly well below the cap, and there the series to x^9 is as exact (|x| up to
+                // 0.4: 4e-7 of the cap) and leaves the special function units to the weights
+                float far = 0.0f;
+                scores([&](uint64_t x) {
+                    const uint64_t y = mul2(x, x);
+                    const float2 yy = halves(y);
+                    far = max3(far, yy.x, yy.y);
+                    return mul2(x, mad2(mad2(mad2(mad2(t4, y, t3), y, t2), y, t1), y, t0));
+                });
+                if (!__all_sync(0xffffffffu, far <= 0.16f))
+                    scores([&](uint64_t x) {
+                        const float2 xx = halves(x);
+                        return pair_of(fmaf(-c2, fast_rcp(1.0f + fast_exp2(xx.x * (2.0f * LOG2E))), c1),
+                                       fmaf(-c2, fast_rcp(1.0f + fast_exp2(xx.y * (2.0f * LOG2E))), c1));
+                    });
+            } else {
+                scores([&](uint64_t x) { return x; });
+            }
+            if (edge) {
+#pragma unroll
+                for (int c = 0; c < W / 2; ++c) {
+                    float2 x = halves(z[c]);
+                    if (2 * c > hi || 2 * c < lo) x.x = -INFINITY;
+                    if (2 * c + 1 > hi || 2 * c + 1 < lo) x.y = -INFINITY;
+                    z[c] = pair_of(x.x, x.y);
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < W / 2; ++c) {
+                const float2 x = halves(z[c]);
+                top[c / 16] = max3(top[c / 16], x.x, x.y);
+            }
+            float e[2];
+            bool apart = false;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (ve[h] == BAD) {                          // a NaN block: whoever sees a key of it gets NaN
+                    sees_bad = sees_bad || (hi >= 32 * h && lo < 32 * h + 32);
+                    ve[h] = 0;
+                }
+                apart = apart || ve[h] < -60;
+                e[h] = (float)ve[h];
+                top[h] += e[h];
+            }
+            float m_t = fmaxf(top[0], top[1]);
+            xch[(s * 2 + half) * BM + r] = m_t;              // double-buffered by the tile's parity
+            // after this barrier both threads of the row hold their scores in registers, so the weights may go over the
+            // partner's score columns
+            ok = both_ok(1 + quarter, ok);                   // (a wait that ran out ends both, or one would wait for the other)
+            if (!ok) break;
+            m_t = fmaxf(m_t, xch[(s * 2 + (half ^ 1)) * BM + r]);
+            const bool raise = m_t > m_ref + RESCALE_GAP;    // also true for the first visible tile of a row
+            const float m_new = raise ? m_t : m_ref;
+            const float corr = (raise && m_ref > -INFINITY) ? fast_exp2(m_ref - m_new) : 1.0f;
+            if (j > 0 && __any_sync(0xffffffffu, corr != 1.0f)) {
+                // rare: the accumulator has to be at rest (the product of the tile before is done), then every row of the
+                // warp is scaled anew; each warp of the pair takes half of the entries
+                ok = wait_warp(bar(PV_DONE + (s ^ 1)), ((j - 1) >> 1) & 1, give_up, 12);
+                fence_after_sync();
+#pragma unroll 1
+                for (int c = half * (HD / 2); c < (half + 1) * (HD / 2); c += 32) {
+                    uint32_t ov[32];
+                    tmem_ld32(tmem + lane_addr + O_COL + c, ov);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * corr);
+                    tmem_st32(tmem + lane_addr + O_COL + c, ov);
+                }
+            }
+            l *= corr;
+            m_ref = m_new;
+            // weights -> tensor memory, f16 pairs: keys 2c, 2c+1 of this thread in column c of its 32
+            uint64_t sums[2] = {0ull, 0ull};
+            const float m_sub = m_ref > -INFINITY ? m_ref : 0.0f;    // a row that has seen nothing: 2^(-inf - 0) = 0
+            uint32_t pw[W / 2];
+#pragma unroll
+            for (int c = 0; c < W / 2; ++c) {
+                const float2 x = halves(add2(z[c], pair_of(e[c / 16] - m_sub, e[c / 16] - m_sub)));
+                const float p0 = fast_exp2(x.x), p1 = fast_exp2(x.y);
+                sums[c / 16] = add2(sums[c / 16], pair_of(p0, p1));
+                const __half2 t = __floats2half2_rn(p0, p1);
+                pw[c] = *reinterpret_cast<const uint32_t*>(&t);
+            }
+            if (!apart) {
+                const float2 s0 = halves(sums[0]), s1 = halves(sums[1]);
+                l += fmaf(s0.x + s0.y, power_of_two(-ve[0]), (s1.x + s1.y) * power_of_two(-ve[1]));
+            } else {
+                // scales more than 2^60 apart: what a weight is without its scale may be lost with it.  (It may be infinite
+                // here: the row's result is then 0, which it is beside the values of the largest scale.)
+                float sum = 0.0f;
+#pragma unroll
+                for (int c = 0; c < W / 2; ++c) {
+                    const float2 x = halves(z[c]);
+                    sum += fast_exp2(x.x - m_sub) + fast_exp2(x.y - m_sub);
+                }
+                l += sum;
+            }
+            tmem_st32(tmem + lane_addr + S_COL + s * BN + half * (W / 2), pw);
+            tmem_wait_st();
+            fence_before_sync();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(bar(P_FULL + s));
+                if (j % CHUNK == CHUNK - 1) mbar_arrive(bar(META_EMPTY + ((j / CHUNK) & 1)));
+            }
+        }
+        if (ok && n_tiles > 0) ok = wait_warp(bar(PV_DONE + ((n_tiles - 1) & 1)), ((n_tiles - 1) >> 1) & 1, give_up, 11);
+        // the row's sum is that of the two halves (always added in the same order), and so is what they have seen
+        const int fin = (n_tiles & 1) * 2;                   // the buffer that the next tile would have used
+        xch[(fin + half) * BM + r] = sees_bad || qs != qs ? __int_as_float(0x7fc00000) : l;
+        asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
+        const float total = xch[fin * BM + r] + xch[(fin + 1) * BM + r];
+        if (ok) {
+            fence_after_sync();
+            const float inv = total > 0.0f ? 1.0f / total : 0.0f;
+            const float v0 = power_of_two(e0);
+            const bool nan = total != total && pos >= 0;
+            const int row = row0 + r, tok = first_tok + row / a.group, head = g * a.group + row % a.group;
+            bf16* dst = a.out + (size_t)tok * a.out_stride + (size_t)head * HD;
+            const bool wide = ((uintptr_t)a.out & 15) == 0 && (a.out_stride & 7) == 0;
+#pragma unroll 1
+            for (int c = half * (HD / 2); c < (half + 1) * (HD / 2); c += 32) {
+                uint32_t ov[32];
+                if (n_tiles > 0) {
+                    tmem_ld32(tmem + lane_addr + O_COL + c, ov);
+                    tmem_wait_ld();
+                }
+                if (row_ok) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        uint4 pk;
+                        __nv_bfloat162* p2 = reinterpret_cast<__nv_bfloat162*>(&pk);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float x = n_tiles > 0 ? __uint_as_float(ov[i + 2 * e]) * inv * v0 : 0.0f;
+                            float y = n_tiles > 0 ? __uint_as_float(ov[i + 2 * e + 1]) * inv * v0 : 0.0f;
+                            if (nan) x = y = total;
+                            p2[e] = __floats2bfloat162_rn(x, y);
+                        }
+                        if (wide) *reinterpret_cast<uint4*>(dst + c + i) = pk;
+                        else {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) dst[c + i + e] = reinterpret_cast<const bf16*>(&pk)[e];
+                        }
+                    }
+                }
+            }
+        }
+    }
+    fence_before_sync();
+    __syncthreads();
+    if (warp == ISSUER) tmem_dealloc(tmem, TMEM_COLS);
+}
+
+// The rows of the pages [rows][hd] of bytes; box = box_bytes x 32 rows.
+int make_map(CUtensorMap* map, const void* ptr, long long rows, int hd, int box_bytes) {
+    EncodeTiled enc = encoder();
+    if (!enc) return BROLM_ERR_BAD_SIZE;
+    const cuuint64_t dims[2] = {(cuuint64_t)hd, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)hd};
+    const cuuint32_t box[2] = {(cuuint32_t)box_bytes, 32}, elem[2] = {1, 1};
+    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, elem,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? BROLM_OK : BROLM_ERR_ALIGNMENT;
+}
+
+template <int HD>
+int launch(const TcArgs& a, cudaStream_t stream) {
+    using SH = Shape<HD>;
+    constexpr size_t smem = (size_t)SH::Q_BYTES + (size_t)SH::SLOTS * UNIT + SH::RAWS * RAW + 2 * CHUNK * 4 * sizeof(Meta) + 5 * BM * 4 +
+                            (U_FULL + 2 * SH::SLOTS + 2 * SH::RAWS) * 8 + 32;
+    static_assert(smem <= 232448, "shared memory of a block");
+    static OncePerDevice raised;
+    int st = allow_shared_memory(attn_kv8_tc_kernel<HD>, smem, raised);
+    if (st) return st;
+    const long long blocks = (long long)a.row_tiles * a.n_kv * a.rows, rows = (long long)a.n_blocks * a.n_kv * a.block;
+    if (blocks > 0x7fffffffll || rows > 0x7fffffffll) return BROLM_ERR_TOO_LARGE;
+    CUtensorMap mk, mv;
+    st = make_map(&mk, a.k_pages, rows, HD, 64);
+    if (st) return st;
+    st = make_map(&mv, a.v_pages, rows, HD, HD);
+    if (st) return st;
+    return launch_pdl(attn_kv8_tc_kernel<HD>, dim3((unsigned)blocks), dim3(THREADS), smem, stream, mk, mv, a);
+}
+
+}  // namespace
+
+struct AttnTcCall {
+    const void* q;
+    void* out;
+    const void *cu_q, *kv_len, *slots, *tables, *k_pages, *v_pages, *k_scale, *v_scale;
+    cudaStream_t stream;
+    int q_stride, out_stride, tokens, rows, n_kv, group, dim, block, n_blocks, n_slots, width, ring, window, max_q_len;
+    float scale, cap;
+};
+
+// bfloat16, heads of 64, 128 or 256 entries.
+BROLM_API int brolm_attn_kv8_tc(const AttnTcCall* c) {
+    const int n_kv = c->n_kv, group = c->group, block = c->block;
+    if (c->dim != 64 && c->dim != 128 && c->dim != 256) return BROLM_ERR_BAD_SIZE;
+    if (c->tokens < 0 || c->rows < 0 || n_kv <= 0 || group <= 0 || block <= 0 || block % 32) return BROLM_ERR_BAD_SIZE;
+    if (c->n_blocks <= 0 || c->n_slots <= 0 || c->width <= 0 || c->ring < 0 || c->ring % block || c->window < 0 || c->max_q_len <= 0) return BROLM_ERR_BAD_SIZE;
+    if (block > MAX_BLOCK || (long long)n_kv * group > 65535 || (long long)c->max_q_len * group > 0x3fffffff) return BROLM_ERR_TOO_LARGE;
+    if ((long long)c->n_blocks * block > 0x7fffffffll || c->tokens > 0x3fffffff) return BROLM_ERR_TOO_LARGE;
+    if (((uintptr_t)c->k_pages | (uintptr_t)c->v_pages) & 15) return BROLM_ERR_ALIGNMENT;
+    if (c->tokens == 0 || c->rows == 0) return BROLM_OK;
+    const int wide = ((uintptr_t)c->q & 15) == 0 && c->q_stride % 8 == 0;
+    TcArgs a{(const bf16*)c->q, (bf16*)c->out, c->q_stride, c->out_stride, (const int32_t*)c->cu_q, (const int32_t*)c->kv_len,
+             (const int32_t*)c->slots, (const int32_t*)c->tables, (const int8_t*)c->k_pages, (const int8_t*)c->v_pages,
+             (const float*)c->k_scale, (const float*)c->v_scale, c->tokens, c->rows, n_kv, group, block, c->n_blocks, c->n_slots,
+             c->width, c->ring, c->window, (c->max_q_len * group + BM - 1) / BM, wide, c->scale, c->cap};
+    if (c->dim == 64) return launch<64>(a, c->stream);
+    if (c->dim == 128) return launch<128>(a, c->stream);
+    return launch<256>(a, c->stream);
+}
+
+BROLM_API int brolm_attn_kv8_tc_status(int reset) {
+    int v = 0;
+    if (cudaMemcpyFromSymbol(&v, g_attn_kv8_tc_error, sizeof(int)) != cudaSuccess) return -1;
+    if (reset && v) {
+        const int zero = 0;
+        cudaMemcpyToSymbol(g_attn_kv8_tc_error, &zero, sizeof(int));
+    }
+    return v;
+}
+
+BROLM_WAIT_CONTROL(attn_kv8_tc)

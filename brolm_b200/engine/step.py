@@ -238,7 +238,8 @@ class Engine:
         if self.model.dtype == torch.bfloat16:
             codes |= {"gemm_tc": kernels.gemm_tc_status(reset=True), "attn_tc": kernels.attention_tc_status(reset=True),
                       "gemm_stream": kernels.gemm_stream_status(reset=True),
-                      "grouped_tc": kernels.grouped_tc_status(reset=True)}
+                      "grouped_tc": kernels.grouped_tc_status(reset=True),
+                      "attn_kv8_tc": kernels.attention_kv8_tc_status(reset=True)}
         self._checked_at = launched
         bad = {k: v for k, v in codes.items() if v}
         if bad:

@@ -1478,7 +1478,7 @@ def gemm_tc_status(reset: bool = False) -> int:
     return f(1 if reset else 0)
 
 
-WAIT_LIBRARIES = ("linear_f32_tc", "gemm_tc", "gemm_tc2", "gemm_stream", "attn_tc", "grouped_tc")
+WAIT_LIBRARIES = ("linear_f32_tc", "gemm_tc", "gemm_tc2", "gemm_stream", "attn_tc", "grouped_tc", "attn_kv8_tc")
 
 
 def wait_control(library: str, cycles: int = 0, stall_code: int = 0) -> None:
@@ -2203,7 +2203,7 @@ def sample(logits: torch.Tensor, temperature: float, top_k: int, top_p: float, s
              _ptr(streams), counter, _ptr(out), _stream()), "sample")
 
 
-from .kv8 import BLOCKS_STATUS, attention_kv8, blocks_extend, blocks_release, kv8_read, kv8_write  # noqa: E402  (needs the above)
+from .kv8 import BLOCKS_STATUS, attention_kv8, attention_kv8_tc_status, blocks_extend, blocks_release, kv8_read, kv8_write  # noqa: E402  (needs the above)
 
 __all__ = ["KernelBuildError", "KernelError", "build_all", "launch_count", "device_sms", "wait_control", "embed_scale",
            "embed_pairs", "concat_cast", "latent_rows", "route_topk", "route_pick", "group_tiles", "group_pairs", "experts_tc_ok", "gather_rows", "experts_linear_tc", "grouped_tc_status", "heads_linear",
@@ -2212,4 +2212,4 @@ __all__ = ["KernelBuildError", "KernelError", "build_all", "launch_count", "devi
            "gemm_stream_status", "attention_simt", "attention_prefill_mma", "attention_prefill_tc", "attention_prefill_tc_ok", "attention_prefill_tc_split", "attention_tc_status", "attention_decode_mma",
            "decode_splits", "decode_longest_first", "argmax", "sample", "cast", "bias_act", "scaled_sum", "qkv_norm_write", "gate_group_norm", "head_norm_gate", "rotate_heads",
            "layernorm", "residual_layernorm", "table_gate", "delta_step", "delta_prompt", "experts_combine", "causal_conv", "conv_tail", "gated_scan", "ssm_scan", "block_matvec_f32", "block_matvec_ok", "split_halves",
-           "BLOCKS_STATUS", "blocks_extend", "blocks_release", "kv8_write", "kv8_read", "attention_kv8"]
+           "BLOCKS_STATUS", "blocks_extend", "blocks_release", "kv8_write", "kv8_read", "attention_kv8", "attention_kv8_tc_status"]

@@ -18,12 +18,12 @@ come from the device (slots, block ids, cache rows) and lie outside the tensors 
 from __future__ import annotations
 
 import struct
-from ctypes import c_char_p
+from ctypes import c_char_p, c_int
 from typing import Optional
 
 import torch
 
-from . import KernelError, _check, _fn, _stream, device_sms
+from . import KernelError, _check, _fn, _stream, device_sms, library_loaded, load_library
 
 # what the tables' status word says
 BLOCKS_STATUS = {0: "ok", 1: "too few free blocks (or a stack that does not fit)", 2: "a row of the tables is too narrow",
@@ -42,6 +42,7 @@ _RELEASE = struct.Struct("@7P4i")
 _WRITE = struct.Struct("@10P4q8i")
 _READ = struct.Struct("@11P4q10i")
 _ATTN = struct.Struct("@13P17i2f")
+_ATTN_TC = struct.Struct("@11P14i2f")
 _functions: dict = {}
 _NO_CPU = "brolm_b200 kernels run on CUDA tensors only; there is no CPU path"
 
@@ -222,6 +223,19 @@ def kv8_shares(batch: int, n_kv: int, row_tiles: int, keys: int, head_dim: int, 
     return KV8_CLUSTER, (1 if tiles < 96 else want // KV8_CLUSTER)
 
 
+KV8_TC_ROWS = 64      # from how many rows (tokens x heads of a kv head) the products of bfloat16 run on tcgen05
+
+
+def attention_kv8_tc_status(reset: bool = False) -> int:
+    """0 if no bounded wait inside the tcgen05 attention over the 8-bit cache ever ran out; otherwise its code.  Synchronises."""
+    if not library_loaded("attn_kv8_tc"):
+        return 0                   # its kernels never ran: nothing is built or loaded for the question
+    f = load_library("attn_kv8_tc").brolm_attn_kv8_tc_status
+    f.argtypes = [c_int]
+    f.restype = c_int
+    return f(1 if reset else 0)
+
+
 def attention_kv8(q: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, kv_len: torch.Tensor, slots: torch.Tensor,
                   tables: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale: torch.Tensor,
                   v_scale: torch.Tensor, *, n_kv: int, group: int, head_dim: int, scale: float, cap: float, window: int,
@@ -252,6 +266,12 @@ def attention_kv8(q: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, kv_len
         _refuse_ints(what, cu_q=(cu_q, batch + 1), kv_len=(kv_len, batch), slots=(slots, batch), tables=(tables, None))
     T = shape[0]
     rows = max_q_len * group
+    if rows >= KV8_TC_ROWS and dt is torch.bfloat16 and head_dim in (64, 128, 256) and n_blocks * n_kv * block < 1 << 31:
+        _call("attn_kv8_tc", "brolm_attn_kv8_tc", _ATTN_TC.pack(
+            q.data_ptr(), out.data_ptr(), cu_q.data_ptr(), kv_len.data_ptr(), slots.data_ptr(), tables.data_ptr(), k_pages.data_ptr(),
+            v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), _stream(), q0[0], o0[0], T, batch, n_kv, group, head_dim,
+            block, n_blocks, S, W, ring, window, max_q_len, scale, cap), what)
+        return
     keys = min(max_kv_len, window + max_q_len) if window > 0 else max_kv_len
     shares, spans = kv8_shares(batch, n_kv, 1 if rows <= 8 else -(-rows // 16), keys, head_dim)
     part_o = part_ml = 0

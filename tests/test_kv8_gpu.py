@@ -526,3 +526,91 @@ def test_launchers_refuse_sizes():
         kernels.blocks_extend(ints([0]), ints([0]), ints([1]), c.tables, ints([0]), ints([0]), ints([1]), block=32, ring=40,
                               cu_q=ints([0, 0]), kv_len=ints([0]), positions=ints([0]), tok_seq=ints([0]), cache_rows=ints([0]),
                               status=ints([0]))
+
+
+# --- pieces of prompts on tcgen05 --------------------------------------------------------------------------------------
+@pytest.mark.parametrize("D,G,group,P,cap", [(64, 2, 3, 32, 0.0), (128, 1, 5, 96, 30.0), (256, 2, 2, 64, 50.0), (256, 1, 1, 256, 0.0),
+                                             (128, 3, 4, 128, 3.0)])
+def test_pieces_of_prompts(D, G, group, P, cap):
+    """More rows than a block of threads has, row tiles that end inside a token's heads, sequences that bring little or
+    nothing (their rows of the tile are empty), lengths that end inside a tile, a window that begins inside one."""
+    lens = [300, 1, 129, 0, 515, 128]
+    c = filled(len(lens), -(-576 // P), G, P, D, [max(1, n) for n in lens], seed=D + P)
+    c.lens[3] = 0
+    for new, window in (([150, 1, 129, 0, 70, 128], 0), ([1, 0, 60, 0, 200, 33], 100), ([80, 1, 0, 0, 300, 1], 1)):
+        compare(c, torch.bfloat16, list(range(6)), new, group, D ** -0.5, cap, window, seed=sum(new), q_spread=2.0)
+    compare(c, torch.bfloat16, [4, -1, 0], [100, 3, 90], group, D ** -0.5, cap, 0)
+    for window in (31, 130):
+        compare(c, torch.bfloat16, [4, 0], [100, 128], group, D ** -0.5, cap, window)
+
+
+def test_a_piece_over_a_ring_of_unusual_blocks():
+    P, window, new = 96, 50, 70
+    ring = (window + new + P - 2 + P - 1) // P * P
+    c = filled(2, ring // P, 2, P, 128, [1, 90], ring=ring, seed=new)
+    g = torch.Generator().manual_seed(8)
+    for _ in range(5):
+        c.write([0, 1], [new] * 2, rows_of(2 * new, 2, 128, torch.bfloat16, g), rows_of(2 * new, 2, 128, torch.bfloat16, g))
+        compare(c, torch.bfloat16, [1, 0], [new] * 2, 3, 0.1, 0.0, window, seed=c.lens[0])
+
+
+def test_queries_and_results_of_a_piece_that_begin_off_sixteen_bytes():
+    c = filled(1, 4, 2, 64, 64, [200], seed=2)
+    wide = torch.randn((100, 300)).bfloat16().to(DEV)
+    for at in (1, 4, 8):
+        out = torch.full((100, 300), 7.0, dtype=torch.bfloat16, device=DEV)
+        args = dict(n_kv=2, group=2, head_dim=64, scale=0.125, cap=0.0, window=0, ring=0, batch=1, max_q_len=100, max_kv_len=200)
+        rest = (ints([0, 100]), ints([200]), ints([0]), c.tables, *c.dev)
+        kernels.attention_kv8(wide[:, at:at + 256], out[:, at:at + 256], *rest, **args)
+        q, plain_out = wide[:, at:at + 256].contiguous(), torch.empty((100, 256), dtype=torch.bfloat16, device=DEV)
+        kernels.attention_kv8(q, plain_out, *rest, **args)
+        assert torch.equal(out[:, at:at + 256], plain_out)
+        assert bool((out[:, :at] == 7.0).all()) and bool((out[:, at + 256:] == 7.0).all())
+
+
+def test_a_query_of_a_piece_that_is_not_a_number():
+    c = filled(1, 3, 1, 64, 64, [150], seed=3)
+    q = torch.randn((90, 2 * 64)).bfloat16().to(DEV)
+    q[17, 70] = INF
+    out = torch.empty_like(q)
+    kernels.attention_kv8(q, out, ints([0, 90]), ints([150]), ints([0]), c.tables, *c.dev, n_kv=1, group=2, head_dim=64, scale=0.1,
+                          cap=0.0, window=0, ring=0, batch=1, max_q_len=90, max_kv_len=150)
+    bad = torch.isnan(out)
+    assert bool(bad[17, 64:].all()) and int(bad.sum()) == 64
+
+
+def test_a_piece_whose_values_scales_lie_2_to_the_100_apart():
+    """Blocks of values of size 1, 2^-70 and 2^-110 beside each other: rows that see only small ones keep their bits, and rows
+    that see large ones lose nothing by them."""
+    c = Cached(1, 6, 1, 32, 64, seed=7)
+    g = torch.Generator().manual_seed(3)
+    for step in range(6):
+        k, v = (rows_of(32, 1, 64, torch.float32, g, 0.2) for _ in range(2))
+        c.write([0], [32], k, v * 2.0 ** (-110, -70, -110, 0, -70, 0)[step])
+    compare(c, torch.bfloat16, [0], [100], 1, 0.125, 0.0, 20)        # windows of 20: most rows see one or two blocks
+    compare(c, torch.bfloat16, [0], [192], 1, 0.125, 0.0, 0)
+
+
+@pytest.mark.parametrize("code", [8, 9])
+def test_a_piece_whose_wait_runs_out(code):
+    """The softmax warps' waits for a score tile and for the lookups never end: the launch gives up, says so, and the next
+    one is right."""
+    c = filled(1, 10, 2, 64, 128, [600], seed=5)
+    q = torch.randn((200, 4 * 128)).bfloat16().to(DEV)
+
+    def run():
+        out = torch.empty_like(q)
+        kernels.attention_kv8(q, out, ints([0, 200]), ints([600]), ints([0]), c.tables, *c.dev, n_kv=2, group=2, head_dim=128,
+                              scale=0.09, cap=0.0, window=0, ring=0, batch=1, max_q_len=200, max_kv_len=600)
+        torch.cuda.synchronize()
+        return out
+
+    good = run()
+    assert kernels.attention_kv8_tc_status(reset=True) == 0
+    kernels.wait_control("attn_kv8_tc", cycles=8_000_000, stall_code=code)
+    try:
+        run()
+        assert kernels.attention_kv8_tc_status(reset=True) == code and kernels.attention_kv8_tc_status() == 0
+    finally:
+        kernels.wait_control("attn_kv8_tc", 0, 0)
+    assert torch.equal(run(), good) and kernels.attention_kv8_tc_status() == 0
