@@ -25,7 +25,7 @@
 //
 // The shares of a row's keys are joined inside the launch: they form a cluster, whose blocks read each other's partial
 // results out of shared memory.  Nothing is kept between launches.
-#include "kv8.cuh"
+#include "attn_kv8_join.cuh"
 
 #include <cuda_fp16.h>
 
@@ -33,7 +33,6 @@ namespace {
 
 using namespace kv8;
 
-constexpr float LOG2E = 1.4426950408889634f;
 constexpr int WARPS = 4, THREADS = 32 * WARPS;
 constexpr int MAX_SHARES = 8;             // blocks of a cluster
 constexpr int KT = 32;                    // keys of a tile: a divisor of every block size
@@ -52,11 +51,6 @@ struct AttnArgs {
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ float rcp(float x) {
     float y;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -130,21 +124,6 @@ __device__ __forceinline__ int value_offset(int row, int c) {
         const int at = (row & ~7) | ((row >> 1) & 3) | ((row & 1) << 2);
         return at * DP + ((c ^ (((at >> 1) & 1) << 1)) << 4);
     }
-}
-
-__device__ __forceinline__ void add_part(float4& acc, float& sum, const float4& x, float l, float f) {
-    sum = fmaf(l, f, sum);
-    acc.x = fmaf(x.x, f, acc.x); acc.y = fmaf(x.y, f, acc.y); acc.z = fmaf(x.z, f, acc.z); acc.w = fmaf(x.w, f, acc.w);
-}
-// Four entries of a row: zeros where nothing was seen, NaN where something was not a number.
-template <typename T>
-__device__ __forceinline__ void store_row(const AttnArgs& a, int tok, int head, int d, const float4& acc, float sum) {
-    const float inv = sum > 0.0f ? 1.0f / sum : sum != 0.0f ? sum : acc.x != acc.x ? 1.0f : 0.0f;
-    T* dst = reinterpret_cast<T*>(a.out) + (size_t)tok * a.out_stride + head * a.dim + d;
-    dst[0] = from_float<T>(acc.x * inv);
-    dst[1] = from_float<T>(acc.y * inv);
-    dst[2] = from_float<T>(acc.z * inv);
-    dst[3] = from_float<T>(acc.w * inv);
 }
 
 __device__ __forceinline__ int ld_now(const int32_t* p) {
@@ -386,7 +365,7 @@ __device__ __forceinline__ void merge(const AttnArgs& a, const Item& it, const f
             *reinterpret_cast<float4*>(a.part_o + at * a.dim + d) = acc;
             if (d == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(most, sum);
         } else {
-            store_row<T>(a, tok, head, d, acc, sum);
+            store_row<T>(a.out, a.out_stride, a.dim, tok, head, d, acc, sum);
         }
     }
     if (a.shares > 1) cluster_barrier();                       // nobody leaves while its results are being read
@@ -959,43 +938,6 @@ __global__ void __launch_bounds__(THREADS, 2) attn_kv8_kernel(AttnArgs a) {
     merge<T, ROWS, SH::PITCH>(a, it, wo, wml, co, cml, q_scale);
 }
 
-// Rows whose keys were shared by several clusters: a block of threads for every (token, head).
-template <typename T>
-__global__ void __launch_bounds__(64) attn_kv8_join_kernel(AttnArgs a) {
-    pdl_trigger();
-    pdl_wait();
-    const int tok = blockIdx.x, head = blockIdx.y;
-    if (tok >= a.cu_q[a.rows]) return;
-    const size_t at = ((size_t)tok * a.n_kv * a.group + head) * a.spans;
-    const int d = threadIdx.x * 4;
-    if (d >= a.dim) return;
-    float most = -INFINITY, sum = 0.0f;
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int s0 = 0; s0 < a.spans; s0 += 8) {                  // (eight parts are asked for at once)
-        float2 ml[8];
-        float4 x[8];
-        float top = most;
-#pragma unroll
-        for (int s = 0; s < 8; ++s) {
-            ml[s] = make_float2(-INFINITY, 0.0f);
-            x[s] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (s0 + s < a.spans) {
-                ml[s] = *reinterpret_cast<const float2*>(a.part_ml + (at + s0 + s) * 2);
-                x[s] = *reinterpret_cast<const float4*>(a.part_o + (at + s0 + s) * a.dim + d);
-            }
-            top = fmaxf(top, ml[s].x);
-        }
-        const float keep = most > -INFINITY ? ex2(most - top) : 1.0f;
-        most = top;
-        sum *= keep;
-        acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
-#pragma unroll
-        for (int s = 0; s < 8; ++s)
-            if (s0 + s < a.spans) add_part(acc, sum, x[s], ml[s].y, top > -INFINITY ? ex2(ml[s].x - top) : 0.0f);
-    }
-    store_row<T>(a, tok, head, d, acc, sum);
-}
-
 template <typename T>
 int launch(void (*kernel)(AttnArgs), size_t smem, OncePerDevice& raised, const AttnArgs& a, cudaStream_t stream) {
     const int st = allow_shared_memory(kernel, smem, raised);
@@ -1017,7 +959,7 @@ int launch(void (*kernel)(AttnArgs), size_t smem, OncePerDevice& raised, const A
     cfg.numAttrs = 2;
     const int e = (int)cudaLaunchKernelEx(&cfg, kernel, a);
     if (e || a.spans == 1) return e;
-    return launch_pdl(attn_kv8_join_kernel<T>, dim3(a.tokens, a.n_kv * a.group), dim3(64), 0, stream, a);
+    return launch_join<T>(JoinArgs{a.part_o, a.part_ml, a.out, a.cu_q, a.out_stride, a.rows, a.tokens, a.n_kv * a.group, a.dim, a.spans}, stream);
 }
 
 template <typename T, int DP>

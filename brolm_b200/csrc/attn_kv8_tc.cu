@@ -35,7 +35,7 @@
 // Every mbarrier wait is bounded; a wait that runs out records a code that brolm_attn_kv8_tc_status() returns, and the
 // launch ends without its results.
 #include "tcgen05.cuh"
-#include "kv8.cuh"
+#include "attn_kv8_join.cuh"
 
 #include <cuda_fp16.h>
 
@@ -55,7 +55,6 @@ constexpr int TMEM_COLS = 512;
 constexpr int UNIT = 16384;               // bytes of a slot: 128 keys x 64 entries, or the same number of values
 constexpr int RAW = UNIT / 2;             // .. as they come from the cache
 constexpr int CHUNK = 8;                  // tiles whose places and scales are looked up at a time (32 groups of 32 keys)
-constexpr float LOG2E = 1.4426950408889634f;
 constexpr float RESCALE_GAP = 8.0f;
 
 __device__ int g_attn_kv8_tc_error;
@@ -69,6 +68,8 @@ struct TcArgs {
     const float *k_scale, *v_scale;
     int tokens, rows, n_kv, group, block, n_blocks, n_slots, width, ring, window, row_tiles, wide;
     float scale, cap;
+    int spans;                            // blocks that share a row tile's keys; more than one: joined by a second launch
+    float *part_o, *part_ml;
 };
 
 template <int HD>
@@ -232,8 +233,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_wait();
     // blocks start in the order of their index: the last rows, which see the most keys, of every sequence and head first
-    const int per = a.n_kv * a.rows;
-    const int xt = a.row_tiles - 1 - (int)(blockIdx.x / per), which = blockIdx.x % per;
+    const int per = a.n_kv * a.rows * a.spans;
+    const int xt = a.row_tiles - 1 - (int)(blockIdx.x / per), which = blockIdx.x % per / a.spans, span = blockIdx.x % a.spans;
     const int b = which / a.n_kv, g = which - b * a.n_kv;
     const int first_tok = a.cu_q[b], n_tok = min(a.cu_q[b + 1], a.tokens) - first_tok;
     const int kv_len = a.kv_len[b], slot = a.slots[b];
@@ -246,7 +247,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
     if (pos_hi >= 0 && slot >= 0 && slot < a.n_slots) {
         t_first = max(0, pos_lo - window + 1) / BN;
         n_tiles = pos_hi / BN - t_first + 1;
+        const int share = (n_tiles + a.spans - 1) / a.spans;
+        t_first += span * share;
+        n_tiles = max(0, min(share, n_tiles - span * share));
     }
+    const int key_hi = min(pos_hi, (t_first + n_tiles) * BN - 1);     // the last key of this block's share
     const int32_t* table = a.tables + (size_t)max(slot, 0) * a.width;
 
     if (threadIdx.x == 0) {
@@ -282,10 +287,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
     };
     if (n_tiles > 0) {
         // e0: the largest exponent among the value scales of the keys that this block sees
-        const int first32 = t_first * (BN / 32), n32 = pos_hi / 32 - first32 + 1;
+        const int first32 = t_first * (BN / 32), n32 = key_hi / 32 - first32 + 1;
         int top = -126;
         for (int i = threadIdx.x; i * block32 < n32 + block32; i += THREADS) {
-            const int at = min(first32 + i * block32, pos_hi / 32);
+            const int at = min(first32 + i * block32, key_hi / 32);
             const float s = a.v_scale[(size_t)block_of(a.ring > 0 ? at % (a.ring >> 5) : at) * a.n_kv + g];
             if (s == s) top = max(top, (int)(__float_as_uint(s) >> 23 & 255u) - 127);
         }
@@ -340,7 +345,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
                 if (!wait_warp(bar(META_EMPTY + (m & 1)), ((m >> 1) & 1) ^ 1, give_up, 3)) break;
                 const int at32 = (t_first + m * CHUNK) * (BN / 32) + lane;
                 Meta x{0, 0.0f, 0};
-                if (at32 <= pos_hi / 32) {
+                if (at32 <= key_hi / 32) {
                     const int place32 = a.ring > 0 ? at32 % (a.ring >> 5) : at32;
                     const size_t bh = (size_t)block_of(place32) * a.n_kv + g;
                     x.row = (int)bh * a.block + (place32 % block32) * 32;
@@ -645,6 +650,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
             const bool nan = total != total && pos >= 0;
             const int row = row0 + r, tok = first_tok + row / a.group, head = g * a.group + row % a.group;
             bf16* dst = a.out + (size_t)tok * a.out_stride + (size_t)head * HD;
+            const size_t part = ((size_t)tok * a.n_kv * a.group + head) * a.spans + span;
+            if (a.spans > 1 && row_ok && half == 0) *reinterpret_cast<float2*>(a.part_ml + part * 2) = make_float2(m_ref, total);
             const bool wide = ((uintptr_t)a.out & 15) == 0 && (a.out_stride & 7) == 0;
 #pragma unroll 1
             for (int c = half * (HD / 2); c < (half + 1) * (HD / 2); c += 32) {
@@ -653,7 +660,16 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
                     tmem_ld32(tmem + lane_addr + O_COL + c, ov);
                     tmem_wait_ld();
                 }
-                if (row_ok) {
+                if (row_ok && a.spans > 1) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        if (n_tiles > 0)
+                            x = make_float4(__uint_as_float(ov[i]) * v0, __uint_as_float(ov[i + 1]) * v0, __uint_as_float(ov[i + 2]) * v0,
+                                            __uint_as_float(ov[i + 3]) * v0);
+                        *reinterpret_cast<float4*>(a.part_o + part * HD + c + i) = x;
+                    }
+                } else if (row_ok) {
 #pragma unroll
                     for (int i = 0; i < 32; i += 8) {
                         uint4 pk;
@@ -702,14 +718,16 @@ int launch(const TcArgs& a, cudaStream_t stream) {
     static OncePerDevice raised;
     int st = allow_shared_memory(attn_kv8_tc_kernel<HD>, smem, raised);
     if (st) return st;
-    const long long blocks = (long long)a.row_tiles * a.n_kv * a.rows, rows = (long long)a.n_blocks * a.n_kv * a.block;
+    const long long blocks = (long long)a.row_tiles * a.n_kv * a.rows * a.spans, rows = (long long)a.n_blocks * a.n_kv * a.block;
     if (blocks > 0x7fffffffll || rows > 0x7fffffffll) return BROLM_ERR_TOO_LARGE;
     CUtensorMap mk, mv;
     st = make_map(&mk, a.k_pages, rows, HD, 64);
     if (st) return st;
     st = make_map(&mv, a.v_pages, rows, HD, HD);
     if (st) return st;
-    return launch_pdl(attn_kv8_tc_kernel<HD>, dim3((unsigned)blocks), dim3(THREADS), smem, stream, mk, mv, a);
+    st = launch_pdl(attn_kv8_tc_kernel<HD>, dim3((unsigned)blocks), dim3(THREADS), smem, stream, mk, mv, a);
+    if (st || a.spans == 1) return st;
+    return launch_join<bf16>(JoinArgs{a.part_o, a.part_ml, a.out, a.cu_q, a.out_stride, a.rows, a.tokens, a.n_kv * a.group, HD, a.spans}, stream);
 }
 
 }  // namespace
@@ -718,8 +736,9 @@ struct AttnTcCall {
     const void* q;
     void* out;
     const void *cu_q, *kv_len, *slots, *tables, *k_pages, *v_pages, *k_scale, *v_scale;
+    void *part_o, *part_ml;               // spans > 1: [tokens * n_kv * group * spans * dim] and [.. * 2]
     cudaStream_t stream;
-    int q_stride, out_stride, tokens, rows, n_kv, group, dim, block, n_blocks, n_slots, width, ring, window, max_q_len;
+    int q_stride, out_stride, tokens, rows, n_kv, group, dim, block, n_blocks, n_slots, width, ring, window, max_q_len, spans;
     float scale, cap;
 };
 
@@ -731,13 +750,14 @@ BROLM_API int brolm_attn_kv8_tc(const AttnTcCall* c) {
     if (c->n_blocks <= 0 || c->n_slots <= 0 || c->width <= 0 || c->ring < 0 || c->ring % block || c->window < 0 || c->max_q_len <= 0) return BROLM_ERR_BAD_SIZE;
     if (block > MAX_BLOCK || (long long)n_kv * group > 65535 || (long long)c->max_q_len * group > 0x3fffffff) return BROLM_ERR_TOO_LARGE;
     if ((long long)c->n_blocks * block > 0x7fffffffll || c->tokens > 0x3fffffff) return BROLM_ERR_TOO_LARGE;
-    if (((uintptr_t)c->k_pages | (uintptr_t)c->v_pages) & 15) return BROLM_ERR_ALIGNMENT;
+    if (c->spans < 1 || (c->spans > 1 && (!c->part_o || !c->part_ml))) return BROLM_ERR_BAD_SIZE;
+    if (((uintptr_t)c->k_pages | (uintptr_t)c->v_pages | (uintptr_t)c->part_o) & 15) return BROLM_ERR_ALIGNMENT;
     if (c->tokens == 0 || c->rows == 0) return BROLM_OK;
     const int wide = ((uintptr_t)c->q & 15) == 0 && c->q_stride % 8 == 0;
     TcArgs a{(const bf16*)c->q, (bf16*)c->out, c->q_stride, c->out_stride, (const int32_t*)c->cu_q, (const int32_t*)c->kv_len,
              (const int32_t*)c->slots, (const int32_t*)c->tables, (const int8_t*)c->k_pages, (const int8_t*)c->v_pages,
              (const float*)c->k_scale, (const float*)c->v_scale, c->tokens, c->rows, n_kv, group, block, c->n_blocks, c->n_slots,
-             c->width, c->ring, c->window, (c->max_q_len * group + BM - 1) / BM, wide, c->scale, c->cap};
+             c->width, c->ring, c->window, (c->max_q_len * group + BM - 1) / BM, wide, c->scale, c->cap, c->spans, (float*)c->part_o, (float*)c->part_ml};
     if (c->dim == 64) return launch<64>(a, c->stream);
     if (c->dim == 128) return launch<128>(a, c->stream);
     return launch<256>(a, c->stream);

@@ -60,7 +60,7 @@ LIBRARIES: dict[str, list[str]] = {
     "attn_kv8": ["attn_kv8.cu"],
     "attn_kv8_tc": ["attn_kv8_tc.cu"],
 }
-HEADERS = ["common.cuh", "once_per_device.h", "attn_mma.cuh", "attn_decode_noalloc.h", "tcgen05.cuh", "kv8.cuh"]
+HEADERS = ["common.cuh", "once_per_device.h", "attn_mma.cuh", "attn_decode_noalloc.h", "tcgen05.cuh", "kv8.cuh", "attn_kv8_join.cuh"]
 
 _loaded: dict[str, ctypes.CDLL] = {}
 _lock = threading.Lock()

@@ -17,10 +17,9 @@ come from the device (slots, block ids, cache rows) and lie outside the tensors 
 """
 from __future__ import annotations
 
+import functools
 import struct
 from ctypes import c_char_p, c_int
-from typing import Optional
-
 import torch
 
 from . import KernelError, _check, _fn, _stream, device_sms, library_loaded, load_library
@@ -42,7 +41,7 @@ _RELEASE = struct.Struct("@7P4i")
 _WRITE = struct.Struct("@10P4q8i")
 _READ = struct.Struct("@11P4q10i")
 _ATTN = struct.Struct("@13P17i2f")
-_ATTN_TC = struct.Struct("@11P14i2f")
+_ATTN_TC = struct.Struct("@13P15i2f")
 _functions: dict = {}
 _NO_CPU = "brolm_b200 kernels run on CUDA tensors only; there is no CPU path"
 
@@ -194,7 +193,8 @@ def kv8_read(cu_q: torch.Tensor, kv_len: torch.Tensor, slots: torch.Tensor, tabl
 KV8_TILE, KV8_WARPS, KV8_CLUSTER = 32, 4, 8       # keys of a tile, warps of a block, blocks that join their results themselves
 
 
-def kv8_shares(batch: int, n_kv: int, row_tiles: int, keys: int, head_dim: int, sms: Optional[int] = None) -> tuple[int, int]:
+@functools.lru_cache(maxsize=256)
+def kv8_shares(batch: int, n_kv: int, row_tiles: int, keys: int, head_dim: int, sms: int) -> tuple[int, int]:
     """How many blocks share the keys of one (sequence, kv head, tile of query rows): (blocks of a cluster, clusters).
 
     Two blocks run on an SM (three, of heads of up to 64 entries), and there are as many shares as give every SM its blocks,
@@ -206,7 +206,6 @@ def kv8_shares(batch: int, n_kv: int, row_tiles: int, keys: int, head_dim: int, 
     are cut into rounds of blocks that the SMs take as they come free, if the shares stay long enough (24 tiles) and fill
     their rounds (16 sequences of 129 to 6,145 keys under a window of 4,096, 8 kv heads: 36.9 us as 2 x 1, 32.1 as 1 x 4; of
     equal ones 32 of 2,048, 4 kv heads: 28.3 as 2 x 1, 30.6 as 1 x 4, which is what it costs)."""
-    sms = sms or device_sms()
     places = (3 if head_dim <= 64 else 2) * sms
     items = max(1, batch * n_kv * row_tiles)
     tiles = max(1, -(-keys // KV8_TILE))
@@ -223,7 +222,32 @@ def kv8_shares(batch: int, n_kv: int, row_tiles: int, keys: int, head_dim: int, 
     return KV8_CLUSTER, (1 if tiles < 96 else want // KV8_CLUSTER)
 
 
-KV8_TC_ROWS = 64      # from how many rows (tokens x heads of a kv head) the products of bfloat16 run on tcgen05
+def _parts(n: int, head_dim: int, device) -> tuple:
+    """Room for n parts of rows: the tensor that holds it, and where the sums and their (maximum, weight) begin."""
+    parts = torch.empty(n * (head_dim + 2), dtype=_F32, device=device)
+    at = parts.data_ptr()
+    return parts, at, at + 4 * n * head_dim
+
+
+@functools.lru_cache(maxsize=256)
+def kv8_tc_spans(tokens: int, batch: int, n_kv: int, group: int, max_q_len: int, keys: int, head_dim: int, sms: int) -> int:
+    """How many blocks share the keys of a tile of 128 query rows on tcgen05: one block runs on an SM, so what counts is how
+    many rounds of blocks there are and how long a block's share is.  In tiles of 128 keys (3 us each at 256 entries): a
+    block begins and ends in three, and joining costs another three and what the parts take to memory and back."""
+    items = batch * n_kv * -(-max_q_len * group // 128)
+    tiles = -(-keys // 128)
+    traffic = tokens * n_kv * group * head_dim * 8 / 6.5e12 / (3e-6 * head_dim / 256)
+
+    def cost(k):
+        return -(-items * k // sms) * (-(-tiles // k) + 3) + (3 + k * traffic if k > 1 else 0)
+    return min(range(1, max(2, min(32, tiles // 2) + 1)), key=cost)
+
+
+# From how many rows of a kv head (tokens x query heads), and from how many of rows x kv heads x keys x entries, a step of
+# bfloat16 runs on tcgen05, whose blocks take 128 rows and 18 us to begin and end.  8 kv heads of 256, two query heads each,
+# us on mma.sync / tcgen05: 32 tokens on 1,000 keys (1.3e8) 14.7 / 20.2, 128 on 300 (1.6e8) 17.1 / 23.3, 16 on 4,096 (2.7e8)
+# 27.0 / 22.5, 64 on 4,096 (1.1e9) 39.4 / 30.4, 512 on 8,192 (1.7e10) 450 / 123; 4 x 64 on 1,000 (5.2e8) 38.9 / 31.9.
+KV8_TC_ROWS, KV8_TC_WORK = 32, 2.5e8
 
 
 def attention_kv8_tc_status(reset: bool = False) -> int:
@@ -266,20 +290,22 @@ def attention_kv8(q: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, kv_len
         _refuse_ints(what, cu_q=(cu_q, batch + 1), kv_len=(kv_len, batch), slots=(slots, batch), tables=(tables, None))
     T = shape[0]
     rows = max_q_len * group
-    if rows >= KV8_TC_ROWS and dt is torch.bfloat16 and head_dim in (64, 128, 256) and n_blocks * n_kv * block < 1 << 31:
+    keys = min(max_kv_len, window + max_q_len) if window > 0 else max_kv_len
+    if rows >= KV8_TC_ROWS and dt is torch.bfloat16 and head_dim in (64, 128, 256) and n_blocks * n_kv * block < 1 << 31 and \
+            float(T) * group * n_kv * keys * head_dim >= KV8_TC_WORK:
+        spans = kv8_tc_spans(T, batch, n_kv, group, max_q_len, keys, head_dim, device_sms())
+        part_o = part_ml = 0
+        if spans > 1:
+            parts, part_o, part_ml = _parts(T * n_kv * group * spans, head_dim, q.device)
         _call("attn_kv8_tc", "brolm_attn_kv8_tc", _ATTN_TC.pack(
             q.data_ptr(), out.data_ptr(), cu_q.data_ptr(), kv_len.data_ptr(), slots.data_ptr(), tables.data_ptr(), k_pages.data_ptr(),
-            v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), _stream(), q0[0], o0[0], T, batch, n_kv, group, head_dim,
-            block, n_blocks, S, W, ring, window, max_q_len, scale, cap), what)
+            v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), part_o, part_ml, _stream(), q0[0], o0[0], T, batch, n_kv, group,
+            head_dim, block, n_blocks, S, W, ring, window, max_q_len, spans, scale, cap), what)
         return
-    keys = min(max_kv_len, window + max_q_len) if window > 0 else max_kv_len
-    shares, spans = kv8_shares(batch, n_kv, 1 if rows <= 8 else -(-rows // 16), keys, head_dim)
+    shares, spans = kv8_shares(batch, n_kv, 1 if rows <= 8 else -(-rows // 16), keys, head_dim, device_sms())
     part_o = part_ml = 0
     if spans > 1:
-        n = T * n_kv * group * spans
-        parts = torch.empty(n * (head_dim + 2), dtype=_F32, device=q.device)
-        part_o = parts.data_ptr()
-        part_ml = part_o + 4 * n * head_dim
+        parts, part_o, part_ml = _parts(T * n_kv * group * spans, head_dim, q.device)
     _call("attn_kv8", "brolm_attn_kv8", _ATTN.pack(
         q.data_ptr(), out.data_ptr(), cu_q.data_ptr(), kv_len.data_ptr(), slots.data_ptr(), tables.data_ptr(), k_pages.data_ptr(),
         v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), part_o, part_ml, _stream(), q0[0], o0[0], _CODES[dt], T, batch,

@@ -359,10 +359,21 @@ def test_attention_of_one_token(dtype, D, G, group, P):
     compare(c, dtype, list(range(8)), [1] * 8, group, D ** -0.5, 20.0, 0, q_spread=4.0)
 
 
+@pytest.fixture(params=[False, True], ids=["mma", "tcgen05"])
+def either(request, monkeypatch):
+    """Steps of many rows on mma.sync, and on tcgen05 where it takes their sizes."""
+    monkeypatch.setattr(kernels.kv8, "KV8_TC_WORK", 0.0 if request.param else math.inf)
+
+
+@pytest.fixture
+def on_tcgen05(monkeypatch):
+    monkeypatch.setattr(kernels.kv8, "KV8_TC_WORK", 0.0)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("D,G,group,P", [(64, 2, 2, 64), (128, 1, 4, 32), (256, 2, 2, 64), (256, 1, 16, 64), (80, 1, 3, 32), (64, 1, 128, 32)])
 @pytest.mark.parametrize("window", [0, 1, 50])
-def test_attention_of_several_tokens(dtype, D, G, group, P, window):
+def test_attention_of_several_tokens(dtype, D, G, group, P, window, either):
     lens = [3, 70, 140, 1, 257]
     c = filled(len(lens), -(-288 // P), G, P, D, lens, seed=D + window)
     for new in ([3, 1, 5, 1, 2], [3, 70, 40, 1, 131]):
@@ -371,7 +382,7 @@ def test_attention_of_several_tokens(dtype, D, G, group, P, window):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("new", [1, 4, 67])
-def test_attention_over_a_ring(dtype, new):
+def test_attention_over_a_ring(dtype, new, either):
     P, window = 32, 41
     ring = (window + new + P - 2 + P - 1) // P * P
     c = filled(3, ring // P, 2, P, 64, [1, 33, 90], ring=ring, seed=new)
@@ -393,7 +404,7 @@ def test_attention_over_long_sequences_is_split_and_joined(dtype):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("new", [1, 3, 80])
-def test_blocks_that_a_token_does_not_see_change_nothing(dtype, new):
+def test_blocks_that_a_token_does_not_see_change_nothing(dtype, new, either):
     """A NaN block before the window, or behind the token, must not reach it; one that it sees makes it NaN."""
     for value, at in ((NAN, 10), (INF, 140), (NAN, 295)):
         c = Cached(2, 10, 2, 32, 64, seed=6)
@@ -410,7 +421,7 @@ def test_blocks_that_a_token_does_not_see_change_nothing(dtype, new):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("new", [1, 40])
-def test_attention_where_numbers_are_of_all_sizes(dtype, new):
+def test_attention_where_numbers_are_of_all_sizes(dtype, new, either):
     """Keys and values whose blocks differ by powers of ten, queries that are very large or small, scores that leave one
     key all the weight."""
     c = Cached(2, 6, 1, 32, 64, seed=7)
@@ -439,8 +450,8 @@ def test_a_query_that_is_not_a_number(new):
         assert bool(bad[0, 32:64].all()) and int(bad.sum()) == 32
 
 
-@pytest.mark.parametrize("new", [1, 33])
-def test_cache_of_more_than_31_bits_of_bytes(new):
+@pytest.mark.parametrize("new", [1, 33, 200])
+def test_cache_of_more_than_31_bits_of_bytes(new, on_tcgen05):
     """Blocks whose bytes lie beyond 2^31, of a sequence and of its neighbours' heads."""
     G, P, D = 16, 64, 256
     N = (1 << 31) // (G * P * D) + 40
@@ -531,7 +542,7 @@ def test_launchers_refuse_sizes():
 # --- pieces of prompts on tcgen05 --------------------------------------------------------------------------------------
 @pytest.mark.parametrize("D,G,group,P,cap", [(64, 2, 3, 32, 0.0), (128, 1, 5, 96, 30.0), (256, 2, 2, 64, 50.0), (256, 1, 1, 256, 0.0),
                                              (128, 3, 4, 128, 3.0)])
-def test_pieces_of_prompts(D, G, group, P, cap):
+def test_pieces_of_prompts(D, G, group, P, cap, on_tcgen05):
     """More rows than a block of threads has, row tiles that end inside a token's heads, sequences that bring little or
     nothing (their rows of the tile are empty), lengths that end inside a tile, a window that begins inside one."""
     lens = [300, 1, 129, 0, 515, 128]
@@ -544,7 +555,7 @@ def test_pieces_of_prompts(D, G, group, P, cap):
         compare(c, torch.bfloat16, [4, 0], [100, 128], group, D ** -0.5, cap, window)
 
 
-def test_a_piece_over_a_ring_of_unusual_blocks():
+def test_a_piece_over_a_ring_of_unusual_blocks(on_tcgen05):
     P, window, new = 96, 50, 70
     ring = (window + new + P - 2 + P - 1) // P * P
     c = filled(2, ring // P, 2, P, 128, [1, 90], ring=ring, seed=new)
@@ -554,7 +565,7 @@ def test_a_piece_over_a_ring_of_unusual_blocks():
         compare(c, torch.bfloat16, [1, 0], [new] * 2, 3, 0.1, 0.0, window, seed=c.lens[0])
 
 
-def test_queries_and_results_of_a_piece_that_begin_off_sixteen_bytes():
+def test_queries_and_results_of_a_piece_that_begin_off_sixteen_bytes(on_tcgen05):
     c = filled(1, 4, 2, 64, 64, [200], seed=2)
     wide = torch.randn((100, 300)).bfloat16().to(DEV)
     for at in (1, 4, 8):
@@ -568,7 +579,7 @@ def test_queries_and_results_of_a_piece_that_begin_off_sixteen_bytes():
         assert bool((out[:, :at] == 7.0).all()) and bool((out[:, at + 256:] == 7.0).all())
 
 
-def test_a_query_of_a_piece_that_is_not_a_number():
+def test_a_query_of_a_piece_that_is_not_a_number(on_tcgen05):
     c = filled(1, 3, 1, 64, 64, [150], seed=3)
     q = torch.randn((90, 2 * 64)).bfloat16().to(DEV)
     q[17, 70] = INF
@@ -579,7 +590,7 @@ def test_a_query_of_a_piece_that_is_not_a_number():
     assert bool(bad[17, 64:].all()) and int(bad.sum()) == 64
 
 
-def test_a_piece_whose_values_scales_lie_2_to_the_100_apart():
+def test_a_piece_whose_values_scales_lie_2_to_the_100_apart(on_tcgen05):
     """Blocks of values of size 1, 2^-70 and 2^-110 beside each other: rows that see only small ones keep their bits, and rows
     that see large ones lose nothing by them."""
     c = Cached(1, 6, 1, 32, 64, seed=7)
@@ -592,7 +603,7 @@ def test_a_piece_whose_values_scales_lie_2_to_the_100_apart():
 
 
 @pytest.mark.parametrize("code", [8, 9])
-def test_a_piece_whose_wait_runs_out(code):
+def test_a_piece_whose_wait_runs_out(code, on_tcgen05):
     """The softmax warps' waits for a score tile and for the lookups never end: the launch gives up, says so, and the next
     one is right."""
     c = filled(1, 10, 2, 64, 128, [600], seed=5)
