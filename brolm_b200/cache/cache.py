@@ -29,6 +29,16 @@ A schedule entry may keep several things at once (a mixer made of two: keys
 and values for one, a state for the other): its spec is then a tuple of specs
 and its entry a ``CacheEntries`` with one ``CacheEntry`` per spec, in order.
 
+A cache in 8 bits (``Cache(int8=True)``) keeps int8 keys and values and a float32
+scale for every page and kv head of each (``kernels/kv8.py`` has the numbers'
+meaning); its page tables and free pages live on the device, where
+``kernels.blocks_extend`` hands pages out in the same steps as ``reserve`` counts
+them here, so the host knows how many pages every slot holds but not which.  A
+ring of such a group has room for the page that is being filled, whose old
+numbers go when its first place is written: ``window + max_piece + page_size - 2``
+places and the rest of the last page, ``max_piece`` being the most tokens that a
+step adds to a sequence that holds some already.
+
 Storage of a key/value group is ``[layer][page][kv_head][page_size][head_dim]``
 for keys and the same for values; all layers of a group share the page ids, so
 one page table per group serves all of them.  Pages and slots go back to their
@@ -84,6 +94,14 @@ def kept_span(spec: KVSpec) -> Optional[int]:
     return min(spans) if spans else None
 
 
+def ring_places(spec: KVSpec, page_size: int, int8: bool = False, max_piece: int = 1) -> Optional[int]:
+    """How many places the ring of a group has (None: it keeps all keys)."""
+    span = kept_span(spec)
+    if not span:
+        return None
+    return _round_up(span + max_piece + page_size - 2, page_size) if int8 else _round_up(span, page_size)
+
+
 def shared_spec(own: KVSpec, readers: Sequence[KVSpec]) -> KVSpec:
     """What an entry has to keep so that its own mask and those of the entries that read its keys and values find
     all they see: the widest span of the newest keys (all keys if one of them sees all), the most kept first keys."""
@@ -101,15 +119,25 @@ def shared_spec(own: KVSpec, readers: Sequence[KVSpec]) -> KVSpec:
 
 
 class KVGroup:
-    def __init__(self, spec: KVSpec, entries: list[int], num_pages: int, page_size: int, dtype, device):
+    def __init__(self, spec: KVSpec, entries: list[int], num_pages: int, page_size: int, dtype, device, int8: bool = False,
+                 max_piece: int = 1, num_slots: int = 0, max_positions: int = 0):
         self.spec = spec
         self.entries = entries
         self.page_size = page_size
-        self.ring = _round_up(kept_span(spec), page_size) if kept_span(spec) else None
+        self.int8 = int8
+        self.ring = ring_places(spec, page_size, int8, max_piece)
         # places ahead of the ring that are held for good (the first keys a window keeps)
         self.head = _round_up(spec.keep_first, page_size) if (self.ring and spec.keep_first) else 0
         self.pool = PagePool(num_pages)
         shape = (len(entries), num_pages, spec.n_kv, page_size, spec.head_dim)
+        self.tables = None
+        if int8:
+            if not spec.values or spec.v_dim not in (None, spec.head_dim) or spec.chunk or spec.keep_first:
+                raise CacheError(f"a cache in 8 bits keeps keys and values of one size under a window or none, not {spec!r}")
+            self.tables = DeviceTables(num_pages, num_slots, self.pages_for(max_positions), device)
+            self.k_scale = torch.zeros(shape[:3], dtype=torch.float32, device=device)
+            self.v_scale = torch.zeros(shape[:3], dtype=torch.float32, device=device)
+            dtype = torch.int8
         self.k = torch.zeros(shape, dtype=dtype, device=device)
         if not spec.values:
             self.v = self.k
@@ -138,6 +166,20 @@ class KVGroup:
         return pos if pos < self.head else self.head + (pos - self.head) % self.ring
 
 
+class DeviceTables:
+    """The page tables of a group on the device: a row of page ids and a count per slot, a stack of free pages."""
+
+    def __init__(self, num_pages: int, num_slots: int, width: int, device):
+        new = lambda *shape: torch.zeros(shape, dtype=torch.int32, device=device)
+        self.tables, self.held = new(num_slots, max(1, width)), new(num_slots)
+        self.free = torch.arange(num_pages - 1, -1, -1, dtype=torch.int32, device=device)
+        self.free_count = torch.full((1,), num_pages, dtype=torch.int32, device=device)
+        self.status = new(1)
+
+    def state(self) -> tuple:
+        return self.tables, self.held, self.free, self.free_count
+
+
 class StateGroup:
     def __init__(self, spec: StateSpec, entries: list[int], num_slots: int, dtype, device):
         self.spec = spec
@@ -164,6 +206,11 @@ class CacheEntry:
         return self.group.v[self.index]
 
     @property
+    def scales(self) -> tuple:
+        """The scales of a group in 8 bits: (keys', values'), [pages, kv heads] each."""
+        return self.group.k_scale[self.index], self.group.v_scale[self.index]
+
+    @property
     def state(self) -> torch.Tensor:
         return self.group.data[self.index]
 
@@ -184,7 +231,7 @@ class Cache:
 
     def __init__(self, specs: Sequence[Optional[CacheSpec]], max_tokens: int, dtype: torch.dtype,
                  device: Union[str, torch.device], page_size: int = PAGE_SIZE, max_slots: Optional[int] = None,
-                 keep_last_token: bool = False):
+                 keep_last_token: bool = False, int8: bool = False, max_piece: int = 1, max_positions: Optional[int] = None):
         if max_tokens <= 0:
             raise CacheError("max_tokens must be positive")
         if page_size <= 0 or page_size % 32 != 0:
@@ -195,7 +242,11 @@ class Cache:
         self.max_slots = max_slots if max_slots is not None else min(self.num_pages, 1024)
         if self.max_slots <= 0:
             raise CacheError("max_slots must be positive")
+        if max_piece < 1:
+            raise CacheError("max_piece must be at least 1")
         self.dtype, self.device = dtype, torch.device(device)
+        self.int8, self.max_piece = bool(int8), int(max_piece)
+        self.max_positions = min(max_positions or self.max_tokens, self.max_tokens)
         self.slots = SlotTable(self.max_slots)
         self.padding_slot = self.max_slots        # the slot number of padding rows: a spare row of every state group
         self.lengths = [0] * self.max_slots
@@ -221,9 +272,10 @@ class Cache:
             if isinstance(spec, KVSpec):
                 pages = self.num_pages
                 if kept_span(spec):
-                    ring_pages = (_round_up(kept_span(spec), page_size) + _round_up(spec.keep_first, page_size)) // page_size
+                    ring_pages = (ring_places(spec, page_size, self.int8, self.max_piece) + _round_up(spec.keep_first, page_size)) // page_size
                     pages = min(pages, self.max_slots * ring_pages)
-                g = KVGroup(spec, [i for i, _ in idxs], pages, page_size, dtype, self.device)
+                g = KVGroup(spec, [i for i, _ in idxs], pages, page_size, dtype, self.device, self.int8, self.max_piece,
+                            self.max_slots, self.max_positions)
                 gid = len(self.kv_groups)
                 self.kv_groups.append(g)
             elif isinstance(spec, StateSpec):
@@ -363,6 +415,7 @@ class Cache:
         n = 0
         for g in self.kv_groups:
             n += g.k.numel() * g.k.element_size() + (g.v.numel() * g.v.element_size() if g.spec.values else 0)
+            n += 8 * g.k_scale.numel() if g.int8 else 0
         for g in self.state_groups:
             n += g.data.numel() * g.data.element_size()
         return n

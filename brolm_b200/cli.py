@@ -45,6 +45,7 @@ def main(argv=None) -> int:
     ap.add_argument("--no-eos", action="store_true", help="do not stop at EOS")
     ap.add_argument("--stop-id", type=int, action="append", default=[], help="further stop token (may be repeated)")
     ap.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
+    ap.add_argument("--cache-dtype", choices=["int8"], help="keep keys and values in 8 bits (default: in --dtype)")
     ap.add_argument("--batch", type=int, default=0, help="most requests run together (default: as the cache allows)")
     ap.add_argument("--device", default="cuda:0")
     args = ap.parse_args(argv)
@@ -97,7 +98,7 @@ def main(argv=None) -> int:
             prompts = [[bos] + p for p in prompts]
         batch = args.batch or len(prompts)
         need = sum(sorted(((len(p) + args.max_new + 63) // 64 * 64 for p in prompts), reverse=True)[:batch])
-        engine = bb.Engine(model, max_tokens=max(need, 64), max_slots=batch)
+        engine = bb.Engine(model, max_tokens=max(need, 64), max_slots=batch, cache_dtype=args.cache_dtype)
         opts = bb.GenerateOptions(
             max_new_tokens=args.max_new,
             sampling=bb.SamplingParams(temperature=args.temp, top_k=args.top_k, top_p=args.top_p, seed=args.seed),

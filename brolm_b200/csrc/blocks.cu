@@ -248,6 +248,8 @@ __global__ void __launch_bounds__(THREADS) blocks_release_kernel(ReleaseArgs a) 
         if (slot_s[k] >= 0) a.held[slot_s[k]] = 0;
 }
 
+__global__ void settle_kernel() {}
+
 // One cluster of 1, 2, 4 or 8 blocks of threads: as many as give a thread a token, or an entry, of its own.
 template <typename Args>
 int launch_cluster(void (*kernel)(Args), const Args& a, long long work, size_t smem, OncePerDevice& raised, cudaStream_t stream) {
@@ -279,7 +281,7 @@ struct ExtendCall {
     const void* stack;
     void *count, *cu_q, *kv_len, *positions, *tok_seq, *cache_rows, *status;
     cudaStream_t stream;
-    int rows, n_slots, width, stack_size, block, ring, tokens;
+    int rows, n_slots, width, stack_size, block, ring, tokens, settle;
 };
 struct ReleaseCall {
     const void *slots, *tables;
@@ -299,7 +301,12 @@ BROLM_API int brolm_blocks_extend(const ExtendCall* c) {
                  c->width, c->stack_size, c->block, c->ring, c->tokens};
     static OncePerDevice raised;
     const size_t smem = (size_t)(5 * c->rows + 2 + (c->n_slots + 31) / 32) * 4;
-    return launch_cluster(blocks_extend_kernel, a, c->tokens, smem, raised, c->stream);
+    const int st = launch_cluster(blocks_extend_kernel, a, c->tokens, smem, raised, c->stream);
+    if (st || !c->settle) return st;
+    // A launch in plain stream order begins when this one has ended and its results are in memory: whatever is launched
+    // behind it may read them before it waits for its predecessor, as many kernels read a step's description.
+    settle_kernel<<<1, 32, 0, c->stream>>>();
+    return launch_status();
 }
 
 BROLM_API int brolm_blocks_release(const ReleaseCall* c) {

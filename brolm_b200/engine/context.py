@@ -20,7 +20,7 @@ class StepContext:
     every state group that belongs to no sequence; no kernel reads or writes
     keys and values for them.
     """
-    mode: str                      # "prefill" | "decode"
+    mode: str                      # "prefill" | "decode" | "piece" (cache in 8 bits: several tokens on sequences that hold some)
     dtype: torch.dtype             # element type of activations and of the cache
     device: torch.device
     cache: Cache
@@ -52,6 +52,12 @@ class StepContext:
         """(k_pages, v_pages, page_table, ring, page_size) of a key/value entry."""
         g: KVGroup = entry.group
         return entry.k, entry.v, self.page_tables[entry.group_id], g.ring_tokens, g.page_size
+
+    def kv8(self, entry: CacheEntry):
+        """((k_pages, v_pages, k_scale, v_scale), tables, ring or 0) of an entry of a cache in 8 bits; the tables have a row
+        per slot, and ``slots_dev`` says which is a sequence's."""
+        g: KVGroup = entry.group
+        return (entry.k, entry.v, *entry.scales), g.tables.tables, g.ring or 0
 
     def ring_from(self, entry: CacheEntry) -> int:
         """How many places ahead of the ring a key/value entry holds for good (0: none)."""

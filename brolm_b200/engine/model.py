@@ -153,13 +153,28 @@ class DecoderModel:
             specs.append(shared_spec(own, readers) if readers else own)
         return specs
 
-    def new_cache(self, max_tokens: int, max_slots: Optional[int] = None, max_seq_len: Optional[int] = None) -> Cache:
+    def new_cache(self, max_tokens: int, max_slots: Optional[int] = None, max_seq_len: Optional[int] = None,
+                  cache_dtype=None, max_piece: int = 1) -> Cache:
+        """``cache_dtype``: None (keys and values in the model's element type) or "int8" (8 bits, with a scale for every
+        page and kv head); then a step may bring up to ``max_piece`` tokens to sequences that hold some already."""
+        if cache_dtype not in (None, "int8", torch.int8):
+            raise ValueError(f"unknown cache_dtype {cache_dtype!r} (None or 'int8')")
+        int8 = cache_dtype is not None
+        if int8:
+            for call in self.layout.schedule:
+                for part in self.blocks[call.block].parts().values():
+                    if part is not None and part.cache_spec() is not None and not part.int8_cache:
+                        raise ValueError(f"cache_dtype='int8' is built for models whose mixers are all plain attention; this one "
+                                         f"has a {type(part).__name__} that keeps {part.cache_spec()!r}")
+            if self.layout.embedding.pairs is not None or all(s is None for s in self.cache_specs()):
+                raise ValueError("cache_dtype='int8' is built for models whose mixers are all plain attention")
+        elif max_piece != 1:
+            raise ValueError("max_piece goes with cache_dtype='int8'")
         cache = Cache(self.cache_specs(), max_tokens, self.dtype, self.device, max_slots=max_slots,
-                      keep_last_token=self.layout.embedding.pairs is not None)
-        positions = min(max_seq_len or cache.max_tokens, cache.max_tokens)
+                      keep_last_token=self.layout.embedding.pairs is not None, int8=int8, max_piece=max_piece,
+                      max_positions=max_seq_len)
         for part, _ in self._tensor_names:
-            part.prepare(positions, self.device)
-        cache.max_positions = positions
+            part.prepare(cache.max_positions, self.device)
         return cache
 
     # the pass -------------------------------------------------------------

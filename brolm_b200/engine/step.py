@@ -5,6 +5,12 @@ of unequal lengths, run packed back to back) or extends each of them by one
 token.  It runs only the tokens it is given, reads what earlier steps left in
 the cache, and returns float32 logits at the wanted places.
 
+With a cache in 8 bits (``Engine(..., cache_dtype="int8")``) the host sends
+lengths alone: page tables, positions and the new tokens' places are made on
+the device (``kernels.blocks_extend``), of a captured step as its first
+launches, and a step may bring several tokens to sequences that hold some
+already (up to ``max_piece``): a long prompt in pieces, or drafted tokens.
+
 Decode steps are replayed from a captured CUDA graph: the step's tokens,
 positions, lengths and page tables live in a device buffer of fixed layout
 that one host-to-device copy refreshes, so the ~300 launches of a step cost
@@ -65,11 +71,26 @@ def _ragged(lengths: Sequence[int]) -> bool:
     return len(lengths) > 1 and max(lengths) * len(lengths) > 1.25 * sum(lengths)
 
 
+def _extend(cache: Cache, slots, lengths, new, cu_q, kv_len, positions, tok_seq, cache_rows, again) -> None:
+    """The page tables and places of a step on the device; the groups agree on all but ``cache_rows``, so the others' go to
+    ``again``, a tensor of as many numbers as cu_q, kv_len, positions and tok_seq have."""
+    B, T = slots.numel(), positions.numel()
+    outs = (cu_q, kv_len, positions, tok_seq)
+    for i, g in enumerate(cache.kv_groups):
+        if i == 1:
+            outs = (again[:B + 1], again[B + 1:2 * B + 1], again[2 * B + 1:2 * B + 1 + T], again[2 * B + 1 + T:2 * B + 1 + 2 * T])
+        t = g.tables
+        kernels.blocks_extend(slots, lengths, new, *t.state(), block=g.page_size, ring=g.ring or 0, cu_q=outs[0], kv_len=outs[1],
+                              positions=outs[2], tok_seq=outs[3], cache_rows=cache_rows[i], status=t.status,
+                              settle=i == len(cache.kv_groups) - 1)
+
+
 class _DecodeGraph:
     """One captured decode step for a padded batch size and a bound on the lengths."""
 
     def __init__(self, engine: "Engine", rows: int, kv_cap: int, ragged: bool = False):
         cache, dev = engine.cache, engine.device
+        self.before = lambda: None             # what the step launches ahead of the model
         self.rows, self.kv_cap = rows, kv_cap
         self.widths = []
         for g in cache.kv_groups:
@@ -77,6 +98,10 @@ class _DecodeGraph:
             if g.ring:
                 w = min(w, (g.head + g.ring) // g.page_size)
             self.widths.append(max(1, w))
+        if cache.int8:
+            self._init_int8(engine, rows, kv_cap, ragged)
+            self._capture(engine)
+            return
         n = 4 * rows + sum(rows * w for w in self.widths) + rows * len(self.widths)
         self.pick_off = n                    # last: which element of a tensor of drawn ids each row's token is
         n += rows
@@ -106,10 +131,43 @@ class _DecodeGraph:
         self.hv[rows:2 * rows] = -1
         self.hv[3 * rows:4 * rows] = cache.padding_slot
         self.hv[self.rows_off:self.pick_off] = -1
+        self._capture(engine)
+
+    def _init_int8(self, engine: "Engine", rows: int, kv_cap: int, ragged: bool) -> None:
+        """The buffers of a step whose tables live on the device: tokens, lengths before it, new tokens, the slots as the
+        parts see them (padding: the spare row) and as the tables do (-1), and the places of drawn ids."""
+        cache, dev = engine.cache, engine.device
+        self.pick_off = 5 * rows
+        self.host = torch.zeros(6 * rows, dtype=torch.int32, pin_memory=True)
+        self.hv = self.host.numpy()
+        self.dev = torch.zeros(6 * rows, dtype=torch.int32, device=dev)
+        seg = [self.dev[i * rows:(i + 1) * rows] for i in range(6)]
+        self.tokens, self.pick = seg[0], seg[5]
+        G = len(cache.kv_groups)
+        made = torch.zeros((3 + G) * rows + rows + 1, dtype=torch.int32, device=dev)
+        part = [made[i * rows:(i + 1) * rows] for i in range(3 + G)]
+        cu_q = made[(3 + G) * rows:]
+        again = torch.zeros(4 * rows + 1, dtype=torch.int32, device=dev)
+        cache_rows = part[3:]
+        self.before = lambda: _extend(cache, seg[4], seg[1], seg[2], cu_q, part[0], part[1], part[2], cache_rows, again)
+        self.ctx = StepContext(
+            mode="decode", dtype=engine.model.dtype, device=dev, cache=cache, batch=rows, n_tokens=rows, slots=[],
+            positions=part[1], tok_seq=part[2], cu_q=cu_q, kv_len=part[0], slots_dev=seg[3], max_q_len=1,
+            page_tables=[g.tables.tables for g in cache.kv_groups], cache_rows=cache_rows, host_lengths=[], max_kv_len=kv_cap,
+            ragged=ragged, beside=engine.beside)
+        self.all_rows = torch.arange(rows, dtype=torch.int32, device=dev)
+        self.hv[2 * rows:3 * rows] = 1
+        self.hv[3 * rows:4 * rows] = cache.padding_slot
+        self.hv[4 * rows:5 * rows] = -1
+
+    def _capture(self, engine: "Engine") -> None:
+        """A warm-up pass over padding alone, then the capture."""
+        dev = engine.device
         self.dev.copy_(self.host)
         side = torch.cuda.Stream(device=dev)
         side.wait_stream(torch.cuda.current_stream(dev))
         with torch.cuda.stream(side):
+            self.before()
             engine.model.forward(self.ctx, self.tokens, self.all_rows)
         torch.cuda.current_stream(dev).wait_stream(side)
         torch.cuda.synchronize(dev)
@@ -125,6 +183,7 @@ class _DecodeGraph:
         gc.disable()
         try:
             with torch.cuda.graph(self.graph, pool=engine._graph_pool):
+                self.before()
                 self.logits = engine.model.forward(self.ctx, self.tokens, self.all_rows)
                 self.hidden = engine.model.last_hidden
         finally:
@@ -146,6 +205,13 @@ class _DecodeGraph:
         hv[R:R + B] = plan.old
         hv[2 * R:2 * R + B] = plan.new_len
         hv[3 * R:3 * R + B] = plan.slots
+        if cache.int8:
+            hv[2 * R:3 * R] = 1
+            hv[R:2 * R] = 0
+            hv[R:R + B] = plan.old
+            hv[4 * R:5 * R] = -1
+            hv[4 * R:4 * R + B] = plan.slots
+            return self._replay(B, ids, pick)
         off = 4 * R
         for g, w in enumerate(self.widths):
             # the page tables change only when a sequence begins a page or the batch changes
@@ -164,8 +230,6 @@ class _DecodeGraph:
         hv[off:self.pick_off] = -1
         for g in range(len(self.widths)):
             hv[off + g * R:off + g * R + B] = cache.decode_rows(g, plan.slots, plan.old)
-        if ids is not None:
-            hv[self.pick_off:self.pick_off + B] = pick
         if debug.ENABLED:
             tables, o = [], 4 * R
             for w in self.widths:
@@ -174,6 +238,11 @@ class _DecodeGraph:
             _checked(cache, "decode", 1 << 62, None if ids is not None else hv[0:B], list(hv[3 * R:4 * R]), hv[R:2 * R],
                      np.arange(R), hv[2 * R:3 * R], tables, [hv[off + g * R:off + (g + 1) * R] for g in range(len(self.widths))],
                      None)
+        return self._replay(B, ids, pick)
+
+    def _replay(self, B: int, ids: Optional[torch.Tensor], pick: Optional[Sequence[int]]) -> torch.Tensor:
+        if ids is not None:
+            self.hv[self.pick_off:self.pick_off + B] = pick
         self.dev.copy_(self.host, non_blocking=True)
         self.copied.record()
         if ids is not None:
@@ -187,9 +256,12 @@ class Engine:
     """A model with a cache: slots, steps, and nothing else."""
 
     def __init__(self, model: DecoderModel, max_tokens: int, max_slots: Optional[int] = None,
-                 max_seq_len: Optional[int] = None, use_graphs: bool = True):
+                 max_seq_len: Optional[int] = None, use_graphs: bool = True, cache_dtype=None, max_piece: int = 1):
+        """``cache_dtype="int8"``: keys and values in 8 bits with a scale for every page and kv head, half the bytes of
+        bfloat16 (models whose mixers are all plain attention); ``max_piece``: the most tokens that a step of such an engine
+        brings to sequences that hold some already."""
         self.model = model
-        self.cache: Cache = model.new_cache(max_tokens, max_slots, max_seq_len)
+        self.cache: Cache = model.new_cache(max_tokens, max_slots, max_seq_len, cache_dtype, max_piece)
         self.device = model.device
         self.vocab = model.layout.embedding.vocab
         parts = [p for blk in model.blocks for p in blk.parts().values() if p is not None] + [model.final_norm]
@@ -219,8 +291,19 @@ class Engine:
         return [self.cache.alloc_slot() for _ in range(n)]
 
     def close(self, slots: Sequence[int]) -> None:
-        for s in slots:
-            self.cache.free_slot(s)
+        freed = []
+        try:
+            for s in slots:
+                self.cache.free_slot(s)
+                freed.append(s)
+        finally:
+            if self.cache.int8 and freed:
+                # their pages go back on the device, behind the steps that used them
+                self._follow()
+                gone = torch.tensor(freed, dtype=torch.int32).to(self.device)
+                for g in self.cache.kv_groups:
+                    kernels.blocks_release(gone, *g.tables.state(), status=g.tables.status)
+                self._mark_end()
         # decode steps are queued without a look at the kernels' status words (that would cost a
         # synchronisation per step); the end of a batch is where a wait that ran out is reported
         self._check_waits("close", "the tokens decoded for these sequences are not valid")
@@ -241,6 +324,11 @@ class Engine:
                       "grouped_tc": kernels.grouped_tc_status(reset=True),
                       "attn_kv8_tc": kernels.attention_kv8_tc_status(reset=True)}
         self._checked_at = launched
+        for g in self.cache.kv_groups if self.cache.int8 else ():
+            status = int(g.tables.status)
+            if status:
+                raise StepError(f"{where}: the page tables on the device refused a step "
+                                f"({kernels.BLOCKS_STATUS.get(status, status)}); {consequence}")
         bad = {k: v for k, v in codes.items() if v}
         if bad:
             raise StepError(f"{where}: a wait inside a tensor-core kernel ran out ({bad}), in this step or in a "
@@ -255,6 +343,15 @@ class Engine:
         if not self._on_default:
             self._done = self._done or torch.cuda.Event()
             self._done.record(stream)
+
+    def _follow(self) -> None:
+        """Make the current stream wait for the last step, if that ran on another: tables that live on the device are the
+        engine's, not a stream's."""
+        cur = torch.cuda.current_stream(self.device)
+        if self._on_default and cur.cuda_stream != 0:
+            cur.wait_stream(torch.cuda.default_stream(self.device))
+        elif not self._on_default and self._done is not None:
+            cur.wait_event(self._done)
 
     # the step -------------------------------------------------------------
     def step(self, slots: Sequence[int], tokens: Sequence[Sequence[int]],
@@ -271,6 +368,8 @@ class Engine:
         (wlejon/brolm's ``hidden_out``, include/brolm/gemma2.h:121-125).
         """
         plan = self._plan(slots, tokens, want)
+        if self.cache.int8:
+            self._follow()
         if plan.mode == "decode" and self.use_graphs:
             graph = self._graph_for(plan)
             logits = graph.run(plan, self.cache)
@@ -286,7 +385,7 @@ class Engine:
             logits = self.model.forward(ctx, tok_dev, rows)
             rows_h = self.model.last_hidden
         self._mark_end()
-        if plan.mode == "prefill":
+        if plan.mode != "decode":
             self._check_waits("step", "the results of this step are not valid")
         self.cache.commit(dict(zip(plan.slots, plan.new_len)))
         return (logits, rows_h) if hidden else logits
@@ -303,6 +402,8 @@ class Engine:
         plan = self._plan(slots, [[0]] * len(slots), None)
         if plan.mode != "decode":
             raise StepError("step_from: only sequences that already hold tokens can go on")
+        if self.cache.int8:
+            self._follow()
         if self.use_graphs:
             graph = self._graph_for(plan)
             logits = graph.run(plan, self.cache, ids, [int(p) for p in pick])[:len(plan.slots)]
@@ -346,6 +447,11 @@ class Engine:
             mode = "prefill"
         elif all(n == 1 for n in n_new) and all(o > 0 for o in old):
             mode = "decode"
+        elif cache.int8 and max(n_new) <= cache.max_piece:
+            mode = "piece"
+        elif cache.int8 and cache.max_piece > 1:
+            raise StepError(f"step: sequences that hold tokens already go on by up to {cache.max_piece} (the engine's max_piece), "
+                            f"and so do all of a step that are beside one")
         else:
             raise StepError("step: the sequences of a step must either all start at their first token "
                             "or all go on by one token")
@@ -376,6 +482,8 @@ class Engine:
     def _context(self, plan: _Plan):
         cache, B = self.cache, len(plan.slots)
         T = int(sum(plan.n_new))
+        if cache.int8:
+            return self._context_int8(plan, B, T)
         cu = np.zeros(B + 1, dtype=np.int64)
         np.cumsum(plan.n_new, out=cu[1:])
         positions = np.concatenate([np.arange(o, o + n) for o, n in zip(plan.old, plan.n_new)])
@@ -389,6 +497,40 @@ class Engine:
         if debug.ENABLED:
             _checked(cache, plan.mode, self.vocab, plan.flat, plan.slots, positions, tok_seq, np.asarray(plan.new_len),
                      tables, parts[7 + len(tables):], np.asarray(plan.rows, dtype=np.int64))
+        seg = self._send(parts)
+        page_tables = [seg[7 + g].view(B, tables[g].shape[1]) for g in range(len(tables))]
+        cache_rows = [seg[7 + len(tables) + g] for g in range(len(tables))]
+        ctx = StepContext(mode=plan.mode, dtype=self.model.dtype, device=self.device, cache=cache, batch=B,
+                          n_tokens=T, slots=plan.slots, positions=seg[1], tok_seq=seg[2], cu_q=seg[3],
+                          kv_len=seg[4], slots_dev=seg[5], max_q_len=int(max(plan.n_new)), page_tables=page_tables,
+                          cache_rows=cache_rows, host_lengths=plan.new_len,
+                          ragged=plan.mode == "decode" and _ragged(plan.new_len))
+        return ctx, seg[0], seg[6]
+
+    def _context_int8(self, plan: _Plan, B: int, T: int):
+        """The same for a cache in 8 bits: lengths go over, the device makes the rest."""
+        cache, G = self.cache, len(self.cache.kv_groups)
+        tokens, rows, slots, old, new = self._send([plan.flat, np.asarray(plan.rows, dtype=np.int64), np.asarray(plan.slots),
+                                                    np.asarray(plan.old), np.asarray(plan.n_new)])
+        made = torch.empty(4 * B + 2 + (4 + G) * T, dtype=torch.int32, device=self.device)
+        cut = lambda at, n: made[at:at + n]
+        cu_q, kv_len = cut(0, B + 1), cut(B + 1, B)
+        positions, tok_seq = cut(2 * B + 1, T), cut(2 * B + 1 + T, T)
+        cache_rows = [cut(2 * B + 1 + (2 + g) * T, T) for g in range(G)]
+        _extend(cache, slots, old, new, cu_q, kv_len, positions, tok_seq, cache_rows, made[2 * B + 1 + (2 + G) * T:])
+        if debug.ENABLED:
+            for g in cache.kv_groups:
+                if int(g.tables.status):
+                    raise StepError(f"debug: {kernels.BLOCKS_STATUS.get(int(g.tables.status))}")
+        ctx = StepContext(mode=plan.mode, dtype=self.model.dtype, device=self.device, cache=cache, batch=B, n_tokens=T,
+                          slots=plan.slots, positions=positions, tok_seq=tok_seq, cu_q=cu_q, kv_len=kv_len, slots_dev=slots,
+                          max_q_len=int(max(plan.n_new)), page_tables=[g.tables.tables for g in cache.kv_groups],
+                          cache_rows=cache_rows, host_lengths=plan.new_len,
+                          ragged=plan.mode == "decode" and _ragged(plan.new_len))
+        return ctx, tokens, rows
+
+    def _send(self, parts: list) -> list:
+        """Arrays of a step to the device, as int32, through one buffer and one copy."""
         sizes = [p.size for p in parts]
         offs = np.concatenate([[0], np.cumsum([(s + 3) // 4 * 4 for s in sizes])])
         n = int(offs[-1])
@@ -411,12 +553,4 @@ class Engine:
         if self.device.type == "cuda":
             self._pin_copied.record()
         self.last_h2d_bytes = host.numel() * 4
-        seg = [dev[int(o):int(o) + s] for o, s in zip(offs[:-1], sizes)]
-        page_tables = [seg[7 + g].view(B, tables[g].shape[1]) for g in range(len(tables))]
-        cache_rows = [seg[7 + len(tables) + g] for g in range(len(tables))]
-        ctx = StepContext(mode=plan.mode, dtype=self.model.dtype, device=self.device, cache=cache, batch=B,
-                          n_tokens=T, slots=plan.slots, positions=seg[1], tok_seq=seg[2], cu_q=seg[3],
-                          kv_len=seg[4], slots_dev=seg[5], max_q_len=int(max(plan.n_new)), page_tables=page_tables,
-                          cache_rows=cache_rows, host_lengths=plan.new_len,
-                          ragged=plan.mode == "decode" and _ragged(plan.new_len))
-        return ctx, seg[0], seg[6]
+        return [dev[int(o):int(o) + s] for o, s in zip(offs[:-1], sizes)]

@@ -36,7 +36,7 @@ _CODES = {torch.float32: 0, torch.bfloat16: 1}
 # one struct, packed here as C lays it out (converting a pointer and 35 numbers one by one costs ctypes 3.4 us a call,
 # packing them 0.4 and passing the one pointer 0.3), and the checks of the arguments are one expression each; which of
 # them failed is found out only then.
-_EXTEND = struct.Struct("@14P7i")
+_EXTEND = struct.Struct("@14P8i")
 _RELEASE = struct.Struct("@7P4i")
 _WRITE = struct.Struct("@10P4q8i")
 _READ = struct.Struct("@11P4q10i")
@@ -71,7 +71,7 @@ def _odd_ints(t: torch.Tensor, n: int) -> bool:
 def blocks_extend(slots: torch.Tensor, lengths: torch.Tensor, new: torch.Tensor, tables: torch.Tensor, held: torch.Tensor,
                   free: torch.Tensor, free_count: torch.Tensor, *, block: int, cu_q: torch.Tensor, kv_len: torch.Tensor,
                   positions: torch.Tensor, tok_seq: torch.Tensor, cache_rows: torch.Tensor, status: torch.Tensor,
-                  ring: int = 0) -> None:
+                  ring: int = 0, settle: bool = False) -> None:
     """A step's block tables and slot map, on the device.  All tensors are int32.
 
     Row i of the step goes on with slot ``slots[i]`` (-1: padding), which holds ``lengths[i]`` tokens, by ``new[i]``.  The
@@ -79,6 +79,10 @@ def blocks_extend(slots: torch.Tensor, lengths: torch.Tensor, new: torch.Tensor,
     and are entered behind those that ``tables[slot]`` holds.  Written: ``cu_q`` [rows + 1] (sums of ``new``), ``kv_len``
     [rows] (0 for padding), and for every token, rows back to back, ``positions``, ``tok_seq`` (its row) and ``cache_rows``
     (block * block size + place, -1 where the ring does not keep the token); places beyond the last token get -1, 0, -1.
+
+    ``settle``: kernels launched behind this call may read what it writes (all but the tables and ``cache_rows``, which are
+    read after the wait) before they wait for the launch before them; the kernels of this package that read a step's
+    positions, sums and lengths do so, since the host used to write them.  It costs an empty launch.
 
     A step that does not fit changes neither ``tables``, ``held`` nor the stack: its outputs read as padding and ``status``
     holds a key of ``BLOCKS_STATUS``.  The same step again takes no more blocks.  Up to 4,096 rows and 65,536 slots."""
@@ -97,7 +101,7 @@ def blocks_extend(slots: torch.Tensor, lengths: torch.Tensor, new: torch.Tensor,
     _call("blocks", "brolm_blocks_extend", _EXTEND.pack(
         slots.data_ptr(), lengths.data_ptr(), new.data_ptr(), tables.data_ptr(), held.data_ptr(), free.data_ptr(),
         free_count.data_ptr(), cu_q.data_ptr(), kv_len.data_ptr(), positions.data_ptr(), tok_seq.data_ptr(),
-        cache_rows.data_ptr(), status.data_ptr(), _stream(), n, S, W, N, block, ring, T), what)
+        cache_rows.data_ptr(), status.data_ptr(), _stream(), n, S, W, N, block, ring, T, 1 if settle else 0), what)
 
 
 def blocks_release(slots: torch.Tensor, tables: torch.Tensor, held: torch.Tensor, free: torch.Tensor, free_count: torch.Tensor, *,

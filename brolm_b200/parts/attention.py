@@ -168,6 +168,8 @@ class Attention(Part):
         self.rowwise = (self.v_dim != head_dim or qk_norm != "none" or self.chunk is not None) and not self.headwise
         if self.headwise and (self.v_dim > 512 or n_q > 128):
             raise ValueError("attention: v_dim beyond 512 or more than 128 heads are beyond the head-wise kernels")
+        # plain attention can keep its keys and values in 8 bits
+        self.int8_cache = not self.headwise and not self.rowwise and head_dim <= 256
         if self.rowwise:
             if self.v_dim > 512:
                 raise ValueError(f"attention: v_dim {self.v_dim} is beyond the kernels' limit of 512")
@@ -278,7 +280,8 @@ class Attention(Part):
             return self._forward_rowwise(x, ctx, entry, writes_cache)
         rot = self.position.rotary_dim if self.position is not None else 0
         cos_sin = self.position.table if self.position is not None else None
-        kept = (k_pages, v_pages, ctx.cache_rows[entry.group_id]) if writes_cache else (None, None, None)
+        int8 = entry.group.int8
+        kept = (k_pages, v_pages, ctx.cache_rows[entry.group_id]) if writes_cache and not int8 else (None, None, None)
         if kernels.skinny_ok(x, self.w_qkv) and (cos_sin is None or rot == self.head_dim):
             # a few tokens: the rotation and the write into the cache are the product's epilogue
             qkv = torch.empty((x.shape[0], self.q_dim + 2 * self.kv_dim), dtype=ctx.dtype, device=x.device)
@@ -300,14 +303,22 @@ class Attention(Part):
         out = torch.empty((qkv.shape[0], self.q_dim), dtype=ctx.dtype, device=x.device)
         common = dict(n_kv=self.n_kv, group=self.n_q // self.n_kv, head_dim=self.head_dim, scale=self.scale,
                       cap=self.softcap, window=self.window or 0, batch=ctx.batch, max_q_len=ctx.max_q_len)
+        if int8 and writes_cache:
+            heads = qkv[:, self.q_dim:].unflatten(1, (2 * self.n_kv, self.head_dim))
+            kernels.kv8_write(heads[:, :self.n_kv], heads[:, self.n_kv:], ctx.cu_q, ctx.positions, ctx.cache_rows[entry.group_id],
+                              *ctx.kv8(entry)[0], max_q_len=ctx.max_q_len)
         if ctx.mode == "prefill" and writes_cache:
             # the step's own keys and values, still packed: a prompt longer than
             # the window needs keys the ring no longer holds
             k = qkv[:, self.q_dim:self.q_dim + self.kv_dim]
             v = qkv[:, self.q_dim + self.kv_dim:]
             self.attend_packed(q, k, v, out, ctx, common)
+        elif int8 and (ctx.mode != "prefill" or not self.window):
+            cache, tables, ring = ctx.kv8(entry)
+            kernels.attention_kv8(q, out, ctx.cu_q, ctx.kv_len, ctx.slots_dev, tables, *cache, ring=ring,
+                                  max_kv_len=ctx.max_kv_len, **common)
         else:
-            if ctx.mode == "prefill" and self.window and ctx.max_kv_len > ring:
+            if ctx.mode == "prefill" and self.window and (int8 or ctx.max_kv_len > ring):
                 raise NotImplementedError("a layer that reads another layer's windowed cache cannot take a "
                                           "prompt longer than the ring in one step")
             self.attend_paged(q, out, ctx, common, k_pages, v_pages, table, ring, page)

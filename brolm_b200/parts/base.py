@@ -40,6 +40,9 @@ class Part:
     # True when its kernels may run at the same time as another part's: none of them keeps tickets, counters or scratch
     # of its own on the device that another kernel of the step uses, too.
     runs_beside: bool = False
+    # True when it can keep its keys and values in 8 bits (mixers): it then finds a cache entry of that kind, and steps may
+    # bring several tokens to a sequence that holds some already.
+    int8_cache: bool = False
     # True when it forks a branch of a captured step onto the context's second stream.
     branches: bool = False
 

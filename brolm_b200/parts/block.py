@@ -87,7 +87,8 @@ class Block(Part):
                 next_norm: Optional[Part]) -> Optional[torch.Tensor]:
         """h: residual stream (updated in place); x = pre_mixer_norm(h).
         Returns next_norm(h) for the block that follows, if there is one."""
-        if ctx.mode == "prefill" and writes_cache and x.dtype == torch.bfloat16 and self._launches_at_once(x, ctx, next_norm):
+        if ctx.mode == "prefill" and writes_cache and x.dtype == torch.bfloat16 and not ctx.cache.int8 and \
+                self._launches_at_once(x, ctx, next_norm):
             return self._forward_at_once(h, x, ctx, entry, next_norm)
         y = self.mixer.forward(x, ctx, entry, writes_cache)
         if self.feedforward is None:
