@@ -954,7 +954,10 @@ int launch(void (*kernel)(AttnArgs), size_t smem, OncePerDevice& raised, const A
     attr[0].val.clusterDim.x = a.shares;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+    // A launch that fills the device begins when the one before it has ended: let in early, its blocks land wherever that one
+    // leaves room, several on one SM and none on another, and stay there (8 sequences of 8,192 keys behind a product of few
+    // tokens: 42 us for 29).  A small one is let in.
+    attr[1].val.programmaticStreamSerializationAllowed = pdl_enabled() && blocks * a.n_kv <= device_sm_count() ? 1 : 0;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
     const int e = (int)cudaLaunchKernelEx(&cfg, kernel, a);

@@ -32,7 +32,7 @@ struct ExtendArgs {
     int32_t *tables, *held, *count;
     const int32_t* stack;
     int32_t *cu_q, *kv_len, *positions, *tok_seq, *cache_rows, *status;
-    int rows, n_slots, width, stack_size, block, ring, tokens;
+    int rows, n_slots, width, stack_size, block, shift, ring, tokens;      // shift: of a block that is a power of two, else -1
 };
 
 __device__ __forceinline__ void cluster_barrier() {
@@ -164,25 +164,46 @@ __global__ void __launch_bounds__(THREADS) blocks_extend_kernel(ExtendArgs a) {
         const int i = last_not_above(block0, a.rows, k);
         a.tables[(size_t)slot_s[i] * a.width + held_s[i] + k - block0[i]] = a.stack[count - 1 - k];
     }
-    for (int t = me; t < a.tokens; t += all) {
-        int pos = -1, seq = 0, row = -1;
-        if (t < n_tok) {
-            seq = last_not_above(token0, a.rows, t);
-            if (before[seq] >= 0) {
-                pos = before[seq] + t - token0[seq];
-                const int last = before[seq] + token0[seq + 1] - token0[seq] - 1;
-                if (a.ring == 0 || pos / a.block + a.ring / a.block > last / a.block) {
-                    const int place = a.ring > 0 ? pos % a.ring : pos;
-                    const int e = place / a.block;
-                    const int id = e < held_s[seq] ? a.tables[(size_t)slot_s[seq] * a.width + e]
-                                                   : a.stack[count - 1 - (block0[seq] + e - held_s[seq])];
-                    row = id * a.block + place - e * a.block;
-                }
+    // the tokens, EACH a thread and 32 EACH a warp at a time: the rows of a warp's first and last token are looked for once,
+    // a token's own among them (mostly there is one)
+    constexpr int EACH = 4;
+    const int lane = threadIdx.x & 31;
+    auto block_of = [&](int place) { return a.shift >= 0 ? place >> a.shift : place / a.block; };
+    for (int base = (me >> 5) * 32 * EACH; base < a.tokens; base += all * EACH) {
+        const int from = n_tok > 0 ? last_not_above(token0, a.rows, min(base, n_tok - 1)) : 0;
+        const int to = n_tok > 0 ? last_not_above(token0, a.rows, min(base + 32 * EACH - 1, n_tok - 1)) : 0;
+        int pos[EACH], seq[EACH], row[EACH];
+        const int32_t* where[EACH];
+#pragma unroll
+        for (int j = 0; j < EACH; ++j) {
+            const int t = base + 32 * j + lane;
+            pos[j] = -1;
+            seq[j] = 0;
+            row[j] = -1;
+            where[j] = nullptr;
+            if (t >= n_tok) continue;
+            const int s = from + (from < to ? last_not_above(token0 + from, to - from + 1, t) : 0);
+            seq[j] = s;
+            if (before[s] < 0) continue;
+            const int p = before[s] + t - token0[s], last = before[s] + token0[s + 1] - token0[s] - 1;
+            pos[j] = p;
+            if (a.ring > 0 && block_of(p) + block_of(a.ring) <= block_of(last)) continue;
+            const int place = a.ring > 0 ? (int)((unsigned)p % (unsigned)a.ring) : p, e = block_of(place);
+            row[j] = place - e * a.block;
+            where[j] = e < held_s[s] ? a.tables + (size_t)slot_s[s] * a.width + e : a.stack + (count - 1 - (block0[s] + e - held_s[s]));
+        }
+#pragma unroll
+        for (int j = 0; j < EACH; ++j)
+            if (where[j]) row[j] += *where[j] * a.block;
+#pragma unroll
+        for (int j = 0; j < EACH; ++j) {
+            const int t = base + 32 * j + lane;
+            if (t < a.tokens) {
+                a.positions[t] = pos[j];
+                a.tok_seq[t] = seq[j];
+                a.cache_rows[t] = row[j];
             }
         }
-        a.positions[t] = pos;
-        a.tok_seq[t] = seq;
-        a.cache_rows[t] = row;
     }
 }
 
@@ -295,10 +316,13 @@ BROLM_API int brolm_blocks_extend(const ExtendCall* c) {
     if (c->ring < 0 || c->ring % c->block) return BROLM_ERR_BAD_SIZE;
     if (c->rows > MAX_ROWS || c->n_slots > MAX_SLOTS) return BROLM_ERR_TOO_LARGE;
     if ((long long)c->stack_size * c->block > 0x7fffffffll) return BROLM_ERR_TOO_LARGE;    // (a cache row is 31 bits)
+    int shift = -1;
+    for (int s = 0; s < 31; ++s)
+        if (c->block == 1 << s) shift = s;
     ExtendArgs a{(const int32_t*)c->slots, (const int32_t*)c->lengths, (const int32_t*)c->fresh, (int32_t*)c->tables,
                  (int32_t*)c->held, (int32_t*)c->count, (const int32_t*)c->stack, (int32_t*)c->cu_q, (int32_t*)c->kv_len,
                  (int32_t*)c->positions, (int32_t*)c->tok_seq, (int32_t*)c->cache_rows, (int32_t*)c->status, c->rows, c->n_slots,
-                 c->width, c->stack_size, c->block, c->ring, c->tokens};
+                 c->width, c->stack_size, c->block, shift, c->ring, c->tokens};
     static OncePerDevice raised;
     const size_t smem = (size_t)(5 * c->rows + 2 + (c->n_slots + 31) / 32) * 4;
     const int st = launch_cluster(blocks_extend_kernel, a, c->tokens, smem, raised, c->stream);

@@ -50,15 +50,18 @@ __global__ void __launch_bounds__(512) kv8_write_kernel(WriteArgs a) {
         i = lo;
         k = blockIdx.x - (a.cu_q[i] / P + 2 * i);
     }
+    // (where every row brings one token, token i is row i's: its position and place are asked for with the sums, not after)
+    const int likely = min(i, a.tokens - 1);
+    const int likely_pos = a.positions[likely], likely_row = a.cache_rows[likely];
     const int first = max(0, a.cu_q[i]), end = min(a.tokens, a.cu_q[i + 1]);
     if (first >= end) return;
-    const int p0 = a.positions[first];
+    const int p0 = first == likely ? likely_pos : a.positions[first];
     if (p0 < 0) return;                                        // padding
     const int in_block = p0 % P;
     const long long t0 = first + (k == 0 ? 0ll : (long long)k * P - in_block);
     if (t0 >= end) return;
     const int n = (int)min((long long)end - t0, (long long)(k == 0 ? P - in_block : P));
-    const int row = a.cache_rows[t0];
+    const int row = t0 == likely ? likely_row : a.cache_rows[t0];
     if (row < 0 || row / P >= a.n_blocks) return;              // the ring keeps none of these
     const int b = row / P, at = row % P, h = blockIdx.y, which = blockIdx.z;
     if (at + n > P) return;                                    // (not a slot map: nothing is written)
