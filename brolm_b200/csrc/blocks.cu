@@ -17,6 +17,9 @@
 // threads of one cluster adds up all rows by itself (three short arrays out of the L2), which costs less than handing sums
 // around, the cluster's barrier then lets the state be written that all have read, and tokens and new table entries are
 // shared out.  A token's block is looked up in the stack where it is new, so nothing waits for the tables' new entries.
+// A cluster is eight SMs, and 32,768 tokens take them 4.3 us; steps of more tokens run on all SMs without a cluster, and a
+// second, small launch writes what the blocks of the first still read (300 rows of 100,559 tokens in all: 17.8 us in one
+// cluster).
 #include "common.cuh"
 
 namespace {
@@ -84,6 +87,8 @@ __device__ __forceinline__ int last_not_above(const int* at, int n, int x) {
     return lo;
 }
 
+// CLUSTER: the launch is one cluster and does everything.  Else `held` and `count` are left to commit_kernel.
+template <bool CLUSTER>
 __global__ void __launch_bounds__(THREADS) blocks_extend_kernel(ExtendArgs a) {
     extern __shared__ int rows_s[];
     int* token0 = rows_s;                       // [rows + 1] tokens ahead of the row
@@ -142,7 +147,8 @@ __global__ void __launch_bounds__(THREADS) blocks_extend_kernel(ExtendArgs a) {
         token0[a.rows] = (int)sums.x;
         block0[a.rows] = (int)sums.y;
     }
-    cluster_barrier();                          // everyone has read the state (and every thread's shared stores are seen)
+    if constexpr (CLUSTER) cluster_barrier();   // everyone has read the state (and every thread's shared stores are seen)
+    else __syncthreads();
     int status = bad;
     if (sums.x > a.tokens) status = max(status, (int)ST_TOO_MANY_TOKENS);
     if (sums.y > count || count > a.stack_size) status = max(status, (int)ST_NO_BLOCKS);
@@ -151,14 +157,14 @@ __global__ void __launch_bounds__(THREADS) blocks_extend_kernel(ExtendArgs a) {
     const int n_new = ok ? (int)sums.y : 0, n_tok = ok ? (int)sums.x : 0;
     if (me == 0) {
         *a.status = status;
-        *a.count = count - n_new;
+        if constexpr (CLUSTER) *a.count = count - n_new;
         a.cu_q[a.rows] = n_tok;
     }
     for (int i = me; i < a.rows; i += all) {
         const bool live = ok && before[i] >= 0;
         a.cu_q[i] = ok ? token0[i] : 0;
         a.kv_len[i] = live ? before[i] + token0[i + 1] - token0[i] : 0;
-        if (live && block0[i + 1] != block0[i]) a.held[slot_s[i]] = held_s[i] + block0[i + 1] - block0[i];
+        if (CLUSTER && live && block0[i + 1] != block0[i]) a.held[slot_s[i]] = held_s[i] + block0[i + 1] - block0[i];
     }
     for (int k = me; k < n_new; k += all) {
         const int i = last_not_above(block0, a.rows, k);
@@ -166,7 +172,7 @@ __global__ void __launch_bounds__(THREADS) blocks_extend_kernel(ExtendArgs a) {
     }
     // the tokens, EACH a thread and 32 EACH a warp at a time: the rows of a warp's first and last token are looked for once,
     // a token's own among them (mostly there is one)
-    constexpr int EACH = 4;
+    constexpr int EACH = CLUSTER ? 4 : 1;
     const int lane = threadIdx.x & 31;
     auto block_of = [&](int place) { return a.shift >= 0 ? place >> a.shift : place / a.block; };
     for (int base = (me >> 5) * 32 * EACH; base < a.tokens; base += all * EACH) {
@@ -205,6 +211,27 @@ __global__ void __launch_bounds__(THREADS) blocks_extend_kernel(ExtendArgs a) {
             }
         }
     }
+}
+
+// What blocks_extend_kernel<false> leaves: the slots' blocks and the stack's height, if the step was taken.
+__global__ void __launch_bounds__(THREADS) commit_kernel(ExtendArgs a) {
+    __shared__ int taken;
+    if (threadIdx.x == 0) taken = 0;
+    __syncthreads();
+    if (*a.status != ST_OK) return;
+    int mine = 0;
+    for (int i = threadIdx.x; i < a.rows; i += THREADS) {
+        const int s = a.slots[i];
+        if (s < 0) continue;
+        const int have = a.held[s], need = blocks_for((long long)a.lengths[i] + a.fresh[i], a.block, a.ring);
+        if (need > have) {
+            a.held[s] = need;
+            mine += need - have;
+        }
+    }
+    if (mine) atomicAdd(&taken, mine);
+    __syncthreads();
+    if (threadIdx.x == 0) *a.count -= taken;
 }
 
 // The blocks of the rows' slots go back to the stack, the last row's last block first: what one extend took, one release
@@ -325,7 +352,17 @@ BROLM_API int brolm_blocks_extend(const ExtendCall* c) {
                  c->width, c->stack_size, c->block, shift, c->ring, c->tokens};
     static OncePerDevice raised;
     const size_t smem = (size_t)(5 * c->rows + 2 + (c->n_slots + 31) / 32) * 4;
-    const int st = launch_cluster(blocks_extend_kernel, a, c->tokens, smem, raised, c->stream);
+    if (c->tokens > 8 * THREADS * 4) {
+        static OncePerDevice raised_wide;
+        int st = allow_shared_memory(blocks_extend_kernel<false>, 200 * 1024, raised_wide);
+        if (st) return st;
+        st = launch_pdl(blocks_extend_kernel<false>, dim3(min(device_sm_count(), (c->tokens + THREADS - 1) / THREADS)), dim3(THREADS), smem,
+                        c->stream, a);
+        if (st) return st;
+        commit_kernel<<<1, THREADS, 0, c->stream>>>(a);      // (in plain stream order: it settles the first one's results, too)
+        return launch_status();
+    }
+    const int st = launch_cluster(blocks_extend_kernel<true>, a, c->tokens, smem, raised, c->stream);
     if (st || !c->settle) return st;
     // A launch in plain stream order begins when this one has ended and its results are in memory: whatever is launched
     // behind it may read them before it waits for its predecessor, as many kernels read a step's description.

@@ -108,6 +108,22 @@ def test_tables_of_many_rows_and_tokens():
     assert t.free == free                          # the stack is as it was
 
 
+def test_tables_of_a_step_that_all_sms_share():
+    """Long prompts and short ones, padding between them, 40,000 tokens and more; once refused, once taken, once again."""
+    new = [15000, 1, 0, 300, 20000, 64, 7000, 33]
+    slots = [4, 0, 9, -1, 2, 7, 1, 5]
+    t = Tables(12, 400, 900, 64, 0, 5)
+    assert t.step(slots, [0] * 8, [700 * 64] + new[1:], 80000) == 2
+    assert t.step(slots, [0] * 8, [390 * 64, 1, 0, 300, 390 * 64] + new[5:], 80000) == 1
+    for _ in range(2):
+        assert t.step(slots, [0] * 8, new, sum(new) + 100) == 0
+    assert t.step([2, 4], [20000, 15000], [500, 40000 - 15000 - 500], 40000) == 1
+    assert t.step([2, 4], [20000, 15000], [500, 9000], 40000) == 0
+    t.release(slots)
+    r = Tables(6, 20, 100, 64, 1280, 6)
+    assert r.step([3, 1, 0], [0, 100, 0], [30000, 10000, 1], 40001) == 0
+
+
 @pytest.mark.parametrize("slots,lengths,new,tokens,status", [
     ([0, 1, 0], [0, 0, 0], [1, 1, 1], 3, 4), ([0, 9], [0, 0], [1, 1], 2, 4), ([0, -2], [0, 0], [1, 1], 2, 4),
     ([0, 1], [0, -1], [1, 1], 2, 4), ([0, 1], [0, 0], [1, -1], 2, 4), ([0, 1], [0, 0], [3, 4], 6, 3),
