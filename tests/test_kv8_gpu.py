@@ -112,12 +112,12 @@ def test_tables_of_a_step_that_all_sms_share():
     """Long prompts and short ones, padding between them, 40,000 tokens and more; once refused, once taken, once again."""
     new = [15000, 1, 0, 300, 20000, 64, 7000, 33]
     slots = [4, 0, 9, -1, 2, 7, 1, 5]
-    t = Tables(12, 400, 900, 64, 0, 5)
+    t = Tables(12, 400, 850, 64, 0, 5)
     assert t.step(slots, [0] * 8, [700 * 64] + new[1:], 80000) == 2
     assert t.step(slots, [0] * 8, [390 * 64, 1, 0, 300, 390 * 64] + new[5:], 80000) == 1
     for _ in range(2):
         assert t.step(slots, [0] * 8, new, sum(new) + 100) == 0
-    assert t.step([2, 4], [20000, 15000], [500, 40000 - 15000 - 500], 40000) == 1
+    assert t.step([2, 4], [20000, 15000], [500, 24500], 40000) == 2
     assert t.step([2, 4], [20000, 15000], [500, 9000], 40000) == 0
     t.release(slots)
     r = Tables(6, 20, 100, 64, 1280, 6)
