@@ -7,17 +7,20 @@
 // One block owns 128 rows of one (sequence, kv head); a row is a (token, query head of the group) pair.  The cache's
 // numbers become f16 in shared memory, exactly, and both products are f16 with float sums:
 //
-//   warps 0-7   softmax: two threads own each row, 64 of a tile's 128 scores each.  Scores come out of tensor memory, the
-//               weights go back over them as f16 pairs, and at the end the thread scales and stores its half of the row;
-//   warps 8-15  turn keys and values into f16 (1024 + 128 + q has the bits 0x6400 | (q + 128): one byte permutation makes
+//   warps 0-15  softmax: four threads own each row, 32 of a tile's 128 scores each (a group of keys with one scale).  Scores
+//               come out of tensor memory, the weights go back over them as f16 pairs, and at the end the thread scales and
+//               stores its quarter of the row.  (Eight warps with 64 scores a thread took 5,600 cycles a tile: two warps on a
+//               scheduler do not cover what each waits for.)
+//   warps 16-23 turn keys and values into f16 (1024 + 128 + q has the bits 0x6400 | (q + 128): one byte permutation makes
 //               two, one subtraction takes 1152 away) and store them as the tensor core reads them: keys in units of 64
-//               entries of a head, values in units of as many bytes, all in one ring of slots in the order of their use, four
+//               entries of a head, values in units of as many bytes, all in one ring of slots in the order of their use (the
+//               keys of tile 0; then the keys of tile j + 1 and the values of tile j; the values of the last tile), four
 //               warps every other unit (with four warps for all of them a tile took 8,600 cycles: a unit is 260 of
 //               arithmetic and 500 of waiting for shared memory and barriers);
-//   warp 16     one thread issues tcgen05.mma: S = Q K^T (128 x 128) into one of two buffers in tensor memory, O += P V
+//   warp 24     one thread issues tcgen05.mma: S = Q K^T (128 x 128) into one of two buffers in tensor memory, O += P V
 //               (128 x head size, P from tensor memory, the values as they lie, keys x entries);
-//   warp 17     looks up where the keys lie and what their scales are, 32 groups of 32 keys at a time, for all the others;
-//   warp 18, 19 issue the TMA loads of the units' bytes, of keys and of values, into a ring of their own.  (Loads into the
+//   warp 25     looks up where the keys lie and what their scales are, 32 groups of 32 keys at a time, for all the others;
+//   warp 26, 27 issue the TMA loads of the units' bytes, of keys and of values, into a ring of their own.  (Loads into the
 //               converting threads' registers were as many, but what tells the tensor core of a thread's stores waits for its
 //               loads too: 6.4 us a tile of 128 keys and 256 entries.  One thread for all loads needs 1,000 cycles a unit.)
 //
@@ -39,18 +42,20 @@
 
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 namespace {
 
 using namespace tc;
 using namespace kv8;
 
 constexpr int BM = 128, BN = 128;
-constexpr int SOFTMAX_WARPS = 8, CONVERT_WARPS = 4, CONVERT_GROUPS = 2;       // (warps of a group)
+constexpr int SOFTMAX_WARPS = 16, CONVERT_WARPS = 4, CONVERT_GROUPS = 2;      // (warps of a group)
 constexpr int ISSUER = SOFTMAX_WARPS + CONVERT_GROUPS * CONVERT_WARPS, LOOKUP = ISSUER + 1, LOADER = LOOKUP + 1;
-constexpr int THREADS = 32 * (LOADER + 2);   // five groups of four warps
-// registers of a thread: 96 at launch, 61,440 in all, then 256 x 152 + 256 x 64 + 128 x 48 = 61,440
-constexpr int LAUNCH_REGS = 96, SOFTMAX_REGS = 152, CONVERT_REGS = 64, OTHER_REGS = 48;
-static_assert(THREADS * LAUNCH_REGS == 256 * SOFTMAX_REGS + 256 * CONVERT_REGS + 128 * OTHER_REGS, "registers of the block");
+constexpr int THREADS = 32 * (LOADER + 2);   // seven groups of four warps
+// registers of a thread: 72 at launch, 64,512 in all, then 512 x 88 + 256 x 56 + 128 x 40 = 64,512
+constexpr int LAUNCH_REGS = 72, SOFTMAX_REGS = 88, CONVERT_REGS = 56, OTHER_REGS = 40;
+static_assert(THREADS * LAUNCH_REGS == 512 * SOFTMAX_REGS + 256 * CONVERT_REGS + 128 * OTHER_REGS, "registers of the block");
 constexpr int TMEM_COLS = 512;
 constexpr int UNIT = 16384;               // bytes of a slot: 128 keys x 64 entries, or the same number of values
 constexpr int RAW = UNIT / 2;             // .. as they come from the cache
@@ -122,26 +127,6 @@ __device__ __forceinline__ uint4 ld_shared16(uint32_t p) {
     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(p) : "memory");
     return v;
 }
-// Units in the order of their use: K(0); then K(j + 1), V(j) for every tile j but the last; V(last).
-template <int PARTS>
-struct UnitOrder {
-    int n_tiles, tile = 0, part = 0;
-    bool keys = true;
-    __device__ __forceinline__ explicit UnitOrder(int n) : n_tiles(n) {}
-    __device__ __forceinline__ void step() {
-        if (++part < PARTS) return;
-        part = 0;
-        if (keys) {
-            if (tile == 0 && n_tiles > 1) tile = 1;
-            else { keys = false; tile = max(0, tile - 1); }
-        } else if (tile + 2 < n_tiles) {
-            keys = true;
-            tile += 2;
-        } else {
-            ++tile;
-        }
-    }
-};
 // Two floats in one instruction, and the largest of three.
 __device__ __forceinline__ uint64_t pair_of(float a, float b) {
     uint64_t v;
@@ -174,10 +159,10 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return v;
 }
 
-// A barrier of 64 threads that tells whether all of them are well.
-__device__ __forceinline__ bool both_ok(int id, bool ok) {
+// A barrier of the four warps that share 32 rows; tells whether all of them are well.
+__device__ __forceinline__ bool all_ok(int id, bool ok) {
     uint32_t all;
-    asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 q, %2, 0;\nbarrier.cta.red.and.aligned.pred p, %1, 64, q;\nselp.u32 %0, 1, 0, p;\n}"
+    asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 q, %2, 0;\nbarrier.cta.red.and.aligned.pred p, %1, 128, q;\nselp.u32 %0, 1, 0, p;\n}"
                  : "=r"(all) : "r"(id), "r"((uint32_t)ok) : "memory");
     return all != 0;
 }
@@ -217,8 +202,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
     const uint32_t raw_s = ring + SLOTS * UNIT;
     uint8_t* rest = smem_raw + SH::Q_BYTES + SLOTS * UNIT + RAWS * RAW;
     Meta* meta = reinterpret_cast<Meta*>(rest);              // [2][CHUNK][4]
-    float* xch = reinterpret_cast<float*>(meta + 2 * CHUNK * 4);     // [2][2][BM]: maxima by tile parity and half; the sums reuse it
-    float* q_scale = xch + 4 * BM;                           // [BM]
+    float* xch = reinterpret_cast<float*>(meta + 2 * CHUNK * 4);     // [2][4][BM]: maxima by tile parity and part; the sums reuse it
+    float* q_scale = xch + 8 * BM;                           // [BM]
     uint64_t* bars = reinterpret_cast<uint64_t*>(q_scale + BM);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + U_FULL + 2 * SLOTS + 2 * RAWS);
     volatile int* give_up = reinterpret_cast<volatile int*>(tmem_slot + 1);       // three
@@ -453,43 +438,51 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
         // VK / 4 further each.  Lanes are laid out so that eight of them store to all banks.
         const int group = (warp - SOFTMAX_WARPS) / CONVERT_WARPS, t = threadIdx.x & (32 * CONVERT_WARPS - 1);
         const int k_row = t >> 2, k_c = t & 3;
-        const int v_c = (t & 3) | (((t >> 3) % PARTS) << 2), v_row = ((t >> 2) & 1) + ((t >> 3) / PARTS) * 2;
+        // (values: the second four of eight lanes take the other four pieces of 128 bytes in the other of two rows, so that
+        // neither the loads nor the stores of the eight meet a bank twice)
+        const int v_c = PARTS == 1 ? t & 3 : (t & 3) | ((((t >> 2) ^ (t >> 3)) & 1) << 2) | (PARTS == 4 ? ((t >> 4) & 1) << 3 : 0);
+        const int v_row = ((t >> 2) & 1) | (PARTS == 1 ? t >> 3 : PARTS == 2 ? t >> 4 : t >> 5) << 1;
         const uint32_t k_src = k_row * 64 + k_c * 16, v_src = v_row * HD + v_c * 16;
         const uint32_t k_dst = k_row * 128, v_dst = (v_c >> 2) * (VK * 128) + v_row * 128;
         const int k_piece = (2 * k_c) ^ (k_row & 7), v_piece = (2 * (v_c & 3)) ^ (v_row & 7);
-        UnitOrder<PARTS> x(n_tiles);
-        const int units = 2 * PARTS * n_tiles;
-        if (group) x.step();
-        for (int u = group; u < units; u += CONVERT_GROUPS) {
+        bool ok = true;
+        auto convert = [&](auto kind, int u) {
+            constexpr bool KEYS = decltype(kind)::value;
             const int sl = u % SLOTS, rs = u % RAWS;
-            if (!wait_soon(r_full(rs), (u / RAWS) & 1, give_up, 5)) break;
-            const uint32_t src = raw_s + rs * RAW + (x.keys ? k_src : v_src), far = x.keys ? 32 * 64 : VK / 4 * HD;
+            ok = ok && wait_soon(r_full(rs), (u / RAWS) & 1, give_up, 5);
+            if (!ok) return;
             uint4 raw[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) raw[i] = ld_shared16(src + i * far);
-            if (!wait_soon(u_empty(sl), ((u / SLOTS) & 1) ^ 1, give_up, 14)) break;
-            const uint32_t at = ring + sl * UNIT + (x.keys ? k_dst : v_dst), stride = x.keys ? 32 * 128 : VK / 4 * 128;
-            const int piece = x.keys ? k_piece : v_piece;
+            for (int i = 0; i < 4; ++i) raw[i] = ld_shared16(raw_s + rs * RAW + (KEYS ? k_src + i * (32 * 64) : v_src + i * (VK / 4 * HD)));
+            ok = wait_soon(u_empty(sl), ((u / SLOTS) & 1) ^ 1, give_up, 14);
+            if (!ok) return;
+            const uint32_t at = ring + sl * UNIT + (KEYS ? k_dst : v_dst);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) put_f16(at + i * stride, piece, raw[i]);
+            for (int i = 0; i < 4; ++i) put_f16(at + i * (KEYS ? 32 * 128 : VK / 4 * 128), KEYS ? k_piece : v_piece, raw[i]);
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) {
                 mbar_arrive(r_empty(rs));
                 mbar_arrive(u_full(sl));
             }
-            x.step();
-            x.step();
+        };
+        // every other unit (where a tile is one unit: one group the keys, one the values), each group's in the ring's order
+        const int first = PARTS > 1 ? group : 0, stride = PARTS > 1 ? CONVERT_GROUPS : 1;
+        const bool keys = PARTS > 1 || group == 0, values = PARTS > 1 || group == 1;
+        for (int j = -1; j < n_tiles && ok; ++j) {
+            if (keys && j + 1 < n_tiles)
+                for (int p = first; p < PARTS; p += stride) convert(std::true_type(), (j < 0 ? 0 : 2 * j + 1) * PARTS + p);
+            if (values && j >= 0)
+                for (int p = first; p < PARTS; p += stride) convert(std::false_type(), min(2 * j + 2, 2 * n_tiles - 1) * PARTS + p);
         }
     } else {
         more_registers<SOFTMAX_REGS>();
-        // Two warps share each quarter of the rows (a warp may only touch the 32 lanes of tensor memory of its quarter):
-        // warp w and warp w + 4 own the same 32 rows, the first takes score columns 0-63, the second 64-127.  They agree on
-        // the row's reference maximum through shared memory and a 64-thread barrier.
-        constexpr int W = BN / 2;
-        const int quarter = warp & 3, half = warp >> 2;
+        // Four warps share each quarter of the rows (a warp may only touch the 32 lanes of tensor memory of its quarter), 32
+        // score columns each.  They agree on the rows' reference maxima through shared memory and a barrier of their own.
+        constexpr int W = BN / 4, OUT = HD / 4;
+        const int quarter = warp & 3, part = warp >> 2;
         const int r = quarter * 32 + lane;
-        const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
+        const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
         const bool row_ok = r < rows_here;
         const int pos = pos0 + (row0 + r) / a.group;
         const float qs = q_scale[r];
@@ -503,32 +496,23 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
         for (int j = 0; j < n_tiles; ++j) {
             const int s = j & 1;
             if (ok && j % CHUNK == 0) ok = wait_warp(bar(META_FULL + ((j / CHUNK) & 1)), (j / CHUNK >> 1) & 1, give_up, 9);
-            const Meta* m = meta + ((j / CHUNK) & 1) * CHUNK * 4 + (j % CHUNK) * 4 + 2 * half;
-            float f[2];
-            int ve[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                f[h] = m[h].k_scale * unit;
-                ve[h] = m[h].v_exp;
-            }
+            const Meta& m = meta[((j / CHUNK) & 1) * CHUNK * 4 + (j % CHUNK) * 4 + part];
+            const float f = m.k_scale * unit;
+            int ve = m.v_exp;
             if (ok) ok = wait_warp(bar(S_FULL + s), (j >> 1) & 1, give_up, 8);
             fence_after_sync();
-            const int key_base = (t_first + j) * BN, kp0 = key_base + half * W;
+            const int key_base = (t_first + j) * BN, kp0 = key_base + part * W;
             const bool edge = key_base + BN - 1 > pos_lo || key_base < pos_hi - window + 1;
             // visible: lo <= c <= hi for column c of this thread
             const int hi = row_ok ? pos - kp0 : -1, lo = pos - window + 1 - kp0;
             uint64_t z[W / 2];                               // scores in log2 units, two by two
-            float top[2] = {-INFINITY, -INFINITY};
             auto scores = [&](auto&& to_z) {
                 uint32_t sv[W];
-                uint32_t(&x0)[32] = *reinterpret_cast<uint32_t(*)[32]>(&sv[0]);
-                uint32_t(&x1)[32] = *reinterpret_cast<uint32_t(*)[32]>(&sv[32]);
-                tmem_ld32(tmem + lane_addr + S_COL + s * BN + half * W, x0);
-                tmem_ld32(tmem + lane_addr + S_COL + s * BN + half * W + 32, x1);
+                tmem_ld32(lane_addr + S_COL + s * BN + part * W, sv);
                 tmem_wait_ld();
 #pragma unroll
                 for (int c = 0; c < W / 2; ++c)
-                    z[c] = to_z(mul2(pair_of(__uint_as_float(sv[2 * c]), __uint_as_float(sv[2 * c + 1])), pair_of(f[c / 16], f[c / 16])));
+                    z[c] = to_z(mul2(pair_of(__uint_as_float(sv[2 * c]), __uint_as_float(sv[2 * c + 1])), pair_of(f, f)));
             };
             if (a.cap > 0.0f) {
                 // cap log2e tanh(x).  Scores are mostly well below the cap, and there the series to x^9 is as exact (|x| up to
@@ -558,77 +542,67 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
                     z[c] = pair_of(x.x, x.y);
                 }
             }
+            float m_t = -INFINITY;
 #pragma unroll
             for (int c = 0; c < W / 2; ++c) {
                 const float2 x = halves(z[c]);
-                top[c / 16] = max3(top[c / 16], x.x, x.y);
+                m_t = max3(m_t, x.x, x.y);
             }
-            float e[2];
-            bool apart = false;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                if (ve[h] == BAD) {                          // a NaN block: whoever sees a key of it gets NaN
-                    sees_bad = sees_bad || (hi >= 32 * h && lo < 32 * h + 32);
-                    ve[h] = 0;
-                }
-                apart = apart || ve[h] < -60;
-                e[h] = (float)ve[h];
-                top[h] += e[h];
+            if (ve == BAD) {                                 // a NaN block: whoever sees a key of it gets NaN
+                sees_bad = sees_bad || (hi >= 0 && lo < W);
+                ve = 0;
             }
-            float m_t = fmaxf(top[0], top[1]);
-            xch[(s * 2 + half) * BM + r] = m_t;              // double-buffered by the tile's parity
-            // after this barrier both threads of the row hold their scores in registers, so the weights may go over the
-            // partner's score columns
-            ok = both_ok(1 + quarter, ok);                   // (a wait that ran out ends both, or one would wait for the other)
+            const float e = (float)ve;
+            xch[(s * 4 + part) * BM + r] = m_t + e;          // double-buffered by the tile's parity
+            // after this barrier all four threads of the row hold their scores in registers, so the weights may go over them
+            ok = all_ok(1 + quarter, ok);                    // (a wait that ran out ends all four, or some would wait for the others)
             if (!ok) break;
-            m_t = fmaxf(m_t, xch[(s * 2 + (half ^ 1)) * BM + r]);
+            m_t = max3(fmaxf(xch[s * 4 * BM + r], xch[(s * 4 + 1) * BM + r]), xch[(s * 4 + 2) * BM + r], xch[(s * 4 + 3) * BM + r]);
             const bool raise = m_t > m_ref + RESCALE_GAP;    // also true for the first visible tile of a row
             const float m_new = raise ? m_t : m_ref;
             const float corr = (raise && m_ref > -INFINITY) ? fast_exp2(m_ref - m_new) : 1.0f;
             if (j > 0 && __any_sync(0xffffffffu, corr != 1.0f)) {
                 // rare: the accumulator has to be at rest (the product of the tile before is done), then every row of the
-                // warp is scaled anew; each warp of the pair takes half of the entries
+                // warp is scaled anew; each of the four warps takes a quarter of the entries
                 ok = wait_warp(bar(PV_DONE + (s ^ 1)), ((j - 1) >> 1) & 1, give_up, 12);
                 fence_after_sync();
 #pragma unroll 1
-                for (int c = half * (HD / 2); c < (half + 1) * (HD / 2); c += 32) {
-                    uint32_t ov[32];
-                    tmem_ld32(tmem + lane_addr + O_COL + c, ov);
+                for (int c = part * OUT; c < (part + 1) * OUT; c += 16) {
+                    uint32_t ov[16];
+                    tmem_ld16(lane_addr + O_COL + c, ov);
                     tmem_wait_ld();
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * corr);
-                    tmem_st32(tmem + lane_addr + O_COL + c, ov);
+                    for (int i = 0; i < 16; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * corr);
+                    tmem_st16(lane_addr + O_COL + c, ov);
                 }
             }
             l *= corr;
             m_ref = m_new;
-            // weights -> tensor memory, f16 pairs: keys 2c, 2c+1 of this thread in column c of its 32
-            uint64_t sums[2] = {0ull, 0ull};
+            // weights -> tensor memory, f16 pairs: keys 2c, 2c+1 of this thread in column c of its 16
             const float m_sub = m_ref > -INFINITY ? m_ref : 0.0f;    // a row that has seen nothing: 2^(-inf - 0) = 0
+            uint64_t sums = 0ull;
             uint32_t pw[W / 2];
 #pragma unroll
             for (int c = 0; c < W / 2; ++c) {
-                const float2 x = halves(add2(z[c], pair_of(e[c / 16] - m_sub, e[c / 16] - m_sub)));
+                const float2 x = halves(add2(z[c], pair_of(e - m_sub, e - m_sub)));
                 const float p0 = fast_exp2(x.x), p1 = fast_exp2(x.y);
-                sums[c / 16] = add2(sums[c / 16], pair_of(p0, p1));
+                sums = add2(sums, pair_of(p0, p1));
                 const __half2 t = __floats2half2_rn(p0, p1);
                 pw[c] = *reinterpret_cast<const uint32_t*>(&t);
             }
-            if (!apart) {
-                const float2 s0 = halves(sums[0]), s1 = halves(sums[1]);
-                l += fmaf(s0.x + s0.y, power_of_two(-ve[0]), (s1.x + s1.y) * power_of_two(-ve[1]));
+            tmem_st16(lane_addr + S_COL + s * BN + part * (W / 2), pw);
+            if (ve >= -60) {
+                const float2 sum = halves(sums);
+                l = fmaf(sum.x + sum.y, power_of_two(-ve), l);
             } else {
                 // scales more than 2^60 apart: what a weight is without its scale may be lost with it.  (It may be infinite
                 // here: the row's result is then 0, which it is beside the values of the largest scale.)
-                float sum = 0.0f;
 #pragma unroll
                 for (int c = 0; c < W / 2; ++c) {
                     const float2 x = halves(z[c]);
-                    sum += fast_exp2(x.x - m_sub) + fast_exp2(x.y - m_sub);
+                    l += fast_exp2(x.x - m_sub) + fast_exp2(x.y - m_sub);
                 }
-                l += sum;
             }
-            tmem_st32(tmem + lane_addr + S_COL + s * BN + half * (W / 2), pw);
             tmem_wait_st();
             fence_before_sync();
             __syncwarp();
@@ -638,53 +612,53 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
             }
         }
         if (ok && n_tiles > 0) ok = wait_warp(bar(PV_DONE + ((n_tiles - 1) & 1)), ((n_tiles - 1) >> 1) & 1, give_up, 11);
-        // the row's sum is that of the two halves (always added in the same order), and so is what they have seen
-        const int fin = (n_tiles & 1) * 2;                   // the buffer that the next tile would have used
-        xch[(fin + half) * BM + r] = sees_bad || qs != qs ? __int_as_float(0x7fc00000) : l;
-        asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
-        const float total = xch[fin * BM + r] + xch[(fin + 1) * BM + r];
+        // the row's sum is that of its four threads (always added in the same order), and so is what they have seen
+        float* last = xch + (n_tiles & 1) * 4 * BM;          // the buffer that the next tile would have used
+        last[part * BM + r] = sees_bad || (qs != qs && pos >= 0) ? __int_as_float(0x7fc00000) : qs != qs ? 0.0f : l;
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + quarter) : "memory");
+        const float total = (last[r] + last[BM + r]) + (last[2 * BM + r] + last[3 * BM + r]);
         if (ok) {
             fence_after_sync();
             const float inv = total > 0.0f ? 1.0f / total : 0.0f;
             const float v0 = power_of_two(e0);
-            const bool nan = total != total && pos >= 0;
+            const bool nan = total != total;
             const int row = row0 + r, tok = first_tok + row / a.group, head = g * a.group + row % a.group;
             bf16* dst = a.out + (size_t)tok * a.out_stride + (size_t)head * HD;
-            const size_t part = ((size_t)tok * a.n_kv * a.group + head) * a.spans + span;
-            if (a.spans > 1 && row_ok && half == 0) *reinterpret_cast<float2*>(a.part_ml + part * 2) = make_float2(m_ref, total);
+            const size_t share = ((size_t)tok * a.n_kv * a.group + head) * a.spans + span;
+            if (a.spans > 1 && row_ok && part == 0) *reinterpret_cast<float2*>(a.part_ml + share * 2) = make_float2(m_ref, total);
             const bool wide = ((uintptr_t)a.out & 15) == 0 && (a.out_stride & 7) == 0;
 #pragma unroll 1
-            for (int c = half * (HD / 2); c < (half + 1) * (HD / 2); c += 32) {
-                uint32_t ov[32];
+            for (int c = part * OUT; c < (part + 1) * OUT; c += 16) {
+                uint32_t ov[16];
                 if (n_tiles > 0) {
-                    tmem_ld32(tmem + lane_addr + O_COL + c, ov);
+                    tmem_ld16(lane_addr + O_COL + c, ov);
                     tmem_wait_ld();
                 }
                 if (row_ok && a.spans > 1) {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
+                    for (int i = 0; i < 16; i += 4) {
                         float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                         if (n_tiles > 0)
                             x = make_float4(__uint_as_float(ov[i]) * v0, __uint_as_float(ov[i + 1]) * v0, __uint_as_float(ov[i + 2]) * v0,
                                             __uint_as_float(ov[i + 3]) * v0);
-                        *reinterpret_cast<float4*>(a.part_o + part * HD + c + i) = x;
+                        *reinterpret_cast<float4*>(a.part_o + share * HD + c + i) = x;
                     }
                 } else if (row_ok) {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 8) {
+                    for (int i = 0; i < 16; i += 8) {
                         uint4 pk;
                         __nv_bfloat162* p2 = reinterpret_cast<__nv_bfloat162*>(&pk);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            float x = n_tiles > 0 ? __uint_as_float(ov[i + 2 * e]) * inv * v0 : 0.0f;
-                            float y = n_tiles > 0 ? __uint_as_float(ov[i + 2 * e + 1]) * inv * v0 : 0.0f;
+                        for (int h = 0; h < 4; ++h) {
+                            float x = n_tiles > 0 ? __uint_as_float(ov[i + 2 * h]) * inv * v0 : 0.0f;
+                            float y = n_tiles > 0 ? __uint_as_float(ov[i + 2 * h + 1]) * inv * v0 : 0.0f;
                             if (nan) x = y = total;
-                            p2[e] = __floats2bfloat162_rn(x, y);
+                            p2[h] = __floats2bfloat162_rn(x, y);
                         }
                         if (wide) *reinterpret_cast<uint4*>(dst + c + i) = pk;
                         else {
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) dst[c + i + e] = reinterpret_cast<const bf16*>(&pk)[e];
+                            for (int h = 0; h < 8; ++h) dst[c + i + h] = reinterpret_cast<const bf16*>(&pk)[h];
                         }
                     }
                 }
@@ -712,7 +686,7 @@ int make_map(CUtensorMap* map, const void* ptr, long long rows, int hd, int box_
 template <int HD>
 int launch(const TcArgs& a, cudaStream_t stream) {
     using SH = Shape<HD>;
-    constexpr size_t smem = (size_t)SH::Q_BYTES + (size_t)SH::SLOTS * UNIT + SH::RAWS * RAW + 2 * CHUNK * 4 * sizeof(Meta) + 5 * BM * 4 +
+    constexpr size_t smem = (size_t)SH::Q_BYTES + (size_t)SH::SLOTS * UNIT + SH::RAWS * RAW + 2 * CHUNK * 4 * sizeof(Meta) + 9 * BM * 4 +
                             (U_FULL + 2 * SH::SLOTS + 2 * SH::RAWS) * 8 + 32;
     static_assert(smem <= 232448, "shared memory of a block");
     static OncePerDevice raised;

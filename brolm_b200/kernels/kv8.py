@@ -203,8 +203,9 @@ def kv8_shares(batch: int, n_kv: int, row_tiles: int, keys: int, head_dim: int, 
 
     Two blocks run on an SM (three, of heads of up to 64 entries), and there are as many shares as give every SM its blocks,
     but none whose four warps would not have a tile of keys each.  Up to eight join their results inside the launch; more
-    are joined by a second one, which pays from about 100 tiles on (1 sequence of 8,192 keys, 4 kv heads of 256: 18.3 us as
-    8 x 1, 11.1 as 8 x 8; 2 of 2,000: 8.6 as 8 x 1, 10.2 as 8 x 2).
+    are joined by a second one, which pays from about 100 tiles on where eight shares leave SMs without a block (1 sequence
+    of 8,192 keys, 4 kv heads of 256: 18.3 us as 8 x 1, 11.1 as 8 x 8; 2 of 2,000: 8.6 as 8 x 1, 10.2 as 8 x 2; 12 of 4,000,
+    2 kv heads of 64, float32: 12.9 as 8 x 1, 20.8 as 8 x 2).
 
     Where the items give no more than two shares, the longest sequences' blocks would run alone at the end: such steps
     are cut into rounds of blocks that the SMs take as they come free, if the shares stay long enough (24 tiles) and fill
@@ -223,7 +224,7 @@ def kv8_shares(batch: int, n_kv: int, row_tiles: int, keys: int, head_dim: int, 
         return max(1, want), 1
     if want <= KV8_CLUSTER:
         return want, 1
-    return KV8_CLUSTER, (1 if tiles < 96 else want // KV8_CLUSTER)
+    return KV8_CLUSTER, (want // KV8_CLUSTER if tiles >= 96 and items * KV8_CLUSTER < sms else 1)
 
 
 def _parts(n: int, head_dim: int, device) -> tuple:
