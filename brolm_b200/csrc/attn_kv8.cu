@@ -24,7 +24,8 @@
 // ring of its own of key and value tiles in flight (cp.async, no barrier but its own), two blocks on an SM.
 //
 // The shares of a row's keys are joined inside the launch: they form a cluster, whose blocks read each other's partial
-// results out of shared memory.  Nothing is kept between launches.
+// results out of shared memory.  Where that is not enough, or where clusters are dealt out over sequences of different
+// lengths, the clusters' results are joined by a second launch (attn_kv8_join.cuh).  Nothing is kept between launches.
 #include "attn_kv8_join.cuh"
 
 #include <cuda_fp16.h>
@@ -47,7 +48,9 @@ struct AttnArgs {
     int tokens, rows, n_kv, group, dim, block, n_blocks, n_slots, width, ring, window;
     float scale, cap;
     int shares, spans, row_tiles, wide;   // blocks of a cluster, clusters that share a row's keys, row tiles of a sequence
+    int dealt;                            // 0, or: clusters dealt out over the sequences by their lengths (then spans = 1)
     float *part_o, *part_ml;              // [token][head][span][dim] and [..][2] where spans > 1
+    int2* plan;                           // dealt: where the parts of a (token, head) begin, and how many there are
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -169,23 +172,99 @@ struct Eight {
 
 // What a block works on: rows of one sequence and kv head, and the tiles [t_begin, t_end) of their keys.
 struct Item {
-    int share, span, g, first_tok, row0, n_rows, pos0, pos_lo, pos_hi, slot, t_begin, t_end;
+    int share, span, spans, part0, g, first_tok, row0, n_rows, pos0, pos_lo, pos_hi, slot, t_begin, t_end;
 };
+// Sequences of different lengths: the launch's clusters are dealt out over them, so that no cluster has more than w rounds of
+// its warps' tiles, w the least for which there are enough.  Every warp finds that out for itself: which sequence its
+// cluster c is given, the how manieth of its clusters it is and of how many (none where clusters are left over).
+constexpr int MAX_DEALT = 128;                                 // sequences of such a launch
+__device__ __forceinline__ void deal(const AttnArgs& a, int c, Item& it, int& end_tok, int& kv_len) {
+    constexpr int PER = MAX_DEALT / 32;
+    const int lane = threadIdx.x & 31, round = WARPS * a.shares;
+    int first[PER], end[PER], len[PER], slot[PER], work[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int b = lane + 32 * j;
+        first[j] = end[j] = len[j] = slot[j] = 0;
+        if (b < a.rows) {
+            first[j] = ld_now(a.cu_q + b);
+            end[j] = ld_now(a.cu_q + b + 1);
+            len[j] = ld_now(a.kv_len + b);
+            slot[j] = ld_now(a.slots + b);
+        }
+    }
+    int total = 0, most = 1;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int pos0 = len[j] - (min(end[j], a.tokens) - first[j]), from = a.window > 0 ? max(0, pos0 - a.window + 1) / KT : 0;
+        work[j] = lane + 32 * j < a.rows ? max(1, ((max(0, len[j] - 1) / KT - from + 1) + round - 1) / round) : 0;
+        total += work[j];
+        most = max(most, work[j]);
+    }
+    total = __reduce_add_sync(0xffffffffu, total);
+    most = __reduce_max_sync(0xffffffffu, most);
+    int lo = min(most, (total + a.dealt - 1) / a.dealt), hi = most;
+    while (lo < hi) {                                          // (hi is enough: there are no fewer clusters than sequences)
+        const int w = (lo + hi) >> 1;
+        int need = 0;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) need += (work[j] + w - 1) / w;
+        if (__reduce_add_sync(0xffffffffu, need) <= a.dealt) hi = w;
+        else lo = w + 1;
+    }
+    it.first_tok = it.slot = -1;
+    it.span = 0;
+    end_tok = kv_len = 0;
+    int before = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        if (32 * j >= a.rows) break;
+        const int mine = (work[j] + lo - 1) / lo;
+        int upto = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const int x = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= d) upto += x;
+        }
+        const int at = c - (before + upto - mine);
+        const uint32_t found = __ballot_sync(0xffffffffu, at >= 0 && at < mine);
+        if (found) {
+            const int from = __ffs(found) - 1;
+            it.span = __shfl_sync(0xffffffffu, at, from);
+            it.spans = __shfl_sync(0xffffffffu, mine, from);
+            it.first_tok = __shfl_sync(0xffffffffu, first[j], from);
+            end_tok = __shfl_sync(0xffffffffu, end[j], from);
+            kv_len = __shfl_sync(0xffffffffu, len[j], from);
+            it.slot = __shfl_sync(0xffffffffu, slot[j], from);
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+}
+
 // Three round trips to memory lie before the first product: what the sequence is; its row of the tables and the queries;
 // the tiles and their scales.  What one trip can fetch is asked for before anything of it is looked at.
 template <int ROWS>
 __device__ __forceinline__ Item find_item(const AttnArgs& a) {
     Item it;
     it.share = blockIdx.x % a.shares;
-    int rest = blockIdx.x / a.shares;
-    it.span = rest % a.spans;
-    rest /= a.spans;
-    const int b = rest / a.row_tiles;
-    it.row0 = (rest - b * a.row_tiles) * ROWS;
+    int rest = blockIdx.x / a.shares, end_tok, kv_len;
     it.g = blockIdx.y;
-    it.first_tok = ld_now(a.cu_q + b);
-    const int end_tok = ld_now(a.cu_q + b + 1), kv_len = ld_now(a.kv_len + b);
-    it.slot = ld_now(a.slots + b);
+    it.spans = a.spans;
+    if (a.dealt > 0) {
+        const int c = rest / a.row_tiles;
+        it.row0 = (rest - c * a.row_tiles) * ROWS;
+        it.part0 = (rest * a.n_kv + it.g) * ROWS;
+        deal(a, c, it, end_tok, kv_len);
+    } else {
+        it.span = rest % a.spans;
+        rest /= a.spans;
+        const int b = rest / a.row_tiles;
+        it.row0 = (rest - b * a.row_tiles) * ROWS;
+        it.first_tok = ld_now(a.cu_q + b);
+        end_tok = ld_now(a.cu_q + b + 1);
+        kv_len = ld_now(a.kv_len + b);
+        it.slot = ld_now(a.slots + b);
+    }
     const int n_tok = min(end_tok, a.tokens) - it.first_tok;
     it.n_rows = it.first_tok < 0 ? 0 : (int)min((long long)ROWS, (long long)n_tok * a.group - it.row0);
     it.pos0 = kv_len - n_tok;                                  // position of the sequence's first new token
@@ -194,7 +273,7 @@ __device__ __forceinline__ Item find_item(const AttnArgs& a) {
     it.t_begin = it.t_end = 0;
     if (it.n_rows > 0 && it.pos_hi >= 0 && it.slot >= 0 && it.slot < a.n_slots) {
         const int t_lo = a.window > 0 ? max(0, it.pos_lo - a.window + 1) / KT : 0, t_hi = it.pos_hi / KT;
-        const int parts = a.shares * a.spans, per = (t_hi - t_lo + parts) / parts;
+        const int parts = a.shares * it.spans, per = (t_hi - t_lo + parts) / parts;
         it.t_begin = t_lo + (it.span * a.shares + it.share) * per;
         it.t_end = min(t_hi + 1, it.t_begin + per);
     }
@@ -360,8 +439,10 @@ __device__ __forceinline__ void merge(const AttnArgs& a, const Item& it, const f
         }
         const int row = it.row0 + r, tok = it.first_tok + row / a.group, head = it.g * a.group + row % a.group;
         if (q_scale[r] != q_scale[r]) acc.x = acc.y = acc.z = acc.w = it.pos0 + row / a.group >= 0 ? q_scale[r] : 0.0f;
-        if (a.spans > 1) {
-            const size_t at = ((size_t)tok * a.n_kv * a.group + head) * a.spans + it.span;
+        if (a.dealt > 0 && it.span == 0 && d == 0)
+            a.plan[(size_t)tok * a.n_kv * a.group + head] = make_int2(it.part0 + r, it.spans);
+        if (it.spans > 1) {
+            const size_t at = a.dealt > 0 ? (size_t)it.part0 + r : ((size_t)tok * a.n_kv * a.group + head) * a.spans + it.span;
             *reinterpret_cast<float4*>(a.part_o + at * a.dim + d) = acc;
             if (d == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(most, sum);
         } else {
@@ -939,11 +1020,11 @@ __global__ void __launch_bounds__(THREADS, 2) attn_kv8_kernel(AttnArgs a) {
 }
 
 template <typename T>
-int launch(void (*kernel)(AttnArgs), size_t smem, OncePerDevice& raised, const AttnArgs& a, cudaStream_t stream) {
+int launch(void (*kernel)(AttnArgs), size_t smem, OncePerDevice& raised, const AttnArgs& a, int tile_rows, cudaStream_t stream) {
     const int st = allow_shared_memory(kernel, smem, raised);
     if (st) return st;
     cudaLaunchConfig_t cfg = {};
-    const long long blocks = (long long)a.rows * a.row_tiles * a.spans * a.shares;
+    const long long blocks = (a.dealt > 0 ? (long long)a.dealt : (long long)a.rows * a.spans) * a.row_tiles * a.shares;
     if (blocks > 0x7fffffffll) return BROLM_ERR_TOO_LARGE;
     cfg.gridDim = dim3((unsigned)blocks, a.n_kv);
     cfg.blockDim = dim3(THREADS);
@@ -961,17 +1042,23 @@ int launch(void (*kernel)(AttnArgs), size_t smem, OncePerDevice& raised, const A
     cfg.attrs = attr;
     cfg.numAttrs = 2;
     const int e = (int)cudaLaunchKernelEx(&cfg, kernel, a);
-    if (e || a.spans == 1) return e;
-    return launch_join<T>(JoinArgs{a.part_o, a.part_ml, a.out, a.cu_q, a.out_stride, a.rows, a.tokens, a.n_kv * a.group, a.dim, a.spans}, stream);
+    if (e || (a.spans == 1 && a.dealt == 0)) return e;
+    JoinArgs j{a.part_o, a.part_ml, a.out, a.cu_q, a.out_stride, a.rows, a.tokens, a.n_kv * a.group, a.dim, a.spans};
+    if (a.dealt > 0) {
+        j.plan = a.plan;
+        j.step = a.row_tiles * a.n_kv * tile_rows;
+        j.parts = a.dealt * j.step;
+    }
+    return launch_join<T>(j, stream);
 }
 
 template <typename T, int DP>
 int launch_rows(const AttnArgs& a, int rows, cudaStream_t stream) {
     static OncePerDevice raised[4];
-    if (rows == 2) return launch<T>(attn_kv8_few_kernel<T, DP, 2>, FewShape<T, DP, 2>::SMEM, raised[0], a, stream);
-    if (rows == 4) return launch<T>(attn_kv8_few_kernel<T, DP, 4>, FewShape<T, DP, 4>::SMEM, raised[1], a, stream);
-    if (rows == 8) return launch<T>(attn_kv8_few_kernel<T, DP, 8>, FewShape<T, DP, 8>::SMEM, raised[2], a, stream);
-    return launch<T>(attn_kv8_kernel<T, DP>, Shape<T, DP>::SMEM, raised[3], a, stream);
+    if (rows == 2) return launch<T>(attn_kv8_few_kernel<T, DP, 2>, FewShape<T, DP, 2>::SMEM, raised[0], a, rows, stream);
+    if (rows == 4) return launch<T>(attn_kv8_few_kernel<T, DP, 4>, FewShape<T, DP, 4>::SMEM, raised[1], a, rows, stream);
+    if (rows == 8) return launch<T>(attn_kv8_few_kernel<T, DP, 8>, FewShape<T, DP, 8>::SMEM, raised[2], a, rows, stream);
+    return launch<T>(attn_kv8_kernel<T, DP>, Shape<T, DP>::SMEM, raised[3], a, rows, stream);
 }
 
 template <typename T>
@@ -985,12 +1072,14 @@ int launch_dim(const AttnArgs& a, int rows, cudaStream_t stream) {
 }  // namespace
 
 // shares (1 .. 8): blocks of a cluster that share a row's keys; spans: clusters that do, joined by a second launch through
-// part_o [tokens * n_kv * group * spans * dim] and part_ml [.. * 2].
+// part_o [tokens * n_kv * group * spans * dim] and part_ml [.. * 2].  spans < 0: -spans clusters for every kv head and tile of
+// query rows are dealt out over the sequences (at most 128, and no more than clusters) by their lengths; part_o then holds
+// [-spans * n_kv * tiles * rows of a tile * dim], part_ml [.. * 2] and plan [tokens * n_kv * group * 2].
 struct AttnCall {
     const void* q;
     void* out;
     const void *cu_q, *kv_len, *slots, *tables, *k_pages, *v_pages, *k_scale, *v_scale;
-    void *part_o, *part_ml;
+    void *part_o, *part_ml, *plan;
     cudaStream_t stream;
     int q_stride, out_stride, dtype, tokens, rows, n_kv, group, dim, block, n_blocks, n_slots, width, ring, window, max_q_len, shares, spans;
     float scale, cap;
@@ -1001,17 +1090,19 @@ BROLM_API int brolm_attn_kv8(const AttnCall* c) {
     if (c->dtype != BROLM_F32 && c->dtype != BROLM_BF16) return BROLM_ERR_BAD_DTYPE;
     if (c->tokens < 0 || c->rows < 0 || n_kv <= 0 || group <= 0 || dim <= 0 || dim % 16 || block <= 0 || block % 32) return BROLM_ERR_BAD_SIZE;
     if (c->n_blocks <= 0 || c->n_slots <= 0 || c->width <= 0 || c->ring < 0 || c->ring % block || c->window < 0 || c->max_q_len <= 0) return BROLM_ERR_BAD_SIZE;
-    if (c->shares < 1 || c->shares > MAX_SHARES || c->spans < 1 || (c->spans > 1 && (!c->part_o || !c->part_ml))) return BROLM_ERR_BAD_SIZE;
+    if (c->shares < 1 || c->shares > MAX_SHARES || c->spans == 0 || (c->spans != 1 && (!c->part_o || !c->part_ml))) return BROLM_ERR_BAD_SIZE;
+    if (c->spans < 0 && (c->rows > MAX_DEALT || c->rows > -(long long)c->spans || !c->plan)) return BROLM_ERR_BAD_SIZE;
     if (dim > MAX_DIM || block > MAX_BLOCK || (long long)n_kv * group > 65535 || (long long)c->max_q_len * group > 0x3fffffff) return BROLM_ERR_TOO_LARGE;
     if ((long long)c->n_blocks * block > 0x7fffffffll || c->tokens > 0x3fffffff) return BROLM_ERR_TOO_LARGE;
-    if (((uintptr_t)c->k_pages | (uintptr_t)c->v_pages | (uintptr_t)c->part_o) & 15) return BROLM_ERR_ALIGNMENT;
+    if (((uintptr_t)c->k_pages | (uintptr_t)c->v_pages | (uintptr_t)c->part_o) & 15 || (uintptr_t)c->plan & 7) return BROLM_ERR_ALIGNMENT;
     if (c->tokens == 0 || c->rows == 0) return BROLM_OK;
     const int size = c->dtype == BROLM_F32 ? 4 : 2, most = c->max_q_len * group, per = most <= 2 ? 2 : most <= 4 ? 4 : most <= 8 ? 8 : 16;
     const int wide = ((uintptr_t)c->q & 15) == 0 && (long long)c->q_stride * size % 16 == 0;
     AttnArgs a{c->q, c->out, c->q_stride, c->out_stride, (const int32_t*)c->cu_q, (const int32_t*)c->kv_len,
                (const int32_t*)c->slots, (const int32_t*)c->tables, (const int8_t*)c->k_pages, (const int8_t*)c->v_pages,
                (const float*)c->k_scale, (const float*)c->v_scale, c->tokens, c->rows, n_kv, group, dim, block, c->n_blocks,
-               c->n_slots, c->width, c->ring, c->window, c->scale, c->cap, c->shares, c->spans, (most + per - 1) / per, wide,
-               (float*)c->part_o, (float*)c->part_ml};
+               c->n_slots, c->width, c->ring, c->window, c->scale, c->cap, c->shares, max(c->spans, 1), (most + per - 1) / per, wide,
+               max(-c->spans, 0), (float*)c->part_o, (float*)c->part_ml, (int2*)c->plan};
+    if ((long long)a.dealt * a.row_tiles * n_kv * per > 0x7fffffffll) return BROLM_ERR_TOO_LARGE;
     return c->dtype == BROLM_F32 ? launch_dim<float>(a, per, c->stream) : launch_dim<bf16>(a, per, c->stream);
 }

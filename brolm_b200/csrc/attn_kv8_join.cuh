@@ -34,6 +34,8 @@ struct JoinArgs {
     void* out;
     const int32_t* cu_q;
     int out_stride, rows, tokens, heads, dim, spans;
+    const int2* plan = nullptr;           // where given, [token][head]: the first part and how many, every `step` parts
+    int step = 1, parts = 0;              // (the parts that there are: nothing is read beyond them)
 };
 
 // Rows whose keys were shared by several blocks that do not join their results themselves: a block of threads for every
@@ -44,12 +46,20 @@ __global__ void __launch_bounds__(64) attn_kv8_join_kernel(JoinArgs a) {
     pdl_wait();
     const int tok = blockIdx.x, head = blockIdx.y;
     if (tok >= a.cu_q[a.rows]) return;
-    const size_t at = ((size_t)tok * a.heads + head) * a.spans;
+    size_t at = ((size_t)tok * a.heads + head) * a.spans;
+    int spans = a.spans;
+    if (a.plan) {
+        const int2 p = a.plan[(size_t)tok * a.heads + head];
+        at = p.x;
+        spans = p.y;
+        if (spans <= 1 || p.x < 0 || p.x + (long long)(spans - 1) * a.step >= a.parts) return;     // (one part is in its place)
+    }
+    const size_t step = a.step;
     const int d = threadIdx.x * 4;
     if (d >= a.dim) return;
     float most = -INFINITY, sum = 0.0f;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int s0 = 0; s0 < a.spans; s0 += 8) {                  // (eight parts are asked for at once)
+    for (int s0 = 0; s0 < spans; s0 += 8) {                  // (eight parts are asked for at once)
         float2 ml[8];
         float4 x[8];
         float top = most;
@@ -57,9 +67,9 @@ __global__ void __launch_bounds__(64) attn_kv8_join_kernel(JoinArgs a) {
         for (int s = 0; s < 8; ++s) {
             ml[s] = make_float2(-INFINITY, 0.0f);
             x[s] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (s0 + s < a.spans) {
-                ml[s] = *reinterpret_cast<const float2*>(a.part_ml + (at + s0 + s) * 2);
-                x[s] = *reinterpret_cast<const float4*>(a.part_o + (at + s0 + s) * a.dim + d);
+            if (s0 + s < spans) {
+                ml[s] = *reinterpret_cast<const float2*>(a.part_ml + (at + (s0 + s) * step) * 2);
+                x[s] = *reinterpret_cast<const float4*>(a.part_o + (at + (s0 + s) * step) * a.dim + d);
             }
             top = fmaxf(top, ml[s].x);
         }
@@ -69,7 +79,7 @@ __global__ void __launch_bounds__(64) attn_kv8_join_kernel(JoinArgs a) {
         acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
 #pragma unroll
         for (int s = 0; s < 8; ++s)
-            if (s0 + s < a.spans) add_part(acc, sum, x[s], ml[s].y, top > -INFINITY ? ex2(ml[s].x - top) : 0.0f);
+            if (s0 + s < spans) add_part(acc, sum, x[s], ml[s].y, top > -INFINITY ? ex2(ml[s].x - top) : 0.0f);
     }
     store_row<T>(a.out, a.out_stride, a.dim, tok, head, d, acc, sum);
 }

@@ -40,7 +40,7 @@ _EXTEND = struct.Struct("@14P8i")
 _RELEASE = struct.Struct("@7P4i")
 _WRITE = struct.Struct("@10P4q8i")
 _READ = struct.Struct("@11P4q10i")
-_ATTN = struct.Struct("@13P17i2f")
+_ATTN = struct.Struct("@14P17i2f")
 _ATTN_TC = struct.Struct("@13P15i2f")
 _functions: dict = {}
 _NO_CPU = "brolm_b200 kernels run on CUDA tensors only; there is no CPU path"
@@ -195,26 +195,50 @@ def kv8_read(cu_q: torch.Tensor, kv_len: torch.Tensor, slots: torch.Tensor, tabl
 
 
 KV8_TILE, KV8_WARPS, KV8_CLUSTER = 32, 4, 8       # keys of a tile, warps of a block, blocks that join their results themselves
+KV8_DEALT = 128                                   # sequences of a launch whose clusters are dealt out by length
 
 
 @functools.lru_cache(maxsize=256)
-def kv8_shares(batch: int, n_kv: int, row_tiles: int, keys: int, head_dim: int, sms: int) -> tuple[int, int]:
-    """How many blocks share the keys of one (sequence, kv head, tile of query rows): (blocks of a cluster, clusters).
+def kv8_shares(batch: int, n_kv: int, row_tiles: int, keys: int, head_dim: int, sms: int, many: bool = False) -> tuple[int, int]:
+    """How many blocks share the keys of one (sequence, kv head, tile of query rows): (blocks of a cluster, clusters), or
+    (blocks of a cluster, -n): n clusters of a (kv head, tile of query rows) are dealt out over the sequences by their lengths
+    on the device.  ``many``: more than eight query rows of a kv head, whose tiles take twice as long.
 
     Two blocks run on an SM (three, of heads of up to 64 entries), and there are as many shares as give every SM its blocks,
-    but none whose four warps would not have a tile of keys each.  Up to eight join their results inside the launch; more
-    are joined by a second one, which pays from about 100 tiles on where eight shares leave SMs without a block (1 sequence
-    of 8,192 keys, 4 kv heads of 256: 18.3 us as 8 x 1, 11.1 as 8 x 8; 2 of 2,000: 8.6 as 8 x 1, 10.2 as 8 x 2; 12 of 4,000,
-    2 kv heads of 64, float32: 12.9 as 8 x 1, 20.8 as 8 x 2).
+    but none whose four warps would not have a tile of keys each.  A cluster lies inside one group of SMs, so clusters of
+    three to eight leave up to an eighth of the places empty; where one too many is asked for, it runs alone at the end (48
+    items of 2,000 keys, float32: 28.6 us as 6 x 1, of which 45 fit, 19.7 as 5 x 1; 12 of 4,000 at 4 kv heads of 256, one
+    query row each: 35.8 and 23.3).  Up to eight join their results inside the launch; more are joined by a second one, which
+    pays from about 100 tiles on where eight shares leave SMs without a block (1 sequence of 8,192 keys, 4 kv heads of 256:
+    18.3 us as 8 x 1, 11.1 as 8 x 8; 2 of 2,000: 8.6 as 8 x 1, 10.2 as 8 x 2; 24 items of 4,000, float32, heads of 64: 12.9 as
+    8 x 1, 20.8 as 8 x 2).
 
-    Where the items give no more than two shares, the longest sequences' blocks would run alone at the end: such steps
-    are cut into rounds of blocks that the SMs take as they come free, if the shares stay long enough (24 tiles) and fill
-    their rounds (16 sequences of 129 to 6,145 keys under a window of 4,096, 8 kv heads: 36.9 us as 2 x 1, 32.1 as 1 x 4; of
-    equal ones 32 of 2,048, 4 kv heads: 28.3 as 2 x 1, 30.6 as 1 x 4, which is what it costs)."""
+    Where the longest sequence's warps would have more than eight tiles each, what counts is that sequence, and dealing pays:
+    24 sequences of 100 to 4,000 keys, 4 kv heads of 256, 32.5 us as 3 x 1, 18.3 dealt; 16 of 129 to 6,145 under a window of
+    4,096, 8 kv heads, 33 and 26.5; 4 of 1,000 to 12,000, 4 kv heads, 21.8 and 17.2.  It costs 1.5 to 2.5 us (finding out, and
+    the second launch) where all are equally long (24 of 3,000, 8 kv heads of 128: 35.0 and 37.9), and more than it brings
+    where there are few clusters to deal (48 sequences of 3,000 on 74: 57.9 and 64.7).  What is dealt out is one round of
+    blocks (two rounds: 24.2 us for the first), in clusters of so many that a sequence has about eight parts to join.
+
+    With more sequences, where an item would have no more than two shares, the longest ones' blocks would run alone at the
+    end: such steps are cut into rounds of blocks that the SMs take as they come free, if the shares stay long enough (24
+    tiles) and fill their rounds (40 sequences of 100 to 3,000 keys, 8 kv heads: 52.9 us as 1 x 1, 43.7 as 1 x 2)."""
     places = (3 if head_dim <= 64 else 2) * sms
-    items = max(1, batch * n_kv * row_tiles)
+    heads = n_kv * row_tiles
+    items = max(1, batch * heads)
     tiles = max(1, -(-keys // KV8_TILE))
+
+    def fit(cluster):                             # clusters of a (kv head, tile of rows) that run at a time
+        return (places if cluster <= 2 else places * 7 // 8) // (cluster * heads)
     want = min(places // items, -(-tiles // KV8_WARPS))
+    if want > 2:
+        want = max(2, min(want, places * 7 // 8 // items))
+    if batch > 1 and tiles * (2 if many else 1) > 8 * KV8_WARPS * max(1, min(want, KV8_CLUSTER)):
+        for cluster in (1, 2, 4, 8):
+            if fit(cluster) <= 8 * batch or cluster == 8:
+                break
+        if batch <= KV8_DEALT and fit(cluster) >= 1.5 * batch:
+            return cluster, -fit(cluster)
     if want <= 2:
         if batch > 1 and items < 4 * places:
             for k in (2, 3, 4):
@@ -227,11 +251,12 @@ def kv8_shares(batch: int, n_kv: int, row_tiles: int, keys: int, head_dim: int, 
     return KV8_CLUSTER, (want // KV8_CLUSTER if tiles >= 96 and items * KV8_CLUSTER < sms else 1)
 
 
-def _parts(n: int, head_dim: int, device) -> tuple:
-    """Room for n parts of rows: the tensor that holds it, and where the sums and their (maximum, weight) begin."""
-    parts = torch.empty(n * (head_dim + 2), dtype=_F32, device=device)
+def _parts(n: int, head_dim: int, device, plans: int = 0) -> tuple:
+    """Room for n parts of rows and for ``plans`` pairs of whole numbers: the tensor that holds it, and where the sums, their
+    (maximum, weight) and the pairs begin."""
+    parts = torch.empty(n * (head_dim + 2) + 2 * plans, dtype=_F32, device=device)
     at = parts.data_ptr()
-    return parts, at, at + 4 * n * head_dim
+    return parts, at, at + 4 * n * head_dim, at + 4 * n * (head_dim + 2)
 
 
 @functools.lru_cache(maxsize=256)
@@ -301,17 +326,20 @@ def attention_kv8(q: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, kv_len
         spans = kv8_tc_spans(T, batch, n_kv, group, max_q_len, keys, head_dim, device_sms())
         part_o = part_ml = 0
         if spans > 1:
-            parts, part_o, part_ml = _parts(T * n_kv * group * spans, head_dim, q.device)
+            parts, part_o, part_ml, _ = _parts(T * n_kv * group * spans, head_dim, q.device)
         _call("attn_kv8_tc", "brolm_attn_kv8_tc", _ATTN_TC.pack(
             q.data_ptr(), out.data_ptr(), cu_q.data_ptr(), kv_len.data_ptr(), slots.data_ptr(), tables.data_ptr(), k_pages.data_ptr(),
             v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), part_o, part_ml, _stream(), q0[0], o0[0], T, batch, n_kv, group,
             head_dim, block, n_blocks, S, W, ring, window, max_q_len, spans, scale, cap), what)
         return
-    shares, spans = kv8_shares(batch, n_kv, 1 if rows <= 8 else -(-rows // 16), keys, head_dim, device_sms())
-    part_o = part_ml = 0
+    shares, spans = kv8_shares(batch, n_kv, 1 if rows <= 8 else -(-rows // 16), keys, head_dim, device_sms(), rows > 8)
+    part_o = part_ml = plan = 0
     if spans > 1:
-        parts, part_o, part_ml = _parts(T * n_kv * group * spans, head_dim, q.device)
+        parts, part_o, part_ml, _ = _parts(T * n_kv * group * spans, head_dim, q.device)
+    elif spans < 0:
+        tile = 2 if rows <= 2 else 4 if rows <= 4 else 8 if rows <= 8 else 16
+        parts, part_o, part_ml, plan = _parts(-spans * n_kv * -(-rows // tile) * tile, head_dim, q.device, T * n_kv * group)
     _call("attn_kv8", "brolm_attn_kv8", _ATTN.pack(
         q.data_ptr(), out.data_ptr(), cu_q.data_ptr(), kv_len.data_ptr(), slots.data_ptr(), tables.data_ptr(), k_pages.data_ptr(),
-        v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), part_o, part_ml, _stream(), q0[0], o0[0], _CODES[dt], T, batch,
+        v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), part_o, part_ml, plan, _stream(), q0[0], o0[0], _CODES[dt], T, batch,
         n_kv, group, head_dim, block, n_blocks, S, W, ring, window, max_q_len, shares, spans, scale, cap), what)

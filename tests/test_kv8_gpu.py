@@ -418,6 +418,52 @@ def test_attention_over_long_sequences_is_split_and_joined(dtype):
     compare(c, dtype, [0, 2], [6, 3], 2, 0.125, 50.0, 0)
 
 
+@pytest.fixture(params=[(1, -9), (1, -50), (2, -17), (8, -30)], ids=str)
+def dealt(request, monkeypatch):
+    """Clusters dealt out over the sequences by their lengths: as few as sequences, and more than they have tiles for."""
+    monkeypatch.setattr(kernels.kv8, "KV8_TC_WORK", math.inf)
+    monkeypatch.setattr(kernels.kv8, "kv8_shares", lambda *a: request.param)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D,G,group", [(64, 2, 2), (256, 1, 5), (80, 1, 3)])
+@pytest.mark.parametrize("window", [0, 300])
+def test_attention_dealt_out_by_length(dtype, D, G, group, window, dealt):
+    lens = [3, 900, 140, 1, 257, 64, 500]
+    c = filled(len(lens), 15, G, 64, D, lens, seed=D + window)
+    cap = 30.0 if window else 0.0
+    compare(c, dtype, [4, -1, 0, 6, 1, 3, 2, 5, -1], [1] * 9, group, D ** -0.5, cap, window)
+    compare(c, dtype, [1, 3, 5, 0, 2, -1, 6], [1, 1, 0, 3, 5, 1, 2], group, D ** -0.5, cap, window, seed=1)
+    compare(c, dtype, [6, 2, 1], [20, 1, 33], group, D ** -0.5, cap, window, seed=2)
+    compare(c, dtype, [1], [2], group, D ** -0.5, cap, window, seed=3)
+
+
+@pytest.mark.parametrize("new", [1, 9])
+def test_dealt_out_over_a_ring_with_blocks_that_are_not_numbers(new, dealt):
+    ring = 160
+    c = Cached(3, ring // 32, 2, 32, 64, ring, seed=4)
+    g = torch.Generator().manual_seed(5)
+    k, v = (rows_of(490, 2, 64, torch.float32, g, 0.5) for _ in range(2))
+    k[40, 1, 3], v[483, 0, 9] = NAN, INF                     # (the first sequence's, long overwritten, and the last one's newest block)
+    c.write([0, 1, 2], [400, 30, 60], k, v)
+    for dtype in (torch.bfloat16, torch.float32):
+        got = compare(c, dtype, [2, 0, 1], [new] * 3, 2, 0.125, 0.0, 100)
+        assert torch.isnan(got[:new]).any() and not torch.isnan(got[new:]).any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_sequences_of_very_different_lengths(dtype):
+    """What the rule deals out by itself, up to as many sequences as it does."""
+    lens = [1900, 40, 700, 1, 1300] + [11 * i + 1 for i in range(123)]
+    assert kernels.kv8.kv8_shares(128, 1, 1, 9000, 32, 148)[1] < 0
+    c = filled(len(lens), 30, 1, 64, 32, lens, seed=12)
+    for rows in (list(range(128)), list(range(20)), [3, 0], [0, 1, 2, 3, 4, -1]):
+        compare(c, dtype, rows, [1] * len(rows), 2, 0.2, 0.0, 0, max_kv_len=9000)
+    compare(c, dtype, [0, 1, 2, 4], [1, 7, 9, 2], 2, 0.2, 20.0, 600, max_kv_len=9000)
+    c.lens[1] = 0                                            # (a length of zero: its token sees nothing)
+    compare(c, dtype, [0, 1, 2, 4], [1, 1, 1, 1], 2, 0.2, 0.0, 0, max_kv_len=9000)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("new", [1, 3, 80])
 def test_blocks_that_a_token_does_not_see_change_nothing(dtype, new, either):
@@ -545,6 +591,11 @@ def test_launchers_refuse_sizes():
     with pytest.raises(kernels.KernelError, match="size"):
         kernels.attention_kv8(q, q.clone(), ints([0, 1]), ints([1]), ints([0]), c.tables, *block, n_kv=1, group=1, head_dim=16, scale=1.0,
                               cap=0.0, window=0, ring=0, batch=1, max_q_len=1, max_kv_len=1)
+    with pytest.MonkeyPatch.context() as m:                  # fewer clusters than sequences
+        m.setattr(kernels.kv8, "kv8_shares", lambda *a: (1, -1))
+        with pytest.raises(kernels.KernelError, match="size"):
+            kernels.attention_kv8(q.repeat(2, 1), q.repeat(2, 1), ints([0, 1, 2]), ints([1, 1]), ints([0, 0]), c.tables, *c.dev, n_kv=1, group=1,
+                                  head_dim=16, scale=1.0, cap=0.0, window=0, ring=0, batch=2, max_q_len=1, max_kv_len=1)
     k = torch.zeros((2, 1, 16), device=DEV)
     off = torch.zeros(40, device=DEV)[1:33].view(2, 1, 16)
     with pytest.raises(kernels.KernelError, match="aligned"):
