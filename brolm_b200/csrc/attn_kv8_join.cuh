@@ -36,16 +36,20 @@ struct JoinArgs {
     int out_stride, rows, tokens, heads, dim, spans;
     const int2* plan = nullptr;           // where given, [token][head]: the first part and how many, every `step` parts
     int step = 1, parts = 0;              // (the parts that there are: nothing is read beyond them)
+    bool some = false;                    // some rows are in their places: their first part's sum is -1
 };
 
-// Rows whose keys were shared by several blocks that do not join their results themselves: a block of threads for every
+// Rows whose keys were shared by several blocks that do not join their results themselves: a thread for four entries of a
 // (token, head) adds up its parts in their order,  out = sum_s o_s 2^(m_s - m) / sum_s l_s 2^(m_s - m).
+constexpr int JOIN_THREADS = 256;
 template <typename T>
-__global__ void __launch_bounds__(64) attn_kv8_join_kernel(JoinArgs a) {
+__global__ void __launch_bounds__(JOIN_THREADS) attn_kv8_join_kernel(JoinArgs a) {
     pdl_trigger();
     pdl_wait();
-    const int tok = blockIdx.x, head = blockIdx.y;
-    if (tok >= a.cu_q[a.rows]) return;
+    const int per = a.dim >> 2, mine = threadIdx.x / per, d = (threadIdx.x - mine * per) * 4;
+    const long long row = (long long)blockIdx.x * (JOIN_THREADS / per) + mine;
+    const int tok = (int)(row / a.heads), head = (int)(row - (long long)tok * a.heads);
+    if (mine >= JOIN_THREADS / per || tok >= min(a.tokens, a.cu_q[a.rows])) return;
     size_t at = ((size_t)tok * a.heads + head) * a.spans;
     int spans = a.spans;
     if (a.plan) {
@@ -54,9 +58,8 @@ __global__ void __launch_bounds__(64) attn_kv8_join_kernel(JoinArgs a) {
         spans = p.y;
         if (spans <= 1 || p.x < 0 || p.x + (long long)(spans - 1) * a.step >= a.parts) return;     // (one part is in its place)
     }
+    if (a.some && a.part_ml[at * 2 + 1] < 0.0f) return;
     const size_t step = a.step;
-    const int d = threadIdx.x * 4;
-    if (d >= a.dim) return;
     float most = -INFINITY, sum = 0.0f;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (int s0 = 0; s0 < spans; s0 += 8) {                  // (eight parts are asked for at once)
@@ -86,7 +89,9 @@ __global__ void __launch_bounds__(64) attn_kv8_join_kernel(JoinArgs a) {
 
 template <typename T>
 int launch_join(const JoinArgs& a, cudaStream_t stream) {
-    return launch_pdl(attn_kv8_join_kernel<T>, dim3(a.tokens, a.heads), dim3(64), 0, stream, a);
+    const long long rows = (long long)a.tokens * a.heads, each = JOIN_THREADS / (a.dim >> 2), blocks = (rows + each - 1) / each;
+    if (blocks > 0x7fffffffll) return BROLM_ERR_TOO_LARGE;
+    return launch_pdl(attn_kv8_join_kernel<T>, dim3((unsigned)blocks), dim3(JOIN_THREADS), 0, stream, a);
 }
 
 }  // namespace kv8

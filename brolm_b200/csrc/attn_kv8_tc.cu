@@ -73,7 +73,8 @@ struct TcArgs {
     const float *k_scale, *v_scale;
     int tokens, rows, n_kv, group, block, n_blocks, n_slots, width, ring, window, row_tiles, wide;
     float scale, cap;
-    int spans;                            // blocks that share a row tile's keys; more than one: joined by a second launch
+    int whole, spans;                     // the first `whole` row tiles have a block each, the others' keys are shared by `spans`,
+                                          // whose parts a second launch joins
     float *part_o, *part_ml;
 };
 
@@ -87,12 +88,12 @@ struct Shape {
 };
 
 // barriers
-enum : int { S_FULL = 0, P_FULL = 2, PV_DONE = 4, META_FULL = 6, META_EMPTY = 8, U_FULL = 10 };
+enum : int { S_FULL = 0, P_FULL = 2, PV_DONE = 4, META_FULL = 6, META_EMPTY = 8, Q_FULL = 10, U_FULL = 11 };
 
 struct Meta {                             // of a group of 32 keys
     int row;                              // the group's first row in the pages
     float k_scale;
-    int v_exp;                            // exponent of the value scale less e0; BAD: a scale that is NaN
+    int v_exp;                            // exponent of the value scale; BAD: a scale that is NaN
 };
 constexpr int BAD = 0x7fffffff;
 
@@ -105,7 +106,8 @@ __device__ __forceinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile 
 template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 // Waits that are mostly over when they begin: the limit and the flags are looked at only if they are not (which takes 190
-// cycles).  Only the softmax warps' waits, codes 8 and 9, can be stalled by brolm_attn_kv8_tc_wait_control at any time.
+// cycles).  Only the softmax warps' waits, codes 8 and 9, and that for the queries,
+// 15, can be stalled by brolm_attn_kv8_tc_wait_control at any time.
 __device__ __forceinline__ bool wait_one(uint32_t bar, uint32_t parity, volatile int* give_up, int code) {
     return mbar_try(bar, parity) || wait_on(bar, parity, give_up, code);
 }
@@ -207,7 +209,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
     uint64_t* bars = reinterpret_cast<uint64_t*>(q_scale + BM);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + U_FULL + 2 * SLOTS + 2 * RAWS);
     volatile int* give_up = reinterpret_cast<volatile int*>(tmem_slot + 1);       // three
-    int* top_exp = reinterpret_cast<int*>(tmem_slot + 4);
+    volatile int* top_exp = reinterpret_cast<volatile int*>(tmem_slot + 4);
     const uint32_t bar0 = smem_u32(bars);
     auto bar = [&](int i) { return bar0 + 8u * i; };
     auto u_full = [&](int sl) { return bar0 + 8u * (U_FULL + sl); };
@@ -218,8 +220,13 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_wait();
     // blocks start in the order of their index: the last rows, which see the most keys, of every sequence and head first
-    const int per = a.n_kv * a.rows * a.spans;
-    const int xt = a.row_tiles - 1 - (int)(blockIdx.x / per), which = blockIdx.x % per / a.spans, span = blockIdx.x % a.spans;
+    int item = blockIdx.x, span = 0, spans = 1;
+    if (item >= a.whole) {
+        span = (item - a.whole) % a.spans;
+        item = a.whole + (item - a.whole) / a.spans;
+        spans = a.spans;
+    }
+    const int per = a.n_kv * a.rows, xt = a.row_tiles - 1 - item / per, which = item % per;
     const int b = which / a.n_kv, g = which - b * a.n_kv;
     const int first_tok = a.cu_q[b], n_tok = min(a.cu_q[b + 1], a.tokens) - first_tok;
     const int kv_len = a.kv_len[b], slot = a.slots[b];
@@ -232,7 +239,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
     if (pos_hi >= 0 && slot >= 0 && slot < a.n_slots) {
         t_first = max(0, pos_lo - window + 1) / BN;
         n_tiles = pos_hi / BN - t_first + 1;
-        const int share = (n_tiles + a.spans - 1) / a.spans;
+        const int share = (n_tiles + spans - 1) / spans;
         t_first += span * share;
         n_tiles = max(0, min(share, n_tiles - span * share));
     }
@@ -247,6 +254,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
             mbar_init(bar(META_FULL + s), 1);
             mbar_init(bar(META_EMPTY + s), SOFTMAX_WARPS + 2);
         }
+        mbar_init(bar(Q_FULL), 1);
         for (int s = 0; s < SLOTS; ++s) {
             mbar_init(u_full(s), CONVERT_WARPS);
             mbar_init(u_empty(s), 1);
@@ -262,7 +270,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
         mbar_init_fence();
     }
     if (warp == ISSUER) tmem_alloc(smem_u32(tmem_slot), TMEM_COLS);
+    fence_before_sync();
     __syncthreads();
+    fence_after_sync();
+    const uint32_t tmem = *tmem_slot;
     // where a key's block is, from its place in units of 32 (a block is a multiple of that)
     const int block32 = a.block >> 5;
     auto block_of = [&](int place32) -> int {
@@ -270,58 +281,6 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
         const int id = e < a.width ? table[e] : 0;
         return id >= 0 && id < a.n_blocks ? id : 0;          // (never followed out of the cache)
     };
-    if (n_tiles > 0) {
-        // e0: the largest exponent among the value scales of the keys that this block sees
-        const int first32 = t_first * (BN / 32), n32 = key_hi / 32 - first32 + 1;
-        int top = -126;
-        for (int i = threadIdx.x; i * block32 < n32 + block32; i += THREADS) {
-            const int at = min(first32 + i * block32, key_hi / 32);
-            const float s = a.v_scale[(size_t)block_of(a.ring > 0 ? at % (a.ring >> 5) : at) * a.n_kv + g];
-            if (s == s) top = max(top, (int)(__float_as_uint(s) >> 23 & 255u) - 127);
-        }
-        top = __reduce_max_sync(0xffffffffu, top);
-        if (lane == 0 && top > -126) atomicMax(top_exp, top);
-    }
-    // the queries: a warp a row, eight entries a lane, rows of 128 bytes per 64 entries, pieces of 16 bytes swizzled
-    for (int r = warp; r < BM; r += THREADS / 32) {
-        float v[8] = {};
-        if (r < rows_here && lane * 8 < HD) {
-            const int row = row0 + r;
-            const bf16* src = a.q + (size_t)(first_tok + row / a.group) * a.q_stride + (g * a.group + row % a.group) * HD + lane * 8;
-            if (a.wide) load8(src, v);
-            else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = to_float(src[e]);
-            }
-        }
-        float most = 0.0f;
-        bool finite = true;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            most = fmaxf(most, fabsf(v[e]));
-            finite = finite && fabsf(v[e]) < INFINITY;
-        }
-        most = warp_max(most);
-        finite = __all_sync(0xffffffffu, finite);
-        const int up = max(min(13 + 127 - (int)(__float_as_uint(most) >> 23), 120), -126);
-        const float f = power_of_two(up);
-        if (lane == 0) q_scale[r] = finite ? power_of_two(-up) : __int_as_float(0x7fc00000);
-        if (lane * 8 < HD) {
-            uint32_t h[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const __half2 t = __floats2half2_rn(finite ? v[2 * e] * f : 0.0f, finite ? v[2 * e + 1] * f : 0.0f);
-                h[e] = *reinterpret_cast<const uint32_t*>(&t);
-            }
-            st_shared16(q_s + (lane >> 3) * (BM * 128) + r * 128 + (((lane & 7) ^ (r & 7)) << 4), h[0], h[1], h[2], h[3]);
-        }
-    }
-    fence_proxy_async();
-    fence_before_sync();
-    __syncthreads();
-    fence_after_sync();
-    const uint32_t tmem = *tmem_slot;
-    const int e0 = *top_exp;
 
     if (warp >= ISSUER) {
         fewer_registers<OTHER_REGS>();
@@ -336,7 +295,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
                     x.row = (int)bh * a.block + (place32 % block32) * 32;
                     x.k_scale = a.k_scale[bh];
                     const float sv = a.v_scale[bh];
-                    x.v_exp = max((int)(__float_as_uint(sv) >> 23 & 255u) - 127, -126) - e0;
+                    x.v_exp = max((int)(__float_as_uint(sv) >> 23 & 255u) - 127, -126);
                     if (x.k_scale != x.k_scale || sv != sv) {
                         x.k_scale = 0.0f;
                         x.v_exp = BAD;
@@ -367,7 +326,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
                     umma_commit(bar(S_FULL + s));
                     return true;
                 };
-                bool ok = issue_qk(0);
+                bool ok = wait_on(bar(Q_FULL), 0, give_up, 15) && issue_qk(0);
                 for (int j = 0; j < n_tiles && ok; ++j) {
                     if (j + 1 < n_tiles) { ok = issue_qk(j + 1); if (!ok) break; }
                     const int s = j & 1;
@@ -477,6 +436,69 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
         }
     } else {
         more_registers<SOFTMAX_REGS>();
+        // While the first tiles are on their way: e0, the largest exponent among the value scales of the keys that this block
+        // sees, and the queries, a warp a row, eight entries a lane, rows of 128 bytes per 64 entries, pieces of 16 bytes
+        // swizzled.  (Done by all warps before the roles part: 64 tokens on 4,096 keys 30.0 us for 27.0, 2,048 on 2,048 77.1
+        // for 74.2.)
+        constexpr int Q_ROWS = BM / SOFTMAX_WARPS / 2;
+#pragma unroll 1
+        for (int r0 = warp; r0 < BM; r0 += BM / 2) {
+            uint4 raw[Q_ROWS];
+#pragma unroll
+            for (int i = 0; i < Q_ROWS; ++i) {
+                const int r = r0 + i * SOFTMAX_WARPS, row = row0 + r;
+                raw[i] = make_uint4(0u, 0u, 0u, 0u);
+                if (r < rows_here && lane * 8 < HD) {
+                    const bf16* src = a.q + (size_t)(first_tok + row / a.group) * a.q_stride + (g * a.group + row % a.group) * HD + lane * 8;
+                    if (a.wide) raw[i] = *reinterpret_cast<const uint4*>(src);
+                    else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) reinterpret_cast<bf16*>(&raw[i])[e] = src[e];
+                    }
+                }
+            }
+            if (n_tiles > 0 && r0 == warp) {
+                const int first32 = t_first * (BN / 32), n32 = key_hi / 32 - first32 + 1;
+                int top = -126;
+                for (int i = threadIdx.x; i * block32 < n32 + block32; i += 32 * SOFTMAX_WARPS) {
+                    const int at = min(first32 + i * block32, key_hi / 32);
+                    const float s = a.v_scale[(size_t)block_of(a.ring > 0 ? at % (a.ring >> 5) : at) * a.n_kv + g];
+                    if (s == s) top = max(top, (int)(__float_as_uint(s) >> 23 & 255u) - 127);
+                }
+                top = __reduce_max_sync(0xffffffffu, top);
+                if (lane == 0 && top > -126) atomicMax(const_cast<int*>(top_exp), top);
+            }
+#pragma unroll
+            for (int i = 0; i < Q_ROWS; ++i) {
+                const int r = r0 + i * SOFTMAX_WARPS;
+                float v[8], most = 0.0f;
+                bool finite = true;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    v[e] = to_float(reinterpret_cast<const bf16*>(&raw[i])[e]);
+                    most = fmaxf(most, fabsf(v[e]));
+                    finite = finite && fabsf(v[e]) < INFINITY;
+                }
+                most = warp_max(most);
+                finite = __all_sync(0xffffffffu, finite);
+                const int up = max(min(13 + 127 - (int)(__float_as_uint(most) >> 23), 120), -126);
+                const float f = power_of_two(up);
+                if (lane == 0) q_scale[r] = finite ? power_of_two(-up) : __int_as_float(0x7fc00000);
+                if (lane * 8 < HD) {
+                    uint32_t h[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const __half2 t = __floats2half2_rn(finite ? v[2 * e] * f : 0.0f, finite ? v[2 * e + 1] * f : 0.0f);
+                        h[e] = *reinterpret_cast<const uint32_t*>(&t);
+                    }
+                    st_shared16(q_s + (lane >> 3) * (BM * 128) + r * 128 + (((lane & 7) ^ (r & 7)) << 4), h[0], h[1], h[2], h[3]);
+                }
+            }
+        }
+        fence_proxy_async();
+        asm volatile("bar.sync 5, %0;" ::"n"(32 * SOFTMAX_WARPS) : "memory");
+        if (threadIdx.x == 0) mbar_arrive(bar(Q_FULL));
+        const int e0 = *top_exp;
         // Four warps share each quarter of the rows (a warp may only touch the 32 lanes of tensor memory of its quarter), 32
         // score columns each.  They agree on the rows' reference maxima through shared memory and a barrier of their own.
         constexpr int W = BN / 4, OUT = HD / 4;
@@ -498,7 +520,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
             if (ok && j % CHUNK == 0) ok = wait_warp(bar(META_FULL + ((j / CHUNK) & 1)), (j / CHUNK >> 1) & 1, give_up, 9);
             const Meta& m = meta[((j / CHUNK) & 1) * CHUNK * 4 + (j % CHUNK) * 4 + part];
             const float f = m.k_scale * unit;
-            int ve = m.v_exp;
+            int ve = m.v_exp == BAD ? BAD : m.v_exp - e0;
             if (ok) ok = wait_warp(bar(S_FULL + s), (j >> 1) & 1, give_up, 8);
             fence_after_sync();
             const int key_base = (t_first + j) * BN, kp0 = key_base + part * W;
@@ -625,7 +647,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
             const int row = row0 + r, tok = first_tok + row / a.group, head = g * a.group + row % a.group;
             bf16* dst = a.out + (size_t)tok * a.out_stride + (size_t)head * HD;
             const size_t share = ((size_t)tok * a.n_kv * a.group + head) * a.spans + span;
-            if (a.spans > 1 && row_ok && part == 0) *reinterpret_cast<float2*>(a.part_ml + share * 2) = make_float2(m_ref, total);
+            if (a.spans > 1 && row_ok && part == 0)          // (a row that is in its place: a sum that cannot be)
+                *reinterpret_cast<float2*>(a.part_ml + share * 2) = spans > 1 ? make_float2(m_ref, total) : make_float2(-INFINITY, -1.0f);
             const bool wide = ((uintptr_t)a.out & 15) == 0 && (a.out_stride & 7) == 0;
 #pragma unroll 1
             for (int c = part * OUT; c < (part + 1) * OUT; c += 16) {
@@ -634,7 +657,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
                     tmem_ld16(lane_addr + O_COL + c, ov);
                     tmem_wait_ld();
                 }
-                if (row_ok && a.spans > 1) {
+                if (row_ok && spans > 1) {
 #pragma unroll
                     for (int i = 0; i < 16; i += 4) {
                         float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -692,7 +715,7 @@ int launch(const TcArgs& a, cudaStream_t stream) {
     static OncePerDevice raised;
     int st = allow_shared_memory(attn_kv8_tc_kernel<HD>, smem, raised);
     if (st) return st;
-    const long long blocks = (long long)a.row_tiles * a.n_kv * a.rows * a.spans, rows = (long long)a.n_blocks * a.n_kv * a.block;
+    const long long blocks = a.whole + ((long long)a.row_tiles * a.n_kv * a.rows - a.whole) * a.spans, rows = (long long)a.n_blocks * a.n_kv * a.block;
     if (blocks > 0x7fffffffll || rows > 0x7fffffffll) return BROLM_ERR_TOO_LARGE;
     CUtensorMap mk, mv;
     st = make_map(&mk, a.k_pages, rows, HD, 64);
@@ -701,7 +724,11 @@ int launch(const TcArgs& a, cudaStream_t stream) {
     if (st) return st;
     st = launch_pdl(attn_kv8_tc_kernel<HD>, dim3((unsigned)blocks), dim3(THREADS), smem, stream, mk, mv, a);
     if (st || a.spans == 1) return st;
-    return launch_join<bf16>(JoinArgs{a.part_o, a.part_ml, a.out, a.cu_q, a.out_stride, a.rows, a.tokens, a.n_kv * a.group, HD, a.spans}, stream);
+    JoinArgs j{a.part_o, a.part_ml, a.out, a.cu_q, a.out_stride, a.rows, a.tokens, a.n_kv * a.group, HD, a.spans};
+    j.some = a.whole > 0;
+    if (a.rows == 1)                      // (one sequence: the tiles that are shared are those of its first tokens)
+        j.tokens = min(a.tokens, ((a.row_tiles - a.whole / a.n_kv) * BM + a.group - 1) / a.group);
+    return launch_join<bf16>(j, stream);
 }
 
 }  // namespace
@@ -710,9 +737,9 @@ struct AttnTcCall {
     const void* q;
     void* out;
     const void *cu_q, *kv_len, *slots, *tables, *k_pages, *v_pages, *k_scale, *v_scale;
-    void *part_o, *part_ml;               // spans > 1: [tokens * n_kv * group * spans * dim] and [.. * 2]
+    void *part_o, *part_ml;               // spans > 1, for all row tiles but the first `whole`: [tokens * n_kv * group * spans * dim] and [.. * 2]
     cudaStream_t stream;
-    int q_stride, out_stride, tokens, rows, n_kv, group, dim, block, n_blocks, n_slots, width, ring, window, max_q_len, spans;
+    int q_stride, out_stride, tokens, rows, n_kv, group, dim, block, n_blocks, n_slots, width, ring, window, max_q_len, whole, spans;
     float scale, cap;
 };
 
@@ -727,11 +754,15 @@ BROLM_API int brolm_attn_kv8_tc(const AttnTcCall* c) {
     if (c->spans < 1 || (c->spans > 1 && (!c->part_o || !c->part_ml))) return BROLM_ERR_BAD_SIZE;
     if (((uintptr_t)c->k_pages | (uintptr_t)c->v_pages | (uintptr_t)c->part_o) & 15) return BROLM_ERR_ALIGNMENT;
     if (c->tokens == 0 || c->rows == 0) return BROLM_OK;
+    const int row_tiles = (c->max_q_len * group + BM - 1) / BM;
+    const long long items = (long long)row_tiles * n_kv * c->rows;
+    if (items > 0x7fffffffll) return BROLM_ERR_TOO_LARGE;
+    if (c->whole < 0 || c->whole > items) return BROLM_ERR_BAD_SIZE;
     const int wide = ((uintptr_t)c->q & 15) == 0 && c->q_stride % 8 == 0;
     TcArgs a{(const bf16*)c->q, (bf16*)c->out, c->q_stride, c->out_stride, (const int32_t*)c->cu_q, (const int32_t*)c->kv_len,
              (const int32_t*)c->slots, (const int32_t*)c->tables, (const int8_t*)c->k_pages, (const int8_t*)c->v_pages,
              (const float*)c->k_scale, (const float*)c->v_scale, c->tokens, c->rows, n_kv, group, block, c->n_blocks, c->n_slots,
-             c->width, c->ring, c->window, (c->max_q_len * group + BM - 1) / BM, wide, c->scale, c->cap, c->spans, (float*)c->part_o, (float*)c->part_ml};
+             c->width, c->ring, c->window, row_tiles, wide, c->scale, c->cap, c->whole, c->spans, (float*)c->part_o, (float*)c->part_ml};
     if (c->dim == 64) return launch<64>(a, c->stream);
     if (c->dim == 128) return launch<128>(a, c->stream);
     return launch<256>(a, c->stream);

@@ -41,7 +41,7 @@ _RELEASE = struct.Struct("@7P4i")
 _WRITE = struct.Struct("@10P4q8i")
 _READ = struct.Struct("@11P4q10i")
 _ATTN = struct.Struct("@14P17i2f")
-_ATTN_TC = struct.Struct("@13P15i2f")
+_ATTN_TC = struct.Struct("@13P16i2f")
 _functions: dict = {}
 _NO_CPU = "brolm_b200 kernels run on CUDA tensors only; there is no CPU path"
 
@@ -260,17 +260,29 @@ def _parts(n: int, head_dim: int, device, plans: int = 0) -> tuple:
 
 
 @functools.lru_cache(maxsize=256)
-def kv8_tc_spans(tokens: int, batch: int, n_kv: int, group: int, max_q_len: int, keys: int, head_dim: int, sms: int) -> int:
-    """How many blocks share the keys of a tile of 128 query rows on tcgen05: one block runs on an SM, so what counts is how
-    many rounds of blocks there are and how long a block's share is.  In tiles of 128 keys (3 us each at 256 entries): a
-    block begins and ends in three, and joining costs another three and what the parts take to memory and back."""
+def kv8_tc_spans(tokens: int, batch: int, n_kv: int, group: int, max_q_len: int, keys: int, head_dim: int, sms: int) -> tuple[int, int]:
+    """How many of the tiles of 128 query rows have a block each on tcgen05, and how many blocks share the keys of each of the
+    others: one block runs on an SM, so what counts is how many rounds of blocks there are and how long a block's share is.
+    In tiles of 128 keys (3 us each at 256 entries): a block begins and ends in three, and joining costs another three and
+    what the parts take to memory and back.  Where the last round would be far from full, its tiles alone are shared
+    (on 14,336 keys, 8 kv heads of 256, two query heads each, us with a block for a tile / four / the last round's
+    shared: 1,280 tokens, 160 tiles on 148 SMs, 644 / 502 / 400; 1,700, 216 tiles, 656 / 616 / 535; 2,048, 256, 657 / 715 / 657)."""
     items = batch * n_kv * -(-max_q_len * group // 128)
     tiles = -(-keys // 128)
     traffic = tokens * n_kv * group * head_dim * 8 / 6.5e12 / (3e-6 * head_dim / 256)
 
-    def cost(k):
-        return -(-items * k // sms) * (-(-tiles // k) + 3) + (3 + k * traffic if k > 1 else 0)
-    return min(range(1, max(2, min(32, tiles // 2) + 1)), key=cost)
+    def cost(choice):
+        whole, k = choice
+        t = -(-whole // sms) * (tiles + 3)
+        if k > 1:
+            t += -(-(items - whole) * k // sms) * (-(-tiles // k) + 3) + 3 + k * traffic * (items - whole) / items
+        return t
+    most = min(32, tiles // 2)
+    full = items // sms * sms
+    choices = [(items, 1)] + [(0, k) for k in range(2, most + 1)]
+    if tokens == batch * max_q_len and 0 < full < items:
+        choices += [(full, k) for k in range(2, most + 1)]
+    return min(choices, key=cost)
 
 
 # From how many rows of a kv head (tokens x query heads), and from how many of rows x kv heads x keys x entries, a step of
@@ -323,14 +335,14 @@ def attention_kv8(q: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, kv_len
     keys = min(max_kv_len, window + max_q_len) if window > 0 else max_kv_len
     if rows >= KV8_TC_ROWS and dt is torch.bfloat16 and head_dim in (64, 128, 256) and n_blocks * n_kv * block < 1 << 31 and \
             float(T) * group * n_kv * keys * head_dim >= KV8_TC_WORK:
-        spans = kv8_tc_spans(T, batch, n_kv, group, max_q_len, keys, head_dim, device_sms())
+        whole, spans = kv8_tc_spans(T, batch, n_kv, group, max_q_len, keys, head_dim, device_sms())
         part_o = part_ml = 0
         if spans > 1:
             parts, part_o, part_ml, _ = _parts(T * n_kv * group * spans, head_dim, q.device)
         _call("attn_kv8_tc", "brolm_attn_kv8_tc", _ATTN_TC.pack(
             q.data_ptr(), out.data_ptr(), cu_q.data_ptr(), kv_len.data_ptr(), slots.data_ptr(), tables.data_ptr(), k_pages.data_ptr(),
             v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), part_o, part_ml, _stream(), q0[0], o0[0], T, batch, n_kv, group,
-            head_dim, block, n_blocks, S, W, ring, window, max_q_len, spans, scale, cap), what)
+            head_dim, block, n_blocks, S, W, ring, window, max_q_len, whole, spans, scale, cap), what)
         return
     shares, spans = kv8_shares(batch, n_kv, 1 if rows <= 8 else -(-rows // 16), keys, head_dim, device_sms(), rows > 8)
     part_o = part_ml = plan = 0

@@ -669,7 +669,28 @@ def test_a_piece_whose_values_scales_lie_2_to_the_100_apart(on_tcgen05):
     compare(c, torch.bfloat16, [0], [192], 1, 0.125, 0.0, 0)
 
 
-@pytest.mark.parametrize("code", [8, 9])
+@pytest.mark.parametrize("shared", [(0, 3), (1, 2), (5, 4), (7, 30)], ids=str)
+@pytest.mark.parametrize("D,window", [(64, 0), (256, 0), (128, 90)])
+def test_a_piece_some_of_whose_tiles_are_shared(D, window, shared, on_tcgen05, monkeypatch):
+    """The first tiles with a block each, the others' keys shared by several; tokens before a sequence's first, and a query
+    that is not a number, on both sides."""
+    monkeypatch.setattr(kernels.kv8, "kv8_tc_spans", lambda *a: shared)
+    c = filled(3, 12, 2, 64, D, [700, 150, 333], seed=D)
+    compare(c, torch.bfloat16, [0], [260], 2, D ** -0.5, 25.0, window)                       # (ten tiles)
+    compare(c, torch.bfloat16, [2, 0, 1], [130, 70, 150], 2, D ** -0.5, 0.0, window)         # (eighteen)
+    c.lens[1] = 60                                           # of 150 new tokens 90 come before the first
+    compare(c, torch.bfloat16, [1], [150], 3, D ** -0.5, 0.0, window)
+    c.lens[1] = 150
+    q = torch.randn((260, 4 * D), generator=torch.Generator().manual_seed(1)).bfloat16().to(DEV)
+    q[3, 5] = q[200, 3 * D] = NAN
+    out = torch.empty_like(q)
+    kernels.attention_kv8(q, out, ints([0, 260]), ints([700]), ints([0]), c.tables, *c.dev, n_kv=2, group=2, head_dim=D, scale=0.1, cap=0.0,
+                          window=window, ring=0, batch=1, max_q_len=260, max_kv_len=700)
+    bad = torch.isnan(out)
+    assert bool(bad[3, :D].all()) and bool(bad[200, 3 * D:].all()) and int(bad.sum()) == 2 * D
+
+
+@pytest.mark.parametrize("code", [8, 9, 15])
 def test_a_piece_whose_wait_runs_out(code, on_tcgen05):
     """The softmax warps' waits for a score tile and for the lookups never end: the launch gives up, says so, and the next
     one is right."""
