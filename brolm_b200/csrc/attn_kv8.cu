@@ -4,24 +4,20 @@
 //     z = scale * q . k,   cap tanh(z / cap),   key j visible from position p iff 0 <= p - j < window,
 //     out = sum_j softmax_j(z) v_j,   zeros where a token sees no key.
 //
-// A row is a (token, query head of the group) pair; a block of threads owns 8 or 16 rows of one (sequence, kv head) and a
+// A row is a (token, query head of the group) pair; a block of threads owns 2 to 16 rows of one (sequence, kv head) and a
 // share of its keys, and its four warps take tiles of 32 keys in turn.  A tile lies inside one cache block, so it has one
 // scale for its keys and one for its values:
 //
 //     S^T [32 keys x rows] = K q^T,    m_t = max over the tile,  p = 2^(z - m_t),    O^T += s_v 2^(m_t - m) (V^T p)
 //
-// Both products run on mma.sync (f16, float sums) with the cache's numbers as the left operand, where the 16 rows of an
-// instruction are keys or entries of a head and its 8 columns are query rows, so that two to eight query heads waste
-// little.  int8 becomes f16 exactly and without a conversion instruction: 1024 + 128 + q has the bits 0x6400 | (q + 128),
-// one byte permutation makes two of them and one subtraction takes 1152 away.  The weights of a tile are relative to the
-// tile's own maximum and its sums are scaled in 32 bits when they join the row's, so blocks whose scales differ by any
-// factor keep all their bits.  A query row is scaled by a power of two to below 2^14, so that it is held by one f16 a
-// number (bfloat16 queries, exactly but for numbers 2^-38 of the row's largest) or two (float32: 22 bits or more).
-// Weights are one f16 (bfloat16) or two (float32).
+// The weights of a tile are relative to the tile's own maximum and its sums are scaled in 32 bits when they join the row's,
+// so blocks whose scales differ by any factor keep all their bits.  Both products run on mma.sync with the cache's numbers as
+// the left operand, where the 16 rows of an instruction are keys or entries of a head and its 8 columns are query rows or
+// their digits: whole numbers for up to eight rows, f16 for more (each at its kernel below).
 //
-// What bounds it is reading the cache: a tile of 32 keys of 256 entries is 16 KB and some 1,200 instructions of a warp,
-// 300 cycles of an SM's four schedulers, while an SM's share of the memory's rate brings 16 KB in 700.  Every warp keeps a
-// ring of its own of key and value tiles in flight (cp.async, no barrier but its own), two blocks on an SM.
+// What bounds it is reading the cache, with 16 KB in flight a warp, 128 an SM: every warp keeps a ring of its own of key and
+// value tiles on their way (cp.async, no barrier but its own), two blocks on an SM.  A launch takes 7 us more than its bytes:
+// three round trips to memory before the first product, the warps' and the cluster's merge behind the last.
 //
 // The shares of a row's keys are joined inside the launch: they form a cluster, whose blocks read each other's partial
 // results out of shared memory.  Where that is not enough, or where clusters are dealt out over sequences of different
@@ -466,6 +462,11 @@ __device__ __forceinline__ void merge(const AttnArgs& a, const Item& it, const f
 // A thread has two neighbouring digits' sums, joins them as whole numbers (below 2^31: 127 * 255 * 256 * 33 in both
 // products) and then in floats.  The keys are read as the instruction wants them; of the values, four keys' bytes of an
 // entry are gathered into a word by eight byte permutations for sixteen bytes.
+//
+// 8 sequences of 8,192 keys, 4 kv heads of 256, two query heads each, bfloat16: 29.2 us, 4.6 TB/s, with 28 % of the issue
+// slots and 7 % of the tensor pipe in use (f16 products: 30.2, and for 16 sequences of unequal lengths under a window 45.6
+// where these took 32.6 with the same shares); 1 of 1,280: 7.6 us, which is round trips.  A fixed number of blocks that walk
+// runs of equal length over all sequences took 38.8: each further sequence of a block costs 5 us of round trips.
 __device__ __forceinline__ void mma_s8(int (&d)[4], const uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -756,6 +757,16 @@ __global__ void __launch_bounds__(THREADS, 2) attn_kv8_few_kernel(AttnArgs a) {
 }
 
 // --- more rows: f16 products, 16 rows a block ---------------------------------------------------------------------------
+//
+// int8 becomes f16 exactly and without a conversion instruction: 1024 + 128 + q has the bits 0x6400 | (q + 128), one byte
+// permutation makes two of them and one subtraction takes 1152 away.  A query row is scaled by a power of two to below 2^14,
+// so that it is held by one f16 a number (bfloat16 queries, exactly but for numbers 2^-38 of the row's largest) or two
+// (float32: 22 bits or more).  Weights are one f16 (bfloat16) or two (float32).
+//
+// What bounds it is a warp's own chain, 1.8 us a tile of 32 keys of 128 entries in float32 (128 products, as many bytes to
+// turn, two exponentials and a tanh a score) with one or two warps a scheduler: 6 sequences of 13 to 4,001 keys with five
+// tokens each, 4 kv heads of 128, four query heads each, float32, take 22.0 us (21.0 in bfloat16, 24.3 without the cap, as
+// 5 x 1 shares of the longest 26.5).
 
 template <typename T, int DP>
 struct Shape {

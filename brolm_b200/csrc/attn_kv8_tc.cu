@@ -31,9 +31,11 @@
 // would be passed by more than 8: the accumulator in tensor memory is then scaled anew.)  A query row is scaled by a power
 // of two to below 2^14 and held in f16, exactly but for numbers 2^-38 of the row's largest.
 //
-// What bounds it: a tile of 128 keys and 256 entries takes the tensor core 2,770 cycles, the 3 x 16,384 exponentials and
-// reciprocals of a capped softmax 3,070 cycles of the special function units, and the instructions of softmax and of
-// turning bytes into f16 about 2,400 issue cycles of each scheduler.
+// What bounds it: of a tile of 128 keys and 256 entries, about 5,600 cycles (2,048 tokens on 14,336 keys, 8 kv heads of 256,
+// two query heads each: 638 to 657 us, 680 to 700 TFLOP/s of 1,700), the tensor core takes 2,770, shared memory 3,500 (bytes
+// in, f16 out, f16 to the tensor core: 448 KB), the softmax of a row's scores and then of its weights, which wait for each
+// other and for the products, 1,700 and 1,200, and the instructions of all roles 57 % of the issue slots.  Two sets of softmax
+// warps that take turns on tiles were slower (845 us): the scores of a tile wait for the values of the tile before the last.
 //
 // Every mbarrier wait is bounded; a wait that runs out records a code that brolm_attn_kv8_tc_status() returns, and the
 // launch ends without its results.

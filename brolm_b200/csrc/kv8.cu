@@ -196,7 +196,7 @@ struct ReadArgs {
 constexpr int READ_TOKENS = 8;
 
 // The last n_i = cu_r[i + 1] - cu_r[i] tokens of row i, back to back; what the ring no longer holds reads as zero.  A thread
-// makes sixteen numbers from sixteen bytes.  Bounded by the memory: 53,144 bfloat16 tokens of 8 heads of 256 (327 MB) in 57.1
+// makes sixteen numbers from sixteen bytes.  Bounded by the memory: 26,575 bfloat16 tokens of 8 heads of 256 (327 MB) in 57.1
 // us, 5.7 TB/s, 0.87 of a copy's rate.  Eight bytes a thread, so that its store fills half a sector by itself, took 97 us, and
 // two threads that swap halves, so that each store of theirs fills one, 69.
 template <typename T>
