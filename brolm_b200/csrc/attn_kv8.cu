@@ -193,7 +193,7 @@ __device__ __forceinline__ void deal(const AttnArgs& a, int c, Item& it, int& en
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
         const int pos0 = len[j] - (min(end[j], a.tokens) - first[j]), from = a.window > 0 ? max(0, pos0 - a.window + 1) / KT : 0;
-        work[j] = lane + 32 * j < a.rows ? max(1, ((max(0, len[j] - 1) / KT - from + 1) + round - 1) / round) : 0;
+        work[j] = lane + 32 * j < a.rows ? min(1 << 20, max(1, ((max(0, len[j] - 1) / KT - from + 1) + round - 1) / round)) : 0;
         total += work[j];
         most = max(most, work[j]);
     }

@@ -73,7 +73,7 @@ struct TcArgs {
     const int32_t *cu_q, *kv_len, *slots, *tables;
     const int8_t *k_pages, *v_pages;
     const float *k_scale, *v_scale;
-    int tokens, rows, n_kv, group, block, n_blocks, n_slots, width, ring, window, row_tiles, wide;
+    int tokens, rows, n_kv, group, dim, block, n_blocks, n_slots, width, ring, window, row_tiles, wide;
     float scale, cap;
     int whole, spans;                     // the first `whole` row tiles have a block each, the others' keys are shared by `spans`,
                                           // whose parts a second launch joins
@@ -450,8 +450,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
             for (int i = 0; i < Q_ROWS; ++i) {
                 const int r = r0 + i * SOFTMAX_WARPS, row = row0 + r;
                 raw[i] = make_uint4(0u, 0u, 0u, 0u);
-                if (r < rows_here && lane * 8 < HD) {
-                    const bf16* src = a.q + (size_t)(first_tok + row / a.group) * a.q_stride + (g * a.group + row % a.group) * HD + lane * 8;
+                if (r < rows_here && lane * 8 < a.dim) {
+                    const bf16* src = a.q + (size_t)(first_tok + row / a.group) * a.q_stride + (g * a.group + row % a.group) * a.dim + lane * 8;
                     if (a.wide) raw[i] = *reinterpret_cast<const uint4*>(src);
                     else {
 #pragma unroll
@@ -647,13 +647,13 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
             const float v0 = power_of_two(e0);
             const bool nan = total != total;
             const int row = row0 + r, tok = first_tok + row / a.group, head = g * a.group + row % a.group;
-            bf16* dst = a.out + (size_t)tok * a.out_stride + (size_t)head * HD;
+            bf16* dst = a.out + (size_t)tok * a.out_stride + (size_t)head * a.dim;
             const size_t share = ((size_t)tok * a.n_kv * a.group + head) * a.spans + span;
             if (a.spans > 1 && row_ok && part == 0)          // (a row that is in its place: a sum that cannot be)
                 *reinterpret_cast<float2*>(a.part_ml + share * 2) = spans > 1 ? make_float2(m_ref, total) : make_float2(-INFINITY, -1.0f);
             const bool wide = ((uintptr_t)a.out & 15) == 0 && (a.out_stride & 7) == 0;
 #pragma unroll 1
-            for (int c = part * OUT; c < (part + 1) * OUT; c += 16) {
+            for (int c = part * OUT; c < min((part + 1) * OUT, a.dim); c += 16) {
                 uint32_t ov[16];
                 if (n_tiles > 0) {
                     tmem_ld16(lane_addr + O_COL + c, ov);
@@ -666,7 +666,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
                         if (n_tiles > 0)
                             x = make_float4(__uint_as_float(ov[i]) * v0, __uint_as_float(ov[i + 1]) * v0, __uint_as_float(ov[i + 2]) * v0,
                                             __uint_as_float(ov[i + 3]) * v0);
-                        *reinterpret_cast<float4*>(a.part_o + share * HD + c + i) = x;
+                        *reinterpret_cast<float4*>(a.part_o + share * a.dim + c + i) = x;
                     }
                 } else if (row_ok) {
 #pragma unroll
@@ -695,12 +695,12 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
     if (warp == ISSUER) tmem_dealloc(tmem, TMEM_COLS);
 }
 
-// The rows of the pages [rows][hd] of bytes; box = box_bytes x 32 rows.
-int make_map(CUtensorMap* map, const void* ptr, long long rows, int hd, int box_bytes) {
+// The rows of the pages [rows][dim] of bytes; box = box_bytes x 32 rows, zeros beyond a row's end.
+int make_map(CUtensorMap* map, const void* ptr, long long rows, int dim, int box_bytes) {
     EncodeTiled enc = encoder();
     if (!enc) return BROLM_ERR_BAD_SIZE;
-    const cuuint64_t dims[2] = {(cuuint64_t)hd, (cuuint64_t)rows};
-    const cuuint64_t strides[1] = {(cuuint64_t)hd};
+    const cuuint64_t dims[2] = {(cuuint64_t)dim, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)dim};
     const cuuint32_t box[2] = {(cuuint32_t)box_bytes, 32}, elem[2] = {1, 1};
     const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, elem,
                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -720,13 +720,13 @@ int launch(const TcArgs& a, cudaStream_t stream) {
     const long long blocks = a.whole + ((long long)a.row_tiles * a.n_kv * a.rows - a.whole) * a.spans, rows = (long long)a.n_blocks * a.n_kv * a.block;
     if (blocks > 0x7fffffffll || rows > 0x7fffffffll) return BROLM_ERR_TOO_LARGE;
     CUtensorMap mk, mv;
-    st = make_map(&mk, a.k_pages, rows, HD, 64);
+    st = make_map(&mk, a.k_pages, rows, a.dim, 64);
     if (st) return st;
-    st = make_map(&mv, a.v_pages, rows, HD, HD);
+    st = make_map(&mv, a.v_pages, rows, a.dim, HD);
     if (st) return st;
     st = launch_pdl(attn_kv8_tc_kernel<HD>, dim3((unsigned)blocks), dim3(THREADS), smem, stream, mk, mv, a);
     if (st || a.spans == 1) return st;
-    JoinArgs j{a.part_o, a.part_ml, a.out, a.cu_q, a.out_stride, a.rows, a.tokens, a.n_kv * a.group, HD, a.spans};
+    JoinArgs j{a.part_o, a.part_ml, a.out, a.cu_q, a.out_stride, a.rows, a.tokens, a.n_kv * a.group, a.dim, a.spans};
     j.some = a.whole > 0;
     if (a.rows == 1)                      // (one sequence: the tiles that are shared are those of its first tokens)
         j.tokens = min(a.tokens, ((a.row_tiles - a.whole / a.n_kv) * BM + a.group - 1) / a.group);
@@ -745,13 +745,13 @@ struct AttnTcCall {
     float scale, cap;
 };
 
-// bfloat16, heads of 64, 128 or 256 entries.
+// bfloat16, heads of up to 256 entries; what is between 64, 128 and 256 takes the time of the next, its last columns zeros.
 BROLM_API int brolm_attn_kv8_tc(const AttnTcCall* c) {
     const int n_kv = c->n_kv, group = c->group, block = c->block;
-    if (c->dim != 64 && c->dim != 128 && c->dim != 256) return BROLM_ERR_BAD_SIZE;
+    if (c->dim <= 0 || c->dim % 16) return BROLM_ERR_BAD_SIZE;
     if (c->tokens < 0 || c->rows < 0 || n_kv <= 0 || group <= 0 || block <= 0 || block % 32) return BROLM_ERR_BAD_SIZE;
     if (c->n_blocks <= 0 || c->n_slots <= 0 || c->width <= 0 || c->ring < 0 || c->ring % block || c->window < 0 || c->max_q_len <= 0) return BROLM_ERR_BAD_SIZE;
-    if (block > MAX_BLOCK || (long long)n_kv * group > 65535 || (long long)c->max_q_len * group > 0x3fffffff) return BROLM_ERR_TOO_LARGE;
+    if (c->dim > MAX_DIM || block > MAX_BLOCK || (long long)n_kv * group > 65535 || (long long)c->max_q_len * group > 0x3fffffff) return BROLM_ERR_TOO_LARGE;
     if ((long long)c->n_blocks * block > 0x7fffffffll || c->tokens > 0x3fffffff) return BROLM_ERR_TOO_LARGE;
     if (c->spans < 1 || (c->spans > 1 && (!c->part_o || !c->part_ml))) return BROLM_ERR_BAD_SIZE;
     if (((uintptr_t)c->k_pages | (uintptr_t)c->v_pages | (uintptr_t)c->part_o) & 15) return BROLM_ERR_ALIGNMENT;
@@ -763,10 +763,10 @@ BROLM_API int brolm_attn_kv8_tc(const AttnTcCall* c) {
     const int wide = ((uintptr_t)c->q & 15) == 0 && c->q_stride % 8 == 0;
     TcArgs a{(const bf16*)c->q, (bf16*)c->out, c->q_stride, c->out_stride, (const int32_t*)c->cu_q, (const int32_t*)c->kv_len,
              (const int32_t*)c->slots, (const int32_t*)c->tables, (const int8_t*)c->k_pages, (const int8_t*)c->v_pages,
-             (const float*)c->k_scale, (const float*)c->v_scale, c->tokens, c->rows, n_kv, group, block, c->n_blocks, c->n_slots,
+             (const float*)c->k_scale, (const float*)c->v_scale, c->tokens, c->rows, n_kv, group, c->dim, block, c->n_blocks, c->n_slots,
              c->width, c->ring, c->window, row_tiles, wide, c->scale, c->cap, c->whole, c->spans, (float*)c->part_o, (float*)c->part_ml};
-    if (c->dim == 64) return launch<64>(a, c->stream);
-    if (c->dim == 128) return launch<128>(a, c->stream);
+    if (c->dim <= 64) return launch<64>(a, c->stream);
+    if (c->dim <= 128) return launch<128>(a, c->stream);
     return launch<256>(a, c->stream);
 }
 

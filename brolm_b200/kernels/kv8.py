@@ -199,12 +199,13 @@ KV8_DEALT = 128                                   # sequences of a launch whose 
 
 
 @functools.lru_cache(maxsize=256)
-def kv8_shares(batch: int, n_kv: int, row_tiles: int, keys: int, head_dim: int, sms: int, many: bool = False) -> tuple[int, int]:
+def kv8_shares(batch: int, n_kv: int, row_tiles: int, keys: int, head_dim: int, sms: int, many: bool = False,
+               per_sm: int = 3) -> tuple[int, int]:
     """How many blocks share the keys of one (sequence, kv head, tile of query rows): (blocks of a cluster, clusters), or
     (blocks of a cluster, -n): n clusters of a (kv head, tile of query rows) are dealt out over the sequences by their lengths
     on the device.  ``many``: more than eight query rows of a kv head, whose tiles take twice as long.
 
-    Two blocks run on an SM (three, of heads of up to 64 entries), and there are as many shares as give every SM its blocks,
+    Two blocks run on an SM (``per_sm`` of heads of up to 64 entries), and there are as many shares as give every SM its blocks,
     but none whose four warps would not have a tile of keys each.  A cluster lies inside one group of SMs, so clusters of
     three to eight leave up to an eighth of the places empty; where one too many is asked for, it runs alone at the end (48
     items of 2,000 keys, float32: 28.6 us as 6 x 1, of which 45 fit, 19.7 as 5 x 1; 12 of 4,000 at 4 kv heads of 256, one
@@ -223,7 +224,7 @@ def kv8_shares(batch: int, n_kv: int, row_tiles: int, keys: int, head_dim: int, 
     With more sequences, where an item would have no more than two shares, the longest ones' blocks would run alone at the
     end: such steps are cut into rounds of blocks that the SMs take as they come free, if the shares stay long enough (24
     tiles) and fill their rounds (40 sequences of 100 to 3,000 keys, 8 kv heads: 52.9 us as 1 x 1, 43.7 as 1 x 2)."""
-    places = (3 if head_dim <= 64 else 2) * sms
+    places = (per_sm if head_dim <= 64 else 2) * sms
     heads = n_kv * row_tiles
     items = max(1, batch * heads)
     tiles = max(1, -(-keys // KV8_TILE))
@@ -285,10 +286,11 @@ def kv8_tc_spans(tokens: int, batch: int, n_kv: int, group: int, max_q_len: int,
     return min(choices, key=cost)
 
 
-# From how many rows of a kv head (tokens x query heads), and from how many of rows x kv heads x keys x entries, a step of
-# bfloat16 runs on tcgen05, whose blocks take 128 rows and 18 us to begin and end.  8 kv heads of 256, two query heads each,
-# us on mma.sync / tcgen05: 32 tokens on 1,000 keys (1.3e8) 14.7 / 20.2, 128 on 300 (1.6e8) 17.1 / 23.3, 16 on 4,096 (2.7e8)
-# 27.0 / 22.5, 64 on 4,096 (1.1e9) 39.4 / 30.4, 512 on 8,192 (1.7e10) 450 / 123; 4 x 64 on 1,000 (5.2e8) 38.9 / 31.9.
+# From how many rows of a kv head (tokens x query heads), and from how many of rows x kv heads x keys x entries (64 at least),
+# a step of bfloat16 runs on tcgen05, whose blocks take 128 rows and heads of 64, 128 or 256 entries, smaller ones filled up
+# with zeros.  8 kv heads, two query heads each, us on mma.sync / tcgen05.  256 entries: 32 tokens on 1,000 keys (1.3e8) 14.6 /
+# 19.1, 128 on 300 (1.6e8) 18.0 / 21.7, 16 on 4,096 (2.7e8) 20.6 / 20.8, 64 on 4,096 (1.1e9) 40.1 / 26.9, 4 x 64 on 1,000
+# (1.0e9) 40.0 / 28.8, 1,024 on 8,192 (3.4e10) 813 / 199, and of 192 748 / 197, of 96 490 / 157, of 32 336 / 146.
 KV8_TC_ROWS, KV8_TC_WORK = 32, 2.5e8
 
 
@@ -333,8 +335,8 @@ def attention_kv8(q: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, kv_len
     T = shape[0]
     rows = max_q_len * group
     keys = min(max_kv_len, window + max_q_len) if window > 0 else max_kv_len
-    if rows >= KV8_TC_ROWS and dt is torch.bfloat16 and head_dim in (64, 128, 256) and n_blocks * n_kv * block < 1 << 31 and \
-            float(T) * group * n_kv * keys * head_dim >= KV8_TC_WORK:
+    if rows >= KV8_TC_ROWS and dt is torch.bfloat16 and n_blocks * n_kv * block < 1 << 31 and \
+            float(T) * group * n_kv * keys * max(head_dim, 64) >= KV8_TC_WORK:
         whole, spans = kv8_tc_spans(T, batch, n_kv, group, max_q_len, keys, head_dim, device_sms())
         part_o = part_ml = 0
         if spans > 1:
@@ -344,7 +346,8 @@ def attention_kv8(q: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, kv_len
             v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), part_o, part_ml, _stream(), q0[0], o0[0], T, batch, n_kv, group,
             head_dim, block, n_blocks, S, W, ring, window, max_q_len, whole, spans, scale, cap), what)
         return
-    shares, spans = kv8_shares(batch, n_kv, 1 if rows <= 8 else -(-rows // 16), keys, head_dim, device_sms(), rows > 8)
+    shares, spans = kv8_shares(batch, n_kv, 1 if rows <= 8 else -(-rows // 16), keys, head_dim, device_sms(), rows > 8,
+                               3 if rows <= (4 if dt is _F32 else 8) else 2)
     part_o = part_ml = plan = 0
     if spans > 1:
         parts, part_o, part_ml, _ = _parts(T * n_kv * group * spans, head_dim, q.device)

@@ -669,6 +669,16 @@ def test_a_piece_whose_values_scales_lie_2_to_the_100_apart(on_tcgen05):
     compare(c, torch.bfloat16, [0], [192], 1, 0.125, 0.0, 0)
 
 
+@pytest.mark.parametrize("D", [16, 48, 80, 96, 112, 192, 240])
+def test_pieces_of_heads_between_the_sizes(D, on_tcgen05, monkeypatch):
+    """Heads whose rows end inside a copied box, or a whole box before the last."""
+    c = filled(2, 10, 3, 32, D, [310, 200], seed=D)
+    compare(c, torch.bfloat16, [1, 0], [140, 75], 3, D ** -0.5, 30.0, 0)
+    compare(c, torch.bfloat16, [0], [200], 1, D ** -0.5, 0.0, 150)
+    monkeypatch.setattr(kernels.kv8, "kv8_tc_spans", lambda *a: (2, 3))
+    compare(c, torch.bfloat16, [0, 1], [129, 130], 2, D ** -0.5, 0.0, 0)
+
+
 @pytest.mark.parametrize("shared", [(0, 3), (1, 2), (5, 4), (7, 30)], ids=str)
 @pytest.mark.parametrize("D,window", [(64, 0), (256, 0), (128, 90)])
 def test_a_piece_some_of_whose_tiles_are_shared(D, window, shared, on_tcgen05, monkeypatch):
