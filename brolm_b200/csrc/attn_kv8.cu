@@ -55,6 +55,30 @@ __device__ __forceinline__ float rcp(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// cap tanh(x) of float32 scores, in log2 units.  Scores are mostly well below the cap, and there the series to x^13 is as exact
+// as a float (|x| up to 0.4: the next term is 2e-9).
+__device__ __forceinline__ float near_tanh(float x) {
+    const float y = x * x;
+    float p = fmaf(21844.0f / 6081075.0f, y, -1382.0f / 155925.0f);
+    p = fmaf(p, y, 62.0f / 2835.0f);
+    p = fmaf(p, y, -17.0f / 315.0f);
+    p = fmaf(p, y, 2.0f / 15.0f);
+    p = fmaf(p, y, -1.0f / 3.0f);
+    return fmaf(x * y, p, x);
+}
+template <int N>
+__device__ __forceinline__ void cap_exactly(float (&x)[N], float c1) {
+    float far = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) far = fmaxf(far, fabsf(x[i]));
+    if (__all_sync(0xffffffffu, far <= 0.4f)) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = c1 * near_tanh(x[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = c1 * tanhf(x[i]);
+    }
+}
 __device__ __forceinline__ void cluster_barrier() {
     asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;\n" ::: "memory");
 }
@@ -610,8 +634,15 @@ __global__ void __launch_bounds__(THREADS, 2) attn_kv8_few_kernel(AttnArgs a) {
                     if constexpr (SUMS == 2) { hi += zs[1][mt][q][2 * h]; lo += zs[1][mt][q][2 * h + 1]; }
                     float x = (float)(hi * 256 + lo) * weight;
                     x += __shfl_xor_sync(0xffffffffu, x, 1);
-                    x *= to_z;
-                    if (a.cap > 0.0f) x = EXACT ? c1 * tanhf(x) : fmaf(-c2, rcp(1.0f + ex2(x)), c1);
+                    z[mt][h] = x * to_z;
+                }
+            if (EXACT && a.cap > 0.0f) cap_exactly(reinterpret_cast<float(&)[4]>(z), c1);
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float x = z[mt][h];
+                    if (!EXACT && a.cap > 0.0f) x = fmaf(-c2, rcp(1.0f + ex2(x)), c1);
                     if (edge) {
                         const int back = pos[q] - (key0 + 16 * mt + 8 * h + g8);
                         if (back < 0 || back >= window) x = -INFINITY;
@@ -897,13 +928,16 @@ __global__ void __launch_bounds__(THREADS, 2) attn_kv8_kernel(AttnArgs a) {
         uint32_t pf[PARTS][2][NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            float mt_max[2] = {-INFINITY, -INFINITY};
+            float mt_max[2] = {-INFINITY, -INFINITY}, s8[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s8[i] = z[i >> 2][nt][i & 3] * (qf[nt][i & 1] * sc.x);
+            if (EXACT && a.cap > 0.0f) cap_exactly(s8, c1);
 #pragma unroll
             for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    float x = z[mt][nt][e] * (qf[nt][e & 1] * sc.x);
-                    if (a.cap > 0.0f) x = EXACT ? c1 * tanhf(x) : fmaf(-c2, rcp(1.0f + ex2(x)), c1);
+                    float x = s8[4 * mt + e];
+                    if (!EXACT && a.cap > 0.0f) x = fmaf(-c2, rcp(1.0f + ex2(x)), c1);
                     if (edge) {
                         const int back = pos[nt][e & 1] - (key0 + 16 * mt + g8 + (e & 2) * 4);
                         if (back < 0 || back >= window) x = -INFINITY;
