@@ -796,7 +796,7 @@ __global__ void __launch_bounds__(THREADS, 2) attn_kv8_few_kernel(AttnArgs a) {
 //
 // What bounds it is a warp's own chain, 1.8 us a tile of 32 keys of 128 entries in float32 (128 products, as many bytes to
 // turn, two exponentials and a tanh a score) with one or two warps a scheduler: 6 sequences of 13 to 4,001 keys with five
-// tokens each, 4 kv heads of 128, four query heads each, float32, take 22.0 us (21.0 in bfloat16, 24.3 without the cap, as
+// tokens each, 4 kv heads of 128, four query heads each, float32, take 21.7 us (19.5 in bfloat16, 21.2 without the cap, as
 // 5 x 1 shares of the longest 26.5).
 
 template <typename T, int DP>

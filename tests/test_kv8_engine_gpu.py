@@ -127,6 +127,26 @@ def test_captured_steps_give_the_bits_of_uncaptured_ones(name, dtype, monkeypatc
     assert torch.equal(*results)
 
 
+@pytest.mark.parametrize("name,dtype", [("B", "float32"), ("wide", "bfloat16")])
+def test_captured_steps_whose_clusters_are_dealt_out(name, dtype, monkeypatch):
+    """Who gets how many hangs on the lengths alone, which a captured step reads anew: the same bits as uncaptured ones."""
+    monkeypatch.setattr(kernels.kv8, "kv8_shares", lambda *a: (1, -20))
+    model = build(name, dtype)
+    prompts = random_prompts(model.config.vocab_size, [250, 3, 120], seed=14)
+    results = []
+    for graphs in (True, False):
+        e = bb.Engine(model, 64 * 20, max_slots=3, cache_dtype="int8", use_graphs=graphs)
+        s = e.open(3)
+        logits, out = e.step(s, prompts), []
+        for _ in range(40):
+            ids = logits.argmax(dim=1).to(torch.int32)
+            out.append(logits.clone())
+            logits = e.step_from(s, ids, [0, 1, 2])
+        results.append(torch.stack(out))
+        check_tables(e)
+    assert torch.equal(*results) and bool(torch.isfinite(results[0]).all())
+
+
 @pytest.mark.parametrize("name,dtype,most", [("A", "float32", 50), ("B", "bfloat16", 7), ("wide", "bfloat16", 200), ("wide", "float32", 64)])
 def test_prompts_in_pieces(name, dtype, most):
     """A prompt brought a piece at a time, beside sequences that go on by one token and that begin."""
