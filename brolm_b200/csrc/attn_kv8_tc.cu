@@ -32,10 +32,13 @@
 // of two to below 2^14 and held in f16, exactly but for numbers 2^-38 of the row's largest.
 //
 // What bounds it: of a tile of 128 keys and 256 entries, about 5,600 cycles (2,048 tokens on 14,336 keys, 8 kv heads of 256,
-// two query heads each: 638 to 657 us, 680 to 700 TFLOP/s of 1,700), the tensor core takes 2,770, shared memory 3,500 (bytes
+// two query heads each: 626 us, 710 TFLOP/s of 1,700), the tensor core takes 2,770, shared memory 3,500 (bytes
 // in, f16 out, f16 to the tensor core: 448 KB), the softmax of a row's scores and then of its weights, which wait for each
-// other and for the products, 1,700 and 1,200, and the instructions of all roles 57 % of the issue slots.  Two sets of softmax
-// warps that take turns on tiles were slower (845 us): the scores of a tile wait for the values of the tile before the last.
+// other and for the products, 1,700 to 2,200 (fma units) and 1,200 to 1,400 (special function units), and the instructions of
+// all roles 57 % of the issue slots.  To put those two side by side was slower, both as two sets of softmax warps that take
+// turns on tiles (845 us) and as rounds that take the next tile's scores while they make this one's weights (828, and with
+// three score buffers for heads of 64 311 us for 263): with two score buffers a tile's scores then wait for the values of the
+// tile before the last, and a thread has too few registers for both.
 //
 // Every mbarrier wait is bounded; a wait that runs out records a code that brolm_attn_kv8_tc_status() returns, and the
 // launch ends without its results.
@@ -512,9 +515,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
         const float qs = q_scale[r];
         const float unit = qs * (a.cap > 0.0f ? a.scale / a.cap : a.scale * LOG2E);
         const float c1 = a.cap * LOG2E, c2 = 2.0f * a.cap * LOG2E;
-        const uint64_t t0 = pair_of(c1, c1), t1 = pair_of(c1 * (-1.0f / 3.0f), c1 * (-1.0f / 3.0f));
-        const uint64_t t2 = pair_of(c1 * (2.0f / 15.0f), c1 * (2.0f / 15.0f)), t3 = pair_of(c1 * (-17.0f / 315.0f), c1 * (-17.0f / 315.0f));
-        const uint64_t t4 = pair_of(c1 * (62.0f / 2835.0f), c1 * (62.0f / 2835.0f));
+        // tanh(x) / x up to |x| = 0.4, of the third degree in x^2 with the least largest error (1e-7; an exchange of the points
+        // where it is largest gives the four numbers; the series to x^9 has 4e-7)
+        const uint64_t t0 = pair_of(c1 * 0.9999999f, c1 * 0.9999999f), t1 = pair_of(c1 * -0.33331362f, c1 * -0.33331362f);
+        const uint64_t t2 = pair_of(c1 * 0.13270977f, c1 * 0.13270977f), t3 = pair_of(c1 * -0.047553604f, c1 * -0.047553604f);
         float m_ref = -INFINITY, l = 0.0f;                   // l: the sum over this thread's columns only
         bool ok = true, sees_bad = false;
         for (int j = 0; j < n_tiles; ++j) {
@@ -539,14 +543,14 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
                     z[c] = to_z(mul2(pair_of(__uint_as_float(sv[2 * c]), __uint_as_float(sv[2 * c + 1])), pair_of(f, f)));
             };
             if (a.cap > 0.0f) {
-                // cap log2e tanh(x).  Scores are mostly well below the cap, and there the series to x^9 is as exact (|x| up to
-                // 0.4: 4e-7 of the cap) and leaves the special function units to the weights
+                // cap log2e tanh(x).  Scores are mostly well below the cap, and there a polynomial is as exact and leaves the
+                // special function units to the weights
                 float far = 0.0f;
                 scores([&](uint64_t x) {
                     const uint64_t y = mul2(x, x);
                     const float2 yy = halves(y);
                     far = max3(far, yy.x, yy.y);
-                    return mul2(x, mad2(mad2(mad2(mad2(t4, y, t3), y, t2), y, t1), y, t0));
+                    return mul2(x, mad2(mad2(mad2(t3, y, t2), y, t1), y, t0));
                 });
                 if (!__all_sync(0xffffffffu, far <= 0.16f))
                     scores([&](uint64_t x) {
@@ -583,9 +587,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
             if (!ok) break;
             m_t = max3(fmaxf(xch[s * 4 * BM + r], xch[(s * 4 + 1) * BM + r]), xch[(s * 4 + 2) * BM + r], xch[(s * 4 + 3) * BM + r]);
             const bool raise = m_t > m_ref + RESCALE_GAP;    // also true for the first visible tile of a row
-            const float m_new = raise ? m_t : m_ref;
-            const float corr = (raise && m_ref > -INFINITY) ? fast_exp2(m_ref - m_new) : 1.0f;
-            if (j > 0 && __any_sync(0xffffffffu, corr != 1.0f)) {
+            if (__any_sync(0xffffffffu, raise && m_ref > -INFINITY)) {
+                const float corr = raise && m_ref > -INFINITY ? fast_exp2(m_ref - m_t) : 1.0f;
+                l *= corr;
                 // rare: the accumulator has to be at rest (the product of the tile before is done), then every row of the
                 // warp is scaled anew; each of the four warps takes a quarter of the entries
                 ok = wait_warp(bar(PV_DONE + (s ^ 1)), ((j - 1) >> 1) & 1, give_up, 12);
@@ -600,8 +604,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
                     tmem_st16(lane_addr + O_COL + c, ov);
                 }
             }
-            l *= corr;
-            m_ref = m_new;
+            if (raise) m_ref = m_t;
             // weights -> tensor memory, f16 pairs: keys 2c, 2c+1 of this thread in column c of its 16
             const float m_sub = m_ref > -INFINITY ? m_ref : 0.0f;    // a row that has seen nothing: 2^(-inf - 0) = 0
             uint64_t sums = 0ull;
