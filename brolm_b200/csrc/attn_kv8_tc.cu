@@ -17,7 +17,7 @@
 //               keys of tile 0; then the keys of tile j + 1 and the values of tile j; the values of the last tile), four
 //               warps every other unit (with four warps for all of them a tile took 8,600 cycles: a unit is 260 of
 //               arithmetic and 500 of waiting for shared memory and barriers);
-//   warp 24     one thread issues tcgen05.mma: S = Q K^T (128 x 128) into one of two buffers in tensor memory, O += P V
+//   warp 24     one thread (of elect.sync) issues tcgen05.mma: S = Q K^T (128 x 128) into one of two buffers in tensor memory, O += P V
 //               (128 x head size, P from tensor memory, the values as they lie, keys x entries);
 //   warp 25     looks up where the keys lie and what their scales are, 32 groups of 32 keys at a time, for all the others;
 //   warp 26, 27 issue the TMA loads of the units' bytes, of keys and of values, into a ring of their own.  (Loads into the
@@ -31,14 +31,16 @@
 // would be passed by more than 8: the accumulator in tensor memory is then scaled anew.)  A query row is scaled by a power
 // of two to below 2^14 and held in f16, exactly but for numbers 2^-38 of the row's largest.
 //
-// What bounds it: of a tile of 128 keys and 256 entries, about 5,600 cycles (2,048 tokens on 14,336 keys, 8 kv heads of 256,
-// two query heads each: 626 us, 710 TFLOP/s of 1,700), the tensor core takes 2,770, shared memory 3,500 (bytes
-// in, f16 out, f16 to the tensor core: 448 KB), the softmax of a row's scores and then of its weights, which wait for each
-// other and for the products, 1,700 to 2,200 (fma units) and 1,200 to 1,400 (special function units), and the instructions of
-// all roles 57 % of the issue slots.  To put those two side by side was slower, both as two sets of softmax warps that take
-// turns on tiles (845 us) and as rounds that take the next tile's scores while they make this one's weights (828, and with
-// three score buffers for heads of 64 311 us for 263): with two score buffers a tile's scores then wait for the values of the
-// tile before the last, and a thread has too few registers for both.
+// What bounds it: of a tile of 128 keys and 256 entries, about 5,000 cycles (2,048 tokens on 14,336 keys, 8 kv heads of 256,
+// two query heads each: 565 us, 790 TFLOP/s of 1,700), the tensor core takes 2,050, shared memory 3,500 (bytes in, f16 out, f16
+// to the tensor core: 448 KB), the softmax of a row's scores and then of its weights, which wait for each other and for the
+// products, 1,700 to 2,000 (fma units) and 1,200 to 1,400 (special function units), and the instructions of all roles 57 % of
+// the issue slots; the tensor core now waits for what is turned into f16 (1,400 cycles a tile for keys, 1,300 for values).
+// Four groups of two converting warps instead of two of four were slower (609 us).  To put scores and weights side by side
+// was slower too, both as two sets of softmax warps that take turns on tiles and as rounds that take the next tile's scores
+// while they make this one's weights (681 us; with three score buffers for heads of 128 entries 144 us for 158, which is
+// another kernel's worth of code): with two score buffers a tile's scores then wait for the values of the tile before the
+// last, and a thread has too few registers for both.
 //
 // Every mbarrier wait is bounded; a wait that runs out records a code that brolm_attn_kv8_tc_status() returns, and the
 // launch ends without its results.
@@ -107,6 +109,14 @@ __device__ __forceinline__ uint32_t idesc_f16(int m, int n, int b_mn_major) {
 }
 __device__ __forceinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile int* give_up, int code) {
     return mbar_wait(bar, parity, give_up, &g_attn_kv8_tc_error, code);
+}
+// One lane of a warp that is there as a whole.  The compiler knows of this one that it is alone, and keeps what the products
+// are given in uniform registers: a tile of 256 entries is 24 products, and where `lane == 0` issued them the tensor core
+// waited for their issue (2,048 tokens on 14,336 keys 626 us for 565).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(one));
+    return one != 0;
 }
 template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -311,7 +321,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
                 if (lane == 0) mbar_arrive(bar(META_FULL + (m & 1)));
             }
         } else if (warp == ISSUER) {
-            if (lane == 0 && n_tiles > 0) {
+            if (n_tiles > 0 && elect_one()) {
                 const uint32_t id_qk = idesc_f16(BM, BN, 0), id_pv = idesc_f16(BM, HD, 1);
                 int u = 0;
                 // S(j) goes over the buffer that P(j-2) was read from: the product that read it was issued before
