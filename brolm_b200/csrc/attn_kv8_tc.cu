@@ -20,7 +20,7 @@
 //   warp 24     one thread (of elect.sync) issues tcgen05.mma: S = Q K^T (128 x 128) into one of two buffers in tensor memory, O += P V
 //               (128 x head size, P from tensor memory, the values as they lie, keys x entries);
 //   warp 25     looks up where the keys lie and what their scales are, 32 groups of 32 keys at a time, for all the others;
-//   warp 26, 27 issue the TMA loads of the units' bytes, of keys and of values, into a ring of their own.  (Loads into the
+//   warp 26, 27 issue the TMA loads of the units' bytes, of keys and of values, each into a ring of its own.  (Loads into the
 //               converting threads' registers were as many, but what tells the tensor core of a thread's stores waits for its
 //               loads too: 6.4 us a tile of 128 keys and 256 entries.  One thread for all loads needs 1,000 cycles a unit.)
 //
@@ -32,7 +32,7 @@
 // of two to below 2^14 and held in f16, exactly but for numbers 2^-38 of the row's largest.
 //
 // What bounds it: of a tile of 128 keys and 256 entries, about 5,000 cycles (2,048 tokens on 14,336 keys, 8 kv heads of 256,
-// two query heads each: 565 us, 790 TFLOP/s of 1,700), the tensor core takes 2,050, shared memory 3,500 (bytes in, f16 out, f16
+// two query heads each: 562 to 577 us, 775 to 795 TFLOP/s of 1,700), the tensor core takes 2,050, shared memory 3,500 (bytes in, f16 out, f16
 // to the tensor core: 448 KB), the softmax of a row's scores and then of its weights, which wait for each other and for the
 // products, 1,700 to 2,000 (fma units) and 1,200 to 1,400 (special function units), and the instructions of all roles 57 % of
 // the issue slots; the tensor core now waits for what is turned into f16 (1,400 cycles a tile for keys, 1,300 for values).
@@ -89,10 +89,15 @@ template <int HD>
 struct Shape {
     static constexpr int PARTS = HD / 64;                    // units of a key tile, and of a value tile
     static constexpr int VK = BN / PARTS;                    // keys of a value unit
-    static constexpr int SLOTS = HD == 256 ? 5 : 8;
-    static constexpr int RAWS = HD == 256 ? 8 : 7;           // units on their way from the cache
+    static constexpr int SLOTS = HD == 256 ? 5 : HD == 128 ? 7 : 8;
     static constexpr int Q_BYTES = BM * HD * 2;
 };
+
+// Units on their way from the cache: a ring for keys and one for values.  A wait tells a slot's uses apart by their parity
+// alone, so whoever waits for one must have waited for, or worked on, the one before: each ring has one loading warp, and an
+// even number of slots gives a slot's units to one group of converting warps.
+constexpr int KIND_RAWS = 4, RAWS = 2 * KIND_RAWS;
+static_assert(KIND_RAWS % CONVERT_GROUPS == 0, "a raw slot's units belong to one group");
 
 // barriers
 enum : int { S_FULL = 0, P_FULL = 2, PV_DONE = 4, META_FULL = 6, META_EMPTY = 8, Q_FULL = 10, U_FULL = 11 };
@@ -207,7 +212,7 @@ template <int HD>
 __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_constant__ CUtensorMap map_k,
                                                                  const __grid_constant__ CUtensorMap map_v, TcArgs a) {
     using SH = Shape<HD>;
-    constexpr int PARTS = SH::PARTS, VK = SH::VK, SLOTS = SH::SLOTS, RAWS = SH::RAWS;
+    constexpr int PARTS = SH::PARTS, VK = SH::VK, SLOTS = SH::SLOTS;
     constexpr uint32_t S_COL = 0, O_COL = 2 * BN;            // tensor-memory columns: two score buffers, then the output
     static_assert(O_COL + HD <= TMEM_COLS, "tensor memory");
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -371,40 +376,33 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
             const bool keys = warp == LOADER;
             const int boxes = keys ? 4 : VK / 32;
             const uint32_t box_bytes = keys ? RAW / 4 : 32 * HD;
-            int u = 0, tile = 0;
+            const int raw0 = keys ? 0 : KIND_RAWS;
+            int asked = 0;                         // units of this kind
             bool ok = true;
-            for (; tile < n_tiles && ok; ++tile) {
+            for (int tile = 0; tile < n_tiles && ok; ++tile) {
                 const int chunk = tile / CHUNK;
                 if (tile % CHUNK == 0) ok = wait_soon(bar(META_FULL + (chunk & 1)), (chunk >> 1) & 1, give_up, 2);
                 const Meta* m = meta + (chunk & 1) * CHUNK * 4 + (tile % CHUNK) * 4;
-                const int first = keys ? (tile == 0 ? 0 : 2 * tile - 1) * PARTS : min(2 * tile + 2, 2 * n_tiles - 1) * PARTS;
 #pragma unroll
                 for (int part = 0; part < PARTS; ++part) {
                     if (!ok) break;
-                    u = first + part;
-                    const int sl = u % RAWS;
-                    ok = wait_soon(r_empty(sl), ((u / RAWS) & 1) ^ 1, give_up, 1);
+                    const int sl = raw0 + asked % KIND_RAWS;
+                    ok = wait_soon(r_empty(sl), ((asked / KIND_RAWS) & 1) ^ 1, give_up, 1);
                     if (!ok) break;
                     if (lane == 0) mbar_expect_tx(r_full(sl), RAW);
                     __syncwarp();
                     if (lane < boxes)
                         tma_load_2d(raw_s + sl * RAW + lane * box_bytes, keys ? &map_k : &map_v, keys ? part * 64 : 0,
                                     m[keys ? lane : part * (VK / 32) + lane].row, r_full(sl));
+                    ++asked;
                 }
                 __syncwarp();
                 if (lane == 0 && tile % CHUNK == CHUNK - 1) mbar_arrive(bar(META_EMPTY + (chunk & 1)));
             }
             if (lane == 0) pdl_trigger();      // every tile is asked for: the next kernel may move in
-            if (*give_up) {                    // let the loads in flight land before the block goes away
-                // (this warp's last units, whichever of the ring's slots they went to; a slot that the other warp's load came
-                // to is drained by that warp)
-                for (int t = max(0, tile - 1 - RAWS); t < tile; ++t) {
-                    const int first = keys ? (t == 0 ? 0 : 2 * t - 1) * PARTS : min(2 * t + 2, 2 * n_tiles - 1) * PARTS;
-                    for (int part = 0; part < PARTS; ++part)
-                        if (first + part < u || (first + part == u && ok))
-                            mbar_wait(r_full((first + part) % RAWS), ((first + part) / RAWS) & 1, give_up, &g_attn_kv8_tc_error, 10, true);
-                }
-            }
+            if (*give_up)                      // let the loads in flight land before the block goes away
+                for (int i = max(0, asked - KIND_RAWS); i < asked; ++i)
+                    mbar_wait(r_full(raw0 + i % KIND_RAWS), (i / KIND_RAWS) & 1, give_up, &g_attn_kv8_tc_error, 10, true);
         }
     } else if (warp >= SOFTMAX_WARPS) {
         fewer_registers<CONVERT_REGS>();
@@ -420,10 +418,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
         const uint32_t k_dst = k_row * 128, v_dst = (v_c >> 2) * (VK * 128) + v_row * 128;
         const int k_piece = (2 * k_c) ^ (k_row & 7), v_piece = (2 * (v_c & 3)) ^ (v_row & 7);
         bool ok = true;
-        auto convert = [&](auto kind, int u) {
+        // unit u, the i-th of its kind
+        auto convert = [&](auto kind, int u, int i_kind) {
             constexpr bool KEYS = decltype(kind)::value;
-            const int sl = u % SLOTS, rs = u % RAWS;
-            ok = ok && wait_soon(r_full(rs), (u / RAWS) & 1, give_up, 5);
+            const int sl = u % SLOTS, rs = (KEYS ? 0 : KIND_RAWS) + i_kind % KIND_RAWS;
+            ok = ok && wait_soon(r_full(rs), (i_kind / KIND_RAWS) & 1, give_up, 5);
             if (!ok) return;
             uint4 raw[4];
 #pragma unroll
@@ -445,9 +444,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
         const bool keys = PARTS > 1 || group == 0, values = PARTS > 1 || group == 1;
         for (int j = -1; j < n_tiles && ok; ++j) {
             if (keys && j + 1 < n_tiles)
-                for (int p = first; p < PARTS; p += stride) convert(std::true_type(), (j < 0 ? 0 : 2 * j + 1) * PARTS + p);
+                for (int p = first; p < PARTS; p += stride) convert(std::true_type(), (j < 0 ? 0 : 2 * j + 1) * PARTS + p, (j + 1) * PARTS + p);
             if (values && j >= 0)
-                for (int p = first; p < PARTS; p += stride) convert(std::false_type(), min(2 * j + 2, 2 * n_tiles - 1) * PARTS + p);
+                for (int p = first; p < PARTS; p += stride) convert(std::false_type(), min(2 * j + 2, 2 * n_tiles - 1) * PARTS + p, j * PARTS + p);
         }
     } else {
         more_registers<SOFTMAX_REGS>();
@@ -724,8 +723,8 @@ int make_map(CUtensorMap* map, const void* ptr, long long rows, int dim, int box
 template <int HD>
 int launch(const TcArgs& a, cudaStream_t stream) {
     using SH = Shape<HD>;
-    constexpr size_t smem = (size_t)SH::Q_BYTES + (size_t)SH::SLOTS * UNIT + SH::RAWS * RAW + 2 * CHUNK * 4 * sizeof(Meta) + 9 * BM * 4 +
-                            (U_FULL + 2 * SH::SLOTS + 2 * SH::RAWS) * 8 + 32;
+    constexpr size_t smem = (size_t)SH::Q_BYTES + (size_t)SH::SLOTS * UNIT + RAWS * RAW + 2 * CHUNK * 4 * sizeof(Meta) + 9 * BM * 4 +
+                            (U_FULL + 2 * SH::SLOTS + 2 * RAWS) * 8 + 32;
     static_assert(smem <= 232448, "shared memory of a block");
     static OncePerDevice raised;
     int st = allow_shared_memory(attn_kv8_tc_kernel<HD>, smem, raised);
