@@ -346,7 +346,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
                     umma_commit(bar(S_FULL + s));
                     return true;
                 };
-                bool ok = wait_on(bar(Q_FULL), 0, give_up, 15) && issue_qk(0);
+                const bool begun = wait_on(bar(Q_FULL), 0, give_up, 15);
+                bool ok = begun && issue_qk(0);
                 for (int j = 0; j < n_tiles && ok; ++j) {
                     if (j + 1 < n_tiles) { ok = issue_qk(j + 1); if (!ok) break; }
                     const int s = j & 1;
@@ -369,6 +370,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
                     }
                     if (!ok) break;
                     umma_commit(bar(PV_DONE + s));
+                }
+                if (begun) {                       // products in flight end before their operands go
+                    umma_commit(bar(Q_FULL));
+                    mbar_wait(bar(Q_FULL), 1, give_up, &g_attn_kv8_tc_error, 16, true);
                 }
             }
         } else {
