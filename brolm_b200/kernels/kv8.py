@@ -264,10 +264,10 @@ def _parts(n: int, head_dim: int, device, plans: int = 0) -> tuple:
 def kv8_tc_spans(tokens: int, batch: int, n_kv: int, group: int, max_q_len: int, keys: int, head_dim: int, sms: int) -> tuple[int, int]:
     """How many of the tiles of 128 query rows have a block each on tcgen05, and how many blocks share the keys of each of the
     others: one block runs on an SM, so what counts is how many rounds of blocks there are and how long a block's share is.
-    In tiles of 128 keys (3 us each at 256 entries): a block begins and ends in three, and joining costs another three and
+    In tiles of 128 keys (about 2.6 us each at 256 entries, counted as 3): a block begins and ends in three, and joining costs another three and
     what the parts take to memory and back.  Where the last round would be far from full, its tiles alone are shared
     (on 14,336 keys, 8 kv heads of 256, two query heads each, us with a block for a tile / four / the last round's
-    shared: 1,280 tokens, 160 tiles on 148 SMs, 644 / 502 / 400; 1,700, 216 tiles, 656 / 616 / 535; 2,048, 256, 657 / 715 / 657)."""
+    shared: 1,280 tokens, 160 tiles on 148 SMs, 571 / 446 / 353; 1,700, 216 tiles, 573 / 545 / 472; 2,048, 256, 568 / 653 / 564)."""
     items = batch * n_kv * -(-max_q_len * group // 128)
     tiles = -(-keys // 128)
     traffic = tokens * n_kv * group * head_dim * 8 / 6.5e12 / (3e-6 * head_dim / 256)
@@ -290,7 +290,7 @@ def kv8_tc_spans(tokens: int, batch: int, n_kv: int, group: int, max_q_len: int,
 # a step of bfloat16 runs on tcgen05, whose blocks take 128 rows and heads of 64, 128 or 256 entries, smaller ones filled up
 # with zeros.  8 kv heads, two query heads each, us on mma.sync / tcgen05.  256 entries: 32 tokens on 1,000 keys (1.3e8) 14.6 /
 # 19.1, 128 on 300 (1.6e8) 18.0 / 21.7, 16 on 4,096 (2.7e8) 20.6 / 20.8, 64 on 4,096 (1.1e9) 40.1 / 26.9, 4 x 64 on 1,000
-# (1.0e9) 40.0 / 28.8, 1,024 on 8,192 (3.4e10) 813 / 199, and of 192 748 / 197, of 96 490 / 157, of 32 336 / 146.
+# (1.0e9) 40.0 / 28.5, 1,024 on 8,192 (3.4e10) 803 / 179, and of 192 736 / 178, of 96 472 / 157, of 32 343 / 137.
 KV8_TC_ROWS, KV8_TC_WORK = 32, 2.5e8
 
 
