@@ -22,7 +22,7 @@ import struct
 from ctypes import c_char_p, c_int
 import torch
 
-from . import KernelError, _check, _fn, _stream, device_sms, library_loaded, load_library
+from . import KernelError, _check, _fn, _sms, device_sms, library_loaded, load_library
 
 # what the tables' status word says
 BLOCKS_STATUS = {0: "ok", 1: "too few free blocks (or a stack that does not fit)", 2: "a row of the tables is too narrow",
@@ -43,6 +43,8 @@ _READ = struct.Struct("@11P4q10i")
 _ATTN = struct.Struct("@14P17i2f")
 _ATTN_TC = struct.Struct("@13P16i2f")
 _functions: dict = {}
+# (a call gets here with tensors of the device, so that there is one has been found out)
+_raw_stream, _device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 _NO_CPU = "brolm_b200 kernels run on CUDA tensors only; there is no CPU path"
 
 
@@ -50,7 +52,9 @@ def _call(lib: str, name: str, packed: bytes, what: str) -> None:
     f = _functions.get(name)
     if f is None:
         f = _functions[name] = _fn(lib, name, [c_char_p])
-    _check(f(packed), what)
+    status = f(packed)
+    if status:
+        _check(status, what)
 
 
 def _refuse_ints(what: str, **named) -> None:
@@ -101,7 +105,7 @@ def blocks_extend(slots: torch.Tensor, lengths: torch.Tensor, new: torch.Tensor,
     _call("blocks", "brolm_blocks_extend", _EXTEND.pack(
         slots.data_ptr(), lengths.data_ptr(), new.data_ptr(), tables.data_ptr(), held.data_ptr(), free.data_ptr(),
         free_count.data_ptr(), cu_q.data_ptr(), kv_len.data_ptr(), positions.data_ptr(), tok_seq.data_ptr(),
-        cache_rows.data_ptr(), status.data_ptr(), _stream(), n, S, W, N, block, ring, T, 1 if settle else 0), what)
+        cache_rows.data_ptr(), status.data_ptr(), _raw_stream(_device()), n, S, W, N, block, ring, T, 1 if settle else 0), what)
 
 
 def blocks_release(slots: torch.Tensor, tables: torch.Tensor, held: torch.Tensor, free: torch.Tensor, free_count: torch.Tensor, *,
@@ -118,7 +122,7 @@ def blocks_release(slots: torch.Tensor, tables: torch.Tensor, held: torch.Tensor
         _refuse_ints(what, slots=(slots, n), tables=(tables, None), held=(held, S), free=(free, N), free_count=(free_count, 1),
                      status=(status, 1))
     _call("blocks", "brolm_blocks_release", _RELEASE.pack(
-        slots.data_ptr(), tables.data_ptr(), held.data_ptr(), free.data_ptr(), free_count.data_ptr(), status.data_ptr(), _stream(),
+        slots.data_ptr(), tables.data_ptr(), held.data_ptr(), free.data_ptr(), free_count.data_ptr(), status.data_ptr(), _raw_stream(_device()),
         n, S, W, N), what)
 
 
@@ -167,7 +171,7 @@ def kv8_write(k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, positions: t
         _refuse_ints(what, cu_q=(cu_q, None), positions=(positions, T), cache_rows=(cache_rows, T))
     _call("kv8", "brolm_kv8_write", _WRITE.pack(
         k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), positions.data_ptr(), cache_rows.data_ptr(), k_pages.data_ptr(),
-        v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), _stream(), k0, v0, k1, v1, code, T, rows, n_kv, dim, block,
+        v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), _raw_stream(_device()), k0, v0, k1, v1, code, T, rows, n_kv, dim, block,
         n_blocks, max_q_len), what)
 
 
@@ -190,7 +194,7 @@ def kv8_read(cu_q: torch.Tensor, kv_len: torch.Tensor, slots: torch.Tensor, tabl
         _refuse_ints(what, cu_q=(cu_q, None), kv_len=(kv_len, rows), slots=(slots, rows), tables=(tables, None))
     _call("kv8", "brolm_kv8_read", _READ.pack(
         cu_q.data_ptr(), kv_len.data_ptr(), slots.data_ptr(), tables.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-        k_scale.data_ptr(), v_scale.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), _stream(), k0, v0, k1, v1, code, T, rows, n_kv,
+        k_scale.data_ptr(), v_scale.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), _raw_stream(_device()), k0, v0, k1, v1, code, T, rows, n_kv,
         dim, block, n_blocks, S, W, ring), what)
 
 
@@ -333,20 +337,21 @@ def attention_kv8(q: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, kv_len
     if _odd_ints(cu_q, batch + 1) or _odd_ints(kv_len, batch) or _odd_ints(slots, batch) or _odd_ints(tables, S * W):
         _refuse_ints(what, cu_q=(cu_q, batch + 1), kv_len=(kv_len, batch), slots=(slots, batch), tables=(tables, None))
     T = shape[0]
+    sms = _sms.get(_device()) or device_sms()
     rows = max_q_len * group
     keys = min(max_kv_len, window + max_q_len) if window > 0 else max_kv_len
     if rows >= KV8_TC_ROWS and dt is torch.bfloat16 and n_blocks * n_kv * block < 1 << 31 and \
             float(T) * group * n_kv * keys * max(head_dim, 64) >= KV8_TC_WORK:
-        whole, spans = kv8_tc_spans(T, batch, n_kv, group, max_q_len, keys, head_dim, device_sms())
+        whole, spans = kv8_tc_spans(T, batch, n_kv, group, max_q_len, keys, head_dim, sms)
         part_o = part_ml = 0
         if spans > 1:
             parts, part_o, part_ml, _ = _parts(T * n_kv * group * spans, head_dim, q.device)
         _call("attn_kv8_tc", "brolm_attn_kv8_tc", _ATTN_TC.pack(
             q.data_ptr(), out.data_ptr(), cu_q.data_ptr(), kv_len.data_ptr(), slots.data_ptr(), tables.data_ptr(), k_pages.data_ptr(),
-            v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), part_o, part_ml, _stream(), q0[0], o0[0], T, batch, n_kv, group,
+            v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), part_o, part_ml, _raw_stream(_device()), q0[0], o0[0], T, batch, n_kv, group,
             head_dim, block, n_blocks, S, W, ring, window, max_q_len, whole, spans, scale, cap), what)
         return
-    shares, spans = kv8_shares(batch, n_kv, 1 if rows <= 8 else -(-rows // 16), keys, head_dim, device_sms(), rows > 8,
+    shares, spans = kv8_shares(batch, n_kv, 1 if rows <= 8 else -(-rows // 16), keys, head_dim, sms, rows > 8,
                                3 if rows <= (4 if dt is _F32 else 8) else 2)
     part_o = part_ml = plan = 0
     if spans > 1:
@@ -356,5 +361,5 @@ def attention_kv8(q: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, kv_len
         parts, part_o, part_ml, plan = _parts(-spans * n_kv * -(-rows // tile) * tile, head_dim, q.device, T * n_kv * group)
     _call("attn_kv8", "brolm_attn_kv8", _ATTN.pack(
         q.data_ptr(), out.data_ptr(), cu_q.data_ptr(), kv_len.data_ptr(), slots.data_ptr(), tables.data_ptr(), k_pages.data_ptr(),
-        v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), part_o, part_ml, plan, _stream(), q0[0], o0[0], _CODES[dt], T, batch,
+        v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), part_o, part_ml, plan, _raw_stream(_device()), q0[0], o0[0], _CODES[dt], T, batch,
         n_kv, group, head_dim, block, n_blocks, S, W, ring, window, max_q_len, shares, spans, scale, cap), what)
