@@ -28,6 +28,37 @@ __device__ __forceinline__ void store_row(void* out, int out_stride, int dim, in
     dst[3] = from_float<T>(acc.w * inv);
 }
 
+// Four entries of a row from its parts at, at + step, ..., in their order, and the sum of its weights:
+// sum_s o_s 2^(m_s - m),  sum_s l_s 2^(m_s - m).
+__device__ __forceinline__ float4 join_parts(const float* part_o, const float* part_ml, size_t at, size_t step, int spans, int dim, int d,
+                                             float& sum) {
+    float most = -INFINITY;
+    sum = 0.0f;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int s0 = 0; s0 < spans; s0 += 8) {                  // (eight parts are asked for at once)
+        float2 ml[8];
+        float4 x[8];
+        float top = most;
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+            ml[s] = make_float2(-INFINITY, 0.0f);
+            x[s] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (s0 + s < spans) {
+                ml[s] = *reinterpret_cast<const float2*>(part_ml + (at + (s0 + s) * step) * 2);
+                x[s] = *reinterpret_cast<const float4*>(part_o + (at + (s0 + s) * step) * dim + d);
+            }
+            top = fmaxf(top, ml[s].x);
+        }
+        const float keep = most > -INFINITY ? ex2(most - top) : 1.0f;
+        most = top;
+        sum *= keep;
+        acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+            if (s0 + s < spans) add_part(acc, sum, x[s], ml[s].y, top > -INFINITY ? ex2(ml[s].x - top) : 0.0f);
+    }
+    return acc;
+}
 
 struct JoinArgs {
     const float *part_o, *part_ml;        // [token][head][span][dim] and [..][2]
@@ -36,7 +67,6 @@ struct JoinArgs {
     int out_stride, rows, tokens, heads, dim, spans;
     const int2* plan = nullptr;           // where given, [token][head]: the first part and how many, every `step` parts
     int step = 1, parts = 0;              // (the parts that there are: nothing is read beyond them)
-    bool some = false;                    // some rows are in their places: their first part's sum is -1
 };
 
 // Rows whose keys were shared by several blocks that do not join their results themselves: a thread for four entries of a
@@ -58,32 +88,8 @@ __global__ void __launch_bounds__(JOIN_THREADS) attn_kv8_join_kernel(JoinArgs a)
         spans = p.y;
         if (spans <= 1 || p.x < 0 || p.x + (long long)(spans - 1) * a.step >= a.parts) return;     // (one part is in its place)
     }
-    if (a.some && a.part_ml[at * 2 + 1] < 0.0f) return;
-    const size_t step = a.step;
-    float most = -INFINITY, sum = 0.0f;
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int s0 = 0; s0 < spans; s0 += 8) {                  // (eight parts are asked for at once)
-        float2 ml[8];
-        float4 x[8];
-        float top = most;
-#pragma unroll
-        for (int s = 0; s < 8; ++s) {
-            ml[s] = make_float2(-INFINITY, 0.0f);
-            x[s] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (s0 + s < spans) {
-                ml[s] = *reinterpret_cast<const float2*>(a.part_ml + (at + (s0 + s) * step) * 2);
-                x[s] = *reinterpret_cast<const float4*>(a.part_o + (at + (s0 + s) * step) * a.dim + d);
-            }
-            top = fmaxf(top, ml[s].x);
-        }
-        const float keep = most > -INFINITY ? ex2(most - top) : 1.0f;
-        most = top;
-        sum *= keep;
-        acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
-#pragma unroll
-        for (int s = 0; s < 8; ++s)
-            if (s0 + s < spans) add_part(acc, sum, x[s], ml[s].y, top > -INFINITY ? ex2(ml[s].x - top) : 0.0f);
-    }
+    float sum;
+    const float4 acc = join_parts(a.part_o, a.part_ml, at, a.step, spans, a.dim, d, sum);
     store_row<T>(a.out, a.out_stride, a.dim, tok, head, d, acc, sum);
 }
 

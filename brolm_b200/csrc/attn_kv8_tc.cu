@@ -665,9 +665,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
             const bool nan = total != total;
             const int row = row0 + r, tok = first_tok + row / a.group, head = g * a.group + row % a.group;
             bf16* dst = a.out + (size_t)tok * a.out_stride + (size_t)head * a.dim;
-            const size_t share = ((size_t)tok * a.n_kv * a.group + head) * a.spans + span;
-            if (a.spans > 1 && row_ok && part == 0)          // (a row that is in its place: a sum that cannot be)
-                *reinterpret_cast<float2*>(a.part_ml + share * 2) = spans > 1 ? make_float2(m_ref, total) : make_float2(-INFINITY, -1.0f);
+            const size_t share = ((size_t)(item - a.whole) * spans + span) * BM + r;      // (where there are several)
+            if (spans > 1 && row_ok && part == 0) *reinterpret_cast<float2*>(a.part_ml + share * 2) = make_float2(m_ref, total);
             const bool wide = ((uintptr_t)a.out & 15) == 0 && (a.out_stride & 7) == 0;
 #pragma unroll 1
             for (int c = part * OUT; c < min((part + 1) * OUT, a.dim); c += 16) {
@@ -712,6 +711,22 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
     if (warp == ISSUER) tmem_dealloc(tmem, TMEM_COLS);
 }
 
+// The rows of the tiles whose keys were shared: a thread for four entries of a row.
+constexpr int JOIN_CHUNK = 256;
+__global__ void __launch_bounds__(JOIN_CHUNK) attn_kv8_tc_join_kernel(TcArgs a) {
+    pdl_trigger();
+    pdl_wait();
+    const int per = a.dim >> 2, each = JOIN_CHUNK / per, chunks = (BM + each - 1) / each, mine = threadIdx.x / per;
+    const int tile = blockIdx.x / chunks, r = (blockIdx.x - tile * chunks) * each + mine, d = (threadIdx.x - mine * per) * 4;
+    const int item = a.whole + tile, xt = a.row_tiles - 1 - item / (a.n_kv * a.rows), which = item % (a.n_kv * a.rows);
+    const int b = which / a.n_kv, g = which - b * a.n_kv, row = xt * BM + r;
+    const int first_tok = a.cu_q[b], n_tok = min(a.cu_q[b + 1], a.tokens) - first_tok;
+    if (mine >= each || r >= BM || first_tok < 0 || row >= (long long)n_tok * a.group) return;
+    float sum;
+    const float4 acc = join_parts(a.part_o, a.part_ml, (size_t)tile * a.spans * BM + r, BM, a.spans, a.dim, d, sum);
+    store_row<bf16>(a.out, a.out_stride, a.dim, first_tok + row / a.group, g * a.group + row % a.group, d, acc, sum);
+}
+
 // The rows of the pages [rows][dim] of bytes; box = box_bytes x 32 rows, zeros beyond a row's end.
 int make_map(CUtensorMap* map, const void* ptr, long long rows, int dim, int box_bytes) {
     EncodeTiled enc = encoder();
@@ -743,11 +758,11 @@ int launch(const TcArgs& a, cudaStream_t stream) {
     if (st) return st;
     st = launch_pdl(attn_kv8_tc_kernel<HD>, dim3((unsigned)blocks), dim3(THREADS), smem, stream, mk, mv, a);
     if (st || a.spans == 1) return st;
-    JoinArgs j{a.part_o, a.part_ml, a.out, a.cu_q, a.out_stride, a.rows, a.tokens, a.n_kv * a.group, a.dim, a.spans};
-    j.some = a.whole > 0;
-    if (a.rows == 1)                      // (one sequence: the tiles that are shared are those of its first tokens)
-        j.tokens = min(a.tokens, ((a.row_tiles - a.whole / a.n_kv) * BM + a.group - 1) / a.group);
-    return launch_join<bf16>(j, stream);
+    const int each = JOIN_CHUNK / (a.dim >> 2);
+    const long long shared = (long long)a.row_tiles * a.n_kv * a.rows - a.whole, joins = shared * ((BM + each - 1) / each);
+    if (shared == 0) return st;
+    if (joins > 0x7fffffffll) return BROLM_ERR_TOO_LARGE;
+    return launch_pdl(attn_kv8_tc_join_kernel, dim3((unsigned)joins), dim3(JOIN_CHUNK), 0, stream, a);
 }
 
 }  // namespace
@@ -756,7 +771,7 @@ struct AttnTcCall {
     const void* q;
     void* out;
     const void *cu_q, *kv_len, *slots, *tables, *k_pages, *v_pages, *k_scale, *v_scale;
-    void *part_o, *part_ml;               // spans > 1, for all row tiles but the first `whole`: [tokens * n_kv * group * spans * dim] and [.. * 2]
+    void *part_o, *part_ml;               // spans > 1: [(tiles of 128 rows - whole) * spans * 128 * dim] and [.. * 2]
     cudaStream_t stream;
     int q_stride, out_stride, tokens, rows, n_kv, group, dim, block, n_blocks, n_slots, width, ring, window, max_q_len, whole, spans;
     float scale, cap;

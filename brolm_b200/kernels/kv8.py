@@ -345,7 +345,7 @@ def attention_kv8(q: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, kv_len
         whole, spans = kv8_tc_spans(T, batch, n_kv, group, max_q_len, keys, head_dim, sms)
         part_o = part_ml = 0
         if spans > 1:
-            parts, part_o, part_ml, _ = _parts(T * n_kv * group * spans, head_dim, q.device)
+            parts, part_o, part_ml, _ = _parts((batch * n_kv * -(-rows // 128) - whole) * spans * 128, head_dim, q.device)
         _call("attn_kv8_tc", "brolm_attn_kv8_tc", _ATTN_TC.pack(
             q.data_ptr(), out.data_ptr(), cu_q.data_ptr(), kv_len.data_ptr(), slots.data_ptr(), tables.data_ptr(), k_pages.data_ptr(),
             v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), part_o, part_ml, _raw_stream(_device()), q0[0], o0[0], T, batch, n_kv, group,
