@@ -271,7 +271,7 @@ def kv8_tc_spans(tokens: int, batch: int, n_kv: int, group: int, max_q_len: int,
     In tiles of 128 keys (about 2.6 us each at 256 entries, counted as 3): a block begins and ends in three, and joining costs another three and
     what the parts take to memory and back.  Where the last round would be far from full, its tiles alone are shared
     (on 14,336 keys, 8 kv heads of 256, two query heads each, us with a block for a tile / four / the last round's
-    shared: 1,280 tokens, 160 tiles on 148 SMs, 571 / 446 / 353; 1,700, 216 tiles, 573 / 545 / 472; 2,048, 256, 568 / 653 / 564)."""
+    shared: 1,280 tokens, 160 tiles on 148 SMs, 560 / 449 / 343; 1,700, 216 tiles, 564 / 553 / 459; 2,048, 256, 560 / 638 / 573)."""
     items = batch * n_kv * -(-max_q_len * group // 128)
     tiles = -(-keys // 128)
     traffic = tokens * n_kv * group * head_dim * 8 / 6.5e12 / (3e-6 * head_dim / 256)
