@@ -28,7 +28,9 @@
 // 2^(z - m) 2^(e - e0), e0 the largest exponent of the keys this block of threads sees, and m the row's running maximum of
 // z + e - e0, so that what is rounded to f16 is at most 2^8 and exact to 11 bits for all that matters to the sum, however
 // the blocks' scales differ; the sum of 2^(z - m) is kept in 32 bits, without the values' scales.  (m is raised only when it
-// would be passed by more than 8: the accumulator in tensor memory is then scaled anew.)  A query row is scaled by a power
+// would be passed by more than 8: the accumulator in tensor memory is then scaled anew.)  Beside a block whose scale is 2^60
+// above a key's, 2^(z - m) may be beyond a float (a block of zeros has the least scale there is): such keys' weights go into
+// a sum of their own, relative to the largest of their own z, and the two are added up at the end.  A query row is scaled by a power
 // of two to below 2^14 and held in f16, exactly but for numbers 2^-38 of the row's largest.
 //
 // What bounds it: of a tile of 128 keys and 256 entries, about 5,000 cycles (2,048 tokens on 14,336 keys, 8 kv heads of 256,
@@ -226,7 +228,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
     Meta* meta = reinterpret_cast<Meta*>(rest);              // [2][CHUNK][4]
     float* xch = reinterpret_cast<float*>(meta + 2 * CHUNK * 4);     // [2][4][BM]: maxima by tile parity and part; the sums reuse it
     float* q_scale = xch + 8 * BM;                           // [BM]
-    uint64_t* bars = reinterpret_cast<uint64_t*>(q_scale + BM);
+    float2* far_sums = reinterpret_cast<float2*>(q_scale + BM);   // [4][BM]: sums of weights of values far below the largest, and their reference
+    uint64_t* bars = reinterpret_cast<uint64_t*>(far_sums + 4 * BM);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + U_FULL + 2 * SLOTS + 2 * RAWS);
     volatile int* give_up = reinterpret_cast<volatile int*>(tmem_slot + 1);       // three
     volatile int* top_exp = reinterpret_cast<volatile int*>(tmem_slot + 4);
@@ -534,6 +537,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
         const uint64_t t0 = pair_of(c1 * 0.9999999f, c1 * 0.9999999f), t1 = pair_of(c1 * -0.33331362f, c1 * -0.33331362f);
         const uint64_t t2 = pair_of(c1 * 0.13270977f, c1 * 0.13270977f), t3 = pair_of(c1 * -0.047553604f, c1 * -0.047553604f);
         float m_ref = -INFINITY, l = 0.0f;                   // l: the sum over this thread's columns only
+        far_sums[part * BM + r] = make_float2(0.0f, -INFINITY);
         bool ok = true, sees_bad = false;
         for (int j = 0; j < n_tiles; ++j) {
             const int s = j & 1;
@@ -636,12 +640,23 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
                 const float2 sum = halves(sums);
                 l = fmaf(sum.x + sum.y, power_of_two(-ve), l);
             } else {
-                // scales more than 2^60 apart: what a weight is without its scale may be lost with it.  (It may be infinite
-                // here: the row's result is then 0, which it is beside the values of the largest scale.)
+                // scales more than 2^60 apart: what a weight is without its scale may be lost with it, or pass a float's range
+                // relative to m
+                float2 sum = far_sums[part * BM + r];
+                float top = sum.y;
 #pragma unroll
                 for (int c = 0; c < W / 2; ++c) {
                     const float2 x = halves(z[c]);
-                    l += fast_exp2(x.x - m_sub) + fast_exp2(x.y - m_sub);
+                    top = max3(top, x.x, x.y);
+                }
+                if (top > -INFINITY) {
+                    sum.x *= fast_exp2(sum.y - top);
+#pragma unroll
+                    for (int c = 0; c < W / 2; ++c) {
+                        const float2 x = halves(z[c]);
+                        sum.x += fast_exp2(x.x - top) + fast_exp2(x.y - top);
+                    }
+                    far_sums[part * BM + r] = make_float2(sum.x, top);
                 }
             }
             tmem_wait_st();
@@ -657,16 +672,24 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
         float* last = xch + (n_tiles & 1) * 4 * BM;          // the buffer that the next tile would have used
         last[part * BM + r] = sees_bad || (qs != qs && pos >= 0) ? __int_as_float(0x7fc00000) : qs != qs ? 0.0f : l;
         asm volatile("bar.sync %0, 128;" ::"r"(1 + quarter) : "memory");
-        const float total = (last[r] + last[BM + r]) + (last[2 * BM + r] + last[3 * BM + r]);
+        float total = (last[r] + last[BM + r]) + (last[2 * BM + r] + last[3 * BM + r]);
         if (ok) {
             fence_after_sync();
+            float v0 = power_of_two(e0), ref = m_ref;
+            const float far_ref = max3(fmaxf(far_sums[r].y, far_sums[BM + r].y), far_sums[2 * BM + r].y, far_sums[3 * BM + r].y);
+            if (far_ref > -INFINITY) {                       // (m is finite, too)
+                ref = fmaxf(m_ref, far_ref);
+                total *= fast_exp2(m_ref - ref);
+#pragma unroll
+                for (int p = 0; p < 4; ++p) total = fmaf(far_sums[p * BM + r].x, fast_exp2(far_sums[p * BM + r].y - ref), total);
+                v0 = fast_exp2((float)e0 + (m_ref - ref));
+            }
             const float inv = total > 0.0f ? 1.0f / total : 0.0f;
-            const float v0 = power_of_two(e0);
             const bool nan = total != total;
             const int row = row0 + r, tok = first_tok + row / a.group, head = g * a.group + row % a.group;
             bf16* dst = a.out + (size_t)tok * a.out_stride + (size_t)head * a.dim;
             const size_t share = ((size_t)(item - a.whole) * spans + span) * BM + r;      // (where there are several)
-            if (spans > 1 && row_ok && part == 0) *reinterpret_cast<float2*>(a.part_ml + share * 2) = make_float2(m_ref, total);
+            if (spans > 1 && row_ok && part == 0) *reinterpret_cast<float2*>(a.part_ml + share * 2) = make_float2(ref, total);
             const bool wide = ((uintptr_t)a.out & 15) == 0 && (a.out_stride & 7) == 0;
 #pragma unroll 1
             for (int c = part * OUT; c < min((part + 1) * OUT, a.dim); c += 16) {
@@ -743,7 +766,7 @@ int make_map(CUtensorMap* map, const void* ptr, long long rows, int dim, int box
 template <int HD>
 int launch(const TcArgs& a, cudaStream_t stream) {
     using SH = Shape<HD>;
-    constexpr size_t smem = (size_t)SH::Q_BYTES + (size_t)SH::SLOTS * UNIT + RAWS * RAW + 2 * CHUNK * 4 * sizeof(Meta) + 9 * BM * 4 +
+    constexpr size_t smem = (size_t)SH::Q_BYTES + (size_t)SH::SLOTS * UNIT + RAWS * RAW + 2 * CHUNK * 4 * sizeof(Meta) + 9 * BM * 4 + 4 * BM * 8 +
                             (U_FULL + 2 * SH::SLOTS + 2 * RAWS) * 8 + 32;
     static_assert(smem <= 232448, "shared memory of a block");
     static OncePerDevice raised;

@@ -723,3 +723,51 @@ def test_a_piece_whose_wait_runs_out(code, on_tcgen05):
     finally:
         kernels.wait_control("attn_kv8_tc", 0, 0)
     assert torch.equal(run(), good) and kernels.attention_kv8_tc_status() == 0
+
+
+# --- sums of weights beside values of other sizes ------------------------------------------------------------------------
+def small_beside_large(sizes, dtype=torch.float32):
+    """A sequence of blocks of 64 tokens whose values are about 1 times ``sizes``, one after the other."""
+    c = Cached(1, len(sizes), 1, 64, 64, seed=7)
+    g = torch.Generator().manual_seed(3)
+    for size in sizes:
+        k, v = (rows_of(64, 1, 64, torch.float32, g, 0.2) for _ in range(2))
+        c.write([0], [64], k, (v.abs() + 1.0) * size)
+    return c
+
+
+@pytest.mark.parametrize("shared", [None, (0, 1), (0, 3), (1, 2)], ids=str)
+@pytest.mark.parametrize("new", [1, 5, 100])
+def test_many_values_of_zero_before_values_that_are_not(new, shared, either, monkeypatch):
+    """Blocks of zeros have the least scale there is, 2^-126: their weights count in the sum all the same, however many come
+    before the first value, and whatever its size."""
+    if shared:
+        monkeypatch.setattr(kernels.kv8, "kv8_tc_spans", lambda *a: shared)
+    for sizes in ([0.0] * 40 + [1.0], [0.0] * 20 + [1.0] + [0.0] * 20 + [2.0 ** 12] * 2, [1.0] + [0.0] * 30 + [2.0 ** 40, 0.0, 0.0]):
+        c = small_beside_large(sizes)
+        for dtype in (torch.bfloat16, torch.float32):
+            got = compare(c, dtype, [0], [new], 2, 0.125, 0.0, 0)
+            assert not torch.isnan(got).any()
+
+
+@pytest.mark.parametrize("shared", [None, (0, 1), (0, 2)], ids=str)
+def test_rows_that_see_small_values_alone_keep_them(shared, either, monkeypatch):
+    """Rows of one tile under a window of 20: those that see values of 2^-60 alone are as near to 64 bits, beside what they
+    see, as those that see values of 2^70 (or of both)."""
+    if shared:
+        monkeypatch.setattr(kernels.kv8, "kv8_tc_spans", lambda *a: shared)
+    c = small_beside_large([2.0 ** -60, 2.0 ** 70, 2.0 ** -60, 2.0 ** -60, 2.0 ** 70])
+    n, new = 320, 250
+    for dtype in (torch.bfloat16, torch.float32):
+        q = torch.randn((new, 64), generator=torch.Generator().manual_seed(5)).to(dtype).to(DEV)
+        out = torch.empty_like(q)
+        kernels.attention_kv8(q, out, ints([0, new]), ints([n]), ints([0]), c.tables, *c.dev, n_kv=1, group=1, head_dim=64, scale=0.125,
+                              cap=0.0, window=20, ring=0, batch=1, max_q_len=new, max_kv_len=n)
+        keys, values = c.values(0, 0)[1], c.values(1, 0)[1]
+        for j in range(new):
+            p = n - new + j
+            lo = max(0, p - 19)
+            qj = q[j].cpu().view(1, 64)
+            ref = plain.attend(qj, keys, values, 0, p, 0.125, 0.0, 20)
+            off = (out[j].cpu().double().view(1, 64) - ref).abs() - bound(dtype, ref, qj, keys[lo:p + 1], values[lo:p + 1], 0.125)
+            assert float(off.max()) <= 0.0, (dtype, j, float(off.max()))
