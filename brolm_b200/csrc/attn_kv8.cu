@@ -566,7 +566,7 @@ __global__ void __launch_bounds__(THREADS, 2) attn_kv8_few_kernel(AttnArgs a) {
     // this thread's row of a tile: 2 q + t4 / 2 (and the two low digits of its scores where t4 is odd)
     const float unit = a.cap > 0.0f ? (EXACT ? a.scale / a.cap : a.scale / a.cap * (2.0f * LOG2E)) : a.scale * LOG2E;
     const float c1 = a.cap * LOG2E, c2 = 2.0f * a.cap * LOG2E;
-    const int window = a.window > 0 ? a.window : 0x3fffffff;
+    const int window = a.window > 0 ? a.window : ALL_KEYS;
     const float weight = t4 & 1 ? 1.0f : 65536.0f;
     float qf[QT], m[QT], l[QT];
     int pos[QT];
@@ -880,7 +880,7 @@ __global__ void __launch_bounds__(THREADS, 2) attn_kv8_kernel(AttnArgs a) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) o[s][i][nt][0] = o[s][i][nt][1] = o[s][i][nt][2] = o[s][i][nt][3] = 0.0f;
 
-    const int window = a.window > 0 ? a.window : 0x3fffffff;
+    const int window = a.window > 0 ? a.window : ALL_KEYS;
     const uint32_t q_frag = smem_addr(smem) + lane * 16;
 
     for (int n = 0; n < tiles.n_tiles; ++n) {
@@ -1146,7 +1146,7 @@ BROLM_API int brolm_attn_kv8(const AttnCall* c) {
     AttnArgs a{c->q, c->out, c->q_stride, c->out_stride, (const int32_t*)c->cu_q, (const int32_t*)c->kv_len,
                (const int32_t*)c->slots, (const int32_t*)c->tables, (const int8_t*)c->k_pages, (const int8_t*)c->v_pages,
                (const float*)c->k_scale, (const float*)c->v_scale, c->tokens, c->rows, n_kv, group, dim, block, c->n_blocks,
-               c->n_slots, c->width, c->ring, c->window, c->scale, c->cap, c->shares, max(c->spans, 1), (most + per - 1) / per, wide,
+               c->n_slots, c->width, c->ring, min(c->window, ALL_KEYS), c->scale, c->cap, c->shares, max(c->spans, 1), (most + per - 1) / per, wide,
                max(-c->spans, 0), (float*)c->part_o, (float*)c->part_ml, (int2*)c->plan};
     if ((long long)a.dealt * a.row_tiles * n_kv * per > 0x7fffffffll) return BROLM_ERR_TOO_LARGE;
     return c->dtype == BROLM_F32 ? launch_dim<float>(a, per, c->stream) : launch_dim<bf16>(a, per, c->stream);

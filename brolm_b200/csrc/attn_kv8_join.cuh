@@ -7,6 +7,9 @@
 namespace kv8 {
 
 constexpr float LOG2E = 1.4426950408889634f;
+// What a window is where there is none, and at most: a cache has fewer than 2^31 places, and a position less this many tokens
+// and a tile or two is still a whole number of 32 bits.
+constexpr int ALL_KEYS = 0x7ffff000;
 
 __device__ __forceinline__ float ex2(float x) {
     float y;

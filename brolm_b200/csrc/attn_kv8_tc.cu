@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
     const int row0 = xt * BM;
     const int rows_here = first_tok < 0 ? 0 : (int)min((long long)BM, (long long)n_tok * a.group - row0);
     if (rows_here <= 0) return;                              // (the whole block)
-    const int window = a.window > 0 ? a.window : 0x3fffffff;
+    const int window = a.window > 0 ? a.window : ALL_KEYS;
     const int pos0 = kv_len - n_tok, pos_lo = pos0 + row0 / a.group, pos_hi = pos0 + (row0 + rows_here - 1) / a.group;
     int t_first = 0, n_tiles = 0;
     if (pos_hi >= 0 && slot >= 0 && slot < a.n_slots) {
@@ -819,7 +819,7 @@ BROLM_API int brolm_attn_kv8_tc(const AttnTcCall* c) {
     TcArgs a{(const bf16*)c->q, (bf16*)c->out, c->q_stride, c->out_stride, (const int32_t*)c->cu_q, (const int32_t*)c->kv_len,
              (const int32_t*)c->slots, (const int32_t*)c->tables, (const int8_t*)c->k_pages, (const int8_t*)c->v_pages,
              (const float*)c->k_scale, (const float*)c->v_scale, c->tokens, c->rows, n_kv, group, c->dim, block, c->n_blocks, c->n_slots,
-             c->width, c->ring, c->window, row_tiles, wide, c->scale, c->cap, c->whole, c->spans, (float*)c->part_o, (float*)c->part_ml};
+             c->width, c->ring, min(c->window, ALL_KEYS), row_tiles, wide, c->scale, c->cap, c->whole, c->spans, (float*)c->part_o, (float*)c->part_ml};
     if (c->dim <= 64) return launch<64>(a, c->stream);
     if (c->dim <= 128) return launch<128>(a, c->stream);
     return launch<256>(a, c->stream);

@@ -771,3 +771,32 @@ def test_rows_that_see_small_values_alone_keep_them(shared, either, monkeypatch)
             ref = plain.attend(qj, keys, values, 0, p, 0.125, 0.0, 20)
             off = (out[j].cpu().double().view(1, 64) - ref).abs() - bound(dtype, ref, qj, keys[lo:p + 1], values[lo:p + 1], 0.125)
             assert float(off.max()) <= 0.0, (dtype, j, float(off.max()))
+
+
+@pytest.mark.parametrize("dtype,new", [(torch.bfloat16, 1), (torch.float32, 1), (torch.bfloat16, 10), (torch.float32, 10),
+                                       (torch.bfloat16, 40)])
+def test_a_sequence_of_more_than_2_to_the_30_tokens(dtype, new, on_tcgen05):
+    """Without a window the newest token sees the first ones.  The first 4,096 keys lie in one block's worth of numbers and
+    all others in another's; scores of 15 and 0 give the first e^15 2^12 of e^15 2^12 + 2^30 parts of the weight, values of 1
+    and -1 so 0.8515.  (Sums of so many equal numbers lose up to 2^-25 of themselves with each: 2^18 of them, a warp's or a
+    thread's share, 2^-7.)"""
+    P, D, n = 256, 16, (1 << 30) + 4096
+    key = torch.zeros((2 * P, 1, D), device=DEV)
+    key[:P, 0, 0] = 15.0
+    value = torch.ones((2 * P, 1, D), device=DEV)
+    value[P:] = -1.0
+    dev = [torch.zeros((2, 1, P, D), dtype=torch.int8, device=DEV) for _ in range(2)] + [torch.zeros((2, 1), device=DEV) for _ in range(2)]
+    kernels.kv8_write(key, value, ints([0, 2 * P]), ints(range(2 * P)), ints(range(2 * P)), *dev, max_q_len=2 * P)
+    table = torch.ones((1, n // P), dtype=I32, device=DEV)
+    table[0, :4096 // P] = 0
+    q = torch.zeros((new, D), dtype=dtype, device=DEV)
+    q[:, 0] = 1.0
+    out = torch.empty_like(q)
+    kernels.attention_kv8(q, out, ints([0, new]), ints([n]), ints([0]), table, *dev, n_kv=1, group=1, head_dim=D, scale=1.0, cap=0.0,
+                          window=0, ring=0, batch=1, max_q_len=new, max_kv_len=n)
+    share = math.exp(15.0) * 4096 / (math.exp(15.0) * 4096 + 2.0 ** 30)
+    off = (out.cpu().double() - (2.0 * share - 1.0)).abs().max()
+    assert kernels.attention_kv8_tc_status() == 0 and float(off) <= 2.0 ** -7 + 2.0 ** -8
+    k, v = torch.empty((2, 3, 1, D), device=DEV)
+    kernels.kv8_read(ints([0, 3]), ints([n]), ints([0]), table, *dev, k, v, max_q_len=3)
+    assert bool((v == -1.0).all()) and not k.any()
