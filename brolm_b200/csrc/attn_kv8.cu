@@ -300,7 +300,9 @@ __device__ __forceinline__ Item find_item(const AttnArgs& a) {
     return it;
 }
 
-// A warp's tiles of keys and values on their way into its part of shared memory.
+// A warp's tiles of keys and values on their way into its part of shared memory.  A tile whose place in the tables is none of
+// the cache's has the value scale GONE, and nobody sees its keys.
+constexpr float GONE = -1.0f;
 template <int DP, int SLOTS>
 struct TileRing {
     static constexpr int UNIT = KT * DP;                       // a key or value tile
@@ -328,12 +330,16 @@ struct TileRing {
         if (n + lane < n_tiles) {
             const long long key = (long long)(t0 + (n + lane) * WARPS) * KT;
             const int place = a.ring > 0 ? (int)(key % a.ring) : (int)key, e = place / a.block;
-            int id = e < a.width ? table[e] : 0;
-            if (id < 0 || id >= a.n_blocks) id = 0;            // (never followed out of the cache)
+            int id = e < a.width ? table[e] : -1;
+            const bool gone = id < 0 || id >= a.n_blocks;      // (never followed out of the cache: its tile is read elsewhere)
+            if (gone) id = 0;
             const size_t bh = (size_t)id * a.n_kv + g;
             place_l = (long long)bh * a.block + (place - e * a.block);
-            sk_l = a.k_scale[bh];
-            sv_l = a.v_scale[bh];                              // (nothing waits for the scales before their first use)
+            sv_l = GONE;
+            if (!gone) {
+                sk_l = a.k_scale[bh];
+                sv_l = a.v_scale[bh];                          // (nothing waits for the scales before their first use)
+            }
         }
     }
     __device__ __forceinline__ void load(int u) {              // key tile u / 2 or value tile u / 2 into slot u % SLOTS
@@ -589,7 +595,7 @@ __global__ void __launch_bounds__(THREADS, 2) attn_kv8_few_kernel(AttnArgs a) {
 
     for (int n = 0; n < tiles.n_tiles; ++n) {
         const float2 sc = tiles.scales(n);
-        const int key0 = (tiles.t0 + n * WARPS) * KT;
+        const int key0 = sc.y == GONE ? NOWHERE : (tiles.t0 + n * WARPS) * KT;
         uint32_t tile = tiles.next();
 
         // S^T: keys 16 mt + g8 (+ 8) by digits 2 t4 (+ 1); two sums where there are few, so that one need not wait for the last
@@ -885,7 +891,7 @@ __global__ void __launch_bounds__(THREADS, 2) attn_kv8_kernel(AttnArgs a) {
 
     for (int n = 0; n < tiles.n_tiles; ++n) {
         const float2 sc = tiles.scales(n);
-        const int key0 = (tiles.t0 + n * WARPS) * KT;
+        const int key0 = sc.y == GONE ? NOWHERE : (tiles.t0 + n * WARPS) * KT;
         uint32_t tile = tiles.next();
 
         // S^T: keys 16 mt + g8 (+ 8) by query rows 2 t4 (+ 1)

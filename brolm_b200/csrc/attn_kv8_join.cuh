@@ -10,6 +10,8 @@ constexpr float LOG2E = 1.4426950408889634f;
 // What a window is where there is none, and at most: a cache has fewer than 2^31 places, and a position less this many tokens
 // and a tile or two is still a whole number of 32 bits.
 constexpr int ALL_KEYS = 0x7ffff000;
+// Where keys lie whose place in the tables is none of the cache's: behind every token, so that none sees them.
+constexpr int NOWHERE = 0x7fffff00;
 
 __device__ __forceinline__ float ex2(float x) {
     float y;

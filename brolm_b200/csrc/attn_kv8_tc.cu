@@ -107,9 +107,9 @@ enum : int { S_FULL = 0, P_FULL = 2, PV_DONE = 4, META_FULL = 6, META_EMPTY = 8,
 struct Meta {                             // of a group of 32 keys
     int row;                              // the group's first row in the pages
     float k_scale;
-    int v_exp;                            // exponent of the value scale; BAD: a scale that is NaN
+    int v_exp;                            // exponent of the value scale; BAD: a scale that is NaN; GONE: no block of the cache
 };
-constexpr int BAD = 0x7fffffff;
+constexpr int BAD = 0x7fffffff, GONE = 0x7ffffffe;
 
 __device__ __forceinline__ uint32_t idesc_f16(int m, int n, int b_mn_major) {
     return (1u << 4) | ((uint32_t)b_mn_major << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
@@ -301,8 +301,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
     const int block32 = a.block >> 5;
     auto block_of = [&](int place32) -> int {
         const int e = place32 / block32;
-        const int id = e < a.width ? table[e] : 0;
-        return id >= 0 && id < a.n_blocks ? id : 0;          // (never followed out of the cache)
+        const int id = e < a.width ? table[e] : -1;
+        return id < a.n_blocks ? id : -1;                    // (below 0: none of the cache's, and nobody sees its keys)
     };
 
     if (warp >= ISSUER) {
@@ -314,14 +314,18 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
                 Meta x{0, 0.0f, 0};
                 if (at32 <= key_hi / 32) {
                     const int place32 = a.ring > 0 ? at32 % (a.ring >> 5) : at32;
-                    const size_t bh = (size_t)block_of(place32) * a.n_kv + g;
-                    x.row = (int)bh * a.block + (place32 % block32) * 32;
-                    x.k_scale = a.k_scale[bh];
-                    const float sv = a.v_scale[bh];
-                    x.v_exp = max((int)(__float_as_uint(sv) >> 23 & 255u) - 127, -126);
-                    if (x.k_scale != x.k_scale || sv != sv) {
-                        x.k_scale = 0.0f;
-                        x.v_exp = BAD;
+                    const int id = block_of(place32);
+                    x.v_exp = GONE;
+                    if (id >= 0) {
+                        const size_t bh = (size_t)id * a.n_kv + g;
+                        x.row = (int)bh * a.block + (place32 % block32) * 32;
+                        x.k_scale = a.k_scale[bh];
+                        const float sv = a.v_scale[bh];
+                        x.v_exp = max((int)(__float_as_uint(sv) >> 23 & 255u) - 127, -126);
+                        if (x.k_scale != x.k_scale || sv != sv) {
+                            x.k_scale = 0.0f;
+                            x.v_exp = BAD;
+                        }
                     }
                 }
                 meta[(m & 1) * CHUNK * 4 + lane] = x;
@@ -484,7 +488,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
                 int top = -126;
                 for (int i = threadIdx.x; i * block32 < n32 + block32; i += 32 * SOFTMAX_WARPS) {
                     const int at = min(first32 + i * block32, key_hi / 32);
-                    const float s = a.v_scale[(size_t)block_of(a.ring > 0 ? at % (a.ring >> 5) : at) * a.n_kv + g];
+                    const int id = block_of(a.ring > 0 ? at % (a.ring >> 5) : at);
+                    const float s = id >= 0 ? a.v_scale[(size_t)id * a.n_kv + g] : 0.0f;
                     if (s == s) top = max(top, (int)(__float_as_uint(s) >> 23 & 255u) - 127);
                 }
                 top = __reduce_max_sync(0xffffffffu, top);
@@ -544,7 +549,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
             if (ok && j % CHUNK == 0) ok = wait_warp(bar(META_FULL + ((j / CHUNK) & 1)), (j / CHUNK >> 1) & 1, give_up, 9);
             const Meta& m = meta[((j / CHUNK) & 1) * CHUNK * 4 + (j % CHUNK) * 4 + part];
             const float f = m.k_scale * unit;
-            int ve = m.v_exp == BAD ? BAD : m.v_exp - e0;
+            int ve = m.v_exp >= GONE ? m.v_exp : m.v_exp - e0;
             if (ok) ok = wait_warp(bar(S_FULL + s), (j >> 1) & 1, give_up, 8);
             fence_after_sync();
             const int key_base = (t_first + j) * BN, kp0 = key_base + part * W;
@@ -594,11 +599,12 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const __grid_co
                 const float2 x = halves(z[c]);
                 m_t = max3(m_t, x.x, x.y);
             }
-            if (ve == BAD) {                                 // a NaN block: whoever sees a key of it gets NaN
-                sees_bad = sees_bad || (hi >= 0 && lo < W);
+            float e = (float)ve;
+            if (ve >= GONE) {                                // a NaN block: whoever sees a key of it gets NaN; none: weights of 0
+                if (ve == BAD) sees_bad = sees_bad || (hi >= 0 && lo < W);
+                e = ve == BAD ? 0.0f : -INFINITY;
                 ve = 0;
             }
-            const float e = (float)ve;
             xch[(s * 4 + part) * BM + r] = m_t + e;          // double-buffered by the tile's parity
             // after this barrier all four threads of the row hold their scores in registers, so the weights may go over them
             ok = all_ok(1 + quarter, ok);                    // (a wait that ran out ends all four, or some would wait for the others)

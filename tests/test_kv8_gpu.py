@@ -800,3 +800,42 @@ def test_a_sequence_of_more_than_2_to_the_30_tokens(dtype, new, on_tcgen05):
     k, v = torch.empty((2, 3, 1, D), device=DEV)
     kernels.kv8_read(ints([0, 3]), ints([n]), ints([0]), table, *dev, k, v, max_q_len=3)
     assert bool((v == -1.0).all()) and not k.any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("new", [1, 5, 70])
+@pytest.mark.parametrize("P", [32, 128])
+def test_blocks_that_are_not_the_caches_are_passed_over(dtype, new, P, either):
+    """Ids outside the cache, and places beyond the table's width: nobody's keys are seen there."""
+    c = filled(3, -(-512 // P), 2, P, 64, [500, 300, 64], seed=9)
+    n, group, scale = c.pages[0].shape[0], 2, 0.125
+    table = c.tables.clone()
+    gone = [set(), set(), set()]
+    for i, e, bad in ((0, 1, -1), (0, 3, n), (1, 0, 2 ** 31 - 1), (1, 2, -2 ** 31), (2, 0, -1)):
+        if P == 128 or i < 2:
+            table[i, e] = bad
+            gone[i].add(e)
+    if P == 32:
+        table[2, :2] = n + 5                                 # (a sequence that has nothing left)
+        gone[2] = {0, 1}
+    for width in (table.shape[1], 384 // P):
+        q = torch.randn((3 * new, 4 * 64), generator=torch.Generator().manual_seed(new)).to(dtype).to(DEV)
+        out = torch.full_like(q, 9.0)
+        kernels.attention_kv8(q, out, ints([0, new, 2 * new, 3 * new]), ints(c.lens), ints([0, 1, 2]), table[:, :width].contiguous(), *c.dev,
+                              n_kv=2, group=group, head_dim=64, scale=scale, cap=0.0, window=0, ring=0, batch=3, max_q_len=new,
+                              max_kv_len=500)
+        k, v = (torch.empty((sum(c.lens), 2, 64), device=DEV) for _ in range(2))
+        kernels.kv8_read(ints([0, 500, 800, 864]), ints(c.lens), ints([0, 1, 2]), table[:, :width].contiguous(), *c.dev, k, v, max_q_len=500)
+        at = 0
+        for i, length in enumerate(c.lens):
+            keys, values = c.values(0, i)[1], c.values(1, i)[1]
+            here = torch.tensor([p // P not in gone[i] and p // P < width for p in range(length)])
+            assert same(k[at:at + length].cpu().double(), torch.where(here[:, None, None], keys, 0.0))
+            at += length
+            for j in range(new):
+                p = length - new + j
+                sees = here.nonzero()[:, 0][here.nonzero()[:, 0] <= p]
+                qj = q[i * new + j].cpu().view(4, 64)
+                ref = plain.attend(qj, keys[sees], values[sees], 0, len(sees) - 1, scale, 0.0, 0) if p >= 0 else torch.zeros(4, 64).double()
+                off = (out[i * new + j].cpu().double().view(4, 64) - ref).abs() - bound(dtype, ref, qj, keys, values, scale)
+                assert float(off.max()) <= 0.0, (width, i, j, float(off.max()))
