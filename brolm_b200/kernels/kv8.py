@@ -52,9 +52,7 @@ def _call(lib: str, name: str, packed: bytes, what: str) -> None:
     f = _functions.get(name)
     if f is None:
         f = _functions[name] = _fn(lib, name, [c_char_p])
-    status = f(packed)
-    if status:
-        _check(status, what)
+    _check(f(packed), what)
 
 
 def _refuse_ints(what: str, **named) -> None:

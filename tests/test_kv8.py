@@ -127,3 +127,17 @@ def test_extend_and_release_refusals(change):
     if change in ("tables", "free", "status", "cpu"):
         with pytest.raises(kernels.KernelError):
             kernels.blocks_release(pos["slots"], pos["tables"], pos["held"], pos["free"], pos["free_count"], status=out["status"])
+
+
+def test_calls_are_counted_as_launches(monkeypatch):
+    """What the engine looks at to know whether anything ran since its last check, and what a captured step adds a replay."""
+    from brolm_b200.kernels import kv8
+    results = {"good": 0, "bad": 10002}
+    for name, status in results.items():
+        monkeypatch.setitem(kv8._functions, name, lambda packed, status=status: status)
+    before = kernels.launch_count()
+    kv8._call("kv8", "good", b"", "a call")
+    assert kernels.launch_count() == before + 1
+    with pytest.raises(kernels.KernelError, match="a call"):
+        kv8._call("kv8", "bad", b"", "a call")
+    assert kernels.launch_count() == before + 1
