@@ -174,7 +174,8 @@ class DeviceTables:
         self.tables, self.held = new(num_slots, max(1, width)), new(num_slots)
         self.free = torch.arange(num_pages - 1, -1, -1, dtype=torch.int32, device=device)
         self.free_count = torch.full((1,), num_pages, dtype=torch.int32, device=device)
-        self.status = new(1)
+        # the last call's status, and the first that was not 0 (until the engine, which looks at it now and then, sets it back)
+        self.status, self.refused = new(1), new(1)
 
     def state(self) -> tuple:
         return self.tables, self.held, self.free, self.free_count

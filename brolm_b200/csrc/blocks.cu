@@ -11,7 +11,8 @@
 //
 // A row with slot -1 is padding: its tokens get position and cache row -1, its length is 0.  All or nothing: where the
 // free blocks, a row of the tables or the outputs do not suffice, or a slot is wrong, the state stays as it is, every
-// output reads as padding (lengths and sums 0) and `status` says why.
+// output reads as padding (lengths and sums 0) and `status` says why.  `refused`, where given, keeps the first status that
+// was not 0: the status of a step whose results nobody waits for is soon overwritten by the next one's.
 //
 // What bounds it is latency: a decode step of 64 rows reads and writes 2.6 KB.  One launch does all of it: every block of
 // threads of one cluster adds up all rows by itself (three short arrays out of the L2), which costs less than handing sums
@@ -34,12 +35,18 @@ struct ExtendArgs {
     const int32_t *slots, *lengths, *fresh;        // of the step's rows
     int32_t *tables, *held, *count;
     const int32_t* stack;
-    int32_t *cu_q, *kv_len, *positions, *tok_seq, *cache_rows, *status;
+    int32_t *cu_q, *kv_len, *positions, *tok_seq, *cache_rows, *status, *refused;
     int rows, n_slots, width, stack_size, block, shift, ring, tokens;      // shift: of a block that is a power of two, else -1
 };
 
 __device__ __forceinline__ void cluster_barrier() {
     asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;\n" ::: "memory");
+}
+
+// (by one thread of a launch, and launches that share the words run one after the other)
+__device__ __forceinline__ void tell(int32_t* status, int32_t* refused, int value) {
+    *status = value;
+    if (refused && value != ST_OK && *refused == ST_OK) *refused = value;
 }
 
 __device__ __forceinline__ int blocks_for(long long n, int block, int ring) {
@@ -156,7 +163,7 @@ __global__ void __launch_bounds__(THREADS) blocks_extend_kernel(ExtendArgs a) {
     const int rank = blockIdx.x, me = rank * THREADS + threadIdx.x, all = gridDim.x * THREADS;
     const int n_new = ok ? (int)sums.y : 0, n_tok = ok ? (int)sums.x : 0;
     if (me == 0) {
-        *a.status = status;
+        tell(a.status, a.refused, status);
         if constexpr (CLUSTER) *a.count = count - n_new;
         a.cu_q[a.rows] = n_tok;
     }
@@ -238,7 +245,7 @@ __global__ void __launch_bounds__(THREADS) commit_kernel(ExtendArgs a) {
 // of the same rows puts back in its old order.  Rows with slot -1 are left out; a wrong slot changes nothing.
 struct ReleaseArgs {
     const int32_t *slots, *tables;
-    int32_t *held, *stack, *count, *status;
+    int32_t *held, *stack, *count, *status, *refused;
     int rows, n_slots, width, stack_size;
 };
 
@@ -285,7 +292,7 @@ __global__ void __launch_bounds__(THREADS) blocks_release_kernel(ReleaseArgs a) 
     const int me = blockIdx.x * THREADS + threadIdx.x, all = gridDim.x * THREADS;
     const int n_back = status == ST_OK ? (int)sum : 0;
     if (me == 0) {
-        *a.status = status;
+        tell(a.status, a.refused, status);
         *a.count = count + n_back;
     }
     for (int b = me; b < n_back; b += all) {
@@ -327,13 +334,13 @@ struct ExtendCall {
     const void *slots, *lengths, *fresh;
     void *tables, *held;
     const void* stack;
-    void *count, *cu_q, *kv_len, *positions, *tok_seq, *cache_rows, *status;
+    void *count, *cu_q, *kv_len, *positions, *tok_seq, *cache_rows, *status, *refused;
     cudaStream_t stream;
     int rows, n_slots, width, stack_size, block, ring, tokens, settle;
 };
 struct ReleaseCall {
     const void *slots, *tables;
-    void *held, *stack, *count, *status;
+    void *held, *stack, *count, *status, *refused;
     cudaStream_t stream;
     int rows, n_slots, width, stack_size;
 };
@@ -348,8 +355,8 @@ BROLM_API int brolm_blocks_extend(const ExtendCall* c) {
         if (c->block == 1 << s) shift = s;
     ExtendArgs a{(const int32_t*)c->slots, (const int32_t*)c->lengths, (const int32_t*)c->fresh, (int32_t*)c->tables,
                  (int32_t*)c->held, (int32_t*)c->count, (const int32_t*)c->stack, (int32_t*)c->cu_q, (int32_t*)c->kv_len,
-                 (int32_t*)c->positions, (int32_t*)c->tok_seq, (int32_t*)c->cache_rows, (int32_t*)c->status, c->rows, c->n_slots,
-                 c->width, c->stack_size, c->block, shift, c->ring, c->tokens};
+                 (int32_t*)c->positions, (int32_t*)c->tok_seq, (int32_t*)c->cache_rows, (int32_t*)c->status, (int32_t*)c->refused, c->rows,
+                 c->n_slots, c->width, c->stack_size, c->block, shift, c->ring, c->tokens};
     static OncePerDevice raised;
     const size_t smem = (size_t)(5 * c->rows + 2 + (c->n_slots + 31) / 32) * 4;
     if (c->tokens > 8 * THREADS * 4) {
@@ -374,7 +381,7 @@ BROLM_API int brolm_blocks_release(const ReleaseCall* c) {
     if (c->rows < 0 || c->n_slots <= 0 || c->width <= 0 || c->stack_size < 0) return BROLM_ERR_BAD_SIZE;
     if (c->rows > MAX_ROWS || c->n_slots > MAX_SLOTS) return BROLM_ERR_TOO_LARGE;
     ReleaseArgs a{(const int32_t*)c->slots, (const int32_t*)c->tables, (int32_t*)c->held, (int32_t*)c->stack, (int32_t*)c->count,
-                  (int32_t*)c->status, c->rows, c->n_slots, c->width, c->stack_size};
+                  (int32_t*)c->status, (int32_t*)c->refused, c->rows, c->n_slots, c->width, c->stack_size};
     static OncePerDevice raised;
     const size_t smem = (size_t)(2 * c->rows + 1 + (c->n_slots + 31) / 32) * 4;
     return launch_cluster(blocks_release_kernel, a, (long long)c->rows * 16, smem, raised, c->stream);

@@ -82,7 +82,7 @@ def _extend(cache: Cache, slots, lengths, new, cu_q, kv_len, positions, tok_seq,
         t = g.tables
         kernels.blocks_extend(slots, lengths, new, *t.state(), block=g.page_size, ring=g.ring or 0, cu_q=outs[0], kv_len=outs[1],
                               positions=outs[2], tok_seq=outs[3], cache_rows=cache_rows[i], status=t.status,
-                              settle=i == len(cache.kv_groups) - 1)
+                              refused=t.refused, settle=i == len(cache.kv_groups) - 1)
 
 
 class _DecodeGraph:
@@ -302,14 +302,15 @@ class Engine:
                 self._follow()
                 gone = torch.tensor(freed, dtype=torch.int32).to(self.device)
                 for g in self.cache.kv_groups:
-                    kernels.blocks_release(gone, *g.tables.state(), status=g.tables.status)
+                    kernels.blocks_release(gone, *g.tables.state(), status=g.tables.status, refused=g.tables.refused)
                 self._mark_end()
         # decode steps are queued without a look at the kernels' status words (that would cost a
         # synchronisation per step); the end of a batch is where a wait that ran out is reported
         self._check_waits("close", "the tokens decoded for these sequences are not valid")
 
     def _check_waits(self, where: str, consequence: str) -> None:
-        """Raise if a bounded wait inside one of the tcgen05 kernels ran out since the last check.
+        """Raise if a bounded wait inside one of the tcgen05 kernels ran out since the last check, or if page tables that
+        live on the device refused a step.
         Reads and resets every status word, behind the last step: the words are read on the default stream,
         which waits for no other, so a step on one of those is waited for first."""
         launched = kernels.launch_count()
@@ -324,15 +325,19 @@ class Engine:
                       "grouped_tc": kernels.grouped_tc_status(reset=True),
                       "attn_kv8_tc": kernels.attention_kv8_tc_status(reset=True)}
         self._checked_at = launched
+        wrong = []
         for g in self.cache.kv_groups if self.cache.int8 else ():
-            status = int(g.tables.status)
-            if status:
-                raise StepError(f"{where}: the page tables on the device refused a step "
-                                f"({kernels.BLOCKS_STATUS.get(status, status)}); {consequence}")
+            refused = int(g.tables.refused)
+            if refused:
+                g.tables.refused.zero_()
+                self._mark_end()
+                wrong.append(f"the page tables on the device refused a step ({kernels.BLOCKS_STATUS.get(refused, refused)})")
         bad = {k: v for k, v in codes.items() if v}
         if bad:
-            raise StepError(f"{where}: a wait inside a tensor-core kernel ran out ({bad}), in this step or in a "
-                            f"decode step since the last check; {consequence}")
+            wrong.append(f"a wait inside a tensor-core kernel ran out ({bad})")
+        if wrong:
+            raise StepError(f"{where}: {' and '.join(dict.fromkeys(wrong))}, in this step or in a decode step since the last "
+                            f"check; {consequence}")
 
     def _mark_end(self) -> None:
         """What ``_check_waits`` waits for (an event: a caller's stream may be gone by then)."""

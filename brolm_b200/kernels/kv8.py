@@ -20,6 +20,8 @@ from __future__ import annotations
 import functools
 import struct
 from ctypes import c_char_p, c_int
+from typing import Optional
+
 import torch
 
 from . import KernelError, _check, _fn, _sms, device_sms, library_loaded, load_library
@@ -36,8 +38,8 @@ _CODES = {torch.float32: 0, torch.bfloat16: 1}
 # one struct, packed here as C lays it out (converting a pointer and 35 numbers one by one costs ctypes 3.4 us a call,
 # packing them 0.4 and passing the one pointer 0.3), and the checks of the arguments are one expression each; which of
 # them failed is found out only then.
-_EXTEND = struct.Struct("@14P8i")
-_RELEASE = struct.Struct("@7P4i")
+_EXTEND = struct.Struct("@15P8i")
+_RELEASE = struct.Struct("@8P4i")
 _WRITE = struct.Struct("@10P4q8i")
 _READ = struct.Struct("@11P4q10i")
 _ATTN = struct.Struct("@14P17i2f")
@@ -73,7 +75,7 @@ def _odd_ints(t: torch.Tensor, n: int) -> bool:
 def blocks_extend(slots: torch.Tensor, lengths: torch.Tensor, new: torch.Tensor, tables: torch.Tensor, held: torch.Tensor,
                   free: torch.Tensor, free_count: torch.Tensor, *, block: int, cu_q: torch.Tensor, kv_len: torch.Tensor,
                   positions: torch.Tensor, tok_seq: torch.Tensor, cache_rows: torch.Tensor, status: torch.Tensor,
-                  ring: int = 0, settle: bool = False) -> None:
+                  ring: int = 0, settle: bool = False, refused: Optional[torch.Tensor] = None) -> None:
     """A step's block tables and slot map, on the device.  All tensors are int32.
 
     Row i of the step goes on with slot ``slots[i]`` (-1: padding), which holds ``lengths[i]`` tokens, by ``new[i]``.  The
@@ -87,7 +89,9 @@ def blocks_extend(slots: torch.Tensor, lengths: torch.Tensor, new: torch.Tensor,
     positions, sums and lengths do so, since the host used to write them.  It costs an empty launch.
 
     A step that does not fit changes neither ``tables``, ``held`` nor the stack: its outputs read as padding and ``status``
-    holds a key of ``BLOCKS_STATUS``.  The same step again takes no more blocks.  Up to 4,096 rows and 65,536 slots."""
+    holds a key of ``BLOCKS_STATUS``.  ``refused``, one number where given, then gets that key, too, unless it holds one:
+    whoever queues steps without looking at each one's status finds the first refusal there, and sets it back to 0.  The
+    same step again takes no more blocks.  Up to 4,096 rows and 65,536 slots."""
     what = "blocks_extend"
     n, T = slots.numel(), positions.numel()
     if tables.dim() != 2:
@@ -96,32 +100,36 @@ def blocks_extend(slots: torch.Tensor, lengths: torch.Tensor, new: torch.Tensor,
     N = free.numel()
     if _odd_ints(slots, n) or _odd_ints(lengths, n) or _odd_ints(new, n) or _odd_ints(tables, S * W) or _odd_ints(held, S) or \
             _odd_ints(free, N) or _odd_ints(free_count, 1) or _odd_ints(cu_q, n + 1) or _odd_ints(kv_len, n) or \
-            _odd_ints(positions, T) or _odd_ints(tok_seq, T) or _odd_ints(cache_rows, T) or _odd_ints(status, 1):
+            _odd_ints(positions, T) or _odd_ints(tok_seq, T) or _odd_ints(cache_rows, T) or _odd_ints(status, 1) or \
+            (refused is not None and _odd_ints(refused, 1)):
         _refuse_ints(what, slots=(slots, n), lengths=(lengths, n), new=(new, n), tables=(tables, None), held=(held, S), free=(free, N),
                      free_count=(free_count, 1), cu_q=(cu_q, n + 1), kv_len=(kv_len, n), positions=(positions, T),
-                     tok_seq=(tok_seq, T), cache_rows=(cache_rows, T), status=(status, 1))
+                     tok_seq=(tok_seq, T), cache_rows=(cache_rows, T), status=(status, 1),
+                     refused=(status if refused is None else refused, 1))
     _call("blocks", "brolm_blocks_extend", _EXTEND.pack(
         slots.data_ptr(), lengths.data_ptr(), new.data_ptr(), tables.data_ptr(), held.data_ptr(), free.data_ptr(),
         free_count.data_ptr(), cu_q.data_ptr(), kv_len.data_ptr(), positions.data_ptr(), tok_seq.data_ptr(),
-        cache_rows.data_ptr(), status.data_ptr(), _raw_stream(_device()), n, S, W, N, block, ring, T, 1 if settle else 0), what)
+        cache_rows.data_ptr(), status.data_ptr(), 0 if refused is None else refused.data_ptr(), _raw_stream(_device()), n, S, W, N, block,
+        ring, T, 1 if settle else 0), what)
 
 
 def blocks_release(slots: torch.Tensor, tables: torch.Tensor, held: torch.Tensor, free: torch.Tensor, free_count: torch.Tensor, *,
-                   status: torch.Tensor) -> None:
+                   status: torch.Tensor, refused: Optional[torch.Tensor] = None) -> None:
     """Give the blocks of ``slots`` (-1: left out) back to the stack, the last row's last block first, so that releasing
-    the rows of an extend restores the order it found.  ``status`` as in ``blocks_extend``; a wrong slot changes nothing."""
+    the rows of an extend restores the order it found.  ``status`` and ``refused`` as in ``blocks_extend``; a wrong slot
+    changes nothing."""
     what = "blocks_release"
     if tables.dim() != 2:
         raise KernelError(f"{what}: tables must be [slots, width]")
     S, W = tables.shape
     n, N = slots.numel(), free.numel()
     if _odd_ints(slots, n) or _odd_ints(tables, S * W) or _odd_ints(held, S) or _odd_ints(free, N) or _odd_ints(free_count, 1) or \
-            _odd_ints(status, 1):
+            _odd_ints(status, 1) or (refused is not None and _odd_ints(refused, 1)):
         _refuse_ints(what, slots=(slots, n), tables=(tables, None), held=(held, S), free=(free, N), free_count=(free_count, 1),
-                     status=(status, 1))
+                     status=(status, 1), refused=(status if refused is None else refused, 1))
     _call("blocks", "brolm_blocks_release", _RELEASE.pack(
-        slots.data_ptr(), tables.data_ptr(), held.data_ptr(), free.data_ptr(), free_count.data_ptr(), status.data_ptr(), _raw_stream(_device()),
-        n, S, W, N), what)
+        slots.data_ptr(), tables.data_ptr(), held.data_ptr(), free.data_ptr(), free_count.data_ptr(), status.data_ptr(),
+        0 if refused is None else refused.data_ptr(), _raw_stream(_device()), n, S, W, N), what)
 
 
 def _cache(what: str, k_pages, v_pages, k_scale, v_scale) -> tuple:

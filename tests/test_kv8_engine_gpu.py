@@ -280,3 +280,34 @@ def test_decoding_against_the_stepwise_restatement_with_rounded_pages(name, tmp_
             assert off <= 0.01, (t, i, off)
         want = [o.push(row[t]) for o, row in zip(oracles, more)]
         got = e.step(s, [[row[t]] for row in more])
+
+
+@pytest.mark.parametrize("graphs", [True, False])
+def test_a_decode_step_that_the_tables_refuse_is_reported(graphs):
+    """The device has fewer free pages than the host counts: the step that needs one is refused, the next is fine again; who
+    closes the sequences (or begins another) learns of it, once, and the engine goes on."""
+    model = build("B", "float32")
+    e = bb.Engine(model, 64 * 12, max_slots=3, cache_dtype="int8", use_graphs=graphs)
+    prompts = random_prompts(model.config.vocab_size, [64, 64], seed=4)
+    for end in ("close", "step"):
+        s = e.open(2)
+        e.step(s, prompts)
+        counts = [g.tables.free_count.clone() for g in e.cache.kv_groups]
+        for g in e.cache.kv_groups:
+            g.tables.free_count.zero_()
+        e.step(s, [[1], [2]])                                    # the 65th token wants a page
+        for g, n in zip(e.cache.kv_groups, counts):
+            g.tables.free_count.copy_(n)
+        for t in range(3):
+            e.step(s, [[3], [4]])
+        if end == "step":
+            other = e.open(1)
+            with pytest.raises(bb.StepError, match="refused a step.*too few free blocks"):
+                e.step(other, [[5]])
+            e.step(other, [[5]])
+            e.close(other)
+            e.close(s)
+        else:
+            with pytest.raises(bb.StepError, match="refused a step.*too few free blocks"):
+                e.close(s)
+        check_tables(e)

@@ -839,3 +839,31 @@ def test_blocks_that_are_not_the_caches_are_passed_over(dtype, new, P, either):
                 ref = plain.attend(qj, keys[sees], values[sees], 0, len(sees) - 1, scale, 0.0, 0) if p >= 0 else torch.zeros(4, 64).double()
                 off = (out[i * new + j].cpu().double().view(4, 64) - ref).abs() - bound(dtype, ref, qj, keys, values, scale)
                 assert float(off.max()) <= 0.0, (width, i, j, float(off.max()))
+
+
+@pytest.mark.parametrize("tokens", [8, 40000])
+def test_the_first_refusal_is_kept_until_someone_has_seen_it(tokens):
+    """Behind one launch and behind the steps that all SMs share; calls that are fine in between, and the release."""
+    t = Tables(4, 3, 7, 32, 0, 0)
+    refused = ints([0])
+
+    def step(slots, lengths, new):
+        out = dict(cu_q=ints([7] * (len(slots) + 1)), kv_len=ints([7] * len(slots)), positions=ints([7] * tokens),
+                   tok_seq=ints([7] * tokens), cache_rows=ints([7] * tokens), status=ints([7]))
+        kernels.blocks_extend(ints(slots), ints(lengths), ints(new), *t.dev.values(), block=32, refused=refused, **out)
+        return int(out["status"]), int(refused)
+
+    def release(slots):
+        status = ints([7])
+        kernels.blocks_release(ints(slots), *t.dev.values(), status=status, refused=refused)
+        return int(status), int(refused)
+
+    assert step([0], [0], [5]) == (0, 0) and release([1]) == (0, 0)
+    assert step([0, 1], [5, 0], [1, 97 if tokens > 100 else 2 ** 20]) == (2 if tokens > 100 else 3, 2 if tokens > 100 else 3)
+    assert step([0], [5], [1])[0] == 0 and release([0, 9])[0] == 4 and release([0])[0] == 0
+    assert int(refused) == (2 if tokens > 100 else 3)
+    refused.zero_()
+    assert release([2, 2]) == (4, 4) and step([0], [0], [1]) == (0, 4)
+    for wrong in (ints([0, 0]), torch.zeros(1, device=DEV)):
+        with pytest.raises(kernels.KernelError, match="refused"):
+            kernels.blocks_release(ints([0]), *t.dev.values(), status=ints([0]), refused=wrong)
