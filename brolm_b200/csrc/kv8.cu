@@ -190,12 +190,13 @@ struct ReadArgs {
     void* out[2];
     long long token_stride[2], head_stride[2];
     const int32_t *cu_r, *kv_len, *slots, *tables;
-    int tokens, rows, n_kv, dim, block, n_blocks, n_slots, width, ring;
+    int tokens, rows, n_kv, dim, block, n_blocks, n_slots, width, ring, most;
 };
 
 constexpr int READ_TOKENS = 8;
 
-// The last n_i = cu_r[i + 1] - cu_r[i] tokens of row i, back to back; what the ring no longer holds reads as zero.  A thread
+// The last n_i = cu_r[i + 1] - cu_r[i] tokens of row i, back to back; what the ring no longer holds reads as zero, and so does
+// what comes before the last `most`.  A thread
 // makes sixteen numbers from sixteen bytes.  Bounded by the memory: 26,575 bfloat16 tokens of 8 heads of 256 (327 MB) in 57.1
 // us, 5.7 TB/s, 0.87 of a copy's rate.  Eight bytes a thread, so that its store fills half a sector by itself, took 97 us, and
 // two threads that swap halves, so that each store of theirs fills one, 69.
@@ -216,8 +217,8 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(ReadArgs a) {
                 else hi = mid;
             }
             const int len = a.kv_len[lo], s = a.slots[lo];
-            const int pos = len - (a.cu_r[lo + 1] - t);
-            if (pos >= 0 && s >= 0 && s < a.n_slots && (a.ring == 0 || pos / P + a.ring / P > (len - 1) / P)) {
+            const int back = a.cu_r[lo + 1] - t, pos = len - back;
+            if (pos >= 0 && back <= a.most && s >= 0 && s < a.n_slots && (a.ring == 0 || pos / P + a.ring / P > (len - 1) / P)) {
                 at = a.ring > 0 ? pos % a.ring : pos;
                 if (at / P < a.width) b = a.tables[(size_t)s * a.width + at / P];
                 at %= P;
@@ -283,7 +284,7 @@ struct ReadCall {
     void *k, *v;
     cudaStream_t stream;
     long long k_token, v_token, k_head, v_head;
-    int dtype, tokens, rows, n_kv, dim, block, n_blocks, n_slots, width, ring;
+    int dtype, tokens, rows, n_kv, dim, block, n_blocks, n_slots, width, ring, max_q_len;
 };
 
 BROLM_API int brolm_kv8_write(const WriteCall* c) {
@@ -316,7 +317,7 @@ BROLM_API int brolm_kv8_read(const ReadCall* c) {
     ReadArgs a{{(const int8_t*)c->k_pages, (const int8_t*)c->v_pages}, {(const float*)c->k_scale, (const float*)c->v_scale}, {c->k, c->v},
                {c->k_token, c->v_token}, {c->k_head, c->v_head}, (const int32_t*)c->cu_r, (const int32_t*)c->kv_len,
                (const int32_t*)c->slots, (const int32_t*)c->tables, c->tokens, c->rows, c->n_kv, c->dim, c->block, c->n_blocks,
-               c->n_slots, c->width, c->ring};
+               c->n_slots, c->width, c->ring, c->max_q_len};
     const dim3 grid((c->tokens + READ_TOKENS - 1) / READ_TOKENS, 2);
     if (c->dtype == BROLM_F32) return launch_pdl(kv8_read_kernel<float>, grid, dim3(256), 0, c->stream, a);
     return launch_pdl(kv8_read_kernel<bf16>, grid, dim3(256), 0, c->stream, a);

@@ -41,7 +41,7 @@ _CODES = {torch.float32: 0, torch.bfloat16: 1}
 _EXTEND = struct.Struct("@15P8i")
 _RELEASE = struct.Struct("@8P4i")
 _WRITE = struct.Struct("@10P4q8i")
-_READ = struct.Struct("@11P4q10i")
+_READ = struct.Struct("@11P4q11i")
 _ATTN = struct.Struct("@14P17i2f")
 _ATTN_TC = struct.Struct("@13P16i2f")
 _functions: dict = {}
@@ -184,9 +184,10 @@ def kv8_write(k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, positions: t
 def kv8_read(cu_q: torch.Tensor, kv_len: torch.Tensor, slots: torch.Tensor, tables: torch.Tensor, k_pages: torch.Tensor,
              v_pages: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, k_out: torch.Tensor, v_out: torch.Tensor, *,
              max_q_len: int, ring: int = 0) -> None:
-    """The newest ``cu_q[i + 1] - cu_q[i]`` tokens of every row (at most ``max_q_len`` of each) as numbers: ``k_out``,
-    ``v_out`` [tokens, kv heads, head_dim], float32 or bfloat16 (both hold them exactly).  Tokens before a sequence's first,
-    or that the ring no longer holds, read as zero."""
+    """The newest ``cu_q[i + 1] - cu_q[i]`` tokens of every row as numbers: ``k_out``, ``v_out`` [tokens, kv heads,
+    head_dim], float32 or bfloat16 (both hold them exactly), on 16 bytes, with strides between tokens and heads that are
+    multiples of 16 bytes.  Tokens before a sequence's first, that the ring no longer holds, or that come before the row's
+    newest ``max_q_len``, read as zero."""
     what = "kv8_read"
     n_blocks, n_kv, block, dim = _cache(what, k_pages, v_pages, k_scale, v_scale)
     T, code, k0, k1, v0, v1 = _two(what, "k_out and v_out", k_out, v_out, n_kv, dim)
@@ -201,7 +202,7 @@ def kv8_read(cu_q: torch.Tensor, kv_len: torch.Tensor, slots: torch.Tensor, tabl
     _call("kv8", "brolm_kv8_read", _READ.pack(
         cu_q.data_ptr(), kv_len.data_ptr(), slots.data_ptr(), tables.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
         k_scale.data_ptr(), v_scale.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), _raw_stream(_device()), k0, v0, k1, v1, code, T, rows, n_kv,
-        dim, block, n_blocks, S, W, ring), what)
+        dim, block, n_blocks, S, W, ring, max_q_len), what)
 
 
 KV8_TILE, KV8_WARPS, KV8_CLUSTER = 32, 4, 8       # keys of a tile, warps of a block, blocks that join their results themselves

@@ -867,3 +867,17 @@ def test_the_first_refusal_is_kept_until_someone_has_seen_it(tokens):
     for wrong in (ints([0, 0]), torch.zeros(1, device=DEV)):
         with pytest.raises(kernels.KernelError, match="refused"):
             kernels.blocks_release(ints([0]), *t.dev.values(), status=ints([0]), refused=wrong)
+
+
+def test_read_gives_no_more_of_a_row_than_it_is_told():
+    c = Cached(2, 5, 2, 32, 48, seed=5)
+    g = torch.Generator().manual_seed(1)
+    c.write([0, 1], [130, 90], rows_of(220, 2, 48, torch.float32, g), rows_of(220, 2, 48, torch.float32, g))
+    for most in (1, 37, 90, 130):
+        k, v = torch.full((2, 220, 2, 48), 5.0, device=DEV)
+        kernels.kv8_read(ints([0, 130, 220]), ints([130, 90]), ints([0, 1]), c.tables, *c.dev, k, v, max_q_len=most)
+        for which, got in ((0, k), (1, v)):
+            for i, (at, n) in enumerate(((0, 130), (130, 90))):
+                want = c.values(which, i)[1]
+                want[:max(0, n - most)] = 0.0
+                assert same(got[at:at + n].cpu().double(), want)
