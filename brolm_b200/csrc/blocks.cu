@@ -207,7 +207,11 @@ __global__ void __launch_bounds__(THREADS) blocks_extend_kernel(ExtendArgs a) {
         }
 #pragma unroll
         for (int j = 0; j < EACH; ++j)
-            if (where[j]) row[j] += *where[j] * a.block;
+            if (where[j]) {                     // (an id that no cache of 31 bits of places has gives no place)
+                const int id = *where[j];
+                const long long at = (long long)id * a.block + row[j];
+                row[j] = id >= 0 && at <= 0x7fffffffll ? (int)at : -1;
+            }
 #pragma unroll
         for (int j = 0; j < EACH; ++j) {
             const int t = base + 32 * j + lane;

@@ -881,3 +881,17 @@ def test_read_gives_no_more_of_a_row_than_it_is_told():
                 want = c.values(which, i)[1]
                 want[:max(0, n - most)] = 0.0
                 assert same(got[at:at + n].cpu().double(), want)
+
+
+@pytest.mark.parametrize("tokens", [200, 40000])
+def test_block_ids_that_no_cache_has_give_no_places(tokens):
+    """Ids whose places pass 31 bits, or come before the first, must not come back as another block's."""
+    ids = [5, 2 ** 27, -1, -2 ** 27, 2 ** 31 - 1, 2 ** 26 - 1, -2 ** 31]
+    free = ints(reversed(ids))
+    state = dict(tables=torch.zeros((2, 8), dtype=I32, device=DEV), held=ints([0, 0]), free=free, free_count=ints([len(ids)]))
+    for before, n in ((0, 200), (200, 24)):                       # taken from the stack, then found in the table
+        out = dict(cu_q=ints([7, 7]), kv_len=ints([7]), positions=ints([7] * tokens), tok_seq=ints([7] * tokens),
+                   cache_rows=ints([7] * tokens), status=ints([7]))
+        kernels.blocks_extend(ints([1]), ints([before]), ints([n]), *state.values(), block=32, **out)
+        want = [ids[p // 32] * 32 + p % 32 if ids[p // 32] in (5, 2 ** 26 - 1) else -1 for p in range(before, before + n)]
+        assert int(out["status"]) == 0 and out["cache_rows"][:n].tolist() == want
