@@ -168,6 +168,8 @@ class KVGroup:
 
 class DeviceTables:
     """The page tables of a group on the device: a row of page ids and a count per slot, a stack of free pages."""
+    # what kernels.blocks_extend and blocks_release take at most
+    MAX_ROWS, MAX_SLOTS = 4096, 65536
 
     def __init__(self, num_pages: int, num_slots: int, width: int, device):
         new = lambda *shape: torch.zeros(shape, dtype=torch.int32, device=device)
@@ -247,6 +249,8 @@ class Cache:
             raise CacheError("max_piece must be at least 1")
         self.dtype, self.device = dtype, torch.device(device)
         self.int8, self.max_piece = bool(int8), int(max_piece)
+        if self.int8 and self.max_slots > DeviceTables.MAX_SLOTS:
+            raise CacheError(f"a cache in 8 bits has at most {DeviceTables.MAX_SLOTS} slots, not {self.max_slots}")
         self.max_positions = min(max_positions or self.max_tokens, self.max_tokens)
         self.slots = SlotTable(self.max_slots)
         self.padding_slot = self.max_slots        # the slot number of padding rows: a spare row of every state group

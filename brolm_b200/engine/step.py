@@ -34,6 +34,7 @@ import torch
 
 from .. import kernels
 from ..cache import Cache, CacheError
+from ..cache.cache import DeviceTables
 from . import debug
 from .context import StepContext
 from .model import DecoderModel
@@ -302,7 +303,8 @@ class Engine:
                 self._follow()
                 gone = torch.tensor(freed, dtype=torch.int32).to(self.device)
                 for g in self.cache.kv_groups:
-                    kernels.blocks_release(gone, *g.tables.state(), status=g.tables.status, refused=g.tables.refused)
+                    for some in gone.split(g.tables.MAX_ROWS):
+                        kernels.blocks_release(some, *g.tables.state(), status=g.tables.status, refused=g.tables.refused)
                 self._mark_end()
         # decode steps are queued without a look at the kernels' status words (that would cost a
         # synchronisation per step); the end of a batch is where a wait that ran out is reported
@@ -444,6 +446,8 @@ class Engine:
         if len(set(slots)) != B:
             raise StepError("step: a slot is named twice")
         cache = self.cache
+        if cache.int8 and B > DeviceTables.MAX_ROWS:
+            raise StepError(f"step: {B} sequences; with a cache in 8 bits a step has at most {DeviceTables.MAX_ROWS}")
         old = [cache.length(s) for s in slots]
         n_new = [len(t) for t in tokens]         # (lists, NumPy arrays and host tensors all have a length)
         if min(n_new) <= 0:

@@ -58,3 +58,24 @@ def test_models_and_arguments_that_are_refused():
     with pytest.raises(ValueError, match="plain attention"):
         other.new_cache(640, cache_dtype="int8")
 
+
+
+def test_limits_of_the_tables_are_said_before_a_step_is_begun():
+    import os
+    import re
+    from brolm_b200.cache.cache import DeviceTables
+    with open(os.path.join(os.path.dirname(__file__), "..", "brolm_b200", "csrc", "blocks.cu")) as fh:
+        source = fh.read()
+    assert [int(re.search(rf"MAX_{n} = (\d+)", source).group(1)) for n in ("ROWS", "SLOTS")] == [DeviceTables.MAX_ROWS, DeviceTables.MAX_SLOTS]
+    spec = [KVSpec(1, 16, 32)]
+    with pytest.raises(CacheError, match="65536 slots"):
+        Cache(spec, 64, torch.bfloat16, "cpu", max_slots=65537, int8=True)
+    assert Cache(spec, 64, torch.bfloat16, "cpu", max_slots=65537).max_slots == 65537
+    assert Cache(spec, 64, torch.bfloat16, "cpu", max_slots=65536, int8=True).max_slots == 65536
+    model = bb.Model(bb.Gemma2Config(**TINY["A"][0]), dtype="float32", device="cpu")
+    e = bb.Engine(model, 64 * 4200, max_slots=4200, max_seq_len=64, cache_dtype="int8")
+    slots = e.open(4097)
+    free = [g.pool.free_pages for g in e.cache.kv_groups]
+    with pytest.raises(bb.StepError, match="at most 4096"):
+        e.step(slots, [[1]] * 4097)
+    assert [g.pool.free_pages for g in e.cache.kv_groups] == free

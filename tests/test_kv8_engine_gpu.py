@@ -311,3 +311,16 @@ def test_a_decode_step_that_the_tables_refuse_is_reported(graphs):
             with pytest.raises(bb.StepError, match="refused a step.*too few free blocks"):
                 e.close(s)
         check_tables(e)
+
+
+def test_more_slots_than_a_step_has_rows_are_closed_at_once():
+    model = build("A", "float32")
+    e = bb.Engine(model, 64 * 4300, max_slots=4300, max_seq_len=64, cache_dtype="int8")
+    s = e.open(4200)
+    for at, n in ((0, 3000), (3000, 1100)):
+        e.step(s[at:at + n], [[1 + i % 7] for i in range(n)])
+    e.step(s[10:4100], [[2]] * 4090)
+    check_tables(e)
+    e.close(s)
+    check_tables(e)
+    assert e.cache.live_slots == 0
