@@ -6,8 +6,12 @@ keys and values in the cache, the rows whose logits are wanted, the slots.  A
 wrong one would read or write someone else's pages, or fault the GPU.  With
 ``BROLM_DEBUG=1`` in the environment every step's arrays are checked against
 the cache's own bookkeeping before they are copied to the device, and a step
-that fails raises ``StepError`` without launching anything.  The checks cost a
-few passes over arrays of the step's size; they are off by default.
+that fails raises ``StepError`` without launching anything.  With a cache in 8
+bits the device writes most of them itself (its kernels follow no index out of
+the cache): what it made of the host's lengths is read back and compared with
+the host's counts, before the model runs or, of a captured step, behind it.
+The checks cost a few passes over arrays of the step's size, and reading back a
+synchronisation; they are off by default.
 """
 from __future__ import annotations
 
@@ -101,3 +105,45 @@ def check_step(cache, mode: str, vocab: int, tokens: Optional[np.ndarray], slots
             r = int(tok_seq[t])
             if not grp.ring or int(positions[t]) + grp.ring >= int(kv_len[r]) or int(positions[t]) < grp.head:
                 fail(f"group {g}, token {t}: not kept, although nothing of this step takes its place")
+
+
+def check_tables(cache, slots: Sequence[int], old: Sequence[int], new_len: Sequence[int], kv_len: np.ndarray, positions: np.ndarray,
+                 cache_rows: Sequence[np.ndarray]) -> None:
+    """Raise ``StepCheckError`` where what the device made of a step (a cache in 8 bits) is not what the host counts: the
+    status, the pages of the step's ``slots``, no page twice, and the lengths, positions and places of its tokens; rows and
+    tokens beyond them are padding."""
+    from .. import kernels
+
+    def fail(what: str):
+        raise StepCheckError(f"debug: {what}")
+
+    def padded(values, n):
+        return np.concatenate([np.asarray(values, dtype=np.int64), np.full(n - len(values), -1, dtype=np.int64)])
+
+    rows, tokens = len(slots), sum(new_len) - sum(old)
+    for gi, g in enumerate(cache.kv_groups):
+        status = int(g.tables.status)
+        if status:
+            fail(f"group {gi}: {kernels.BLOCKS_STATUS.get(status, status)}")
+    if list(kv_len[:rows]) != list(new_len) or np.any(kv_len[rows:] != 0):
+        fail(f"the device has lengths {kv_len.tolist()}, the host {list(new_len)}")
+    want = [np.arange(a, b) for a, b in zip(old, new_len)]
+    if np.any(positions != padded(np.concatenate(want), len(positions))):
+        fail("the device's positions are not the host's")
+    for gi, g in enumerate(cache.kv_groups):
+        t = g.tables
+        held, count, tables = t.held.cpu().numpy(), int(t.free_count), t.tables.cpu().numpy()
+        for s, n in zip(slots, new_len):
+            # (a step that failed behind the host's count leaves it pages that the device has not handed out yet)
+            if not g.pages_for(n) <= held[s] <= len(g.pages[s]):
+                fail(f"group {gi}: slot {s} holds {held[s]} pages on the device, {len(g.pages[s])} on the host")
+        out = np.concatenate([tables[s, :n] for s, n in enumerate(held)] + [t.free.cpu().numpy()[:max(0, count)]])
+        if len(out) != g.pool.num_pages or np.any(np.sort(out) != np.arange(g.pool.num_pages)):
+            fail(f"group {gi}: the pages held and the {count} free ones are not the pool of {g.pool.num_pages}, each once")
+        places = []
+        for s, pos, n in zip(slots, want, new_len):
+            at = g.place(pos)
+            kept = pos // g.page_size + g.ring // g.page_size > (n - 1) // g.page_size if g.ring else np.ones(len(pos), dtype=bool)
+            places.append(np.where(kept, tables[s, at // g.page_size].astype(np.int64) * g.page_size + at % g.page_size, -1))
+        if np.any(cache_rows[gi] != padded(np.concatenate(places), len(positions))):
+            fail(f"group {gi}: the device's places of the step's {tokens} tokens are not where their positions live")

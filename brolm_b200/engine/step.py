@@ -67,6 +67,16 @@ def _checked(*args) -> None:
         raise StepError(str(e)) from None
 
 
+def _checked_tables(cache: Cache, plan: "_Plan", ctx: StepContext) -> None:
+    """What the device made of a step against the cache's bookkeeping (``BROLM_DEBUG=1``, a cache in 8 bits)."""
+    host = lambda t: t.cpu().numpy()
+    try:
+        debug.check_tables(cache, plan.slots, plan.old, plan.new_len, host(ctx.kv_len), host(ctx.positions),
+                           [host(r) for r in ctx.cache_rows])
+    except debug.StepCheckError as e:
+        raise StepError(str(e)) from None
+
+
 def _ragged(lengths: Sequence[int]) -> bool:
     """Whether the longest sequence of a decode step is well beyond the mean (by a quarter)."""
     return len(lengths) > 1 and max(lengths) * len(lengths) > 1.25 * sum(lengths)
@@ -212,7 +222,10 @@ class _DecodeGraph:
             hv[R:R + B] = plan.old
             hv[4 * R:5 * R] = -1
             hv[4 * R:4 * R + B] = plan.slots
-            return self._replay(B, ids, pick)
+            logits = self._replay(B, ids, pick)
+            if debug.ENABLED:
+                _checked_tables(cache, plan, self.ctx)
+            return logits
         off = 4 * R
         for g, w in enumerate(self.widths):
             # the page tables change only when a sequence begins a page or the batch changes
@@ -527,15 +540,13 @@ class Engine:
         positions, tok_seq = cut(2 * B + 1, T), cut(2 * B + 1 + T, T)
         cache_rows = [cut(2 * B + 1 + (2 + g) * T, T) for g in range(G)]
         _extend(cache, slots, old, new, cu_q, kv_len, positions, tok_seq, cache_rows, made[2 * B + 1 + (2 + G) * T:])
-        if debug.ENABLED:
-            for g in cache.kv_groups:
-                if int(g.tables.status):
-                    raise StepError(f"debug: {kernels.BLOCKS_STATUS.get(int(g.tables.status))}")
         ctx = StepContext(mode=plan.mode, dtype=self.model.dtype, device=self.device, cache=cache, batch=B, n_tokens=T,
                           slots=plan.slots, positions=positions, tok_seq=tok_seq, cu_q=cu_q, kv_len=kv_len, slots_dev=slots,
                           max_q_len=int(max(plan.n_new)), page_tables=[g.tables.tables for g in cache.kv_groups],
                           cache_rows=cache_rows, host_lengths=plan.new_len,
                           ragged=plan.mode == "decode" and _ragged(plan.new_len))
+        if debug.ENABLED:
+            _checked_tables(cache, plan, ctx)
         return ctx, tokens, rows
 
     def _send(self, parts: list) -> list:

@@ -79,3 +79,57 @@ def test_limits_of_the_tables_are_said_before_a_step_is_begun():
     with pytest.raises(bb.StepError, match="at most 4096"):
         e.step(slots, [[1]] * 4097)
     assert [g.pool.free_pages for g in e.cache.kv_groups] == free
+
+
+@pytest.mark.parametrize("change,says", [
+    (None, None), ("status", "too few free blocks"), ("held", "holds 3 pages on the device, 2 on the host"), ("count", "each once"),
+    ("twice", "each once"), ("kv_len", "lengths"), ("positions", "positions"), ("padding", "positions"), ("rows", "group 1.*places"),
+    ("spare", "group 0.*places")])
+def test_what_the_device_made_of_a_step_against_the_hosts_counts(change, says):
+    """The debug checks of such a cache, on tables that the plain restatement fills."""
+    import numpy as np
+    from brolm_b200.engine import debug
+    from tests.plain import kv8_plain as plain
+    c = Cache([KVSpec(1, 16, None), KVSpec(1, 16, 100)], 64 * 20, torch.bfloat16, "cpu", max_slots=4, int8=True, max_positions=640)
+    slots = [c.alloc_slot() for _ in range(3)][::2]
+
+    def step(old, new, tokens):
+        c.reserve(dict(zip(slots, [a + n for a, n in zip(old, new)])))
+        made = []
+        for g in c.kv_groups:
+            t = g.tables
+            status, _, kv_len, pos, _, rows, tables, held, count = plain.extend(
+                slots + [-1], old + [0], new + [1], t.tables.tolist(), t.held.tolist(), t.free.tolist(), int(t.free_count), 64, g.ring or 0, tokens)
+            for x, y in ((t.tables, tables), (t.held, held), (t.free_count, [count]), (t.status, [status])):
+                x.copy_(torch.tensor(y))
+            made.append((np.array(kv_len), np.array(pos), np.array(rows)))
+        return [made[0][0], made[0][1], [m[2] for m in made]]
+
+    new_len = [300, 66]
+    debug.check_tables(c, slots, [0, 0], new_len, *step([0, 0], new_len, 380))
+    kv_len, positions, rows = step(new_len, [1, 1], 5)
+    t = c.kv_groups[1].tables
+    if change == "status":
+        t.status.fill_(1)
+    elif change == "held":
+        t.held[slots[1]] += 1
+    elif change == "count":
+        t.free_count -= 1
+    elif change == "twice":
+        t.tables[slots[1], 0] = t.tables[slots[0], 0]
+    elif change == "kv_len":
+        kv_len[1] += 1
+    elif change == "positions":
+        positions[0] += 1
+    elif change == "padding":
+        positions[2] = 0
+    elif change == "rows":
+        rows[1][1] += 1
+    elif change == "spare":
+        rows[0][4] = 7
+    args = (c, slots, new_len, [n + 1 for n in new_len], kv_len, positions, rows)
+    if change is None:
+        debug.check_tables(*args)
+    else:
+        with pytest.raises(debug.StepCheckError, match=says):
+            debug.check_tables(*args)

@@ -324,3 +324,33 @@ def test_more_slots_than_a_step_has_rows_are_closed_at_once():
     e.close(s)
     check_tables(e)
     assert e.cache.live_slots == 0
+
+
+@pytest.mark.parametrize("graphs", [True, False])
+def test_steps_pass_the_debug_checks_and_tables_that_differ_do_not(graphs, monkeypatch):
+    from brolm_b200.engine import debug
+    monkeypatch.setattr(debug, "ENABLED", True)
+    model = build("B", "float32")
+    e = bb.Engine(model, 64 * 20, max_slots=3, cache_dtype="int8", max_piece=60, use_graphs=graphs)
+    s = e.open(3)
+    prompts = random_prompts(model.config.vocab_size, [60, 130, 7], seed=4)
+    e.step(s, prompts)
+    e.step(s[:2], [[1] * 30, [2] * 11])
+    for t in range(70):
+        e.step(s, [[3], [4], [5]])
+    at = [g.ring for g in e.cache.kv_groups].index(None)            # (a ring's pages are all held by now)
+    tables = e.cache.kv_groups[at].tables
+    before = tables.free_count.clone()
+    tables.free_count -= 1                     # (a page that nobody has any more)
+    for tokens in ([[1], [2], [3]], [[1, 2], [3], [4]]):
+        with pytest.raises(bb.StepError, match=f"debug: group {at}.*each once"):
+            e.step(s, tokens)
+    tables.free_count.zero_()
+    with pytest.raises(bb.StepError, match=f"debug: group {at}: too few free blocks"):
+        e.step(s, [[1] * 60, [2] * 50, [3]])
+    tables.free_count.copy_(before)
+    with pytest.raises(bb.StepError, match="refused a step"):       # (that step, told once more where the waits are looked at)
+        e.step(s, [[1] * 3, [2], [3]])
+    e.step(s, [[1], [2], [3]])
+    e.close(s)
+    check_tables(e)
