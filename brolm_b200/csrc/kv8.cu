@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(ReadArgs a) {
         float s = 0.0f;
         if (b >= 0 && b < a.n_blocks) {
             const size_t bh = (size_t)b * a.n_kv + h;
-            w = __ldg(reinterpret_cast<const int4*>(a.pages[which] + (bh * P + place_s[j]) * a.dim) + c);
+            w = reinterpret_cast<const int4*>(a.pages[which] + (bh * P + place_s[j]) * a.dim)[c];
             s = a.scales[which][bh];
         }
         const int8_t* q = reinterpret_cast<const int8_t*>(&w);

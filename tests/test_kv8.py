@@ -141,3 +141,14 @@ def test_calls_are_counted_as_launches(monkeypatch):
     with pytest.raises(kernels.KernelError, match="a call"):
         kv8._call("kv8", "bad", b"", "a call")
     assert kernels.launch_count() == before + 1
+
+
+def test_what_an_earlier_launch_may_still_be_writing_is_not_read_as_constant():
+    """The kernels are let in before the launch ahead of them has ended, so what that one writes is not constant for as long
+    as they are resident: no load of theirs may go past the ordinary caches' order, by intrinsic, by PTX or by __restrict__."""
+    import os
+    import re
+    folder = os.path.join(os.path.dirname(__file__), "..", "brolm_b200", "csrc")
+    for name in ("blocks.cu", "kv8.cu", "attn_kv8.cu", "attn_kv8_tc.cu", "attn_kv8_join.cuh"):
+        with open(os.path.join(folder, name)) as fh:
+            assert not re.search(r"__ldg\b|ld\.global\S*\.nc|__restrict__", fh.read()), name
