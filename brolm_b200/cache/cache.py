@@ -166,6 +166,10 @@ class KVGroup:
         return pos if pos < self.head else self.head + (pos - self.head) % self.ring
 
 
+# the most tokens of a page in 8 bits (what the kernels take)
+INT8_MAX_PAGE = 256
+
+
 class DeviceTables:
     """The page tables of a group on the device: a row of page ids and a count per slot, a stack of free pages."""
     # what kernels.blocks_extend and blocks_release take at most
@@ -251,6 +255,8 @@ class Cache:
         self.int8, self.max_piece = bool(int8), int(max_piece)
         if self.int8 and self.max_slots > DeviceTables.MAX_SLOTS:
             raise CacheError(f"a cache in 8 bits has at most {DeviceTables.MAX_SLOTS} slots, not {self.max_slots}")
+        if self.int8 and page_size > INT8_MAX_PAGE:
+            raise CacheError(f"a page of a cache in 8 bits has at most {INT8_MAX_PAGE} tokens, not {page_size}")
         self.max_positions = min(max_positions or self.max_tokens, self.max_tokens)
         self.slots = SlotTable(self.max_slots)
         self.padding_slot = self.max_slots        # the slot number of padding rows: a spare row of every state group

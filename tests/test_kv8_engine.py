@@ -133,3 +133,11 @@ def test_what_the_device_made_of_a_step_against_the_hosts_counts(change, says):
     else:
         with pytest.raises(debug.StepCheckError, match=says):
             debug.check_tables(*args)
+
+
+def test_pages_that_the_kernels_do_not_take_are_refused_where_the_cache_is_made():
+    spec = [KVSpec(1, 16, None)]
+    with pytest.raises(CacheError, match="256 tokens"):
+        Cache(spec, 640, torch.bfloat16, "cpu", page_size=320, int8=True)
+    assert Cache(spec, 640, torch.bfloat16, "cpu", page_size=256, int8=True).page_size == 256
+    assert Cache(spec, 640, torch.bfloat16, "cpu", page_size=320).page_size == 320
