@@ -489,9 +489,11 @@ __device__ __forceinline__ void merge(const AttnArgs& a, const Item& it, const f
 //     p     = sum_i e_i 256^-i,      two unsigned digits (bfloat16: 16 bits of the tile's largest weight, four rows an
 //                                    instruction) or four (float32: 31 bits, two rows).
 //
-// A thread has two neighbouring digits' sums, joins them as whole numbers (below 2^31: 127 * 255 * 256 * 33 in both
-// products) and then in floats.  The keys are read as the instruction wants them; of the values, four keys' bytes of an
-// entry are gathered into a word by eight byte permutations for sixteen bytes.
+// A thread has two neighbouring digits' sums, joins them as whole numbers and then in floats.  Both stay below 2^31: scores are
+// sums over a head's entries of products up to 127 * 128, the higher digit's times 256 (127 * 128 * 256 * 257 = 1.07e9 at 256
+// entries), results are sums over a tile's 32 keys of products up to 127 * 255 (127 * 255 * 32 * 257 = 2.7e8).  The keys
+// are read as the instruction wants them; of the values, four keys' bytes of an entry are gathered into a word by eight byte
+// permutations for sixteen bytes.
 //
 // 8 sequences of 8,192 keys, 4 kv heads of 256, two query heads each, bfloat16: 29.2 us, 4.6 TB/s, with 28 % of the issue
 // slots and 7 % of the tensor pipe in use (f16 products: 30.2, and for 16 sequences of unequal lengths under a window 45.6
@@ -525,6 +527,7 @@ __global__ void __launch_bounds__(THREADS, 2) attn_kv8_few_kernel(AttnArgs a) {
     using SH = FewShape<T, DP, ROWS>;
     constexpr int SEGS = SH::SEGS, QT = SH::QT, PT = SH::PT, PER_WARP = (ROWS + WARPS - 1) / WARPS;
     constexpr bool EXACT = sizeof(T) == 4;
+    static_assert(127ll * 128 * DP * 257 < 1ll << 31 && 127ll * 255 * KT * 257 < 1ll << 31, "joined digits' sums");
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ float q_scale[ROWS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, t4 = lane & 3;

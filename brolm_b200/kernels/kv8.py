@@ -322,7 +322,8 @@ def attention_kv8(q: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, kv_len
     """The newest ``cu_q[i + 1] - cu_q[i]`` tokens of every row i against the ``kv_len[i]`` that its slot holds, themselves
     among them (``kv8_write`` comes first).  ``q`` and ``out`` [tokens, n_kv * group * head_dim], float32 or bfloat16, query
     head h reads kv head h // group; ``scale``, ``cap`` (<= 0: none) and ``window`` (0: all keys) as everywhere.  A token
-    that sees no key (padding) gets zeros.  ``max_q_len`` and ``max_kv_len`` bound the rows' new tokens and lengths."""
+    that sees no key (a padding row's) gets zeros; places of ``out`` that are no row's (all of them, behind a step that the
+    tables refused) stay as they are.  ``max_q_len`` and ``max_kv_len`` bound the rows' new tokens and lengths."""
     what = "attention_kv8"
     n_blocks, G, block, dim = _cache(what, k_pages, v_pages, k_scale, v_scale)
     if G != n_kv or dim != head_dim:
