@@ -803,10 +803,12 @@ __global__ void __launch_bounds__(THREADS, 2) attn_kv8_few_kernel(AttnArgs a) {
 // so that it is held by one f16 a number (bfloat16 queries, exactly but for numbers 2^-38 of the row's largest) or two
 // (float32: 22 bits or more).  Weights are one f16 (bfloat16) or two (float32).
 //
-// What bounds it is a warp's own chain, 1.8 us a tile of 32 keys of 128 entries in float32 (128 products, as many bytes to
-// turn, two exponentials and a tanh a score) with one or two warps a scheduler: 6 sequences of 13 to 4,001 keys with five
-// tokens each, 4 kv heads of 128, four query heads each, float32, take 21.7 us (19.5 in bfloat16, 21.2 without the cap, as
-// 5 x 1 shares of the longest 26.5).
+// What bounds it is a warp's own chain, 1.9 us a tile of 32 keys of 128 entries in float32 (128 products, as many bytes to
+// turn, two exponentials and a tanh a score) where a scheduler has one warp, 3.1 where it has two, and what lies around it:
+// with one tile a warp or less a launch takes 8.9 us, of which the chain is 1.9.  6 sequences of 13 to 4,001 keys with five
+// tokens each, 4 kv heads of 128, four query heads each, float32, take 21.7 us: dealing and joining put 2.6 on the 8.9, two
+// blocks an SM and up to 11 parts a row some 4, and the longest warps' three tiles are two more than one (19.5 us in bfloat16,
+// 21.0 without the cap, 22.1 with scores beyond 0.4 of it; as 5 x 1 shares of the longest 26.2, as 1 x 1 66).
 
 template <typename T, int DP>
 struct Shape {

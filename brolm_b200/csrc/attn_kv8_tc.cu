@@ -33,11 +33,14 @@
 // a sum of their own, relative to the largest of their own z, and the two are added up at the end.  A query row is scaled by a power
 // of two to below 2^14 and held in f16, exactly but for numbers 2^-38 of the row's largest.
 //
-// What bounds it: of a tile of 128 keys and 256 entries, about 5,000 cycles (2,048 tokens on 14,336 keys, 8 kv heads of 256,
-// two query heads each: 562 to 577 us, 775 to 795 TFLOP/s of 1,700), the tensor core takes 2,050, shared memory 3,500 (bytes in, f16 out, f16
-// to the tensor core: 448 KB), the softmax of a row's scores and then of its weights, which wait for each other and for the
-// products, 1,700 to 2,000 (fma units) and 1,200 to 1,400 (special function units), and the instructions of all roles 57 % of
-// the issue slots; the tensor core now waits for what is turned into f16 (1,400 cycles a tile for keys, 1,300 for values).
+// What bounds it: of a tile of 128 keys and 256 entries, about 5,300 cycles, a block's start and end in them (2,048 tokens on
+// 14,336 keys, 8 kv heads of 256, two query heads each: 569 to 581 us, 770 to 786 TFLOP/s of 1,700), the tensor core takes
+// 2,050, shared memory 3,500 (bytes in, f16 out, f16 to the tensor core: 448 KB), the softmax of a row's scores and then of its
+// weights, which wait for each other and for the products, 1,700 to 2,000 (fma units) and 1,200 to 1,400 (special function
+// units), and the instructions of all roles 61 % of the issue slots; the tensor core waits for what is turned into f16 (1,400
+// cycles a tile for keys, 1,300 for values).  That is with scores below 0.4 of the cap.  A tile of which a warp finds one beyond
+// that takes its scores twice, the second time by exponentials: 775 us with queries of 20 times the size (without a cap 504).
+// The sum of far values' weights put 1.5 % on heads of 256 and nothing on smaller ones (561.7 us without it, and wrong).
 // Four groups of two converting warps instead of two of four were slower (609 us).  To put scores and weights side by side
 // was slower too, both as two sets of softmax warps that take turns on tiles and as rounds that take the next tile's scores
 // while they make this one's weights (681 us; with three score buffers for heads of 128 entries 144 us for 158, which is

@@ -278,7 +278,9 @@ def kv8_tc_spans(tokens: int, batch: int, n_kv: int, group: int, max_q_len: int,
     In tiles of 128 keys (about 2.6 us each at 256 entries, counted as 3): a block begins and ends in three, and joining costs another three and
     what the parts take to memory and back.  Where the last round would be far from full, its tiles alone are shared
     (on 14,336 keys, 8 kv heads of 256, two query heads each, us with a block for a tile / four / the last round's
-    shared: 1,280 tokens, 160 tiles on 148 SMs, 560 / 449 / 343; 1,700, 216 tiles, 564 / 553 / 459; 2,048, 256, 560 / 638 / 573)."""
+    shared as the rule has it: 1,280 tokens, 160 tiles on 148 SMs, 570 / 453 / 351 by 12; 1,700, 216 tiles, 571 / 555 / 470 by 2;
+    2,048, 256 tiles, 569 / 655 / 580 by 4).  The model is 2 % off in the last of these: where the last round is three quarters
+    full, a block a tile is as good or a little better, and it counts what sharing costs too low."""
     items = batch * n_kv * -(-max_q_len * group // 128)
     tiles = -(-keys // 128)
     traffic = tokens * n_kv * group * head_dim * 8 / 6.5e12 / (3e-6 * head_dim / 256)
