@@ -94,7 +94,8 @@ __device__ __forceinline__ int last_not_above(const int* at, int n, int x) {
     return lo;
 }
 
-// CLUSTER: the launch is one cluster and does everything.  Else `held` and `count` are left to commit_kernel.
+// CLUSTER: the launch is one cluster and does everything.  Else `held`, `count` and `kv_len` (which may be `lengths`, in place)
+// are left to commit_kernel.
 template <bool CLUSTER>
 __global__ void __launch_bounds__(THREADS) blocks_extend_kernel(ExtendArgs a) {
     extern __shared__ int rows_s[];
@@ -170,7 +171,7 @@ __global__ void __launch_bounds__(THREADS) blocks_extend_kernel(ExtendArgs a) {
     for (int i = me; i < a.rows; i += all) {
         const bool live = ok && before[i] >= 0;
         a.cu_q[i] = ok ? token0[i] : 0;
-        a.kv_len[i] = live ? before[i] + token0[i + 1] - token0[i] : 0;
+        if constexpr (CLUSTER) a.kv_len[i] = live ? before[i] + token0[i + 1] - token0[i] : 0;
         if (CLUSTER && live && block0[i + 1] != block0[i]) a.held[slot_s[i]] = held_s[i] + block0[i + 1] - block0[i];
     }
     for (int k = me; k < n_new; k += all) {
@@ -224,17 +225,18 @@ __global__ void __launch_bounds__(THREADS) blocks_extend_kernel(ExtendArgs a) {
     }
 }
 
-// What blocks_extend_kernel<false> leaves: the slots' blocks and the stack's height, if the step was taken.
+// What blocks_extend_kernel<false> leaves: the lengths, and, if the step was taken, the slots' blocks and the stack's height.
 __global__ void __launch_bounds__(THREADS) commit_kernel(ExtendArgs a) {
     __shared__ int taken;
     if (threadIdx.x == 0) taken = 0;
     __syncthreads();
-    if (*a.status != ST_OK) return;
+    const bool ok = *a.status == ST_OK;
     int mine = 0;
     for (int i = threadIdx.x; i < a.rows; i += THREADS) {
-        const int s = a.slots[i];
+        const int s = ok ? a.slots[i] : -1, len = s >= 0 ? a.lengths[i] + a.fresh[i] : 0;
+        a.kv_len[i] = len;
         if (s < 0) continue;
-        const int have = a.held[s], need = blocks_for((long long)a.lengths[i] + a.fresh[i], a.block, a.ring);
+        const int have = a.held[s], need = blocks_for(len, a.block, a.ring);
         if (need > have) {
             a.held[s] = need;
             mine += need - have;
@@ -242,7 +244,7 @@ __global__ void __launch_bounds__(THREADS) commit_kernel(ExtendArgs a) {
     }
     if (mine) atomicAdd(&taken, mine);
     __syncthreads();
-    if (threadIdx.x == 0) *a.count -= taken;
+    if (threadIdx.x == 0 && taken) *a.count -= taken;
 }
 
 // The blocks of the rows' slots go back to the stack, the last row's last block first: what one extend took, one release
@@ -370,11 +372,13 @@ BROLM_API int brolm_blocks_extend(const ExtendCall* c) {
         st = launch_pdl(blocks_extend_kernel<false>, dim3(min(device_sm_count(), (c->tokens + THREADS - 1) / THREADS)), dim3(THREADS), smem,
                         c->stream, a);
         if (st) return st;
-        commit_kernel<<<1, THREADS, 0, c->stream>>>(a);      // (in plain stream order: it settles the first one's results, too)
-        return launch_status();
+        commit_kernel<<<1, THREADS, 0, c->stream>>>(a);
+        st = launch_status();
+        if (st || !c->settle) return st;
+    } else {
+        const int st = launch_cluster(blocks_extend_kernel<true>, a, c->tokens, smem, raised, c->stream);
+        if (st || !c->settle) return st;
     }
-    const int st = launch_cluster(blocks_extend_kernel<true>, a, c->tokens, smem, raised, c->stream);
-    if (st || !c->settle) return st;
     // A launch in plain stream order begins when this one has ended and its results are in memory: whatever is launched
     // behind it may read them before it waits for its predecessor, as many kernels read a step's description.
     settle_kernel<<<1, 32, 0, c->stream>>>();

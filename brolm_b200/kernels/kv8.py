@@ -83,6 +83,7 @@ def blocks_extend(slots: torch.Tensor, lengths: torch.Tensor, new: torch.Tensor,
     and are entered behind those that ``tables[slot]`` holds.  Written: ``cu_q`` [rows + 1] (sums of ``new``), ``kv_len``
     [rows] (0 for padding), and for every token, rows back to back, ``positions``, ``tok_seq`` (its row) and ``cache_rows``
     (block * block size + place, -1 where the ring does not keep the token); places beyond the last token get -1, 0, -1.
+    ``kv_len`` may be ``lengths``, which then go on in place; the other outputs are tensors of their own.
 
     ``settle``: kernels launched behind this call may read what it writes (all but the tables and ``cache_rows``, which are
     read after the wait) before they wait for the launch before them; the kernels of this package that read a step's

@@ -895,3 +895,30 @@ def test_block_ids_that_no_cache_has_give_no_places(tokens):
         kernels.blocks_extend(ints([1]), ints([before]), ints([n]), *state.values(), block=32, **out)
         want = [ids[p // 32] * 32 + p % 32 if ids[p // 32] in (5, 2 ** 26 - 1) else -1 for p in range(before, before + n)]
         assert int(out["status"]) == 0 and out["cache_rows"][:n].tolist() == want
+
+
+@pytest.mark.parametrize("tokens", [3000, 120000])
+def test_lengths_that_go_on_in_place(tokens):
+    """`kv_len` is `lengths`: many rows, so that some blocks of threads still read while others write."""
+    n, block = 4000, 32
+    rng = random.Random(tokens)
+    new = [rng.choice([0, 1, 1]) if tokens < 4000 else rng.choice([1, 20, 40]) for _ in range(n)]
+    new = [0 if sum(new[:i]) > tokens - 50 else m for i, m in enumerate(new)] if sum(new) > tokens else new
+    slots = [i if rng.random() < 0.95 else -1 for i in rng.sample(range(n), n)]
+    state = dict(tables=torch.zeros((n, 12), dtype=I32, device=DEV), held=ints([0] * n), free=ints(range(30000)), free_count=ints([30000]))
+    lengths, want = ints([5] * n), [5] * n
+    out = dict(cu_q=ints([0] * (n + 1)), positions=ints([0] * tokens), tok_seq=ints([0] * tokens), cache_rows=ints([0] * tokens), status=ints([7]))
+    for turn in range(4):
+        kernels.blocks_extend(ints(slots), lengths, ints(new), *state.values(), block=block, kv_len=lengths, **out)
+        want = [w + m if s >= 0 else 0 for w, m, s in zip(want, new, slots)]
+        assert int(out["status"]) == 0 and lengths.tolist() == want
+        held = [0] * n
+        for w, s in zip(want, slots):
+            if s >= 0:
+                held[s] = -(-w // block)
+        assert state["held"].tolist() == held and int(state["free_count"]) == 30000 - sum(held)
+        pos = [p for w, m, s in zip(want, new, slots) for p in (range(w - m, w) if s >= 0 else [-1] * m)]
+        assert out["positions"][:len(pos)].tolist() == pos
+    before = lengths.clone()
+    kernels.blocks_extend(ints(slots), lengths, ints([10000] + new[1:]), *state.values(), block=block, kv_len=lengths, **out)
+    assert int(out["status"]) > 0 and not lengths.any() and bool(before.any())
