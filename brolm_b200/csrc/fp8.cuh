@@ -1,0 +1,89 @@
+// Rows of 8-bit floating point numbers with a scale for every 128 numbers of a row, as the fp8 kernels keep them.
+//
+// A number is e4m3 (largest 448) times 2^(s - 127), s being the byte of its block: the least from 0 on under which none of
+// the block's numbers is beyond 448 * 2^(s - 127).  A power of two because x * 2^(127 - s) is then exact, so that a number is
+// rounded once and the same wherever it is rounded, and because tcgen05.mma takes such scales itself (kind::mxf8f6f4: an
+// exponent for every 32 numbers along K; a block of 128 is four of them with one exponent).  A block with a number that is
+// not finite has the byte 255 and NaN for every number: all that is computed from it is NaN.
+//
+// Scales lie as the tensor core wants them in tensor memory: a tile of 512 bytes holds 128 rows times four blocks; row r,
+// block b of the tile at byte (r % 32) * 16 + (r / 32) * 4 + b, so that tcgen05.cp with the shape 32x128b makes of it four columns of
+// tensor memory, row r in lane r % 32 of column r / 32, its four blocks in the four bytes of that word.  Tiles are ordered
+// [128 rows][512 columns].
+#pragma once
+
+#include "tcgen05.cuh"
+
+namespace fp8 {
+
+constexpr int BLOCK = 128;                 // numbers that share a scale
+constexpr int SF_TILE = 512;               // bytes of scales for 128 rows x 4 blocks
+
+__host__ __device__ __forceinline__ int blocks_of(int cols) { return (cols + BLOCK - 1) / BLOCK; }
+__host__ __device__ __forceinline__ int quads_of(int cols) { return (cols + 4 * BLOCK - 1) / (4 * BLOCK); }
+
+// where the four scales of row r (of the matrix, or r of the tile's rows with `tile0` its first tile) and blocks 4 q .. lie
+__device__ __forceinline__ size_t scale_at(long row, int q, int quads) {
+    return ((size_t)(row >> 7) * quads + q) * SF_TILE + (row & 31) * 16 + ((row >> 5) & 3) * 4;
+}
+
+// the scale's byte for a block whose largest magnitude has these bits
+__device__ __forceinline__ uint32_t scale_byte(uint32_t bits) {
+    const int e = (int)(bits >> 23);
+    if (e >= 255) return 255u;
+    // 448 = 1.75 * 2^8: an exponent of eight less, one more where the mantissa is beyond 0.75
+    return (uint32_t)max(e - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0), 0);
+}
+__device__ __forceinline__ float scale_inverse(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }      // byte <= 247
+__device__ __forceinline__ float scale_value(uint32_t byte) {
+    return byte == 255u ? __uint_as_float(0x7fc00000u) : byte == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(byte << 23);
+}
+// four numbers, scaled by `inv` (exact), rounded to nearest even
+__device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d, float inv) {
+    uint32_t r;
+    asm("{\n.reg .b16 lo, hi;\ncvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\ncvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\nmov.b32 %0, {lo, hi};\n}"
+        : "=r"(r) : "f"(a * inv), "f"(b * inv), "f"(c * inv), "f"(d * inv));
+    return r;
+}
+constexpr uint32_t NAN4 = 0x7f7f7f7fu;
+
+// ---- tensor core, operands e4m3, scales ue8m0
+// Instruction descriptor of kind::mxf8f6f4 without the scales' byte numbers (a: bits 29-30, b: bits 4-5).
+__device__ __forceinline__ uint32_t idesc_mx(int m, int n) {
+    return (1u << 23) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+__device__ __forceinline__ uint32_t with_block(uint32_t id, int a_byte, int b_byte) {
+    return id | ((uint32_t)a_byte << 29) | ((uint32_t)b_byte << 4);
+}
+__device__ __forceinline__ void umma_mx(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %6, 0;\n"
+                 "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+}
+// A scale tile in shared memory: 32 rows of 16 bytes, eight rows (128 bytes) to the next group, no swizzle.
+__device__ __forceinline__ uint64_t desc_scales(uint32_t addr) {
+    return (uint64_t)((addr >> 4) & 0x3fffu) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
+}
+__device__ __forceinline__ void scales_to_tmem(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// an untiled copy; both addresses and the size multiples of 16 bytes
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+// ---- host: rows x cols bytes, row-major with `ld` bytes between rows; box = box_rows x 128 columns, 128-byte swizzle
+static inline int make_map_u8(CUtensorMap* map, const void* ptr, long long rows, long long cols, long long ld, int box_rows) {
+    tc::EncodeTiled enc = tc::encoder();
+    if (!enc) return BROLM_ERR_BAD_SIZE;
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)ld};
+    const cuuint32_t box[2] = {128, (cuuint32_t)box_rows}, elem[2] = {1, 1};
+    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, elem,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? BROLM_OK : BROLM_ERR_ALIGNMENT;
+}
+
+}  // namespace fp8

@@ -1,0 +1,493 @@
+// Products with a matrix in 8-bit floating point for many rows (the format is in fp8.cuh), on pairs of SMs:
+//     Y[m,n] = sum over blocks b of 2^(sx[m,b] + sw[n,b]) * (sum over the block's k of X[m,k] W[n,k]),  float sums.
+//
+// Two blocks of a cluster make a tile of 256 x 256 (tcgen05.mma.cta_group::2.kind::mxf8f6f4, which multiplies by the scales
+// itself): each loads its 128 rows of X and its half of the 256 rows of W.  A stage is one block of 128 along K, 32 KB a block
+// of the pair; with the first block of every four come their scales, 512 bytes for the block's rows of X and 1,024 for all 256
+// rows of W, which tcgen05.cp carries into both blocks' tensor memory.
+//
+//   warp 0 (both blocks)   one thread: TMA loads, their bytes counted on the first block's barrier
+//   warp 1 (first block)   one thread: copies of scales, products, commits to both blocks
+//   warps 2-9 (both)       epilogue: a thread has a row of the tile and half of its columns
+//
+// Tensor memory has 512 columns: two accumulators of 256 leave no room for the scales.  So the second accumulator begins 32
+// columns before the first ends.  A tile's products begin when the epilogue has taken those 32 columns of the tile before
+// (its first loads), and when the accumulator's own tile, two before, has been taken whole.
+//
+// The tensor core cuts off where an fma rounds, so float results are summed in pieces of `piece` blocks of K, which the
+// epilogue adds in registers; results that are rounded to fewer bits are one piece.
+//
+// Epilogues: the product (with the square of relu, or a gated activation of neighbouring rows of W) as bfloat16, as float, or
+// rounded to 8 bits as rows for the next product: a block of 128 results of a row is within a tile.  Experts: a list made on
+// the device names for every tile of 256 rows its expert and its first row.
+//
+// Every mbarrier wait is bounded (tcgen05.cuh).
+#include "fp8.cuh"
+
+#include <type_traits>
+
+namespace {
+
+using namespace tc;
+using namespace fp8;
+
+constexpr int BM = 128, PM = 256, BN = 256, HN = 128, BK = 128, STAGES = 6;
+constexpr int A_BYTES = BM * BK, B_BYTES = HN * BK, STAGE_BYTES = A_BYTES + B_BYTES, SCALES = 3 * SF_TILE;
+constexpr int THREADS = 320;
+constexpr int TMEM_COLS = 512, ACC1 = 224, SF_COL = 480;
+constexpr int ROWS_BYTES = 2 * BM * 4;      // largest magnitudes of a row's two halves
+
+enum : int { EPI_STORE = 0, EPI_GATED = 1 };
+enum : int { OUT_BF16 = 0, OUT_F32 = 1, OUT_FP8 = 2 };
+enum : int { ACT_NONE = 0, ACT_RELU2 = 1 };
+
+__device__ int g_fp8_gemm_error;
+
+struct GemmArgs {
+    void* y;
+    long ldy;                // elements (OUT_FP8: bytes)
+    uint8_t* y_scales;
+    int y_quads;
+    int M, N;                // rows; output columns
+    int act;
+    float limit;
+    int nkb, piece;
+    int quads;               // words of scales of a row of X and W
+    int m_tiles, n_tiles;
+    // experts
+    const int32_t* tile_group;      // null: dense
+    const int32_t* tile_row0;
+    const int32_t* offsets;
+    const int32_t* perm;
+    const float* scale;
+    int down, top, tokens, group_rows;
+};
+
+__device__ __forceinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile int* give_up, int code) {
+    return mbar_wait(bar, parity, give_up, &g_fp8_gemm_error, code);
+}
+__device__ __forceinline__ bool drain_on(uint32_t bar, uint32_t parity, volatile int* give_up, int code) {
+    return mbar_wait(bar, parity, give_up, &g_fp8_gemm_error, code, true);
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync_all() {
+    asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
+}
+// The cta_group::2 forms.  A shared-memory address with bit 24 cleared names the same place in the first block of the pair.
+constexpr uint32_t PEER_MASK = 0xFEFFFFFFu;
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar & PEER_MASK) : "memory");
+}
+__device__ __forceinline__ void umma_mx_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %6, 0;\n"
+                 "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void scales_to_tmem_pair(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+__device__ __forceinline__ void umma_commit_pair(uint32_t bar) {      // arrives on the barrier in both blocks
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t slot_smem, uint32_t cols) {     // whole warp, in both blocks
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot_smem), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t cols) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
+}
+__device__ __forceinline__ void arrive_first_block(uint32_t bar) {                       // from either block
+    asm volatile("{\n.reg .b32 remote;\nmapa.shared::cluster.u32 remote, %0, 0;\nmbarrier.arrive.shared::cluster.b64 _, [remote];\n}"
+                 ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ float act_of(float v, int act) {
+    if (act == ACT_RELU2) {
+        v = fmaxf(v, 0.0f);
+        return v * v;
+    }
+    return v;
+}
+
+// n results of a row from column `col` on, those below `cols` alone
+template <int N>
+__device__ __forceinline__ void store_row(bf16* dst, const float* o, int col, int cols, bool wide) {
+    if (wide && col + N <= cols) {
+#pragma unroll
+        for (int i = 0; i < N; i += 8) {
+            uint4 p;
+            __nv_bfloat162* p2 = reinterpret_cast<__nv_bfloat162*>(&p);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) p2[e] = __floats2bfloat162_rn(o[i + 2 * e], o[i + 2 * e + 1]);
+            *reinterpret_cast<uint4*>(dst + i) = p;
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) if (col + i < cols) dst[i] = __float2bfloat16_rn(o[i]);
+}
+template <int N>
+__device__ __forceinline__ void store_row(float* dst, const float* o, int col, int cols, bool wide) {
+    if (wide && col + N <= cols) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(dst + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) if (col + i < cols) dst[i] = o[i];
+}
+
+__device__ __forceinline__ void load_columns(uint32_t taddr, uint32_t (&v)[32]) { tmem_ld32(taddr, v); }
+__device__ __forceinline__ void load_columns(uint32_t taddr, uint32_t (&v)[16]) { tmem_ld16(taddr, v); }
+// f(part, turn) for the 128 / CW parts, the last BACK of them first
+template <int CW, int BACK, int TURN = 0, typename F>
+__device__ __forceinline__ void in_order(F&& f) {
+    constexpr int PARTS = 128 / CW;
+    f(std::integral_constant<int, (TURN + PARTS - BACK) % PARTS>{}, TURN);
+    if constexpr (TURN + 1 < PARTS) in_order<CW, BACK, TURN + 1>(f);
+}
+
+template <int EPI, int OUT, bool EXPERTS>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+                const __grid_constant__ CUtensorMap map_xs, const __grid_constant__ CUtensorMap map_ws, GemmArgs g) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* base = smem_raw;
+    const uint32_t rank = cluster_rank();
+    uint64_t* bars = reinterpret_cast<uint64_t*>(base + STAGES * (STAGE_BYTES + SCALES));
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 6);
+    volatile int* give_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    uint32_t* most_of = tmem_slot + 4;                        // [2][128]
+    const uint32_t stage0 = smem_u32(base), scale0 = stage0 + STAGES * STAGE_BYTES;
+    const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * STAGES, acc_full0 = empty0 + 8 * STAGES,
+                   acc_free0 = acc_full0 + 16, lap_free = acc_free0 + 16;
+    const bool aligned = (stage0 & 1023u) == 0;               // both blocks have the same layout
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int total = g.m_tiles * g.n_tiles;
+    const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
+    constexpr int OUT_COLS = EPI == EPI_GATED ? BN / 2 : BN;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(full0 + 8 * s, 1);
+            mbar_init(empty0 + 8 * s, 1);
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(acc_full0 + 8 * s, 1);
+            mbar_init(acc_free0 + 8 * s, 16);     // eight epilogue warps of each block
+        }
+        mbar_init(lap_free, 8);                   // the four of each whose columns lie in both accumulators
+        give_up[0] = aligned ? 0 : 1;
+        give_up[1] = 0;
+        give_up[2] = tc::g_stall_code;
+        if (!aligned) atomicCAS(&g_fp8_gemm_error, 0, 13);
+        mbar_init_fence();
+    }
+    if (warp == 1) tmem_alloc_pair(smem_u32(tmem_slot), TMEM_COLS);
+    fence_before_sync();
+    cluster_sync_all();
+    fence_after_sync();
+    const uint32_t tmem = *tmem_slot;
+
+    // what a tile is: false behind the experts' last
+    auto find = [&](int tile, int& mt, int& nt, int& group, int& row0) {
+        if (!EXPERTS) {
+            nt = tile / g.m_tiles;
+            mt = tile - nt * g.m_tiles;
+            group = 0;
+            row0 = mt * PM;
+            return true;
+        }
+        mt = tile / g.n_tiles;
+        nt = tile - mt * g.n_tiles;
+        group = g.tile_group[mt];
+        if (group < 0) return false;
+        row0 = g.tile_row0[mt];
+        return true;
+    };
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int it = 0, s = 0, phase = 0;
+            bool ok = !*give_up;
+            // Launched with programmatic stream serialization: nothing of this kernel touches memory before its first
+            // operands have arrived, so (but for the experts' lists) the loader's wait is the kernel's.
+            pdl_wait();
+            int mt, nt, group, row0;
+            for (int tile = pair; tile < total && ok; tile += n_pairs) {
+                if (!find(tile, mt, nt, group, row0)) break;
+                const int w_row = group * g.group_rows + nt * BN;
+                const int xs_row = (EXPERTS ? mt * (PM / 128) : row0 >> 7) + (int)rank, ws_row = w_row >> 7;
+                for (int kb = 0; kb < g.nkb; ++kb, ++it) {
+                    if (!wait_on(empty0 + 8 * s, phase ^ 1, give_up, 1)) { ok = false; break; }
+                    const uint32_t full = full0 + 8 * s, a_dst = stage0 + s * STAGE_BYTES, s_dst = scale0 + s * SCALES;
+                    const bool with_scales = (kb & 3) == 0;
+                    if (rank == 0) mbar_expect_tx(full, 2 * (STAGE_BYTES + (with_scales ? SCALES : 0)));   // both blocks' bytes
+                    tma_load_pair(a_dst, &map_x, kb * BK, row0 + (int)rank * BM, full);
+                    tma_load_pair(a_dst + A_BYTES, &map_w, kb * BK, w_row + (int)rank * HN, full);
+                    if (with_scales) {
+                        const int q = kb >> 2;
+                        tma_load_pair(s_dst, &map_xs, 0, xs_row * g.quads + q, full);
+                        tma_load_pair(s_dst + SF_TILE, &map_ws, 0, ws_row * g.quads + q, full);
+                        tma_load_pair(s_dst + 2 * SF_TILE, &map_ws, 0, (ws_row + 1) * g.quads + q, full);
+                    }
+                    if (++s == STAGES) { s = 0; phase ^= 1; }
+                }
+            }
+            pdl_trigger();                                  // the operands are asked for: the next kernel may move in
+            if (*give_up && rank == 0) {
+                for (int j = max(0, it - STAGES); j < it; ++j) drain_on(full0 + 8 * (j % STAGES), (j / STAGES) & 1, give_up, 4);
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            const uint32_t id = idesc_mx(PM, BN);
+            int s = 0, phase = 0, local = 0, set = 0;
+            bool ok = !*give_up;
+            if (EXPERTS) pdl_wait();
+            int mt, nt, group, row0;
+            for (int tile = pair; tile < total && ok; tile += n_pairs) {
+                if (!find(tile, mt, nt, group, row0)) break;
+                uint32_t sfw = 0, sfx = 0;
+                for (int lo = 0; lo < g.nkb && ok; lo += g.piece, ++local) {
+                    const int as = local & 1, hi = min(g.nkb, lo + g.piece);
+                    ok = wait_on(acc_free0 + 8 * as, ((local >> 1) & 1) ^ 1, give_up, 5) && wait_on(lap_free, (local & 1) ^ 1, give_up, 6);
+                    if (!ok) break;
+                    fence_after_sync();
+                    const uint32_t acc = tmem + as * ACC1;
+                    for (int kb = lo; kb < hi; ++kb) {
+                        ok = wait_on(full0 + 8 * s, phase, give_up, 2);
+                        if (!ok) break;
+                        fence_after_sync();
+                        if ((kb & 3) == 0) {
+                            sfw = tmem + SF_COL + 16 * set;
+                            sfx = sfw + 8;
+                            set ^= 1;
+                            const uint32_t src = scale0 + s * SCALES;
+                            scales_to_tmem_pair(sfx, desc_scales(src));
+                            scales_to_tmem_pair(sfw, desc_scales(src + SF_TILE));
+                            scales_to_tmem_pair(sfw + 4, desc_scales(src + 2 * SF_TILE));
+                        }
+                        const uint32_t idk = with_block(id, kb & 3, kb & 3);
+                        const uint64_t a = desc_kmajor(stage0 + s * STAGE_BYTES), b = desc_kmajor(stage0 + s * STAGE_BYTES + A_BYTES);
+#pragma unroll
+                        for (int k = 0; k < BK / 32; ++k) umma_mx_pair(acc, a + 2 * k, b + 2 * k, idk, sfx, sfw, (kb > lo) | (k > 0));
+                        umma_commit_pair(empty0 + 8 * s);
+                        if (++s == STAGES) { s = 0; phase ^= 1; }
+                    }
+                    if (ok) umma_commit_pair(acc_full0 + 8 * as);
+                }
+            }
+        }
+    } else {
+        const int quarter = warp & 3, half = (warp - 2) >> 2;
+        const int trow = quarter * 32 + lane;                   // row of this block's half of the tile
+        int local = 0;
+        if (EXPERTS) pdl_wait();
+        int mt, nt, group, row0;
+        bool ok = true;
+        for (int tile = pair; tile < total && ok; tile += n_pairs) {
+            if (!find(tile, mt, nt, group, row0)) break;
+            const int row = row0 + (int)rank * BM + trow;
+            const bool valid = row < (EXPERTS ? g.offsets[group + 1] : g.M);
+            long at = row;
+            float mul = 1.0f;
+            if (EXPERTS && valid) {
+                if (g.down) {
+                    const int p = g.perm[row], tok = p / g.top;
+                    at = (long)(p - tok * g.top) * g.tokens + tok;
+                }
+                if (g.scale) mul = g.scale[g.perm[row]];
+            }
+            constexpr int CW = OUT == OUT_BF16 ? 32 : 16;       // (as many registers as there are)
+            float sum[128];                                     // OUT_F32: the pieces' sum; OUT_FP8: the row's half
+            for (int lo = 0; lo < g.nkb; lo += g.piece, ++local) {
+                const int as = local & 1;
+                const bool ready = wait_on(acc_full0 + 8 * as, (local >> 1) & 1, give_up, 3);
+                if (!__all_sync(0xffffffffu, ready)) { ok = false; break; }
+                fence_after_sync();
+                const uint32_t acc = tmem + as * ACC1 + half * 128 + ((uint32_t)(quarter * 32) << 16);
+                // CW columns: the first 32 read are those that the other accumulator wants
+                auto take = [&](auto part, int turn) {
+                    constexpr int C = decltype(part)::value * CW;
+                    uint32_t v[CW];
+                    load_columns(acc + C, v);
+                    tmem_wait_ld();
+                    if (turn == 32 / CW - 1 && half != as) {
+                        fence_before_sync();
+                        __syncwarp();
+                        if (lane == 0) arrive_first_block(lap_free);
+                    }
+                    if (turn == 128 / CW - 1) {
+                        fence_before_sync();
+                        __syncwarp();
+                        if (lane == 0) arrive_first_block(acc_free0 + 8 * as);
+                    }
+                    if (OUT == OUT_F32) {
+#pragma unroll
+                        for (int i = 0; i < CW; ++i) sum[C + i] = lo == 0 ? __uint_as_float(v[i]) : sum[C + i] + __uint_as_float(v[i]);
+                        return;
+                    }
+                    float o[CW];
+#pragma unroll
+                    for (int i = 0; i < CW; ++i) o[i] = EXPERTS ? __uint_as_float(v[i]) * mul : __uint_as_float(v[i]);
+                    if (EPI == EPI_GATED) {
+#pragma unroll
+                        for (int i = 0; i < CW / 2; ++i) o[i] = fast_gate_pair(o[2 * i], o[2 * i + 1], g.act, g.limit);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < CW; ++i) o[i] = act_of(o[i], g.act);
+                    }
+                    constexpr int W = EPI == EPI_GATED ? CW / 2 : CW, OC = EPI == EPI_GATED ? C / 2 : C;
+                    if (OUT == OUT_FP8) {
+#pragma unroll
+                        for (int i = 0; i < W; ++i) sum[OC + i] = o[i];
+                        return;
+                    }
+                    const int col = nt * OUT_COLS + half * (OUT_COLS / 2) + OC;
+                    if (valid && col < g.N) store_row<W>((bf16*)g.y + at * g.ldy + col, o, col, g.N, (g.ldy & 7) == 0);
+                };
+                if (as == 0) in_order<CW, 32 / CW>(take);
+                else in_order<CW, 0>(take);
+            }
+            if (!ok) break;
+            if (OUT == OUT_F32) {
+                if (EXPERTS) {
+#pragma unroll
+                    for (int i = 0; i < 128; ++i) sum[i] *= mul;
+                }
+                constexpr int W = EPI == EPI_GATED ? 64 : 128;
+                if (EPI == EPI_GATED) {
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) sum[i] = fast_gate_pair(sum[2 * i], sum[2 * i + 1], g.act, g.limit);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 128; ++i) sum[i] = act_of(sum[i], g.act);
+                }
+                const int col = nt * OUT_COLS + half * W;
+                if (valid && col < g.N) store_row<W>((float*)g.y + at * g.ldy + col, sum, col, g.N, (g.ldy & 3) == 0);
+            }
+            if (OUT == OUT_FP8) {
+                constexpr int W = EPI == EPI_GATED ? 64 : 128;
+                const int col = nt * OUT_COLS + half * W;
+                uint32_t most = 0;
+#pragma unroll
+                for (int i = 0; i < W; ++i) {
+                    if (col + i >= g.N) sum[i] = 0.0f;          // columns of no output are no part of the block
+                    most = max(most, __float_as_uint(sum[i]) & 0x7fffffffu);
+                }
+                if (EPI == EPI_GATED) {                         // the block's other half is another warp's
+                    most_of[half * 128 + trow] = most;
+                    asm volatile("bar.sync 1, 256;" ::: "memory");
+                    most = max(most, most_of[(half ^ 1) * 128 + trow]);
+                    asm volatile("bar.sync 1, 256;" ::: "memory");
+                }
+                const uint32_t byte = scale_byte(most);
+                const float inv = byte == 255u ? 1.0f : scale_inverse(byte);
+                if (valid && col < g.N) {
+                    uint8_t* dst = (uint8_t*)g.y + at * g.ldy + col;
+#pragma unroll
+                    for (int i = 0; i < W; i += 16) {
+                        uint4 q = make_uint4(NAN4, NAN4, NAN4, NAN4);
+                        if (byte != 255u)
+                            q = make_uint4(pack4(sum[i], sum[i + 1], sum[i + 2], sum[i + 3], inv), pack4(sum[i + 4], sum[i + 5], sum[i + 6], sum[i + 7], inv),
+                                           pack4(sum[i + 8], sum[i + 9], sum[i + 10], sum[i + 11], inv), pack4(sum[i + 12], sum[i + 13], sum[i + 14], sum[i + 15], inv));
+                        if (col + i < g.ldy) *reinterpret_cast<uint4*>(dst + i) = q;       // ldy is a multiple of 16
+                    }
+                    const int b = col >> 7;
+                    // scales by the row's tile: rows of the matrix (dense), rows of the list's tile (experts)
+                    const long s_row = EXPERTS ? (long)mt * PM + rank * BM + trow : row;
+                    if (EPI != EPI_GATED || half == 0) g.y_scales[scale_at(s_row, b >> 2, g.y_quads) + (b & 3)] = (uint8_t)byte;
+                }
+            }
+        }
+    }
+    fence_before_sync();
+    __syncwarp();
+    cluster_sync_all();                 // neither block frees memory the other may still signal
+    if (warp == 1) tmem_dealloc_pair(tmem, TMEM_COLS);
+}
+
+constexpr size_t SMEM_BYTES = (size_t)STAGES * (STAGE_BYTES + SCALES) + (2 * STAGES + 6) * 8 + 16 + ROWS_BYTES;
+
+// a matrix of scale tiles: rows of 512 bytes
+int make_map_scales(CUtensorMap* map, const void* ptr, long long tiles) {
+    EncodeTiled enc = encoder();
+    if (!enc) return BROLM_ERR_BAD_SIZE;
+    const cuuint64_t dims[2] = {128, (cuuint64_t)tiles}, strides[1] = {SF_TILE};
+    const cuuint32_t box[2] = {128, 1}, elem[2] = {1, 1};
+    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_INT32, 2, const_cast<void*>(ptr), dims, strides, box, elem,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? BROLM_OK : BROLM_ERR_ALIGNMENT;
+}
+
+struct Maps { CUtensorMap x, w, xs, ws; };
+
+template <int EPI, int OUT, bool EXPERTS>
+int launch(const Maps& m, const GemmArgs& g, cudaStream_t stream) {
+    static OncePerDevice done;
+    const int st = allow_shared_memory(fp8_gemm_kernel<EPI, OUT, EXPERTS>, SMEM_BYTES, done);
+    if (st) return st;
+    const int tiles = g.m_tiles * g.n_tiles, most = device_sms() / 2, pairs = tiles < most ? tiles : most;
+    return launch_pdl(fp8_gemm_kernel<EPI, OUT, EXPERTS>, dim3(2 * pairs), dim3(THREADS), SMEM_BYTES, stream, m.x, m.w, m.xs, m.ws, g);
+}
+template <bool EXPERTS>
+int dispatch(const Maps& m, const GemmArgs& g, int epilogue, int out, cudaStream_t stream) {
+    if (epilogue == EPI_GATED) {
+        if (out == OUT_BF16) return launch<EPI_GATED, OUT_BF16, EXPERTS>(m, g, stream);
+        if (out == OUT_F32) return launch<EPI_GATED, OUT_F32, EXPERTS>(m, g, stream);
+        return launch<EPI_GATED, OUT_FP8, EXPERTS>(m, g, stream);
+    }
+    if (out == OUT_BF16) return launch<EPI_STORE, OUT_BF16, EXPERTS>(m, g, stream);
+    if (out == OUT_F32) return launch<EPI_STORE, OUT_F32, EXPERTS>(m, g, stream);
+    return launch<EPI_STORE, OUT_FP8, EXPERTS>(m, g, stream);
+}
+
+}  // namespace
+
+// Y [M, N] = X W^T (epilogue 0, act 0 or the square of relu) or the gated activation of W's neighbouring rows (epilogue 1: W
+// has 2 N rows).  X and W as brolm_fp8_quantize leaves them.  out 0: bfloat16, 1: float (sums in pieces of `piece` blocks of
+// K), 2: 8 bits (ldy bytes, a multiple of 16, and scales of ceil(N / 512) words).
+BROLM_API int brolm_fp8_gemm(const void* x, long long ldx, const void* x_scales, const void* w, long long ldw, const void* w_scales,
+                             void* y, long long ldy, void* y_scales, int out, int M, int N, int K, int epilogue, int act, float limit,
+                             int piece, cudaStream_t stream) {
+    if (M <= 0 || N <= 0) return BROLM_OK;
+    if (K <= 0 || ldx % 16 || ldw % 16 || (((uintptr_t)x | (uintptr_t)w | (uintptr_t)x_scales | (uintptr_t)w_scales) & 15)) return BROLM_ERR_ALIGNMENT;
+    if (((uintptr_t)y & 15) || (out == OUT_FP8 && (ldy % 16 || ldy < N || !y_scales))) return BROLM_ERR_ALIGNMENT;
+    if (epilogue < 0 || epilogue > 1 || out < 0 || out > 2 || act < 0 || act > 2 || (epilogue == EPI_STORE && act > ACT_RELU2)) return BROLM_ERR_BAD_SIZE;
+    const int w_rows = epilogue == EPI_GATED ? 2 * N : N;
+    Maps m;
+    GemmArgs g = {};
+    g.quads = quads_of(K);
+    int st = make_map_u8(&m.x, x, M, K, ldx, BM);
+    if (!st) st = make_map_u8(&m.w, w, w_rows, K, ldw, HN);
+    if (!st) st = make_map_scales(&m.xs, x_scales, (long long)((M + 127) / 128) * g.quads);
+    if (!st) st = make_map_scales(&m.ws, w_scales, (long long)((w_rows + 127) / 128) * g.quads);
+    if (st) return st;
+    g.y = y; g.ldy = (long)ldy; g.y_scales = (uint8_t*)y_scales; g.y_quads = quads_of(N);
+    g.M = M; g.N = N; g.act = act; g.limit = limit; g.nkb = blocks_of(K);
+    g.piece = out == OUT_F32 && piece > 0 && piece < g.nkb ? piece : g.nkb;
+    g.m_tiles = (M + PM - 1) / PM;
+    const int out_cols = epilogue == EPI_GATED ? BN / 2 : BN;
+    g.n_tiles = (N + out_cols - 1) / out_cols;
+    return dispatch<false>(m, g, epilogue, out, stream);
+}
+
+BROLM_API int brolm_fp8_gemm_status(int reset) {
+    int v = 0;
+    if (cudaMemcpyFromSymbol(&v, g_fp8_gemm_error, sizeof(int)) != cudaSuccess) return -1;
+    if (reset && v) {
+        const int zero = 0;
+        cudaMemcpyToSymbol(g_fp8_gemm_error, &zero, sizeof(int));
+    }
+    return v;
+}
+
+BROLM_WAIT_CONTROL(fp8_gemm)

@@ -28,7 +28,7 @@ NVCC_FLAGS = [
     "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden", "-shared",
 ]
 
-# library name -> sources (headers are hashed with every library)
+# library name -> sources (HEADERS are hashed with every library)
 LIBRARIES: dict[str, list[str]] = {
     "core": ["core.cu"],
     "linear_f32": ["linear_f32.cu"],
@@ -59,8 +59,12 @@ LIBRARIES: dict[str, list[str]] = {
     "kv8": ["kv8.cu"],
     "attn_kv8": ["attn_kv8.cu"],
     "attn_kv8_tc": ["attn_kv8_tc.cu"],
+    "fp8_rows": ["fp8_rows.cu"],
+    "fp8_stream": ["fp8_stream.cu"],
+    "fp8_gemm": ["fp8_gemm.cu"],
 }
 HEADERS = ["common.cuh", "once_per_device.h", "attn_mma.cuh", "attn_decode_noalloc.h", "tcgen05.cuh", "kv8.cuh", "attn_kv8_join.cuh"]
+OWN_HEADERS = {"fp8_rows": ["fp8.cuh"], "fp8_stream": ["fp8.cuh"], "fp8_gemm": ["fp8.cuh"]}       # hashed with those libraries alone
 
 _loaded: dict[str, ctypes.CDLL] = {}
 _lock = threading.Lock()
@@ -106,7 +110,7 @@ def _build_dir() -> str:
 def _digest(name: str) -> str:
     h = hashlib.sha256()
     h.update(" ".join(NVCC_FLAGS).encode())
-    for rel in HEADERS + LIBRARIES[name]:
+    for rel in HEADERS + OWN_HEADERS.get(name, []) + LIBRARIES[name]:
         with open(os.path.join(CSRC, rel), "rb") as fh:
             h.update(rel.encode())
             h.update(fh.read())
