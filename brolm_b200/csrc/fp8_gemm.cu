@@ -480,6 +480,41 @@ BROLM_API int brolm_fp8_gemm(const void* x, long long ldx, const void* x_scales,
     return dispatch<false>(m, g, epilogue, out, stream);
 }
 
+// The products of experts, as brolm_fp8_experts_stream's but over tiles of 256 rows: x_scales has two tiles of 128 rows for every
+// tile of the list.  out as above; with `down` float [top, tokens, N].
+BROLM_API int brolm_fp8_experts_gemm(const void* x, long long ldx, const void* x_scales, const void* w, long long ldw, const void* w_scales,
+                                     void* y, long long ldy, void* y_scales, int out, int pairs, int N, int K, int experts, int group_rows,
+                                     int epilogue, int act, float limit, int piece, const void* tile_group, const void* tile_row0,
+                                     const void* offsets, const void* perm, const void* scale, int down, int top, int tokens,
+                                     int max_tiles, cudaStream_t stream) {
+    if (pairs <= 0 || N <= 0 || experts <= 0) return BROLM_OK;
+    if (K <= 0 || ldx % 16 || ldw % 16 || (((uintptr_t)x | (uintptr_t)w | (uintptr_t)x_scales | (uintptr_t)w_scales) & 15)) return BROLM_ERR_ALIGNMENT;
+    if (((uintptr_t)y & 15) || (out == OUT_FP8 && (ldy % 16 || ldy < N || !y_scales))) return BROLM_ERR_ALIGNMENT;
+    if (epilogue < 0 || epilogue > 1 || out < 0 || out > 2 || act < 0 || act > 2 || (epilogue == EPI_STORE && act > ACT_RELU2)) return BROLM_ERR_BAD_SIZE;
+    if (group_rows % 128 || (down && out != OUT_F32)) return BROLM_ERR_BAD_SIZE;
+    const int w_rows = epilogue == EPI_GATED ? 2 * N : N;
+    const long long all = (long long)experts * group_rows;
+    Maps m;
+    GemmArgs g = {};
+    g.quads = quads_of(K);
+    const int out_cols = epilogue == EPI_GATED ? BN / 2 : BN;
+    g.n_tiles = (N + out_cols - 1) / out_cols;
+    if (all > 0x7fffffff || (long long)max_tiles * g.n_tiles > 0x7fffffff) return BROLM_ERR_TOO_LARGE;
+    int st = make_map_u8(&m.x, x, pairs, K, ldx, BM);
+    if (!st) st = make_map_u8(&m.w, w, all, K, ldw, HN);
+    if (!st) st = make_map_scales(&m.xs, x_scales, 2LL * max_tiles * g.quads);
+    if (!st) st = make_map_scales(&m.ws, w_scales, all / 128 * g.quads);
+    if (st) return st;
+    g.y = y; g.ldy = (long)ldy; g.y_scales = (uint8_t*)y_scales; g.y_quads = quads_of(N);
+    g.N = N; g.act = act; g.limit = limit; g.nkb = blocks_of(K);
+    g.piece = out == OUT_F32 && piece > 0 && piece < g.nkb ? piece : g.nkb;
+    g.m_tiles = max_tiles;
+    g.tile_group = (const int32_t*)tile_group; g.tile_row0 = (const int32_t*)tile_row0; g.offsets = (const int32_t*)offsets;
+    g.perm = (const int32_t*)perm; g.scale = (const float*)scale;
+    g.down = down; g.top = top; g.tokens = tokens; g.group_rows = group_rows;
+    return dispatch<true>(m, g, epilogue, out, stream);
+}
+
 BROLM_API int brolm_fp8_gemm_status(int reset) {
     int v = 0;
     if (cudaMemcpyFromSymbol(&v, g_fp8_gemm_error, sizeof(int)) != cudaSuccess) return -1;

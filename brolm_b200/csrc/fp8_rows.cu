@@ -2,8 +2,11 @@
 //
 //   fp8_quantize   rows of float or bfloat16 numbers -> e4m3 numbers and a scale byte for every 128 of them
 //   fp8_read       the values that they stand for
+//   fp8_group      (token, choice) pairs sorted by expert, and the list of the experts' tiles of rows
+//   fp8_gather     the pairs' rows in that order in 8 bits
+//   fp8_combine    a token's results, multiplied by their weights and added
 //
-// Both are one pass over the data: a warp takes four blocks of a row at a time (512 numbers, one word of scales), eight
+// The first two are one pass over the data: a warp takes four blocks of a row at a time (512 numbers, one word of scales), eight
 // lanes a block and sixteen numbers a lane; the block's largest magnitude goes round its eight lanes in three shuffles.
 #include "fp8.cuh"
 
@@ -147,6 +150,141 @@ __global__ void __launch_bounds__(THREADS) read_kernel(RowsArgs g, T* __restrict
     pdl_trigger();
 }
 
+// The pairs sorted by expert, by one block: counts of the experts, their first rows by a scan, every pair's place by a counter in
+// shared memory (which of an expert's pairs comes first is left open: a pair's result hangs on its own row alone).  A choice
+// that is no expert's is in no group.  scale_row: of row s of the order, where its scales lie (row r of tile t of the list:
+// `pad` t + r, pad being the tile's rows rounded up to 128); -1 behind the last row.
+__global__ void __launch_bounds__(1024) group_kernel(const int32_t* __restrict__ ids, int P, int E, int tile_rows, int pad,
+                                                     int32_t* __restrict__ perm, int32_t* __restrict__ scale_row,
+                                                     int32_t* __restrict__ offsets, int32_t* __restrict__ tile_group,
+                                                     int32_t* __restrict__ tile_row0, int max_tiles) {
+    extern __shared__ int sh[];                        // counts (then places) [E], first rows [E + 1], first tiles [E + 1]
+    int *counts = sh, *starts = sh + E, *tiles = starts + E + 1;
+    __shared__ int carry[2][33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int e = threadIdx.x; e < E; e += 1024) counts[e] = 0;
+    __syncthreads();
+    pdl_wait();
+    for (int p = threadIdx.x; p < P; p += 1024) {
+        const int e = ids[p];
+        if (e >= 0 && e < E) atomicAdd(&counts[e], 1);
+    }
+    __syncthreads();
+    int rows_before = 0, tiles_before = 0;
+    for (int e0 = 0; e0 < E; e0 += 1024) {
+        const int e = e0 + threadIdx.x, n = e < E ? counts[e] : 0, t = (n + tile_rows - 1) / tile_rows;
+        int a = n, b = t;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, a, o), y = __shfl_up_sync(0xffffffffu, b, o);
+            if (lane >= o) { a += x; b += y; }
+        }
+        if (lane == 31) { carry[0][warp] = a; carry[1][warp] = b; }
+        __syncthreads();
+        if (warp == 0) {
+            int x = carry[0][lane], y = carry[1][lane];
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, x, o), v = __shfl_up_sync(0xffffffffu, y, o);
+                if (lane >= o) { x += u; y += v; }
+            }
+            carry[0][lane] = x; carry[1][lane] = y;
+        }
+        __syncthreads();
+        if (e < E) {
+            starts[e] = rows_before + a - n + (warp ? carry[0][warp - 1] : 0);
+            tiles[e] = tiles_before + b - t + (warp ? carry[1][warp - 1] : 0);
+            offsets[e] = starts[e];
+        }
+        rows_before += carry[0][31];
+        tiles_before += carry[1][31];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) {
+        starts[E] = offsets[E] = rows_before;
+        tiles[E] = tiles_before;
+    }
+    __syncthreads();
+    for (int t = threadIdx.x; t < max_tiles; t += 1024) {
+        int group = -1, row0 = 0;
+        if (t < tiles_before) {
+            int lo = 0, hi = E;                        // the last expert whose first tile is not behind t and that has one
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) / 2;
+                if (tiles[mid] <= t) lo = mid; else hi = mid;
+            }
+            group = lo;
+            row0 = starts[lo] + (t - tiles[lo]) * tile_rows;
+        }
+        tile_group[t] = group;
+        tile_row0[t] = row0;
+    }
+    for (int e = threadIdx.x; e < E; e += 1024) counts[e] = 0;
+    __syncthreads();
+    for (int p = threadIdx.x; p < P; p += 1024) {
+        const int e = ids[p];
+        if (e >= 0 && e < E) {
+            const int r = atomicAdd(&counts[e], 1), s = starts[e] + r;
+            perm[s] = p;
+            scale_row[s] = (tiles[e] + r / tile_rows) * pad + r % tile_rows;
+        }
+    }
+    for (int s = rows_before + threadIdx.x; s < P; s += 1024) {
+        perm[s] = 0;
+        scale_row[s] = -1;
+    }
+    pdl_trigger();
+}
+
+// Row s of the order: the row perm[s] / top of x (top 0: row s itself) in 8 bits.
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(THREADS) gather_kernel(RowsArgs g, const int32_t* __restrict__ perm, const int32_t* __restrict__ scale_row, int top) {
+    const int lane = threadIdx.x & 31;
+    const long items = g.rows * g.quads;
+    pdl_wait();
+    for (long item = (long)blockIdx.x * WARPS + (threadIdx.x >> 5); item < items; item += (long)gridDim.x * WARPS) {
+        const long s = item / g.quads;
+        const int quad = (int)(item - s * g.quads), c = quad * 512 + lane * 16;
+        const int place = scale_row[s];
+        if (place < 0) continue;
+        const long row = top ? perm[s] / top : s;
+        float v[16];
+        load16<WIDE>((const T*)g.x + row * g.ldx, c, g.cols, v);
+        uint32_t word;
+        const uint4 q = round16(v, word);
+        if (c < g.ldv) *reinterpret_cast<uint4*>(g.values + s * g.ldv + c) = q;
+        if (lane == 0) *reinterpret_cast<uint32_t*>(g.scales + scale_at(place, quad, g.quads)) = word;
+    }
+    pdl_trigger();
+}
+
+// out[t] = sum over t's choices, in their order, of weight * y[choice][t]; those that are no expert's give nothing.
+template <typename T>
+__global__ void __launch_bounds__(THREADS) combine_kernel(const float* __restrict__ y, const int32_t* __restrict__ ids, const float* __restrict__ weights,
+                                                          int top, int experts, int tokens, int cols, T* __restrict__ out, long ldo, int wide) {
+    pdl_wait();
+    const int t = blockIdx.x, c = (blockIdx.y * THREADS + threadIdx.x) * 4;
+    if (c < cols) {
+        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int k = 0; k < top; ++k) {
+            const int e = ids[(long)t * top + k];
+            if (e < 0 || e >= experts) continue;
+            const float w = weights ? weights[(long)t * top + k] : 1.0f;
+            const float* row = y + ((long)k * tokens + t) * cols + c;
+            if (wide) {
+                const float4 v = *reinterpret_cast<const float4*>(row);
+                acc[0] = fmaf(w, v.x, acc[0]); acc[1] = fmaf(w, v.y, acc[1]); acc[2] = fmaf(w, v.z, acc[2]); acc[3] = fmaf(w, v.w, acc[3]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) if (c + i < cols) acc[i] = fmaf(w, row[i], acc[i]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) if (c + i < cols) out[(long)t * ldo + c + i] = from_float<T>(acc[i]);
+    }
+    pdl_trigger();
+}
+
 int grid_for(long items) {
     const long blocks = (items + WARPS - 1) / WARPS, most = 16L * tc::device_sms();
     return (int)(blocks < most ? blocks : most);
@@ -184,4 +322,50 @@ BROLM_API int brolm_fp8_read(int dtype, const void* values, long long ldv, const
     if (dtype == BROLM_BF16) return launch_pdl(read_kernel<bf16>, grid, block, 0, stream, g, (bf16*)y, (long)ldy, base && ldy % 8 == 0);
     if (dtype != BROLM_F32) return BROLM_ERR_BAD_DTYPE;
     return launch_pdl(read_kernel<float>, grid, block, 0, stream, g, (float*)y, (long)ldy, base && ldy % 4 == 0);
+}
+
+// ids [pairs] -> perm, scale_row [pairs], offsets [experts + 1], the list [max_tiles] (expert -1 behind its end).
+BROLM_API int brolm_fp8_group(const void* ids, int pairs, int experts, int tile_rows, void* perm, void* scale_row, void* offsets,
+                              void* tile_group, void* tile_row0, int max_tiles, cudaStream_t stream) {
+    if (pairs <= 0) return BROLM_OK;
+    if (experts <= 0 || experts > 4096) return BROLM_ERR_TOO_LARGE;
+    if (tile_rows < 16 || max_tiles < (pairs + tile_rows - 1) / tile_rows + (experts < pairs ? experts : pairs)) return BROLM_ERR_BAD_SIZE;
+    const size_t smem = (3 * (size_t)experts + 2) * sizeof(int);
+    static OncePerDevice done;
+    const int st = allow_shared_memory(group_kernel, (3 * 4096 + 2) * sizeof(int), done);
+    if (st) return st;
+    return launch_pdl(group_kernel, dim3(1), dim3(1024), smem, stream, (const int32_t*)ids, pairs, experts, tile_rows, (tile_rows + 127) / 128 * 128,
+                      (int32_t*)perm, (int32_t*)scale_row, (int32_t*)offsets, (int32_t*)tile_group, (int32_t*)tile_row0, max_tiles);
+}
+
+// The rows of the order in 8 bits: row perm[s] / top of x, or with top 0 row s of it.
+BROLM_API int brolm_fp8_gather(int dtype, const void* x, long long ldx, const void* perm, const void* scale_row, int top, void* values,
+                               long long ldv, void* scales, int pairs, int cols, cudaStream_t stream) {
+    if (pairs <= 0 || cols <= 0) return BROLM_OK;
+    if (ldv % 16 != 0 || ldv < cols || ((uintptr_t)values & 15) || ((uintptr_t)scales & 15)) return BROLM_ERR_ALIGNMENT;
+    RowsArgs g = {x, (long)ldx, (uint8_t*)values, (long)ldv, (uint8_t*)scales, pairs, cols, fp8::quads_of(cols), 1, 1, 1};
+    const dim3 grid(grid_for((long)pairs * g.quads)), block(THREADS);
+    const int32_t *pm = (const int32_t*)perm, *sr = (const int32_t*)scale_row;
+    const bool base = ((uintptr_t)x & 15) == 0;
+    if (dtype == BROLM_BF16) {
+        if (base && ldx % 8 == 0) return launch_pdl(gather_kernel<bf16, true>, grid, block, 0, stream, g, pm, sr, top);
+        return launch_pdl(gather_kernel<bf16, false>, grid, block, 0, stream, g, pm, sr, top);
+    }
+    if (dtype != BROLM_F32) return BROLM_ERR_BAD_DTYPE;
+    if (base && ldx % 4 == 0) return launch_pdl(gather_kernel<float, true>, grid, block, 0, stream, g, pm, sr, top);
+    return launch_pdl(gather_kernel<float, false>, grid, block, 0, stream, g, pm, sr, top);
+}
+
+// y float [top, tokens, cols]; weights [tokens, top], or null for ones; out float or bfloat16.
+BROLM_API int brolm_fp8_combine(const void* y, const void* ids, const void* weights, int top, int experts, int tokens, int cols, void* out,
+                                long long ldo, int out_f32, cudaStream_t stream) {
+    if (tokens <= 0 || cols <= 0) return BROLM_OK;
+    const dim3 grid(tokens, (cols + 4 * THREADS - 1) / (4 * THREADS)), block(THREADS);
+    if (grid.y > 65535) return BROLM_ERR_TOO_LARGE;
+    const int wide = cols % 4 == 0 && ((uintptr_t)y & 15) == 0;
+    if (out_f32)
+        return launch_pdl(combine_kernel<float>, grid, block, 0, stream, (const float*)y, (const int32_t*)ids, (const float*)weights, top, experts, tokens,
+                          cols, (float*)out, (long)ldo, wide);
+    return launch_pdl(combine_kernel<bf16>, grid, block, 0, stream, (const float*)y, (const int32_t*)ids, (const float*)weights, top, experts, tokens, cols,
+                      (bf16*)out, (long)ldo, wide);
 }

@@ -417,6 +417,38 @@ BROLM_API int brolm_fp8_stream(const void* x, long long ldx, const void* x_scale
     return dispatch<EPI_STORE, false>(mw, mx, g, bt, slices, stream);
 }
 
+// The products of experts: rows [pairs] in the order of their experts, w the experts' matrices of w_rows rows, group_rows apart (a
+// multiple of 128).  The list (expert, first row) of tiles of `rows` (16, 32, 64 or 128) rows and what it stands on come from
+// brolm_fp8_group; x_scales has a tile of 128 rows for every tile of the list.  Y [pairs, N], or with `down` the float
+// [top, tokens, N]; `scale` (or null): a number for every pair that multiplies its sums before the activation.
+BROLM_API int brolm_fp8_experts_stream(const void* x, long long ldx, const void* x_scales, const void* w, long long ldw, const void* w_scales,
+                                       void* y, long long ldy, int out_f32, int pairs, int N, int K, int experts, int group_rows, int epilogue,
+                                       int act, float limit, const void* tile_group, const void* tile_row0, const void* offsets,
+                                       const void* perm, const void* scale, int down, int top, int tokens, int rows, int max_tiles,
+                                       cudaStream_t stream) {
+    if (pairs <= 0 || N <= 0 || experts <= 0) return BROLM_OK;
+    if (K <= 0 || ldx % 16 || ldw % 16 || (((uintptr_t)x | (uintptr_t)w | (uintptr_t)x_scales | (uintptr_t)w_scales) & 15)) return BROLM_ERR_ALIGNMENT;
+    if (epilogue < 0 || epilogue > 1 || act < 0 || act > 2 || (epilogue == EPI_STORE && act > ACT_RELU2)) return BROLM_ERR_BAD_SIZE;
+    if (group_rows % BR || (rows != 16 && rows != 32 && rows != 64 && rows != 128) || (down && !out_f32)) return BROLM_ERR_BAD_SIZE;
+    const int w_rows = epilogue == EPI_GATED ? 2 * N : N;
+    const long long all = (long long)experts * group_rows;
+    if (all > 0x7fffffff || (long long)max_tiles * ((w_rows + BR - 1) / BR) > 0x7fffffff) return BROLM_ERR_TOO_LARGE;
+    StreamArgs g = {};
+    CUtensorMap mw, mx;
+    int st = make_map_u8(&mw, w, all, K, ldw, BR);
+    if (!st) st = make_map_u8(&mx, x, pairs, K, ldx, rows);
+    if (st) return st;
+    g.y = y; g.ldy = (long)ldy; g.N = N; g.out_f32 = out_f32; g.act = act; g.limit = limit;
+    g.nkb = blocks_of(K); g.quads = quads_of(K); g.per = g.nkb;
+    g.row_tiles = (w_rows + BR - 1) / BR; g.items = g.row_tiles * max_tiles;
+    g.w_scales = (const uint8_t*)w_scales; g.x_scales = (const uint8_t*)x_scales;
+    g.tile_group = (const int32_t*)tile_group; g.tile_row0 = (const int32_t*)tile_row0; g.offsets = (const int32_t*)offsets;
+    g.perm = (const int32_t*)perm; g.scale = (const float*)scale;
+    g.down = down; g.top = top; g.tokens = tokens; g.group_rows = group_rows;
+    if (epilogue == EPI_GATED) return dispatch<EPI_GATED, true>(mw, mx, g, rows, 1, stream);
+    return dispatch<EPI_STORE, true>(mw, mx, g, rows, 1, stream);
+}
+
 BROLM_API int brolm_fp8_stream_status(int reset) {
     int v = 0;
     if (cudaMemcpyFromSymbol(&v, g_fp8_stream_error, sizeof(int)) != cudaSuccess) return -1;

@@ -230,6 +230,100 @@ def feedforward_fp8(x, gate_up: Fp8Matrix, down: Fp8Matrix, out: torch.Tensor, a
     _product(h8, down, out, 0, 0.0)
 
 
+# --- routed experts -----------------------------------------------------------
+def experts_fp8_rows(pairs: int, experts: int) -> int:
+    """How many rows a tile of an expert's pairs has."""
+    mean = pairs / max(experts, 1)
+    for rows in (16, 32, 64, 128):
+        if mean <= 0.75 * rows:
+            return rows
+    return 256
+
+
+def experts_fp8_pairs(x: torch.Tensor, ids: torch.Tensor, up: Fp8Matrix, down: Fp8Matrix, out: torch.Tensor, activation: str = "silu",
+                      limit: float = 0.0, scale: Optional[torch.Tensor] = None) -> None:
+    """Every (token, choice) pair through its expert: out float32 [top, tokens, down.rows], a pair's result at [its choice, its
+    token].  ``ids`` int32 [tokens, top]: a number that is no expert's has no result (its place stays as it was).  ``up`` a stack
+    [experts, ...], gated or not, ``down`` the stack of the second matrices; ``scale`` float32 [tokens, top] multiplies a pair's
+    sums before the activation."""
+    what = "experts_fp8"
+    x = _rows(what, x)
+    if len(up.shape) != 3 or len(down.shape) != 3 or down.gated or up.shape[0] != down.shape[0] or up.outputs != down.cols:
+        raise KernelError(f"{what}: stacks of shapes {tuple(up.shape)} and {tuple(down.shape)} do not follow one another")
+    if x.dim() != 2 or x.shape[1] != up.cols:
+        raise KernelError(f"{what}: rows of {up.cols} numbers are wanted, not {tuple(x.shape)}")
+    T = x.shape[0]
+    if ids.dim() != 2 or ids.shape[0] != T or ids.dtype != torch.int32 or not ids.is_contiguous():
+        raise KernelError(f"{what}: ids are a packed int32 [tokens, top]")
+    E, top, dev = up.shape[0], ids.shape[1], x.device
+    if tuple(out.shape) != (top, T, down.rows) or out.dtype != torch.float32 or not out.is_contiguous():
+        raise KernelError(f"{what}: the pairs' results are a packed float32 {(top, T, down.rows)}")
+    if scale is not None and (scale.dtype != torch.float32 or scale.shape != ids.shape or not scale.is_contiguous()):
+        raise KernelError(f"{what}: the pairs' scales are a packed float32 [tokens, top]")
+    for t in (ids, up, down, out, scale):
+        if t is not None and t.device != dev:
+            raise KernelError(f"{what}: tensors on {dev} and {t.device}")
+    act = _act_code(what, up, activation)
+    P, K, inter, N = T * top, x.shape[1], up.outputs, down.rows
+    if not P or not E or not N:
+        return
+    rows = experts_fp8_rows(P, E)
+    pad = _round_up(rows, 128)
+    most = (P + rows - 1) // rows + min(E, P)
+    lists = torch.empty(2 * P + E + 1 + 2 * most, dtype=torch.int32, device=dev)
+    at = lists.data_ptr()
+    perm, place, offsets, group, row0 = at, at + 4 * P, at + 8 * P, at + 8 * P + 4 * (E + 1), at + 8 * P + 4 * (E + 1 + most)
+    stream = _stream()
+    f = _fn("fp8_rows", "brolm_fp8_group", [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p])
+    _check(f(ids.data_ptr(), P, E, rows, perm, place, offsets, group, row0, most, stream), what)
+    gather = _fn("fp8_rows", "brolm_fp8_gather", [c_int, c_void_p, c_longlong, c_void_p, c_void_p, c_int, c_void_p, c_longlong, c_void_p, c_int, c_int, c_void_p])
+    a = _empty((P, K), dev, scale_rows=most * pad)
+    _check(gather(_CODES[x.dtype], x.data_ptr(), x.stride(0), perm, place, top, a.values.data_ptr(), a.values.stride(0), a.scales.data_ptr(), P, K, stream), what)
+    s = scale.data_ptr() if scale is not None else None
+    h8 = _empty((P, inter), dev, scale_rows=most * pad)
+    if rows <= STREAM_ROWS:
+        f = _fn("fp8_stream", "brolm_fp8_experts_stream", [c_void_p, c_longlong, c_void_p, c_void_p, c_longlong, c_void_p, c_void_p, c_longlong, c_int, c_int,
+                                                           c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                                           c_int, c_int, c_int, c_int, c_int, c_void_p])
+
+        def product(m, w, y, ldy, n, k, code, sc, last):
+            _check(f(m.values.data_ptr(), m.values.stride(0), m.scales.data_ptr(), w.values.data_ptr(), w.values.stride(0), w.scales.data_ptr(), y, ldy, 1, P, n, k,
+                     E, w.group_rows, 1 if w.gated else 0, code, float(limit), group, row0, offsets, perm, sc, last, top, T, rows, most, stream), what)
+        h = torch.empty((P, inter), dtype=torch.float32, device=dev)
+        product(a, up, h.data_ptr(), inter, inter, K, act, s, 0)
+        _check(gather(0, h.data_ptr(), inter, perm, place, 0, h8.values.data_ptr(), h8.values.stride(0), h8.scales.data_ptr(), P, inter, stream), what)
+        product(h8, down, out.data_ptr(), N, N, inter, 0, None, 1)
+        return
+    f = _fn("fp8_gemm", "brolm_fp8_experts_gemm", [c_void_p, c_longlong, c_void_p, c_void_p, c_longlong, c_void_p, c_void_p, c_longlong, c_void_p, c_int, c_int,
+                                                   c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                                   c_int, c_int, c_int, c_int, c_void_p])
+
+    def product(m, w, y, ldy, ys, kind, n, k, code, sc, last):
+        _check(f(m.values.data_ptr(), m.values.stride(0), m.scales.data_ptr(), w.values.data_ptr(), w.values.stride(0), w.scales.data_ptr(), y, ldy, ys, kind, P, n,
+                 k, E, w.group_rows, 1 if w.gated else 0, code, float(limit), _PIECE, group, row0, offsets, perm, sc, last, top, T, most, stream), what)
+    product(a, up, h8.values.data_ptr(), h8.values.stride(0), h8.scales.data_ptr(), 2, inter, K, act, s, 0)
+    product(h8, down, out.data_ptr(), N, None, 1, N, inter, 0, None, 1)
+
+
+def experts_fp8(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, up: Fp8Matrix, down: Fp8Matrix, out: torch.Tensor, activation: str = "silu",
+                limit: float = 0.0, scale_input: bool = False) -> None:
+    """out [tokens, down.rows] (float32 or bfloat16) = the sum over a token's choices of ``weights`` times its expert's result, in
+    the order of the choices; a number in ``ids`` that is no expert's adds nothing.  With ``scale_input`` the weight multiplies
+    the sums before the activation and not the result."""
+    what = "experts_fp8"
+    if weights.shape != ids.shape or weights.dtype != torch.float32 or not weights.is_contiguous() or weights.device != x.device:
+        raise KernelError(f"{what}: weights are a packed float32 [tokens, top] beside the tokens")
+    T, top = ids.shape
+    _out_check(what, out, T, down.rows)
+    y = torch.empty((top, T, down.rows), dtype=torch.float32, device=out.device)
+    experts_fp8_pairs(x, ids, up, down, y, activation, limit, weights if scale_input else None)
+    if not T or not down.rows:
+        return
+    f = _fn("fp8_rows", "brolm_fp8_combine", [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_longlong, c_int, c_void_p])
+    _check(f(y.data_ptr(), ids.data_ptr(), None if scale_input else weights.data_ptr(), top, up.shape[0], T, down.rows, out.data_ptr(), out.stride(0),
+             1 if out.dtype == torch.float32 else 0, _stream()), what)
+
+
 def fp8_stream_status(reset: bool = False) -> int:
     """0 if no bounded wait of the products of few rows ever ran out; otherwise its code.  Synchronises."""
     return _status("fp8_stream", reset)

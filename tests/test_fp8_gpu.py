@@ -176,3 +176,75 @@ def test_no_rows_and_no_waits_that_ran_out():
     y = torch.empty(0, 64, device=DEV)
     kernels.linear_fp8(torch.empty(0, 256, device=DEV), w, y)
     assert kernels.fp8_stream_status() == 0 and kernels.fp8_gemm_status() == 0
+
+
+def routed(g, t, top, e, style):
+    z = torch.randn(t, e, generator=g, device=DEV)
+    if style == "skewed":
+        z += 4.0 * torch.randn(e, generator=g, device=DEV)
+    if style == "one":                                       # the same expert for all, several times a token
+        return torch.full((t, top), e - 1, dtype=torch.int32, device=DEV)
+    ids = torch.topk(z, top, dim=1).indices.to(torch.int32).contiguous()
+    if style == "outside":
+        ids[torch.rand(t, top, generator=g, device=DEV) < 0.4] = e + 2
+        ids[t // 2] = -1
+    return ids
+
+
+@pytest.mark.parametrize("t, top, e, width, inter, act, style, scale_input", [
+    (1, 1, 1, 128, 64, "silu", "even", False),
+    (1, 2, 4, 100, 30, "gelu_tanh", "even", False),
+    (8, 4, 32, 256, 128, "silu", "even", False),
+    (9, 3, 8, 300, 130, "relu2", "skewed", True),
+    (40, 2, 3, 640, 200, "clamped_gate", "skewed", False),
+    (33, 4, 5, 256, 256, "none", "one", False),
+    (70, 2, 2, 130, 513, "silu", "even", True),
+    (150, 2, 2, 256, 384, "silu", "outside", False),
+    (300, 2, 3, 500, 130, "relu2", "skewed", True),
+    (333, 3, 2, 384, 640, "gelu_tanh", "one", False),
+    (200, 6, 64, 128, 48, "silu", "skewed", False),
+    (5, 2, 4, 128, 64, "silu", "outside", False)])
+def test_experts(t, top, e, width, inter, act, style, scale_input):
+    g = gen(t + e + width)
+    ids = routed(g, t, top, e, style)
+    weights = torch.rand(t, top, generator=g, device=DEV) + 0.1
+    x = rows_of(g, t, width, torch.bfloat16, 0.5)
+    plain_up = act in ("relu2", "none")
+    up, down = (rows_of(g, e * a, b, torch.bfloat16, 0.3).view(e, a, b) * b ** -0.5 for a, b in ((inter, width), (width, inter)))
+    gate = None if plain_up else rows_of(g, e * inter, width, torch.bfloat16, 0.3).view(e, inter, width) * width ** -0.5
+    xe, ue, de = plain.values(x), plain.values(up), plain.values(down)
+    ge = None if plain_up else plain.values(gate)
+    # per pair: what it is, and how far it may be off (as for the feed-forward)
+    exact, bound = torch.zeros(t, width, dtype=torch.float64, device=DEV), torch.zeros(t, width, dtype=torch.float64, device=DEV)
+    for k in range(e):
+        chose = ids == k
+        tok, ch = chose.nonzero(as_tuple=True)
+        if not len(tok):
+            continue
+        s = weights[tok, ch].double()[:, None]
+        si = s if scale_input else 1.0
+        z, zb = (xe[tok] @ ue[k].T) * si, sum_bound(xe[tok], ue[k]) * si
+        if plain_up:
+            h = plain.act(z, act)
+            off = zb if act == "none" else 2 * z.abs() * zb + zb ** 2 + 2.0 ** -23 * z ** 2
+        else:
+            h, off = gated_bound((xe[tok] @ ge[k].T) * si, z, sum_bound(xe[tok], ge[k]) * si, zb, act, 2.0)
+        h8 = plain.values(h)
+        tight = (plain.values(h + off) != h8) | (plain.values(h - off) != h8)
+        step = 2.0 ** -3 * h.abs() + 2.0 ** -8 * h.abs().amax(dim=1, keepdim=True) / 224.0
+        so = 1.0 if scale_input else s
+        y = (h8 @ de[k].T) * so
+        exact.index_add_(0, tok, y)
+        bound.index_add_(0, tok, (sum_bound(h8, de[k]) + (tight * step) @ de[k].abs().T) * so + 2.0 ** -22 * y.abs())
+    up8 = kernels.fp8_quantize(up) if plain_up else kernels.fp8_gate_up(gate, up)
+    d8 = kernels.fp8_quantize(down)
+    for dtype in (torch.float32, torch.bfloat16):
+        out = torch.full((t, width + 3), 7.0, dtype=dtype, device=DEV)
+        kernels.experts_fp8(x, ids, weights, up8, d8, out[:, :width], act, 2.0, scale_input)
+        near(out[:, :width], exact, rounded(bound, exact, dtype))
+        assert bool((out[:, width:] == 7.0).all())
+    pairs = torch.full((top, t, width), 7.0, dtype=torch.float32, device=DEV)
+    kernels.experts_fp8_pairs(x, ids, up8, d8, pairs, act, 2.0, weights if scale_input else None)
+    none = ((ids < 0) | (ids >= e)).T
+    assert bool((pairs[none] == 7.0).all())
+    assert kernels.fp8_stream_status() == 0 and kernels.fp8_gemm_status() == 0
