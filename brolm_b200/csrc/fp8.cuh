@@ -73,6 +73,25 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                  ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 
+// ---- host: what the launchers take, packed by the host as C lays it out
+struct RowsCall {                // brolm_fp8_quantize, brolm_fp8_read
+    void *x, *values, *scales;
+    cudaStream_t stream;
+    long long ldx, ldv, rows;
+    int dtype, cols, group, group_pad, early;
+};
+struct ProductCall {             // brolm_fp8_stream, brolm_fp8_gemm and, with the second half, their forms for experts
+    const void *x, *x_scales, *w, *w_scales;
+    void *y, *y_scales;
+    cudaStream_t stream;
+    long long ldx, ldw, ldy;
+    int M, N, K, epilogue, act, out, fused, cut;       // cut: slices (stream), blocks of a piece (gemm)
+    float limit;
+    int experts;
+    const void *tile_group, *tile_row0, *offsets, *perm, *scale;
+    int group_rows, down, top, tokens, rows, max_tiles;
+};
+
 // ---- host: rows x cols bytes, row-major with `ld` bytes between rows; box = box_rows x 128 columns, 128-byte swizzle
 static inline int make_map_u8(CUtensorMap* map, const void* ptr, long long rows, long long cols, long long ld, int box_rows) {
     tc::EncodeTiled enc = tc::encoder();

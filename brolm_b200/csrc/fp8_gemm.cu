@@ -47,7 +47,7 @@ struct GemmArgs {
     void* y;
     long ldy;                // elements (OUT_FP8: bytes)
     uint8_t* y_scales;
-    int y_quads;
+    int y_quads, y_wide;
     int M, N;                // rows; output columns
     int act;
     float limit;
@@ -351,7 +351,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                         return;
                     }
                     const int col = nt * OUT_COLS + half * (OUT_COLS / 2) + OC;
-                    if (valid && col < g.N) store_row<W>((bf16*)g.y + at * g.ldy + col, o, col, g.N, (g.ldy & 7) == 0);
+                    if (valid && col < g.N) store_row<W>((bf16*)g.y + at * g.ldy + col, o, col, g.N, g.y_wide);
                 };
                 if (as == 0) in_order<CW, 32 / CW>(take);
                 else in_order<CW, 0>(take);
@@ -371,7 +371,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                     for (int i = 0; i < 128; ++i) sum[i] = act_of(sum[i], g.act);
                 }
                 const int col = nt * OUT_COLS + half * W;
-                if (valid && col < g.N) store_row<W>((float*)g.y + at * g.ldy + col, sum, col, g.N, (g.ldy & 3) == 0);
+                if (valid && col < g.N) store_row<W>((float*)g.y + at * g.ldy + col, sum, col, g.N, g.y_wide);
             }
             if (OUT == OUT_FP8) {
                 constexpr int W = EPI == EPI_GATED ? 64 : 128;
@@ -452,67 +452,40 @@ int dispatch(const Maps& m, const GemmArgs& g, int epilogue, int out, cudaStream
 
 }  // namespace
 
-// Y [M, N] = X W^T (epilogue 0, act 0 or the square of relu) or the gated activation of W's neighbouring rows (epilogue 1: W
-// has 2 N rows).  X and W as brolm_fp8_quantize leaves them.  out 0: bfloat16, 1: float (sums in pieces of `piece` blocks of
-// K), 2: 8 bits (ldy bytes, a multiple of 16, and scales of ceil(N / 512) words).
-BROLM_API int brolm_fp8_gemm(const void* x, long long ldx, const void* x_scales, const void* w, long long ldw, const void* w_scales,
-                             void* y, long long ldy, void* y_scales, int out, int M, int N, int K, int epilogue, int act, float limit,
-                             int piece, cudaStream_t stream) {
+// As brolm_fp8_stream, for any M and, for experts, tiles of 256 rows: x_scales then has two tiles of 128 rows for every tile of the
+// list.  out 1: float, summed in pieces of `cut` blocks of K; 2: 8 bits (ldy bytes between rows, a multiple of 16; for experts
+// scales as x_scales has them).
+BROLM_API int brolm_fp8_gemm(const fp8::ProductCall* c) {
+    const int M = c->M, N = c->N, K = c->K;
     if (M <= 0 || N <= 0) return BROLM_OK;
-    if (K <= 0 || ldx % 16 || ldw % 16 || (((uintptr_t)x | (uintptr_t)w | (uintptr_t)x_scales | (uintptr_t)w_scales) & 15)) return BROLM_ERR_ALIGNMENT;
-    if (((uintptr_t)y & 15) || (out == OUT_FP8 && (ldy % 16 || ldy < N || !y_scales))) return BROLM_ERR_ALIGNMENT;
-    if (epilogue < 0 || epilogue > 1 || out < 0 || out > 2 || act < 0 || act > 2 || (epilogue == EPI_STORE && act > ACT_RELU2)) return BROLM_ERR_BAD_SIZE;
-    const int w_rows = epilogue == EPI_GATED ? 2 * N : N;
+    if (K <= 0 || c->ldx % 16 || c->ldw % 16 || (((uintptr_t)c->x | (uintptr_t)c->w | (uintptr_t)c->x_scales | (uintptr_t)c->w_scales) & 15)) return BROLM_ERR_ALIGNMENT;
+    if (c->out == OUT_FP8 && (c->ldy % 16 || c->ldy < N || !c->y_scales || ((uintptr_t)c->y & 15))) return BROLM_ERR_ALIGNMENT;
+    if (c->epilogue < 0 || c->epilogue > 1 || c->out < 0 || c->out > 2 || c->act < 0 || c->act > 2 || (c->epilogue == EPI_STORE && c->act > ACT_RELU2)) return BROLM_ERR_BAD_SIZE;
+    const long long w_rows = c->epilogue == EPI_GATED ? 2LL * N : N;
+    const long long all = c->experts ? (long long)c->experts * c->group_rows : w_rows;
     Maps m;
     GemmArgs g = {};
     g.quads = quads_of(K);
-    int st = make_map_u8(&m.x, x, M, K, ldx, BM);
-    if (!st) st = make_map_u8(&m.w, w, w_rows, K, ldw, HN);
-    if (!st) st = make_map_scales(&m.xs, x_scales, (long long)((M + 127) / 128) * g.quads);
-    if (!st) st = make_map_scales(&m.ws, w_scales, (long long)((w_rows + 127) / 128) * g.quads);
+    const long long m_tiles = c->experts ? c->max_tiles : ((long long)M + PM - 1) / PM;
+    const int out_cols = c->epilogue == EPI_GATED ? BN / 2 : BN;
+    const long long n_tiles = ((long long)N + out_cols - 1) / out_cols;
+    if (all > 0x7fffffff - BN || m_tiles * n_tiles > 0x7fffffff - 1024) return BROLM_ERR_TOO_LARGE;
+    if (c->experts && (c->group_rows % 128 || (c->down && c->out != OUT_F32))) return BROLM_ERR_BAD_SIZE;
+    int st = make_map_u8(&m.x, c->x, M, K, c->ldx, BM);
+    if (!st) st = make_map_u8(&m.w, c->w, all, K, c->ldw, HN);
+    if (!st) st = make_map_scales(&m.xs, c->x_scales, (c->experts ? 2 * m_tiles : ((long long)M + 127) / 128) * g.quads);
+    if (!st) st = make_map_scales(&m.ws, c->w_scales, (all + 127) / 128 * g.quads);
     if (st) return st;
-    g.y = y; g.ldy = (long)ldy; g.y_scales = (uint8_t*)y_scales; g.y_quads = quads_of(N);
-    g.M = M; g.N = N; g.act = act; g.limit = limit; g.nkb = blocks_of(K);
-    g.piece = out == OUT_F32 && piece > 0 && piece < g.nkb ? piece : g.nkb;
-    g.m_tiles = (M + PM - 1) / PM;
-    const int out_cols = epilogue == EPI_GATED ? BN / 2 : BN;
-    g.n_tiles = (N + out_cols - 1) / out_cols;
-    return dispatch<false>(m, g, epilogue, out, stream);
-}
-
-// The products of experts, as brolm_fp8_experts_stream's but over tiles of 256 rows: x_scales has two tiles of 128 rows for every
-// tile of the list.  out as above; with `down` float [top, tokens, N].
-BROLM_API int brolm_fp8_experts_gemm(const void* x, long long ldx, const void* x_scales, const void* w, long long ldw, const void* w_scales,
-                                     void* y, long long ldy, void* y_scales, int out, int pairs, int N, int K, int experts, int group_rows,
-                                     int epilogue, int act, float limit, int piece, const void* tile_group, const void* tile_row0,
-                                     const void* offsets, const void* perm, const void* scale, int down, int top, int tokens,
-                                     int max_tiles, cudaStream_t stream) {
-    if (pairs <= 0 || N <= 0 || experts <= 0) return BROLM_OK;
-    if (K <= 0 || ldx % 16 || ldw % 16 || (((uintptr_t)x | (uintptr_t)w | (uintptr_t)x_scales | (uintptr_t)w_scales) & 15)) return BROLM_ERR_ALIGNMENT;
-    if (((uintptr_t)y & 15) || (out == OUT_FP8 && (ldy % 16 || ldy < N || !y_scales))) return BROLM_ERR_ALIGNMENT;
-    if (epilogue < 0 || epilogue > 1 || out < 0 || out > 2 || act < 0 || act > 2 || (epilogue == EPI_STORE && act > ACT_RELU2)) return BROLM_ERR_BAD_SIZE;
-    if (group_rows % 128 || (down && out != OUT_F32)) return BROLM_ERR_BAD_SIZE;
-    const int w_rows = epilogue == EPI_GATED ? 2 * N : N;
-    const long long all = (long long)experts * group_rows;
-    Maps m;
-    GemmArgs g = {};
-    g.quads = quads_of(K);
-    const int out_cols = epilogue == EPI_GATED ? BN / 2 : BN;
-    g.n_tiles = (N + out_cols - 1) / out_cols;
-    if (all > 0x7fffffff || (long long)max_tiles * g.n_tiles > 0x7fffffff) return BROLM_ERR_TOO_LARGE;
-    int st = make_map_u8(&m.x, x, pairs, K, ldx, BM);
-    if (!st) st = make_map_u8(&m.w, w, all, K, ldw, HN);
-    if (!st) st = make_map_scales(&m.xs, x_scales, 2LL * max_tiles * g.quads);
-    if (!st) st = make_map_scales(&m.ws, w_scales, all / 128 * g.quads);
-    if (st) return st;
-    g.y = y; g.ldy = (long)ldy; g.y_scales = (uint8_t*)y_scales; g.y_quads = quads_of(N);
-    g.N = N; g.act = act; g.limit = limit; g.nkb = blocks_of(K);
-    g.piece = out == OUT_F32 && piece > 0 && piece < g.nkb ? piece : g.nkb;
-    g.m_tiles = max_tiles;
-    g.tile_group = (const int32_t*)tile_group; g.tile_row0 = (const int32_t*)tile_row0; g.offsets = (const int32_t*)offsets;
-    g.perm = (const int32_t*)perm; g.scale = (const float*)scale;
-    g.down = down; g.top = top; g.tokens = tokens; g.group_rows = group_rows;
-    return dispatch<true>(m, g, epilogue, out, stream);
+    g.y = c->y; g.ldy = (long)c->ldy; g.y_scales = (uint8_t*)c->y_scales; g.y_quads = quads_of(N);
+    g.y_wide = ((uintptr_t)c->y & 15) == 0 && c->ldy % (c->out == OUT_F32 ? 4 : 8) == 0;
+    g.M = M; g.N = N; g.act = c->act; g.limit = c->limit; g.nkb = blocks_of(K);
+    g.piece = c->out == OUT_F32 && c->cut > 0 && c->cut < g.nkb ? c->cut : g.nkb;
+    g.m_tiles = (int)m_tiles; g.n_tiles = (int)n_tiles;
+    if (!c->experts) return dispatch<false>(m, g, c->epilogue, c->out, c->stream);
+    g.tile_group = (const int32_t*)c->tile_group; g.tile_row0 = (const int32_t*)c->tile_row0; g.offsets = (const int32_t*)c->offsets;
+    g.perm = (const int32_t*)c->perm; g.scale = (const float*)c->scale;
+    g.down = c->down; g.top = c->top; g.tokens = c->tokens; g.group_rows = c->group_rows;
+    return dispatch<true>(m, g, c->epilogue, c->out, c->stream);
 }
 
 BROLM_API int brolm_fp8_gemm_status(int reset) {

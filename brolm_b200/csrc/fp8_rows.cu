@@ -8,7 +8,7 @@
 //
 // The first two are one pass over the data: a warp takes four blocks of a row at a time (512 numbers, one word of scales), eight
 // lanes a block and sixteen numbers a lane; the block's largest magnitude goes round its eight lanes in three shuffles.
-#include "fp8.cuh"
+#include "fp8_round.cuh"
 
 namespace {
 
@@ -26,56 +26,6 @@ struct RowsArgs {
     int group, group_pad;
     int early;                      // the next kernel may begin before this one's results are there
 };
-
-// Sixteen numbers of a row from column c on; zeros from `cols` on.
-template <bool WIDE>
-__device__ __forceinline__ void load16(const bf16* row, int c, int cols, float (&v)[16]) {
-    if (WIDE && c + 16 <= cols) {
-        float a[8], b[8];
-        load8(row + c, a);
-        load8(row + c + 8, b);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) { v[i] = a[i]; v[8 + i] = b[i]; }
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = c + i < cols ? __bfloat162float(row[c + i]) : 0.0f;
-}
-template <bool WIDE>
-__device__ __forceinline__ void load16(const float* row, int c, int cols, float (&v)[16]) {
-    if (WIDE && c + 16 <= cols) {
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-            const float4 f = *reinterpret_cast<const float4*>(row + c + i);
-            v[i] = f.x; v[i + 1] = f.y; v[i + 2] = f.z; v[i + 3] = f.w;
-        }
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = c + i < cols ? row[c + i] : 0.0f;
-}
-
-// The warp's 512 numbers to 8 bits: this lane's sixteen, and (in every lane) the word of the four blocks' scales.
-__device__ __forceinline__ uint4 round16(const float (&v)[16], uint32_t& word) {
-    uint32_t most = 0;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) most = max(most, __float_as_uint(v[i]) & 0x7fffffffu);
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-    const uint32_t byte = scale_byte(most);
-    uint4 q = make_uint4(NAN4, NAN4, NAN4, NAN4);
-    if (byte != 255u) {
-        const float inv = scale_inverse(byte);
-        q.x = pack4(v[0], v[1], v[2], v[3], inv);
-        q.y = pack4(v[4], v[5], v[6], v[7], inv);
-        q.z = pack4(v[8], v[9], v[10], v[11], inv);
-        q.w = pack4(v[12], v[13], v[14], v[15], inv);
-    }
-    word = byte << (8 * ((threadIdx.x & 31) >> 3));
-    word |= __shfl_xor_sync(0xffffffffu, word, 8);
-    word |= __shfl_xor_sync(0xffffffffu, word, 16);
-    return q;
-}
 
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(THREADS) quantize_kernel(RowsArgs g) {
@@ -294,78 +244,97 @@ int grid_for(long items) {
 
 // x [rows, cols] (float or bfloat16, ldx elements between rows) -> values (ldv bytes between rows, a multiple of 16, at least
 // cols) and scales.  Rows come in groups of `group`, which lie `group_pad` rows (a multiple of 128 if not `group`) apart.
-BROLM_API int brolm_fp8_quantize(int dtype, const void* x, long long ldx, void* values, long long ldv, void* scales, long long rows,
-                                 int cols, int group, int group_pad, int early, cudaStream_t stream) {
-    if (rows <= 0 || cols <= 0) return BROLM_OK;
-    if (ldv % 16 != 0 || ldv < cols || ((uintptr_t)values & 15) || ((uintptr_t)scales & 15)) return BROLM_ERR_ALIGNMENT;
-    if (group <= 0 || group_pad < group) return BROLM_ERR_BAD_SIZE;
-    RowsArgs g = {x, (long)ldx, (uint8_t*)values, (long)ldv, (uint8_t*)scales, (long)rows, cols, fp8::quads_of(cols), group, group_pad, early};
-    const dim3 grid(grid_for(rows * g.quads)), block(THREADS);
-    if (dtype == BROLM_BF16) {
-        if (((uintptr_t)x & 15) == 0 && ldx % 8 == 0) return launch_pdl(quantize_kernel<bf16, true>, grid, block, 0, stream, g);
-        return launch_pdl(quantize_kernel<bf16, false>, grid, block, 0, stream, g);
+BROLM_API int brolm_fp8_quantize(const fp8::RowsCall* c) {
+    if (c->rows <= 0 || c->cols <= 0) return BROLM_OK;
+    if (c->ldv % 16 != 0 || c->ldv < c->cols || ((uintptr_t)c->values & 15) || ((uintptr_t)c->scales & 15)) return BROLM_ERR_ALIGNMENT;
+    if (c->group <= 0 || c->group_pad < c->group) return BROLM_ERR_BAD_SIZE;
+    RowsArgs g = {c->x, (long)c->ldx, (uint8_t*)c->values, (long)c->ldv, (uint8_t*)c->scales, (long)c->rows, c->cols, fp8::quads_of(c->cols),
+                  c->group, c->group_pad, c->early};
+    const dim3 grid(grid_for(c->rows * g.quads)), block(THREADS);
+    const bool base = ((uintptr_t)c->x & 15) == 0;
+    if (c->dtype == BROLM_BF16) {
+        if (base && c->ldx % 8 == 0) return launch_pdl(quantize_kernel<bf16, true>, grid, block, 0, c->stream, g);
+        return launch_pdl(quantize_kernel<bf16, false>, grid, block, 0, c->stream, g);
     }
-    if (dtype != BROLM_F32) return BROLM_ERR_BAD_DTYPE;
-    if (((uintptr_t)x & 15) == 0 && ldx % 4 == 0) return launch_pdl(quantize_kernel<float, true>, grid, block, 0, stream, g);
-    return launch_pdl(quantize_kernel<float, false>, grid, block, 0, stream, g);
+    if (c->dtype != BROLM_F32) return BROLM_ERR_BAD_DTYPE;
+    if (base && c->ldx % 4 == 0) return launch_pdl(quantize_kernel<float, true>, grid, block, 0, c->stream, g);
+    return launch_pdl(quantize_kernel<float, false>, grid, block, 0, c->stream, g);
 }
 
-BROLM_API int brolm_fp8_read(int dtype, const void* values, long long ldv, const void* scales, void* y, long long ldy, long long rows,
-                             int cols, int group, int group_pad, cudaStream_t stream) {
-    if (rows <= 0 || cols <= 0) return BROLM_OK;
-    if (ldv % 16 != 0 || ldv < cols || ((uintptr_t)values & 15)) return BROLM_ERR_ALIGNMENT;
-    if (group <= 0 || group_pad < group) return BROLM_ERR_BAD_SIZE;
-    RowsArgs g = {nullptr, 0, (uint8_t*)const_cast<void*>(values), (long)ldv, (uint8_t*)const_cast<void*>(scales), (long)rows, cols,
-                  fp8::quads_of(cols), group, group_pad, 1};
-    const dim3 grid(grid_for(rows * g.quads)), block(THREADS);
-    const bool base = ((uintptr_t)y & 15) == 0;
-    if (dtype == BROLM_BF16) return launch_pdl(read_kernel<bf16>, grid, block, 0, stream, g, (bf16*)y, (long)ldy, base && ldy % 8 == 0);
-    if (dtype != BROLM_F32) return BROLM_ERR_BAD_DTYPE;
-    return launch_pdl(read_kernel<float>, grid, block, 0, stream, g, (float*)y, (long)ldy, base && ldy % 4 == 0);
+// The same the other way: x the result.
+BROLM_API int brolm_fp8_read(const fp8::RowsCall* c) {
+    if (c->rows <= 0 || c->cols <= 0) return BROLM_OK;
+    if (c->ldv % 16 != 0 || c->ldv < c->cols || ((uintptr_t)c->values & 15)) return BROLM_ERR_ALIGNMENT;
+    if (c->group <= 0 || c->group_pad < c->group) return BROLM_ERR_BAD_SIZE;
+    RowsArgs g = {nullptr, 0, (uint8_t*)c->values, (long)c->ldv, (uint8_t*)c->scales, (long)c->rows, c->cols, fp8::quads_of(c->cols), c->group, c->group_pad, 1};
+    const dim3 grid(grid_for(c->rows * g.quads)), block(THREADS);
+    const bool base = ((uintptr_t)c->x & 15) == 0;
+    if (c->dtype == BROLM_BF16)
+        return launch_pdl(read_kernel<bf16>, grid, block, 0, c->stream, g, (bf16*)c->x, (long)c->ldx, base && c->ldx % 8 == 0);
+    if (c->dtype != BROLM_F32) return BROLM_ERR_BAD_DTYPE;
+    return launch_pdl(read_kernel<float>, grid, block, 0, c->stream, g, (float*)c->x, (long)c->ldx, base && c->ldx % 4 == 0);
 }
 
 // ids [pairs] -> perm, scale_row [pairs], offsets [experts + 1], the list [max_tiles] (expert -1 behind its end).
-BROLM_API int brolm_fp8_group(const void* ids, int pairs, int experts, int tile_rows, void* perm, void* scale_row, void* offsets,
-                              void* tile_group, void* tile_row0, int max_tiles, cudaStream_t stream) {
-    if (pairs <= 0) return BROLM_OK;
-    if (experts <= 0 || experts > 4096) return BROLM_ERR_TOO_LARGE;
-    if (tile_rows < 16 || max_tiles < (pairs + tile_rows - 1) / tile_rows + (experts < pairs ? experts : pairs)) return BROLM_ERR_BAD_SIZE;
-    const size_t smem = (3 * (size_t)experts + 2) * sizeof(int);
+struct GroupCall {
+    const void* ids;
+    void *perm, *scale_row, *offsets, *tile_group, *tile_row0;
+    cudaStream_t stream;
+    int pairs, experts, tile_rows, max_tiles;
+};
+BROLM_API int brolm_fp8_group(const GroupCall* c) {
+    if (c->pairs <= 0) return BROLM_OK;
+    const int E = c->experts;
+    if (E <= 0 || E > 4096) return BROLM_ERR_TOO_LARGE;
+    if (c->tile_rows < 16 || c->max_tiles < (c->pairs + c->tile_rows - 1) / c->tile_rows + (E < c->pairs ? E : c->pairs)) return BROLM_ERR_BAD_SIZE;
     static OncePerDevice done;
     const int st = allow_shared_memory(group_kernel, (3 * 4096 + 2) * sizeof(int), done);
     if (st) return st;
-    return launch_pdl(group_kernel, dim3(1), dim3(1024), smem, stream, (const int32_t*)ids, pairs, experts, tile_rows, (tile_rows + 127) / 128 * 128,
-                      (int32_t*)perm, (int32_t*)scale_row, (int32_t*)offsets, (int32_t*)tile_group, (int32_t*)tile_row0, max_tiles);
+    return launch_pdl(group_kernel, dim3(1), dim3(1024), (3 * (size_t)E + 2) * sizeof(int), c->stream, (const int32_t*)c->ids, c->pairs, E, c->tile_rows,
+                      (c->tile_rows + 127) / 128 * 128, (int32_t*)c->perm, (int32_t*)c->scale_row, (int32_t*)c->offsets, (int32_t*)c->tile_group,
+                      (int32_t*)c->tile_row0, c->max_tiles);
 }
 
 // The rows of the order in 8 bits: row perm[s] / top of x, or with top 0 row s of it.
-BROLM_API int brolm_fp8_gather(int dtype, const void* x, long long ldx, const void* perm, const void* scale_row, int top, void* values,
-                               long long ldv, void* scales, int pairs, int cols, cudaStream_t stream) {
-    if (pairs <= 0 || cols <= 0) return BROLM_OK;
-    if (ldv % 16 != 0 || ldv < cols || ((uintptr_t)values & 15) || ((uintptr_t)scales & 15)) return BROLM_ERR_ALIGNMENT;
-    RowsArgs g = {x, (long)ldx, (uint8_t*)values, (long)ldv, (uint8_t*)scales, pairs, cols, fp8::quads_of(cols), 1, 1, 1};
-    const dim3 grid(grid_for((long)pairs * g.quads)), block(THREADS);
-    const int32_t *pm = (const int32_t*)perm, *sr = (const int32_t*)scale_row;
-    const bool base = ((uintptr_t)x & 15) == 0;
-    if (dtype == BROLM_BF16) {
-        if (base && ldx % 8 == 0) return launch_pdl(gather_kernel<bf16, true>, grid, block, 0, stream, g, pm, sr, top);
-        return launch_pdl(gather_kernel<bf16, false>, grid, block, 0, stream, g, pm, sr, top);
+struct GatherCall {
+    const void *x, *perm, *scale_row;
+    void *values, *scales;
+    cudaStream_t stream;
+    long long ldx, ldv;
+    int dtype, top, pairs, cols;
+};
+BROLM_API int brolm_fp8_gather(const GatherCall* c) {
+    if (c->pairs <= 0 || c->cols <= 0) return BROLM_OK;
+    if (c->ldv % 16 != 0 || c->ldv < c->cols || ((uintptr_t)c->values & 15) || ((uintptr_t)c->scales & 15)) return BROLM_ERR_ALIGNMENT;
+    RowsArgs g = {c->x, (long)c->ldx, (uint8_t*)c->values, (long)c->ldv, (uint8_t*)c->scales, c->pairs, c->cols, fp8::quads_of(c->cols), 1, 1, 1};
+    const dim3 grid(grid_for((long)c->pairs * g.quads)), block(THREADS);
+    const int32_t *pm = (const int32_t*)c->perm, *sr = (const int32_t*)c->scale_row;
+    const bool base = ((uintptr_t)c->x & 15) == 0;
+    if (c->dtype == BROLM_BF16) {
+        if (base && c->ldx % 8 == 0) return launch_pdl(gather_kernel<bf16, true>, grid, block, 0, c->stream, g, pm, sr, c->top);
+        return launch_pdl(gather_kernel<bf16, false>, grid, block, 0, c->stream, g, pm, sr, c->top);
     }
-    if (dtype != BROLM_F32) return BROLM_ERR_BAD_DTYPE;
-    if (base && ldx % 4 == 0) return launch_pdl(gather_kernel<float, true>, grid, block, 0, stream, g, pm, sr, top);
-    return launch_pdl(gather_kernel<float, false>, grid, block, 0, stream, g, pm, sr, top);
+    if (c->dtype != BROLM_F32) return BROLM_ERR_BAD_DTYPE;
+    if (base && c->ldx % 4 == 0) return launch_pdl(gather_kernel<float, true>, grid, block, 0, c->stream, g, pm, sr, c->top);
+    return launch_pdl(gather_kernel<float, false>, grid, block, 0, c->stream, g, pm, sr, c->top);
 }
 
 // y float [top, tokens, cols]; weights [tokens, top], or null for ones; out float or bfloat16.
-BROLM_API int brolm_fp8_combine(const void* y, const void* ids, const void* weights, int top, int experts, int tokens, int cols, void* out,
-                                long long ldo, int out_f32, cudaStream_t stream) {
-    if (tokens <= 0 || cols <= 0) return BROLM_OK;
-    const dim3 grid(tokens, (cols + 4 * THREADS - 1) / (4 * THREADS)), block(THREADS);
+struct CombineCall {
+    const void *y, *ids, *weights;
+    void* out;
+    cudaStream_t stream;
+    long long ldo;
+    int top, experts, tokens, cols, out_f32;
+};
+BROLM_API int brolm_fp8_combine(const CombineCall* c) {
+    if (c->tokens <= 0 || c->cols <= 0) return BROLM_OK;
+    const dim3 grid(c->tokens, (c->cols + 4 * THREADS - 1) / (4 * THREADS)), block(THREADS);
     if (grid.y > 65535) return BROLM_ERR_TOO_LARGE;
-    const int wide = cols % 4 == 0 && ((uintptr_t)y & 15) == 0;
-    if (out_f32)
-        return launch_pdl(combine_kernel<float>, grid, block, 0, stream, (const float*)y, (const int32_t*)ids, (const float*)weights, top, experts, tokens,
-                          cols, (float*)out, (long)ldo, wide);
-    return launch_pdl(combine_kernel<bf16>, grid, block, 0, stream, (const float*)y, (const int32_t*)ids, (const float*)weights, top, experts, tokens, cols,
-                      (bf16*)out, (long)ldo, wide);
+    const int wide = c->cols % 4 == 0 && ((uintptr_t)c->y & 15) == 0;
+    const float *y = (const float*)c->y, *w = (const float*)c->weights;
+    const int32_t* ids = (const int32_t*)c->ids;
+    if (c->out_f32)
+        return launch_pdl(combine_kernel<float>, grid, block, 0, c->stream, y, ids, w, c->top, c->experts, c->tokens, c->cols, (float*)c->out, (long)c->ldo, wide);
+    return launch_pdl(combine_kernel<bf16>, grid, block, 0, c->stream, y, ids, w, c->top, c->experts, c->tokens, c->cols, (bf16*)c->out, (long)c->ldo, wide);
 }

@@ -20,7 +20,7 @@
 // the gate of output j and row 2 j + 1 its partner: the two lie in neighbouring lanes.
 //
 // Every mbarrier wait is bounded (tcgen05.cuh).
-#include "fp8.cuh"
+#include "fp8_round.cuh"
 
 namespace {
 
@@ -28,9 +28,9 @@ using namespace tc;
 using namespace fp8;
 
 constexpr int BR = 128, BK = 128;
-constexpr int THREADS = 192;
 constexpr int W_BYTES = BR * BK;
 constexpr int MAX_STAGES = 12;
+constexpr int FUSED_BLOCKS = 24;       // 48 KB of the rows, five stages beside them
 
 enum : int { EPI_STORE = 0, EPI_GATED = 1 };
 enum : int { ACT_NONE = 0, ACT_RELU2 = 1 };
@@ -46,6 +46,9 @@ struct StreamArgs {
     int nkb, quads;          // blocks of K, words of scales
     int row_tiles, items, stages;
     int per;                 // blocks of K of a slice (dense; the cluster's rank is the slice)
+    const void* x;           // rows that are no 8-bit numbers yet (FUSED), elements apart
+    long ldx;
+    int x_wide, K;
     const uint8_t* w_scales;
     const uint8_t* x_scales;
     // experts
@@ -93,33 +96,74 @@ __device__ __forceinline__ void put(const StreamArgs& g, long at, float v) {
     else reinterpret_cast<bf16*>(g.y)[at] = __float2bfloat16_rn(v);
 }
 
-template <int BT>
+// The rows of X of this block's slice of K, in 8 bits as the products want them: row r of block kb at r * 128 bytes of its
+// X_BYTES, its sixteen-byte pieces swapped as a TMA load with the 128-byte swizzle would leave them; scales in tiles of four
+// blocks.  A warp takes four blocks of a row at a time and asks for four such pieces before it rounds the first.
+template <typename T, int BT>
+__device__ __forceinline__ void round_rows(const StreamArgs& g, uint8_t* x_blocks, uint8_t* x_scales, int lo, int hi, int w, int lane) {
+    constexpr int DEEP = 4;
+    const int q0 = lo >> 2, n = ((hi + 3) >> 2) - q0, tasks = n * g.M;
+    for (int t0 = w; t0 < tasks; t0 += 8 * DEEP) {
+        float v[DEEP][16];
+#pragma unroll
+        for (int d = 0; d < DEEP; ++d) {
+            const int t = t0 + 8 * d, r = t / n, q = q0 + t - r * n, c = q * 512 + lane * 16;
+            if (t < tasks) {
+                if (g.x_wide) load16<true>((const T*)g.x + r * g.ldx, c, g.K, v[d]);
+                else load16<false>((const T*)g.x + r * g.ldx, c, g.K, v[d]);
+            }
+        }
+#pragma unroll
+        for (int d = 0; d < DEEP; ++d) {
+            const int t = t0 + 8 * d, r = t / n, q = t - r * n, kb = (q0 + q) * 4 + (lane >> 3);
+            if (t < tasks) {                                    // (the same for the whole warp)
+                uint32_t word;
+                const uint4 u = round16(v[d], word);
+                if (kb >= lo && kb < hi)
+                    *reinterpret_cast<uint4*>(x_blocks + (kb - lo) * (BT * BK) + r * BK + (((lane & 7) ^ (r & 7)) << 4)) = u;
+                if (lane == 0) *reinterpret_cast<uint32_t*>(x_scales + q * SF_TILE + r * 16) = word;
+            }
+        }
+    }
+}
+
+// FUSED: 0 the rows are 8-bit numbers in memory; 1, 2: they are bfloat16, float numbers, and every block rounds what it needs.
+template <int BT, int FUSED>
 struct Shape {
+    static constexpr int THREADS = FUSED ? 320 : 192;                   // (eight warps that round, of which four have an epilogue)
     static constexpr int X_BYTES = BT * BK;
-    static constexpr int STAGE_BYTES = W_BYTES + X_BYTES;              // multiples of 1024
-    static constexpr int COLS = 2 * BT + 16;                            // two accumulators, two pairs of scales
-    static constexpr int TMEM_COLS = COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
-    static constexpr int SCALES = 2 * SF_TILE;                          // of a stage
-    static size_t smem(int stages, bool split) {
-        return (size_t)stages * (STAGE_BYTES + SCALES) + (2 * MAX_STAGES + 4) * 8 + 16 + (split ? (size_t)BT * BR * 4 : 0);
+    static constexpr int STAGE_BYTES = FUSED ? W_BYTES : W_BYTES + X_BYTES;      // multiples of 1024
+    // accumulators and two pairs of scales in at most half of tensor memory, so that an SM holds two blocks
+    static constexpr int ACCS = BT == 128 ? 1 : 2;
+    static constexpr int COLS = ACCS * BT + 16;
+    static constexpr int TMEM_COLS = COLS <= 64 ? 64 : COLS <= 128 ? 128 : 256;
+    static constexpr int SCALES = FUSED ? SF_TILE : 2 * SF_TILE;        // of a stage
+    static size_t x_room(int per) { return FUSED ? (size_t)per * X_BYTES + (size_t)((per + 3) / 4 + 1) * SF_TILE : 0; }
+    static size_t smem(int stages, int per) {
+        return x_room(per) + (size_t)stages * (STAGE_BYTES + SCALES) + (2 * MAX_STAGES + 5) * 8 + 16;
     }
 };
 
-template <int BT, int EPI, bool EXPERTS>
-__global__ void __launch_bounds__(THREADS) fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w,
+template <int BT, int EPI, bool EXPERTS, int FUSED>
+__global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS) fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w,
                                                              const __grid_constant__ CUtensorMap map_x, StreamArgs g) {
-    using S = Shape<BT>;
+    using S = Shape<BT, FUSED>;
+    constexpr int ACCS = S::ACCS;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* base = smem_raw;
     const int stages = g.stages;
-    uint8_t* scale_slots = base + stages * S::STAGE_BYTES;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(scale_slots + stages * S::SCALES);
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * MAX_STAGES + 4);
+    // the ring, (FUSED) the slice's rows in 8 bits, the scales of the ring, (FUSED) those of the rows, barriers
+    uint8_t* x_blocks = base + stages * S::STAGE_BYTES;
+    uint8_t* scale_slots = x_blocks + (FUSED ? g.per * S::X_BYTES : 0);
+    uint8_t* x_scales = scale_slots + stages * S::SCALES;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(x_scales + (FUSED ? ((g.per + 3) / 4 + 1) * SF_TILE : 0));
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * MAX_STAGES + 5);
     volatile int* give_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    float* sums = reinterpret_cast<float*>(tmem_slot + 4);             // slices: this one's [rows of X][128]
+    // slices: this one's sums [rows of X][128], in the ring, which is read to its end by then
+    float* sums = reinterpret_cast<float*>(base);
     const uint32_t stage0 = smem_u32(base), scale0 = smem_u32(scale_slots);
     const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * MAX_STAGES, acc_full0 = empty0 + 8 * MAX_STAGES,
-                   acc_empty0 = acc_full0 + 16;
+                   acc_empty0 = acc_full0 + 16, x_ready = acc_empty0 + 16;
     const bool aligned = (stage0 & 1023u) == 0;
     const int slices = EXPERTS ? 1 : (int)cluster_size(), slice = EXPERTS ? 0 : (int)cluster_rank();
     const int first = EXPERTS ? blockIdx.x : blockIdx.x / slices, step = EXPERTS ? gridDim.x : gridDim.x / slices;
@@ -135,6 +179,7 @@ __global__ void __launch_bounds__(THREADS) fp8_stream_kernel(const __grid_consta
             mbar_init(acc_full0 + 8 * s, 1);
             mbar_init(acc_empty0 + 8 * s, 4);
         }
+        mbar_init(x_ready, 8);
         give_up[0] = aligned ? 0 : 1;
         give_up[1] = 0;
         give_up[2] = tc::g_stall_code;
@@ -173,6 +218,7 @@ __global__ void __launch_bounds__(THREADS) fp8_stream_kernel(const __grid_consta
                     bulk_load(scale0 + s * S::SCALES, g.w_scales + ((size_t)(row >> 7) * g.quads + (kb >> 2)) * SF_TILE, SF_TILE, full);
             };
             auto load_x = [&](int s, int row0, int tile, int kb) {
+                if (FUSED) return;
                 const uint32_t full = full0 + 8 * s;
                 tma_load_2d(stage0 + s * S::STAGE_BYTES + W_BYTES, &map_x, kb * BK, row0, full);
                 if ((kb & 3) == 0 || kb == lo)
@@ -224,8 +270,9 @@ __global__ void __launch_bounds__(THREADS) fp8_stream_kernel(const __grid_consta
             int rt, group, row0, tile;
             for (int item = first; item < g.items && lo < hi && ok; item += step, ++local) {
                 if (!find(item, rt, group, row0, tile)) break;
-                const int as = local & 1;
-                ok = wait_on(acc_empty0 + 8 * as, ((local >> 1) & 1) ^ 1, give_up, 5);
+                const int as = local % ACCS;
+                ok = wait_on(acc_empty0 + 8 * as, ((local / ACCS) & 1) ^ 1, give_up, 5);
+                if (FUSED && ok && local == 0) ok = wait_on(x_ready, 0, give_up, 6);
                 if (!ok) break;
                 fence_after_sync();
                 const uint32_t acc = tmem + as * BT;
@@ -235,14 +282,15 @@ __global__ void __launch_bounds__(THREADS) fp8_stream_kernel(const __grid_consta
                     if (!ok) break;
                     fence_after_sync();
                     if ((kb & 3) == 0 || kb == lo) {
-                        sfw = tmem + 2 * BT + 8 * set;
+                        sfw = tmem + ACCS * BT + 8 * set;
                         sfx = sfw + 4;
                         set ^= 1;
                         scales_to_tmem(sfw, desc_scales(scale0 + s * S::SCALES));
-                        scales_to_tmem(sfx, desc_scales(scale0 + s * S::SCALES + SF_TILE));
+                        scales_to_tmem(sfx, desc_scales(FUSED ? smem_u32(x_scales) + ((kb >> 2) - (lo >> 2)) * SF_TILE : scale0 + s * S::SCALES + SF_TILE));
                     }
                     const uint32_t idk = with_block(id, kb & 3, kb & 3);
-                    const uint64_t a = desc_kmajor(stage0 + s * S::STAGE_BYTES), b = desc_kmajor(stage0 + s * S::STAGE_BYTES + W_BYTES);
+                    const uint64_t a = desc_kmajor(stage0 + s * S::STAGE_BYTES);
+                    const uint64_t b = desc_kmajor(FUSED ? smem_u32(x_blocks) + (kb - lo) * S::X_BYTES : stage0 + s * S::STAGE_BYTES + W_BYTES);
 #pragma unroll
                     for (int k = 0; k < BK / 32; ++k) umma_mx(acc, a + 2 * k, b + 2 * k, idk, sfw, sfx, (kb > lo) | (k > 0));
                     umma_commit(empty0 + 8 * s);
@@ -255,11 +303,19 @@ __global__ void __launch_bounds__(THREADS) fp8_stream_kernel(const __grid_consta
         const int quarter = warp & 3;
         const int lrow = quarter * 32 + lane;                   // row of the tile of W = lane of tensor memory
         if (EXPERTS) pdl_wait();
+        if (FUSED) {
+            pdl_wait();
+            if (FUSED == 1) round_rows<bf16, BT>(g, x_blocks, x_scales, lo, hi, warp - 2, lane);
+            else round_rows<float, BT>(g, x_blocks, x_scales, lo, hi, warp - 2, lane);
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(x_ready);
+        }
         int local = 0, rt, group, row0, tile;
-        for (int item = first; item < g.items && lo < hi; item += step, ++local) {
+        for (int item = first; item < g.items && lo < hi && warp < 6; item += step, ++local) {
             if (!find(item, rt, group, row0, tile)) break;
-            const int as = local & 1;
-            const bool ready = !*give_up && wait_on(acc_full0 + 8 * as, (local >> 1) & 1, give_up, 3);
+            const int as = local % ACCS;
+            const bool ready = !*give_up && wait_on(acc_full0 + 8 * as, (local / ACCS) & 1, give_up, 3);
             if (!__all_sync(0xffffffffu, ready)) break;
             fence_after_sync();
             const uint32_t acc = tmem + as * BT + ((uint32_t)(quarter * 32) << 16);
@@ -323,7 +379,7 @@ __global__ void __launch_bounds__(THREADS) fp8_stream_kernel(const __grid_consta
         // one tile a cluster: the slices' sums are added in their order, every block takes some of the rows
         __syncwarp();
         cluster_sync_all();
-        if (warp >= 2 && !*give_up) {
+        if (warp >= 2 && warp < 6 && !*give_up) {
             const uint32_t mine = smem_u32(sums);
             const int t = threadIdx.x - 64, rt = first;
             for (int r = slice; r < g.M; r += slices) {
@@ -347,26 +403,26 @@ __global__ void __launch_bounds__(THREADS) fp8_stream_kernel(const __grid_consta
     if (warp == 1) tmem_dealloc(tmem, S::TMEM_COLS);
 }
 
-template <int BT, int EPI, bool EXPERTS>
+template <int BT, int EPI, bool EXPERTS, int FUSED>
 int launch(const CUtensorMap& mw, const CUtensorMap& mx, StreamArgs g, int slices, cudaStream_t stream) {
-    using S = Shape<BT>;
+    using S = Shape<BT, FUSED>;
     const int sms = device_sms();
     const bool split = slices > 1;
-    // two blocks an SM where there are more items than SMs (and tensor memory holds both)
-    const int per_sm = S::TMEM_COLS <= 256 && g.items * slices > sms ? 2 : 1;
-    const size_t room = per_sm == 2 ? 112 * 1024 : 220 * 1024;
+    // Two blocks an SM: one streams while the other starts or ends, and clusters of up to eight find room.
+    constexpr size_t ROOM = 112 * 1024;
     int stages = MAX_STAGES;
-    while (stages > 2 && S::smem(stages, split) > room) --stages;
+    while (stages > 2 && S::smem(stages, g.per) > ROOM) --stages;
+    const size_t smem = S::smem(stages, g.per);
+    if (smem > ROOM || (split && (size_t)stages * S::STAGE_BYTES < (size_t)BT * BR * 4)) return BROLM_ERR_TOO_LARGE;
     g.stages = stages;
-    const size_t smem = S::smem(stages, split);
     static OncePerDevice done;
-    const int st = allow_shared_memory(fp8_stream_kernel<BT, EPI, EXPERTS>, 225 * 1024, done);
+    const int st = allow_shared_memory(fp8_stream_kernel<BT, EPI, EXPERTS, FUSED>, ROOM, done);
     if (st) return st;
-    const int places = per_sm * sms;
+    const int places = 2 * sms;
     const int grid = split ? g.items * slices : g.items < places ? g.items : places;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(THREADS);
+    cfg.blockDim = dim3(S::THREADS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
@@ -377,76 +433,79 @@ int launch(const CUtensorMap& mw, const CUtensorMap& mx, StreamArgs g, int slice
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = EXPERTS ? 1 : 2;
-    return (int)cudaLaunchKernelEx(&cfg, fp8_stream_kernel<BT, EPI, EXPERTS>, mw, mx, g);
+    return (int)cudaLaunchKernelEx(&cfg, fp8_stream_kernel<BT, EPI, EXPERTS, FUSED>, mw, mx, g);
 }
 
 template <int EPI, bool EXPERTS>
-int dispatch(const CUtensorMap& mw, const CUtensorMap& mx, const StreamArgs& g, int bt, int slices, cudaStream_t stream) {
-    if (bt == 16) return launch<16, EPI, EXPERTS>(mw, mx, g, slices, stream);
-    if (bt == 32) return launch<32, EPI, EXPERTS>(mw, mx, g, slices, stream);
-    if (bt == 64) return launch<64, EPI, EXPERTS>(mw, mx, g, slices, stream);
-    return launch<128, EPI, EXPERTS>(mw, mx, g, slices, stream);
+int dispatch(const CUtensorMap& mw, const CUtensorMap& mx, const StreamArgs& g, int bt, int slices, int fused, cudaStream_t stream) {
+    if constexpr (!EXPERTS) {
+        if (fused == 1) return launch<16, EPI, false, 1>(mw, mx, g, slices, stream);
+        if (fused == 2) return launch<16, EPI, false, 2>(mw, mx, g, slices, stream);
+    }
+    if (bt == 16) return launch<16, EPI, EXPERTS, 0>(mw, mx, g, slices, stream);
+    if (bt == 32) return launch<32, EPI, EXPERTS, 0>(mw, mx, g, slices, stream);
+    if (bt == 64) return launch<64, EPI, EXPERTS, 0>(mw, mx, g, slices, stream);
+    return launch<128, EPI, EXPERTS, 0>(mw, mx, g, slices, stream);
 }
 
 }  // namespace
 
-// Y [M, N] = X W^T (epilogue 0) or the gated activation of W's neighbouring rows (epilogue 1: W has 2 N rows).  X and W as
-// brolm_fp8_quantize leaves them; K is cut into `slices` (1 to 8), none of which is empty.  M <= 128.
-BROLM_API int brolm_fp8_stream(const void* x, long long ldx, const void* x_scales, const void* w, long long ldw, const void* w_scales,
-                               void* y, long long ldy, int out_f32, int M, int N, int K, int epilogue, int act, float limit, int slices,
-                               cudaStream_t stream) {
+// Y [M, N] = X W^T (epilogue 0, act 0 or the square of relu) or the gated activation of W's neighbouring rows (epilogue 1: W
+// has 2 N rows); out 0: bfloat16, 1: float.  X and W as brolm_fp8_quantize leaves them.
+// Dense (experts 0): M <= 128; K is cut into `cut` slices (1 to 8), none of which is empty.  fused 1, 2: X are bfloat16, float
+// numbers (ldx elements between rows, x_scales unused), M <= 16, and a slice has at most FUSED_BLOCKS blocks of 128 of K.
+// Experts: M pairs' rows in the order of their experts, W the experts' matrices, group_rows (a multiple of 128) rows each.  The
+// list (expert, first row) of tiles of `rows` (16, 32, 64 or 128) rows and what it stands on come from brolm_fp8_group; x_scales
+// has a tile of 128 rows for every tile of the list.  Y [M, N], or with `down` float [top, tokens, N]; `scale` (or null): a
+// number for every pair that multiplies its sums before the activation.
+BROLM_API int brolm_fp8_stream(const fp8::ProductCall* c) {
+    const int M = c->M, N = c->N, K = c->K;
     if (M <= 0 || N <= 0) return BROLM_OK;
-    if (M > 128) return BROLM_ERR_TOO_LARGE;
-    if (K <= 0 || ldx % 16 || ldw % 16 || (((uintptr_t)x | (uintptr_t)w | (uintptr_t)x_scales | (uintptr_t)w_scales) & 15)) return BROLM_ERR_ALIGNMENT;
-    if (epilogue < 0 || epilogue > 1 || act < 0 || act > 2 || (epilogue == EPI_STORE && act > ACT_RELU2)) return BROLM_ERR_BAD_SIZE;
-    const int nkb = blocks_of(K), w_rows = epilogue == EPI_GATED ? 2 * N : N;
-    if (slices < 1 || slices > 8 || slices > nkb) return BROLM_ERR_BAD_SIZE;
+    if (K <= 0 || c->ldw % 16 || (((uintptr_t)c->w | (uintptr_t)c->w_scales) & 15)) return BROLM_ERR_ALIGNMENT;
+    if (!c->fused && (c->ldx % 16 || (((uintptr_t)c->x | (uintptr_t)c->x_scales) & 15))) return BROLM_ERR_ALIGNMENT;
+    if (c->fused < 0 || c->fused > 2 || (c->fused && (M > 16 || c->experts))) return BROLM_ERR_BAD_SIZE;
+    if (c->epilogue < 0 || c->epilogue > 1 || c->act < 0 || c->act > 2 || (c->epilogue == EPI_STORE && c->act > ACT_RELU2)) return BROLM_ERR_BAD_SIZE;
+    if (c->out < 0 || c->out > 1) return BROLM_ERR_BAD_SIZE;
+    const long long w_rows = c->epilogue == EPI_GATED ? 2LL * N : N;
     StreamArgs g = {};
-    g.per = (nkb + slices - 1) / slices;
-    if ((slices - 1) * g.per >= nkb) return BROLM_ERR_BAD_SIZE;
+    g.y = c->y; g.ldy = (long)c->ldy; g.M = M; g.N = N; g.out_f32 = c->out; g.act = c->act; g.limit = c->limit;
+    g.nkb = blocks_of(K); g.quads = quads_of(K);
+    g.w_scales = (const uint8_t*)c->w_scales; g.x_scales = (const uint8_t*)c->x_scales;
+    const long long row_tiles = (w_rows + BR - 1) / BR;
+    CUtensorMap mw, mx;
+    if (c->experts) {
+        const int rows = c->rows;
+        if (c->group_rows % BR || (rows != 16 && rows != 32 && rows != 64 && rows != 128) || (c->down && !c->out)) return BROLM_ERR_BAD_SIZE;
+        const long long all = (long long)c->experts * c->group_rows;
+        if (all > 0x7fffffff || c->max_tiles * row_tiles > 0x7fffffff) return BROLM_ERR_TOO_LARGE;
+        int st = make_map_u8(&mw, c->w, all, K, c->ldw, BR);
+        if (!st) st = make_map_u8(&mx, c->x, M, K, c->ldx, rows);
+        if (st) return st;
+        g.per = g.nkb; g.row_tiles = (int)row_tiles; g.items = (int)(row_tiles * c->max_tiles);
+        g.tile_group = (const int32_t*)c->tile_group; g.tile_row0 = (const int32_t*)c->tile_row0; g.offsets = (const int32_t*)c->offsets;
+        g.perm = (const int32_t*)c->perm; g.scale = (const float*)c->scale;
+        g.down = c->down; g.top = c->top; g.tokens = c->tokens; g.group_rows = c->group_rows;
+        if (c->epilogue == EPI_GATED) return dispatch<EPI_GATED, true>(mw, mx, g, rows, 1, 0, c->stream);
+        return dispatch<EPI_STORE, true>(mw, mx, g, rows, 1, 0, c->stream);
+    }
+    const int slices = c->cut;
+    if (M > 128 || w_rows > 0x7fffffff - BR) return BROLM_ERR_TOO_LARGE;
+    if (slices < 1 || slices > 8 || slices > g.nkb) return BROLM_ERR_BAD_SIZE;
+    g.per = (g.nkb + slices - 1) / slices;
+    if ((slices - 1) * g.per >= g.nkb) return BROLM_ERR_BAD_SIZE;
     const int bt = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
-    CUtensorMap mw, mx;
-    int st = make_map_u8(&mw, w, w_rows, K, ldw, BR);
-    if (!st) st = make_map_u8(&mx, x, M, K, ldx, bt);
+    int st = make_map_u8(&mw, c->w, w_rows, K, c->ldw, BR);
+    if (!st && !c->fused) st = make_map_u8(&mx, c->x, M, K, c->ldx, bt);
     if (st) return st;
-    g.y = y; g.ldy = (long)ldy; g.M = M; g.N = N; g.out_f32 = out_f32; g.act = act; g.limit = limit;
-    g.nkb = nkb; g.quads = quads_of(K);
-    g.row_tiles = (w_rows + BR - 1) / BR; g.items = g.row_tiles;
-    g.w_scales = (const uint8_t*)w_scales; g.x_scales = (const uint8_t*)x_scales;
-    if (epilogue == EPI_GATED) return dispatch<EPI_GATED, false>(mw, mx, g, bt, slices, stream);
-    return dispatch<EPI_STORE, false>(mw, mx, g, bt, slices, stream);
-}
-
-// The products of experts: rows [pairs] in the order of their experts, w the experts' matrices of w_rows rows, group_rows apart (a
-// multiple of 128).  The list (expert, first row) of tiles of `rows` (16, 32, 64 or 128) rows and what it stands on come from
-// brolm_fp8_group; x_scales has a tile of 128 rows for every tile of the list.  Y [pairs, N], or with `down` the float
-// [top, tokens, N]; `scale` (or null): a number for every pair that multiplies its sums before the activation.
-BROLM_API int brolm_fp8_experts_stream(const void* x, long long ldx, const void* x_scales, const void* w, long long ldw, const void* w_scales,
-                                       void* y, long long ldy, int out_f32, int pairs, int N, int K, int experts, int group_rows, int epilogue,
-                                       int act, float limit, const void* tile_group, const void* tile_row0, const void* offsets,
-                                       const void* perm, const void* scale, int down, int top, int tokens, int rows, int max_tiles,
-                                       cudaStream_t stream) {
-    if (pairs <= 0 || N <= 0 || experts <= 0) return BROLM_OK;
-    if (K <= 0 || ldx % 16 || ldw % 16 || (((uintptr_t)x | (uintptr_t)w | (uintptr_t)x_scales | (uintptr_t)w_scales) & 15)) return BROLM_ERR_ALIGNMENT;
-    if (epilogue < 0 || epilogue > 1 || act < 0 || act > 2 || (epilogue == EPI_STORE && act > ACT_RELU2)) return BROLM_ERR_BAD_SIZE;
-    if (group_rows % BR || (rows != 16 && rows != 32 && rows != 64 && rows != 128) || (down && !out_f32)) return BROLM_ERR_BAD_SIZE;
-    const int w_rows = epilogue == EPI_GATED ? 2 * N : N;
-    const long long all = (long long)experts * group_rows;
-    if (all > 0x7fffffff || (long long)max_tiles * ((w_rows + BR - 1) / BR) > 0x7fffffff) return BROLM_ERR_TOO_LARGE;
-    StreamArgs g = {};
-    CUtensorMap mw, mx;
-    int st = make_map_u8(&mw, w, all, K, ldw, BR);
-    if (!st) st = make_map_u8(&mx, x, pairs, K, ldx, rows);
-    if (st) return st;
-    g.y = y; g.ldy = (long)ldy; g.N = N; g.out_f32 = out_f32; g.act = act; g.limit = limit;
-    g.nkb = blocks_of(K); g.quads = quads_of(K); g.per = g.nkb;
-    g.row_tiles = (w_rows + BR - 1) / BR; g.items = g.row_tiles * max_tiles;
-    g.w_scales = (const uint8_t*)w_scales; g.x_scales = (const uint8_t*)x_scales;
-    g.tile_group = (const int32_t*)tile_group; g.tile_row0 = (const int32_t*)tile_row0; g.offsets = (const int32_t*)offsets;
-    g.perm = (const int32_t*)perm; g.scale = (const float*)scale;
-    g.down = down; g.top = top; g.tokens = tokens; g.group_rows = group_rows;
-    if (epilogue == EPI_GATED) return dispatch<EPI_GATED, true>(mw, mx, g, rows, 1, stream);
-    return dispatch<EPI_STORE, true>(mw, mx, g, rows, 1, stream);
+    if (c->fused) {
+        if (g.per > FUSED_BLOCKS) return BROLM_ERR_TOO_LARGE;
+        g.x = c->x; g.ldx = (long)c->ldx; g.K = K;
+        g.x_wide = ((uintptr_t)c->x & 15) == 0 && c->ldx % (c->fused == 1 ? 8 : 4) == 0;
+        mx = mw;
+    }
+    g.row_tiles = g.items = (int)row_tiles;
+    if (c->epilogue == EPI_GATED) return dispatch<EPI_GATED, false>(mw, mx, g, bt, slices, c->fused, c->stream);
+    return dispatch<EPI_STORE, false>(mw, mx, g, bt, slices, c->fused, c->stream);
 }
 
 BROLM_API int brolm_fp8_stream_status(int reset) {

@@ -3,115 +3,136 @@ feed-forward, routed experts.
 
 A number is e4m3 (a sign, four bits of exponent, three of mantissa; largest 448) times a power of two that 128 consecutive
 numbers of a row share: the least from 2^-127 on under which none of them is beyond 448 times it.  Rounding is to nearest, ties
-to even.  A block with a number that is not finite is NaN as a whole, and so is what is computed from it.  Both sides of a
-product are such rows; products are exact, sums are float32.
+to even (numbers beyond 240 * 2^120 may become 2^128, which a float32 reads as infinity).  A block with a number that is not
+finite is NaN as a whole, and so is what is computed from it.  Both sides of a product are such rows; products are exact, sums
+are float32.
 
 ``Fp8Matrix`` holds rows in the order the kernels want them: ``fp8_quantize`` makes one from rows or a matrix, or from a stack
 of experts' matrices; ``fp8_gate_up`` from the two matrices of a gated feed-forward, whose rows then alternate.  A matrix in
 use as a weight may be read before what runs ahead of the product in its stream has ended, except for ``fp8_quantize`` itself;
 it is made once and kept.
 
-The functions launch on the current stream, like all of this package, and wait for nothing.
+The functions launch on the current stream, like all of this package; they wait for nothing and keep nothing.
 """
 from __future__ import annotations
 
-import dataclasses
-from ctypes import c_float, c_int, c_longlong, c_void_p
+import functools
+import struct
+from ctypes import c_char_p, c_int
 from typing import Optional
 
 import torch
 
-from . import ACTIVATIONS, EXPERT_ACTS, KernelError, _check, _fn, _ptr, _stream, device_sms, library_loaded, load_library
+from . import ACTIVATIONS, EXPERT_ACTS, KernelError, _check, _fn, device_sms, library_loaded, load_library
 
 BLOCK = 128              # numbers that share a scale
 _TILE = 512              # bytes of scales of 128 rows and four blocks
-_CODES = {torch.float32: 0, torch.bfloat16: 1}
-_PIECE = 16              # blocks of K that a float32 result is summed over before the sum goes to registers
+_BF16, _F32 = torch.bfloat16, torch.float32
+_CODES = {_F32: 0, _BF16: 1}
+_OUT = {_BF16: 0, _F32: 1}
+_FUSED = {_BF16: 1, _F32: 2}
+_NO_CPU = "brolm_b200 kernels run on CUDA tensors only; there is no CPU path"
+_raw_stream, _device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+
+# A product of few rows is a few microseconds on the device, so what the host does for it counts: the launchers take one
+# struct, packed here as C lays it out, and the checks of a call's arguments are one expression; which of them failed is found
+# out only then.
+_ROWS = struct.Struct("@4P3q5i")
+_PRODUCT = struct.Struct("@7P3q8ifi5P6i")
+_GROUP = struct.Struct("@6PP4i")
+_GATHER = struct.Struct("@6P2q4i")
+_COMBINE = struct.Struct("@5Pq5i")
+_functions: dict = {}
 
 
-@dataclasses.dataclass
+def _call(lib: str, name: str, packed: bytes, what: str) -> None:
+    f = _functions.get(name)
+    if f is None:
+        f = _functions[name] = _fn(lib, name, [c_char_p])
+    _check(f(packed), what)
+
+
 class Fp8Matrix:
     """Rows of 8-bit numbers.  ``shape``: (rows, columns) or (experts, rows, columns).  ``gated``: the rows of a gate and of its
-    partner alternate, so that a product has half as many results as there are rows."""
-    values: torch.Tensor         # uint8 [rows of all experts, columns rounded up to 16]
-    scales: torch.Tensor         # uint8 [rows / 128, columns / 512, 512]
-    shape: tuple
-    gated: bool = False
+    partner alternate, so that a product has half as many results as there are rows.  ``values``: uint8 [rows of all experts,
+    columns rounded up to 16], an expert's matrix beginning on a multiple of 128 rows; ``scales``: uint8 [rows / 128, columns /
+    512, 512].  It is not to be changed once it is in use."""
+    __slots__ = ("values", "scales", "shape", "gated", "rows", "cols", "outputs", "group_rows", "device", "index", "packed")
 
-    @property
-    def rows(self) -> int:
-        return self.shape[-2]
-
-    @property
-    def cols(self) -> int:
-        return self.shape[-1]
-
-    @property
-    def outputs(self) -> int:
-        """How many results a row's product with this matrix has."""
-        return self.shape[-2] // 2 if self.gated else self.shape[-2]
-
-    @property
-    def group_rows(self) -> int:
-        """Rows that an expert's matrix takes."""
-        return self.values.shape[0] // self.shape[0] if len(self.shape) == 3 else self.shape[0]
-
-    @property
-    def device(self) -> torch.device:
-        return self.values.device
+    def __init__(self, values: torch.Tensor, scales: torch.Tensor, shape: tuple, gated: bool = False):
+        self.values, self.scales, self.shape, self.gated = values, scales, tuple(shape), bool(gated)
+        self.rows, self.cols = self.shape[-2], self.shape[-1]
+        # how many results a row's product with this matrix has
+        self.outputs = self.rows // 2 if self.gated else self.rows
+        # rows that an expert's matrix takes
+        self.group_rows = values.shape[0] // max(self.shape[0], 1) if len(self.shape) == 3 else self.rows
+        self.device = values.device
+        self.index = values.get_device()
+        self.packed = (values.data_ptr(), scales.data_ptr(), values.stride(0))
 
     @property
     def nbytes(self) -> int:
         return self.values.numel() + self.scales.numel()
+
+    def __repr__(self) -> str:
+        return f"Fp8Matrix({self.shape}, gated={self.gated}, {self.device})"
 
 
 def _round_up(n: int, m: int) -> int:
     return (n + m - 1) // m * m
 
 
-def _empty(shape: tuple, device, gated: bool = False, scale_rows: Optional[int] = None) -> Fp8Matrix:
+def _empty(shape: tuple, device, gated: bool = False) -> Fp8Matrix:
     rows, cols = shape[-2:]
-    # an expert's matrix begins with a tile of scales
     total = rows if len(shape) == 2 else shape[0] * _round_up(rows, 128)
     values = torch.empty((total, _round_up(cols, 16)), dtype=torch.uint8, device=device)
-    scales = torch.empty((((scale_rows or total) + 127) // 128, (cols + 511) // 512, _TILE), dtype=torch.uint8, device=device)
+    scales = torch.empty(((total + 127) // 128, (cols + 511) // 512, _TILE), dtype=torch.uint8, device=device)
     return Fp8Matrix(values, scales, tuple(shape), gated)
 
 
-def _rows(what: str, x: torch.Tensor) -> torch.Tensor:
-    if x.dtype not in _CODES:
-        raise KernelError(f"{what}: element type {x.dtype} is not float32 or bfloat16")
-    if not x.is_cuda:
-        raise KernelError("brolm_b200 kernels run on CUDA tensors only; there is no CPU path")
-    if x.device.index != torch.cuda.current_device():
-        raise KernelError(f"{what}: a tensor lives on {x.device}, the current device is cuda:{torch.cuda.current_device()}")
-    if x.stride(-1) != 1 and x.shape[-1] > 1:
-        raise KernelError(f"{what}: rows must be packed (strides {tuple(x.stride())})")
-    return x
+def _scratch(rows: int, cols: int, device, scale_rows: Optional[int] = None) -> tuple:
+    """Room for rows in 8 bits within one call: what keeps it alive, and values, scales and stride as a launcher takes them."""
+    ld = (cols + 15) & -16
+    begin = (rows * ld + 511) & -512
+    held = torch.empty(begin + (((scale_rows or rows) + 127) >> 7) * ((cols + 511) >> 9) * _TILE, dtype=torch.uint8, device=device)
+    at = held.data_ptr()
+    return held, (at, at + begin, ld)
 
 
-_Q_ARGS = [c_int, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_longlong, c_int, c_int, c_int, c_int, c_void_p]
+def _refuse(what: str, t: torch.Tensor, name: str, dim: int = 2) -> None:
+    """Names what is wrong with a tensor of rows; returns if nothing is."""
+    if t.dtype not in _CODES:
+        raise KernelError(f"{what}: {name} has the element type {t.dtype}, not float32 or bfloat16")
+    if not t.is_cuda:
+        raise KernelError(_NO_CPU)
+    if t.get_device() != _device():
+        raise KernelError(f"{what}: {name} lives on {t.device}, the current device is cuda:{_device()}")
+    if t.dim() != dim:
+        raise KernelError(f"{what}: {name} has {t.dim()} dimensions, not {dim}")
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        raise KernelError(f"{what}: the rows of {name} must be packed (strides {tuple(t.stride())})")
 
 
-def _quantize(x: torch.Tensor, m: Fp8Matrix, early: int) -> None:
-    rows = x.shape[0]
-    group = m.shape[-2] if len(m.shape) == 3 else max(rows, 1)
-    f = _fn("fp8_rows", "brolm_fp8_quantize", _Q_ARGS)
-    _check(f(_CODES[x.dtype], x.data_ptr(), x.stride(0), m.values.data_ptr(), m.values.stride(0), m.scales.data_ptr(), rows, x.shape[1],
-             group, m.group_rows if len(m.shape) == 3 else group, early, _stream()), "fp8_quantize")
+def _quantize(x: torch.Tensor, packed: tuple, group: int, pad: int, early: int) -> None:
+    rows, cols = x.shape
+    _call("fp8_rows", "brolm_fp8_quantize", _ROWS.pack(x.data_ptr(), packed[0], packed[1], _raw_stream(_device()), x.stride(0), packed[2], rows,
+                                                       _CODES[x.dtype], cols, group, pad, early), "fp8_quantize")
 
 
 def fp8_quantize(x: torch.Tensor) -> Fp8Matrix:
     """x [rows, columns] or [experts, rows, columns], float32 or bfloat16, packed rows (any stride between them; a stack of
     experts contiguous) -> the same in 8 bits."""
-    x = _rows("fp8_quantize", x)
-    if x.dim() not in (2, 3) or x.shape[-1] == 0:
-        raise KernelError(f"fp8_quantize: rows or a stack of matrices, not a tensor of shape {tuple(x.shape)}")
+    if not isinstance(x, torch.Tensor) or x.dim() not in (2, 3) or x.shape[-1] == 0:
+        raise KernelError(f"fp8_quantize: rows or a stack of matrices are wanted, not {tuple(getattr(x, 'shape', ()))}")
+    _refuse("fp8_quantize", x, "x", x.dim())
     if x.dim() == 3 and not x.is_contiguous():
         raise KernelError("fp8_quantize: a stack of matrices must be contiguous")
     m = _empty(tuple(x.shape), x.device)
     if x.numel():
-        _quantize(x.view(-1, x.shape[-1]) if x.dim() == 3 else x, m, 0)
+        if x.dim() == 3:
+            _quantize(x.view(-1, x.shape[-1]), m.packed, m.rows, m.group_rows, 0)
+        else:
+            _quantize(x, m.packed, m.rows, m.rows, 0)
     return m
 
 
@@ -120,114 +141,138 @@ def fp8_gate_up(gate: torch.Tensor, up: torch.Tensor) -> Fp8Matrix:
     if gate.shape != up.shape or gate.dtype != up.dtype or gate.device != up.device:
         raise KernelError(f"fp8_gate_up: two matrices of a kind are wanted, not {tuple(gate.shape)} {gate.dtype} and {tuple(up.shape)} {up.dtype}")
     m = fp8_quantize(torch.stack((gate, up), dim=-2).flatten(-3, -2))
-    m.gated = True
-    return m
+    return Fp8Matrix(m.values, m.scales, m.shape, True)
 
 
 def fp8_read(m: Fp8Matrix, out: torch.Tensor) -> None:
     """out (the matrix's shape, float32 or bfloat16, packed rows; a stack contiguous) = the values that ``m`` stands for."""
-    out = _rows("fp8_read", out)
-    if tuple(out.shape) != tuple(m.shape) or (out.dim() == 3 and not out.is_contiguous()):
-        raise KernelError(f"fp8_read: a matrix of shape {tuple(m.shape)} goes into such a tensor, not into {tuple(out.shape)}")
+    _refuse("fp8_read", out, "out", len(m.shape))
+    if tuple(out.shape) != m.shape or (out.dim() == 3 and not out.is_contiguous()):
+        raise KernelError(f"fp8_read: a matrix of shape {m.shape} goes into such a (packed) tensor, not into {tuple(out.shape)}")
     if m.device != out.device:
         raise KernelError("fp8_read: the matrix and the result live on two devices")
     if not out.numel():
         return
     y = out.view(-1, out.shape[-1]) if out.dim() == 3 else out
-    group = m.shape[-2] if len(m.shape) == 3 else y.shape[0]
-    f = _fn("fp8_rows", "brolm_fp8_read", [c_int, c_void_p, c_longlong, c_void_p, c_void_p, c_longlong, c_longlong, c_int, c_int, c_int, c_void_p])
-    _check(f(_CODES[y.dtype], m.values.data_ptr(), m.values.stride(0), m.scales.data_ptr(), y.data_ptr(), y.stride(0), y.shape[0], m.cols, group,
-             m.group_rows if len(m.shape) == 3 else group, _stream()), "fp8_read")
+    _call("fp8_rows", "brolm_fp8_read", _ROWS.pack(y.data_ptr(), m.packed[0], m.packed[1], _raw_stream(_device()), y.stride(0), m.packed[2], y.shape[0],
+                                                   _CODES[y.dtype], m.cols, m.rows, m.group_rows, 1), "fp8_read")
 
 
 # --- products ----------------------------------------------------------------
 STREAM_ROWS = 128        # up to as many rows W is streamed; more are tiles of 256 x 256
+FUSED_ROWS = 16          # up to as many rows the stream of W can round the rows itself ...
+_FUSED_BLOCKS = 24       # ... where a block keeps no more than as many blocks of K of them
+_PIECE = 16              # blocks of K that a float32 result is summed over before the sum goes to registers
+_ACTS = {(gated, name): code for gated, table in ((True, ACTIVATIONS), (False, EXPERT_ACTS)) for name, code in table.items()}
 
 
+@functools.lru_cache(maxsize=1024)
 def fp8_slices(tiles: int, nkb: int, sms: int) -> int:
-    """Into how many slices K is cut for a product of few rows, ``tiles`` tiles of 128 rows of W and ``nkb`` blocks of K."""
+    """Into how many slices K is cut for a product of few rows, ``tiles`` tiles of 128 rows of W and ``nkb`` blocks of K: as many
+    as find room at a time (two blocks an SM, of which clusters leave an eighth empty), of two blocks of K at least.
+    8 rows, 1 / 4 / 8 slices: 2,304 x 9,216 27 / 9.3 / 7.1 us; 4,608 x 36,864 in 1 / 4 / 7 / 8: 107 / 36 / 31.6 / 36."""
     best = 1
     for s in range(2, 9):
         per = (nkb + s - 1) // s
-        if per >= 2 and (s - 1) * per < nkb and tiles * s <= sms:
+        if per >= 2 and (s - 1) * per < nkb and 8 * tiles * s <= 14 * sms:
             best = s
     return best
 
 
-def _out_check(what: str, out: torch.Tensor, rows: int, cols: int) -> None:
-    _rows(what, out)
-    if tuple(out.shape) != (rows, cols):
-        raise KernelError(f"{what}: the result has the shape {(rows, cols)}, not {tuple(out.shape)}")
+def fp8_fused(rows: int, nkb: int, slices: int) -> bool:
+    """Whether the stream of W rounds the rows itself: every block those of its slice, four blocks of K of a row a warp."""
+    per = (nkb + slices - 1) // slices
+    return rows <= FUSED_ROWS and per <= _FUSED_BLOCKS and rows * ((per + 6) // 4) <= 64
 
 
 def _act_code(what: str, w: Fp8Matrix, activation: str) -> int:
-    table = ACTIVATIONS if w.gated else EXPERT_ACTS
-    if activation not in table:
+    code = _ACTS.get((w.gated, activation))
+    if code is None:
+        table = ACTIVATIONS if w.gated else EXPERT_ACTS
         raise KernelError(f"{what}: unknown activation '{activation}' for {'gated' if w.gated else 'plain'} rows (known: {sorted(table)})")
-    return table[activation]
+    return code
 
 
-def _to8(what: str, x, cols: int) -> Fp8Matrix:
-    if isinstance(x, Fp8Matrix):
-        if len(x.shape) != 2 or x.cols != cols:
-            raise KernelError(f"{what}: rows of {cols} numbers are wanted, not {tuple(x.shape)}")
-        return x
-    x = _rows(what, x)
-    if x.dim() != 2 or x.shape[1] != cols:
-        raise KernelError(f"{what}: rows of {cols} numbers are wanted, not {tuple(x.shape)}")
-    m = _empty(tuple(x.shape), x.device)
-    if x.shape[0]:
-        _quantize(x, m, 1)
-    return m
+def _checked(what: str, x, w: Fp8Matrix, out: torch.Tensor, outputs: int) -> None:
+    """Refuses rows, a matrix and a result that do not go together."""
+    if type(x) is Fp8Matrix:
+        if len(x.shape) != 2 or x.cols != w.cols:
+            raise KernelError(f"{what}: rows of {w.cols} numbers are wanted, not {x.shape}")
+        fine = x.index == w.index
+    else:
+        fine = x.dtype in _CODES and x.dim() == 2 and x.shape[1] == w.cols and x.get_device() == w.index and (x.stride(1) == 1 or w.cols == 1)
+    if fine and len(w.shape) == 2 and w.index >= 0 and w.index == _device() and out.dtype in _CODES and out.get_device() == w.index and out.dim() == 2 \
+            and out.shape[0] == x.shape[0] and out.shape[1] == outputs and (out.stride(1) == 1 or outputs == 1):
+        return
+    if len(w.shape) != 2:
+        raise KernelError(f"{what}: a stack of experts' matrices goes to experts_fp8")
+    if type(x) is not Fp8Matrix:
+        _refuse(what, x, "x")
+        if x.shape[1] != w.cols:
+            raise KernelError(f"{what}: rows of {w.cols} numbers are wanted, not {tuple(x.shape)}")
+    _refuse(what, out, "out")
+    if tuple(out.shape) != (x.shape[0], outputs):
+        raise KernelError(f"{what}: the result has the shape {(x.shape[0], outputs)}, not {tuple(out.shape)}")
+    raise KernelError(f"{what}: the rows, the matrix and the result live on {x.device}, {w.device} and {out.device}; the current device is cuda:{_device()}")
 
 
-def _product(x: Fp8Matrix, w: Fp8Matrix, out, act: int, limit: float) -> None:
-    M, K, N = x.rows, x.cols, w.outputs
+_NO_EXPERTS = (0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
+
+
+def _product(x, M: int, w: Fp8Matrix, y: tuple, out: int, act: int, limit: float) -> None:
+    """``x``: a tensor of rows, or 8-bit rows as (values, scales, stride); ``y`` (result, its scales, stride), ``out`` its kind."""
+    K, N = w.cols, w.outputs
     if not M or not N:
         return
-    to8 = isinstance(out, Fp8Matrix)
-    if M <= STREAM_ROWS and not to8:
-        slices = fp8_slices((w.rows + 127) // 128, (K + 127) // 128, device_sms())
-        f = _fn("fp8_stream", "brolm_fp8_stream", [c_void_p, c_longlong, c_void_p, c_void_p, c_longlong, c_void_p, c_void_p, c_longlong, c_int, c_int, c_int,
-                                                   c_int, c_int, c_int, c_float, c_int, c_void_p])
-        _check(f(x.values.data_ptr(), x.values.stride(0), x.scales.data_ptr(), w.values.data_ptr(), w.values.stride(0), w.scales.data_ptr(), out.data_ptr(),
-                 out.stride(0), 1 if out.dtype == torch.float32 else 0, M, N, K, 1 if w.gated else 0, act, limit, slices, _stream()), "linear_fp8")
-        return
-    y, kind = (out.values, 2) if to8 else (out, 1 if out.dtype == torch.float32 else 0)
-    f = _fn("fp8_gemm", "brolm_fp8_gemm", [c_void_p, c_longlong, c_void_p, c_void_p, c_longlong, c_void_p, c_void_p, c_longlong, c_void_p, c_int, c_int, c_int,
-                                           c_int, c_int, c_int, c_float, c_int, c_void_p])
-    _check(f(x.values.data_ptr(), x.values.stride(0), x.scales.data_ptr(), w.values.data_ptr(), w.values.stride(0), w.scales.data_ptr(), y.data_ptr(), y.stride(0),
-             out.scales.data_ptr() if to8 else None, kind, M, N, K, 1 if w.gated else 0, act, limit, _PIECE, _stream()), "linear_fp8")
+    device = w.index
+    stream = _raw_stream(device)
+    held = None
+    if M <= STREAM_ROWS and out != 2:
+        nkb = (K + 127) >> 7
+        cut = fp8_slices((w.rows + 127) >> 7, nkb, device_sms(w.device))
+        fused, lib, name = 0, "fp8_stream", "brolm_fp8_stream"
+        if type(x) is not tuple and fp8_fused(M, nkb, cut):
+            fused = _FUSED[x.dtype]
+            x = (x.data_ptr(), 0, x.stride(0))
+    else:
+        fused, cut, lib, name = 0, _PIECE, "fp8_gemm", "brolm_fp8_gemm"
+    if type(x) is not tuple:
+        held, packed = _scratch(M, K, w.device)
+        _quantize(x, packed, M, M, 1)
+        x = packed
+    wv, ws, ldw = w.packed
+    _call(lib, name, _PRODUCT.pack(x[0], x[1], wv, ws, y[0], y[1], stream, x[2], ldw, y[2], M, N, K, 1 if w.gated else 0, act, out, fused, cut, limit,
+                                   *_NO_EXPERTS), "linear_fp8")
 
 
 def linear_fp8(x, w: Fp8Matrix, out: torch.Tensor, activation: str = "none", limit: float = 0.0) -> None:
     """out [rows, w.outputs] (float32 or bfloat16) = act(x w^T).  x [rows, columns]: float32 or bfloat16, which is rounded to 8
     bits first, or such rows.  With a plain matrix ``activation`` is "none" or "relu2" (the square of relu), with a gated one one
     of ``ACTIVATIONS``: act(gate) * partner."""
-    if len(w.shape) != 2:
-        raise KernelError("linear_fp8: a stack of experts' matrices goes to experts_fp8")
     act = _act_code("linear_fp8", w, activation)
-    x8 = _to8("linear_fp8", x, w.cols)
-    _out_check("linear_fp8", out, x8.rows, w.outputs)
-    _product(x8, w, out, act, float(limit))
+    _checked("linear_fp8", x, w, out, w.outputs)
+    _product(x.packed if type(x) is Fp8Matrix else x, x.shape[0], w, (out.data_ptr(), 0, out.stride(0)), _OUT[out.dtype], act, limit)
 
 
 def feedforward_fp8(x, gate_up: Fp8Matrix, down: Fp8Matrix, out: torch.Tensor, activation: str = "gelu_tanh", limit: float = 0.0) -> None:
-    """out [rows, down.rows] = (act(x Wg^T) * (x Wu^T)) Wd^T; what goes into the second product is rounded to 8 bits, too."""
-    if len(gate_up.shape) != 2 or len(down.shape) != 2 or down.gated or gate_up.outputs != down.cols:
-        raise KernelError(f"feedforward_fp8: matrices of shapes {tuple(gate_up.shape)} and {tuple(down.shape)} do not follow one another")
+    """out [rows, down.rows] = (act(x Wg^T) * (x Wu^T)) Wd^T; what goes into the second product is rounded to 8 bits, too.
+    ``gate_up`` may be a plain matrix with "relu2" or "none" for an ``activation``: out = act(x W^T) Wd^T."""
+    if len(gate_up.shape) != 2 or len(down.shape) != 2 or down.gated or gate_up.outputs != down.cols or gate_up.index != down.index:
+        raise KernelError(f"feedforward_fp8: matrices of shapes {gate_up.shape} and {down.shape} do not follow one another")
     act = _act_code("feedforward_fp8", gate_up, activation)
-    x8 = _to8("feedforward_fp8", x, gate_up.cols)
-    M, inter = x8.rows, gate_up.outputs
-    _out_check("feedforward_fp8", out, M, down.rows)
+    _checked("feedforward_fp8", x, gate_up, out, down.rows)
+    M, inter = x.shape[0], down.cols
+    if type(x) is Fp8Matrix:
+        x = x.packed
+    y = (out.data_ptr(), 0, out.stride(0))
     if M <= STREAM_ROWS:
-        h = torch.empty((M, inter), dtype=torch.float32, device=out.device)
-        _product(x8, gate_up, h, act, float(limit))
-        h8 = _to8("feedforward_fp8", h, inter)
+        # (a stream's tile holds parts of a block only)
+        h = torch.empty((M, inter), dtype=_F32, device=down.device)
+        _product(x, M, gate_up, (h.data_ptr(), 0, inter), 1, act, limit)
     else:
-        h8 = _empty((M, inter), out.device)
-        _product(x8, gate_up, h8, act, float(limit))
-    _product(h8, down, out, 0, 0.0)
+        held, h = _scratch(M, inter, down.device)
+        _product(x, M, gate_up, h, 2, act, limit)
+    _product(h, M, down, y, _OUT[out.dtype], 0, 0.0)
 
 
 # --- routed experts -----------------------------------------------------------
@@ -240,6 +285,23 @@ def experts_fp8_rows(pairs: int, experts: int) -> int:
     return 256
 
 
+def _experts_checked(what: str, x, ids, up: Fp8Matrix, down: Fp8Matrix, scale) -> None:
+    _refuse(what, x, "x")
+    if len(up.shape) != 3 or len(down.shape) != 3 or down.gated or up.shape[0] != down.shape[0] or up.outputs != down.cols:
+        raise KernelError(f"{what}: stacks of shapes {up.shape} and {down.shape} do not follow one another")
+    if up.shape[0] > 4096:
+        raise KernelError(f"{what}: {up.shape[0]} experts are more than 4,096")
+    if x.shape[1] != up.cols:
+        raise KernelError(f"{what}: rows of {up.cols} numbers are wanted, not {tuple(x.shape)}")
+    if ids.dim() != 2 or ids.shape[0] != x.shape[0] or ids.dtype != torch.int32 or not ids.is_contiguous():
+        raise KernelError(f"{what}: ids are a packed int32 [tokens, top]")
+    if scale is not None and (scale.dtype != _F32 or scale.shape != ids.shape or not scale.is_contiguous()):
+        raise KernelError(f"{what}: the pairs' numbers are a packed float32 [tokens, top]")
+    for t in (ids, up, down, scale):
+        if t is not None and t.device != x.device:
+            raise KernelError(f"{what}: tensors on {x.device} and {t.device}")
+
+
 def experts_fp8_pairs(x: torch.Tensor, ids: torch.Tensor, up: Fp8Matrix, down: Fp8Matrix, out: torch.Tensor, activation: str = "silu",
                       limit: float = 0.0, scale: Optional[torch.Tensor] = None) -> None:
     """Every (token, choice) pair through its expert: out float32 [top, tokens, down.rows], a pair's result at [its choice, its
@@ -247,22 +309,10 @@ def experts_fp8_pairs(x: torch.Tensor, ids: torch.Tensor, up: Fp8Matrix, down: F
     [experts, ...], gated or not, ``down`` the stack of the second matrices; ``scale`` float32 [tokens, top] multiplies a pair's
     sums before the activation."""
     what = "experts_fp8"
-    x = _rows(what, x)
-    if len(up.shape) != 3 or len(down.shape) != 3 or down.gated or up.shape[0] != down.shape[0] or up.outputs != down.cols:
-        raise KernelError(f"{what}: stacks of shapes {tuple(up.shape)} and {tuple(down.shape)} do not follow one another")
-    if x.dim() != 2 or x.shape[1] != up.cols:
-        raise KernelError(f"{what}: rows of {up.cols} numbers are wanted, not {tuple(x.shape)}")
-    T = x.shape[0]
-    if ids.dim() != 2 or ids.shape[0] != T or ids.dtype != torch.int32 or not ids.is_contiguous():
-        raise KernelError(f"{what}: ids are a packed int32 [tokens, top]")
-    E, top, dev = up.shape[0], ids.shape[1], x.device
-    if tuple(out.shape) != (top, T, down.rows) or out.dtype != torch.float32 or not out.is_contiguous():
-        raise KernelError(f"{what}: the pairs' results are a packed float32 {(top, T, down.rows)}")
-    if scale is not None and (scale.dtype != torch.float32 or scale.shape != ids.shape or not scale.is_contiguous()):
-        raise KernelError(f"{what}: the pairs' scales are a packed float32 [tokens, top]")
-    for t in (ids, up, down, out, scale):
-        if t is not None and t.device != dev:
-            raise KernelError(f"{what}: tensors on {dev} and {t.device}")
+    _experts_checked(what, x, ids, up, down, scale)
+    E, (T, top), dev = up.shape[0], ids.shape, x.device
+    if tuple(out.shape) != (top, T, down.rows) or out.dtype != _F32 or not out.is_contiguous() or out.device != dev:
+        raise KernelError(f"{what}: the pairs' results are a packed float32 {(top, T, down.rows)} on {dev}")
     act = _act_code(what, up, activation)
     P, K, inter, N = T * top, x.shape[1], up.outputs, down.rows
     if not P or not E or not N:
@@ -270,39 +320,32 @@ def experts_fp8_pairs(x: torch.Tensor, ids: torch.Tensor, up: Fp8Matrix, down: F
     rows = experts_fp8_rows(P, E)
     pad = _round_up(rows, 128)
     most = (P + rows - 1) // rows + min(E, P)
+    # the order and the list of tiles
     lists = torch.empty(2 * P + E + 1 + 2 * most, dtype=torch.int32, device=dev)
-    at = lists.data_ptr()
-    perm, place, offsets, group, row0 = at, at + 4 * P, at + 8 * P, at + 8 * P + 4 * (E + 1), at + 8 * P + 4 * (E + 1 + most)
-    stream = _stream()
-    f = _fn("fp8_rows", "brolm_fp8_group", [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p])
-    _check(f(ids.data_ptr(), P, E, rows, perm, place, offsets, group, row0, most, stream), what)
-    gather = _fn("fp8_rows", "brolm_fp8_gather", [c_int, c_void_p, c_longlong, c_void_p, c_void_p, c_int, c_void_p, c_longlong, c_void_p, c_int, c_int, c_void_p])
-    a = _empty((P, K), dev, scale_rows=most * pad)
-    _check(gather(_CODES[x.dtype], x.data_ptr(), x.stride(0), perm, place, top, a.values.data_ptr(), a.values.stride(0), a.scales.data_ptr(), P, K, stream), what)
-    s = scale.data_ptr() if scale is not None else None
-    h8 = _empty((P, inter), dev, scale_rows=most * pad)
+    perm = lists.data_ptr()
+    place = perm + 4 * P
+    offsets = place + 4 * P
+    group = offsets + 4 * (E + 1)
+    row0 = group + 4 * most
+    stream = _raw_stream(_device())
+    _call("fp8_rows", "brolm_fp8_group", _GROUP.pack(ids.data_ptr(), perm, place, offsets, group, row0, stream, P, E, rows, most), what)
+    held, a = _scratch(P, K, dev, most * pad)
+    _call("fp8_rows", "brolm_fp8_gather", _GATHER.pack(x.data_ptr(), perm, place, a[0], a[1], stream, x.stride(0), a[2], _CODES[x.dtype], top, P, K), what)
+    held2, h = _scratch(P, inter, dev, most * pad)
+    lib, name = ("fp8_stream", "brolm_fp8_stream") if rows <= STREAM_ROWS else ("fp8_gemm", "brolm_fp8_gemm")
+
+    def product(m, w, y, kind, n, k, code, lim, s, last):
+        wv, ws, ldw = w.packed
+        _call(lib, name, _PRODUCT.pack(m[0], m[1], wv, ws, y[0], y[1], stream, m[2], ldw, y[2], P, n, k, 1 if w.gated else 0, code, kind, 0, _PIECE, lim, E,
+                                       group, row0, offsets, perm, s, w.group_rows, last, top, T, rows, most), what)
+    s = scale.data_ptr() if scale is not None else 0
     if rows <= STREAM_ROWS:
-        f = _fn("fp8_stream", "brolm_fp8_experts_stream", [c_void_p, c_longlong, c_void_p, c_void_p, c_longlong, c_void_p, c_void_p, c_longlong, c_int, c_int,
-                                                           c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
-                                                           c_int, c_int, c_int, c_int, c_int, c_void_p])
-
-        def product(m, w, y, ldy, n, k, code, sc, last):
-            _check(f(m.values.data_ptr(), m.values.stride(0), m.scales.data_ptr(), w.values.data_ptr(), w.values.stride(0), w.scales.data_ptr(), y, ldy, 1, P, n, k,
-                     E, w.group_rows, 1 if w.gated else 0, code, float(limit), group, row0, offsets, perm, sc, last, top, T, rows, most, stream), what)
-        h = torch.empty((P, inter), dtype=torch.float32, device=dev)
-        product(a, up, h.data_ptr(), inter, inter, K, act, s, 0)
-        _check(gather(0, h.data_ptr(), inter, perm, place, 0, h8.values.data_ptr(), h8.values.stride(0), h8.scales.data_ptr(), P, inter, stream), what)
-        product(h8, down, out.data_ptr(), N, N, inter, 0, None, 1)
-        return
-    f = _fn("fp8_gemm", "brolm_fp8_experts_gemm", [c_void_p, c_longlong, c_void_p, c_void_p, c_longlong, c_void_p, c_void_p, c_longlong, c_void_p, c_int, c_int,
-                                                   c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
-                                                   c_int, c_int, c_int, c_int, c_void_p])
-
-    def product(m, w, y, ldy, ys, kind, n, k, code, sc, last):
-        _check(f(m.values.data_ptr(), m.values.stride(0), m.scales.data_ptr(), w.values.data_ptr(), w.values.stride(0), w.scales.data_ptr(), y, ldy, ys, kind, P, n,
-                 k, E, w.group_rows, 1 if w.gated else 0, code, float(limit), _PIECE, group, row0, offsets, perm, sc, last, top, T, most, stream), what)
-    product(a, up, h8.values.data_ptr(), h8.values.stride(0), h8.scales.data_ptr(), 2, inter, K, act, s, 0)
-    product(h8, down, out.data_ptr(), N, None, 1, N, inter, 0, None, 1)
+        sums = torch.empty((P, inter), dtype=_F32, device=dev)
+        product(a, up, (sums.data_ptr(), 0, inter), 1, inter, K, act, limit, s, 0)
+        _call("fp8_rows", "brolm_fp8_gather", _GATHER.pack(sums.data_ptr(), perm, place, h[0], h[1], stream, inter, h[2], 0, 0, P, inter), what)
+    else:
+        product(a, up, h, 2, inter, K, act, limit, s, 0)
+    product(h, down, (out.data_ptr(), 0, N), 1, N, inter, 0, 0.0, 0, 1)
 
 
 def experts_fp8(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, up: Fp8Matrix, down: Fp8Matrix, out: torch.Tensor, activation: str = "silu",
@@ -311,17 +354,17 @@ def experts_fp8(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, up: F
     the order of the choices; a number in ``ids`` that is no expert's adds nothing.  With ``scale_input`` the weight multiplies
     the sums before the activation and not the result."""
     what = "experts_fp8"
-    if weights.shape != ids.shape or weights.dtype != torch.float32 or not weights.is_contiguous() or weights.device != x.device:
-        raise KernelError(f"{what}: weights are a packed float32 [tokens, top] beside the tokens")
+    _experts_checked(what, x, ids, up, down, weights)
     T, top = ids.shape
-    _out_check(what, out, T, down.rows)
-    y = torch.empty((top, T, down.rows), dtype=torch.float32, device=out.device)
+    _refuse(what, out, "out")
+    if tuple(out.shape) != (T, down.rows):
+        raise KernelError(f"{what}: the result has the shape {(T, down.rows)}, not {tuple(out.shape)}")
+    y = torch.empty((top, T, down.rows), dtype=_F32, device=x.device)
     experts_fp8_pairs(x, ids, up, down, y, activation, limit, weights if scale_input else None)
     if not T or not down.rows:
         return
-    f = _fn("fp8_rows", "brolm_fp8_combine", [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_longlong, c_int, c_void_p])
-    _check(f(y.data_ptr(), ids.data_ptr(), None if scale_input else weights.data_ptr(), top, up.shape[0], T, down.rows, out.data_ptr(), out.stride(0),
-             1 if out.dtype == torch.float32 else 0, _stream()), what)
+    _call("fp8_rows", "brolm_fp8_combine", _COMBINE.pack(y.data_ptr(), ids.data_ptr(), 0 if scale_input else weights.data_ptr(), out.data_ptr(),
+                                                         _raw_stream(_device()), out.stride(0), top, up.shape[0], T, down.rows, _CODES[out.dtype] ^ 1), what)
 
 
 def fp8_stream_status(reset: bool = False) -> int:
