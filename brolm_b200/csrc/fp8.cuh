@@ -47,6 +47,14 @@ __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d, fl
 }
 constexpr uint32_t NAN4 = 0x7f7f7f7fu;
 
+// One lane of a warp that is there as a whole.  The compiler knows of this one that it is alone and keeps what the products are
+// given in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(one));
+    return one != 0;
+}
+
 // ---- tensor core, operands e4m3, scales ue8m0
 // Instruction descriptor of kind::mxf8f6f4 without the scales' byte numbers (a: bits 29-30, b: bits 4-5).
 __device__ __forceinline__ uint32_t idesc_mx(int m, int n) {

@@ -31,10 +31,11 @@ namespace {
 using namespace tc;
 using namespace fp8;
 
-constexpr int BM = 128, PM = 256, BN = 256, HN = 128, BK = 128, STAGES = 6;
+constexpr int BM = 128, PM = 256, BN = 256, HN = 128, BK = 128, STAGES = 5;
 constexpr int A_BYTES = BM * BK, B_BYTES = HN * BK, STAGE_BYTES = A_BYTES + B_BYTES, SCALES = 3 * SF_TILE;
 constexpr int THREADS = 320;
 constexpr int TMEM_COLS = 512, ACC1 = 224, SF_COL = 480;
+constexpr int ROOM_BYTES = 8 * 4096;        // of the epilogue's warps, for results on their way out
 constexpr int ROWS_BYTES = 2 * BM * 4;      // largest magnitudes of a row's two halves
 
 enum : int { EPI_STORE = 0, EPI_GATED = 1 };
@@ -65,6 +66,10 @@ struct GemmArgs {
 
 __device__ __forceinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile int* give_up, int code) {
     return mbar_wait(bar, parity, give_up, &g_fp8_gemm_error, code);
+}
+// a wait that is mostly over when it begins
+__device__ __forceinline__ bool wait_one(uint32_t bar, uint32_t parity, volatile int* give_up, int code) {
+    return mbar_try(bar, parity) || wait_on(bar, parity, give_up, code);
 }
 __device__ __forceinline__ bool drain_on(uint32_t bar, uint32_t parity, volatile int* give_up, int code) {
     return mbar_wait(bar, parity, give_up, &g_fp8_gemm_error, code, true);
@@ -114,32 +119,47 @@ __device__ __forceinline__ float act_of(float v, int act) {
     return v;
 }
 
-// n results of a row from column `col` on, those below `cols` alone
-template <int N>
-__device__ __forceinline__ void store_row(bf16* dst, const float* o, int col, int cols, bool wide) {
-    if (wide && col + N <= cols) {
-#pragma unroll
-        for (int i = 0; i < N; i += 8) {
-            uint4 p;
-            __nv_bfloat162* p2 = reinterpret_cast<__nv_bfloat162*>(&p);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) p2[e] = __floats2bfloat162_rn(o[i + 2 * e], o[i + 2 * e + 1]);
-            *reinterpret_cast<uint4*>(dst + i) = p;
-        }
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i) if (col + i < cols) dst[i] = __float2bfloat16_rn(o[i]);
+// Results on their way out.  A thread has a row, and stores of sixteen bytes in 32 rows are half sectors in 32 lines: they took
+// longer than the products of a tile (2,304 along K: 18,500 cycles a tile, of which 6,400 were that).  So a warp leaves 128
+// bytes of each of its 32 rows in four KB of shared memory of its own, sixteen-byte pieces swapped by the row, and stores whole
+// lines from there, eight lanes a row.
+__device__ __forceinline__ void stage16(uint8_t* room, int lane, int piece, uint4 v) {
+    *reinterpret_cast<uint4*>(room + lane * 128 + ((piece ^ (lane & 7)) << 4)) = v;
 }
-template <int N>
-__device__ __forceinline__ void store_row(float* dst, const float* o, int col, int cols, bool wide) {
-    if (wide && col + N <= cols) {
+// dst: where a row's bytes go (of each lane its own row's; null: nowhere), of which `bytes` are wanted; ROW: bytes staged a row
+template <int ROW>
+__device__ __forceinline__ void flush_rows(const uint8_t* room, int lane, uint8_t* dst, int bytes, bool wide, int unit) {
+    __syncwarp();
+    constexpr int PIECES = ROW / 16, ROWS = 32 / PIECES;       // rows a round
 #pragma unroll
-        for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(dst + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-        return;
+    for (int r0 = 0; r0 < 32; r0 += ROWS) {
+        const int r = r0 + lane / PIECES, piece = lane % PIECES;
+        uint8_t* to = reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), r));
+        const uint4 v = *reinterpret_cast<const uint4*>(room + r * 128 + ((piece ^ (r & 7)) << 4));
+        const int left = bytes - piece * 16;
+        if (to && left > 0) {
+            to += piece * 16;
+            if (wide && left >= 16) *reinterpret_cast<uint4*>(to) = v;
+            else {
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                if (unit == 4) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) if (4 * i < left) reinterpret_cast<uint32_t*>(to)[i] = w[i];
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) if (2 * i < left) reinterpret_cast<uint16_t*>(to)[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+                }
+            }
+        }
     }
+    __syncwarp();
+}
+__device__ __forceinline__ uint4 pack_bf16(const float* o) {
+    uint4 p;
+    __nv_bfloat162* p2 = reinterpret_cast<__nv_bfloat162*>(&p);
 #pragma unroll
-    for (int i = 0; i < N; ++i) if (col + i < cols) dst[i] = o[i];
+    for (int e = 0; e < 4; ++e) p2[e] = __floats2bfloat162_rn(o[2 * e], o[2 * e + 1]);
+    return p;
 }
 
 __device__ __forceinline__ void load_columns(uint32_t taddr, uint32_t (&v)[32]) { tmem_ld32(taddr, v); }
@@ -159,7 +179,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* base = smem_raw;
     const uint32_t rank = cluster_rank();
-    uint64_t* bars = reinterpret_cast<uint64_t*>(base + STAGES * (STAGE_BYTES + SCALES));
+    uint8_t* rooms = base + STAGES * (STAGE_BYTES + SCALES);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(rooms + ROOM_BYTES);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 6);
     volatile int* give_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
     uint32_t* most_of = tmem_slot + 4;                        // [2][128]
@@ -213,7 +234,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     };
 
     if (warp == 0) {
-        if (lane == 0) {
+        if (elect_one()) {
             int it = 0, s = 0, phase = 0;
             bool ok = !*give_up;
             // Launched with programmatic stream serialization: nothing of this kernel touches memory before its first
@@ -225,7 +246,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                 const int w_row = group * g.group_rows + nt * BN;
                 const int xs_row = (EXPERTS ? mt * (PM / 128) : row0 >> 7) + (int)rank, ws_row = w_row >> 7;
                 for (int kb = 0; kb < g.nkb; ++kb, ++it) {
-                    if (!wait_on(empty0 + 8 * s, phase ^ 1, give_up, 1)) { ok = false; break; }
+                    if (!(kb > 0 ? wait_one(empty0 + 8 * s, phase ^ 1, give_up, 1) : wait_on(empty0 + 8 * s, phase ^ 1, give_up, 1))) { ok = false; break; }
                     const uint32_t full = full0 + 8 * s, a_dst = stage0 + s * STAGE_BYTES, s_dst = scale0 + s * SCALES;
                     const bool with_scales = (kb & 3) == 0;
                     if (rank == 0) mbar_expect_tx(full, 2 * (STAGE_BYTES + (with_scales ? SCALES : 0)));   // both blocks' bytes
@@ -246,7 +267,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             }
         }
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
+        if (rank == 0 && elect_one()) {
             const uint32_t id = idesc_mx(PM, BN);
             int s = 0, phase = 0, local = 0, set = 0;
             bool ok = !*give_up;
@@ -262,7 +283,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                     fence_after_sync();
                     const uint32_t acc = tmem + as * ACC1;
                     for (int kb = lo; kb < hi; ++kb) {
-                        ok = wait_on(full0 + 8 * s, phase, give_up, 2);
+                        // (the flags are looked at where a piece begins and where the stage is not there yet)
+                        ok = kb > lo ? wait_one(full0 + 8 * s, phase, give_up, 2) : wait_on(full0 + 8 * s, phase, give_up, 2);
                         if (!ok) break;
                         fence_after_sync();
                         if ((kb & 3) == 0) {
@@ -287,6 +309,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         }
     } else {
         const int quarter = warp & 3, half = (warp - 2) >> 2;
+        uint8_t* room = rooms + (warp - 2) * 4096;
         const int trow = quarter * 32 + lane;                   // row of this block's half of the tile
         int local = 0;
         if (EXPERTS) pdl_wait();
@@ -350,8 +373,11 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                         for (int i = 0; i < W; ++i) sum[OC + i] = o[i];
                         return;
                     }
+                    // parts of 32 columns: (3), 0, 1, 2 or 0, 1, 2, 3, gated ones half as many results
                     const int col = nt * OUT_COLS + half * (OUT_COLS / 2) + OC;
-                    if (valid && col < g.N) store_row<W>((bf16*)g.y + at * g.ldy + col, o, col, g.N, g.y_wide);
+#pragma unroll
+                    for (int i = 0; i < W / 8; ++i) stage16(room, lane, i, pack_bf16(o + 8 * i));
+                    flush_rows<2 * W>(room, lane, valid && col < g.N ? (uint8_t*)((bf16*)g.y + at * g.ldy + col) : nullptr, 2 * (g.N - col), g.y_wide, 2);
                 };
                 if (as == 0) in_order<CW, 32 / CW>(take);
                 else in_order<CW, 0>(take);
@@ -370,8 +396,14 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
 #pragma unroll
                     for (int i = 0; i < 128; ++i) sum[i] = act_of(sum[i], g.act);
                 }
-                const int col = nt * OUT_COLS + half * W;
-                if (valid && col < g.N) store_row<W>((float*)g.y + at * g.ldy + col, sum, col, g.N, g.y_wide);
+#pragma unroll
+                for (int c = 0; c < W; c += 32) {
+                    const int col = nt * OUT_COLS + half * W + c;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        stage16(room, lane, i, make_uint4(__float_as_uint(sum[c + 4 * i]), __float_as_uint(sum[c + 4 * i + 1]), __float_as_uint(sum[c + 4 * i + 2]), __float_as_uint(sum[c + 4 * i + 3])));
+                    flush_rows<128>(room, lane, valid && col < g.N ? (uint8_t*)((float*)g.y + at * g.ldy + col) : nullptr, 4 * (g.N - col), g.y_wide, 4);
+                }
             }
             if (OUT == OUT_FP8) {
                 constexpr int W = EPI == EPI_GATED ? 64 : 128;
@@ -390,16 +422,17 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                 }
                 const uint32_t byte = scale_byte(most);
                 const float inv = byte == 255u ? 1.0f : scale_inverse(byte);
-                if (valid && col < g.N) {
-                    uint8_t* dst = (uint8_t*)g.y + at * g.ldy + col;
 #pragma unroll
-                    for (int i = 0; i < W; i += 16) {
-                        uint4 q = make_uint4(NAN4, NAN4, NAN4, NAN4);
-                        if (byte != 255u)
-                            q = make_uint4(pack4(sum[i], sum[i + 1], sum[i + 2], sum[i + 3], inv), pack4(sum[i + 4], sum[i + 5], sum[i + 6], sum[i + 7], inv),
-                                           pack4(sum[i + 8], sum[i + 9], sum[i + 10], sum[i + 11], inv), pack4(sum[i + 12], sum[i + 13], sum[i + 14], sum[i + 15], inv));
-                        if (col + i < g.ldy) *reinterpret_cast<uint4*>(dst + i) = q;       // ldy is a multiple of 16
-                    }
+                for (int i = 0; i < W; i += 16) {
+                    uint4 q = make_uint4(NAN4, NAN4, NAN4, NAN4);
+                    if (byte != 255u)
+                        q = make_uint4(pack4(sum[i], sum[i + 1], sum[i + 2], sum[i + 3], inv), pack4(sum[i + 4], sum[i + 5], sum[i + 6], sum[i + 7], inv),
+                                       pack4(sum[i + 8], sum[i + 9], sum[i + 10], sum[i + 11], inv), pack4(sum[i + 12], sum[i + 13], sum[i + 14], sum[i + 15], inv));
+                    stage16(room, lane, i / 16, q);
+                }
+                // (a row's bytes are a multiple of 16)
+                flush_rows<W>(room, lane, valid && col < g.N ? (uint8_t*)g.y + at * g.ldy + col : nullptr, (int)g.ldy - col, true, 2);
+                if (valid && col < g.N) {
                     const int b = col >> 7;
                     // scales by the row's tile: rows of the matrix (dense), rows of the list's tile (experts)
                     const long s_row = EXPERTS ? (long)mt * PM + rank * BM + trow : row;
@@ -414,7 +447,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     if (warp == 1) tmem_dealloc_pair(tmem, TMEM_COLS);
 }
 
-constexpr size_t SMEM_BYTES = (size_t)STAGES * (STAGE_BYTES + SCALES) + (2 * STAGES + 6) * 8 + 16 + ROWS_BYTES;
+constexpr size_t SMEM_BYTES = (size_t)STAGES * (STAGE_BYTES + SCALES) + ROOM_BYTES + (2 * STAGES + 6) * 8 + 16 + ROWS_BYTES;
 
 // a matrix of scale tiles: rows of 512 bytes
 int make_map_scales(CUtensorMap* map, const void* ptr, long long tiles) {

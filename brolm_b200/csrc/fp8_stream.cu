@@ -63,6 +63,10 @@ struct StreamArgs {
 __device__ __forceinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile int* give_up, int code) {
     return mbar_wait(bar, parity, give_up, &g_fp8_stream_error, code);
 }
+// a wait that is mostly over when it begins: the flags are looked at only if it is not
+__device__ __forceinline__ bool wait_one(uint32_t bar, uint32_t parity, volatile int* give_up, int code) {
+    return mbar_try(bar, parity) || wait_on(bar, parity, give_up, code);
+}
 __device__ __forceinline__ bool drain_on(uint32_t bar, uint32_t parity, volatile int* give_up, int code) {
     return mbar_wait(bar, parity, give_up, &g_fp8_stream_error, code, true);
 }
@@ -207,7 +211,7 @@ __global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS) fp8_stream_kernel(c
     };
 
     if (warp == 0) {
-        if (lane == 0 && !*give_up) {
+        if (elect_one() && !*give_up) {
             auto bytes_of = [&](int kb) { return (uint32_t)(S::STAGE_BYTES + ((kb & 3) == 0 || kb == lo ? S::SCALES : 0)); };
             auto load_w = [&](int s, int rt, int group, int kb) {
                 const uint32_t full = full0 + 8 * s;
@@ -262,7 +266,7 @@ __global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS) fp8_stream_kernel(c
             }
         }
     } else if (warp == 1) {
-        if (lane == 0 && !*give_up) {
+        if (elect_one() && !*give_up) {
             const uint32_t id = idesc_mx(BR, BT);
             if (EXPERTS) pdl_wait();
             int s = 0, phase = 0, local = 0, set = 0;
@@ -278,7 +282,7 @@ __global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS) fp8_stream_kernel(c
                 const uint32_t acc = tmem + as * BT;
                 uint32_t sfw = 0, sfx = 0;
                 for (int kb = lo; kb < hi; ++kb) {
-                    ok = wait_on(full0 + 8 * s, phase, give_up, 2);
+                    ok = kb > lo ? wait_one(full0 + 8 * s, phase, give_up, 2) : wait_on(full0 + 8 * s, phase, give_up, 2);
                     if (!ok) break;
                     fence_after_sync();
                     if ((kb & 3) == 0 || kb == lo) {
