@@ -8,7 +8,8 @@
 //
 //   warp 0 (both blocks)   one thread: TMA loads, their bytes counted on the first block's barrier
 //   warp 1 (first block)   one thread: copies of scales, products, commits to both blocks
-//   warps 2-9 (both)       epilogue: a thread has a row of the tile and half of its columns
+//   warps 4-11 (both)      epilogue: a thread has a row of the tile and half of its columns, in up to 224 registers, which the first
+//                          four warps leave them (two of those are there for that alone: registers go by four warps)
 //
 // Tensor memory has 512 columns: two accumulators of 256 leave no room for the scales.  So the second accumulator begins 32
 // columns before the first ends.  A tile's products begin when the epilogue has taken those 32 columns of the tile before
@@ -33,10 +34,11 @@ using namespace fp8;
 
 constexpr int BM = 128, PM = 256, BN = 256, HN = 128, BK = 128, STAGES = 5;
 constexpr int A_BYTES = BM * BK, B_BYTES = HN * BK, STAGE_BYTES = A_BYTES + B_BYTES, SCALES = 3 * SF_TILE;
-constexpr int THREADS = 320;
+constexpr int THREADS = 384;
+constexpr int FIRST = 4;             // the epilogue's first warp
 constexpr int TMEM_COLS = 512, ACC1 = 224, SF_COL = 480;
 constexpr int ROOM_BYTES = 8 * 4096;        // of the epilogue's warps, for results on their way out
-constexpr int ROWS_BYTES = 2 * BM * 4;      // largest magnitudes of a row's two halves
+constexpr int ROWS_BYTES = 4 * BM * 4;      // largest magnitudes of a row's two halves
 
 enum : int { EPI_STORE = 0, EPI_GATED = 1 };
 enum : int { OUT_BF16 = 0, OUT_F32 = 1, OUT_FP8 = 2 };
@@ -119,6 +121,21 @@ __device__ __forceinline__ float act_of(float v, int act) {
     return v;
 }
 
+// N / 2 gated pairs of neighbouring numbers, to the front.  Which activation is asked once for all of them.
+template <int N>
+__device__ __forceinline__ void gate_pairs(float (&o)[N], int act, float limit) {
+    if (act == 0) {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) o[i] = fast_gate_pair(o[2 * i], o[2 * i + 1], 0, 0.0f);
+    } else if (act == 1) {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) o[i] = fast_gate_pair(o[2 * i], o[2 * i + 1], 1, 0.0f);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) o[i] = fast_gate_pair(o[2 * i], o[2 * i + 1], 2, limit);
+    }
+}
+
 // Results on their way out.  A thread has a row, and stores of sixteen bytes in 32 rows are half sectors in 32 lines: they took
 // longer than the products of a tile (2,304 along K: 18,500 cycles a tile, of which 6,400 were that).  So a warp leaves 128
 // bytes of each of its 32 rows in four KB of shared memory of its own, sixteen-byte pieces swapped by the row, and stores whole
@@ -126,19 +143,21 @@ __device__ __forceinline__ float act_of(float v, int act) {
 __device__ __forceinline__ void stage16(uint8_t* room, int lane, int piece, uint4 v) {
     *reinterpret_cast<uint4*>(room + lane * 128 + ((piece ^ (lane & 7)) << 4)) = v;
 }
-// dst: where a row's bytes go (of each lane its own row's; null: nowhere), of which `bytes` are wanted; ROW: bytes staged a row
-template <int ROW>
-__device__ __forceinline__ void flush_rows(const uint8_t* room, int lane, uint8_t* dst, int bytes, bool wide, int unit) {
+// Row r of the warp goes to dst + (r or, SCATTER, lane r's `at`) * ld, if r < rows; of its ROW bytes staged `bytes` are wanted,
+// in units of `unit` bytes where they do not lie in sixteens (`wide`).
+template <int ROW, bool SCATTER>
+__device__ __forceinline__ void flush_rows(const uint8_t* room, int lane, uint8_t* dst, long ld, int at, int rows, int bytes, bool wide, int unit) {
     __syncwarp();
     constexpr int PIECES = ROW / 16, ROWS = 32 / PIECES;       // rows a round
+    const int piece = lane % PIECES, left = bytes - piece * 16;
+    dst += piece * 16;
 #pragma unroll
     for (int r0 = 0; r0 < 32; r0 += ROWS) {
-        const int r = r0 + lane / PIECES, piece = lane % PIECES;
-        uint8_t* to = reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), r));
+        const int r = r0 + lane / PIECES;
         const uint4 v = *reinterpret_cast<const uint4*>(room + r * 128 + ((piece ^ (r & 7)) << 4));
-        const int left = bytes - piece * 16;
-        if (to && left > 0) {
-            to += piece * 16;
+        const int place = SCATTER ? __shfl_sync(0xffffffffu, at, r) : r;
+        uint8_t* to = dst + (long)place * ld;
+        if (r < rows && left > 0) {
             if (wide && left >= 16) *reinterpret_cast<uint4*>(to) = v;
             else {
                 const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -162,14 +181,21 @@ __device__ __forceinline__ uint4 pack_bf16(const float* o) {
     return p;
 }
 
-__device__ __forceinline__ void load_columns(uint32_t taddr, uint32_t (&v)[32]) { tmem_ld32(taddr, v); }
-__device__ __forceinline__ void load_columns(uint32_t taddr, uint32_t (&v)[16]) { tmem_ld16(taddr, v); }
-// f(part, turn) for the 128 / CW parts, the last BACK of them first
-template <int CW, int BACK, int TURN = 0, typename F>
-__device__ __forceinline__ void in_order(F&& f) {
-    constexpr int PARTS = 128 / CW;
-    f(std::integral_constant<int, (TURN + PARTS - BACK) % PARTS>{}, TURN);
-    if constexpr (TURN + 1 < PARTS) in_order<CW, BACK, TURN + 1>(f);
+// Numbers that a load from tensor memory brought are not to be touched before the wait for it.
+__device__ __forceinline__ void arrived(uint32_t (&v)[32]) {
+    tmem_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(v[i]));
+}
+// The 128 columns at `acc` in parts of 32, those from BACK parts before the end on first, the next part's load under way while
+// one is used: there(turn) once a part is in registers, use(part, numbers).
+template <int BACK, int TURN, typename T, typename F>
+__device__ __forceinline__ void walk(uint32_t acc, uint32_t (&now)[32], uint32_t (&next)[32], T&& there, F&& use) {
+    arrived(now);
+    there(TURN);
+    if constexpr (TURN < 3) tmem_ld32(acc + (TURN + 1 + 4 - BACK) % 4 * 32, next);
+    use(std::integral_constant<int, (TURN + 4 - BACK) % 4>{}, now);
+    if constexpr (TURN < 3) walk<BACK, TURN + 1>(acc, next, now, there, use);
 }
 
 template <int EPI, int OUT, bool EXPERTS>
@@ -181,12 +207,12 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     const uint32_t rank = cluster_rank();
     uint8_t* rooms = base + STAGES * (STAGE_BYTES + SCALES);
     uint64_t* bars = reinterpret_cast<uint64_t*>(rooms + ROOM_BYTES);
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 6);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 10);
     volatile int* give_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    uint32_t* most_of = tmem_slot + 4;                        // [2][128]
+    uint32_t* most_of = tmem_slot + 4;                        // [2][2][128]
     const uint32_t stage0 = smem_u32(base), scale0 = stage0 + STAGES * STAGE_BYTES;
     const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * STAGES, acc_full0 = empty0 + 8 * STAGES,
-                   acc_free0 = acc_full0 + 16, lap_free = acc_free0 + 16;
+                   acc_free0 = acc_full0 + 16, lap_free = acc_free0 + 16, halves0 = lap_free + 16;
     const bool aligned = (stage0 & 1023u) == 0;               // both blocks have the same layout
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -203,6 +229,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             mbar_init(acc_full0 + 8 * s, 1);
             mbar_init(acc_free0 + 8 * s, 16);     // eight epilogue warps of each block
         }
+        for (int q = 0; q < 4; ++q) mbar_init(halves0 + 8 * q, 2);      // the two warps that share rows
         mbar_init(lap_free, 8);                   // the four of each whose columns lie in both accumulators
         give_up[0] = aligned ? 0 : 1;
         give_up[1] = 0;
@@ -233,6 +260,9 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         return true;
     };
 
+    if (warp < FIRST) {
+    // 128 x 56 + 256 x 224 = 384 x 168, what a block is launched with
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 0) {
         if (elect_one()) {
             int it = 0, s = 0, phase = 0;
@@ -307,9 +337,11 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                 }
             }
         }
+    }
     } else {
-        const int quarter = warp & 3, half = (warp - 2) >> 2;
-        uint8_t* room = rooms + (warp - 2) * 4096;
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        const int quarter = warp & 3, half = (warp - FIRST) >> 2;
+        uint8_t* room = rooms + (warp - FIRST) * 4096;
         const int trow = quarter * 32 + lane;                   // row of this block's half of the tile
         int local = 0;
         if (EXPERTS) pdl_wait();
@@ -317,108 +349,132 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         bool ok = true;
         for (int tile = pair; tile < total && ok; tile += n_pairs) {
             if (!find(tile, mt, nt, group, row0)) break;
-            const int row = row0 + (int)rank * BM + trow;
-            const bool valid = row < (EXPERTS ? g.offsets[group + 1] : g.M);
-            long at = row;
+            const int first = row0 + (int)rank * BM + quarter * 32;             // the warp's first row
+            const int rows = (EXPERTS ? g.offsets[group + 1] : g.M) - first;    // how many of its rows there are (more than 32: all)
+            int at = 0;
             float mul = 1.0f;
-            if (EXPERTS && valid) {
+            if (EXPERTS && lane < rows) {
                 if (g.down) {
-                    const int p = g.perm[row], tok = p / g.top;
-                    at = (long)(p - tok * g.top) * g.tokens + tok;
+                    const int p = g.perm[first + lane], tok = p / g.top;
+                    at = (p - tok * g.top) * g.tokens + tok;
+                } else {
+                    at = first + lane;
                 }
-                if (g.scale) mul = g.scale[g.perm[row]];
+                if (g.scale) mul = g.scale[g.perm[first + lane]];
             }
-            constexpr int CW = OUT == OUT_BF16 ? 32 : 16;       // (as many registers as there are)
-            float sum[128];                                     // OUT_F32: the pieces' sum; OUT_FP8: the row's half
+            constexpr int W = EPI == EPI_GATED ? 64 : 128;      // this thread's results
+            const int col = nt * OUT_COLS + half * W;
+            // results of `unit` bytes from the thread's result c on, staged as ROW bytes a row
+            auto flush = [&](auto row_bytes, int c, int unit, bool wide) {
+                constexpr int ROW = decltype(row_bytes)::value;
+                uint8_t* dst = (uint8_t*)g.y + (EXPERTS ? 0 : first * (g.ldy * unit)) + (long)(col + c) * unit;
+                flush_rows<ROW, EXPERTS>(room, lane, dst, g.ldy * unit, at, rows, (OUT == OUT_FP8 ? (int)g.ldy - col - c : (g.N - col - c) * unit), wide, unit);
+            };
+            float sum[OUT == OUT_BF16 ? 1 : W == 64 && OUT == OUT_FP8 ? 64 : 128];      // OUT_F32: the pieces' sum; OUT_FP8: the row's results
+            uint4 packed[8];                                    // OUT_BF16: 64 results on their way out
             for (int lo = 0; lo < g.nkb; lo += g.piece, ++local) {
                 const int as = local & 1;
                 const bool ready = wait_on(acc_full0 + 8 * as, (local >> 1) & 1, give_up, 3);
                 if (!__all_sync(0xffffffffu, ready)) { ok = false; break; }
                 fence_after_sync();
                 const uint32_t acc = tmem + as * ACC1 + half * 128 + ((uint32_t)(quarter * 32) << 16);
-                // CW columns: the first 32 read are those that the other accumulator wants
-                auto take = [&](auto part, int turn) {
-                    constexpr int C = decltype(part)::value * CW;
-                    uint32_t v[CW];
-                    load_columns(acc + C, v);
-                    tmem_wait_ld();
-                    if (turn == 32 / CW - 1 && half != as) {
-                        fence_before_sync();
-                        __syncwarp();
-                        if (lane == 0) arrive_first_block(lap_free);
-                    }
-                    if (turn == 128 / CW - 1) {
-                        fence_before_sync();
-                        __syncwarp();
-                        if (lane == 0) arrive_first_block(acc_free0 + 8 * as);
-                    }
-                    if (OUT == OUT_F32) {
-#pragma unroll
-                        for (int i = 0; i < CW; ++i) sum[C + i] = lo == 0 ? __uint_as_float(v[i]) : sum[C + i] + __uint_as_float(v[i]);
-                        return;
-                    }
-                    float o[CW];
-#pragma unroll
-                    for (int i = 0; i < CW; ++i) o[i] = EXPERTS ? __uint_as_float(v[i]) * mul : __uint_as_float(v[i]);
-                    if (EPI == EPI_GATED) {
-#pragma unroll
-                        for (int i = 0; i < CW / 2; ++i) o[i] = fast_gate_pair(o[2 * i], o[2 * i + 1], g.act, g.limit);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < CW; ++i) o[i] = act_of(o[i], g.act);
-                    }
-                    constexpr int W = EPI == EPI_GATED ? CW / 2 : CW, OC = EPI == EPI_GATED ? C / 2 : C;
-                    if (OUT == OUT_FP8) {
-#pragma unroll
-                        for (int i = 0; i < W; ++i) sum[OC + i] = o[i];
-                        return;
-                    }
-                    // parts of 32 columns: (3), 0, 1, 2 or 0, 1, 2, 3, gated ones half as many results
-                    const int col = nt * OUT_COLS + half * (OUT_COLS / 2) + OC;
-#pragma unroll
-                    for (int i = 0; i < W / 8; ++i) stage16(room, lane, i, pack_bf16(o + 8 * i));
-                    flush_rows<2 * W>(room, lane, valid && col < g.N ? (uint8_t*)((bf16*)g.y + at * g.ldy + col) : nullptr, 2 * (g.N - col), g.y_wide, 2);
+                // the first 32 columns read are those that the other accumulator wants
+                auto there = [&](int turn) {
+                    if (turn != 3 && (turn != 0 || half == as)) return;
+                    fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) arrive_first_block(turn == 0 ? lap_free : acc_free0 + 8 * as);
                 };
-                if (as == 0) in_order<CW, 32 / CW>(take);
-                else in_order<CW, 0>(take);
+                auto use = [&](auto part, uint32_t (&v)[32]) {
+                    constexpr int P = decltype(part)::value;
+                    if constexpr (OUT == OUT_F32) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) sum[P * 32 + i] = lo == 0 ? __uint_as_float(v[i]) : sum[P * 32 + i] + __uint_as_float(v[i]);
+                    } else {
+                        float o[32];
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = EXPERTS ? __uint_as_float(v[i]) * mul : __uint_as_float(v[i]);
+                        if constexpr (EPI == EPI_GATED) {
+                            gate_pairs<32>(o, g.act, g.limit);
+                        } else if (g.act == ACT_RELU2) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = act_of(o[i], ACT_RELU2);
+                        }
+                        constexpr int R = EPI == EPI_GATED ? 16 : 32;
+                        if constexpr (OUT == OUT_FP8) {
+#pragma unroll
+                            for (int i = 0; i < R; ++i) sum[P * R + i] = o[i];
+                        } else {
+                            constexpr int S = EPI == EPI_GATED ? P * 2 : P % 2 * 4;
+#pragma unroll
+                            for (int i = 0; i < R / 8; ++i) packed[S + i] = pack_bf16(o + 8 * i);
+                        }
+                    }
+                    // plain results in bfloat16 go out 32 at a time where they are read back to front, else 64
+                    if constexpr (OUT == OUT_BF16 && EPI == EPI_STORE) {
+                        if (P % 2 == 1 || as == 0) {
+                            if (as == 0) {
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) stage16(room, lane, i, packed[P % 2 * 4 + i]);
+                                flush(std::integral_constant<int, 64>{}, P * 32, 2, g.y_wide);
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) stage16(room, lane, i, packed[i]);
+                                flush(std::integral_constant<int, 128>{}, P * 32 - 32, 2, g.y_wide);
+                            }
+                        }
+                    }
+                };
+                uint32_t u[32], v[32];
+                if (as == 0) {
+                    tmem_ld32(acc + 96, u);
+                    walk<1, 0>(acc, u, v, there, use);
+                } else {
+                    tmem_ld32(acc, u);
+                    walk<0, 0>(acc, u, v, there, use);
+                }
             }
             if (!ok) break;
-            if (OUT == OUT_F32) {
-                if (EXPERTS) {
+            if constexpr (OUT == OUT_BF16 && EPI == EPI_GATED) {
 #pragma unroll
-                    for (int i = 0; i < 128; ++i) sum[i] *= mul;
-                }
-                constexpr int W = EPI == EPI_GATED ? 64 : 128;
-                if (EPI == EPI_GATED) {
+                for (int i = 0; i < 8; ++i) stage16(room, lane, i, packed[i]);
+                flush(std::integral_constant<int, 128>{}, 0, 2, g.y_wide);
+            }
+            if constexpr (OUT == OUT_F32) {
 #pragma unroll
-                    for (int i = 0; i < 64; ++i) sum[i] = fast_gate_pair(sum[2 * i], sum[2 * i + 1], g.act, g.limit);
-                } else {
+                for (int c = 0; c < 128; c += 32) {
+                    float o[32];
 #pragma unroll
-                    for (int i = 0; i < 128; ++i) sum[i] = act_of(sum[i], g.act);
-                }
+                    for (int i = 0; i < 32; ++i) o[i] = EXPERTS ? sum[c + i] * mul : sum[c + i];
+                    if constexpr (EPI == EPI_GATED) {
+                        gate_pairs<32>(o, g.act, g.limit);
+                    } else if (g.act == ACT_RELU2) {
 #pragma unroll
-                for (int c = 0; c < W; c += 32) {
-                    const int col = nt * OUT_COLS + half * W + c;
+                        for (int i = 0; i < 32; ++i) o[i] = act_of(o[i], ACT_RELU2);
+                    }
+                    constexpr int R = EPI == EPI_GATED ? 16 : 32;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        stage16(room, lane, i, make_uint4(__float_as_uint(sum[c + 4 * i]), __float_as_uint(sum[c + 4 * i + 1]), __float_as_uint(sum[c + 4 * i + 2]), __float_as_uint(sum[c + 4 * i + 3])));
-                    flush_rows<128>(room, lane, valid && col < g.N ? (uint8_t*)((float*)g.y + at * g.ldy + col) : nullptr, 4 * (g.N - col), g.y_wide, 4);
+                    for (int i = 0; i < R / 4; ++i)
+                        stage16(room, lane, i, make_uint4(__float_as_uint(o[4 * i]), __float_as_uint(o[4 * i + 1]), __float_as_uint(o[4 * i + 2]), __float_as_uint(o[4 * i + 3])));
+                    flush(std::integral_constant<int, 4 * R>{}, c * R / 32, 4, g.y_wide);
                 }
             }
-            if (OUT == OUT_FP8) {
-                constexpr int W = EPI == EPI_GATED ? 64 : 128;
-                const int col = nt * OUT_COLS + half * W;
+            if constexpr (OUT == OUT_FP8) {
                 uint32_t most = 0;
 #pragma unroll
                 for (int i = 0; i < W; ++i) {
                     if (col + i >= g.N) sum[i] = 0.0f;          // columns of no output are no part of the block
                     most = max(most, __float_as_uint(sum[i]) & 0x7fffffffu);
                 }
-                if (EPI == EPI_GATED) {                         // the block's other half is another warp's
-                    most_of[half * 128 + trow] = most;
-                    asm volatile("bar.sync 1, 256;" ::: "memory");
-                    most = max(most, most_of[(half ^ 1) * 128 + trow]);
-                    asm volatile("bar.sync 1, 256;" ::: "memory");
+                if constexpr (EPI == EPI_GATED) {               // the block's other half is another warp's
+                    // (two rooms in turn; a wait with a limit like all others: the other warp may have given up)
+                    uint32_t* here = most_of + (local & 1) * 256 + quarter * 32 + lane;
+                    here[half * 128] = most;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(halves0 + 8 * quarter);
+                    const bool both = wait_on(halves0 + 8 * quarter, (local & 1) ^ 1, give_up, 7);
+                    if (!__all_sync(0xffffffffu, both)) { ok = false; break; }
+                    most = max(most, here[(half ^ 1) * 128]);
                 }
                 const uint32_t byte = scale_byte(most);
                 const float inv = byte == 255u ? 1.0f : scale_inverse(byte);
@@ -431,12 +487,12 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                     stage16(room, lane, i / 16, q);
                 }
                 // (a row's bytes are a multiple of 16)
-                flush_rows<W>(room, lane, valid && col < g.N ? (uint8_t*)g.y + at * g.ldy + col : nullptr, (int)g.ldy - col, true, 2);
-                if (valid && col < g.N) {
+                flush(std::integral_constant<int, W>{}, 0, 1, true);
+                if (lane < rows && col < g.N && (EPI != EPI_GATED || half == 0)) {
                     const int b = col >> 7;
                     // scales by the row's tile: rows of the matrix (dense), rows of the list's tile (experts)
-                    const long s_row = EXPERTS ? (long)mt * PM + rank * BM + trow : row;
-                    if (EPI != EPI_GATED || half == 0) g.y_scales[scale_at(s_row, b >> 2, g.y_quads) + (b & 3)] = (uint8_t)byte;
+                    const long s_row = EXPERTS ? (long)mt * PM + rank * BM + quarter * 32 + lane : first + lane;
+                    g.y_scales[scale_at(s_row, b >> 2, g.y_quads) + (b & 3)] = (uint8_t)byte;
                 }
             }
         }
@@ -447,7 +503,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     if (warp == 1) tmem_dealloc_pair(tmem, TMEM_COLS);
 }
 
-constexpr size_t SMEM_BYTES = (size_t)STAGES * (STAGE_BYTES + SCALES) + ROOM_BYTES + (2 * STAGES + 6) * 8 + 16 + ROWS_BYTES;
+constexpr size_t SMEM_BYTES = (size_t)STAGES * (STAGE_BYTES + SCALES) + ROOM_BYTES + (2 * STAGES + 10) * 8 + 16 + ROWS_BYTES;
 
 // a matrix of scale tiles: rows of 512 bytes
 int make_map_scales(CUtensorMap* map, const void* ptr, long long tiles) {

@@ -208,26 +208,53 @@ __global__ void __launch_bounds__(THREADS) gather_kernel(RowsArgs g, const int32
     pdl_trigger();
 }
 
+__device__ __forceinline__ void store4(float* p, const float (&v)[4]) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+__device__ __forceinline__ void store4(bf16* p, const float (&v)[4]) {
+    uint2 u;
+    __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&u);
+    h[0] = __floats2bfloat162_rn(v[0], v[1]);
+    h[1] = __floats2bfloat162_rn(v[2], v[3]);
+    *reinterpret_cast<uint2*>(p) = u;
+}
+
 // out[t] = sum over t's choices, in their order, of weight * y[choice][t]; those that are no expert's give nothing.
 template <typename T>
 __global__ void __launch_bounds__(THREADS) combine_kernel(const float* __restrict__ y, const int32_t* __restrict__ ids, const float* __restrict__ weights,
-                                                          int top, int experts, int tokens, int cols, T* __restrict__ out, long ldo, int wide) {
+                                                          int top, int experts, int tokens, int cols, T* __restrict__ out, long ldo, int wide, int out_wide) {
     pdl_wait();
     const int t = blockIdx.x, c = (blockIdx.y * THREADS + threadIdx.x) * 4;
     if (c < cols) {
         float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int k = 0; k < top; ++k) {
-            const int e = ids[(long)t * top + k];
-            if (e < 0 || e >= experts) continue;
-            const float w = weights ? weights[(long)t * top + k] : 1.0f;
-            const float* row = y + ((long)k * tokens + t) * cols + c;
-            if (wide) {
-                const float4 v = *reinterpret_cast<const float4*>(row);
-                acc[0] = fmaf(w, v.x, acc[0]); acc[1] = fmaf(w, v.y, acc[1]); acc[2] = fmaf(w, v.z, acc[2]); acc[3] = fmaf(w, v.w, acc[3]);
-            } else {
+        for (int k0 = 0; k0 < top; k0 += 4) {                  // four choices' numbers on their way at a time
+            float4 v[4];
+            float w[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) if (c + i < cols) acc[i] = fmaf(w, row[i], acc[i]);
+            for (int j = 0; j < 4; ++j) {
+                const int k = k0 + j, e = k < top ? ids[(long)t * top + k] : -1;
+                v[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                w[j] = 0.0f;
+                if (e < 0 || e >= experts) continue;
+                w[j] = weights ? weights[(long)t * top + k] : 1.0f;
+                const float* row = y + ((long)k * tokens + t) * cols + c;
+                if (wide) {
+                    v[j] = *reinterpret_cast<const float4*>(row);
+                } else {
+                    v[j].x = row[0];
+                    if (c + 1 < cols) v[j].y = row[1];
+                    if (c + 2 < cols) v[j].z = row[2];
+                    if (c + 3 < cols) v[j].w = row[3];
+                }
             }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                acc[0] = fmaf(w[j], v[j].x, acc[0]); acc[1] = fmaf(w[j], v[j].y, acc[1]);
+                acc[2] = fmaf(w[j], v[j].z, acc[2]); acc[3] = fmaf(w[j], v[j].w, acc[3]);
+            }
+        }
+        if (out_wide) {
+            store4(out + (long)t * ldo + c, acc);
+            pdl_trigger();
+            return;
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) if (c + i < cols) out[(long)t * ldo + c + i] = from_float<T>(acc[i]);
@@ -332,9 +359,10 @@ BROLM_API int brolm_fp8_combine(const CombineCall* c) {
     const dim3 grid(c->tokens, (c->cols + 4 * THREADS - 1) / (4 * THREADS)), block(THREADS);
     if (grid.y > 65535) return BROLM_ERR_TOO_LARGE;
     const int wide = c->cols % 4 == 0 && ((uintptr_t)c->y & 15) == 0;
+    const int out_wide = c->cols % 4 == 0 && c->ldo % 4 == 0 && ((uintptr_t)c->out & 15) == 0;
     const float *y = (const float*)c->y, *w = (const float*)c->weights;
     const int32_t* ids = (const int32_t*)c->ids;
     if (c->out_f32)
-        return launch_pdl(combine_kernel<float>, grid, block, 0, c->stream, y, ids, w, c->top, c->experts, c->tokens, c->cols, (float*)c->out, (long)c->ldo, wide);
-    return launch_pdl(combine_kernel<bf16>, grid, block, 0, c->stream, y, ids, w, c->top, c->experts, c->tokens, c->cols, (bf16*)c->out, (long)c->ldo, wide);
+        return launch_pdl(combine_kernel<float>, grid, block, 0, c->stream, y, ids, w, c->top, c->experts, c->tokens, c->cols, (float*)c->out, (long)c->ldo, wide, out_wide);
+    return launch_pdl(combine_kernel<bf16>, grid, block, 0, c->stream, y, ids, w, c->top, c->experts, c->tokens, c->cols, (bf16*)c->out, (long)c->ldo, wide, out_wide);
 }

@@ -162,7 +162,7 @@ def fp8_read(m: Fp8Matrix, out: torch.Tensor) -> None:
 STREAM_ROWS = 128        # up to as many rows W is streamed; more are tiles of 256 x 256
 FUSED_ROWS = 16          # up to as many rows the stream of W can round the rows itself ...
 _FUSED_BLOCKS = 24       # ... where a block keeps no more than as many blocks of K of them
-_PIECE = 16              # blocks of K that a float32 result is summed over before the sum goes to registers
+_PIECE = 32              # blocks of K that a float32 result is summed over before the sum goes to registers
 _ACTS = {(gated, name): code for gated, table in ((True, ACTIVATIONS), (False, EXPERT_ACTS)) for name, code in table.items()}
 
 
