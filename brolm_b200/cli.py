@@ -46,6 +46,7 @@ def main(argv=None) -> int:
     ap.add_argument("--stop-id", type=int, action="append", default=[], help="further stop token (may be repeated)")
     ap.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
     ap.add_argument("--cache-dtype", choices=["int8"], help="keep keys and values in 8 bits (default: in --dtype)")
+    ap.add_argument("--weight-dtype", choices=["fp8"], help="keep the layers' matrices in 8-bit floating point (default: as they are)")
     ap.add_argument("--batch", type=int, default=0, help="most requests run together (default: as the cache allows)")
     ap.add_argument("--device", default="cuda:0")
     args = ap.parse_args(argv)
@@ -83,11 +84,11 @@ def main(argv=None) -> int:
         t0 = time.time()
         if args.model:
             print(f"[load] model: {args.model}")
-            model = bb.load_model(args.model, dtype=args.dtype, device=args.device)
+            model = bb.load_model(args.model, dtype=args.dtype, device=args.device, weight_dtype=args.weight_dtype)
         else:
             cfg = bb.load_config(args.config) if args.config else bb.Gemma2Config()
             print(f"[load] random weights, seed {args.weights_seed}")
-            model = bb.Model(cfg, dtype=args.dtype, device=args.device).init_random(args.weights_seed, on_device=True)
+            model = bb.Model(cfg, dtype=args.dtype, device=args.device, weight_dtype=args.weight_dtype).init_random(args.weights_seed, on_device=True)
         cfg = model.config
         lay = model.layout
         print(f"[info] {type(cfg).architecture}: hidden={lay.embedding.hidden} layer runs={len(lay.schedule)} "

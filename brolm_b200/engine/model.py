@@ -35,7 +35,13 @@ def as_dtype(d) -> torch.dtype:
 
 class DecoderModel:
     def __init__(self, config: ModelConfig, dtype="bfloat16", device="cuda:0",
-                 layout: Optional[ModelLayout] = None):
+                 layout: Optional[ModelLayout] = None, weight_dtype=None):
+        """``weight_dtype``: None (weights as they are loaded) or "fp8": the matrices of attention, latent attention,
+        feed-forwards and routed experts are kept in 8-bit floating point with a scale for every 128 numbers of a row, and
+        meet rows rounded the same way; embedding, output matrix, routers, norms and other mixers stay as they are."""
+        if weight_dtype not in (None, "fp8"):
+            raise ValueError(f"unknown weight_dtype {weight_dtype!r} (None or 'fp8')")
+        self.weight_dtype = weight_dtype
         self.config = config
         self.dtype = as_dtype(dtype)
         self.device = torch.device(device)
@@ -136,6 +142,8 @@ class DecoderModel:
                                missing=[head.tensor])
         for part, names in self._tensor_names:
             part.bind({local: tensors[ck] for local, ck in names.items() if local in part.param_specs()})
+            if self.weight_dtype == "fp8":
+                part.to_fp8()
         self.loaded = True
         self.generation += 1
 
@@ -230,11 +238,12 @@ class DecoderModel:
         return logits
 
 
-def load_model(folder: str, dtype="bfloat16", device="cuda:0") -> DecoderModel:
-    """Folder with config.json and safetensors -> a loaded model of the class config.json names."""
+def load_model(folder: str, dtype="bfloat16", device="cuda:0", weight_dtype=None) -> DecoderModel:
+    """Folder with config.json and safetensors -> a loaded model of the class config.json names; ``weight_dtype="fp8"``: its
+    matrices in 8-bit floating point."""
     from .. import models  # noqa: F401  (registers the architectures)
     config = load_config(folder)
-    return DecoderModel(config, dtype, device).load_weights(folder)
+    return DecoderModel(config, dtype, device, weight_dtype=weight_dtype).load_weights(folder)
 
 
 def write_random_model(config: ModelConfig, folder: str, seed: int = 0, weight_std: Optional[float] = None,

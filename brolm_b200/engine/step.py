@@ -339,6 +339,8 @@ class Engine:
                       "gemm_stream": kernels.gemm_stream_status(reset=True),
                       "grouped_tc": kernels.grouped_tc_status(reset=True),
                       "attn_kv8_tc": kernels.attention_kv8_tc_status(reset=True)}
+        if self.model.weight_dtype == "fp8":
+            codes |= {"fp8_stream": kernels.fp8_stream_status(reset=True), "fp8_gemm": kernels.fp8_gemm_status(reset=True)}
         self._checked_at = launched
         wrong = []
         for g in self.cache.kv_groups if self.cache.int8 else ():

@@ -101,6 +101,7 @@ def distance_buckets(rows: int, far: float) -> list:
 class Attention(Part):
     kind = "mixer"
     graph_safe = True
+    fp8_matrices = ("w_qkv", "w_o")
 
     def __init__(self, hidden: int, n_q: int, n_kv: int, head_dim: int, scale: float, softcap: float = 0.0,
                  window: Optional[int] = None, position: Optional[Part] = None, v_dim: Optional[int] = None,
@@ -282,12 +283,13 @@ class Attention(Part):
         cos_sin = self.position.table if self.position is not None else None
         int8 = entry.group.int8
         kept = (k_pages, v_pages, ctx.cache_rows[entry.group_id]) if writes_cache and not int8 else (None, None, None)
-        if kernels.skinny_ok(x, self.w_qkv) and (cos_sin is None or rot == self.head_dim):
+        fp8 = isinstance(self.w_qkv, kernels.Fp8Matrix)
+        if not fp8 and kernels.skinny_ok(x, self.w_qkv) and (cos_sin is None or rot == self.head_dim):
             # a few tokens: the rotation and the write into the cache are the product's epilogue
             qkv = torch.empty((x.shape[0], self.q_dim + 2 * self.kv_dim), dtype=ctx.dtype, device=x.device)
             kernels.skinny_qkv_rope(x, self.w_qkv, qkv, ctx.positions, cos_sin, self.n_q, self.n_kv, self.head_dim,
                                     *kept, page)
-        elif kernels.stream_rows(x, self.w_qkv) and (cos_sin is None or rot == self.head_dim):
+        elif not fp8 and kernels.stream_rows(x, self.w_qkv) and (cos_sin is None or rot == self.head_dim):
             # 17 to 32 tokens: the weights stream once through tcgen05, cut along K so that every SM takes
             # part; the kernel that rotates q and k and fills the cache adds the slices on its way
             slices = kernels.gemm_stream_parts(x, self.w_qkv)

@@ -15,6 +15,8 @@ from typing import Any, Optional
 
 import torch
 
+from .. import kernels
+
 KINDS = ("mixer", "feedforward", "norm", "position", "block", "stream")
 
 
@@ -43,6 +45,8 @@ class Part:
     # True when it can keep its keys and values in 8 bits (mixers): it then finds a cache entry of that kind, and steps may
     # bring several tokens to a sequence that holds some already.
     int8_cache: bool = False
+    # The matrices, by attribute, that it can keep in 8-bit floating point: each meets its rows in ``linear``.
+    fp8_matrices: tuple = ()
     # True when it forks a branch of a captured step onto the context's second stream.
     branches: bool = False
 
@@ -54,6 +58,13 @@ class Part:
         """Take the loaded tensors (already on the device, in their kept
         element type).  A part may fuse or re-lay them out here."""
         self.params = params
+
+    def to_fp8(self) -> None:
+        """Keep the matrices in 8-bit floating point from here on (after ``bind``)."""
+        for name in self.fp8_matrices:
+            w = getattr(self, name, None)
+            if w is not None:
+                setattr(self, name, kernels.fp8_quantize(w))
 
     def cache_spec(self) -> Optional[Any]:
         """What the part keeps per sequence between steps (mixers only)."""

@@ -103,7 +103,7 @@ class Block(Part):
         tokens are so few that the host sets the pace."""
         m, f = self.mixer, self.feedforward
         norms = [self.post_mixer_norm, self.pre_ffn_norm, self.post_ffn_norm] + ([next_norm] if next_norm is not None else [])
-        if type(m) is not Attention or type(f) is not GatedFeedForward or m.headwise or m.rowwise or not x.is_contiguous() \
+        if type(m) is not Attention or type(f) is not GatedFeedForward or isinstance(m.w_qkv, kernels.Fp8Matrix) or m.headwise or m.rowwise or not x.is_contiguous() \
                 or (m.position is not None and m.position.rotary_dim != m.head_dim) \
                 or any(type(n) is not RMSNorm or n.groups != 1 for n in norms) \
                 or norms[0].weight.dtype != norms[1].weight.dtype or norms[2].weight.dtype != norms[-1].weight.dtype:

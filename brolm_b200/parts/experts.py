@@ -22,7 +22,8 @@ class RoutedExperts(Part):
     tiles of each expert's pairs -> float results [top, tokens, hidden], which the residual kernel
     adds in the order of the choices.  Nothing is read back to the host.  With many pairs per expert (a
     prompt) the products run on tcgen05 over 128-row tiles, the tokens' rows first copied into expert order;
-    with few (decoding) on mma.sync over 64-row tiles, as a stream of the chosen experts' matrices.
+    with few (decoding) on mma.sync over 64-row tiles, as a stream of the chosen experts' matrices.  With matrices
+    in 8-bit floating point both are ``kernels.experts_fp8_pairs``.
 
     Options beside those (any of them selects the second form of the pass, ``_forward_weighted``):
 
@@ -131,6 +132,12 @@ class RoutedExperts(Part):
             self.w_down = torch.stack([params[f"e{e}.down"] for e in range(self.experts)]).contiguous()
         self.params = {}
 
+    def to_fp8(self):
+        if self.experts:
+            n = self.inter
+            self.w_up = kernels.fp8_gate_up(self.w_up[:, :n], self.w_up[:, n:]) if self.gated else kernels.fp8_quantize(self.w_up)
+            self.w_down = kernels.fp8_quantize(self.w_down)
+
     def _route(self, x: torch.Tensor, ids: torch.Tensor, gates: torch.Tensor) -> None:
         n = self.router.shape[0]
         if x.dtype == torch.bfloat16 and x.shape[0] >= self.ROUTER_PRODUCT_ROWS and n <= 1024 and self.hidden % 8 == 0:
@@ -151,7 +158,11 @@ class RoutedExperts(Part):
         gates = torch.empty((T, self.top), dtype=torch.float32, device=dev)
         self._route(x, ids, gates)
         y = None
-        if E:
+        if E and isinstance(self.w_up, kernels.Fp8Matrix):
+            # (choices of identity experts are no expert's there: they have no result)
+            y = torch.empty((self.top, T, self.hidden), dtype=torch.float32, device=dev)
+            kernels.experts_fp8_pairs(x, ids, self.w_up, self.w_down, y, self.activation, self.limit)
+        elif E:
             # pairs that chose an identity expert are in no group; their places in perm stay zero
             perm = torch.zeros(pairs, dtype=torch.int32, device=dev)
             offsets = torch.empty(E + 1, dtype=torch.int32, device=dev)
@@ -198,6 +209,10 @@ class RoutedExperts(Part):
             kernels.route_pick(linear(x, self.router, out_dtype=torch.float32), self.top, ids, gates)
         else:
             kernels.route_topk(x, self.router, self.top, ids, gates)
+        if isinstance(self.w_up, kernels.Fp8Matrix):
+            y = torch.empty((self.top, T, self.hidden), dtype=torch.float32, device=dev)
+            kernels.experts_fp8_pairs(x, ids, self.w_up, self.w_down, y, self.activation, scale=gates)
+            return y
         perm = torch.empty(pairs, dtype=torch.int32, device=dev)
         offsets = torch.empty(self.experts + 1, dtype=torch.int32, device=dev)
         u = torch.empty((pairs, self.inter), dtype=x.dtype, device=dev)

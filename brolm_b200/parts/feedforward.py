@@ -37,8 +37,16 @@ class GatedFeedForward(Part):
         self.w_down = params["down"]
         self.params = {}
 
+    def to_fp8(self):
+        self.w_gate_up = kernels.fp8_gate_up(self.w_gate_up[:self.inter], self.w_gate_up[self.inter:])
+        self.w_down = kernels.fp8_quantize(self.w_down)
+
     def forward(self, x: torch.Tensor, ctx) -> torch.Tensor:
         """x (tokens, hidden) -> (tokens, hidden) float32."""
+        if isinstance(self.w_gate_up, kernels.Fp8Matrix):
+            y = torch.empty((x.shape[0], self.hidden), dtype=torch.float32, device=x.device)
+            kernels.feedforward_fp8(x, self.w_gate_up, self.w_down, y, self.activation, self.limit)
+            return y
         act = torch.empty((x.shape[0], self.inter), dtype=ctx.dtype, device=x.device)
         if ctx.dtype == torch.float32 and kernels.linear_f32_tc_ok(self.w_gate_up) and x.dtype == self.w_gate_up.dtype == torch.float32:
             # float: the activation is the product's last step
@@ -71,6 +79,7 @@ class DenseFeedForward(Part):
 
     kind = "feedforward"
     graph_safe = True
+    fp8_matrices = ("w_up", "w_down")
 
     def __init__(self, hidden: int, inter: int, activation: str = "relu2", bias: bool = True):
         if activation not in kernels.ROW_ACTS:

@@ -48,6 +48,7 @@ def _round_up(n: int, m: int) -> int:
 class LatentAttention(Part):
     kind = "mixer"
     graph_safe = True
+    fp8_matrices = ("w_in", "w_uq", "w_o")
 
     def __init__(self, hidden: int, heads: int, dim: int, rot_dim: int, vdim: int, kv_rank: int, scale: float,
                  eps: float, window: Optional[int] = None, sink: bool = True, position: Optional[Part] = None,
@@ -104,6 +105,7 @@ class LatentAttention(Part):
         if self.has_gate:
             rows.append(params["g"])
         self.w_in = torch.cat(rows, dim=0).contiguous()
+        self.in_dtype = self.w_in.dtype
         self.gain = params["dkv_norm"].contiguous() if not self.borrows_kv else None
         self.w_uq = params["uq"].contiguous() if self.q_rank else None
         self.q_gain = params["dq_norm"].contiguous() if self.q_rank else None
@@ -128,8 +130,8 @@ class LatentAttention(Part):
                                       "one without them on a cache of its own")
         pages, _, table, ring, page = ctx.kv(entry)
         T, H, D = x.shape[0], self.heads, self.row
-        if x.dtype != self.w_in.dtype:
-            x = x.to(self.w_in.dtype)
+        if x.dtype != self.in_dtype:
+            x = x.to(self.in_dtype)
         proj = linear(x, self.w_in, out_dtype=x.dtype)
         pos = self.position
         own = not self.borrows_kv

@@ -2,6 +2,8 @@
 (wlejon/brolm include/brolm/detail/compute.h:49-86 dispatches on the weight's
 element type in the same way).
 
+* weight in 8-bit floating point (``kernels.Fp8Matrix``): the framework's tcgen05
+  products with scales, the rows rounded to 8 bits on the way.
 * float32 weight: the framework's own kernels: for large weights tcgen05 on
   floats taken apart into three bfloat16 numbers, which hold all their bits,
   CUDA cores for the others.
@@ -36,6 +38,12 @@ def linear(x: torch.Tensor, weight: torch.Tensor, out_dtype: Optional[torch.dtyp
     does); the result may then be [parts, M, N] float32, the slices of a
     product that was cut along K so that more blocks stream the weights."""
     M = x.shape[0]
+    if isinstance(weight, kernels.Fp8Matrix):
+        if x.dtype not in (torch.bfloat16, torch.float32):
+            x = x.float()
+        y = out if out is not None else torch.empty((M, weight.outputs), dtype=out_dtype or x.dtype, device=x.device)
+        kernels.linear_fp8(x, weight, y)
+        return y
     N = weight.shape[0]
     if weight.dtype == torch.float32:
         x32 = x if x.dtype == torch.float32 else x.float()

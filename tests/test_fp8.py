@@ -64,3 +64,12 @@ def test_refusals():
         kernels.linear_fp8(_matrix(3, 256), fp8._empty((2, 64, 256), "cpu"), torch.zeros(3, 64))
     with pytest.raises(kernels.KernelError, match="two matrices"):
         kernels.fp8_gate_up(torch.zeros(4, 8), torch.zeros(4, 9))
+
+
+def test_model_refuses_other_types():
+    import brolm_b200 as bb
+    from tests.helpers import TINY_A
+    with pytest.raises(ValueError, match="weight_dtype"):
+        bb.Model(bb.Gemma2Config(**TINY_A), device="cpu", weight_dtype="int4")
+    with pytest.raises(kernels.KernelError, match="CUDA"):
+        bb.Model(bb.Gemma2Config(**TINY_A), device="cpu", weight_dtype="fp8").init_random(0)
