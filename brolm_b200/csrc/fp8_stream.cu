@@ -22,6 +22,8 @@
 // Every mbarrier wait is bounded (tcgen05.cuh).
 #include "fp8_round.cuh"
 
+#include <type_traits>
+
 namespace {
 
 using namespace tc;
@@ -85,7 +87,7 @@ __device__ __forceinline__ void cluster_sync_all() {
 }
 __device__ __forceinline__ float peer_float(uint32_t addr, uint32_t rank) {
     float v;
-    asm volatile("{\n.reg .b32 r;\nmapa.shared::cluster.u32 r, %1, %2;\nld.shared::cluster.f32 %0, [r];\n}" : "=f"(v) : "r"(addr), "r"(rank) : "memory");
+    asm volatile("{\n.reg .b32 r;\nmapa.shared::cluster.u32 r, %1, %2;\nld.shared::cluster.f32 %0, [r];\n}" : "=f"(v) : "r"(addr), "r"(rank));
     return v;
 }
 __device__ __forceinline__ float act_of(float v, int act) {
@@ -103,30 +105,50 @@ __device__ __forceinline__ void put(const StreamArgs& g, long at, float v) {
 // The rows of X of this block's slice of K, in 8 bits as the products want them: row r of block kb at r * 128 bytes of its
 // X_BYTES, its sixteen-byte pieces swapped as a TMA load with the 128-byte swizzle would leave them; scales in tiles of four
 // blocks.  A warp takes four blocks of a row at a time and asks for four such pieces before it rounds the first.
-template <typename T, int BT>
+template <typename T, int BT, bool WIDE>
 __device__ __forceinline__ void round_rows(const StreamArgs& g, uint8_t* x_blocks, uint8_t* x_scales, int lo, int hi, int w, int lane) {
-    constexpr int DEEP = 4;
+    constexpr int DEEP = 4, WORDS = (int)sizeof(T);             // sixteen numbers are 2 or 4 sixteen-byte words
     const int q0 = lo >> 2, n = ((hi + 3) >> 2) - q0, tasks = n * g.M;
     for (int t0 = w; t0 < tasks; t0 += 8 * DEEP) {
-        float v[DEEP][16];
+        uint4 raw[DEEP][WORDS];
+        int row[DEEP], quad[DEEP];
 #pragma unroll
         for (int d = 0; d < DEEP; ++d) {
-            const int t = t0 + 8 * d, r = t / n, q = q0 + t - r * n, c = q * 512 + lane * 16;
-            if (t < tasks) {
-                if (g.x_wide) load16<true>((const T*)g.x + r * g.ldx, c, g.K, v[d]);
-                else load16<false>((const T*)g.x + r * g.ldx, c, g.K, v[d]);
-            }
+            const int t = t0 + 8 * d;
+            row[d] = t / n;
+            quad[d] = t - row[d] * n;
+            const int c = (q0 + quad[d]) * 512 + lane * 16;
+            const uint4* src = reinterpret_cast<const uint4*>((const T*)g.x + row[d] * g.ldx + c);
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i) raw[d][i] = WIDE && t < tasks && c + 16 <= g.K ? src[i] : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
         for (int d = 0; d < DEEP; ++d) {
-            const int t = t0 + 8 * d, r = t / n, q = t - r * n, kb = (q0 + q) * 4 + (lane >> 3);
-            if (t < tasks) {                                    // (the same for the whole warp)
-                uint32_t word;
-                const uint4 u = round16(v[d], word);
-                if (kb >= lo && kb < hi)
-                    *reinterpret_cast<uint4*>(x_blocks + (kb - lo) * (BT * BK) + r * BK + (((lane & 7) ^ (r & 7)) << 4)) = u;
-                if (lane == 0) *reinterpret_cast<uint32_t*>(x_scales + q * SF_TILE + r * 16) = word;
+            if (t0 + 8 * d >= tasks) break;                     // (the same for the whole warp)
+            const int c = (q0 + quad[d]) * 512 + lane * 16, kb = (q0 + quad[d]) * 4 + (lane >> 3);
+            float v[16];
+            if (WIDE && c + 16 <= g.K) {
+#pragma unroll
+                for (int i = 0; i < WORDS; ++i) {
+                    const uint32_t u[4] = {raw[d][i].x, raw[d][i].y, raw[d][i].z, raw[d][i].w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (WORDS == 2) {
+                            v[8 * i + 2 * j] = __uint_as_float(u[j] << 16);
+                            v[8 * i + 2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
+                        } else {
+                            v[4 * i + j] = __uint_as_float(u[j]);
+                        }
+                    }
+                }
+            } else {
+                load16<false>((const T*)g.x + row[d] * g.ldx, c, g.K, v);
             }
+            uint32_t word;
+            const uint4 u = round16(v, word);
+            if (kb >= lo && kb < hi)
+                *reinterpret_cast<uint4*>(x_blocks + (kb - lo) * (BT * BK) + row[d] * BK + (((lane & 7) ^ (row[d] & 7)) << 4)) = u;
+            if (lane == 0) *reinterpret_cast<uint32_t*>(x_scales + quad[d] * SF_TILE + row[d] * 16) = word;
         }
     }
 }
@@ -149,7 +171,7 @@ struct Shape {
 };
 
 template <int BT, int EPI, bool EXPERTS, int FUSED>
-__global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS) fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w,
+__global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS, 2) fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w,
                                                              const __grid_constant__ CUtensorMap map_x, StreamArgs g) {
     using S = Shape<BT, FUSED>;
     constexpr int ACCS = S::ACCS;
@@ -249,7 +271,7 @@ __global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS) fp8_stream_kernel(c
             }
             int s = it % stages, phase = (it / stages) & 1;
             while (more) {
-                if (!wait_on(empty0 + 8 * s, phase ^ 1, give_up, 1)) break;
+                if (!(kb > lo ? wait_one(empty0 + 8 * s, phase ^ 1, give_up, 1) : wait_on(empty0 + 8 * s, phase ^ 1, give_up, 1))) break;
                 load_w(s, rt, group, kb);
                 load_x(s, row0, tile, kb);
                 ++it;
@@ -309,8 +331,9 @@ __global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS) fp8_stream_kernel(c
         if (EXPERTS) pdl_wait();
         if (FUSED) {
             pdl_wait();
-            if (FUSED == 1) round_rows<bf16, BT>(g, x_blocks, x_scales, lo, hi, warp - 2, lane);
-            else round_rows<float, BT>(g, x_blocks, x_scales, lo, hi, warp - 2, lane);
+            using T = typename std::conditional<FUSED == 1, bf16, float>::type;
+            if (g.x_wide) round_rows<T, BT, true>(g, x_blocks, x_scales, lo, hi, warp - 2, lane);
+            else round_rows<T, BT, false>(g, x_blocks, x_scales, lo, hi, warp - 2, lane);
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(x_ready);
@@ -387,8 +410,11 @@ __global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS) fp8_stream_kernel(c
             const uint32_t mine = smem_u32(sums);
             const int t = threadIdx.x - 64, rt = first;
             for (int r = slice; r < g.M; r += slices) {
-                float v = 0.0f;
-                for (int k = 0; k < slices; ++k) v += peer_float(mine + (r * BR + t) * 4, k);
+                float part[8], v = 0.0f;                        // (asked for together, added in their order)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) part[k] = k < slices ? peer_float(mine + (r * BR + t) * 4, k) : 0.0f;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) if (k < slices) v += part[k];
                 int col = rt * BR + t;
                 if (EPI == EPI_GATED) {
                     const float up = __shfl_down_sync(0xffffffffu, v, 1);
