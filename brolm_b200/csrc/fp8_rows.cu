@@ -2,12 +2,6 @@
 //
 //   fp8_quantize   rows of float or bfloat16 numbers -> e4m3 numbers and a scale byte for every 128 of them
 //   fp8_read       the values that they stand for
-//   fp8_group      (token, choice) pairs sorted by expert, and the list of the experts' tiles of rows
-//   fp8_gather     the pairs' rows in that order in 8 bits
-//   fp8_combine    a token's results, multiplied by their weights and added
-//
-// The first two are one pass over the data: a warp takes four blocks of a row at a time (512 numbers, one word of scales), eight
-// lanes a block and sixteen numbers a lane; the block's largest magnitude goes round its eight lanes in three shuffles.
 #include "fp8_round.cuh"
 
 namespace {
@@ -27,19 +21,27 @@ struct RowsArgs {
     int early;                      // the next kernel may begin before this one's results are there
 };
 
+// The row of the matrix that row r of x is.
+__device__ __forceinline__ long place_of(const RowsArgs& g, long r) { return g.group == g.group_pad ? r : r / g.group * g.group_pad + r % g.group; }
+
+// A warp has four blocks of a row at a time.  8,192 x 4,608 bfloat16 numbers take 24.8 us, 4.6 TB/s where a copy of them runs at
+// 5.5; two or four rows at a time (26.8, 28.6 us) or the next one's numbers asked for ahead (24.8 to 26.1) gained nothing.
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(THREADS) quantize_kernel(RowsArgs g) {
     const int lane = threadIdx.x & 31;
     const long items = g.rows * g.quads;
     pdl_wait();
     for (long item = (long)blockIdx.x * WARPS + (threadIdx.x >> 5); item < items; item += (long)gridDim.x * WARPS) {
-        const long row = item / g.quads;
+        const long row = items <= 0xffffffffl ? (long)((uint32_t)item / (uint32_t)g.quads) : item / g.quads;    // (a long division is 70 instructions)
         const int quad = (int)(item - row * g.quads), c = quad * 512 + lane * 16;
-        const long at = g.group == g.group_pad ? row : row / g.group * g.group_pad + row % g.group;
+        const T* x = (const T*)g.x + row * g.ldx;
+        Piece<T, WIDE> piece;
+        piece.ask(x, c, g.cols, true);
         float v[16];
-        load16<WIDE>((const T*)g.x + row * g.ldx, c, g.cols, v);
+        piece.get(x, c, g.cols, v);
         uint32_t word;
         const uint4 q = round16(v, word);
+        const long at = place_of(g, row);
         if (c < g.ldv) *reinterpret_cast<uint4*>(g.values + at * g.ldv + c) = q;     // ldv is a multiple of 16
         if (lane == 0) *reinterpret_cast<uint32_t*>(g.scales + scale_at(at, quad, g.quads)) = word;
     }
@@ -48,225 +50,67 @@ __global__ void __launch_bounds__(THREADS) quantize_kernel(RowsArgs g) {
     if (g.early) pdl_trigger();
 }
 
-template <typename T> __device__ __forceinline__ void store16(T* row, int c, int cols, const float (&v)[16], bool wide);
-template <> __device__ __forceinline__ void store16<float>(float* row, int c, int cols, const float (&v)[16], bool wide) {
-    if (wide && c + 16 <= cols) {
+// For reading back the lanes' words lie side by side: eight bfloat16 numbers or four floats a word of sixteen bytes.  (With
+// sixteen numbers a lane 8,192 x 4,608 floats took 44.7 us for 30.8.)
+template <typename T>
+struct Lay {
+    static constexpr int WORDS = (int)sizeof(T);                 // words of sixteen bytes a lane
+    static constexpr int EACH = 16 / (int)sizeof(T);             // numbers of a word
+    static constexpr int LANES = BLOCK / EACH;                   // lanes of a block
+    // the first column, from the piece's first on, of this lane's word i
+    static __device__ __forceinline__ int column(int i, int lane) { return i * 32 * EACH + lane * EACH; }
+};
+__device__ __forceinline__ void store_wide(float* to, const float (&v)[4]) { *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]); }
+__device__ __forceinline__ void store_wide(bf16* to, const float (&v)[8]) {
+    uint4 p;
+    __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&p);
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(row + c + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) if (c + i < cols) row[c + i] = v[i];
-}
-template <> __device__ __forceinline__ void store16<bf16>(bf16* row, int c, int cols, const float (&v)[16], bool wide) {
-    if (wide && c + 16 <= cols) {
-#pragma unroll
-        for (int i = 0; i < 16; i += 8) {
-            uint4 p;
-            __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&p);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) h[e] = __floats2bfloat162_rn(v[i + 2 * e], v[i + 2 * e + 1]);
-            *reinterpret_cast<uint4*>(row + c + i) = p;
-        }
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) if (c + i < cols) row[c + i] = __float2bfloat16_rn(v[i]);
+    for (int e = 0; e < 4; ++e) h[e] = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+    *reinterpret_cast<uint4*>(to) = p;
 }
 
 template <typename T>
 __global__ void __launch_bounds__(THREADS) read_kernel(RowsArgs g, T* __restrict__ y, long ldy, bool wide) {
-    const int lane = threadIdx.x & 31;
-    const long items = g.rows * g.quads;
+    using L = Lay<T>;
+    const int lane = threadIdx.x & 31, quad = blockIdx.x, c0 = quad * 512;
     pdl_wait();
-    for (long item = (long)blockIdx.x * WARPS + (threadIdx.x >> 5); item < items; item += (long)gridDim.x * WARPS) {
-        const long row = item / g.quads;
-        const int quad = (int)(item - row * g.quads), c = quad * 512 + lane * 16;
-        const long at = g.group == g.group_pad ? row : row / g.group * g.group_pad + row % g.group;
-        if (c >= g.cols) continue;
-        const uint4 q = *reinterpret_cast<const uint4*>(g.values + at * g.ldv + c);
-        const float s = scale_value(g.scales[scale_at(at, quad, g.quads) + (lane >> 3)]);
-        const uint32_t words[4] = {q.x, q.y, q.z, q.w};
-        float v[16];
+    for (long row = (long)blockIdx.y * WARPS + (threadIdx.x >> 5); row < g.rows; row += (long)gridDim.y * WARPS) {
+        const long at = place_of(g, row);
+        const uint32_t scales = *reinterpret_cast<const uint32_t*>(g.scales + scale_at(at, quad, g.quads));
+        uint32_t q[L::WORDS][L::EACH / 4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            uint32_t lo, hi;                     // e4m3 numbers are f16 numbers
-            asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %2;\ncvt.rn.f16x2.e4m3x2 %0, a;\ncvt.rn.f16x2.e4m3x2 %1, b;\n}" : "=r"(lo), "=r"(hi) : "r"(words[i]));
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&lo)), h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-            v[4 * i] = f.x * s; v[4 * i + 1] = f.y * s; v[4 * i + 2] = h.x * s; v[4 * i + 3] = h.y * s;
+        for (int i = 0; i < L::WORDS; ++i) {
+            const int c = c0 + L::column(i, lane);
+#pragma unroll
+            for (int j = 0; j < L::EACH / 4; ++j) q[i][j] = c < g.ldv ? *reinterpret_cast<const uint32_t*>(g.values + at * g.ldv + c + 4 * j) : 0u;
         }
-        store16<T>(y + row * ldy, c, g.cols, v, wide);
+#pragma unroll
+        for (int i = 0; i < L::WORDS; ++i) {
+            const int c = c0 + L::column(i, lane);
+            const float s = scale_value((scales >> (8 * (i * (32 / L::LANES) + lane / L::LANES))) & 255u);
+            float v[L::EACH];
+#pragma unroll
+            for (int j = 0; j < L::EACH / 4; ++j) {
+                uint32_t lo, hi;                     // e4m3 numbers are f16 numbers
+                asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %2;\ncvt.rn.f16x2.e4m3x2 %0, a;\ncvt.rn.f16x2.e4m3x2 %1, b;\n}" : "=r"(lo), "=r"(hi) : "r"(q[i][j]));
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&lo)), h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+                v[4 * j] = f.x * s; v[4 * j + 1] = f.y * s; v[4 * j + 2] = h.x * s; v[4 * j + 3] = h.y * s;
+            }
+            if (wide && c + L::EACH <= g.cols) {
+                store_wide(y + row * ldy + c, v);
+            } else {
+#pragma unroll
+                for (int j = 0; j < L::EACH; ++j) if (c + j < g.cols) y[row * ldy + c + j] = from_float<T>(v[j]);
+            }
+        }
     }
     pdl_trigger();
 }
 
-// The pairs sorted by expert, by one block: counts of the experts, their first rows by a scan, every pair's place by a counter in
-// shared memory (which of an expert's pairs comes first is left open: a pair's result hangs on its own row alone).  A choice
-// that is no expert's is in no group.  scale_row: of row s of the order, where its scales lie (row r of tile t of the list:
-// `pad` t + r, pad being the tile's rows rounded up to 128); -1 behind the last row.
-__global__ void __launch_bounds__(1024) group_kernel(const int32_t* __restrict__ ids, int P, int E, int tile_rows, int pad,
-                                                     int32_t* __restrict__ perm, int32_t* __restrict__ scale_row,
-                                                     int32_t* __restrict__ offsets, int32_t* __restrict__ tile_group,
-                                                     int32_t* __restrict__ tile_row0, int max_tiles) {
-    extern __shared__ int sh[];                        // counts (then places) [E], first rows [E + 1], first tiles [E + 1]
-    int *counts = sh, *starts = sh + E, *tiles = starts + E + 1;
-    __shared__ int carry[2][33];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int e = threadIdx.x; e < E; e += 1024) counts[e] = 0;
-    __syncthreads();
-    pdl_wait();
-    for (int p = threadIdx.x; p < P; p += 1024) {
-        const int e = ids[p];
-        if (e >= 0 && e < E) atomicAdd(&counts[e], 1);
-    }
-    __syncthreads();
-    int rows_before = 0, tiles_before = 0;
-    for (int e0 = 0; e0 < E; e0 += 1024) {
-        const int e = e0 + threadIdx.x, n = e < E ? counts[e] : 0, t = (n + tile_rows - 1) / tile_rows;
-        int a = n, b = t;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int x = __shfl_up_sync(0xffffffffu, a, o), y = __shfl_up_sync(0xffffffffu, b, o);
-            if (lane >= o) { a += x; b += y; }
-        }
-        if (lane == 31) { carry[0][warp] = a; carry[1][warp] = b; }
-        __syncthreads();
-        if (warp == 0) {
-            int x = carry[0][lane], y = carry[1][lane];
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int u = __shfl_up_sync(0xffffffffu, x, o), v = __shfl_up_sync(0xffffffffu, y, o);
-                if (lane >= o) { x += u; y += v; }
-            }
-            carry[0][lane] = x; carry[1][lane] = y;
-        }
-        __syncthreads();
-        if (e < E) {
-            starts[e] = rows_before + a - n + (warp ? carry[0][warp - 1] : 0);
-            tiles[e] = tiles_before + b - t + (warp ? carry[1][warp - 1] : 0);
-            offsets[e] = starts[e];
-        }
-        rows_before += carry[0][31];
-        tiles_before += carry[1][31];
-        __syncthreads();
-    }
-    if (threadIdx.x == 0) {
-        starts[E] = offsets[E] = rows_before;
-        tiles[E] = tiles_before;
-    }
-    __syncthreads();
-    for (int t = threadIdx.x; t < max_tiles; t += 1024) {
-        int group = -1, row0 = 0;
-        if (t < tiles_before) {
-            int lo = 0, hi = E;                        // the last expert whose first tile is not behind t and that has one
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) / 2;
-                if (tiles[mid] <= t) lo = mid; else hi = mid;
-            }
-            group = lo;
-            row0 = starts[lo] + (t - tiles[lo]) * tile_rows;
-        }
-        tile_group[t] = group;
-        tile_row0[t] = row0;
-    }
-    for (int e = threadIdx.x; e < E; e += 1024) counts[e] = 0;
-    __syncthreads();
-    for (int p = threadIdx.x; p < P; p += 1024) {
-        const int e = ids[p];
-        if (e >= 0 && e < E) {
-            const int r = atomicAdd(&counts[e], 1), s = starts[e] + r;
-            perm[s] = p;
-            scale_row[s] = (tiles[e] + r / tile_rows) * pad + r % tile_rows;
-        }
-    }
-    for (int s = rows_before + threadIdx.x; s < P; s += 1024) {
-        perm[s] = 0;
-        scale_row[s] = -1;
-    }
-    pdl_trigger();
+unsigned rows_grid(long long rows) {
+    const long long blocks = (rows + WARPS - 1) / WARPS;
+    return (unsigned)(blocks < 65535 ? blocks : 65535);
 }
-
-// Row s of the order: the row perm[s] / top of x (top 0: row s itself) in 8 bits.
-template <typename T, bool WIDE>
-__global__ void __launch_bounds__(THREADS) gather_kernel(RowsArgs g, const int32_t* __restrict__ perm, const int32_t* __restrict__ scale_row, int top) {
-    const int lane = threadIdx.x & 31;
-    const long items = g.rows * g.quads;
-    pdl_wait();
-    for (long item = (long)blockIdx.x * WARPS + (threadIdx.x >> 5); item < items; item += (long)gridDim.x * WARPS) {
-        const long s = item / g.quads;
-        const int quad = (int)(item - s * g.quads), c = quad * 512 + lane * 16;
-        const int place = scale_row[s];
-        if (place < 0) continue;
-        const long row = top ? perm[s] / top : s;
-        float v[16];
-        load16<WIDE>((const T*)g.x + row * g.ldx, c, g.cols, v);
-        uint32_t word;
-        const uint4 q = round16(v, word);
-        if (c < g.ldv) *reinterpret_cast<uint4*>(g.values + s * g.ldv + c) = q;
-        if (lane == 0) *reinterpret_cast<uint32_t*>(g.scales + scale_at(place, quad, g.quads)) = word;
-    }
-    pdl_trigger();
-}
-
-__device__ __forceinline__ void store4(float* p, const float (&v)[4]) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
-__device__ __forceinline__ void store4(bf16* p, const float (&v)[4]) {
-    uint2 u;
-    __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&u);
-    h[0] = __floats2bfloat162_rn(v[0], v[1]);
-    h[1] = __floats2bfloat162_rn(v[2], v[3]);
-    *reinterpret_cast<uint2*>(p) = u;
-}
-
-// out[t] = sum over t's choices, in their order, of weight * y[choice][t]; those that are no expert's give nothing.
-template <typename T>
-__global__ void __launch_bounds__(THREADS) combine_kernel(const float* __restrict__ y, const int32_t* __restrict__ ids, const float* __restrict__ weights,
-                                                          int top, int experts, int tokens, int cols, T* __restrict__ out, long ldo, int wide, int out_wide) {
-    pdl_wait();
-    const int t = blockIdx.x, c = (blockIdx.y * THREADS + threadIdx.x) * 4;
-    if (c < cols) {
-        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int k0 = 0; k0 < top; k0 += 4) {                  // four choices' numbers on their way at a time
-            float4 v[4];
-            float w[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int k = k0 + j, e = k < top ? ids[(long)t * top + k] : -1;
-                v[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                w[j] = 0.0f;
-                if (e < 0 || e >= experts) continue;
-                w[j] = weights ? weights[(long)t * top + k] : 1.0f;
-                const float* row = y + ((long)k * tokens + t) * cols + c;
-                if (wide) {
-                    v[j] = *reinterpret_cast<const float4*>(row);
-                } else {
-                    v[j].x = row[0];
-                    if (c + 1 < cols) v[j].y = row[1];
-                    if (c + 2 < cols) v[j].z = row[2];
-                    if (c + 3 < cols) v[j].w = row[3];
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                acc[0] = fmaf(w[j], v[j].x, acc[0]); acc[1] = fmaf(w[j], v[j].y, acc[1]);
-                acc[2] = fmaf(w[j], v[j].z, acc[2]); acc[3] = fmaf(w[j], v[j].w, acc[3]);
-            }
-        }
-        if (out_wide) {
-            store4(out + (long)t * ldo + c, acc);
-            pdl_trigger();
-            return;
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) if (c + i < cols) out[(long)t * ldo + c + i] = from_float<T>(acc[i]);
-    }
-    pdl_trigger();
-}
-
-int grid_for(long items) {
-    const long blocks = (items + WARPS - 1) / WARPS, most = 16L * tc::device_sms();
-    return (int)(blocks < most ? blocks : most);
-}
-
 }  // namespace
 
 // x [rows, cols] (float or bfloat16, ldx elements between rows) -> values (ldv bytes between rows, a multiple of 16, at least
@@ -277,7 +121,8 @@ BROLM_API int brolm_fp8_quantize(const fp8::RowsCall* c) {
     if (c->group <= 0 || c->group_pad < c->group) return BROLM_ERR_BAD_SIZE;
     RowsArgs g = {c->x, (long)c->ldx, (uint8_t*)c->values, (long)c->ldv, (uint8_t*)c->scales, (long)c->rows, c->cols, fp8::quads_of(c->cols),
                   c->group, c->group_pad, c->early};
-    const dim3 grid(grid_for(c->rows * g.quads)), block(THREADS);
+    const long long blocks = (c->rows * g.quads + WARPS - 1) / WARPS, most = 16LL * tc::device_sms();
+    const dim3 grid((unsigned)(blocks < most ? blocks : most)), block(THREADS);
     const bool base = ((uintptr_t)c->x & 15) == 0;
     if (c->dtype == BROLM_BF16) {
         if (base && c->ldx % 8 == 0) return launch_pdl(quantize_kernel<bf16, true>, grid, block, 0, c->stream, g);
@@ -294,7 +139,7 @@ BROLM_API int brolm_fp8_read(const fp8::RowsCall* c) {
     if (c->ldv % 16 != 0 || c->ldv < c->cols || ((uintptr_t)c->values & 15)) return BROLM_ERR_ALIGNMENT;
     if (c->group <= 0 || c->group_pad < c->group) return BROLM_ERR_BAD_SIZE;
     RowsArgs g = {nullptr, 0, (uint8_t*)c->values, (long)c->ldv, (uint8_t*)c->scales, (long)c->rows, c->cols, fp8::quads_of(c->cols), c->group, c->group_pad, 1};
-    const dim3 grid(grid_for(c->rows * g.quads)), block(THREADS);
+    const dim3 grid(g.quads, rows_grid(c->rows)), block(THREADS);
     const bool base = ((uintptr_t)c->x & 15) == 0;
     if (c->dtype == BROLM_BF16)
         return launch_pdl(read_kernel<bf16>, grid, block, 0, c->stream, g, (bf16*)c->x, (long)c->ldx, base && c->ldx % 8 == 0);
@@ -302,67 +147,3 @@ BROLM_API int brolm_fp8_read(const fp8::RowsCall* c) {
     return launch_pdl(read_kernel<float>, grid, block, 0, c->stream, g, (float*)c->x, (long)c->ldx, base && c->ldx % 4 == 0);
 }
 
-// ids [pairs] -> perm, scale_row [pairs], offsets [experts + 1], the list [max_tiles] (expert -1 behind its end).
-struct GroupCall {
-    const void* ids;
-    void *perm, *scale_row, *offsets, *tile_group, *tile_row0;
-    cudaStream_t stream;
-    int pairs, experts, tile_rows, max_tiles;
-};
-BROLM_API int brolm_fp8_group(const GroupCall* c) {
-    if (c->pairs <= 0) return BROLM_OK;
-    const int E = c->experts;
-    if (E <= 0 || E > 4096) return BROLM_ERR_TOO_LARGE;
-    if (c->tile_rows < 16 || c->max_tiles < (c->pairs + c->tile_rows - 1) / c->tile_rows + (E < c->pairs ? E : c->pairs)) return BROLM_ERR_BAD_SIZE;
-    static OncePerDevice done;
-    const int st = allow_shared_memory(group_kernel, (3 * 4096 + 2) * sizeof(int), done);
-    if (st) return st;
-    return launch_pdl(group_kernel, dim3(1), dim3(1024), (3 * (size_t)E + 2) * sizeof(int), c->stream, (const int32_t*)c->ids, c->pairs, E, c->tile_rows,
-                      (c->tile_rows + 127) / 128 * 128, (int32_t*)c->perm, (int32_t*)c->scale_row, (int32_t*)c->offsets, (int32_t*)c->tile_group,
-                      (int32_t*)c->tile_row0, c->max_tiles);
-}
-
-// The rows of the order in 8 bits: row perm[s] / top of x, or with top 0 row s of it.
-struct GatherCall {
-    const void *x, *perm, *scale_row;
-    void *values, *scales;
-    cudaStream_t stream;
-    long long ldx, ldv;
-    int dtype, top, pairs, cols;
-};
-BROLM_API int brolm_fp8_gather(const GatherCall* c) {
-    if (c->pairs <= 0 || c->cols <= 0) return BROLM_OK;
-    if (c->ldv % 16 != 0 || c->ldv < c->cols || ((uintptr_t)c->values & 15) || ((uintptr_t)c->scales & 15)) return BROLM_ERR_ALIGNMENT;
-    RowsArgs g = {c->x, (long)c->ldx, (uint8_t*)c->values, (long)c->ldv, (uint8_t*)c->scales, c->pairs, c->cols, fp8::quads_of(c->cols), 1, 1, 1};
-    const dim3 grid(grid_for((long)c->pairs * g.quads)), block(THREADS);
-    const int32_t *pm = (const int32_t*)c->perm, *sr = (const int32_t*)c->scale_row;
-    const bool base = ((uintptr_t)c->x & 15) == 0;
-    if (c->dtype == BROLM_BF16) {
-        if (base && c->ldx % 8 == 0) return launch_pdl(gather_kernel<bf16, true>, grid, block, 0, c->stream, g, pm, sr, c->top);
-        return launch_pdl(gather_kernel<bf16, false>, grid, block, 0, c->stream, g, pm, sr, c->top);
-    }
-    if (c->dtype != BROLM_F32) return BROLM_ERR_BAD_DTYPE;
-    if (base && c->ldx % 4 == 0) return launch_pdl(gather_kernel<float, true>, grid, block, 0, c->stream, g, pm, sr, c->top);
-    return launch_pdl(gather_kernel<float, false>, grid, block, 0, c->stream, g, pm, sr, c->top);
-}
-
-// y float [top, tokens, cols]; weights [tokens, top], or null for ones; out float or bfloat16.
-struct CombineCall {
-    const void *y, *ids, *weights;
-    void* out;
-    cudaStream_t stream;
-    long long ldo;
-    int top, experts, tokens, cols, out_f32;
-};
-BROLM_API int brolm_fp8_combine(const CombineCall* c) {
-    if (c->tokens <= 0 || c->cols <= 0) return BROLM_OK;
-    const dim3 grid(c->tokens, (c->cols + 4 * THREADS - 1) / (4 * THREADS)), block(THREADS);
-    if (grid.y > 65535) return BROLM_ERR_TOO_LARGE;
-    const int wide = c->cols % 4 == 0 && ((uintptr_t)c->y & 15) == 0;
-    const int out_wide = c->cols % 4 == 0 && c->ldo % 4 == 0 && ((uintptr_t)c->out & 15) == 0;
-    const float *y = (const float*)c->y, *w = (const float*)c->weights;
-    const int32_t* ids = (const int32_t*)c->ids;
-    if (c->out_f32)
-        return launch_pdl(combine_kernel<float>, grid, block, 0, c->stream, y, ids, w, c->top, c->experts, c->tokens, c->cols, (float*)c->out, (long)c->ldo, wide, out_wide);
-    return launch_pdl(combine_kernel<bf16>, grid, block, 0, c->stream, y, ids, w, c->top, c->experts, c->tokens, c->cols, (bf16*)c->out, (long)c->ldo, wide, out_wide);
-}

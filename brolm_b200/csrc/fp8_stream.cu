@@ -107,43 +107,25 @@ __device__ __forceinline__ void put(const StreamArgs& g, long at, float v) {
 // blocks.  A warp takes four blocks of a row at a time and asks for four such pieces before it rounds the first.
 template <typename T, int BT, bool WIDE>
 __device__ __forceinline__ void round_rows(const StreamArgs& g, uint8_t* x_blocks, uint8_t* x_scales, int lo, int hi, int w, int lane) {
-    constexpr int DEEP = 4, WORDS = (int)sizeof(T);             // sixteen numbers are 2 or 4 sixteen-byte words
+    constexpr int DEEP = 4;
     const int q0 = lo >> 2, n = ((hi + 3) >> 2) - q0, tasks = n * g.M;
+    const T* x = (const T*)g.x;
     for (int t0 = w; t0 < tasks; t0 += 8 * DEEP) {
-        uint4 raw[DEEP][WORDS];
+        Piece<T, WIDE> piece[DEEP];
         int row[DEEP], quad[DEEP];
 #pragma unroll
         for (int d = 0; d < DEEP; ++d) {
             const int t = t0 + 8 * d;
             row[d] = t / n;
             quad[d] = t - row[d] * n;
-            const int c = (q0 + quad[d]) * 512 + lane * 16;
-            const uint4* src = reinterpret_cast<const uint4*>((const T*)g.x + row[d] * g.ldx + c);
-#pragma unroll
-            for (int i = 0; i < WORDS; ++i) raw[d][i] = WIDE && t < tasks && c + 16 <= g.K ? src[i] : make_uint4(0, 0, 0, 0);
+            piece[d].ask(x + row[d] * g.ldx, (q0 + quad[d]) * 512 + lane * 16, g.K, t < tasks);
         }
 #pragma unroll
         for (int d = 0; d < DEEP; ++d) {
             if (t0 + 8 * d >= tasks) break;                     // (the same for the whole warp)
-            const int c = (q0 + quad[d]) * 512 + lane * 16, kb = (q0 + quad[d]) * 4 + (lane >> 3);
+            const int kb = (q0 + quad[d]) * 4 + (lane >> 3);
             float v[16];
-            if (WIDE && c + 16 <= g.K) {
-#pragma unroll
-                for (int i = 0; i < WORDS; ++i) {
-                    const uint32_t u[4] = {raw[d][i].x, raw[d][i].y, raw[d][i].z, raw[d][i].w};
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if (WORDS == 2) {
-                            v[8 * i + 2 * j] = __uint_as_float(u[j] << 16);
-                            v[8 * i + 2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
-                        } else {
-                            v[4 * i + j] = __uint_as_float(u[j]);
-                        }
-                    }
-                }
-            } else {
-                load16<false>((const T*)g.x + row[d] * g.ldx, c, g.K, v);
-            }
+            piece[d].get(x + row[d] * g.ldx, (q0 + quad[d]) * 512 + lane * 16, g.K, v);
             uint32_t word;
             const uint4 u = round16(v, word);
             if (kb >= lo && kb < hi)
@@ -328,9 +310,8 @@ __global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS, 2) fp8_stream_kerne
     } else {
         const int quarter = warp & 3;
         const int lrow = quarter * 32 + lane;                   // row of the tile of W = lane of tensor memory
-        if (EXPERTS) pdl_wait();
+        if (EXPERTS || FUSED) pdl_wait();
         if (FUSED) {
-            pdl_wait();
             using T = typename std::conditional<FUSED == 1, bf16, float>::type;
             if (g.x_wide) round_rows<T, BT, true>(g, x_blocks, x_scales, lo, hi, warp - 2, lane);
             else round_rows<T, BT, false>(g, x_blocks, x_scales, lo, hi, warp - 2, lane);
@@ -438,7 +419,8 @@ int launch(const CUtensorMap& mw, const CUtensorMap& mx, StreamArgs g, int slice
     using S = Shape<BT, FUSED>;
     const int sms = device_sms();
     const bool split = slices > 1;
-    // Two blocks an SM: one streams while the other starts or ends, and clusters of up to eight find room.
+    // Two blocks an SM: one streams while the other starts or ends, and clusters of up to eight find room.  (Three with 74 KB,
+    // where experts' items fill their rounds better, gained nothing.)
     constexpr size_t ROOM = 112 * 1024;
     int stages = MAX_STAGES;
     while (stages > 2 && S::smem(stages, g.per) > ROOM) --stages;

@@ -62,9 +62,11 @@ LIBRARIES: dict[str, list[str]] = {
     "fp8_rows": ["fp8_rows.cu"],
     "fp8_stream": ["fp8_stream.cu"],
     "fp8_gemm": ["fp8_gemm.cu"],
+    "fp8_experts": ["fp8_experts.cu"],
 }
 HEADERS = ["common.cuh", "once_per_device.h", "attn_mma.cuh", "attn_decode_noalloc.h", "tcgen05.cuh", "kv8.cuh", "attn_kv8_join.cuh"]
-OWN_HEADERS = {"fp8_rows": ["fp8.cuh", "fp8_round.cuh"], "fp8_stream": ["fp8.cuh", "fp8_round.cuh"], "fp8_gemm": ["fp8.cuh"]}       # hashed with those libraries alone
+OWN_HEADERS = {"fp8_rows": ["fp8.cuh", "fp8_round.cuh"], "fp8_stream": ["fp8.cuh", "fp8_round.cuh"], "fp8_gemm": ["fp8.cuh"],
+               "fp8_experts": ["fp8.cuh", "fp8_round.cuh"]}       # hashed with those libraries alone
 
 _loaded: dict[str, ctypes.CDLL] = {}
 _lock = threading.Lock()

@@ -18,12 +18,12 @@ from __future__ import annotations
 
 import functools
 import struct
-from ctypes import c_char_p, c_int
+from ctypes import c_char_p, c_int, c_void_p, cast
 from typing import Optional
 
 import torch
 
-from . import ACTIVATIONS, EXPERT_ACTS, KernelError, _check, _fn, device_sms, library_loaded, load_library
+from . import ACTIVATIONS, EXPERT_ACTS, KernelError, _check, _fn, add_launches, device_sms, library_loaded, load_library
 
 BLOCK = 128              # numbers that share a scale
 _TILE = 512              # bytes of scales of 128 rows and four blocks
@@ -39,10 +39,9 @@ _raw_stream, _device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDev
 # out only then.
 _ROWS = struct.Struct("@4P3q5i")
 _PRODUCT = struct.Struct("@7P3q8ifi5P6i")
-_GROUP = struct.Struct("@6PP4i")
-_GATHER = struct.Struct("@6P2q4i")
-_COMBINE = struct.Struct("@5Pq5i")
+_EXPERTS = struct.Struct("@13P5q14if")
 _functions: dict = {}
+_products: dict = {}         # the launchers that a pass of experts is given
 
 
 def _call(lib: str, name: str, packed: bytes, what: str) -> None:
@@ -54,25 +53,35 @@ def _call(lib: str, name: str, packed: bytes, what: str) -> None:
 
 class Fp8Matrix:
     """Rows of 8-bit numbers.  ``shape``: (rows, columns) or (experts, rows, columns).  ``gated``: the rows of a gate and of its
-    partner alternate, so that a product has half as many results as there are rows.  ``values``: uint8 [rows of all experts,
-    columns rounded up to 16], an expert's matrix beginning on a multiple of 128 rows; ``scales``: uint8 [rows / 128, columns /
-    512, 512].  It is not to be changed once it is in use."""
-    __slots__ = ("values", "scales", "shape", "gated", "rows", "cols", "outputs", "group_rows", "device", "index", "packed")
+    partner alternate, so that a product has half as many results as there are rows.  It is not to be changed once it is in
+    use.  ``data`` holds ``values``, uint8 [rows of all experts, columns rounded up to 16], an expert's matrix beginning on a
+    multiple of 128 rows, and behind them ``scales``, uint8 [rows / 128, columns / 512, 512]."""
+    __slots__ = ("data", "shape", "gated", "rows", "cols", "outputs", "group_rows", "total", "device", "index", "packed")
 
-    def __init__(self, values: torch.Tensor, scales: torch.Tensor, shape: tuple, gated: bool = False):
-        self.values, self.scales, self.shape, self.gated = values, scales, tuple(shape), bool(gated)
-        self.rows, self.cols = self.shape[-2], self.shape[-1]
+    def __init__(self, data: torch.Tensor, shape: tuple, gated: bool = False):
+        self.data, self.shape, self.gated = data, shape, gated
+        self.rows, self.cols = rows, cols = shape[-2], shape[-1]
         # how many results a row's product with this matrix has
-        self.outputs = self.rows // 2 if self.gated else self.rows
-        # rows that an expert's matrix takes
-        self.group_rows = values.shape[0] // max(self.shape[0], 1) if len(self.shape) == 3 else self.rows
-        self.device = values.device
-        self.index = values.get_device()
-        self.packed = (values.data_ptr(), scales.data_ptr(), values.stride(0))
+        self.outputs = rows >> 1 if gated else rows
+        # rows that an expert's matrix takes, and all of them
+        self.group_rows = rows if len(shape) == 2 else (rows + 127) & -128
+        self.total = rows if len(shape) == 2 else shape[0] * self.group_rows
+        self.device = data.device
+        self.index = data.get_device()
+        at, ld = data.data_ptr(), (cols + 15) & -16
+        self.packed = (at, at + ((self.total * ld + 511) & -512), ld)
+
+    @property
+    def values(self) -> torch.Tensor:
+        return self.data[:self.total * self.packed[2]].view(self.total, self.packed[2])
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self.data[self.packed[1] - self.packed[0]:].view((self.total + 127) >> 7, (self.cols + 511) >> 9, _TILE)
 
     @property
     def nbytes(self) -> int:
-        return self.values.numel() + self.scales.numel()
+        return self.data.numel()
 
     def __repr__(self) -> str:
         return f"Fp8Matrix({self.shape}, gated={self.gated}, {self.device})"
@@ -82,21 +91,21 @@ def _round_up(n: int, m: int) -> int:
     return (n + m - 1) // m * m
 
 
+def _bytes(rows: int, cols: int, scale_rows: int) -> int:
+    return ((rows * ((cols + 15) & -16) + 511) & -512) + ((scale_rows + 127) >> 7) * ((cols + 511) >> 9) * _TILE
+
+
 def _empty(shape: tuple, device, gated: bool = False) -> Fp8Matrix:
-    rows, cols = shape[-2:]
-    total = rows if len(shape) == 2 else shape[0] * _round_up(rows, 128)
-    values = torch.empty((total, _round_up(cols, 16)), dtype=torch.uint8, device=device)
-    scales = torch.empty(((total + 127) // 128, (cols + 511) // 512, _TILE), dtype=torch.uint8, device=device)
-    return Fp8Matrix(values, scales, tuple(shape), gated)
+    rows = shape[0] if len(shape) == 2 else shape[0] * _round_up(shape[1], 128)
+    return Fp8Matrix(torch.empty(_bytes(rows, shape[-1], rows), dtype=torch.uint8, device=device), shape, gated)
 
 
 def _scratch(rows: int, cols: int, device, scale_rows: Optional[int] = None) -> tuple:
     """Room for rows in 8 bits within one call: what keeps it alive, and values, scales and stride as a launcher takes them."""
     ld = (cols + 15) & -16
-    begin = (rows * ld + 511) & -512
-    held = torch.empty(begin + (((scale_rows or rows) + 127) >> 7) * ((cols + 511) >> 9) * _TILE, dtype=torch.uint8, device=device)
+    held = torch.empty(_bytes(rows, cols, scale_rows or rows), dtype=torch.uint8, device=device)
     at = held.data_ptr()
-    return held, (at, at + begin, ld)
+    return held, (at, at + ((rows * ld + 511) & -512), ld)
 
 
 def _refuse(what: str, t: torch.Tensor, name: str, dim: int = 2) -> None:
@@ -122,17 +131,17 @@ def _quantize(x: torch.Tensor, packed: tuple, group: int, pad: int, early: int) 
 def fp8_quantize(x: torch.Tensor) -> Fp8Matrix:
     """x [rows, columns] or [experts, rows, columns], float32 or bfloat16, packed rows (any stride between them; a stack of
     experts contiguous) -> the same in 8 bits."""
+    what = "fp8_quantize"
     if not isinstance(x, torch.Tensor) or x.dim() not in (2, 3) or x.shape[-1] == 0:
-        raise KernelError(f"fp8_quantize: rows or a stack of matrices are wanted, not {tuple(getattr(x, 'shape', ()))}")
-    _refuse("fp8_quantize", x, "x", x.dim())
-    if x.dim() == 3 and not x.is_contiguous():
-        raise KernelError("fp8_quantize: a stack of matrices must be contiguous")
-    m = _empty(tuple(x.shape), x.device)
+        raise KernelError(f"{what}: rows or a stack of matrices are wanted, not {tuple(getattr(x, 'shape', ()))}")
+    shape = tuple(x.shape)
+    if x.dtype not in _CODES or x.get_device() < 0 or x.get_device() != _device() or x.stride(-1) != 1:
+        _refuse(what, x, "x", len(shape))
+    if len(shape) == 3 and not x.is_contiguous():
+        raise KernelError(f"{what}: a stack of matrices must be contiguous")
+    m = _empty(shape, x.device)
     if x.numel():
-        if x.dim() == 3:
-            _quantize(x.view(-1, x.shape[-1]), m.packed, m.rows, m.group_rows, 0)
-        else:
-            _quantize(x, m.packed, m.rows, m.rows, 0)
+        _quantize(x.view(-1, shape[-1]) if len(shape) == 3 else x, m.packed, m.rows, m.group_rows, 0)
     return m
 
 
@@ -141,7 +150,7 @@ def fp8_gate_up(gate: torch.Tensor, up: torch.Tensor) -> Fp8Matrix:
     if gate.shape != up.shape or gate.dtype != up.dtype or gate.device != up.device:
         raise KernelError(f"fp8_gate_up: two matrices of a kind are wanted, not {tuple(gate.shape)} {gate.dtype} and {tuple(up.shape)} {up.dtype}")
     m = fp8_quantize(torch.stack((gate, up), dim=-2).flatten(-3, -2))
-    return Fp8Matrix(m.values, m.scales, m.shape, True)
+    return Fp8Matrix(m.data, m.shape, True)
 
 
 def fp8_read(m: Fp8Matrix, out: torch.Tensor) -> None:
@@ -286,6 +295,13 @@ def experts_fp8_rows(pairs: int, experts: int) -> int:
 
 
 def _experts_checked(what: str, x, ids, up: Fp8Matrix, down: Fp8Matrix, scale) -> None:
+    device = x.get_device()
+    if x.dtype in _CODES and device >= 0 and device == _device() and x.dim() == 2 and ids.dim() == 2 and x.stride(1) == 1 \
+            and len(up.shape) == 3 and len(down.shape) == 3 and not down.gated and up.shape[0] == down.shape[0] <= 4096 and up.outputs == down.cols \
+            and x.shape[1] == up.cols and ids.shape[0] == x.shape[0] and ids.dtype == torch.int32 and ids.is_contiguous() \
+            and device == ids.get_device() == up.index == down.index \
+            and (scale is None or (scale.dtype == _F32 and scale.shape == ids.shape and scale.is_contiguous() and scale.get_device() == device)):
+        return
     _refuse(what, x, "x")
     if len(up.shape) != 3 or len(down.shape) != 3 or down.gated or up.shape[0] != down.shape[0] or up.outputs != down.cols:
         raise KernelError(f"{what}: stacks of shapes {up.shape} and {down.shape} do not follow one another")
@@ -302,6 +318,41 @@ def _experts_checked(what: str, x, ids, up: Fp8Matrix, down: Fp8Matrix, scale) -
             raise KernelError(f"{what}: tensors on {x.device} and {t.device}")
 
 
+def _experts(what: str, x, ids, up: Fp8Matrix, down: Fp8Matrix, pairs, out, activation: str, limit: float, scale, weights) -> None:
+    act = _act_code(what, up, activation)
+    E, (T, top), K, inter, N = up.shape[0], ids.shape, up.cols, down.cols, down.rows
+    P = T * top
+    if not P or not E or not N:
+        return
+    rows = experts_fp8_rows(P, E)
+    most = (P + rows - 1) // rows + min(E, P)
+    up512 = lambda n: (n + 511) & -512
+    # the order and the list; the rows of both products in 8 bits with a tile of scales for every tile of the list; floats between
+    need = 3 * up512(4 * P) + up512(4 * E + 4) + 2 * up512(4 * most)
+    for cols in (K, inter):
+        need += up512(P * ((cols + 15) & -16)) + ((rows + 127) >> 7) * most * ((cols + 511) >> 9) * _TILE
+    if rows <= STREAM_ROWS:
+        need += up512(4 * P * inter)
+    held = None
+    if pairs is None:
+        held = torch.empty(need + 4 * P * N, dtype=torch.uint8, device=x.device)
+        y = held.data_ptr() + need
+    else:
+        held, y = torch.empty(need, dtype=torch.uint8, device=x.device), pairs.data_ptr()
+    lib = "fp8_stream" if rows <= STREAM_ROWS else "fp8_gemm"
+    product = _products.get(lib)
+    if product is None:
+        product = _products[lib] = cast(getattr(load_library(lib), "brolm_" + lib), c_void_p).value
+    pack = _EXPERTS.pack(x.data_ptr(), ids.data_ptr(), scale.data_ptr() if scale is not None else 0, weights.data_ptr() if weights is not None else 0,
+                         up.packed[0], up.packed[1], down.packed[0], down.packed[1], y, out.data_ptr() if out is not None else 0, held.data_ptr(),
+                         _raw_stream(x.get_device()), product, x.stride(0), up.packed[2], down.packed[2], out.stride(0) if out is not None else 0, need,
+                         _CODES[x.dtype], T, top, E, K, inter, N, up.group_rows, down.group_rows, 1 if up.gated else 0, act, rows, _PIECE,
+                         1 if out is not None and out.dtype == _F32 else 0, limit)
+    _call("fp8_experts", "brolm_fp8_experts", pack, what)
+    # (a call counts as one launch: the others of this pass)
+    add_launches((1 if P > 256 or E > 256 else 0) + 2 + (1 if rows <= STREAM_ROWS else 0) + (1 if out is not None else 0))
+
+
 def experts_fp8_pairs(x: torch.Tensor, ids: torch.Tensor, up: Fp8Matrix, down: Fp8Matrix, out: torch.Tensor, activation: str = "silu",
                       limit: float = 0.0, scale: Optional[torch.Tensor] = None) -> None:
     """Every (token, choice) pair through its expert: out float32 [top, tokens, down.rows], a pair's result at [its choice, its
@@ -310,42 +361,9 @@ def experts_fp8_pairs(x: torch.Tensor, ids: torch.Tensor, up: Fp8Matrix, down: F
     sums before the activation."""
     what = "experts_fp8"
     _experts_checked(what, x, ids, up, down, scale)
-    E, (T, top), dev = up.shape[0], ids.shape, x.device
-    if tuple(out.shape) != (top, T, down.rows) or out.dtype != _F32 or not out.is_contiguous() or out.device != dev:
-        raise KernelError(f"{what}: the pairs' results are a packed float32 {(top, T, down.rows)} on {dev}")
-    act = _act_code(what, up, activation)
-    P, K, inter, N = T * top, x.shape[1], up.outputs, down.rows
-    if not P or not E or not N:
-        return
-    rows = experts_fp8_rows(P, E)
-    pad = _round_up(rows, 128)
-    most = (P + rows - 1) // rows + min(E, P)
-    # the order and the list of tiles
-    lists = torch.empty(2 * P + E + 1 + 2 * most, dtype=torch.int32, device=dev)
-    perm = lists.data_ptr()
-    place = perm + 4 * P
-    offsets = place + 4 * P
-    group = offsets + 4 * (E + 1)
-    row0 = group + 4 * most
-    stream = _raw_stream(_device())
-    _call("fp8_rows", "brolm_fp8_group", _GROUP.pack(ids.data_ptr(), perm, place, offsets, group, row0, stream, P, E, rows, most), what)
-    held, a = _scratch(P, K, dev, most * pad)
-    _call("fp8_rows", "brolm_fp8_gather", _GATHER.pack(x.data_ptr(), perm, place, a[0], a[1], stream, x.stride(0), a[2], _CODES[x.dtype], top, P, K), what)
-    held2, h = _scratch(P, inter, dev, most * pad)
-    lib, name = ("fp8_stream", "brolm_fp8_stream") if rows <= STREAM_ROWS else ("fp8_gemm", "brolm_fp8_gemm")
-
-    def product(m, w, y, kind, n, k, code, lim, s, last):
-        wv, ws, ldw = w.packed
-        _call(lib, name, _PRODUCT.pack(m[0], m[1], wv, ws, y[0], y[1], stream, m[2], ldw, y[2], P, n, k, 1 if w.gated else 0, code, kind, 0, _PIECE, lim, E,
-                                       group, row0, offsets, perm, s, w.group_rows, last, top, T, rows, most), what)
-    s = scale.data_ptr() if scale is not None else 0
-    if rows <= STREAM_ROWS:
-        sums = torch.empty((P, inter), dtype=_F32, device=dev)
-        product(a, up, (sums.data_ptr(), 0, inter), 1, inter, K, act, limit, s, 0)
-        _call("fp8_rows", "brolm_fp8_gather", _GATHER.pack(sums.data_ptr(), perm, place, h[0], h[1], stream, inter, h[2], 0, 0, P, inter), what)
-    else:
-        product(a, up, h, 2, inter, K, act, limit, s, 0)
-    product(h, down, (out.data_ptr(), 0, N), 1, N, inter, 0, 0.0, 0, 1)
+    if tuple(out.shape) != (ids.shape[1], x.shape[0], down.rows) or out.dtype != _F32 or not out.is_contiguous() or out.device != x.device:
+        raise KernelError(f"{what}: the pairs' results are a packed float32 {(ids.shape[1], x.shape[0], down.rows)} on {x.device}")
+    _experts(what, x, ids, up, down, out, None, activation, limit, scale, None)
 
 
 def experts_fp8(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, up: Fp8Matrix, down: Fp8Matrix, out: torch.Tensor, activation: str = "silu",
@@ -355,16 +373,14 @@ def experts_fp8(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, up: F
     the sums before the activation and not the result."""
     what = "experts_fp8"
     _experts_checked(what, x, ids, up, down, weights)
-    T, top = ids.shape
-    _refuse(what, out, "out")
-    if tuple(out.shape) != (T, down.rows):
-        raise KernelError(f"{what}: the result has the shape {(T, down.rows)}, not {tuple(out.shape)}")
-    y = torch.empty((top, T, down.rows), dtype=_F32, device=x.device)
-    experts_fp8_pairs(x, ids, up, down, y, activation, limit, weights if scale_input else None)
-    if not T or not down.rows:
+    if out.dtype not in _CODES or out.dim() != 2 or out.get_device() != x.get_device() or (out.stride(1) != 1 and down.rows > 1):
+        _refuse(what, out, "out")
+    if out.shape[0] != x.shape[0] or out.shape[1] != down.rows:
+        raise KernelError(f"{what}: the result has the shape {(x.shape[0], down.rows)}, not {tuple(out.shape)}")
+    if ids.shape[1] == 0 or up.shape[0] == 0:
+        out.zero_()
         return
-    _call("fp8_rows", "brolm_fp8_combine", _COMBINE.pack(y.data_ptr(), ids.data_ptr(), 0 if scale_input else weights.data_ptr(), out.data_ptr(),
-                                                         _raw_stream(_device()), out.stride(0), top, up.shape[0], T, down.rows, _CODES[out.dtype] ^ 1), what)
+    _experts(what, x, ids, up, down, None, out, activation, limit, weights if scale_input else None, None if scale_input else weights)
 
 
 def fp8_stream_status(reset: bool = False) -> int:
