@@ -75,6 +75,7 @@ template <int N>
 __device__ __forceinline__ void write_list(const int* starts, const int* tiles, int E, int tile_rows, int32_t* offsets, int32_t* tile_group,
                                            int32_t* tile_row0, int max_tiles) {
     for (int e = threadIdx.x; e <= E; e += N) offsets[e] = starts[e];
+    if (threadIdx.x == 0) offsets[E + 1] = tiles[E];
     for (int t = threadIdx.x; t < max_tiles; t += N) {
         int group = -1, row0 = 0;
         if (t < tiles[E]) {
@@ -92,61 +93,82 @@ __device__ __forceinline__ void write_list(const int* starts, const int* tiles, 
 }
 
 struct Lists {
-    int32_t *perm, *place, *scale_row, *offsets, *tile_group, *tile_row0;
+    int32_t *perm, *place, *scale_row, *offsets, *tile_group, *tile_row0;      // offsets[E + 1]: how many tiles there are
     int max_tiles, tile_rows, pad;
 };
 
-// The pairs sorted by expert, by one block.  Counters in shared memory give every pair its number among those of its expert
-// (four sets of them, each for eight warps, since a favoured expert's counter is where all wait); a scan gives the experts' first
-// rows and tiles; then every pair's place is known.  Which of an expert's pairs come first is left open: a pair's result hangs on
-// its own row alone.  A choice that is no expert's is in no group.  perm: the pair of a row of the order; place: the row of a
-// pair; scale_row: of row s of the order, where its scales lie (row r of tile t of the list: `pad` t + r, pad being the tile's
-// rows rounded up to 128); -1 behind the last row.  (Warps that first found their equal pairs by match.any took 11.5 us for 8,192
-// pairs, 80 for 32,768.)
-constexpr int SETS = 4;
-__global__ void __launch_bounds__(1024) group_kernel(const int32_t* __restrict__ ids, int P, int E, Lists g) {
-    extern __shared__ int sh[];                        // counters [SETS][E], counts [E], first rows [E + 1], first tiles [E + 1]
-    int *sets = sh, *counts = sh + SETS * E, *starts = counts + E, *tiles = starts + E + 1;
+// The pairs sorted by expert, by the eight blocks of a cluster.  Counters in shared memory give every pair its number among those
+// of its expert in its block; the blocks read one another's counters, and a scan gives the experts' first rows and tiles; then
+// every pair's place is known.  Which of an expert's pairs come first within a block is left open: a pair's result hangs on its
+// own row alone.  A choice that is no expert's is in no group.  perm: the pair of a row of the order; place: the row of a pair;
+// scale_row: of row s of the order, where its scales lie (row r of tile t of the list: `pad` t + r, pad being the tile's rows
+// rounded up to 128); -1 behind the last row.  What it takes is the scattered words that are written, two a pair: one block of
+// 1,024 threads took 8.8 us for 8,192 pairs and 37 for 32,768.
+constexpr int BLOCKS = 8;
+__device__ __forceinline__ int peer_int(const int* p, int rank) {
+    const uint32_t at = (uint32_t)__cvta_generic_to_shared(p);
+    int v;
+    asm volatile("{\n.reg .b32 r;\nmapa.shared::cluster.u32 r, %1, %2;\nld.shared::cluster.s32 %0, [r];\n}" : "=r"(v) : "r"(at), "r"(rank));
+    return v;
+}
+__device__ __forceinline__ void cluster_sync_all() {
+    asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
+}
+__global__ void __cluster_dims__(BLOCKS, 1, 1) __launch_bounds__(1024) group_kernel(const int32_t* __restrict__ ids, int P, int E, Lists g) {
+    extern __shared__ int sh[];                        // this block's counters [E], all blocks' [E], first rows [E + 1], first tiles [E + 1]
+    int *mine = sh, *counts = sh + E, *starts = counts + E, *tiles = starts + E + 1;
     __shared__ int carry[66];
-    int* mine = sets + (threadIdx.x >> 8) * E;
-    for (int e = threadIdx.x; e < SETS * E; e += 1024) sets[e] = 0;
+    const int rank = blockIdx.x;
+    for (int e = threadIdx.x; e < E; e += 1024) mine[e] = 0;
     __syncthreads();
     pdl_wait();
     auto id = [&](int p) {
         const int e = p < P ? ids[p] : -1;
         return e >= 0 && e < E ? e : -1;
     };
-    constexpr int DEEP = 8;
-    for (int p0 = threadIdx.x; p0 < P; p0 += 1024 * DEEP) {
+    constexpr int DEEP = 4, STEP = BLOCKS * 1024;
+    const int first = rank * 1024 + threadIdx.x;
+    for (int p0 = first; p0 < P; p0 += STEP * DEEP) {
         int e[DEEP];
 #pragma unroll
-        for (int j = 0; j < DEEP; ++j) e[j] = id(p0 + j * 1024);
+        for (int j = 0; j < DEEP; ++j) e[j] = id(p0 + j * STEP);
 #pragma unroll
-        for (int j = 0; j < DEEP; ++j) if (e[j] >= 0) g.place[p0 + j * 1024] = atomicAdd(&mine[e[j]], 1);
+        for (int j = 0; j < DEEP; ++j) if (e[j] >= 0) g.place[p0 + j * STEP] = atomicAdd(&mine[e[j]], 1);
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < E; e += 1024) {
-        int sum = 0;
-        for (int k = 0; k < SETS; ++k) {
-            const int n = sets[k * E + e];
-            sets[k * E + e] = sum;
-            sum += n;
+    cluster_sync_all();
+    int before[4];                                      // (E is 4,096 at most)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int e = i * 1024 + threadIdx.x;
+        before[i] = 0;
+        if (e < E) {
+            int sum = 0;
+#pragma unroll
+            for (int k = 0; k < BLOCKS; ++k) {
+                const int n = peer_int(&mine[e], k);
+                if (k < rank) before[i] += n;
+                sum += n;
+            }
+            counts[e] = sum;
         }
-        counts[e] = sum;
     }
+    cluster_sync_all();                                 // nobody reads them any more: they become the first places of this block's
+#pragma unroll
+    for (int i = 0; i < 4; ++i) if (i * 1024 + threadIdx.x < E) mine[i * 1024 + threadIdx.x] = before[i];
     __syncthreads();
     scan<1024>(counts, E, g.tile_rows, starts, tiles, carry);
-    write_list<1024>(starts, tiles, E, g.tile_rows, g.offsets, g.tile_group, g.tile_row0, g.max_tiles);
-    for (int p0 = threadIdx.x; p0 < P; p0 += 1024 * DEEP) {
+    if (rank == 0) write_list<1024>(starts, tiles, E, g.tile_rows, g.offsets, g.tile_group, g.tile_row0, g.max_tiles);
+    for (int p0 = first; p0 < P; p0 += STEP * DEEP) {
         int e[DEEP], r[DEEP];
 #pragma unroll
         for (int j = 0; j < DEEP; ++j) {
-            e[j] = id(p0 + j * 1024);
-            r[j] = e[j] >= 0 ? g.place[p0 + j * 1024] : 0;     // (this thread's own)
+            e[j] = id(p0 + j * STEP);
+            r[j] = e[j] >= 0 ? g.place[p0 + j * STEP] : 0;     // (this thread's own)
         }
 #pragma unroll
         for (int j = 0; j < DEEP; ++j) {
-            const int p = p0 + j * 1024;
+            const int p = p0 + j * STEP;
             if (p >= P) break;
             if (e[j] < 0) { g.place[p] = -1; continue; }
             const int n = mine[e[j]] + r[j], s = starts[e[j]] + n;
@@ -155,7 +177,7 @@ __global__ void __launch_bounds__(1024) group_kernel(const int32_t* __restrict__
             g.scale_row[s] = (tiles[e[j]] + n / g.tile_rows) * g.pad + n % g.tile_rows;
         }
     }
-    for (int s = starts[E] + threadIdx.x; s < P; s += 1024) {
+    for (int s = starts[E] + first; s < P; s += STEP) {
         g.perm[s] = 0;
         g.scale_row[s] = -1;
     }
@@ -313,8 +335,8 @@ int group_gather(const RowsArgs& x, const int32_t* ids, int P, int E, int top, c
         return launch_pdl(group_gather_kernel<T, false>, grid, block, 0, stream, x, ids, P, E, top, g);
     }
     static OncePerDevice done;
-    int st = allow_shared_memory(group_kernel, ((SETS + 3) * 4096 + 2) * sizeof(int), done);
-    if (!st) st = launch_pdl(group_kernel, dim3(1), dim3(1024), ((SETS + 3) * (size_t)E + 2) * sizeof(int), stream, ids, P, E, g);
+    int st = allow_shared_memory(group_kernel, (4 * 4096 + 2) * sizeof(int), done);
+    if (!st) st = launch_pdl(group_kernel, dim3(BLOCKS), dim3(1024), (4 * (size_t)E + 2) * sizeof(int), stream, ids, P, E, g);
     return st ? st : gather<T>(x, g.place, g.scale_row, top, stream);
 }
 
@@ -350,7 +372,7 @@ BROLM_API int brolm_fp8_experts(const ExpertsCall* c) {
     };
     Lists g;
     g.perm = (int32_t*)take(4LL * P); g.place = (int32_t*)take(4LL * P); g.scale_row = (int32_t*)take(4LL * P);
-    g.offsets = (int32_t*)take(4LL * (E + 1)); g.tile_group = (int32_t*)take(4LL * most); g.tile_row0 = (int32_t*)take(4LL * most);
+    g.offsets = (int32_t*)take(4LL * (E + 2)); g.tile_group = (int32_t*)take(4LL * most); g.tile_row0 = (int32_t*)take(4LL * most);
     g.max_tiles = most; g.tile_rows = rows; g.pad = pad;
     auto matrix = [&](int cols) {
         RowsArgs m = {};

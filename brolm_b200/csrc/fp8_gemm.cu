@@ -63,7 +63,7 @@ struct GemmArgs {
     const int32_t* offsets;
     const int32_t* perm;
     const float* scale;
-    int down, top, tokens, group_rows;
+    int down, top, tokens, group_rows, experts;
 };
 
 __device__ __forceinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile int* give_up, int code) {
@@ -216,9 +216,16 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     const bool aligned = (stage0 & 1023u) == 0;               // both blocks have the same layout
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int total = g.m_tiles * g.n_tiles;
     const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
     constexpr int OUT_COLS = EPI == EPI_GATED ? BN / 2 : BN;
+    // where the tiles end in a round that keeps half of the pairs or less, those are two items of half the columns each (a
+    // gated row's block of 128 results in 8 bits is a whole tile)
+    constexpr bool HALVES = !(OUT == OUT_FP8 && EPI == EPI_GATED);
+    auto items_of = [&](int tiles, int& whole) {
+        const int rest = tiles % n_pairs;
+        whole = HALVES && 2 * rest <= n_pairs ? tiles - rest : tiles;
+        return tiles + (tiles - whole);
+    };
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
@@ -243,22 +250,24 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     fence_after_sync();
     const uint32_t tmem = *tmem_slot;
 
-    // what a tile is: false behind the experts' last
-    auto find = [&](int tile, int& mt, int& nt, int& group, int& row0) {
+    // what an item is: its tile, and -1 or which half of its columns
+    auto find = [&](int item, int whole, int& mt, int& nt, int& half_of, int& group, int& row0) {
+        const int tile = item < whole ? item : whole + (item - whole) / 2;
+        half_of = item < whole ? -1 : (item - whole) & 1;
         if (!EXPERTS) {
             nt = tile / g.m_tiles;
             mt = tile - nt * g.m_tiles;
             group = 0;
             row0 = mt * PM;
-            return true;
+            return;
         }
         mt = tile / g.n_tiles;
         nt = tile - mt * g.n_tiles;
         group = g.tile_group[mt];
-        if (group < 0) return false;
         row0 = g.tile_row0[mt];
-        return true;
     };
+    // (experts: how many tiles of rows there are stands behind the list's first rows)
+    auto tiles_of = [&]() { return (EXPERTS ? g.offsets[g.experts + 1] : g.m_tiles) * g.n_tiles; };
 
     if (warp < FIRST) {
     // 128 x 56 + 256 x 224 = 384 x 168, what a block is launched with
@@ -270,10 +279,12 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             // Launched with programmatic stream serialization: nothing of this kernel touches memory before its first
             // operands have arrived, so (but for the experts' lists) the loader's wait is the kernel's.
             pdl_wait();
-            int mt, nt, group, row0;
-            for (int tile = pair; tile < total && ok; tile += n_pairs) {
-                if (!find(tile, mt, nt, group, row0)) break;
-                const int w_row = group * g.group_rows + nt * BN;
+            int mt, nt, half_of, group, row0, whole;
+            const int total = items_of(tiles_of(), whole);
+            for (int item = pair; item < total && ok; item += n_pairs) {
+                find(item, whole, mt, nt, half_of, group, row0);
+                // half the columns: a block of the pair needs 64 rows of W (it is brought 128), the scales are one tile
+                const int w_row = group * g.group_rows + nt * BN + (half_of > 0 ? BN / 2 : 0), each = half_of < 0 ? HN : HN / 2;
                 const int xs_row = (EXPERTS ? mt * (PM / 128) : row0 >> 7) + (int)rank, ws_row = w_row >> 7;
                 for (int kb = 0; kb < g.nkb; ++kb, ++it) {
                     if (!(kb > 0 ? wait_one(empty0 + 8 * s, phase ^ 1, give_up, 1) : wait_on(empty0 + 8 * s, phase ^ 1, give_up, 1))) { ok = false; break; }
@@ -281,7 +292,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                     const bool with_scales = (kb & 3) == 0;
                     if (rank == 0) mbar_expect_tx(full, 2 * (STAGE_BYTES + (with_scales ? SCALES : 0)));   // both blocks' bytes
                     tma_load_pair(a_dst, &map_x, kb * BK, row0 + (int)rank * BM, full);
-                    tma_load_pair(a_dst + A_BYTES, &map_w, kb * BK, w_row + (int)rank * HN, full);
+                    tma_load_pair(a_dst + A_BYTES, &map_w, kb * BK, w_row + (int)rank * each, full);
                     if (with_scales) {
                         const int q = kb >> 2;
                         tma_load_pair(s_dst, &map_xs, 0, xs_row * g.quads + q, full);
@@ -298,13 +309,13 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         }
     } else if (warp == 1) {
         if (rank == 0 && elect_one()) {
-            const uint32_t id = idesc_mx(PM, BN);
             int s = 0, phase = 0, local = 0, set = 0;
             bool ok = !*give_up;
             if (EXPERTS) pdl_wait();
-            int mt, nt, group, row0;
-            for (int tile = pair; tile < total && ok; tile += n_pairs) {
-                if (!find(tile, mt, nt, group, row0)) break;
+            int whole;
+            const int total = items_of(tiles_of(), whole);
+            for (int item = pair; item < total && ok; item += n_pairs) {
+                const uint32_t id = idesc_mx(PM, item < whole ? BN : BN / 2);
                 uint32_t sfw = 0, sfx = 0;
                 for (int lo = 0; lo < g.nkb && ok; lo += g.piece, ++local) {
                     const int as = local & 1, hi = min(g.nkb, lo + g.piece);
@@ -342,15 +353,16 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         const int quarter = warp & 3, half = (warp - FIRST) >> 2;
         uint8_t* room = rooms + (warp - FIRST) * 4096;
-        const int trow = quarter * 32 + lane;                   // row of this block's half of the tile
         int local = 0;
         if (EXPERTS) pdl_wait();
-        int mt, nt, group, row0;
+        int mt, nt, half_of, group, row0, whole;
         bool ok = true;
-        for (int tile = pair; tile < total && ok; tile += n_pairs) {
-            if (!find(tile, mt, nt, group, row0)) break;
+        const int total = items_of(tiles_of(), whole);
+        for (int item = pair; item < total && ok; item += n_pairs) {
+            find(item, whole, mt, nt, half_of, group, row0);
             const int first = row0 + (int)rank * BM + quarter * 32;             // the warp's first row
-            const int rows = (EXPERTS ? g.offsets[group + 1] : g.M) - first;    // how many of its rows there are (more than 32: all)
+            // how many of its rows there are (more than 32: all); none where half the columns are the other half's warps'
+            const int rows = half_of >= 0 && half ? 0 : (EXPERTS ? g.offsets[group + 1] : g.M) - first;
             int at = 0;
             float mul = 1.0f;
             if (EXPERTS && lane < rows) {
@@ -363,7 +375,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                 if (g.scale) mul = g.scale[g.perm[first + lane]];
             }
             constexpr int W = EPI == EPI_GATED ? 64 : 128;      // this thread's results
-            const int col = nt * OUT_COLS + half * W;
+            const int col = nt * OUT_COLS + (half_of > 0 || half ? W : 0);
             // results of `unit` bytes from the thread's result c on, staged as ROW bytes a row
             auto flush = [&](auto row_bytes, int c, int unit, bool wide) {
                 constexpr int ROW = decltype(row_bytes)::value;
@@ -524,7 +536,10 @@ int launch(const Maps& m, const GemmArgs& g, cudaStream_t stream) {
     static OncePerDevice done;
     const int st = allow_shared_memory(fp8_gemm_kernel<EPI, OUT, EXPERTS>, SMEM_BYTES, done);
     if (st) return st;
-    const int tiles = g.m_tiles * g.n_tiles, most = device_sms() / 2, pairs = tiles < most ? tiles : most;
+    const int most = device_sms() / 2;
+    int pairs = g.m_tiles * g.n_tiles;
+    if (!(OUT == OUT_FP8 && EPI == EPI_GATED) && 2LL * pairs <= most) pairs *= 2;       // all tiles in halves
+    if (pairs > most) pairs = most;
     return launch_pdl(fp8_gemm_kernel<EPI, OUT, EXPERTS>, dim3(2 * pairs), dim3(THREADS), SMEM_BYTES, stream, m.x, m.w, m.xs, m.ws, g);
 }
 template <bool EXPERTS>
@@ -573,7 +588,7 @@ BROLM_API int brolm_fp8_gemm(const fp8::ProductCall* c) {
     if (!c->experts) return dispatch<false>(m, g, c->epilogue, c->out, c->stream);
     g.tile_group = (const int32_t*)c->tile_group; g.tile_row0 = (const int32_t*)c->tile_row0; g.offsets = (const int32_t*)c->offsets;
     g.perm = (const int32_t*)c->perm; g.scale = (const float*)c->scale;
-    g.down = c->down; g.top = c->top; g.tokens = c->tokens; g.group_rows = c->group_rows;
+    g.down = c->down; g.top = c->top; g.tokens = c->tokens; g.group_rows = c->group_rows; g.experts = c->experts;
     return dispatch<true>(m, g, c->epilogue, c->out, c->stream);
 }
 

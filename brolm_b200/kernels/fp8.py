@@ -328,7 +328,7 @@ def _experts(what: str, x, ids, up: Fp8Matrix, down: Fp8Matrix, pairs, out, acti
     most = (P + rows - 1) // rows + min(E, P)
     up512 = lambda n: (n + 511) & -512
     # the order and the list; the rows of both products in 8 bits with a tile of scales for every tile of the list; floats between
-    need = 3 * up512(4 * P) + up512(4 * E + 4) + 2 * up512(4 * most)
+    need = 3 * up512(4 * P) + up512(4 * E + 8) + 2 * up512(4 * most)
     for cols in (K, inter):
         need += up512(P * ((cols + 15) & -16)) + ((rows + 127) >> 7) * most * ((cols + 511) >> 9) * _TILE
     if rows <= STREAM_ROWS:
