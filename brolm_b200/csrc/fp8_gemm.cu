@@ -355,25 +355,37 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         uint8_t* room = rooms + (warp - FIRST) * 4096;
         int local = 0;
         if (EXPERTS) pdl_wait();
-        int mt, nt, half_of, group, row0, whole;
+        int whole;
         bool ok = true;
         const int total = items_of(tiles_of(), whole);
+        // An expert's item is known by three loads one after the other (its tile's first row and expert, that expert's end, this
+        // row's pair): each is asked for while an item before is at work, or they cost as much as the item's results.
+        struct Item { int mt, nt, half_of, group, row0; };
+        Item now, next;
+        auto look = [&](int item, Item& t) { if (item < total) find(item, whole, t.mt, t.nt, t.half_of, t.group, t.row0); };
+        auto end_of = [&](int item, const Item& t) { return item < total ? (EXPERTS ? g.offsets[t.group + 1] : g.M) : 0; };
+        auto pair_of = [&](int item, const Item& t, int end) {
+            const int row = t.row0 + (int)rank * BM + quarter * 32 + lane;
+            return EXPERTS && item < total && row < end && (g.down || g.scale) ? g.perm[row] : 0;
+        };
+        look(pair, now);
+        look(pair + n_pairs, next);
+        int end = end_of(pair, now), p = pair_of(pair, now, end);
         for (int item = pair; item < total && ok; item += n_pairs) {
-            find(item, whole, mt, nt, half_of, group, row0);
-            const int first = row0 + (int)rank * BM + quarter * 32;             // the warp's first row
+            const int mt = now.mt, nt = now.nt, half_of = now.half_of;
+            const int first = now.row0 + (int)rank * BM + quarter * 32;         // the warp's first row
             // how many of its rows there are (more than 32: all); none where half the columns are the other half's warps'
-            const int rows = half_of >= 0 && half ? 0 : (EXPERTS ? g.offsets[group + 1] : g.M) - first;
-            int at = 0;
+            const int rows = half_of >= 0 && half ? 0 : end - first;
+            int at = first + lane;
             float mul = 1.0f;
-            if (EXPERTS && lane < rows) {
+            if (EXPERTS) {
                 if (g.down) {
-                    const int p = g.perm[first + lane], tok = p / g.top;
+                    const int tok = p / g.top;
                     at = (p - tok * g.top) * g.tokens + tok;
-                } else {
-                    at = first + lane;
                 }
-                if (g.scale) mul = g.scale[g.perm[first + lane]];
+                if (g.scale && lane < rows) mul = g.scale[p];
             }
+            const int next_end = end_of(item + n_pairs, next);
             constexpr int W = EPI == EPI_GATED ? 64 : 128;      // this thread's results
             const int col = nt * OUT_COLS + (half_of > 0 || half ? W : 0);
             // results of `unit` bytes from the thread's result c on, staged as ROW bytes a row
@@ -389,6 +401,12 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                 const bool ready = wait_on(acc_full0 + 8 * as, (local >> 1) & 1, give_up, 3);
                 if (!__all_sync(0xffffffffu, ready)) { ok = false; break; }
                 fence_after_sync();
+                if (lo == 0) {
+                    p = pair_of(item + n_pairs, next, next_end);
+                    now = next;
+                    end = next_end;
+                    look(item + 2 * n_pairs, next);
+                }
                 const uint32_t acc = tmem + as * ACC1 + half * 128 + ((uint32_t)(quarter * 32) << 16);
                 // the first 32 columns read are those that the other accumulator wants
                 auto there = [&](int turn) {
