@@ -55,6 +55,25 @@ __device__ __forceinline__ bool elect_one() {
     return one != 0;
 }
 
+// Activations that leave what is not a number so (a block that is NaN makes NaN of all that is computed from it; fminf and fmaxf
+// would take the other number).
+enum : int { ACT_NONE = 0, ACT_RELU2 = 1 };
+__device__ __forceinline__ float act_of(float v, int act) {
+    if (act == ACT_RELU2) {
+        v = v < 0.0f ? 0.0f : v;
+        return v * v;
+    }
+    return v;
+}
+__device__ __forceinline__ float gate_of(float z, float u, int act, float limit) {
+    if (act == 2) {
+        z = z > limit ? limit : z;
+        u = (u > limit ? limit : u < -limit ? -limit : u) + 1.0f;
+        return z * tc::fast_rcp(1.0f + tc::fast_exp2(-1.4426950408889634f * 1.702f * z)) * u;
+    }
+    return tc::fast_gate_act(z, act) * u;
+}
+
 // ---- tensor core, operands e4m3, scales ue8m0
 // Instruction descriptor of kind::mxf8f6f4 without the scales' byte numbers (a: bits 29-30, b: bits 4-5).
 __device__ __forceinline__ uint32_t idesc_mx(int m, int n) {

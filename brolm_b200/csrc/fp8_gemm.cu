@@ -42,7 +42,6 @@ constexpr int ROWS_BYTES = 4 * BM * 4;      // largest magnitudes of a row's two
 
 enum : int { EPI_STORE = 0, EPI_GATED = 1 };
 enum : int { OUT_BF16 = 0, OUT_F32 = 1, OUT_FP8 = 2 };
-enum : int { ACT_NONE = 0, ACT_RELU2 = 1 };
 
 __device__ int g_fp8_gemm_error;
 
@@ -113,26 +112,19 @@ __device__ __forceinline__ void arrive_first_block(uint32_t bar) {              
     asm volatile("{\n.reg .b32 remote;\nmapa.shared::cluster.u32 remote, %0, 0;\nmbarrier.arrive.shared::cluster.b64 _, [remote];\n}"
                  ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ float act_of(float v, int act) {
-    if (act == ACT_RELU2) {
-        v = fmaxf(v, 0.0f);
-        return v * v;
-    }
-    return v;
-}
 
 // N / 2 gated pairs of neighbouring numbers, to the front.  Which activation is asked once for all of them.
 template <int N>
 __device__ __forceinline__ void gate_pairs(float (&o)[N], int act, float limit) {
     if (act == 0) {
 #pragma unroll
-        for (int i = 0; i < N / 2; ++i) o[i] = fast_gate_pair(o[2 * i], o[2 * i + 1], 0, 0.0f);
+        for (int i = 0; i < N / 2; ++i) o[i] = gate_of(o[2 * i], o[2 * i + 1], 0, 0.0f);
     } else if (act == 1) {
 #pragma unroll
-        for (int i = 0; i < N / 2; ++i) o[i] = fast_gate_pair(o[2 * i], o[2 * i + 1], 1, 0.0f);
+        for (int i = 0; i < N / 2; ++i) o[i] = gate_of(o[2 * i], o[2 * i + 1], 1, 0.0f);
     } else {
 #pragma unroll
-        for (int i = 0; i < N / 2; ++i) o[i] = fast_gate_pair(o[2 * i], o[2 * i + 1], 2, limit);
+        for (int i = 0; i < N / 2; ++i) o[i] = gate_of(o[2 * i], o[2 * i + 1], 2, limit);
     }
 }
 
@@ -212,7 +204,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     uint32_t* most_of = tmem_slot + 4;                        // [2][2][128]
     const uint32_t stage0 = smem_u32(base), scale0 = stage0 + STAGES * STAGE_BYTES;
     const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * STAGES, acc_full0 = empty0 + 8 * STAGES,
-                   acc_free0 = acc_full0 + 16, lap_free = acc_free0 + 16, halves0 = lap_free + 16;
+                   acc_free0 = acc_full0 + 16, lap_free = acc_free0 + 16, halves0 = lap_free + 16, ended = lap_free + 8;
     const bool aligned = (stage0 & 1023u) == 0;               // both blocks have the same layout
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -237,6 +229,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             mbar_init(acc_free0 + 8 * s, 16);     // eight epilogue warps of each block
         }
         for (int q = 0; q < 4; ++q) mbar_init(halves0 + 8 * q, 2);      // the two warps that share rows
+        mbar_init(ended, 1);
         mbar_init(lap_free, 8);                   // the four of each whose columns lie in both accumulators
         give_up[0] = aligned ? 0 : 1;
         give_up[1] = 0;
@@ -346,6 +339,10 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                     }
                     if (ok) umma_commit_pair(acc_full0 + 8 * as);
                 }
+            }
+            if (!ok) {                                      // products in flight end before their operands go
+                umma_commit_pair(ended);
+                drain_on(ended, 0, give_up, 8);
             }
         }
     }

@@ -35,7 +35,6 @@ constexpr int MAX_STAGES = 12;
 constexpr int FUSED_BLOCKS = 24;       // 48 KB of the rows, five stages beside them
 
 enum : int { EPI_STORE = 0, EPI_GATED = 1 };
-enum : int { ACT_NONE = 0, ACT_RELU2 = 1 };
 
 __device__ int g_fp8_stream_error;
 
@@ -90,13 +89,6 @@ __device__ __forceinline__ float peer_float(uint32_t addr, uint32_t rank) {
     asm volatile("{\n.reg .b32 r;\nmapa.shared::cluster.u32 r, %1, %2;\nld.shared::cluster.f32 %0, [r];\n}" : "=f"(v) : "r"(addr), "r"(rank));
     return v;
 }
-__device__ __forceinline__ float act_of(float v, int act) {
-    if (act == ACT_RELU2) {
-        v = fmaxf(v, 0.0f);
-        return v * v;
-    }
-    return v;
-}
 __device__ __forceinline__ void put(const StreamArgs& g, long at, float v) {
     if (g.out_f32) reinterpret_cast<float*>(g.y)[at] = v;
     else reinterpret_cast<bf16*>(g.y)[at] = __float2bfloat16_rn(v);
@@ -148,7 +140,7 @@ struct Shape {
     static constexpr int SCALES = FUSED ? SF_TILE : 2 * SF_TILE;        // of a stage
     static size_t x_room(int per) { return FUSED ? (size_t)per * X_BYTES + (size_t)((per + 3) / 4 + 1) * SF_TILE : 0; }
     static size_t smem(int stages, int per) {
-        return x_room(per) + (size_t)stages * (STAGE_BYTES + SCALES) + (2 * MAX_STAGES + 5) * 8 + 16;
+        return x_room(per) + (size_t)stages * (STAGE_BYTES + SCALES) + (2 * MAX_STAGES + 6) * 8 + 16;
     }
 };
 
@@ -165,13 +157,13 @@ __global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS, 2) fp8_stream_kerne
     uint8_t* scale_slots = x_blocks + (FUSED ? g.per * S::X_BYTES : 0);
     uint8_t* x_scales = scale_slots + stages * S::SCALES;
     uint64_t* bars = reinterpret_cast<uint64_t*>(x_scales + (FUSED ? ((g.per + 3) / 4 + 1) * SF_TILE : 0));
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * MAX_STAGES + 5);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * MAX_STAGES + 6);
     volatile int* give_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
     // slices: this one's sums [rows of X][128], in the ring, which is read to its end by then
     float* sums = reinterpret_cast<float*>(base);
     const uint32_t stage0 = smem_u32(base), scale0 = smem_u32(scale_slots);
     const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * MAX_STAGES, acc_full0 = empty0 + 8 * MAX_STAGES,
-                   acc_empty0 = acc_full0 + 16, x_ready = acc_empty0 + 16;
+                   acc_empty0 = acc_full0 + 16, x_ready = acc_empty0 + 16, ended = x_ready + 8;
     const bool aligned = (stage0 & 1023u) == 0;
     const int slices = EXPERTS ? 1 : (int)cluster_size(), slice = EXPERTS ? 0 : (int)cluster_rank();
     const int first = EXPERTS ? blockIdx.x : blockIdx.x / slices, step = EXPERTS ? gridDim.x : gridDim.x / slices;
@@ -188,6 +180,7 @@ __global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS, 2) fp8_stream_kerne
             mbar_init(acc_empty0 + 8 * s, 4);
         }
         mbar_init(x_ready, 8);
+        mbar_init(ended, 1);
         give_up[0] = aligned ? 0 : 1;
         give_up[1] = 0;
         give_up[2] = tc::g_stall_code;
@@ -306,6 +299,10 @@ __global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS, 2) fp8_stream_kerne
                 }
                 if (ok) umma_commit(acc_full0 + 8 * as);
             }
+            if (!ok) {                                      // products in flight end before their operands go
+                umma_commit(ended);
+                drain_on(ended, 0, give_up, 8);
+            }
         }
     } else {
         const int quarter = warp & 3;
@@ -357,7 +354,7 @@ __global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS, 2) fp8_stream_kerne
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const float got = __shfl_xor_sync(0xffffffffu, odd ? o[2 * i] : o[2 * i + 1], 1);
-                        o[i] = fast_gate_pair(odd ? got : o[2 * i], odd ? o[2 * i + 1] : got, g.act, g.limit);
+                        o[i] = gate_of(odd ? got : o[2 * i], odd ? o[2 * i + 1] : got, g.act, g.limit);
                     }
                     first_row = odd; row_step = 2; col >>= 1;
                 } else {
@@ -399,7 +396,7 @@ __global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS, 2) fp8_stream_kerne
                 int col = rt * BR + t;
                 if (EPI == EPI_GATED) {
                     const float up = __shfl_down_sync(0xffffffffu, v, 1);
-                    v = fast_gate_pair(v, up, g.act, g.limit);
+                    v = gate_of(v, up, g.act, g.limit);
                     col = (col & 1) ? g.N : col >> 1;
                 } else {
                     v = act_of(v, g.act);

@@ -211,7 +211,8 @@ def _checked(what: str, x, w: Fp8Matrix, out: torch.Tensor, outputs: int) -> Non
     else:
         fine = x.dtype in _CODES and x.dim() == 2 and x.shape[1] == w.cols and x.get_device() == w.index and (x.stride(1) == 1 or w.cols == 1)
     if fine and len(w.shape) == 2 and w.index >= 0 and w.index == _device() and out.dtype in _CODES and out.get_device() == w.index and out.dim() == 2 \
-            and out.shape[0] == x.shape[0] and out.shape[1] == outputs and (out.stride(1) == 1 or outputs == 1):
+            and out.shape[0] == x.shape[0] and out.shape[1] == outputs and (out.stride(1) == 1 or outputs == 1) \
+            and (out.stride(0) >= outputs or out.shape[0] <= 1):
         return
     if len(w.shape) != 2:
         raise KernelError(f"{what}: a stack of experts' matrices goes to experts_fp8")
@@ -222,6 +223,8 @@ def _checked(what: str, x, w: Fp8Matrix, out: torch.Tensor, outputs: int) -> Non
     _refuse(what, out, "out")
     if tuple(out.shape) != (x.shape[0], outputs):
         raise KernelError(f"{what}: the result has the shape {(x.shape[0], outputs)}, not {tuple(out.shape)}")
+    if out.shape[0] > 1 and out.stride(0) < out.shape[1]:
+        raise KernelError(f"{what}: the rows of the result lie over one another (strides {tuple(out.stride())})")
     raise KernelError(f"{what}: the rows, the matrix and the result live on {x.device}, {w.device} and {out.device}; the current device is cuda:{_device()}")
 
 
@@ -257,7 +260,7 @@ def _product(x, M: int, w: Fp8Matrix, y: tuple, out: int, act: int, limit: float
 def linear_fp8(x, w: Fp8Matrix, out: torch.Tensor, activation: str = "none", limit: float = 0.0) -> None:
     """out [rows, w.outputs] (float32 or bfloat16) = act(x w^T).  x [rows, columns]: float32 or bfloat16, which is rounded to 8
     bits first, or such rows.  With a plain matrix ``activation`` is "none" or "relu2" (the square of relu), with a gated one one
-    of ``ACTIVATIONS``: act(gate) * partner."""
+    of ``ACTIVATIONS``: act(gate) * partner.  ``out`` does not lie over x or the matrix."""
     act = _act_code("linear_fp8", w, activation)
     _checked("linear_fp8", x, w, out, w.outputs)
     _product(x.packed if type(x) is Fp8Matrix else x, x.shape[0], w, (out.data_ptr(), 0, out.stride(0)), _OUT[out.dtype], act, limit)
@@ -375,8 +378,8 @@ def experts_fp8(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, up: F
     _experts_checked(what, x, ids, up, down, weights)
     if out.dtype not in _CODES or out.dim() != 2 or out.get_device() != x.get_device() or (out.stride(1) != 1 and down.rows > 1):
         _refuse(what, out, "out")
-    if out.shape[0] != x.shape[0] or out.shape[1] != down.rows:
-        raise KernelError(f"{what}: the result has the shape {(x.shape[0], down.rows)}, not {tuple(out.shape)}")
+    if out.shape[0] != x.shape[0] or out.shape[1] != down.rows or (out.shape[0] > 1 and out.stride(0) < down.rows):
+        raise KernelError(f"{what}: the result has the shape {(x.shape[0], down.rows)}, not {tuple(out.shape)} (strides {tuple(out.stride())})")
     if ids.shape[1] == 0 or up.shape[0] == 0:
         out.zero_()
         return

@@ -248,3 +248,262 @@ def test_experts(t, top, e, width, inter, act, style, scale_input):
     none = ((ids < 0) | (ids >= e)).T
     assert bool((pairs[none] == 7.0).all())
     assert kernels.fp8_stream_status() == 0 and kernels.fp8_gemm_status() == 0
+
+
+def case(m, n, k, seed=11, gated=False):
+    g = gen(seed)
+    x, w = rows_of(g, m, k, torch.bfloat16), rows_of(g, n * (2 if gated else 1), k, torch.bfloat16, 0.3) * k ** -0.5
+    return x, (kernels.fp8_gate_up(w[:n].contiguous(), w[n:].contiguous()) if gated else kernels.fp8_quantize(w))
+
+
+LIMIT = 8_000_000            # clock cycles: about four milliseconds
+
+
+@pytest.mark.parametrize("library, code, m, n, k, gated", [
+    ("fp8_stream", 1, 20, 200, 9216, False), ("fp8_stream", 2, 8, 2304, 2304, False), ("fp8_stream", 3, 100, 700, 1000, False),
+    ("fp8_stream", 5, 8, 700, 640, True), ("fp8_stream", 6, 8, 2304, 2304, False), ("fp8_gemm", 1, 300, 700, 2304, False), ("fp8_gemm", 2, 300, 700, 2304, False),
+    ("fp8_gemm", 3, 300, 700, 640, True), ("fp8_gemm", 5, 300, 700, 640, False), ("fp8_gemm", 6, 300, 700, 640, False), ("fp8_gemm", 7, 300, 700, 640, True)])
+def test_a_wait_that_runs_out_is_reported_and_the_next_call_is_right(library, code, m, n, k, gated):
+    status = {"fp8_stream": kernels.fp8_stream_status, "fp8_gemm": kernels.fp8_gemm_status}[library]
+    x, w = case(m, n, k, gated=gated)
+    down = case(1, 40, n)[1]
+
+    def run():
+        out = torch.empty(m, 40 if code == 7 else n, dtype=torch.float32, device=DEV)
+        if code == 7:                                            # the two warps that share a block of 128 results
+            kernels.feedforward_fp8(x, w, down, out, "silu")
+        else:
+            kernels.linear_fp8(x, w, out, "silu" if gated else "none")
+        torch.cuda.synchronize()
+        return out
+    good = run()
+    assert status(reset=True) == 0
+    kernels.wait_control(library, cycles=LIMIT, stall_code=code)
+    try:
+        run()
+        assert status(reset=True) == code and status() == 0
+    finally:
+        kernels.wait_control(library, 0, 0)
+    assert torch.equal(run(), good) and status() == 0
+
+
+@pytest.mark.parametrize("rows", [8, 600])
+def test_experts_whose_wait_runs_out(rows):
+    g = gen(12)
+    x, ids, w = rows_of(g, rows, 256, torch.bfloat16), routed(g, rows, 2, 2, "even"), torch.rand(rows, 2, generator=g, device=DEV)
+    up, down = (kernels.fp8_quantize(rows_of(g, 2 * a, b, torch.bfloat16).view(2, a, b) * 0.1) for a, b in ((128, 256), (256, 128)))
+    library, status = ("fp8_stream", kernels.fp8_stream_status) if rows == 8 else ("fp8_gemm", kernels.fp8_gemm_status)
+
+    def run():
+        out = torch.empty(rows, 256, dtype=torch.float32, device=DEV)
+        kernels.experts_fp8(x, ids, w, up, down, out, "relu2")
+        torch.cuda.synchronize()
+        return out
+    good = run()
+    kernels.wait_control(library, cycles=LIMIT, stall_code=2)
+    try:
+        run()
+        assert status(reset=True) == 2 and status() == 0
+    finally:
+        kernels.wait_control(library, 0, 0)
+    assert torch.equal(run(), good) and status() == 0
+
+
+def test_a_matrix_made_right_before_it_is_used():
+    """The products read their matrix before they wait for the kernel before them; the one that makes it ends before."""
+    g = gen(13)
+    x = rows_of(g, 8, 2304, torch.bfloat16)
+    xs = rows_of(g, 200, 2304, torch.bfloat16)
+    ws = [rows_of(g, 4096, 2304, torch.bfloat16) for _ in range(3)]
+    want = []
+    for w in ws:
+        m = kernels.fp8_quantize(w)
+        torch.cuda.synchronize()
+        want.append([torch.empty(len(t), 4096, device=DEV) for t in (x, xs)])
+        for t, o in zip((x, xs), want[-1]):
+            kernels.linear_fp8(t, m, o)
+    torch.cuda.synchronize()
+    for turn in range(12):
+        w = ws[turn % 3]
+        outs = [torch.full((len(t), 4096), 7.0, device=DEV) for t in (x, xs)]
+        kernels.linear_fp8(x, kernels.fp8_quantize(w), outs[0])
+        kernels.linear_fp8(xs, kernels.fp8_quantize(w), outs[1])
+        for o, good in zip(outs, want[turn % 3]):
+            assert torch.equal(o, good)
+
+
+def passes():
+    """A few calls of every kind: (inputs that change, a function that fills `out`)."""
+    g = gen(14)
+    made = []
+    for m, n, k in ((3, 500, 640), (40, 700, 1100), (300, 600, 640)):
+        x, w = case(m, n, k, seed=m)
+        made.append((x, torch.empty(m, n, device=DEV), lambda x, o, w=w: kernels.linear_fp8(x, w, o)))
+    for m in (5, 200):
+        x, gu = case(m, 320, 256, seed=m, gated=True)
+        d = case(1, 256, 320, seed=m + 1)[1]
+        made.append((x, torch.empty(m, 256, device=DEV), lambda x, o, gu=gu, d=d: kernels.feedforward_fp8(x, gu, d, o, "silu")))
+    for t in (6, 300):
+        ids, w = routed(g, t, 2, 4, "even"), torch.rand(t, 2, generator=g, device=DEV)
+        up, down = (kernels.fp8_quantize(rows_of(g, 4 * a, b, torch.bfloat16).view(4, a, b) * 0.1) for a, b in ((96, 256), (256, 96)))
+        made.append((rows_of(g, t, 256, torch.bfloat16), torch.empty(t, 256, device=DEV),
+                     lambda x, o, ids=ids, w=w, up=up, down=down: kernels.experts_fp8(x, ids, w, up, down, o, "relu2")))
+    return made
+
+
+def test_captured_calls_of_new_inputs_and_two_graphs_at_once():
+    made = passes()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    graphs, statics, outs = [], [], []
+    for i, s in enumerate(streams):
+        xs, os = [x.clone() for x, _, _ in made], [torch.empty_like(o) for _, o, _ in made]
+        with torch.cuda.stream(s):
+            for x, o, (_, _, f) in zip(xs, os, made):
+                f(x, o)                                          # libraries are there before a capture
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            for x, o, (_, _, f) in zip(xs, os, made):
+                f(x, o)
+        graphs.append(graph), statics.append(xs), outs.append(os)
+    for turn in range(4):
+        want = []
+        for i in range(2):
+            for x, (x0, _, _) in zip(statics[i], made):
+                x.copy_(x0 * (1.0 + 0.25 * turn + i))
+            row = []
+            for x, (_, o, f) in zip(statics[i], made):
+                f(x, o)
+                row.append(o.clone())
+            want.append(row)
+        for os in outs:
+            for o in os:
+                o.fill_(7.0)
+        torch.cuda.synchronize()
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                for _ in range(3):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            for o, w in zip(outs[i], want[i]):
+                assert torch.equal(o, w)
+
+
+def test_a_stream_that_is_not_the_default_one():
+    made = passes()
+    want = []
+    for x, o, f in made:
+        f(x, o)
+        want.append(o.clone())
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    slow = torch.randn(4096, 4096, device=DEV)
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for _ in range(10):
+            slow = slow @ slow * 1e-3                            # what follows is behind this
+        got = []
+        for x, o, f in made:
+            fresh = x * 1.0
+            out = torch.full_like(o, 7.0)
+            f(fresh, out)
+            got.append(out)
+    s.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("act", ["relu2", "none", "silu", "gelu_tanh", "clamped_gate"])
+def test_a_token_that_is_not_finite_is_nobody_elses(act):
+    g = gen(15)
+    for t in (6, 300):
+        ids, w = routed(g, t, 2, 3, "even"), torch.rand(t, 2, generator=g, device=DEV)
+        up, gate = (rows_of(g, 3 * 128, 256, torch.bfloat16).view(3, 128, 256) * 0.1 for _ in range(2))
+        down = kernels.fp8_quantize(rows_of(g, 3 * 256, 128, torch.bfloat16).view(3, 256, 128) * 0.1)
+        up = kernels.fp8_quantize(up) if act in ("relu2", "none") else kernels.fp8_gate_up(gate, up)
+        x = rows_of(g, t, 256, torch.bfloat16)
+        out, bad = torch.empty(t, 256, device=DEV), torch.empty(t, 256, device=DEV)
+        kernels.experts_fp8(x, ids, w, up, down, out, act, 2.0)
+        x[2, 5] = float("nan")
+        kernels.experts_fp8(x, ids, w, up, down, bad, act, 2.0)
+        others = torch.arange(t, device=DEV) != 2
+        assert bool(torch.isnan(bad[2]).all()) and torch.equal(bad[others], out[others])
+
+
+def test_many_experts_and_many_pairs():
+    """More experts than a block has threads, and more pairs than the cluster that sorts them looks at in one go."""
+    g = gen(16)
+    e, t, top = 1500, 17000, 3
+    ids = torch.randint(0, e, (t, top), generator=g, device=DEV, dtype=torch.int32)
+    x, w = rows_of(g, t, 32, torch.bfloat16), torch.rand(t, top, generator=g, device=DEV)
+    up, down = (rows_of(g, e * a, b, torch.bfloat16).view(e, a, b) * 0.3 for a, b in ((16, 32), (32, 16)))
+    out = torch.empty(t, 32, device=DEV)
+    kernels.experts_fp8(x, ids, w, kernels.fp8_quantize(up), kernels.fp8_quantize(down), out, "none")
+    some = torch.randint(0, t, (200,), generator=g, device=DEV)
+    xe, ue, de = plain.values(x[some]), read(kernels.fp8_quantize(up)).double(), read(kernels.fp8_quantize(down)).double()
+    for i, tok in enumerate(some.tolist()):
+        want = torch.zeros(32, dtype=torch.float64, device=DEV)
+        for c in range(top):
+            k = int(ids[tok, c])
+            # (sums of 32 and 16 numbers: a border is missed by too little to matter to a number's step)
+            want += float(w[tok, c]) * (plain.values((xe[i] @ ue[k].T)[None])[0] @ de[k].T)
+        assert float((out[tok].double() - want).norm()) <= 0.05 * float(want.norm())
+    assert float((out[some].double()).norm()) > 0
+
+
+def test_matrices_beyond_two_gigabytes():
+    g = gen(17)
+    n, k = 70_000, 32_768
+    w = torch.empty(n, k, dtype=torch.bfloat16, device=DEV)
+    for a in range(0, n, 7000):
+        w[a:a + 7000] = torch.randn(7000, k, generator=g, device=DEV)
+    w8 = kernels.fp8_quantize(w)
+    assert w8.nbytes > 2 ** 31
+    last = plain.values(w[-3:, -2048:])
+    back = torch.empty(n, k, dtype=torch.bfloat16, device=DEV)
+    kernels.fp8_read(w8, back)
+    assert torch.equal(back[-3:, -2048:].double(), last)
+    del back
+    x = rows_of(g, 3, k, torch.bfloat16)
+    y = torch.empty(3, n, device=DEV)
+    kernels.linear_fp8(x, w8, y)
+    xe = plain.values(x)
+    for some in (slice(0, 40), slice(65_500, 65_580), slice(n - 40, n)):
+        we = plain.values(w[some])
+        near(y[:, some], xe @ we.T, sum_bound(xe, we) * 20)     # (256 blocks of K in slices of a part of them)
+    # rows beyond two gigabytes, a result beyond two billion numbers
+    few = kernels.fp8_quantize(w[:33_000])
+    del w, w8
+    wide = kernels.fp8_quantize(torch.randn(66_000, 128, generator=g, device=DEV))
+    x = rows_of(g, 33_000, 128, torch.bfloat16)
+    y = torch.empty(33_000, 66_000, dtype=torch.bfloat16, device=DEV)
+    kernels.linear_fp8(x, wide, y)
+    xe, we = plain.values(x[-200:]), read(wide).double()[-300:]
+    exact = xe @ we.T
+    near(y[-200:, -300:], exact, rounded(sum_bound(xe, we), exact, torch.bfloat16))
+    del y, few
+
+
+def test_refusals_on_the_device():
+    x, w = case(5, 64, 256)
+    out = torch.empty(5, 64, device=DEV)
+    for bad, what in ((dict(x=x.half()), "float16"), (dict(x=x[:, :128]), "256 numbers"), (dict(out=out[:4]), "shape"), (dict(out=out.half()), "float16"),
+                      (dict(x=x.cpu()), "CUDA"), (dict(out=out.cpu()), "CUDA"), (dict(out=torch.empty(64, 5, device=DEV).T), "packed"),
+                      (dict(x=x.t().contiguous().t()), "packed"), (dict(out=torch.empty(64, device=DEV).expand(5, 64)), "over one another"), (dict(x=x[0]), "dimensions")):
+        args = dict(x=x, w=w, out=out) | bad
+        with pytest.raises(kernels.KernelError, match=what):
+            kernels.linear_fp8(**args)
+    g = gen(18)
+    up, down = (kernels.fp8_quantize(rows_of(g, 3 * a, b, torch.bfloat16).view(3, a, b)) for a, b in ((64, 256), (256, 64)))
+    ids, weights, y = routed(g, 5, 2, 3, "even"), torch.rand(5, 2, device=DEV), torch.empty(5, 256, device=DEV)
+    for bad, what in ((dict(ids=ids.long()), "int32"), (dict(ids=ids[:4]), "ids"), (dict(weights=weights.double()), "float32"), (dict(weights=weights[:, :1]), "float32"),
+                      (dict(up=w), "follow"), (dict(down=up), "follow"), (dict(activation="silu"), "relu2"), (dict(out=y[:3]), "shape"), (dict(x=x[:, :8]), "256 numbers")):
+        args = dict(x=x, ids=ids, weights=weights, up=up, down=down, out=y, activation="relu2") | bad
+        with pytest.raises(kernels.KernelError, match=what):
+            kernels.experts_fp8(**args)
+    with pytest.raises(kernels.KernelError, match="contiguous"):
+        kernels.fp8_quantize(torch.zeros(2, 4, 8, device=DEV).transpose(0, 1))
+    none = torch.empty(5, 256, device=DEV)
+    kernels.experts_fp8(x, ids[:, :0].contiguous(), weights[:, :0].contiguous(), up, down, none, "relu2")
+    assert bool((none == 0).all())
