@@ -117,7 +117,18 @@ struct ProductCall {             // brolm_fp8_stream, brolm_fp8_gemm and, with t
     int experts;
     const void *tile_group, *tile_row0, *offsets, *perm, *scale;
     int group_rows, down, top, tokens, rows, max_tiles;
+    // rows that are still to be rounded into x and x_scales, by brolm_fp8_quantize ahead of the product (null: they are there)
+    int (*quantize)(const RowsCall*);
+    const void* raw;
+    long long ld_raw;
+    int raw_dtype;
 };
+static inline int round_first(const ProductCall* c) {
+    if (!c->quantize) return BROLM_OK;
+    const RowsCall r = {const_cast<void*>(c->raw), const_cast<void*>(c->x), const_cast<void*>(c->x_scales), c->stream, c->ld_raw, c->ldx, c->M,
+                        c->raw_dtype, c->K, c->M, c->M, 1};
+    return c->quantize(&r);
+}
 
 // ---- host: rows x cols bytes, row-major with `ld` bytes between rows; box = box_rows x 128 columns, 128-byte swizzle
 static inline int make_map_u8(CUtensorMap* map, const void* ptr, long long rows, long long cols, long long ld, int box_rows) {

@@ -343,10 +343,10 @@ int group_gather(const RowsArgs& x, const int32_t* ids, int P, int E, int top, c
 }  // namespace
 
 // A pass.  x [tokens, K] (float or bfloat16, ldx elements between rows), ids [tokens, top]; up [experts] matrices of up_rows rows
-// (gated: 2 inter; a multiple of 128 rows apart), down of N.  Tiles have `rows` rows: up to 128 the experts' matrices are
-// streamed (`stream`), 256 they go to the pairs of SMs (`gemm`).  pairs [top, tokens, N] float; out (or null) the combined rows.
+// (gated: 2 inter; a multiple of 128 rows apart), down of N.  Tiles have `rows` rows: of 16 or 32 the experts'
+// matrices are streamed, of 256 they go to the pairs of SMs; `product` is the launcher of the one or the other.  pairs [top, tokens, N] float; out (or null) the combined rows.
 // scale (or null) [tokens, top] multiplies a pair's first sums, weights (or null, for ones) its result.  `work` holds
-// `work_bytes`: the order and the list, then both products' rows in 8 bits, then (rows <= 128) the first product's floats.
+// `work_bytes`: the order and the list, then both products' rows in 8 bits, then (streamed) the first product's floats.
 struct ExpertsCall {
     const void *x, *ids, *scale, *weights, *up, *up_scales, *down, *down_scales;
     void *pairs, *out, *work;
@@ -361,7 +361,7 @@ BROLM_API int brolm_fp8_experts(const ExpertsCall* c) {
     if (T <= 0 || top <= 0 || E <= 0 || c->N <= 0) return BROLM_OK;
     if (E > 4096 || (long long)T * top > 0x7fffffff / 2) return BROLM_ERR_TOO_LARGE;
     if (c->dtype != BROLM_BF16 && c->dtype != BROLM_F32) return BROLM_ERR_BAD_DTYPE;
-    if (rows != 16 && rows != 32 && rows != 64 && rows != 128 && rows != 256) return BROLM_ERR_BAD_SIZE;
+    if (rows != 16 && rows != 32 && rows != 256) return BROLM_ERR_BAD_SIZE;
     const int P = T * top, pad = (rows + 127) / 128 * 128, most = (P + rows - 1) / rows + (E < P ? E : P);
     const bool stream = rows <= 128;
     uint8_t* at = (uint8_t*)c->work;

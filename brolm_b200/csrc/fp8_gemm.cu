@@ -66,7 +66,7 @@ struct GemmArgs {
 };
 
 __device__ __forceinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile int* give_up, int code) {
-    return mbar_wait(bar, parity, give_up, &g_fp8_gemm_error, code);
+    return mbar_wait<4>(bar, parity, give_up, &g_fp8_gemm_error, code);      // (others begin to wait when a stalled one does)
 }
 // a wait that is mostly over when it begins
 __device__ __forceinline__ bool wait_one(uint32_t bar, uint32_t parity, volatile int* give_up, int code) {
@@ -262,6 +262,18 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     // (experts: how many tiles of rows there are stands behind the list's first rows)
     auto tiles_of = [&]() { return (EXPERTS ? g.offsets[g.experts + 1] : g.m_tiles) * g.n_tiles; };
 
+    // a stage's part of W and its scales; all of the stage's bytes, of both blocks, are counted here
+    auto load_w = [&](int s, int kb, int w_row, int each) {
+        const uint32_t full = full0 + 8 * s, s_dst = scale0 + s * SCALES;
+        const bool with_scales = (kb & 3) == 0;
+        if (rank == 0) mbar_expect_tx(full, 2 * (STAGE_BYTES + (with_scales ? SCALES : 0)));
+        tma_load_pair(stage0 + s * STAGE_BYTES + A_BYTES, &map_w, kb * BK, w_row + (int)rank * each, full);
+        if (with_scales) {
+            const int ws_row = w_row >> 7, q = kb >> 2;
+            tma_load_pair(s_dst + SF_TILE, &map_ws, 0, ws_row * g.quads + q, full);
+            tma_load_pair(s_dst + 2 * SF_TILE, &map_ws, 0, (ws_row + 1) * g.quads + q, full);
+        }
+    };
     if (warp < FIRST) {
     // 128 x 56 + 256 x 224 = 384 x 168, what a block is launched with
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
@@ -270,7 +282,17 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             int it = 0, s = 0, phase = 0;
             bool ok = !*give_up;
             // Launched with programmatic stream serialization: nothing of this kernel touches memory before its first
-            // operands have arrived, so (but for the experts' lists) the loader's wait is the kernel's.
+            // operands have arrived, so (but for the experts' lists) the loader's wait is the kernel's.  W depends on no
+            // kernel: the first stages' part of it is asked for before.
+            int early = 0;
+            if (!EXPERTS && ok) {
+                int whole, mt, nt, half_of, group, row0;
+                if (pair < items_of(tiles_of(), whole)) {
+                    find(pair, whole, mt, nt, half_of, group, row0);
+                    early = min(STAGES, g.nkb);
+                    for (int kb = 0; kb < early; ++kb) load_w(kb, kb, nt * BN + (half_of > 0 ? BN / 2 : 0), half_of < 0 ? HN : HN / 2);
+                }
+            }
             pdl_wait();
             int mt, nt, half_of, group, row0, whole;
             const int total = items_of(tiles_of(), whole);
@@ -278,20 +300,13 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                 find(item, whole, mt, nt, half_of, group, row0);
                 // half the columns: a block of the pair needs 64 rows of W (it is brought 128), the scales are one tile
                 const int w_row = group * g.group_rows + nt * BN + (half_of > 0 ? BN / 2 : 0), each = half_of < 0 ? HN : HN / 2;
-                const int xs_row = (EXPERTS ? mt * (PM / 128) : row0 >> 7) + (int)rank, ws_row = w_row >> 7;
+                const int xs_row = (EXPERTS ? mt * (PM / 128) : row0 >> 7) + (int)rank;
                 for (int kb = 0; kb < g.nkb; ++kb, ++it) {
                     if (!(kb > 0 ? wait_one(empty0 + 8 * s, phase ^ 1, give_up, 1) : wait_on(empty0 + 8 * s, phase ^ 1, give_up, 1))) { ok = false; break; }
-                    const uint32_t full = full0 + 8 * s, a_dst = stage0 + s * STAGE_BYTES, s_dst = scale0 + s * SCALES;
-                    const bool with_scales = (kb & 3) == 0;
-                    if (rank == 0) mbar_expect_tx(full, 2 * (STAGE_BYTES + (with_scales ? SCALES : 0)));   // both blocks' bytes
-                    tma_load_pair(a_dst, &map_x, kb * BK, row0 + (int)rank * BM, full);
-                    tma_load_pair(a_dst + A_BYTES, &map_w, kb * BK, w_row + (int)rank * each, full);
-                    if (with_scales) {
-                        const int q = kb >> 2;
-                        tma_load_pair(s_dst, &map_xs, 0, xs_row * g.quads + q, full);
-                        tma_load_pair(s_dst + SF_TILE, &map_ws, 0, ws_row * g.quads + q, full);
-                        tma_load_pair(s_dst + 2 * SF_TILE, &map_ws, 0, (ws_row + 1) * g.quads + q, full);
-                    }
+                    const uint32_t full = full0 + 8 * s;
+                    if (it >= early) load_w(s, kb, w_row, each);
+                    tma_load_pair(stage0 + s * STAGE_BYTES, &map_x, kb * BK, row0 + (int)rank * BM, full);
+                    if ((kb & 3) == 0) tma_load_pair(scale0 + s * SCALES, &map_xs, 0, xs_row * g.quads + (kb >> 2), full);
                     if (++s == STAGES) { s = 0; phase ^= 1; }
                 }
             }
@@ -600,7 +615,10 @@ BROLM_API int brolm_fp8_gemm(const fp8::ProductCall* c) {
     g.M = M; g.N = N; g.act = c->act; g.limit = c->limit; g.nkb = blocks_of(K);
     g.piece = c->out == OUT_F32 && c->cut > 0 && c->cut < g.nkb ? c->cut : g.nkb;
     g.m_tiles = (int)m_tiles; g.n_tiles = (int)n_tiles;
-    if (!c->experts) return dispatch<false>(m, g, c->epilogue, c->out, c->stream);
+    if (!c->experts) {
+        st = round_first(c);
+        return st ? st : dispatch<false>(m, g, c->epilogue, c->out, c->stream);
+    }
     g.tile_group = (const int32_t*)c->tile_group; g.tile_row0 = (const int32_t*)c->tile_row0; g.offsets = (const int32_t*)c->offsets;
     g.perm = (const int32_t*)c->perm; g.scale = (const float*)c->scale;
     g.down = c->down; g.top = c->top; g.tokens = c->tokens; g.group_rows = c->group_rows; g.experts = c->experts;

@@ -42,7 +42,7 @@ struct StreamArgs {
     void* y;
     long ldy;
     int M, N;                // rows of X (dense); output columns
-    int out_f32, act;
+    int out_f32, act, y_wide;
     float limit;
     int nkb, quads;          // blocks of K, words of scales
     int row_tiles, items, stages;
@@ -62,7 +62,7 @@ struct StreamArgs {
 };
 
 __device__ __forceinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile int* give_up, int code) {
-    return mbar_wait(bar, parity, give_up, &g_fp8_stream_error, code);
+    return mbar_wait<4>(bar, parity, give_up, &g_fp8_stream_error, code);      // (others begin to wait when a stalled one does)
 }
 // a wait that is mostly over when it begins: the flags are looked at only if it is not
 __device__ __forceinline__ bool wait_one(uint32_t bar, uint32_t parity, volatile int* give_up, int code) {
@@ -84,9 +84,10 @@ __device__ __forceinline__ uint32_t cluster_size() {
 __device__ __forceinline__ void cluster_sync_all() {
     asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float peer_float(uint32_t addr, uint32_t rank) {
-    float v;
-    asm volatile("{\n.reg .b32 r;\nmapa.shared::cluster.u32 r, %1, %2;\nld.shared::cluster.f32 %0, [r];\n}" : "=f"(v) : "r"(addr), "r"(rank));
+__device__ __forceinline__ float4 peer_floats(uint32_t addr, uint32_t rank) {
+    float4 v;
+    asm volatile("{\n.reg .b32 r;\nmapa.shared::cluster.u32 r, %4, %5;\nld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [r];\n}"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr), "r"(rank));
     return v;
 }
 __device__ __forceinline__ void put(const StreamArgs& g, long at, float v) {
@@ -385,23 +386,41 @@ __global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS, 2) fp8_stream_kerne
         __syncwarp();
         cluster_sync_all();
         if (warp >= 2 && warp < 6 && !*give_up) {
-            const uint32_t mine = smem_u32(sums);
-            const int t = threadIdx.x - 64, rt = first;
-            for (int r = slice; r < g.M; r += slices) {
-                float part[8], v = 0.0f;                        // (asked for together, added in their order)
+            // four neighbouring columns a thread, four rows at a time; the slices' numbers are asked for together
+            const int t = threadIdx.x - 64, at = (t & 31) * 4;
+            const uint32_t mine = smem_u32(sums) + at * 4;
+            for (int r = slice + (t >> 5) * slices; r < g.M; r += 4 * slices) {
+                float4 part[8];
+                float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int k = 0; k < 8; ++k) part[k] = k < slices ? peer_float(mine + (r * BR + t) * 4, k) : 0.0f;
+                for (int k = 0; k < 8; ++k) if (k < slices) part[k] = peer_floats(mine + r * BR * 4, k);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) if (k < slices) v += part[k];
-                int col = rt * BR + t;
-                if (EPI == EPI_GATED) {
-                    const float up = __shfl_down_sync(0xffffffffu, v, 1);
-                    v = gate_of(v, up, g.act, g.limit);
-                    col = (col & 1) ? g.N : col >> 1;
-                } else {
-                    v = act_of(v, g.act);
+                for (int k = 0; k < 8; ++k) {
+                    if (k < slices) { v[0] += part[k].x; v[1] += part[k].y; v[2] += part[k].z; v[3] += part[k].w; }
                 }
-                if (col < g.N) put(g, (long)r * g.ldy + col, v);
+                if (EPI == EPI_GATED) {
+                    const int col = (first * BR + at) >> 1;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) if (col + i < g.N) put(g, (long)r * g.ldy + col + i, gate_of(v[2 * i], v[2 * i + 1], g.act, g.limit));
+                } else {
+                    const int col = first * BR + at;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] = act_of(v[i], g.act);
+                    if (g.y_wide && col + 4 <= g.N) {
+                        if (g.out_f32) {
+                            *reinterpret_cast<float4*>((float*)g.y + (long)r * g.ldy + col) = make_float4(v[0], v[1], v[2], v[3]);
+                        } else {
+                            uint2 u;
+                            __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&u);
+                            h[0] = __floats2bfloat162_rn(v[0], v[1]);
+                            h[1] = __floats2bfloat162_rn(v[2], v[3]);
+                            *reinterpret_cast<uint2*>((bf16*)g.y + (long)r * g.ldy + col) = u;
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) if (col + i < g.N) put(g, (long)r * g.ldy + col + i, v[i]);
+                    }
+                }
             }
         }
         __syncwarp();
@@ -453,8 +472,11 @@ int dispatch(const CUtensorMap& mw, const CUtensorMap& mx, const StreamArgs& g, 
     }
     if (bt == 16) return launch<16, EPI, EXPERTS, 0>(mw, mx, g, slices, stream);
     if (bt == 32) return launch<32, EPI, EXPERTS, 0>(mw, mx, g, slices, stream);
-    if (bt == 64) return launch<64, EPI, EXPERTS, 0>(mw, mx, g, slices, stream);
-    return launch<128, EPI, EXPERTS, 0>(mw, mx, g, slices, stream);
+    if constexpr (!EXPERTS) {
+        if (bt == 64) return launch<64, EPI, false, 0>(mw, mx, g, slices, stream);
+        return launch<128, EPI, false, 0>(mw, mx, g, slices, stream);
+    }
+    return BROLM_ERR_BAD_SIZE;
 }
 
 }  // namespace
@@ -464,7 +486,7 @@ int dispatch(const CUtensorMap& mw, const CUtensorMap& mx, const StreamArgs& g, 
 // Dense (experts 0): M <= 128; K is cut into `cut` slices (1 to 8), none of which is empty.  fused 1, 2: X are bfloat16, float
 // numbers (ldx elements between rows, x_scales unused), M <= 16, and a slice has at most FUSED_BLOCKS blocks of 128 of K.
 // Experts: M pairs' rows in the order of their experts, W the experts' matrices, group_rows (a multiple of 128) rows each.  The
-// list (expert, first row) of tiles of `rows` (16, 32, 64 or 128) rows and what it stands on come from brolm_fp8_group; x_scales
+// list (expert, first row) of tiles of `rows` (16 or 32) rows and what it stands on come from brolm_fp8_group; x_scales
 // has a tile of 128 rows for every tile of the list.  Y [M, N], or with `down` float [top, tokens, N]; `scale` (or null): a
 // number for every pair that multiplies its sums before the activation.
 BROLM_API int brolm_fp8_stream(const fp8::ProductCall* c) {
@@ -478,13 +500,14 @@ BROLM_API int brolm_fp8_stream(const fp8::ProductCall* c) {
     const long long w_rows = c->epilogue == EPI_GATED ? 2LL * N : N;
     StreamArgs g = {};
     g.y = c->y; g.ldy = (long)c->ldy; g.M = M; g.N = N; g.out_f32 = c->out; g.act = c->act; g.limit = c->limit;
+    g.y_wide = ((uintptr_t)c->y & 15) == 0 && c->ldy % 4 == 0;
     g.nkb = blocks_of(K); g.quads = quads_of(K);
     g.w_scales = (const uint8_t*)c->w_scales; g.x_scales = (const uint8_t*)c->x_scales;
     const long long row_tiles = (w_rows + BR - 1) / BR;
     CUtensorMap mw, mx;
     if (c->experts) {
         const int rows = c->rows;
-        if (c->group_rows % BR || (rows != 16 && rows != 32 && rows != 64 && rows != 128) || (c->down && !c->out)) return BROLM_ERR_BAD_SIZE;
+        if (c->group_rows % BR || (rows != 16 && rows != 32) || (c->down && !c->out)) return BROLM_ERR_BAD_SIZE;
         const long long all = (long long)c->experts * c->group_rows;
         if (all > 0x7fffffff || c->max_tiles * row_tiles > 0x7fffffff) return BROLM_ERR_TOO_LARGE;
         int st = make_map_u8(&mw, c->w, all, K, c->ldw, BR);
@@ -513,6 +536,8 @@ BROLM_API int brolm_fp8_stream(const fp8::ProductCall* c) {
         mx = mw;
     }
     g.row_tiles = g.items = (int)row_tiles;
+    st = round_first(c);
+    if (st) return st;
     if (c->epilogue == EPI_GATED) return dispatch<EPI_GATED, false>(mw, mx, g, bt, slices, c->fused, c->stream);
     return dispatch<EPI_STORE, false>(mw, mx, g, bt, slices, c->fused, c->stream);
 }

@@ -38,10 +38,10 @@ _raw_stream, _device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDev
 # struct, packed here as C lays it out, and the checks of a call's arguments are one expression; which of them failed is found
 # out only then.
 _ROWS = struct.Struct("@4P3q5i")
-_PRODUCT = struct.Struct("@7P3q8ifi5P6i")
+_PRODUCT = struct.Struct("@7P3q8ifi5P6i2Pqi")
 _EXPERTS = struct.Struct("@13P5q14if")
 _functions: dict = {}
-_products: dict = {}         # the launchers that a pass of experts is given
+_launchers: dict = {}        # by name, as other launchers are given them
 
 
 def _call(lib: str, name: str, packed: bytes, what: str) -> None:
@@ -49,6 +49,13 @@ def _call(lib: str, name: str, packed: bytes, what: str) -> None:
     if f is None:
         f = _functions[name] = _fn(lib, name, [c_char_p])
     _check(f(packed), what)
+
+
+def _launcher(lib: str, name: str) -> int:
+    f = _launchers.get(name)
+    if f is None:
+        f = _launchers[name] = cast(getattr(load_library(lib), name), c_void_p).value
+    return f
 
 
 class Fp8Matrix:
@@ -189,9 +196,11 @@ def fp8_slices(tiles: int, nkb: int, sms: int) -> int:
 
 
 def fp8_fused(rows: int, nkb: int, slices: int) -> bool:
-    """Whether the stream of W rounds the rows itself: every block those of its slice, four blocks of K of a row a warp."""
+    """Whether the stream of W rounds the rows itself: every block those of its slice, four blocks of K of a row a warp, and so
+    in one round of eight warps with four each.  A launch less, and every block's time: 8 rows 2,304 x 9,216 (slices of nine
+    blocks) 8.8 us fused and 9.8 not, 18,432 x 2,304 (all eighteen) 13.4 and 12.9."""
     per = (nkb + slices - 1) // slices
-    return rows <= FUSED_ROWS and per <= _FUSED_BLOCKS and rows * ((per + 6) // 4) <= 64
+    return rows <= FUSED_ROWS and per <= _FUSED_BLOCKS and rows * ((per + 6) // 4) <= 32
 
 
 def _act_code(what: str, w: Fp8Matrix, activation: str) -> int:
@@ -228,33 +237,45 @@ def _checked(what: str, x, w: Fp8Matrix, out: torch.Tensor, outputs: int) -> Non
     raise KernelError(f"{what}: the rows, the matrix and the result live on {x.device}, {w.device} and {out.device}; the current device is cuda:{_device()}")
 
 
-_NO_EXPERTS = (0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
+_NO_EXPERTS = (0,) * 12
+_THERE = (0, 0, 0, 0)        # rows in 8 bits already
+
+
+@functools.lru_cache(maxsize=1024)
+def fp8_streamed(rows: int, w_rows: int, nkb: int, sms: int) -> bool:
+    """Whether a product streams W (128 rows of it at a time) or goes in tiles of 256 x 256.  Up to 64 rows it does; up to 128
+    but where the tiles come out as one round of the pairs of SMs that is nearly full, or K is short: 128 rows 18,432 x 2,304
+    (72 tiles) 17.7 us streamed and 14.0 in tiles, 1,000 x 640 6.9 and 5.3, but 2,304 x 9,216 (9 tiles) 12.5 and 23.1, 28,672 x
+    3,584 (112 tiles) 28.8 and 29.2; 64 rows 13.7 and 14.0, 5.1 and 5.1."""
+    if rows <= 64 or rows > STREAM_ROWS:
+        return rows <= 64
+    tiles, pairs = (w_rows + 255) // 256, sms // 2
+    return not (nkb <= 6 or (4 * tiles >= 3 * pairs and tiles <= pairs and nkb <= 32))
 
 
 def _product(x, M: int, w: Fp8Matrix, y: tuple, out: int, act: int, limit: float) -> None:
     """``x``: a tensor of rows, or 8-bit rows as (values, scales, stride); ``y`` (result, its scales, stride), ``out`` its kind."""
-    K, N = w.cols, w.outputs
+    K, N, device = w.cols, w.outputs, w.index
     if not M or not N:
         return
-    device = w.index
-    stream = _raw_stream(device)
-    held = None
-    if M <= STREAM_ROWS and out != 2:
-        nkb = (K + 127) >> 7
-        cut = fp8_slices((w.rows + 127) >> 7, nkb, device_sms(w.device))
-        fused, lib, name = 0, "fp8_stream", "brolm_fp8_stream"
+    sms, nkb = device_sms(w.device), (K + 127) >> 7
+    fused, held, raw = 0, None, _THERE
+    if out != 2 and fp8_streamed(M, w.rows, nkb, sms):
+        cut, lib, name = fp8_slices((w.rows + 127) >> 7, nkb, sms), "fp8_stream", "brolm_fp8_stream"
         if type(x) is not tuple and fp8_fused(M, nkb, cut):
             fused = _FUSED[x.dtype]
             x = (x.data_ptr(), 0, x.stride(0))
     else:
-        fused, cut, lib, name = 0, _PIECE, "fp8_gemm", "brolm_fp8_gemm"
+        cut, lib, name = _PIECE, "fp8_gemm", "brolm_fp8_gemm"
     if type(x) is not tuple:
+        # rounded by a kernel ahead of the product, from the same call
         held, packed = _scratch(M, K, w.device)
-        _quantize(x, packed, M, M, 1)
+        raw = (_launcher("fp8_rows", "brolm_fp8_quantize"), x.data_ptr(), x.stride(0), _CODES[x.dtype])
         x = packed
+        add_launches(1)
     wv, ws, ldw = w.packed
-    _call(lib, name, _PRODUCT.pack(x[0], x[1], wv, ws, y[0], y[1], stream, x[2], ldw, y[2], M, N, K, 1 if w.gated else 0, act, out, fused, cut, limit,
-                                   *_NO_EXPERTS), "linear_fp8")
+    _call(lib, name, _PRODUCT.pack(x[0], x[1], wv, ws, y[0], y[1], _raw_stream(device), x[2], ldw, y[2], M, N, K, 1 if w.gated else 0, act, out, fused, cut, limit,
+                                   *_NO_EXPERTS, *raw), "linear_fp8")
 
 
 def linear_fp8(x, w: Fp8Matrix, out: torch.Tensor, activation: str = "none", limit: float = 0.0) -> None:
@@ -277,7 +298,7 @@ def feedforward_fp8(x, gate_up: Fp8Matrix, down: Fp8Matrix, out: torch.Tensor, a
     if type(x) is Fp8Matrix:
         x = x.packed
     y = (out.data_ptr(), 0, out.stride(0))
-    if M <= STREAM_ROWS:
+    if fp8_streamed(M, gate_up.rows, (gate_up.cols + 127) >> 7, device_sms(down.device)):
         # (a stream's tile holds parts of a block only)
         h = torch.empty((M, inter), dtype=_F32, device=down.device)
         _product(x, M, gate_up, (h.data_ptr(), 0, inter), 1, act, limit)
@@ -289,12 +310,11 @@ def feedforward_fp8(x, gate_up: Fp8Matrix, down: Fp8Matrix, out: torch.Tensor, a
 
 # --- routed experts -----------------------------------------------------------
 def experts_fp8_rows(pairs: int, experts: int) -> int:
-    """How many rows a tile of an expert's pairs has."""
+    """How many rows a tile of an expert's pairs has: 16 or 32 with the experts' matrices streamed, 256 on pairs of SMs.  32 experts
+    of 2,048 x 1,024, 4 a token, with 16 / 32 / 256: 128 tokens (16 pairs an expert) 75 / 75 / 87 us, 256 82 / 86 / 90, 512 105 /
+    99 / 91; 8 experts, 2 a token: 128 (32) 42 / 41 / 45, 256 (64) 50 / 46 / 48, 512 (128) - / 58 / 50."""
     mean = pairs / max(experts, 1)
-    for rows in (16, 32, 64, 128):
-        if mean <= 0.75 * rows:
-            return rows
-    return 256
+    return 16 if mean <= 16 else 32 if mean <= 48 else 256
 
 
 def _experts_checked(what: str, x, ids, up: Fp8Matrix, down: Fp8Matrix, scale) -> None:
@@ -334,7 +354,7 @@ def _experts(what: str, x, ids, up: Fp8Matrix, down: Fp8Matrix, pairs, out, acti
     need = 3 * up512(4 * P) + up512(4 * E + 8) + 2 * up512(4 * most)
     for cols in (K, inter):
         need += up512(P * ((cols + 15) & -16)) + ((rows + 127) >> 7) * most * ((cols + 511) >> 9) * _TILE
-    if rows <= STREAM_ROWS:
+    if rows < 256:
         need += up512(4 * P * inter)
     held = None
     if pairs is None:
@@ -342,10 +362,7 @@ def _experts(what: str, x, ids, up: Fp8Matrix, down: Fp8Matrix, pairs, out, acti
         y = held.data_ptr() + need
     else:
         held, y = torch.empty(need, dtype=torch.uint8, device=x.device), pairs.data_ptr()
-    lib = "fp8_stream" if rows <= STREAM_ROWS else "fp8_gemm"
-    product = _products.get(lib)
-    if product is None:
-        product = _products[lib] = cast(getattr(load_library(lib), "brolm_" + lib), c_void_p).value
+    product = _launcher("fp8_gemm", "brolm_fp8_gemm") if rows == 256 else _launcher("fp8_stream", "brolm_fp8_stream")
     pack = _EXPERTS.pack(x.data_ptr(), ids.data_ptr(), scale.data_ptr() if scale is not None else 0, weights.data_ptr() if weights is not None else 0,
                          up.packed[0], up.packed[1], down.packed[0], down.packed[1], y, out.data_ptr() if out is not None else 0, held.data_ptr(),
                          _raw_stream(x.get_device()), product, x.stride(0), up.packed[2], down.packed[2], out.stride(0) if out is not None else 0, need,
@@ -353,7 +370,7 @@ def _experts(what: str, x, ids, up: Fp8Matrix, down: Fp8Matrix, pairs, out, acti
                          1 if out is not None and out.dtype == _F32 else 0, limit)
     _call("fp8_experts", "brolm_fp8_experts", pack, what)
     # (a call counts as one launch: the others of this pass)
-    add_launches((1 if P > 256 or E > 256 else 0) + 2 + (1 if rows <= STREAM_ROWS else 0) + (1 if out is not None else 0))
+    add_launches((1 if P > 256 or E > 256 else 0) + 2 + (1 if rows < 256 else 0) + (1 if out is not None else 0))
 
 
 def experts_fp8_pairs(x: torch.Tensor, ids: torch.Tensor, up: Fp8Matrix, down: Fp8Matrix, out: torch.Tensor, activation: str = "silu",

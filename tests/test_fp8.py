@@ -73,3 +73,14 @@ def test_model_refuses_other_types():
         bb.Model(bb.Gemma2Config(**TINY_A), device="cpu", weight_dtype="int4")
     with pytest.raises(kernels.KernelError, match="CUDA"):
         bb.Model(bb.Gemma2Config(**TINY_A), device="cpu", weight_dtype="fp8").init_random(0)
+
+
+@pytest.mark.parametrize("rows, w_rows, nkb, streamed", [(1, 100, 1, True), (64, 18432, 18, True), (65, 18432, 18, False), (128, 18432, 18, False), (128, 2304, 72, True),
+                                                         (128, 28672, 28, True), (128, 1000, 5, False), (129, 2304, 72, False)])
+def test_which_products_stream_their_matrix(rows, w_rows, nkb, streamed):
+    assert fp8.fp8_streamed(rows, w_rows, nkb, 148) is streamed
+
+
+@pytest.mark.parametrize("pairs, experts, rows", [(1, 32, 16), (512, 32, 16), (513, 32, 32), (1536, 32, 32), (1537, 32, 256), (5, 1, 16), (100000, 8, 256), (3, 0, 16)])
+def test_rows_of_an_experts_tile(pairs, experts, rows):
+    assert fp8.experts_fp8_rows(pairs, experts) == rows
