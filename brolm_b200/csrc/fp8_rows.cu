@@ -147,3 +147,10 @@ BROLM_API int brolm_fp8_read(const fp8::RowsCall* c) {
     return launch_pdl(read_kernel<float>, grid, block, 0, c->stream, g, (float*)c->x, (long)c->ldx, base && c->ldx % 4 == 0);
 }
 
+
+// Two products one after the other, from one call of the host.
+BROLM_API int brolm_fp8_two(const fp8::ProductCall* a, int (*first)(const fp8::ProductCall*), const fp8::ProductCall* b,
+                            int (*second)(const fp8::ProductCall*)) {
+    const int st = first(a);
+    return st ? st : second(b);
+}

@@ -107,14 +107,6 @@ def _empty(shape: tuple, device, gated: bool = False) -> Fp8Matrix:
     return Fp8Matrix(torch.empty(_bytes(rows, shape[-1], rows), dtype=torch.uint8, device=device), shape, gated)
 
 
-def _scratch(rows: int, cols: int, device, scale_rows: Optional[int] = None) -> tuple:
-    """Room for rows in 8 bits within one call: what keeps it alive, and values, scales and stride as a launcher takes them."""
-    ld = (cols + 15) & -16
-    held = torch.empty(_bytes(rows, cols, scale_rows or rows), dtype=torch.uint8, device=device)
-    at = held.data_ptr()
-    return held, (at, at + ((rows * ld + 511) & -512), ld)
-
-
 def _refuse(what: str, t: torch.Tensor, name: str, dim: int = 2) -> None:
     """Names what is wrong with a tensor of rows; returns if nothing is."""
     if t.dtype not in _CODES:
@@ -195,12 +187,13 @@ def fp8_slices(tiles: int, nkb: int, sms: int) -> int:
     return best
 
 
-def fp8_fused(rows: int, nkb: int, slices: int) -> bool:
-    """Whether the stream of W rounds the rows itself: every block those of its slice, four blocks of K of a row a warp, and so
-    in one round of eight warps with four each.  A launch less, and every block's time: 8 rows 2,304 x 9,216 (slices of nine
-    blocks) 8.8 us fused and 9.8 not, 18,432 x 2,304 (all eighteen) 13.4 and 12.9."""
+def fp8_fused(rows: int, nkb: int, slices: int, words: int) -> bool:
+    """Whether the stream of W rounds the rows itself: every block those of its slice, four blocks of K of a row (``words`` words
+    of sixteen bytes a lane: 2 for bfloat16, 4 for float32) a warp, eight warps with eight such words each in one round.  A
+    launch less, and every block's time: 8 bfloat16 rows 2,304 x 9,216 (slices of nine blocks) 8.8 us fused and 9.8 not, float32
+    rows 10.2 and 8.6, 18,432 x 2,304 (all eighteen) 13.4 and 12.9."""
     per = (nkb + slices - 1) // slices
-    return rows <= FUSED_ROWS and per <= _FUSED_BLOCKS and rows * ((per + 6) // 4) <= 32
+    return rows <= FUSED_ROWS and per <= _FUSED_BLOCKS and rows * ((per + 6) // 4) * words <= 64
 
 
 def _act_code(what: str, w: Fp8Matrix, activation: str) -> int:
@@ -253,29 +246,34 @@ def fp8_streamed(rows: int, w_rows: int, nkb: int, sms: int) -> bool:
     return not (nkb <= 6 or (4 * tiles >= 3 * pairs and tiles <= pairs and nkb <= 32))
 
 
-def _product(x, M: int, w: Fp8Matrix, y: tuple, out: int, act: int, limit: float) -> None:
-    """``x``: a tensor of rows, or 8-bit rows as (values, scales, stride); ``y`` (result, its scales, stride), ``out`` its kind."""
-    K, N, device = w.cols, w.outputs, w.index
-    if not M or not N:
-        return
-    sms, nkb = device_sms(w.device), (K + 127) >> 7
-    fused, held, raw = 0, None, _THERE
-    if out != 2 and fp8_streamed(M, w.rows, nkb, sms):
-        cut, lib, name = fp8_slices((w.rows + 127) >> 7, nkb, sms), "fp8_stream", "brolm_fp8_stream"
-        if type(x) is not tuple and fp8_fused(M, nkb, cut):
-            fused = _FUSED[x.dtype]
-            x = (x.data_ptr(), 0, x.stride(0))
-    else:
-        cut, lib, name = _PIECE, "fp8_gemm", "brolm_fp8_gemm"
-    if type(x) is not tuple:
-        # rounded by a kernel ahead of the product, from the same call
-        held, packed = _scratch(M, K, w.device)
-        raw = (_launcher("fp8_rows", "brolm_fp8_quantize"), x.data_ptr(), x.stride(0), _CODES[x.dtype])
-        x = packed
-        add_launches(1)
+def _rounded(M: int, K: int, w_rows: int, out: int, words: int, sms: int) -> tuple:
+    """How a product goes: (streamed, the cut of K, whether the stream rounds the rows itself); ``words`` as ``fp8_fused`` has
+    them, 0 for rows in 8 bits."""
+    nkb = (K + 127) >> 7
+    if out != 2 and fp8_streamed(M, w_rows, nkb, sms):
+        cut = fp8_slices((w_rows + 127) >> 7, nkb, sms)
+        return True, cut, words > 0 and fp8_fused(M, nkb, cut, words)
+    return False, _PIECE, False
+
+
+_rounded = functools.lru_cache(maxsize=4096)(_rounded)
+
+
+def _pack(how: tuple, x, at: int, M: int, w: Fp8Matrix, y: tuple, out: int, act: int, limit: float, stream: int) -> bytes:
+    """A product's struct.  ``x``: (values, scales, stride) of rows in 8 bits, or (numbers, 0, stride, type) of rows that are
+    rounded on the way, into the scratch at ``at`` if not by the product itself."""
+    K = w.cols
+    fused, raw = 0, _THERE
+    if len(x) == 4:
+        if how[2]:
+            fused = _FUSED[x[3]]
+        else:
+            ld = (K + 15) & -16
+            raw = (_launcher("fp8_rows", "brolm_fp8_quantize"), x[0], x[2], _CODES[x[3]])
+            x = (at, at + ((M * ld + 511) & -512), ld)
     wv, ws, ldw = w.packed
-    _call(lib, name, _PRODUCT.pack(x[0], x[1], wv, ws, y[0], y[1], _raw_stream(device), x[2], ldw, y[2], M, N, K, 1 if w.gated else 0, act, out, fused, cut, limit,
-                                   *_NO_EXPERTS, *raw), "linear_fp8")
+    return _PRODUCT.pack(x[0], x[1], wv, ws, y[0], y[1], stream, x[2], ldw, y[2], M, w.outputs, K, 1 if w.gated else 0, act, out, fused, how[1], limit,
+                         *_NO_EXPERTS, *raw)
 
 
 def linear_fp8(x, w: Fp8Matrix, out: torch.Tensor, activation: str = "none", limit: float = 0.0) -> None:
@@ -284,7 +282,25 @@ def linear_fp8(x, w: Fp8Matrix, out: torch.Tensor, activation: str = "none", lim
     of ``ACTIVATIONS``: act(gate) * partner.  ``out`` does not lie over x or the matrix."""
     act = _act_code("linear_fp8", w, activation)
     _checked("linear_fp8", x, w, out, w.outputs)
-    _product(x.packed if type(x) is Fp8Matrix else x, x.shape[0], w, (out.data_ptr(), 0, out.stride(0)), _OUT[out.dtype], act, limit)
+    M, K, device = x.shape[0], w.cols, w.index
+    if not M or not w.outputs:
+        return
+    held, at = None, 0
+    if type(x) is Fp8Matrix:
+        x = x.packed
+        how = _rounded(M, K, w.rows, 0, 0, device_sms(w.device))
+    else:
+        how = _rounded(M, K, w.rows, 0, x.element_size(), device_sms(w.device))
+        if not how[2]:
+            held = torch.empty(_bytes(M, K, M), dtype=torch.uint8, device=w.device)
+            at = held.data_ptr()
+            add_launches(1)
+        x = (x.data_ptr(), 0, x.stride(0), x.dtype)
+    packed = _pack(how, x, at, M, w, (out.data_ptr(), 0, out.stride(0)), _OUT[out.dtype], act, limit, _raw_stream(device))
+    if how[0]:
+        _call("fp8_stream", "brolm_fp8_stream", packed, "linear_fp8")
+    else:
+        _call("fp8_gemm", "brolm_fp8_gemm", packed, "linear_fp8")
 
 
 def feedforward_fp8(x, gate_up: Fp8Matrix, down: Fp8Matrix, out: torch.Tensor, activation: str = "gelu_tanh", limit: float = 0.0) -> None:
@@ -294,18 +310,33 @@ def feedforward_fp8(x, gate_up: Fp8Matrix, down: Fp8Matrix, out: torch.Tensor, a
         raise KernelError(f"feedforward_fp8: matrices of shapes {gate_up.shape} and {down.shape} do not follow one another")
     act = _act_code("feedforward_fp8", gate_up, activation)
     _checked("feedforward_fp8", x, gate_up, out, down.rows)
-    M, inter = x.shape[0], down.cols
-    if type(x) is Fp8Matrix:
-        x = x.packed
-    y = (out.data_ptr(), 0, out.stride(0))
-    if fp8_streamed(M, gate_up.rows, (gate_up.cols + 127) >> 7, device_sms(down.device)):
-        # (a stream's tile holds parts of a block only)
-        h = torch.empty((M, inter), dtype=_F32, device=down.device)
-        _product(x, M, gate_up, (h.data_ptr(), 0, inter), 1, act, limit)
-    else:
-        held, h = _scratch(M, inter, down.device)
-        _product(x, M, gate_up, h, 2, act, limit)
-    _product(h, M, down, y, _OUT[out.dtype], 0, 0.0)
+    M, inter, device = x.shape[0], down.cols, down.index
+    if not M or not down.rows:
+        return
+    sms = device_sms(down.device)
+    # what lies between is rounded by the first product's own end where it goes in tiles (a stream's tile holds parts of a block
+    # only, and leaves floats)
+    words = 0 if type(x) is Fp8Matrix else x.element_size()
+    first = _rounded(M, gate_up.cols, gate_up.rows, 0, words, sms)
+    floats = first[0]
+    second = _rounded(M, inter, down.rows, 0, 4 if floats else 0, sms)
+    # one room: x in 8 bits, what lies between in 8 bits, as floats
+    x8 = _bytes(M, gate_up.cols, M) if words and not first[2] else 0
+    h8 = 0 if second[2] else _bytes(M, inter, M)
+    held = torch.empty(x8 + h8 + (4 * M * inter if floats else 0), dtype=torch.uint8, device=down.device)
+    at = held.data_ptr()
+    x = x.packed if not words else (x.data_ptr(), 0, x.stride(0), x.dtype)
+    ld = (inter + 15) & -16
+    between = (at + x8, at + x8 + ((M * ld + 511) & -512), ld)
+    stream = _raw_stream(device)
+    a = _pack(first, x, at, M, gate_up, (at + x8 + h8, 0, inter) if floats else between, 1 if floats else 2, act, limit, stream)
+    b = _pack(second, (at + x8 + h8, 0, inter, _F32) if floats else between, at + x8, M, down, (out.data_ptr(), 0, out.stride(0)), _OUT[out.dtype], 0, 0.0, stream)
+    f = _functions.get("brolm_fp8_two")
+    if f is None:
+        f = _functions["brolm_fp8_two"] = _fn("fp8_rows", "brolm_fp8_two", [c_char_p, c_void_p, c_char_p, c_void_p])
+    launch = lambda streamed: _launcher("fp8_stream", "brolm_fp8_stream") if streamed else _launcher("fp8_gemm", "brolm_fp8_gemm")
+    _check(f(a, launch(first[0]), b, launch(second[0])), "feedforward_fp8")
+    add_launches(1 + (1 if x8 else 0) + (1 if floats and h8 else 0))
 
 
 # --- routed experts -----------------------------------------------------------
