@@ -117,6 +117,7 @@ struct ProductCall {             // brolm_fp8_stream, brolm_fp8_gemm and, with t
     int experts;
     const void *tile_group, *tile_row0, *offsets, *perm, *scale;
     int group_rows, down, top, tokens, rows, max_tiles;
+    int listed;                  // the list is older than the kernel before, which has waited for its own predecessor before it let this one begin
     // rows that are still to be rounded into x and x_scales, by brolm_fp8_quantize ahead of the product (null: they are there)
     int (*quantize)(const RowsCall*);
     const void* raw;

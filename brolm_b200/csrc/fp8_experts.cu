@@ -208,9 +208,9 @@ template <typename T, bool WIDE>
 __global__ void __launch_bounds__(THREADS) gather_kernel(RowsArgs g, const int32_t* __restrict__ place, const int32_t* __restrict__ scale_row, int top) {
     const int lane = threadIdx.x & 31, quad = blockIdx.x, c = quad * 512 + lane * 16;
     pdl_wait();
+    pdl_trigger();                                      // (a product fetches its matrices meanwhile)
     for (long row = (long)blockIdx.y * WARPS + (threadIdx.x >> 5); row < g.rows; row += (long)gridDim.y * WARPS)
         gather_row<T, WIDE>(g, row, quad, c, lane, place, scale_row, top);
-    pdl_trigger();
 }
 
 // Both at once for up to 256 pairs of up to 256 experts (a step of decoding): every block sorts them for itself, one pair a
@@ -404,7 +404,9 @@ BROLM_API int brolm_fp8_experts(const ExpertsCall* c) {
     }
     p.x = h.values; p.x_scales = h.scales; p.ldx = h.ldv; p.w = c->down; p.w_scales = c->down_scales; p.ldw = c->down_ld;
     p.y = c->pairs; p.y_scales = nullptr; p.ldy = c->N; p.out = 1; p.N = c->N; p.K = c->inter; p.epilogue = 0; p.act = 0; p.limit = 0.0f;
-    p.scale = nullptr; p.group_rows = c->down_rows; p.down = 1;
+    // (the kernel before, the first product or the rounding of its results, has waited before it lets this one begin, and so has
+    // the list been written)
+    p.scale = nullptr; p.group_rows = c->down_rows; p.down = 1; p.listed = 1;
     st = c->product(&p);
     if (st || !c->out) return st;
     const dim3 grid(T, (c->N + 4 * THREADS - 1) / (4 * THREADS)), block(THREADS);

@@ -62,7 +62,7 @@ struct GemmArgs {
     const int32_t* offsets;
     const int32_t* perm;
     const float* scale;
-    int down, top, tokens, group_rows, experts;
+    int down, top, tokens, group_rows, experts, listed;
 };
 
 __device__ __forceinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile int* give_up, int code) {
@@ -256,11 +256,11 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         }
         mt = tile / g.n_tiles;
         nt = tile - mt * g.n_tiles;
-        group = g.tile_group[mt];
-        row0 = g.tile_row0[mt];
+        group = __ldcg(&g.tile_group[mt]);               // (perhaps read before this kernel's wait)
+        row0 = __ldcg(&g.tile_row0[mt]);
     };
     // (experts: how many tiles of rows there are stands behind the list's first rows)
-    auto tiles_of = [&]() { return (EXPERTS ? g.offsets[g.experts + 1] : g.m_tiles) * g.n_tiles; };
+    auto tiles_of = [&]() { return (EXPERTS ? __ldcg(&g.offsets[g.experts + 1]) : g.m_tiles) * g.n_tiles; };
 
     // a stage's part of W and its scales; all of the stage's bytes, of both blocks, are counted here
     auto load_w = [&](int s, int kb, int w_row, int each) {
@@ -283,14 +283,14 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             bool ok = !*give_up;
             // Launched with programmatic stream serialization: nothing of this kernel touches memory before its first
             // operands have arrived, so (but for the experts' lists) the loader's wait is the kernel's.  W depends on no
-            // kernel: the first stages' part of it is asked for before.
+            // kernel: the first stages' part of it is asked for before (experts': where their list is known by then).
             int early = 0;
-            if (!EXPERTS && ok) {
+            if ((!EXPERTS || g.listed) && ok) {
                 int whole, mt, nt, half_of, group, row0;
                 if (pair < items_of(tiles_of(), whole)) {
                     find(pair, whole, mt, nt, half_of, group, row0);
                     early = min(STAGES, g.nkb);
-                    for (int kb = 0; kb < early; ++kb) load_w(kb, kb, nt * BN + (half_of > 0 ? BN / 2 : 0), half_of < 0 ? HN : HN / 2);
+                    for (int kb = 0; kb < early; ++kb) load_w(kb, kb, group * g.group_rows + nt * BN + (half_of > 0 ? BN / 2 : 0), half_of < 0 ? HN : HN / 2);
                 }
             }
             pdl_wait();
@@ -621,7 +621,7 @@ BROLM_API int brolm_fp8_gemm(const fp8::ProductCall* c) {
     }
     g.tile_group = (const int32_t*)c->tile_group; g.tile_row0 = (const int32_t*)c->tile_row0; g.offsets = (const int32_t*)c->offsets;
     g.perm = (const int32_t*)c->perm; g.scale = (const float*)c->scale;
-    g.down = c->down; g.top = c->top; g.tokens = c->tokens; g.group_rows = c->group_rows; g.experts = c->experts;
+    g.down = c->down; g.top = c->top; g.tokens = c->tokens; g.group_rows = c->group_rows; g.experts = c->experts; g.listed = c->listed;
     return dispatch<true>(m, g, c->epilogue, c->out, c->stream);
 }
 

@@ -31,6 +31,9 @@ __global__ void __launch_bounds__(THREADS) quantize_kernel(RowsArgs g) {
     const int lane = threadIdx.x & 31;
     const long items = g.rows * g.quads;
     pdl_wait();
+    // The products read their matrix before they wait for the kernel before them, so a kernel that writes a matrix lets
+    // nothing begin before it has ended; one that writes rows that a product waits for lets it begin at once.
+    if (g.early) pdl_trigger();
     for (long item = (long)blockIdx.x * WARPS + (threadIdx.x >> 5); item < items; item += (long)gridDim.x * WARPS) {
         const long row = items <= 0xffffffffl ? (long)((uint32_t)item / (uint32_t)g.quads) : item / g.quads;    // (a long division is 70 instructions)
         const int quad = (int)(item - row * g.quads), c = quad * 512 + lane * 16;
@@ -45,9 +48,6 @@ __global__ void __launch_bounds__(THREADS) quantize_kernel(RowsArgs g) {
         if (c < g.ldv) *reinterpret_cast<uint4*>(g.values + at * g.ldv + c) = q;     // ldv is a multiple of 16
         if (lane == 0) *reinterpret_cast<uint32_t*>(g.scales + scale_at(at, quad, g.quads)) = word;
     }
-    // The products read their matrix before they wait for the kernel before them, so a kernel that writes a matrix lets
-    // nothing begin before it has ended; one that writes rows that a product waits for may.
-    if (g.early) pdl_trigger();
 }
 
 // For reading back the lanes' words lie side by side: eight bfloat16 numbers or four floats a word of sixteen bytes.  (With

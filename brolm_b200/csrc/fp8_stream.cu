@@ -59,6 +59,7 @@ struct StreamArgs {
     const int32_t* perm;
     const float* scale;      // of a pair, before the activation
     int down, top, tokens, group_rows;
+    int listed;
 };
 
 __device__ __forceinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile int* give_up, int code) {
@@ -202,9 +203,9 @@ __global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS, 2) fp8_stream_kerne
         }
         tile = item / g.row_tiles;
         rt = item - tile * g.row_tiles;
-        group = g.tile_group[tile];
+        group = __ldcg(&g.tile_group[tile]);             // (perhaps read before this kernel's wait)
         if (group < 0) return false;
-        row0 = g.tile_row0[tile];
+        row0 = __ldcg(&g.tile_row0[tile]);
         return true;
     };
 
@@ -228,15 +229,15 @@ __global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS, 2) fp8_stream_kerne
             };
             int item = first, kb = lo, it = 0, rt = 0, group = 0, row0 = 0, tile = 0;
             bool more;
-            if (EXPERTS) pdl_wait();                     // the list of tiles is an earlier kernel's
+            // The ring fills with weights before the kernel before this one has ended; experts' where their list is known by then.
+            const bool ahead = !EXPERTS || g.listed;
+            if (!ahead) pdl_wait();
             more = item < g.items && lo < hi && find(item, rt, group, row0, tile);
-            if (!EXPERTS) {
-                // the ring fills with weights before the kernel before this one has finished
-                const int rt0 = rt;
+            if (ahead) {
                 int n = 0;
-                for (; n < stages && lo + n < hi && more; ++n) load_w(n, rt0, 0, lo + n);
+                for (; n < stages && lo + n < hi && more; ++n) load_w(n, rt, group, lo + n);
                 pdl_wait();
-                for (int i = 0; i < n; ++i) load_x(i, 0, 0, lo + i);
+                for (int i = 0; i < n; ++i) load_x(i, row0, tile, lo + i);
                 it = n;
                 kb = lo + n;
                 if (more && kb >= hi) {
@@ -516,7 +517,7 @@ BROLM_API int brolm_fp8_stream(const fp8::ProductCall* c) {
         g.per = g.nkb; g.row_tiles = (int)row_tiles; g.items = (int)(row_tiles * c->max_tiles);
         g.tile_group = (const int32_t*)c->tile_group; g.tile_row0 = (const int32_t*)c->tile_row0; g.offsets = (const int32_t*)c->offsets;
         g.perm = (const int32_t*)c->perm; g.scale = (const float*)c->scale;
-        g.down = c->down; g.top = c->top; g.tokens = c->tokens; g.group_rows = c->group_rows;
+        g.down = c->down; g.top = c->top; g.tokens = c->tokens; g.group_rows = c->group_rows; g.listed = c->listed;
         if (c->epilogue == EPI_GATED) return dispatch<EPI_GATED, true>(mw, mx, g, rows, 1, 0, c->stream);
         return dispatch<EPI_STORE, true>(mw, mx, g, rows, 1, 0, c->stream);
     }

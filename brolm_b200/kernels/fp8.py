@@ -38,7 +38,7 @@ _raw_stream, _device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDev
 # struct, packed here as C lays it out, and the checks of a call's arguments are one expression; which of them failed is found
 # out only then.
 _ROWS = struct.Struct("@4P3q5i")
-_PRODUCT = struct.Struct("@7P3q8ifi5P6i2Pqi")
+_PRODUCT = struct.Struct("@7P3q8ifi5P7i2Pqi")
 _EXPERTS = struct.Struct("@13P5q14if")
 _functions: dict = {}
 _launchers: dict = {}        # by name, as other launchers are given them
@@ -230,7 +230,7 @@ def _checked(what: str, x, w: Fp8Matrix, out: torch.Tensor, outputs: int) -> Non
     raise KernelError(f"{what}: the rows, the matrix and the result live on {x.device}, {w.device} and {out.device}; the current device is cuda:{_device()}")
 
 
-_NO_EXPERTS = (0,) * 12
+_NO_EXPERTS = (0,) * 13
 _THERE = (0, 0, 0, 0)        # rows in 8 bits already
 
 
