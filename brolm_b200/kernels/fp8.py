@@ -178,7 +178,7 @@ _ACTS = {(gated, name): code for gated, table in ((True, ACTIVATIONS), (False, E
 def fp8_slices(tiles: int, nkb: int, sms: int) -> int:
     """Into how many slices K is cut for a product of few rows, ``tiles`` tiles of 128 rows of W and ``nkb`` blocks of K: as many
     as find room at a time (two blocks an SM, of which clusters leave an eighth empty), of two blocks of K at least.
-    8 rows, 1 / 4 / 8 slices: 2,304 x 9,216 27 / 9.3 / 7.1 us; 4,608 x 36,864 in 1 / 4 / 7 / 8: 107 / 36 / 31.6 / 36."""
+    8 rows in 8 bits, 1 / 4 / 8 slices: 2,304 x 9,216 17.8 / 7.9 / 6.7 us; 4,608 x 36,864 in 1 / 4 / 7 / 8: 68 / 31.4 / 28.4 / 37.1."""
     best = 1
     for s in range(2, 9):
         per = (nkb + s - 1) // s
