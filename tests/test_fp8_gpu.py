@@ -507,3 +507,28 @@ def test_refusals_on_the_device():
     none = torch.empty(5, 256, device=DEV)
     kernels.experts_fp8(x, ids[:, :0].contiguous(), weights[:, :0].contiguous(), up, down, none, "relu2")
     assert bool((none == 0).all())
+
+
+@pytest.mark.parametrize("m", [3, 40, 200])
+def test_products_of_very_small_and_very_large_numbers(m):
+    """Scales at both ends of their range meet in a product: 2^-127 (where nothing is smaller) with 2^100, their sums moderate."""
+    g = gen(19)
+    x, w = torch.randn(m, 512, generator=g, device=DEV), torch.randn(300, 512, generator=g, device=DEV)
+    x[:, :128] *= 2.0 ** -134                          # below the smallest scale's normal numbers
+    w[:, :128] *= 2.0 ** 115
+    x[:, 128:256] *= 2.0 ** -110
+    w[:, 128:256] *= 2.0 ** 108
+    x[:, 256:384] *= 2.0 ** 90
+    w[:, 256:384] *= 2.0 ** -100
+    x[1, 384:] = 0.0
+    y = torch.empty(m, 300, device=DEV)
+    kernels.linear_fp8(x, kernels.fp8_quantize(w), y)
+    xe, we = plain.values(x), plain.values(w)
+    near(y, xe @ we.T, sum_bound(xe, we))
+    for a, b in ((0, 128), (128, 256), (256, 384)):    # every block by itself
+        only = torch.zeros_like(x)
+        only[:, a:b] = x[:, a:b]
+        kernels.linear_fp8(only, kernels.fp8_quantize(w), y)
+        oe = plain.values(only)
+        assert float((oe @ we.T).abs().max()) > 0
+        near(y, oe @ we.T, sum_bound(oe, we))
