@@ -6,7 +6,8 @@
 // of the pair; with the first block of every four come their scales, 512 bytes for the block's rows of X and 1,024 for all 256
 // rows of W, which tcgen05.cp carries into both blocks' tensor memory.
 //
-//   warp 0 (both blocks)   one thread: TMA loads, their bytes counted on the first block's barrier
+//   warp 0 (both blocks)   one thread: TMA loads, their bytes counted on the first block's barrier; the first stages' part of W
+//                          before the kernel before this one has ended
 //   warp 1 (first block)   one thread: copies of scales, products, commits to both blocks
 //   warps 4-11 (both)      epilogue: a thread has a row of the tile and half of its columns, in up to 224 registers, which the first
 //                          four warps leave them (two of those are there for that alone: registers go by four warps)
@@ -312,7 +313,9 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             }
             pdl_trigger();                                  // the operands are asked for: the next kernel may move in
             if (*give_up && rank == 0) {
-                for (int j = max(0, it - STAGES); j < it; ++j) drain_on(full0 + 8 * (j % STAGES), (j / STAGES) & 1, give_up, 4);
+                // (a stage that has its part of W alone is never full: the wait for it is as long as the limit)
+                for (int asked = max(it, early), j = max(0, asked - STAGES); j < asked; ++j)
+                    drain_on(full0 + 8 * (j % STAGES), (j / STAGES) & 1, give_up, 4);
             }
         }
     } else if (warp == 1) {

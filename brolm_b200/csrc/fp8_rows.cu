@@ -48,6 +48,7 @@ __global__ void __launch_bounds__(THREADS) quantize_kernel(RowsArgs g) {
         if (c < g.ldv) *reinterpret_cast<uint4*>(g.values + at * g.ldv + c) = q;     // ldv is a multiple of 16
         if (lane == 0) *reinterpret_cast<uint32_t*>(g.scales + scale_at(at, quad, g.quads)) = word;
     }
+    if (!g.early) __threadfence();                  // (and its stores have arrived by then)
 }
 
 // For reading back the lanes' words lie side by side: eight bfloat16 numbers or four floats a word of sixteen bytes.  (With
@@ -146,7 +147,6 @@ BROLM_API int brolm_fp8_read(const fp8::RowsCall* c) {
     if (c->dtype != BROLM_F32) return BROLM_ERR_BAD_DTYPE;
     return launch_pdl(read_kernel<float>, grid, block, 0, c->stream, g, (float*)c->x, (long)c->ldx, base && c->ldx % 4 == 0);
 }
-
 
 // Two products one after the other, from one call of the host.
 BROLM_API int brolm_fp8_two(const fp8::ProductCall* a, int (*first)(const fp8::ProductCall*), const fp8::ProductCall* b,

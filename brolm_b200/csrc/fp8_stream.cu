@@ -7,8 +7,10 @@
 // four, the 512 bytes of scales of each side, which tcgen05.cp carries into tensor memory ahead of the products that need
 // them (copies and products of one thread are executed in order).
 //
-//   warp 0    one thread: TMA loads, and untiled copies of the scales' tiles
-//   warp 1    one thread: copies of scales and products into one of two accumulators, commits
+//   warp 0    one thread: TMA loads, and untiled copies of the scales' tiles; those of W begin before the kernel before this one
+//             has ended
+//   warp 1    one thread: copies of scales and products into one of two accumulators (128 rows of X: the one there is room for),
+//             commits
 //   warps 2-5 an accumulator's lane is a row of W, its column a row of X: epilogue, Y[row of X][row of W]
 //
 // Dense: X has up to 128 rows.  Where W has fewer tiles of 128 rows than the device has SMs, K is cut into slices that are the

@@ -159,6 +159,8 @@ def fp8_read(m: Fp8Matrix, out: torch.Tensor) -> None:
         raise KernelError(f"fp8_read: a matrix of shape {m.shape} goes into such a (packed) tensor, not into {tuple(out.shape)}")
     if m.device != out.device:
         raise KernelError("fp8_read: the matrix and the result live on two devices")
+    if out.dim() == 2 and out.shape[0] > 1 and out.stride(0) < out.shape[1]:
+        raise KernelError(f"fp8_read: the rows of the result lie over one another (strides {tuple(out.stride())})")
     if not out.numel():
         return
     y = out.view(-1, out.shape[-1]) if out.dim() == 3 else out

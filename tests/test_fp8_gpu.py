@@ -532,3 +532,56 @@ def test_products_of_very_small_and_very_large_numbers(m):
         oe = plain.values(only)
         assert float((oe @ we.T).abs().max()) > 0
         near(y, oe @ we.T, sum_bound(oe, we))
+
+
+def test_rows_that_lie_over_one_another_are_not_read_into():
+    m = kernels.fp8_quantize(rows_of(gen(41), 4, 64, torch.bfloat16))
+    room = torch.full((256,), 7.0, device=DEV)
+    with pytest.raises(kernels.KernelError, match="over one another"):
+        kernels.fp8_read(m, room.as_strided((4, 64), (32, 1)))
+    with pytest.raises(kernels.KernelError, match="over one another"):
+        kernels.fp8_read(m, room[:64].expand(4, 64))
+    assert (room == 7.0).all()
+    kernels.fp8_read(m, room.view(4, 64))
+    assert torch.equal(room.view(4, 64), read(m))
+
+
+@pytest.mark.parametrize("top", [1, 3])
+def test_passes_of_experts_one_right_after_the_other(top):
+    """A pass's kernels begin before those ahead of them have ended: many passes without a wait give what one at a time gives."""
+    g, e, width, inter = gen(42), 6, 512, 256
+    up = kernels.fp8_gate_up(*(rows_of(g, e * inter, width, torch.bfloat16).view(e, inter, width) * 0.1 for _ in range(2)))
+    down = kernels.fp8_quantize(rows_of(g, e * width, inter, torch.bfloat16).view(e, width, inter) * 0.1)
+    calls = []
+    for t in (1, 8, 90, 300, 700):
+        calls.append((rows_of(g, t, width, torch.bfloat16), routed(g, t, top, e, "even"), torch.rand(t, top, generator=g, device=DEV)))
+
+    def run(i):
+        x, ids, w = calls[i]
+        out = torch.full((len(x), width), 7.0, dtype=torch.bfloat16, device=DEV)
+        kernels.experts_fp8(x, ids, w, up, down, out)
+        return out
+    good = []
+    for i in range(len(calls)):
+        good.append(run(i))
+        torch.cuda.synchronize()
+    order = torch.randint(len(calls), (60,), generator=torch.Generator().manual_seed(1)).tolist()
+    outs = [run(i) for i in order]
+    # each pass also reads what the one before left.  (Results are some hundred times the square of what goes in: the first four
+    # are finite, then blocks are NaN; so the bits are compared.)
+    def chain(wait):
+        left = [calls[1][0]]
+        for _ in range(6):
+            left.append(torch.empty_like(left[0]))
+            kernels.experts_fp8(left[-2], calls[1][1], calls[1][2], up, down, left[-1])
+            if wait:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        return left
+    chained, again = chain(False), chain(True)
+    for i, out in zip(order, outs):
+        assert torch.equal(out, good[i])
+    for a, b in zip(chained, again):
+        assert torch.equal(a.view(torch.int16), b.view(torch.int16))
+    assert chained[2].isfinite().all()
+    assert kernels.fp8_stream_status() == 0 and kernels.fp8_gemm_status() == 0
