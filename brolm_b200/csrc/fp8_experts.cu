@@ -122,6 +122,7 @@ __global__ void __cluster_dims__(BLOCKS, 1, 1) __launch_bounds__(1024) group_ker
     for (int e = threadIdx.x; e < E; e += 1024) mine[e] = 0;
     __syncthreads();
     pdl_wait();
+    pdl_trigger();                                      // (what follows waits for this kernel's end)
     auto id = [&](int p) {
         const int e = p < P ? ids[p] : -1;
         return e >= 0 && e < E ? e : -1;
@@ -181,7 +182,6 @@ __global__ void __cluster_dims__(BLOCKS, 1, 1) __launch_bounds__(1024) group_ker
         g.perm[s] = 0;
         g.scale_row[s] = -1;
     }
-    pdl_trigger();
 }
 
 // The rows of x in 8 bits, each at its pairs' places: place[p] is pair p's row of the order, -1 if it is in no group.  With top 0
@@ -225,6 +225,7 @@ __global__ void __launch_bounds__(FEW) group_gather_kernel(RowsArgs x, const int
     place[tid] = scale_row[tid] = -1;
     __syncthreads();
     pdl_wait();
+    pdl_trigger();
     int e = tid < P ? ids[tid] : -1;
     e = e >= 0 && e < E ? e : -1;
     const Match m = match(e, lane);
@@ -257,7 +258,6 @@ __global__ void __launch_bounds__(FEW) group_gather_kernel(RowsArgs x, const int
     const int quad = blockIdx.x, c = quad * 512 + lane * 16;
     for (long row = (long)blockIdx.y * WARPS + warp; row < x.rows; row += (long)gridDim.y * WARPS)
         gather_row<T, WIDE>(x, row, quad, c, lane, place, scale_row, top);
-    pdl_trigger();
 }
 
 __device__ __forceinline__ void store4(float* p, const float (&v)[4]) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
@@ -274,6 +274,7 @@ template <typename T>
 __global__ void __launch_bounds__(THREADS) combine_kernel(const float* __restrict__ y, const int32_t* __restrict__ ids, const float* __restrict__ weights,
                                                           int top, int experts, int tokens, int cols, T* __restrict__ out, long ldo, int wide, int out_wide) {
     pdl_wait();
+    pdl_trigger();
     const int t = blockIdx.x, c = (blockIdx.y * THREADS + threadIdx.x) * 4;
     if (c < cols) {
         float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -305,13 +306,11 @@ __global__ void __launch_bounds__(THREADS) combine_kernel(const float* __restric
         }
         if (out_wide) {
             store4(out + (long)t * ldo + c, acc);
-            pdl_trigger();
             return;
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) if (c + i < cols) out[(long)t * ldo + c + i] = from_float<T>(acc[i]);
     }
-    pdl_trigger();
 }
 
 unsigned rows_grid(long long rows) {
