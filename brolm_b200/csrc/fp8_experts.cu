@@ -4,8 +4,8 @@
 //   gather         the tokens' rows in 8 bits, each at its pairs' places of that order
 //   combine        a token's results, multiplied by their weights and added
 //
-// and the launches of a whole pass, from one call of the host: group and gather, the first product with its activation, (where
-// that leaves floats) its results in 8 bits, the second product, combine.
+// and the launches of a whole pass, from one call of the host: group and gather, the first product with its activation, which
+// leaves 8 bits, the second product, combine.
 #include "fp8_round.cuh"
 
 namespace {
@@ -184,9 +184,7 @@ __global__ void __cluster_dims__(BLOCKS, 1, 1) __launch_bounds__(1024) group_ker
     }
 }
 
-// The rows of x in 8 bits, each at its pairs' places: place[p] is pair p's row of the order, -1 if it is in no group.  With top 0
-// row s of x is row s of the order.
-// One piece of a row of x to each of its pairs' places.
+// One piece of a row of x in 8 bits to each of its pairs' places: place[p] is pair p's row of the order, -1 if it is in no group.
 template <typename T, bool WIDE>
 __device__ __forceinline__ void gather_row(const RowsArgs& g, long row, int quad, int c, int lane, const int32_t* place, const int32_t* scale_row, int top) {
     const T* x = (const T*)g.x + row * g.ldx;
@@ -196,8 +194,8 @@ __device__ __forceinline__ void gather_row(const RowsArgs& g, long row, int quad
     piece.get(x, c, g.cols, v);
     uint32_t word;
     const uint4 q = round16(v, word);
-    for (int k = 0; k < max(top, 1); ++k) {
-        const long s = top ? place[row * top + k] : row;
+    for (int k = 0; k < top; ++k) {
+        const long s = place[row * top + k];
         const int at = s < 0 ? -1 : scale_row[s];
         if (at < 0) continue;
         if (c < g.ldv) *reinterpret_cast<uint4*>(g.values + s * g.ldv + c) = q;
@@ -345,7 +343,7 @@ int group_gather(const RowsArgs& x, const int32_t* ids, int P, int E, int top, c
 // (gated: 2 inter; a multiple of 128 rows apart), down of N.  Tiles have `rows` rows: of 16 or 32 the experts'
 // matrices are streamed, of 256 they go to the pairs of SMs; `product` is the launcher of the one or the other.  pairs [top, tokens, N] float; out (or null) the combined rows.
 // scale (or null) [tokens, top] multiplies a pair's first sums, weights (or null, for ones) its result.  `work` holds
-// `work_bytes`: the order and the list, then both products' rows in 8 bits, then (streamed) the first product's floats.
+// `work_bytes`: the order and the list, then both products' rows in 8 bits.
 struct ExpertsCall {
     const void *x, *ids, *scale, *weights, *up, *up_scales, *down, *down_scales;
     void *pairs, *out, *work;
@@ -362,7 +360,6 @@ BROLM_API int brolm_fp8_experts(const ExpertsCall* c) {
     if (c->dtype != BROLM_BF16 && c->dtype != BROLM_F32) return BROLM_ERR_BAD_DTYPE;
     if (rows != 16 && rows != 32 && rows != 256) return BROLM_ERR_BAD_SIZE;
     const int P = T * top, pad = (rows + 127) / 128 * 128, most = (P + rows - 1) / rows + (E < P ? E : P);
-    const bool stream = rows <= 128;
     uint8_t* at = (uint8_t*)c->work;
     auto take = [&](long long bytes) {
         uint8_t* p = at;
@@ -381,7 +378,6 @@ BROLM_API int brolm_fp8_experts(const ExpertsCall* c) {
         return m;
     };
     RowsArgs a = matrix(c->K), h = matrix(c->inter);
-    float* sums = (float*)take(stream ? 4LL * P * c->inter : 0);
     if (((uintptr_t)c->work & 511) || at - (uint8_t*)c->work > c->work_bytes) return BROLM_ERR_BAD_SIZE;
     a.x = c->x; a.ldx = (long)c->ldx; a.rows = T;
     const int32_t* ids = (const int32_t*)c->ids;
@@ -390,21 +386,14 @@ BROLM_API int brolm_fp8_experts(const ExpertsCall* c) {
     ProductCall p = {};
     p.x = a.values; p.x_scales = a.scales; p.ldx = a.ldv; p.w = c->up; p.w_scales = c->up_scales; p.ldw = c->up_ld; p.stream = c->stream;
     p.M = P; p.N = c->inter; p.K = c->K; p.epilogue = c->gated; p.act = c->act; p.limit = c->limit; p.cut = c->piece;
-    if (stream) { p.y = sums; p.ldy = c->inter; p.out = 1; }
-    else { p.y = h.values; p.y_scales = h.scales; p.ldy = h.ldv; p.out = 2; }
+    p.y = h.values; p.y_scales = h.scales; p.ldy = h.ldv; p.out = 2;
     p.experts = E; p.tile_group = g.tile_group; p.tile_row0 = g.tile_row0; p.offsets = g.offsets; p.perm = g.perm; p.scale = c->scale;
     p.group_rows = c->up_rows; p.top = top; p.tokens = T; p.rows = rows; p.max_tiles = most;
     st = c->product(&p);
     if (st) return st;
-    if (stream) {
-        h.x = sums; h.ldx = c->inter;
-        st = gather<float>(h, g.place, g.scale_row, 0, c->stream);
-        if (st) return st;
-    }
     p.x = h.values; p.x_scales = h.scales; p.ldx = h.ldv; p.w = c->down; p.w_scales = c->down_scales; p.ldw = c->down_ld;
     p.y = c->pairs; p.y_scales = nullptr; p.ldy = c->N; p.out = 1; p.N = c->N; p.K = c->inter; p.epilogue = 0; p.act = 0; p.limit = 0.0f;
-    // (the kernel before, the first product or the rounding of its results, has waited before it lets this one begin, and so has
-    // the list been written)
+    // (the first product has waited before it lets this one begin, and so has the list been written)
     p.scale = nullptr; p.group_rows = c->down_rows; p.down = 1; p.listed = 1;
     st = c->product(&p);
     if (st || !c->out) return st;

@@ -19,7 +19,9 @@
 // so its last one; an item of work is one such tile and 128 rows of its expert's matrix.
 //
 // Epilogues: store (float or bfloat16; with the square of relu), or a gated activation of neighbouring rows of W, row 2 j being
-// the gate of output j and row 2 j + 1 its partner: the two lie in neighbouring lanes.
+// the gate of output j and row 2 j + 1 its partner: the two lie in neighbouring lanes.  Or (K in one piece) 8 bits, as rows for
+// the next product: a block of 128 results of a row is a tile of W, gated two of them, which the two blocks of a cluster make
+// side by side; they tell one another the rows' largest magnitudes.
 //
 // Every mbarrier wait is bounded (tcgen05.cuh).
 #include "fp8_round.cuh"
@@ -48,6 +50,8 @@ struct StreamArgs {
     float limit;
     int nkb, quads;          // blocks of K, words of scales
     int row_tiles, items, stages;
+    uint8_t* y_scales;       // null: results are no 8-bit rows
+    int y_quads, team, last; // team: how many blocks make a block of such results; last: the last tile of W, where row_tiles counts teams of them
     int per;                 // blocks of K of a slice (dense; the cluster's rank is the slice)
     const void* x;           // rows that are no 8-bit numbers yet (FUSED), elements apart
     long ldx;
@@ -93,6 +97,34 @@ __device__ __forceinline__ float4 peer_floats(uint32_t addr, uint32_t rank) {
                  : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr), "r"(rank));
     return v;
 }
+__device__ __forceinline__ void peer_store(const uint32_t* p, uint32_t rank, uint32_t v) {
+    asm volatile("{\n.reg .b32 r;\nmapa.shared::cluster.u32 r, %0, %1;\nst.shared::cluster.b32 [r], %2;\n}"
+                 ::"r"(smem_u32(p)), "r"(rank), "r"(v) : "memory");
+}
+// The largest of four warps' words for a row, which they leave in this block's shared memory with the highest bit telling that they
+// are there; bounded as all waits are (code 7).  No fence goes with them: the words are all there is to read.
+__device__ __forceinline__ bool words_wait(const uint32_t* p, uint32_t tag, uint32_t& most, volatile int* give_up) {
+    volatile const uint32_t* w = p;
+    const bool stalled = give_up[2] == 7;
+    long long t0 = 0;
+    for (uint32_t turn = 1;; ++turn) {
+        const uint32_t a = w[0], b = w[32], c = w[64], d = w[96];
+        most = max(max(a, b), max(c, d)) & 0x7fffffffu;
+        if (!stalled && (tag ? a & b & c & d : ~(a | b | c | d)) >> 31) return true;
+        if (*give_up) return false;
+        if (turn % 1024) continue;                          // (some 30 us; the limit lies in memory, a miss is a microsecond)
+        if (!t0) t0 = clock64();
+        if (clock64() - t0 > (stalled ? g_wait_cycles / 4 : g_wait_cycles)) {
+            *give_up = 1;
+            atomicCAS(&g_fp8_stream_error, 0, 7);
+            return false;
+        }
+    }
+}
+__device__ __forceinline__ void peer_arrive(uint32_t bar, uint32_t rank) {
+    asm volatile("{\n.reg .b32 r;\nmapa.shared::cluster.u32 r, %0, %1;\nmbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [r];\n}"
+                 ::"r"(bar), "r"(rank) : "memory");
+}
 __device__ __forceinline__ void put(const StreamArgs& g, long at, float v) {
     if (g.out_f32) reinterpret_cast<float*>(g.y)[at] = v;
     else reinterpret_cast<bf16*>(g.y)[at] = __float2bfloat16_rn(v);
@@ -131,6 +163,8 @@ __device__ __forceinline__ void round_rows(const StreamArgs& g, uint8_t* x_block
     }
 }
 
+constexpr int MOST = 2 * 8 * 32;         // rows' largest magnitudes: two rooms in turn, eight warps, 32 rows
+
 // FUSED: 0 the rows are 8-bit numbers in memory; 1, 2: they are bfloat16, float numbers, and every block rounds what it needs.
 template <int BT, int FUSED>
 struct Shape {
@@ -144,9 +178,130 @@ struct Shape {
     static constexpr int SCALES = FUSED ? SF_TILE : 2 * SF_TILE;        // of a stage
     static size_t x_room(int per) { return FUSED ? (size_t)per * X_BYTES + (size_t)((per + 3) / 4 + 1) * SF_TILE : 0; }
     static size_t smem(int stages, int per) {
-        return x_room(per) + (size_t)stages * (STAGE_BYTES + SCALES) + (2 * MAX_STAGES + 6) * 8 + 16;
+        return x_room(per) + (size_t)stages * (STAGE_BYTES + SCALES) + (2 * MAX_STAGES + 8) * 8 + 16 + MOST * 4;
     }
 };
+
+// Two numbers of a lane become one: of numbers i and i + HALF the lanes without bit `BIT` keep the first, the others the second,
+// each with the other lane's in it.
+template <int HALF>
+__device__ __forceinline__ void fold(uint32_t* m, int lane, int bit) {
+#pragma unroll
+    for (int i = 0; i < HALF; ++i) {
+        const bool up = lane & bit;
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? m[i] : m[i + HALF], bit);
+        m[i] = max(up ? m[i + HALF] : m[i], got);
+    }
+}
+
+// An accumulator's results as rows of 8-bit numbers: 16 or 32 rows of X at a time, since each time costs a wait for the other
+// warps of the block of 128 results (a microsecond at the end of a launch).  False: that wait ran out.  A launch less: a feed-forward
+// of 8 rows, 2,304 and 9,216, 24.0 -> 21.0 us, 64 rows 23.8 -> 22.5; 8 tokens, 4 of 32 experts, 41.2 -> 38.9, 64 tokens 50.3 -> 46.9.
+template <int EPI, bool EXPERTS, int BT>
+__device__ __forceinline__ bool rounded_results(const StreamArgs& g, uint32_t acc, uint32_t acc_empty, int rows, int row0, int tile, int rt, int side, int quarter,
+                                                int lane, uint32_t* most_of, uint32_t joined, int& turn, volatile int* give_up) {
+    constexpr int ROWS = BT < 32 ? BT : 32, LANES = EPI == EPI_GATED ? 2 : 1, V = ROWS / LANES;      // gated: lanes with an odd number have the odd rows
+    const bool team = g.team > 1;
+    const int odd = EPI == EPI_GATED ? lane & 1 : 0;
+    const int col = (rt * BR + quarter * 32 + lane) / LANES;
+    for (int c = 0; c < rows; c += ROWS) {
+        float o[V];
+#pragma unroll
+        for (int c16 = 0; c16 < ROWS; c16 += 16) {
+            uint32_t v[16];
+            tmem_ld16(acc + c + c16, v);
+            tmem_wait_ld();
+            float z[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) z[i] = __uint_as_float(v[i]);
+            if (EXPERTS && g.scale) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) if (c + c16 + i < rows) z[i] *= g.scale[g.perm[row0 + c + c16 + i]];
+            }
+            if (EPI == EPI_GATED) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float got = __shfl_xor_sync(0xffffffffu, odd ? z[2 * i] : z[2 * i + 1], 1);
+                    o[c16 / 2 + i] = gate_of(odd ? got : z[2 * i], odd ? z[2 * i + 1] : got, g.act, g.limit);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[c16 / LANES + i / LANES] = act_of(z[i], g.act);
+            }
+        }
+        if (c + ROWS >= rows) {                                 // all of this accumulator that is wanted is in registers
+            fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(acc_empty);
+        }
+        // a row's largest magnitude goes round the warp's columns (a lane is left with row `place`'s), then to all of the team's warps
+        uint32_t m[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            if (col >= g.N) o[i] = 0.0f;                        // columns of no output are no part of the block
+            m[i] = __float_as_uint(o[i]) & 0x7fffffffu;
+        }
+        int place = odd;
+        if constexpr (V == 32) { fold<16>(m, lane, 16); fold<8>(m, lane, 8); fold<4>(m, lane, 4); fold<2>(m, lane, 2); fold<1>(m, lane, 1); place = lane; }
+        if constexpr (V == 16) { fold<8>(m, lane, 16); fold<4>(m, lane, 8); fold<2>(m, lane, 4); fold<1>(m, lane, 2); place += (lane >> 1) * LANES; }
+        if constexpr (V == 8) { fold<4>(m, lane, 16); fold<2>(m, lane, 8); fold<1>(m, lane, 4); place += (lane >> 2) * LANES; }
+        if constexpr (V < 32) {
+            constexpr int ANY = V == 8 ? 2 : LANES == 1 ? 1 : 0;          // the lanes that have the same row
+            if constexpr (ANY > 0) m[0] = max(m[0], __shfl_xor_sync(0xffffffffu, m[0], ANY));
+        }
+        // (two rooms in turn: a warp writes into one again when it has read the other, and so has every warp left the first.  The
+        // barrier is where the warps wait; its arrivals are ordered with nothing, for a fence across the cluster cost 0.5 to 1 us a
+        // turn, and the words' tags tell what is there.  Polling the words alone kept the SM from its other work: 1 to 2 us.)
+        uint32_t* room = most_of + (turn & 1) * (MOST / 2);
+        uint32_t* mine = room + (side * 4 + quarter) * 32 + place;
+        const uint32_t tag = (turn >> 1 & 1) ^ 1, word = m[0] | tag << 31;
+        *(volatile uint32_t*)mine = word;                       // (lanes of the same row: the same number)
+        if (team) peer_store(mine, side ^ 1, word);
+        __syncwarp();
+        if (lane == 0) {
+            mbar_arrive(joined);
+            if (team) peer_arrive(joined, side ^ 1);
+        }
+        if (!__all_sync(0xffffffffu, wait_on(joined, turn & 1, give_up, 7))) return false;
+        ++turn;
+        // lane l: of row l (16 rows: l % 16, half of the lanes for each of the team's sides)
+        uint32_t most;
+        bool there = words_wait(room + (ROWS == 16 ? (team ? lane >> 4 : 0) * 128 + (lane & 15) : lane), tag, most, give_up);
+        if (ROWS == 32 && team) {
+            uint32_t other;
+            there = there && words_wait(room + 128 + lane, tag, other, give_up);
+            most = max(most, other);
+        }
+        if (ROWS == 16) most = max(most, __shfl_xor_sync(0xffffffffu, most, 16));
+        if (!__all_sync(0xffffffffu, there)) return false;
+        const uint32_t byte = scale_byte(most);                 // of row c + lane
+        if (quarter == 0 && side == 0 && lane < ROWS && c + lane < rows) {
+            const int b = EPI == EPI_GATED ? rt >> 1 : rt;
+            g.y_scales[scale_at((EXPERTS ? (long)tile * 128 : 0) + c + lane, b >> 2, g.y_quads) + (b & 3)] = (uint8_t)byte;
+        }
+        // four rows at a time: a lane's word is its column's numbers in them; four lanes exchange, and each has four columns of a row
+        const int a = lane / LANES & 3;
+#pragma unroll
+        for (int i = 0; i < V; i += 4) {
+            float u[4];
+            uint32_t nan = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t s = __shfl_sync(0xffffffffu, byte, (i + j) * LANES + odd);
+                u[j] = s == 255u ? 0.0f : o[i + j] * scale_inverse(s);
+                if (s == 255u) nan |= (NAN4 & 255u) << (8 * j);
+            }
+            uint32_t q = pack4(u[0], u[1], u[2], u[3], 1.0f) | nan;
+            uint32_t got = __shfl_xor_sync(0xffffffffu, q, LANES);
+            q = __byte_perm(q, got, a & 1 ? 0x3715 : 0x6240);
+            got = __shfl_xor_sync(0xffffffffu, q, 2 * LANES);
+            q = __byte_perm(q, got, a & 2 ? 0x3276 : 0x5410);
+            const int r = c + (i + a) * LANES + odd, at = col & ~3;
+            if (r < rows && at < g.ldy) *reinterpret_cast<uint32_t*>((uint8_t*)g.y + (EXPERTS ? row0 + r : r) * g.ldy + at) = q;
+        }
+    }
+    return true;
+}
 
 template <int BT, int EPI, bool EXPERTS, int FUSED>
 __global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS, 2) fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w,
@@ -161,16 +316,20 @@ __global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS, 2) fp8_stream_kerne
     uint8_t* scale_slots = x_blocks + (FUSED ? g.per * S::X_BYTES : 0);
     uint8_t* x_scales = scale_slots + stages * S::SCALES;
     uint64_t* bars = reinterpret_cast<uint64_t*>(x_scales + (FUSED ? ((g.per + 3) / 4 + 1) * SF_TILE : 0));
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * MAX_STAGES + 6);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * MAX_STAGES + 8);
     volatile int* give_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    uint32_t* most_of = tmem_slot + 4;                         // [2][8][32]
     // slices: this one's sums [rows of X][128], in the ring, which is read to its end by then
     float* sums = reinterpret_cast<float*>(base);
     const uint32_t stage0 = smem_u32(base), scale0 = smem_u32(scale_slots);
     const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * MAX_STAGES, acc_full0 = empty0 + 8 * MAX_STAGES,
-                   acc_empty0 = acc_full0 + 16, x_ready = acc_empty0 + 16, ended = x_ready + 8;
+                   acc_empty0 = acc_full0 + 16, x_ready = acc_empty0 + 16, ended = x_ready + 8, joined = ended + 8;
     const bool aligned = (stage0 & 1023u) == 0;
-    const int slices = EXPERTS ? 1 : (int)cluster_size(), slice = EXPERTS ? 0 : (int)cluster_rank();
-    const int first = EXPERTS ? blockIdx.x : blockIdx.x / slices, step = EXPERTS ? gridDim.x : gridDim.x / slices;
+    // the blocks of a cluster are the slices of K or the sides of a team
+    const bool team = g.team > 1;
+    const int members = (int)cluster_size(), member = (int)cluster_rank();
+    const int slices = EXPERTS || team ? 1 : members, slice = EXPERTS || team ? 0 : member, side = team ? member : 0;
+    const int first = blockIdx.x / members, step = gridDim.x / members;
     const int lo = slice * g.per, hi = min(g.nkb, lo + g.per);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -185,26 +344,29 @@ __global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS, 2) fp8_stream_kerne
         }
         mbar_init(x_ready, 8);
         mbar_init(ended, 1);
+        mbar_init(joined, 4 * g.team);
         give_up[0] = aligned ? 0 : 1;
         give_up[1] = 0;
         give_up[2] = tc::g_stall_code;
         if (!aligned) atomicCAS(&g_fp8_stream_error, 0, 13);
         mbar_init_fence();
     }
+    for (int i = threadIdx.x; i < MOST; i += S::THREADS) most_of[i] = 0;
     if (warp == 1) tmem_alloc(smem_u32(tmem_slot), S::TMEM_COLS);
     fence_before_sync();
     __syncthreads();
     fence_after_sync();
+    if (team) asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");      // (waited for where the other block is first spoken to)
     const uint32_t tmem = *tmem_slot;
 
     // the tile of rows of X and the tile of rows of W of an item; false behind the experts' last tile
     auto find = [&](int item, int& rt, int& group, int& row0, int& tile) {
         if (!EXPERTS) {
-            rt = item; group = 0; row0 = 0; tile = 0;
+            rt = item * g.team + side; group = 0; row0 = 0; tile = 0;
             return true;
         }
         tile = item / g.row_tiles;
-        rt = item - tile * g.row_tiles;
+        rt = (item - tile * g.row_tiles) * g.team + side;
         group = __ldcg(&g.tile_group[tile]);             // (perhaps read before this kernel's wait)
         if (group < 0) return false;
         row0 = __ldcg(&g.tile_row0[tile]);
@@ -216,7 +378,7 @@ __global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS, 2) fp8_stream_kerne
             auto bytes_of = [&](int kb) { return (uint32_t)(S::STAGE_BYTES + ((kb & 3) == 0 || kb == lo ? S::SCALES : 0)); };
             auto load_w = [&](int s, int rt, int group, int kb) {
                 const uint32_t full = full0 + 8 * s;
-                const int row = group * g.group_rows + rt * BR;
+                const int row = group * g.group_rows + min(rt, g.last) * BR;      // (a team's second tile may lie behind the last)
                 mbar_expect_tx(full, bytes_of(kb));
                 tma_load_2d(stage0 + s * S::STAGE_BYTES, &map_w, kb * BK, row, full);
                 if ((kb & 3) == 0 || kb == lo)
@@ -320,7 +482,9 @@ __global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS, 2) fp8_stream_kerne
             __syncwarp();
             if (lane == 0) mbar_arrive(x_ready);
         }
-        int local = 0, rt, group, row0, tile;
+        __syncwarp();
+        if (team && warp < 6) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+        int local = 0, turn = 0, rt, group, row0, tile;
         for (int item = first; item < g.items && lo < hi && warp < 6; item += step, ++local) {
             if (!find(item, rt, group, row0, tile)) break;
             const int as = local % ACCS;
@@ -330,6 +494,10 @@ __global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS, 2) fp8_stream_kerne
             const uint32_t acc = tmem + as * BT + ((uint32_t)(quarter * 32) << 16);
             const int rows = EXPERTS ? min(BT, g.offsets[group + 1] - row0) : g.M;
             const int wide = (rows + 15) & ~15;
+            if (BT <= 64 && g.y_scales) {
+                if (!rounded_results<EPI, EXPERTS, BT>(g, acc, acc_empty0 + 8 * as, rows, row0, tile, rt, side, quarter, lane, most_of, joined, turn, give_up)) break;
+                continue;
+            }
             for (int c = 0; c < wide; c += 16) {
                 uint32_t v[16];
                 tmem_ld16(acc + c, v);
@@ -384,6 +552,11 @@ __global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS, 2) fp8_stream_kerne
     }
     pdl_trigger();
     fence_before_sync();
+    if (team) {
+        __syncwarp();
+        if (warp < 2 || warp >= 6) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+        cluster_sync_all();                                     // neither block leaves while the other may speak to it
+    }
     if (!EXPERTS && slices > 1) {
         // one tile a cluster: the slices' sums are added in their order, every block takes some of the rows
         __syncwarp();
@@ -438,6 +611,7 @@ int launch(const CUtensorMap& mw, const CUtensorMap& mx, StreamArgs g, int slice
     using S = Shape<BT, FUSED>;
     const int sms = device_sms();
     const bool split = slices > 1;
+    const int members = split ? slices : g.team;
     // Two blocks an SM: one streams while the other starts or ends, and clusters of up to eight find room.  (Three with 74 KB,
     // where experts' items fill their rounds better, gained nothing.)
     constexpr size_t ROOM = 112 * 1024;
@@ -449,8 +623,8 @@ int launch(const CUtensorMap& mw, const CUtensorMap& mx, StreamArgs g, int slice
     static OncePerDevice done;
     const int st = allow_shared_memory(fp8_stream_kernel<BT, EPI, EXPERTS, FUSED>, ROOM, done);
     if (st) return st;
-    const int places = 2 * sms;
-    const int grid = split ? g.items * slices : g.items < places ? g.items : places;
+    const int places = 2 * sms / members;
+    const int grid = members * (split || g.items < places ? g.items : places);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(S::THREADS);
@@ -460,10 +634,10 @@ int launch(const CUtensorMap& mw, const CUtensorMap& mx, StreamArgs g, int slice
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = slices;
+    attr[1].val.clusterDim.x = members;
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = EXPERTS ? 1 : 2;
+    cfg.numAttrs = 2;
     return (int)cudaLaunchKernelEx(&cfg, fp8_stream_kernel<BT, EPI, EXPERTS, FUSED>, mw, mx, g);
 }
 
@@ -485,7 +659,8 @@ int dispatch(const CUtensorMap& mw, const CUtensorMap& mx, const StreamArgs& g, 
 }  // namespace
 
 // Y [M, N] = X W^T (epilogue 0, act 0 or the square of relu) or the gated activation of W's neighbouring rows (epilogue 1: W
-// has 2 N rows); out 0: bfloat16, 1: float.  X and W as brolm_fp8_quantize leaves them.
+// has 2 N rows); out 0: bfloat16, 1: float, 2 (cut 1, M <= 64): 8 bits, ldy bytes between rows, a multiple of 16, for experts scales as
+// x_scales has them.  X and W as brolm_fp8_quantize leaves them.
 // Dense (experts 0): M <= 128; K is cut into `cut` slices (1 to 8), none of which is empty.  fused 1, 2: X are bfloat16, float
 // numbers (ldx elements between rows, x_scales unused), M <= 16, and a slice has at most FUSED_BLOCKS blocks of 128 of K.
 // Experts: M pairs' rows in the order of their experts, W the experts' matrices, group_rows (a multiple of 128) rows each.  The
@@ -499,20 +674,24 @@ BROLM_API int brolm_fp8_stream(const fp8::ProductCall* c) {
     if (!c->fused && (c->ldx % 16 || (((uintptr_t)c->x | (uintptr_t)c->x_scales) & 15))) return BROLM_ERR_ALIGNMENT;
     if (c->fused < 0 || c->fused > 2 || (c->fused && (M > 16 || c->experts))) return BROLM_ERR_BAD_SIZE;
     if (c->epilogue < 0 || c->epilogue > 1 || c->act < 0 || c->act > 2 || (c->epilogue == EPI_STORE && c->act > ACT_RELU2)) return BROLM_ERR_BAD_SIZE;
-    if (c->out < 0 || c->out > 1) return BROLM_ERR_BAD_SIZE;
+    if (c->out < 0 || c->out > 2 || (c->out == 2 && !c->experts && (c->cut != 1 || M > 64))) return BROLM_ERR_BAD_SIZE;
+    if (c->out == 2 && (c->ldy % 16 || c->ldy < N || !c->y_scales || ((uintptr_t)c->y & 15))) return BROLM_ERR_ALIGNMENT;
     const long long w_rows = c->epilogue == EPI_GATED ? 2LL * N : N;
     StreamArgs g = {};
-    g.y = c->y; g.ldy = (long)c->ldy; g.M = M; g.N = N; g.out_f32 = c->out; g.act = c->act; g.limit = c->limit;
+    g.y = c->y; g.ldy = (long)c->ldy; g.M = M; g.N = N; g.out_f32 = c->out == 1; g.act = c->act; g.limit = c->limit;
     g.y_wide = ((uintptr_t)c->y & 15) == 0 && c->ldy % 4 == 0;
     g.nkb = blocks_of(K); g.quads = quads_of(K);
     g.w_scales = (const uint8_t*)c->w_scales; g.x_scales = (const uint8_t*)c->x_scales;
-    const long long row_tiles = (w_rows + BR - 1) / BR;
+    g.last = (int)((w_rows + BR - 1) / BR - 1);
+    if (c->out == 2) { g.y_scales = (uint8_t*)c->y_scales; g.y_quads = quads_of(N); }
+    g.team = c->out == 2 && c->epilogue == EPI_GATED ? 2 : 1;
+    const long long row_tiles = (g.last + g.team) / g.team;      // of a team's W
     CUtensorMap mw, mx;
     if (c->experts) {
         const int rows = c->rows;
-        if (c->group_rows % BR || (rows != 16 && rows != 32) || (c->down && !c->out)) return BROLM_ERR_BAD_SIZE;
+        if (c->group_rows % BR || (rows != 16 && rows != 32) || (c->down && c->out != 1)) return BROLM_ERR_BAD_SIZE;
         const long long all = (long long)c->experts * c->group_rows;
-        if (all > 0x7fffffff || c->max_tiles * row_tiles > 0x7fffffff) return BROLM_ERR_TOO_LARGE;
+        if (all > 0x7fffffff || c->max_tiles * row_tiles > 0x7fffffff - 65536) return BROLM_ERR_TOO_LARGE;
         int st = make_map_u8(&mw, c->w, all, K, c->ldw, BR);
         if (!st) st = make_map_u8(&mx, c->x, M, K, c->ldx, rows);
         if (st) return st;

@@ -316,11 +316,11 @@ def feedforward_fp8(x, gate_up: Fp8Matrix, down: Fp8Matrix, out: torch.Tensor, a
     if not M or not down.rows:
         return
     sms = device_sms(down.device)
-    # what lies between is rounded by the first product's own end where it goes in tiles (a stream's tile holds parts of a block
-    # only, and leaves floats)
+    # what lies between is rounded by the first product's own end, but where K is cut or a stream has more than 64 rows, whose
+    # accumulator is one and waits: then it leaves floats (2,304 and 9,216: 8 rows 21.0 us for 24.0, 64 22.5 for 23.8, 100 26.9 for 25.4)
     words = 0 if type(x) is Fp8Matrix else x.element_size()
     first = _rounded(M, gate_up.cols, gate_up.rows, 0, words, sms)
-    floats = first[0]
+    floats = first[0] and (first[1] > 1 or M > 64)
     second = _rounded(M, inter, down.rows, 0, 4 if floats else 0, sms)
     # one room: x in 8 bits, what lies between in 8 bits, as floats
     x8 = _bytes(M, gate_up.cols, M) if words and not first[2] else 0
@@ -344,8 +344,8 @@ def feedforward_fp8(x, gate_up: Fp8Matrix, down: Fp8Matrix, out: torch.Tensor, a
 # --- routed experts -----------------------------------------------------------
 def experts_fp8_rows(pairs: int, experts: int) -> int:
     """How many rows a tile of an expert's pairs has: 16 or 32 with the experts' matrices streamed, 256 on pairs of SMs.  32 experts
-    of 2,048 x 1,024, 4 a token, with 16 / 32 / 256: 128 tokens (16 pairs an expert) 75 / 75 / 87 us, 256 82 / 86 / 90, 512 105 /
-    99 / 91; 8 experts, 2 a token: 128 (32) 42 / 41 / 45, 256 (64) 50 / 46 / 48, 512 (128) - / 58 / 50."""
+    of 2,048 x 1,024, 4 a token, with 16 / 32 / 256: 128 tokens (16 pairs an expert) 58 / 58 / 72 us, 256 73 / 70 / 77, 384 (48) 83 /
+    77 / 78, 512 98 / 89 / 79; 8 experts, 2 a token: 128 (32) 30 / 28 / 31, 192 (48) 36 / 33 / 34."""
     mean = pairs / max(experts, 1)
     return 16 if mean <= 16 else 32 if mean <= 48 else 256
 
@@ -383,12 +383,10 @@ def _experts(what: str, x, ids, up: Fp8Matrix, down: Fp8Matrix, pairs, out, acti
     rows = experts_fp8_rows(P, E)
     most = (P + rows - 1) // rows + min(E, P)
     up512 = lambda n: (n + 511) & -512
-    # the order and the list; the rows of both products in 8 bits with a tile of scales for every tile of the list; floats between
+    # the order and the list; the rows of both products in 8 bits with a tile of scales for every tile of the list
     need = 3 * up512(4 * P) + up512(4 * E + 8) + 2 * up512(4 * most)
     for cols in (K, inter):
         need += up512(P * ((cols + 15) & -16)) + ((rows + 127) >> 7) * most * ((cols + 511) >> 9) * _TILE
-    if rows < 256:
-        need += up512(4 * P * inter)
     held = None
     if pairs is None:
         held = torch.empty(need + 4 * P * N, dtype=torch.uint8, device=x.device)
@@ -403,7 +401,7 @@ def _experts(what: str, x, ids, up: Fp8Matrix, down: Fp8Matrix, pairs, out, acti
                          1 if out is not None and out.dtype == _F32 else 0, limit)
     _call("fp8_experts", "brolm_fp8_experts", pack, what)
     # (a call counts as one launch: the others of this pass)
-    add_launches((1 if P > 256 or E > 256 else 0) + 2 + (1 if rows < 256 else 0) + (1 if out is not None else 0))
+    add_launches((1 if P > 256 or E > 256 else 0) + 2 + (1 if out is not None else 0))
 
 
 def experts_fp8_pairs(x: torch.Tensor, ids: torch.Tensor, up: Fp8Matrix, down: Fp8Matrix, out: torch.Tensor, activation: str = "silu",

@@ -585,3 +585,50 @@ def test_passes_of_experts_one_right_after_the_other(top):
         assert torch.equal(a.view(torch.int16), b.view(torch.int16))
     assert chained[2].isfinite().all()
     assert kernels.fp8_stream_status() == 0 and kernels.fp8_gemm_status() == 0
+
+
+@pytest.mark.parametrize("m, width, inter, name", [
+    (1, 100, 30, "silu"), (8, 256, 64, "gelu_tanh"), (8, 128, 65, "silu"), (16, 200, 129, "clamped_gate"), (17, 256, 384, "silu"), (33, 130, 200, "gelu_tanh"),
+    (64, 256, 1000, "silu"), (128, 1024, 8500, "silu"), (3, 256, 20000, "gelu_tanh"), (8, 2304, 9216, "gelu_tanh"), (5, 256, 130, "relu2"), (64, 128, 1111, "relu2"),
+    (40, 256, 300, "none"), (2, 64, 40000, "relu2")])
+def test_a_feedforward_is_its_two_products(m, width, inter, name):
+    """What a product leaves in 8 bits is what it leaves as floats, rounded: the same bits come out."""
+    g = gen(m + inter)
+    x = rows_of(g, m, width, torch.bfloat16, 0.5)
+    mats = [rows_of(g, inter, width, torch.bfloat16, 0.3) * width ** -0.5 for _ in range(1 if name in ("relu2", "none") else 2)]
+    up = kernels.fp8_quantize(mats[0]) if len(mats) == 1 else kernels.fp8_gate_up(*mats)
+    down = kernels.fp8_quantize(rows_of(g, width, inter, torch.bfloat16, 0.3) * inter ** -0.5)
+    x[m // 2, width // 3] = float("inf") if m > 2 else 1.0          # a row that is NaN is no other row's
+    for t in (x, kernels.fp8_quantize(x), x.float()):
+        h = torch.empty(m, inter, dtype=torch.float32, device=DEV)
+        kernels.linear_fp8(t, up, h, name, 1.5)
+        good, y = (torch.full((m, width), 7.0, device=DEV) for _ in range(2))
+        kernels.linear_fp8(kernels.fp8_quantize(h), down, good)
+        kernels.feedforward_fp8(t, up, down, y, name, 1.5)
+        assert torch.equal(y.view(torch.int32), good.view(torch.int32))
+        assert y.isnan().any(dim=1).sum() == (1 if m > 2 else 0) and y[0].isfinite().all()
+    assert kernels.fp8_stream_status() == 0 and kernels.fp8_gemm_status() == 0
+
+
+@pytest.mark.parametrize("name", ["silu", "relu2"])
+def test_a_block_of_results_that_waits_in_vain(name):
+    """The warps that share a block of results in 8 bits, of one block and of two, give up in the end."""
+    g = gen(51)
+    x, up, down = rows_of(g, 8, 256, torch.bfloat16), *(rows_of(g, a, b, torch.bfloat16) * 0.1 for a, b in ((600, 256), (256, 300 if name == "silu" else 600)))
+    w = kernels.fp8_quantize(up) if name == "relu2" else kernels.fp8_gate_up(up[:300].contiguous(), up[300:].contiguous())
+    d = kernels.fp8_quantize(down)
+
+    def run():
+        out = torch.empty(8, 256, dtype=torch.float32, device=DEV)
+        kernels.feedforward_fp8(x, w, d, out, name)
+        torch.cuda.synchronize()
+        return out
+    good = run()
+    assert kernels.fp8_stream_status(reset=True) == 0
+    kernels.wait_control("fp8_stream", cycles=LIMIT, stall_code=7)
+    try:
+        run()
+        assert kernels.fp8_stream_status(reset=True) == 7 and kernels.fp8_stream_status() == 0
+    finally:
+        kernels.wait_control("fp8_stream", 0, 0)
+    assert torch.equal(run(), good) and kernels.fp8_stream_status() == 0
