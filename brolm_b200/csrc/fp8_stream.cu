@@ -50,8 +50,8 @@ struct StreamArgs {
     float limit;
     int nkb, quads;          // blocks of K, words of scales
     int row_tiles, items, stages;
-    uint8_t* y_scales;       // null: results are no 8-bit rows
-    int y_quads, team, last; // team: how many blocks make a block of such results; last: the last tile of W, where row_tiles counts teams of them
+    uint8_t* y_scales;       // (ROUND)
+    int y_quads, last;       // last: the last tile of W, of which row_tiles counts pairs where two blocks are a team
     int per;                 // blocks of K of a slice (dense; the cluster's rank is the slice)
     const void* x;           // rows that are no 8-bit numbers yet (FUSED), elements apart
     long ldx;
@@ -166,6 +166,7 @@ __device__ __forceinline__ void round_rows(const StreamArgs& g, uint8_t* x_block
 constexpr int MOST = 2 * 8 * 32;         // rows' largest magnitudes: two rooms in turn, eight warps, 32 rows
 
 // FUSED: 0 the rows are 8-bit numbers in memory; 1, 2: they are bfloat16, float numbers, and every block rounds what it needs.
+// ROUND: results are 8-bit rows (a kernel of its own: as a branch it cost the others 0.4 to 0.8 us a launch).
 template <int BT, int FUSED>
 struct Shape {
     static constexpr int THREADS = FUSED ? 320 : 192;                   // (eight warps that round, of which four have an epilogue)
@@ -201,7 +202,7 @@ template <int EPI, bool EXPERTS, int BT>
 __device__ __forceinline__ bool rounded_results(const StreamArgs& g, uint32_t acc, uint32_t acc_empty, int rows, int row0, int tile, int rt, int side, int quarter,
                                                 int lane, uint32_t* most_of, uint32_t joined, int& turn, volatile int* give_up) {
     constexpr int ROWS = BT < 32 ? BT : 32, LANES = EPI == EPI_GATED ? 2 : 1, V = ROWS / LANES;      // gated: lanes with an odd number have the odd rows
-    const bool team = g.team > 1;
+    constexpr bool team = EPI == EPI_GATED;
     const int odd = EPI == EPI_GATED ? lane & 1 : 0;
     const int col = (rt * BR + quarter * 32 + lane) / LANES;
     for (int c = 0; c < rows; c += ROWS) {
@@ -303,7 +304,7 @@ __device__ __forceinline__ bool rounded_results(const StreamArgs& g, uint32_t ac
     return true;
 }
 
-template <int BT, int EPI, bool EXPERTS, int FUSED>
+template <int BT, int EPI, bool EXPERTS, int FUSED, bool ROUND>
 __global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS, 2) fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w,
                                                              const __grid_constant__ CUtensorMap map_x, StreamArgs g) {
     using S = Shape<BT, FUSED>;
@@ -326,8 +327,9 @@ __global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS, 2) fp8_stream_kerne
                    acc_empty0 = acc_full0 + 16, x_ready = acc_empty0 + 16, ended = x_ready + 8, joined = ended + 8;
     const bool aligned = (stage0 & 1023u) == 0;
     // the blocks of a cluster are the slices of K or the sides of a team
-    const bool team = g.team > 1;
-    const int members = (int)cluster_size(), member = (int)cluster_rank();
+    constexpr bool team = ROUND && EPI == EPI_GATED;
+    constexpr int TEAM = team ? 2 : 1;
+    const int members = EXPERTS && !team ? 1 : (int)cluster_size(), member = EXPERTS && !team ? 0 : (int)cluster_rank();
     const int slices = EXPERTS || team ? 1 : members, slice = EXPERTS || team ? 0 : member, side = team ? member : 0;
     const int first = blockIdx.x / members, step = gridDim.x / members;
     const int lo = slice * g.per, hi = min(g.nkb, lo + g.per);
@@ -344,14 +346,14 @@ __global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS, 2) fp8_stream_kerne
         }
         mbar_init(x_ready, 8);
         mbar_init(ended, 1);
-        mbar_init(joined, 4 * g.team);
+        if (ROUND) mbar_init(joined, 4 * TEAM);
         give_up[0] = aligned ? 0 : 1;
         give_up[1] = 0;
         give_up[2] = tc::g_stall_code;
         if (!aligned) atomicCAS(&g_fp8_stream_error, 0, 13);
         mbar_init_fence();
     }
-    for (int i = threadIdx.x; i < MOST; i += S::THREADS) most_of[i] = 0;
+    if (ROUND) for (int i = threadIdx.x; i < MOST; i += S::THREADS) most_of[i] = 0;
     if (warp == 1) tmem_alloc(smem_u32(tmem_slot), S::TMEM_COLS);
     fence_before_sync();
     __syncthreads();
@@ -362,11 +364,11 @@ __global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS, 2) fp8_stream_kerne
     // the tile of rows of X and the tile of rows of W of an item; false behind the experts' last tile
     auto find = [&](int item, int& rt, int& group, int& row0, int& tile) {
         if (!EXPERTS) {
-            rt = item * g.team + side; group = 0; row0 = 0; tile = 0;
+            rt = item * TEAM + side; group = 0; row0 = 0; tile = 0;
             return true;
         }
         tile = item / g.row_tiles;
-        rt = (item - tile * g.row_tiles) * g.team + side;
+        rt = (item - tile * g.row_tiles) * TEAM + side;
         group = __ldcg(&g.tile_group[tile]);             // (perhaps read before this kernel's wait)
         if (group < 0) return false;
         row0 = __ldcg(&g.tile_row0[tile]);
@@ -493,11 +495,11 @@ __global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS, 2) fp8_stream_kerne
             fence_after_sync();
             const uint32_t acc = tmem + as * BT + ((uint32_t)(quarter * 32) << 16);
             const int rows = EXPERTS ? min(BT, g.offsets[group + 1] - row0) : g.M;
-            const int wide = (rows + 15) & ~15;
-            if (BT <= 64 && g.y_scales) {
+            if constexpr (ROUND) {
                 if (!rounded_results<EPI, EXPERTS, BT>(g, acc, acc_empty0 + 8 * as, rows, row0, tile, rt, side, quarter, lane, most_of, joined, turn, give_up)) break;
                 continue;
             }
+            const int wide = (rows + 15) & ~15;
             for (int c = 0; c < wide; c += 16) {
                 uint32_t v[16];
                 tmem_ld16(acc + c, v);
@@ -606,12 +608,12 @@ __global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS, 2) fp8_stream_kerne
     if (warp == 1) tmem_dealloc(tmem, S::TMEM_COLS);
 }
 
-template <int BT, int EPI, bool EXPERTS, int FUSED>
+template <int BT, int EPI, bool EXPERTS, int FUSED, bool ROUND>
 int launch(const CUtensorMap& mw, const CUtensorMap& mx, StreamArgs g, int slices, cudaStream_t stream) {
     using S = Shape<BT, FUSED>;
     const int sms = device_sms();
     const bool split = slices > 1;
-    const int members = split ? slices : g.team;
+    const int members = split ? slices : ROUND && EPI == EPI_GATED ? 2 : 1;
     // Two blocks an SM: one streams while the other starts or ends, and clusters of up to eight find room.  (Three with 74 KB,
     // where experts' items fill their rounds better, gained nothing.)
     constexpr size_t ROOM = 112 * 1024;
@@ -621,7 +623,7 @@ int launch(const CUtensorMap& mw, const CUtensorMap& mx, StreamArgs g, int slice
     if (smem > ROOM || (split && (size_t)stages * S::STAGE_BYTES < (size_t)BT * BR * 4)) return BROLM_ERR_TOO_LARGE;
     g.stages = stages;
     static OncePerDevice done;
-    const int st = allow_shared_memory(fp8_stream_kernel<BT, EPI, EXPERTS, FUSED>, ROOM, done);
+    const int st = allow_shared_memory(fp8_stream_kernel<BT, EPI, EXPERTS, FUSED, ROUND>, ROOM, done);
     if (st) return st;
     const int places = 2 * sms / members;
     const int grid = members * (split || g.items < places ? g.items : places);
@@ -637,23 +639,32 @@ int launch(const CUtensorMap& mw, const CUtensorMap& mx, StreamArgs g, int slice
     attr[1].val.clusterDim.x = members;
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    return (int)cudaLaunchKernelEx(&cfg, fp8_stream_kernel<BT, EPI, EXPERTS, FUSED>, mw, mx, g);
+    cfg.numAttrs = EXPERTS && members == 1 ? 1 : 2;
+    return (int)cudaLaunchKernelEx(&cfg, fp8_stream_kernel<BT, EPI, EXPERTS, FUSED, ROUND>, mw, mx, g);
 }
 
-template <int EPI, bool EXPERTS>
+template <int EPI, bool EXPERTS, bool ROUND>
 int dispatch(const CUtensorMap& mw, const CUtensorMap& mx, const StreamArgs& g, int bt, int slices, int fused, cudaStream_t stream) {
     if constexpr (!EXPERTS) {
-        if (fused == 1) return launch<16, EPI, false, 1>(mw, mx, g, slices, stream);
-        if (fused == 2) return launch<16, EPI, false, 2>(mw, mx, g, slices, stream);
+        if (fused == 1) return launch<16, EPI, false, 1, ROUND>(mw, mx, g, slices, stream);
+        if (fused == 2) return launch<16, EPI, false, 2, ROUND>(mw, mx, g, slices, stream);
     }
-    if (bt == 16) return launch<16, EPI, EXPERTS, 0>(mw, mx, g, slices, stream);
-    if (bt == 32) return launch<32, EPI, EXPERTS, 0>(mw, mx, g, slices, stream);
+    if (bt == 16) return launch<16, EPI, EXPERTS, 0, ROUND>(mw, mx, g, slices, stream);
+    if (bt == 32) return launch<32, EPI, EXPERTS, 0, ROUND>(mw, mx, g, slices, stream);
     if constexpr (!EXPERTS) {
-        if (bt == 64) return launch<64, EPI, false, 0>(mw, mx, g, slices, stream);
-        return launch<128, EPI, false, 0>(mw, mx, g, slices, stream);
+        if (bt == 64) return launch<64, EPI, false, 0, ROUND>(mw, mx, g, slices, stream);
+        if constexpr (!ROUND) return launch<128, EPI, false, 0, false>(mw, mx, g, slices, stream);
     }
     return BROLM_ERR_BAD_SIZE;
+}
+template <bool EXPERTS>
+int dispatch(const CUtensorMap& mw, const CUtensorMap& mx, const StreamArgs& g, int bt, int slices, int fused, int epilogue, int out, cudaStream_t stream) {
+    if (epilogue == EPI_GATED) {
+        if (out == 2) return dispatch<EPI_GATED, EXPERTS, true>(mw, mx, g, bt, slices, fused, stream);
+        return dispatch<EPI_GATED, EXPERTS, false>(mw, mx, g, bt, slices, fused, stream);
+    }
+    if (out == 2) return dispatch<EPI_STORE, EXPERTS, true>(mw, mx, g, bt, slices, fused, stream);
+    return dispatch<EPI_STORE, EXPERTS, false>(mw, mx, g, bt, slices, fused, stream);
 }
 
 }  // namespace
@@ -684,8 +695,8 @@ BROLM_API int brolm_fp8_stream(const fp8::ProductCall* c) {
     g.w_scales = (const uint8_t*)c->w_scales; g.x_scales = (const uint8_t*)c->x_scales;
     g.last = (int)((w_rows + BR - 1) / BR - 1);
     if (c->out == 2) { g.y_scales = (uint8_t*)c->y_scales; g.y_quads = quads_of(N); }
-    g.team = c->out == 2 && c->epilogue == EPI_GATED ? 2 : 1;
-    const long long row_tiles = (g.last + g.team) / g.team;      // of a team's W
+    const int team = c->out == 2 && c->epilogue == EPI_GATED ? 2 : 1;
+    const long long row_tiles = (g.last + team) / team;          // a team's tiles of W count once
     CUtensorMap mw, mx;
     if (c->experts) {
         const int rows = c->rows;
@@ -699,8 +710,7 @@ BROLM_API int brolm_fp8_stream(const fp8::ProductCall* c) {
         g.tile_group = (const int32_t*)c->tile_group; g.tile_row0 = (const int32_t*)c->tile_row0; g.offsets = (const int32_t*)c->offsets;
         g.perm = (const int32_t*)c->perm; g.scale = (const float*)c->scale;
         g.down = c->down; g.top = c->top; g.tokens = c->tokens; g.group_rows = c->group_rows; g.listed = c->listed;
-        if (c->epilogue == EPI_GATED) return dispatch<EPI_GATED, true>(mw, mx, g, rows, 1, 0, c->stream);
-        return dispatch<EPI_STORE, true>(mw, mx, g, rows, 1, 0, c->stream);
+        return dispatch<true>(mw, mx, g, rows, 1, 0, c->epilogue, c->out, c->stream);
     }
     const int slices = c->cut;
     if (M > 128 || w_rows > 0x7fffffff - BR) return BROLM_ERR_TOO_LARGE;
@@ -720,8 +730,7 @@ BROLM_API int brolm_fp8_stream(const fp8::ProductCall* c) {
     g.row_tiles = g.items = (int)row_tiles;
     st = round_first(c);
     if (st) return st;
-    if (c->epilogue == EPI_GATED) return dispatch<EPI_GATED, false>(mw, mx, g, bt, slices, c->fused, c->stream);
-    return dispatch<EPI_STORE, false>(mw, mx, g, bt, slices, c->fused, c->stream);
+    return dispatch<false>(mw, mx, g, bt, slices, c->fused, c->epilogue, c->out, c->stream);
 }
 
 BROLM_API int brolm_fp8_stream_status(int reset) {
