@@ -2,6 +2,7 @@
 //
 //   fp8_quantize   rows of float or bfloat16 numbers -> e4m3 numbers and a scale byte for every 128 of them
 //   fp8_read       the values that they stand for
+//   norm           a residual sum with the norms around it whose result is rows of 8 bits
 #include "fp8_round.cuh"
 
 namespace {
@@ -108,6 +109,98 @@ __global__ void __launch_bounds__(THREADS) read_kernel(RowsArgs g, T* __restrict
     pdl_trigger();
 }
 
+struct NormArgs {
+    float* h;
+    const float* y;
+    const void *w_post, *w_next;        // (w_post null: y is added as it is)
+    float eps_post, off_post, eps_next, off_next;
+    uint8_t* values; long ldv;
+    uint8_t* scales;
+    int quads, hidden;
+};
+__device__ __forceinline__ void four(const float* p, float (&v)[4]) {
+    const float4 u = *reinterpret_cast<const float4*>(p);
+    v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
+}
+__device__ __forceinline__ void four(const bf16* p, float (&v)[4]) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    v[0] = __uint_as_float(u.x << 16); v[1] = __uint_as_float(u.x & 0xffff0000u);
+    v[2] = __uint_as_float(u.y << 16); v[3] = __uint_as_float(u.y & 0xffff0000u);
+}
+// h += post(y);  values, scales = next(h), both norms being v * rsqrt(mean(v^2) + eps) * (offset + w).  A block has a row and
+// thread t of it numbers 4 t + 1,024 c on: a warp's four numbers each are a block of 128, whose scale is the warp's largest.
+// Statistics and sums are floats; what is rounded is the norm's float result, once.  Rows are few or many, the row stays in
+// registers: 8 x 2,304 numbers take as long as a launch, against two of them.
+template <typename W, int C>
+__global__ void __launch_bounds__(256, C <= 3 ? 4 : 1) residual_rmsnorm_fp8_kernel(NormArgs g) {
+    __shared__ float scratch[64];
+    const long r = blockIdx.x;
+    const W *w_post = (const W*)g.w_post, *w_next = (const W*)g.w_next;
+    pdl_trigger();
+    {
+        const size_t line = (size_t)threadIdx.x * 128;      // the gains are weights: brought near while the kernel before this one ends
+        if (line < (size_t)g.hidden * sizeof(W)) {
+            if (w_post) prefetch_l1(reinterpret_cast<const char*>(w_post) + line);
+            prefetch_l1(reinterpret_cast<const char*>(w_next) + line);
+        }
+    }
+    pdl_wait();
+    float* h = g.h + r * g.hidden;
+    const float* y = g.y + r * g.hidden;
+    float v[C][4], res[C][4];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const int i = (c * 256 + threadIdx.x) * 4;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[c][e] = res[c][e] = 0.0f;
+        if (i < g.hidden) { four(h + i, res[c]); four(y + i, v[c]); }
+    }
+    if (w_post) {
+        float ss = 0.0f;
+#pragma unroll
+        for (int c = 0; c < C; ++c) ss += v[c][0] * v[c][0] + v[c][1] * v[c][1] + v[c][2] * v[c][2] + v[c][3] * v[c][3];
+        ss = block_sum_once(ss, scratch, 0);
+        const float inv = rsqrtf(ss / (float)g.hidden + g.eps_post);
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int i = (c * 256 + threadIdx.x) * 4;
+            float gain[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (i < g.hidden) four(w_post + i, gain);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[c][e] = v[c][e] * inv * (g.off_post + gain[e]);
+        }
+    }
+    float ss = 0.0f;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const int i = (c * 256 + threadIdx.x) * 4;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (i < g.hidden) res[c][e] += v[c][e];
+            ss += res[c][e] * res[c][e];
+        }
+        if (i < g.hidden) *reinterpret_cast<float4*>(h + i) = make_float4(res[c][0], res[c][1], res[c][2], res[c][3]);
+    }
+    ss = block_sum_once(ss, scratch, 1);
+    const float inv = rsqrtf(ss / (float)g.hidden + g.eps_next);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const int i = (c * 256 + threadIdx.x) * 4, b = i >> 7;          // (the same block for the whole warp)
+        float gain[4] = {0.0f, 0.0f, 0.0f, 0.0f}, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (i < g.hidden) {
+            four(w_next + i, gain);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = res[c][e] * inv * (g.off_next + gain[e]);
+        }
+        uint32_t most = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) most = max(most, __float_as_uint(o[e]) & 0x7fffffffu);
+        const uint32_t byte = scale_byte(__reduce_max_sync(0xffffffffu, most));
+        if (i < g.ldv) *reinterpret_cast<uint32_t*>(g.values + r * g.ldv + i) = byte == 255u ? NAN4 : pack4(o[0], o[1], o[2], o[3], scale_inverse(byte));
+        if ((threadIdx.x & 31) == 0 && b < 4 * g.quads) g.scales[scale_at(r, b >> 2, g.quads) + (b & 3)] = (uint8_t)byte;
+    }
+}
+
 unsigned rows_grid(long long rows) {
     const long long blocks = (rows + WARPS - 1) / WARPS;
     return (unsigned)(blocks < 65535 ? blocks : 65535);
@@ -146,6 +239,40 @@ BROLM_API int brolm_fp8_read(const fp8::RowsCall* c) {
         return launch_pdl(read_kernel<bf16>, grid, block, 0, c->stream, g, (bf16*)c->x, (long)c->ldx, base && c->ldx % 8 == 0);
     if (c->dtype != BROLM_F32) return BROLM_ERR_BAD_DTYPE;
     return launch_pdl(read_kernel<float>, grid, block, 0, c->stream, g, (float*)c->x, (long)c->ldx, base && c->ldx % 4 == 0);
+}
+
+// h [rows, hidden] float += post(y), y float alike; values and scales as brolm_fp8_quantize has them (group = rows) = next(h).  Both
+// gains have one element type.  hidden is a multiple of 4, 8,192 at most; all pointers lie on borders of 16 bytes.
+struct NormCall {
+    void *h;
+    const void *y, *w_post, *w_next;
+    void *values, *scales;
+    cudaStream_t stream;
+    long long ldv;
+    int rows, hidden, w_dtype;
+    float eps_post, off_post, eps_next, off_next;
+};
+template <typename W>
+static int norm_launch(const NormArgs& g, int rows, cudaStream_t stream) {
+    const dim3 grid(rows), block(256);
+    const int c = (g.hidden + 1023) / 1024;
+    if (c <= 1) return launch_pdl(residual_rmsnorm_fp8_kernel<W, 1>, grid, block, 0, stream, g);
+    if (c == 2) return launch_pdl(residual_rmsnorm_fp8_kernel<W, 2>, grid, block, 0, stream, g);
+    if (c == 3) return launch_pdl(residual_rmsnorm_fp8_kernel<W, 3>, grid, block, 0, stream, g);
+    if (c <= 5) return launch_pdl(residual_rmsnorm_fp8_kernel<W, 5>, grid, block, 0, stream, g);
+    return launch_pdl(residual_rmsnorm_fp8_kernel<W, 8>, grid, block, 0, stream, g);
+}
+BROLM_API int brolm_residual_rmsnorm_fp8(const NormCall* c) {
+    if (c->rows <= 0) return BROLM_OK;
+    if (c->hidden <= 0 || c->hidden > 8192 || c->hidden % 4 || !c->w_next) return BROLM_ERR_BAD_SIZE;
+    if ((((uintptr_t)c->h | (uintptr_t)c->y | (uintptr_t)c->w_post | (uintptr_t)c->w_next | (uintptr_t)c->values | (uintptr_t)c->scales) & 15) ||
+        c->ldv % 16 || c->ldv < c->hidden || c->ldv >= c->hidden + 16)
+        return BROLM_ERR_ALIGNMENT;
+    const NormArgs g = {(float*)c->h, (const float*)c->y, c->w_post, c->w_next, c->eps_post, c->off_post, c->eps_next, c->off_next,
+                        (uint8_t*)c->values, (long)c->ldv, (uint8_t*)c->scales, fp8::quads_of(c->hidden), c->hidden};
+    if (c->w_dtype == BROLM_F32) return norm_launch<float>(g, c->rows, c->stream);
+    if (c->w_dtype == BROLM_BF16) return norm_launch<bf16>(g, c->rows, c->stream);
+    return BROLM_ERR_BAD_DTYPE;
 }
 
 // Two products one after the other, from one call of the host.

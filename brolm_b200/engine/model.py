@@ -144,6 +144,9 @@ class DecoderModel:
             part.bind({local: tensors[ck] for local, ck in names.items() if local in part.param_specs()})
             if self.weight_dtype == "fp8":
                 part.to_fp8()
+        if self.weight_dtype == "fp8":
+            for block in self.blocks:
+                block.to_fp8()
         self.loaded = True
         self.generation += 1
 

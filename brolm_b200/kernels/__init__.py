@@ -2205,7 +2205,7 @@ def sample(logits: torch.Tensor, temperature: float, top_k: int, top_p: float, s
 
 from .kv8 import BLOCKS_STATUS, attention_kv8, attention_kv8_tc_status, blocks_extend, blocks_release, kv8_read, kv8_write  # noqa: E402  (needs the above)
 
-from .fp8 import Fp8Matrix, experts_fp8, experts_fp8_pairs, feedforward_fp8, fp8_gate_up, fp8_gemm_status, fp8_quantize, fp8_read, fp8_stream_status, linear_fp8  # noqa: E402
+from .fp8 import Fp8Matrix, experts_fp8, experts_fp8_pairs, feedforward_fp8, fp8_gate_up, fp8_gemm_status, fp8_quantize, fp8_read, fp8_stream_status, linear_fp8, residual_rmsnorm_fp8, residual_rmsnorm_fp8_ok  # noqa: E402
 
 __all__ = ["KernelBuildError", "KernelError", "build_all", "launch_count", "device_sms", "wait_control", "embed_scale",
            "embed_pairs", "concat_cast", "latent_rows", "route_topk", "route_pick", "group_tiles", "group_pairs", "experts_tc_ok", "gather_rows", "experts_linear_tc", "grouped_tc_status", "heads_linear",
@@ -2215,4 +2215,4 @@ __all__ = ["KernelBuildError", "KernelError", "build_all", "launch_count", "devi
            "decode_splits", "decode_longest_first", "argmax", "sample", "cast", "bias_act", "scaled_sum", "qkv_norm_write", "gate_group_norm", "head_norm_gate", "rotate_heads",
            "layernorm", "residual_layernorm", "table_gate", "delta_step", "delta_prompt", "experts_combine", "causal_conv", "conv_tail", "gated_scan", "ssm_scan", "block_matvec_f32", "block_matvec_ok", "split_halves",
            "BLOCKS_STATUS", "blocks_extend", "blocks_release", "kv8_write", "kv8_read", "attention_kv8", "attention_kv8_tc_status",
-           "Fp8Matrix", "experts_fp8", "experts_fp8_pairs", "feedforward_fp8", "fp8_gate_up", "fp8_gemm_status", "fp8_quantize", "fp8_read", "fp8_stream_status", "linear_fp8"]
+           "Fp8Matrix", "experts_fp8", "experts_fp8_pairs", "feedforward_fp8", "fp8_gate_up", "fp8_gemm_status", "fp8_quantize", "fp8_read", "fp8_stream_status", "linear_fp8", "residual_rmsnorm_fp8", "residual_rmsnorm_fp8_ok"]

@@ -40,6 +40,7 @@ _raw_stream, _device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDev
 _ROWS = struct.Struct("@4P3q5i")
 _PRODUCT = struct.Struct("@7P3q8ifi5P7i2Pqi")
 _EXPERTS = struct.Struct("@13P5q14if")
+_NORM = struct.Struct("@7Pq3i4f")
 _functions: dict = {}
 _launchers: dict = {}        # by name, as other launchers are given them
 
@@ -89,6 +90,12 @@ class Fp8Matrix:
     @property
     def nbytes(self) -> int:
         return self.data.numel()
+
+    def float(self) -> torch.Tensor:
+        """The values that the matrix stands for."""
+        y = torch.empty(self.shape, dtype=_F32, device=self.device)
+        fp8_read(self, y)
+        return y
 
     def __repr__(self) -> str:
         return f"Fp8Matrix({self.shape}, gated={self.gated}, {self.device})"
@@ -166,6 +173,38 @@ def fp8_read(m: Fp8Matrix, out: torch.Tensor) -> None:
     y = out.view(-1, out.shape[-1]) if out.dim() == 3 else out
     _call("fp8_rows", "brolm_fp8_read", _ROWS.pack(y.data_ptr(), m.packed[0], m.packed[1], _raw_stream(_device()), y.stride(0), m.packed[2], y.shape[0],
                                                    _CODES[y.dtype], m.cols, m.rows, m.group_rows, 1), "fp8_read")
+
+
+def residual_rmsnorm_fp8_ok(hidden: int) -> bool:
+    """Whether ``residual_rmsnorm_fp8`` takes rows of as many numbers."""
+    return 0 < hidden <= 8192 and hidden % 4 == 0
+
+
+def residual_rmsnorm_fp8(h: torch.Tensor, y: torch.Tensor, post_weight: Optional[torch.Tensor], post_eps: float, post_offset: float,
+                         next_weight: torch.Tensor, next_eps: float, next_offset: float) -> Fp8Matrix:
+    """h += rmsnorm(y; post) (or y when ``post_weight`` is None); -> rmsnorm(h; next) as rows of 8 bits, rounded once from its float
+    result.  h and y float32 [rows, hidden], contiguous, ``hidden`` a multiple of 4 and 8,192 at most."""
+    what = "residual_rmsnorm_fp8"
+    device = h.get_device()
+    fine = h.dtype == y.dtype == _F32 and h.dim() == 2 and h.shape == y.shape and h.is_contiguous() and y.is_contiguous() \
+        and device >= 0 and device == _device() == y.get_device() and residual_rmsnorm_fp8_ok(h.shape[1])
+    for w in (next_weight, post_weight):
+        if fine and w is not None:
+            fine = w.dtype == next_weight.dtype and w.dtype in _CODES and w.numel() == h.shape[1] and w.is_contiguous() and w.get_device() == device
+    if not fine:
+        for t, name in ((h, "h"), (y, "y")):
+            _refuse(what, t, name)
+            if t.dtype != _F32 or not t.is_contiguous() or t.shape != h.shape:
+                raise KernelError(f"{what}: {name} is a packed float32 [rows, hidden], not {tuple(t.shape)} {t.dtype}")
+        if not residual_rmsnorm_fp8_ok(h.shape[1]):
+            raise KernelError(f"{what}: rows of {h.shape[1]} numbers (a multiple of 4, 8,192 at most, is wanted)")
+        raise KernelError(f"{what}: the gains are packed rows of {h.shape[1]} numbers of one element type (float32 or bfloat16) on {h.device}")
+    m = _empty(tuple(h.shape), h.device)
+    if m.rows:
+        _call("fp8_rows", "brolm_residual_rmsnorm_fp8",
+              _NORM.pack(h.data_ptr(), y.data_ptr(), post_weight.data_ptr() if post_weight is not None else 0, next_weight.data_ptr(), m.packed[0], m.packed[1],
+                         _raw_stream(device), m.packed[2], m.rows, m.cols, _CODES[next_weight.dtype], post_eps, post_offset, next_eps, next_offset), what)
+    return m
 
 
 # --- products ----------------------------------------------------------------

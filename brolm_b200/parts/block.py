@@ -33,7 +33,7 @@ import torch
 from .. import kernels
 from .attention import Attention
 from .base import Part, PartSpec, register_part
-from .feedforward import GatedFeedForward
+from .feedforward import DenseFeedForward, GatedFeedForward
 from .norm import RMSNorm, add_then_norm
 
 
@@ -83,11 +83,20 @@ class Block(Part):
     def cache_spec(self):
         return self.mixer.cache_spec()
 
+    def to_fp8(self) -> None:
+        """Once the parts keep their matrices in 8-bit floating point: the norms leave their rows so for sublayers that do
+        nothing but multiply them."""
+        for norm, part, weight in ((self.pre_mixer_norm, self.mixer, "w_qkv"), (self.pre_ffn_norm, self.feedforward, "w_gate_up"),
+                                   (self.pre_ffn_norm, self.feedforward, "w_up")):
+            if type(norm) is RMSNorm and type(part) in (Attention, GatedFeedForward, DenseFeedForward) and \
+                    isinstance(getattr(part, weight, None), kernels.Fp8Matrix):
+                norm.eight_bits = norm.groups == 1 and kernels.residual_rmsnorm_fp8_ok(norm.size)
+
     def forward(self, h: torch.Tensor, x: torch.Tensor, ctx, entry, writes_cache: bool,
                 next_norm: Optional[Part]) -> Optional[torch.Tensor]:
         """h: residual stream (updated in place); x = pre_mixer_norm(h).
         Returns next_norm(h) for the block that follows, if there is one."""
-        if ctx.mode == "prefill" and writes_cache and x.dtype == torch.bfloat16 and not ctx.cache.int8 and \
+        if ctx.mode == "prefill" and writes_cache and isinstance(x, torch.Tensor) and x.dtype == torch.bfloat16 and not ctx.cache.int8 and \
                 self._launches_at_once(x, ctx, next_norm):
             return self._forward_at_once(h, x, ctx, entry, next_norm)
         y = self.mixer.forward(x, ctx, entry, writes_cache)

@@ -39,7 +39,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, out_dtype: Optional[torch.dtyp
     product that was cut along K so that more blocks stream the weights."""
     M = x.shape[0]
     if isinstance(weight, kernels.Fp8Matrix):
-        if x.dtype not in (torch.bfloat16, torch.float32):
+        if not isinstance(x, kernels.Fp8Matrix) and x.dtype not in (torch.bfloat16, torch.float32):
             x = x.float()
         y = out if out is not None else torch.empty((M, weight.outputs), dtype=out_dtype or x.dtype, device=x.device)
         kernels.linear_fp8(x, weight, y)

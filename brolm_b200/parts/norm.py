@@ -25,6 +25,8 @@ class RMSNorm(Part):
 
     kind = "norm"
     graph_safe = True
+    # True when what reads its rows takes them in 8-bit floating point (its matrices are kept so) and nothing else reads them
+    eight_bits = False
 
     def __init__(self, size: int, eps: float, offset: float = 0.0, groups: int = 1, scalar: bool = False):
         if groups < 1 or size % groups:
@@ -113,8 +115,12 @@ def add_then_norm(h: torch.Tensor, y: torch.Tensor, post: Optional[Part], nxt: O
 
     h is the float32 residual stream and is updated in place.  Two RMSNorms, or a LayerNorm
     behind one or none, run in one kernel with the sum; any other norm part is applied through its
-    own ``apply`` and only the sum stays fused.
+    own ``apply`` and only the sum stays fused.  A norm whose rows are wanted in 8-bit floating point leaves them so.
     """
+    if type(nxt) is RMSNorm and nxt.eight_bits and (post is None or (type(post) is RMSNorm and post.groups == 1 and post.weight.dtype == nxt.weight.dtype)) \
+            and y.dim() == 2 and y.dtype == torch.float32:
+        return kernels.residual_rmsnorm_fp8(h, y, post.weight if post is not None else None, post.eps if post is not None else 0.0,
+                                            post.offset if post is not None else 0.0, nxt.weight, nxt.eps, nxt.offset)
     if isinstance(nxt, LayerNorm) and y.dtype == torch.float32 and \
             (post is None or (isinstance(post, RMSNorm) and post.groups == 1 and post.weight.dtype == nxt.weight.dtype)):
         out = torch.empty(h.shape, dtype=out_dtype, device=h.device)

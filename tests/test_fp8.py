@@ -84,3 +84,13 @@ def test_which_products_stream_their_matrix(rows, w_rows, nkb, streamed):
 @pytest.mark.parametrize("pairs, experts, rows", [(1, 32, 16), (512, 32, 16), (513, 32, 32), (1536, 32, 32), (1537, 32, 256), (5, 1, 16), (100000, 8, 256), (3, 0, 16)])
 def test_rows_of_an_experts_tile(pairs, experts, rows):
     assert fp8.experts_fp8_rows(pairs, experts) == rows
+
+
+def test_which_rows_a_norm_can_leave_in_8_bits():
+    assert [n for n in (0, 2, 4, 6, 100, 2304, 4608, 8190, 8192, 8196) if kernels.residual_rmsnorm_fp8_ok(n)] == [4, 100, 2304, 4608, 8192]
+
+
+def test_a_norm_in_8_bits_refuses_tensors_of_the_host():
+    h = torch.zeros(2, 64)
+    with pytest.raises(kernels.KernelError, match="CUDA"):
+        kernels.residual_rmsnorm_fp8(h, h.clone(), None, 1e-6, 0.0, torch.ones(64), 1e-6, 0.0)

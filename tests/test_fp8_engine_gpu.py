@@ -179,3 +179,33 @@ def test_from_the_command_line(tmp_path):
                         "--no-eos"], capture_output=True, text=True, timeout=600)
     assert r.returncode == 0, r.stderr
     assert "generated 5 tokens" in r.stdout
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("name", ["B", "wide"])
+def test_norms_that_leave_8_bits_beside_norms_and_roundings(name, dtype, monkeypatch):
+    model = build(name, dtype)
+    assert all(b.pre_mixer_norm.eight_bits and b.pre_ffn_norm.eight_bits and not b.post_ffn_norm.eight_bits for b in model.blocks) and not model.final_norm.eight_bits
+    prompts = random_prompts(model.config.vocab_size, [5, 40, 1, 17], seed=2)
+
+    def steps():
+        engine = bb.Engine(model, max_tokens=64 * 8, max_slots=4, use_graphs=False)
+        slots = engine.open(4)
+        out = [engine.step(slots, prompts).clone()]
+        for t in range(3):
+            out.append(engine.step(slots, [[7 + t]] * 4).clone())
+        return out
+    got = steps()
+    calls = []
+
+    def apart(h, y, post_weight, post_eps, post_offset, next_weight, next_eps, next_offset):
+        calls.append(len(h))
+        out = torch.empty_like(h)
+        residual_rmsnorm(h, y, post_weight, post_eps, post_offset, next_weight, next_eps, next_offset, out)
+        return kernels.fp8_quantize(out)
+    residual_rmsnorm = kernels.residual_rmsnorm
+    monkeypatch.setattr(kernels, "residual_rmsnorm_fp8", apart)
+    want = steps()
+    assert len(calls) == 4 * (2 * len(model.blocks) - 1)
+    for a, b in zip(got, want):
+        assert off(a, b) < SAME

@@ -632,3 +632,64 @@ def test_a_block_of_results_that_waits_in_vain(name):
     finally:
         kernels.wait_control("fp8_stream", 0, 0)
     assert torch.equal(run(), good) and kernels.fp8_stream_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("post", [True, False])
+@pytest.mark.parametrize("m, n", [(1, 4), (3, 100), (2, 128), (1, 1024), (9, 1028), (130, 2304), (8, 2308), (5, 4608), (3, 5124), (2, 8192), (300, 640)])
+def test_a_norm_that_leaves_8_bits(m, n, post, dtype):
+    """Against 64 bits.  Float sums of n squares, 32 additions one after the other at most, a root and three products: 2^-18 of
+    the result, for each of the two norms; the sum of h one rounding.  Then 8 bits: half a step, 2^-4 of the number, or of the
+    smallest one, 2^-10 of a scale that is a 224th of the block's largest number at most."""
+    g = gen(m + n)
+    h, y = (rows_of(g, m, n, torch.float32, 0.5) for _ in range(2))
+    wp, wn = ((0.2 * torch.randn(n, generator=g, device=DEV)).to(dtype) for _ in range(2))
+    v = y.double()
+    if post:
+        v = v * (v.square().mean(dim=1, keepdim=True) + 1e-6).rsqrt() * (1.0 + wp.double())
+    total = h.double() + v
+    off_h = 2.0 ** -18 * v.abs() + 2.0 ** -24 * total.abs()
+    gain = (total.square().mean(dim=1, keepdim=True) + 1e-5).rsqrt() * (0.5 + wn.double())
+    exact = total * gain
+    off = 2.0 ** -17 * exact.abs() + off_h * gain.abs()
+    # the root moves with h: by its largest relative change at most
+    off = off + exact.abs() * (off_h.norm(dim=1, keepdim=True) / total.norm(dim=1, keepdim=True))
+    blocks = torch.nn.functional.pad(exact.abs() + off, (0, -n % 128)).unflatten(1, (-1, 128)).amax(dim=2).repeat_interleave(128, dim=1)[:, :n]
+    bound = off + 2.0 ** -4 * (exact.abs() + off) + 2.0 ** -10 * blocks / 224.0
+    m8 = kernels.residual_rmsnorm_fp8(h, y, wp if post else None, 1e-6, 1.0, wn, 1e-5, 0.5)
+    assert m8.shape == (m, n) and bool(((h.double() - total).abs() <= off_h).all())
+    got = read(m8)
+    near(got, exact, bound)
+    assert torch.equal(read(kernels.fp8_quantize(got)), got) and torch.equal(m8.float(), got)
+    w = kernels.fp8_quantize(rows_of(g, 40, n, torch.bfloat16))
+    a, b = torch.empty(m, 40, device=DEV), torch.empty(m, 40, device=DEV)
+    kernels.linear_fp8(m8, w, a)
+    kernels.linear_fp8(kernels.fp8_quantize(got), w, b)
+    assert torch.equal(a, b)
+
+
+def test_a_norm_in_8_bits_of_rows_that_are_not_finite_and_of_none():
+    g = gen(61)
+    h, y, w = rows_of(g, 4, 300, torch.float32), rows_of(g, 4, 300, torch.float32), torch.ones(300, device=DEV)
+    y[1, 17], y[2, 5] = float("inf"), float("nan")
+    good = [read(kernels.residual_rmsnorm_fp8(h[i:i + 1].clone(), y[i:i + 1].clone(), w, 1e-6, 0.0, w, 1e-6, 0.0)) for i in (0, 3)]
+    got = read(kernels.residual_rmsnorm_fp8(h, y, w, 1e-6, 0.0, w, 1e-6, 0.0))
+    assert torch.equal(got[0:1], good[0]) and torch.equal(got[3:4], good[1]) and bool(got[1:3].isnan().all())
+    assert kernels.residual_rmsnorm_fp8(h[:0], y[:0], None, 0.0, 0.0, w, 1e-6, 0.0).shape == (0, 300)
+    zero = torch.zeros(2, 300, device=DEV)
+    assert not read(kernels.residual_rmsnorm_fp8(zero, zero.clone(), None, 0.0, 0.0, w, 1e-6, 0.0)).any()
+
+
+def test_refusals_of_the_norm_in_8_bits():
+    h, y, w = torch.zeros(2, 64, device=DEV), torch.zeros(2, 64, device=DEV), torch.ones(64, device=DEV)
+    call = lambda h, y, post, nxt: kernels.residual_rmsnorm_fp8(h, y, post, 1e-6, 0.0, nxt, 1e-6, 0.0)
+    for args, what in (((h.bfloat16(), y, None, w), "float32"), ((h, y[:1], None, w), "rows, hidden"), ((h, torch.zeros(2, 128, device=DEV)[:, ::2], None, w), "packed"),
+                       ((h[:, :6].contiguous(), y[:, :6].contiguous(), None, w[:6]), "multiple of 4"), ((h, y, None, w[:60]), "gains"),
+                       ((torch.zeros(1, 8196, device=DEV), torch.zeros(1, 8196, device=DEV), None, torch.ones(8196, device=DEV)), "8,192"),
+                       ((h, y, w.bfloat16(), w), "gains"), ((h, y, None, w.cpu()), "gains"), ((h.cpu(), y, None, w), "CUDA"), ((h, y.half(), None, w), "float32")):
+        with pytest.raises(kernels.KernelError, match=what):
+            call(*args)
+    odd = torch.zeros(2 * 64 + 1, device=DEV)[1:].view(2, 64)           # a base that is no border of 16 bytes
+    with pytest.raises(kernels.KernelError):
+        call(odd, y, None, w)
+    assert not h.any() and not y.any()
