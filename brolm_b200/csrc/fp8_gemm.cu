@@ -330,9 +330,10 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                 uint32_t sfw = 0, sfx = 0;
                 for (int lo = 0; lo < g.nkb && ok; lo += g.piece, ++local) {
                     const int as = local & 1, hi = min(g.nkb, lo + g.piece);
-                    ok = wait_on(acc_free0 + 8 * as, ((local >> 1) & 1) ^ 1, give_up, 5) && wait_on(lap_free, (local & 1) ^ 1, give_up, 6);
+                    // The wait that ends last is the one for the columns that this piece's accumulator shares with the piece
+                    // before; all else that the first block needs comes ahead of it (2,048 x 9,216 x 2,304 gated 80.9 -> 78.8 us).
+                    ok = wait_on(acc_free0 + 8 * as, ((local >> 1) & 1) ^ 1, give_up, 5);
                     if (!ok) break;
-                    fence_after_sync();
                     const uint32_t acc = tmem + as * ACC1;
                     for (int kb = lo; kb < hi; ++kb) {
                         // (the flags are looked at where a piece begins and where the stage is not there yet)
@@ -347,6 +348,11 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                             scales_to_tmem_pair(sfx, desc_scales(src));
                             scales_to_tmem_pair(sfw, desc_scales(src + SF_TILE));
                             scales_to_tmem_pair(sfw + 4, desc_scales(src + 2 * SF_TILE));
+                        }
+                        if (kb == lo) {
+                            ok = wait_on(lap_free, (local & 1) ^ 1, give_up, 6);
+                            if (!ok) break;
+                            fence_after_sync();
                         }
                         const uint32_t idk = with_block(id, kb & 3, kb & 3);
                         const uint64_t a = desc_kmajor(stage0 + s * STAGE_BYTES), b = desc_kmajor(stage0 + s * STAGE_BYTES + A_BYTES);
