@@ -114,18 +114,17 @@ __device__ __forceinline__ void arrive_first_block(uint32_t bar) {              
                  ::"r"(bar) : "memory");
 }
 
-// N / 2 gated pairs of neighbouring numbers, to the front.  Which activation is asked once for all of them.
+// N / 2 gated pairs of neighbouring numbers, to the front.  Code for two kinds of gates and not for three: the shorter the epilogue,
+// the less the issue of products waits for instructions (512 tokens through experts 73 -> 70 us).
 template <int N>
 __device__ __forceinline__ void gate_pairs(float (&o)[N], int act, float limit) {
-    if (act == 0) {
-#pragma unroll
-        for (int i = 0; i < N / 2; ++i) o[i] = gate_of(o[2 * i], o[2 * i + 1], 0, 0.0f);
-    } else if (act == 1) {
-#pragma unroll
-        for (int i = 0; i < N / 2; ++i) o[i] = gate_of(o[2 * i], o[2 * i + 1], 1, 0.0f);
-    } else {
+    if (act == 2) {
 #pragma unroll
         for (int i = 0; i < N / 2; ++i) o[i] = gate_of(o[2 * i], o[2 * i + 1], 2, limit);
+    } else {
+        const int kind = act == 0 ? 0 : 1;
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) o[i] = gate_of(o[2 * i], o[2 * i + 1], kind, 0.0f);
     }
 }
 
@@ -144,23 +143,32 @@ __device__ __forceinline__ void flush_rows(const uint8_t* room, int lane, uint8_
     constexpr int PIECES = ROW / 16, ROWS = 32 / PIECES;       // rows a round
     const int piece = lane % PIECES, left = bytes - piece * 16;
     dst += piece * 16;
+    if (wide && bytes >= ROW) {
+        uint8_t* to = dst + (lane / PIECES) * ld;
 #pragma unroll
-    for (int r0 = 0; r0 < 32; r0 += ROWS) {
-        const int r = r0 + lane / PIECES;
-        const uint4 v = *reinterpret_cast<const uint4*>(room + r * 128 + ((piece ^ (r & 7)) << 4));
-        const int place = SCATTER ? __shfl_sync(0xffffffffu, at, r) : r;
-        uint8_t* to = dst + (long)place * ld;
-        if (r < rows && left > 0) {
-            if (wide && left >= 16) *reinterpret_cast<uint4*>(to) = v;
-            else {
-                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-                if (unit == 4) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) if (4 * i < left) reinterpret_cast<uint32_t*>(to)[i] = w[i];
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) if (2 * i < left) reinterpret_cast<uint16_t*>(to)[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
-                }
+        for (int r0 = 0; r0 < 32; r0 += ROWS) {
+            const int r = r0 + lane / PIECES;
+            const uint4 v = *reinterpret_cast<const uint4*>(room + r * 128 + ((piece ^ (r & 7)) << 4));
+            if (SCATTER) to = dst + (long)__shfl_sync(0xffffffffu, at, r) * ld;
+            if (r < rows) *reinterpret_cast<uint4*>(to) = v;
+            if (!SCATTER) to += ROWS * ld;
+        }
+    } else {
+        // few tiles come here: short code, since the products' issue suffers where the epilogue's is long
+#pragma unroll 1
+        for (int r0 = 0; r0 < 32; r0 += ROWS) {
+            const int r = r0 + lane / PIECES;
+            const uint8_t* from = room + r * 128 + ((piece ^ (r & 7)) << 4);
+            uint8_t* to = dst + (long)(SCATTER ? __shfl_sync(0xffffffffu, at, r) : r) * ld;
+            const int n = r < rows ? min(left, 16) : 0;
+            if (wide && n == 16) {
+                *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(from);
+            } else if (unit == 4) {
+#pragma unroll 1
+                for (int i = 0; i < n; i += 4) *reinterpret_cast<uint32_t*>(to + i) = *reinterpret_cast<const uint32_t*>(from + i);
+            } else {
+#pragma unroll 1
+                for (int i = 0; i < n; i += 2) *reinterpret_cast<uint16_t*>(to + i) = *reinterpret_cast<const uint16_t*>(from + i);
             }
         }
     }
