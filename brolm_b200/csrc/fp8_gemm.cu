@@ -292,9 +292,10 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             bool ok = !*give_up;
             // Launched with programmatic stream serialization: nothing of this kernel touches memory before its first
             // operands have arrived, so (but for the experts' lists) the loader's wait is the kernel's.  W depends on no
-            // kernel: the first stages' part of it is asked for before (experts': where their list is known by then).
+            // kernel, once it is not new: the first stages' part of it is asked for before (experts': where their list is
+            // known by then).
             int early = 0;
-            if ((!EXPERTS || g.listed) && ok) {
+            if (g.listed && ok) {
                 int whole, mt, nt, half_of, group, row0;
                 if (pair < items_of(tiles_of(), whole)) {
                     find(pair, whole, mt, nt, half_of, group, row0);
@@ -633,6 +634,7 @@ BROLM_API int brolm_fp8_gemm(const fp8::ProductCall* c) {
     g.piece = c->out == OUT_F32 && c->cut > 0 && c->cut < g.nkb ? c->cut : g.nkb;
     g.m_tiles = (int)m_tiles; g.n_tiles = (int)n_tiles;
     if (!c->experts) {
+        g.listed = !c->fresh;
         st = round_first(c);
         return st ? st : dispatch<false>(m, g, c->epilogue, c->out, c->stream);
     }

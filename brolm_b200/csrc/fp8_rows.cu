@@ -32,8 +32,9 @@ __global__ void __launch_bounds__(THREADS) quantize_kernel(RowsArgs g) {
     const int lane = threadIdx.x & 31;
     const long items = g.rows * g.quads;
     pdl_wait();
-    // The products read their matrix before they wait for the kernel before them, so a kernel that writes a matrix lets
-    // nothing begin before it has ended; one that writes rows that a product waits for lets it begin at once.
+    // Products read a matrix that is not new before they wait for the kernel before them.  A kernel that writes a matrix lets
+    // nothing begin before its blocks have ended, and the matrix's first product waits for it like any reader (a fence here
+    // instead took 4 of 26 us); one that writes rows that a product waits for lets it begin at once.
     if (g.early) pdl_trigger();
     for (long item = (long)blockIdx.x * WARPS + (threadIdx.x >> 5); item < items; item += (long)gridDim.x * WARPS) {
         const long row = items <= 0xffffffffl ? (long)((uint32_t)item / (uint32_t)g.quads) : item / g.quads;    // (a long division is 70 instructions)
@@ -49,7 +50,6 @@ __global__ void __launch_bounds__(THREADS) quantize_kernel(RowsArgs g) {
         if (c < g.ldv) *reinterpret_cast<uint4*>(g.values + at * g.ldv + c) = q;     // ldv is a multiple of 16
         if (lane == 0) *reinterpret_cast<uint32_t*>(g.scales + scale_at(at, quad, g.quads)) = word;
     }
-    if (!g.early) __threadfence();                  // (and its stores have arrived by then)
 }
 
 // For reading back the lanes' words lie side by side: eight bfloat16 numbers or four floats a word of sixteen bytes.  (With

@@ -65,7 +65,7 @@ struct StreamArgs {
     const int32_t* perm;
     const float* scale;      // of a pair, before the activation
     int down, top, tokens, group_rows;
-    int listed;
+    int listed;              // what names W is there, and W itself, before this kernel's wait
 };
 
 __device__ __forceinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile int* give_up, int code) {
@@ -395,8 +395,9 @@ __global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS, 2) fp8_stream_kerne
             };
             int item = first, kb = lo, it = 0, rt = 0, group = 0, row0 = 0, tile = 0;
             bool more;
-            // The ring fills with weights before the kernel before this one has ended; experts' where their list is known by then.
-            const bool ahead = !EXPERTS || g.listed;
+            // The ring fills with weights before the kernel before this one has ended, if they are not what it writes; experts'
+            // where their list is known by then.
+            const bool ahead = g.listed;
             if (!ahead) pdl_wait();
             more = item < g.items && lo < hi && find(item, rt, group, row0, tile);
             if (ahead) {
@@ -728,6 +729,7 @@ BROLM_API int brolm_fp8_stream(const fp8::ProductCall* c) {
         mx = mw;
     }
     g.row_tiles = g.items = (int)row_tiles;
+    g.listed = !c->fresh;
     st = round_first(c);
     if (st) return st;
     return dispatch<false>(mw, mx, g, bt, slices, c->fused, c->epilogue, c->out, c->stream);

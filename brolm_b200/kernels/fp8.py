@@ -8,9 +8,8 @@ finite is NaN as a whole, and so is what is computed from it.  Both sides of a p
 are float32.
 
 ``Fp8Matrix`` holds rows in the order the kernels want them: ``fp8_quantize`` makes one from rows or a matrix, or from a stack
-of experts' matrices; ``fp8_gate_up`` from the two matrices of a gated feed-forward, whose rows then alternate.  A matrix in
-use as a weight may be read before what runs ahead of the product in its stream has ended, except for ``fp8_quantize`` itself;
-it is made once and kept.
+of experts' matrices; ``fp8_gate_up`` from the two matrices of a gated feed-forward, whose rows then alternate.  A matrix's
+first product waits for what runs ahead of it, later ones may read the matrix before that has ended: it is made once and kept.
 
 The functions launch on the current stream, like all of this package; they wait for nothing and keep nothing.
 """
@@ -38,7 +37,7 @@ _raw_stream, _device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDev
 # struct, packed here as C lays it out, and the checks of a call's arguments are one expression; which of them failed is found
 # out only then.
 _ROWS = struct.Struct("@4P3q5i")
-_PRODUCT = struct.Struct("@7P3q8ifi5P7i2Pqi")
+_PRODUCT = struct.Struct("@7P3q8ifi5P7i2Pqii")
 _EXPERTS = struct.Struct("@13P5q14if")
 _NORM = struct.Struct("@7Pq3i4f")
 _functions: dict = {}
@@ -64,7 +63,7 @@ class Fp8Matrix:
     partner alternate, so that a product has half as many results as there are rows.  It is not to be changed once it is in
     use.  ``data`` holds ``values``, uint8 [rows of all experts, columns rounded up to 16], an expert's matrix beginning on a
     multiple of 128 rows, and behind them ``scales``, uint8 [rows / 128, columns / 512, 512]."""
-    __slots__ = ("data", "shape", "gated", "rows", "cols", "outputs", "group_rows", "total", "device", "index", "packed")
+    __slots__ = ("data", "shape", "gated", "rows", "cols", "outputs", "group_rows", "total", "device", "index", "packed", "fresh")
 
     def __init__(self, data: torch.Tensor, shape: tuple, gated: bool = False):
         self.data, self.shape, self.gated = data, shape, gated
@@ -76,6 +75,8 @@ class Fp8Matrix:
         self.total = rows if len(shape) == 2 else shape[0] * self.group_rows
         self.device = data.device
         self.index = data.get_device()
+        # until its first product, which does not read it ahead of what runs before
+        self.fresh = True
         at, ld = data.data_ptr(), (cols + 15) & -16
         self.packed = (at, at + ((self.total * ld + 511) & -512), ld)
 
@@ -304,7 +305,9 @@ def _pack(how: tuple, x, at: int, M: int, w: Fp8Matrix, y: tuple, out: int, act:
     """A product's struct.  ``x``: (values, scales, stride) of rows in 8 bits, or (numbers, 0, stride, type) of rows that are
     rounded on the way, into the scratch at ``at`` if not by the product itself."""
     K = w.cols
-    fused, raw = 0, _THERE
+    fused, raw, fresh = 0, _THERE, 0
+    if w.fresh:
+        w.fresh, fresh = False, 1
     if len(x) == 4:
         if how[2]:
             fused = _FUSED[x[3]]
@@ -314,7 +317,7 @@ def _pack(how: tuple, x, at: int, M: int, w: Fp8Matrix, y: tuple, out: int, act:
             x = (at, at + ((M * ld + 511) & -512), ld)
     wv, ws, ldw = w.packed
     return _PRODUCT.pack(x[0], x[1], wv, ws, y[0], y[1], stream, x[2], ldw, y[2], M, w.outputs, K, 1 if w.gated else 0, act, out, fused, how[1], limit,
-                         *_NO_EXPERTS, *raw)
+                         *_NO_EXPERTS, *raw, fresh)
 
 
 def linear_fp8(x, w: Fp8Matrix, out: torch.Tensor, activation: str = "none", limit: float = 0.0) -> None:

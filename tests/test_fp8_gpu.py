@@ -693,3 +693,39 @@ def test_refusals_of_the_norm_in_8_bits():
     with pytest.raises(kernels.KernelError):
         call(odd, y, None, w)
     assert not h.any() and not y.any()
+
+
+@pytest.mark.parametrize("m", [3, 60, 300])
+def test_a_new_matrix_is_not_read_ahead_of_what_makes_it(m):
+    """One that is made in the stream right before its first product, by this package's kernel or by another's, through a norm whose
+    next kernel may begin before it has ended, too."""
+    g = gen(71)
+    h, y, gain = rows_of(g, m, 1024, torch.float32), torch.zeros(m, 1024, device=DEV), torch.ones(1024, device=DEV)
+    x = kernels.residual_rmsnorm_fp8(h.clone(), y, None, 0.0, 0.0, gain, 1e-6, 0.0)
+    ws = [rows_of(g, 5000, 1024, torch.bfloat16) for _ in range(3)]
+    want = []
+    for w in ws:
+        m8 = kernels.fp8_quantize(w)
+        assert m8.fresh
+        torch.cuda.synchronize()
+        want.append(torch.empty(m, 5000, device=DEV))
+        kernels.linear_fp8(x, m8, want[-1])
+        assert not m8.fresh
+    old = kernels.fp8_quantize(ws[0])
+    data = [kernels.fp8_quantize(w).data for w in ws]
+    torch.cuda.synchronize()
+    for turn in range(12):
+        out, again, other = (torch.full((m, 5000), 7.0, device=DEV) for _ in range(3))
+        m8 = kernels.fp8_quantize(ws[turn % 3])
+        x2 = kernels.residual_rmsnorm_fp8(h.clone(), y, None, 0.0, 0.0, gain, 1e-6, 0.0) if turn % 2 else x
+        kernels.linear_fp8(x2, m8, out)
+        kernels.linear_fp8(x2, m8, again)
+        copied = kernels.Fp8Matrix(old.data.clone(), old.shape)
+        copied.data.copy_(data[turn % 3])
+        kernels.linear_fp8(x2, copied, other)
+        for o in (out, again, other):
+            assert torch.equal(o, want[turn % 3])
+    up, down = kernels.fp8_gate_up(ws[0], ws[1]), kernels.fp8_quantize(rows_of(g, 64, 5000, torch.bfloat16))
+    assert up.fresh and down.fresh
+    kernels.feedforward_fp8(x, up, down, torch.empty(m, 64, device=DEV), "silu")
+    assert not up.fresh and not down.fresh
