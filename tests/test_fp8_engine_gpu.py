@@ -209,3 +209,20 @@ def test_norms_that_leave_8_bits_beside_norms_and_roundings(name, dtype, monkeyp
     assert len(calls) == 4 * (2 * len(model.blocks) - 1)
     for a, b in zip(got, want):
         assert off(a, b) < SAME
+
+
+def test_matrices_and_the_cache_in_8_bits_together():
+    """Whole prompts and the same in pieces on top of a cache in 8 bits, with rows in 8 bits from norm to product.  A piece reads keys
+    and values off by a 254th of a page's largest, some 1 % of their size; a row that is 1 % off has one number in nine on the other
+    side of a border of 8 bits, a step of 9 %: 3 % of a product, and six products follow one another: 7 %, doubled."""
+    model = build("wide", "bfloat16")
+    prompts = random_prompts(model.config.vocab_size, [70, 9], seed=4)
+    whole = bb.Engine(model, max_tokens=64 * 8, max_slots=2, cache_dtype="int8")
+    slots = whole.open(2)
+    a = [whole.step(slots, prompts).clone()] + [whole.step(slots, [[t], [t + 1]]).clone() for t in (3, 8)]
+    pieces = bb.Engine(model, max_tokens=64 * 8, max_slots=2, cache_dtype="int8", max_piece=128)
+    slots = pieces.open(2)
+    pieces.step(slots, [p[:4] for p in prompts])
+    b = [pieces.step(slots, [p[4:] for p in prompts]).clone()] + [pieces.step(slots, [[t], [t + 1]]).clone() for t in (3, 8)]
+    for x, y in zip(a, b):
+        assert x.isfinite().all() and y.isfinite().all() and off(x, y) < 0.15
