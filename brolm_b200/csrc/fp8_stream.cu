@@ -616,18 +616,21 @@ int launch(const CUtensorMap& mw, const CUtensorMap& mx, StreamArgs g, int slice
     const bool split = slices > 1;
     const int members = split ? slices : ROUND && EPI == EPI_GATED ? 2 : 1;
     // Two blocks an SM: one streams while the other starts or ends, and clusters of up to eight find room.  (Three with 74 KB,
-    // where experts' items fill their rounds better, gained nothing.)
-    constexpr size_t ROOM = 112 * 1024;
-    int stages = MAX_STAGES;
-    while (stages > 2 && S::smem(stages, g.per) > ROOM) --stages;
-    const size_t smem = S::smem(stages, g.per);
-    if (smem > ROOM || (split && (size_t)stages * S::STAGE_BYTES < (size_t)BT * BR * 4)) return BROLM_ERR_TOO_LARGE;
-    g.stages = stages;
-    static OncePerDevice done;
-    const int st = allow_shared_memory(fp8_stream_kernel<BT, EPI, EXPERTS, FUSED, ROUND>, ROOM, done);
-    if (st) return st;
+    // where experts' items fill their rounds better, gained nothing.)  Where no more than half of the SMs get a block, its ring
+    // is longer: a layer of 1,152 and 6,912 with 48 rows 25.2 -> 24.2 us.  (With more blocks the kernel behind
+    // finds no room to begin beside them: 98 of 148 SMs 20.1 -> 21.7, all of them 26.9 -> 28.2.)
+    constexpr size_t HALF = 112 * 1024, MORE = 150 * 1024;
     const int places = 2 * sms / members;
     const int grid = members * (split || g.items < places ? g.items : places);
+    const size_t room = 2 * grid <= sms ? MORE : HALF;
+    int stages = MAX_STAGES;
+    while (stages > 2 && S::smem(stages, g.per) > room) --stages;
+    const size_t smem = S::smem(stages, g.per);
+    if (smem > room || (split && (size_t)stages * S::STAGE_BYTES < (size_t)BT * BR * 4)) return BROLM_ERR_TOO_LARGE;
+    g.stages = stages;
+    static OncePerDevice done;
+    const int st = allow_shared_memory(fp8_stream_kernel<BT, EPI, EXPERTS, FUSED, ROUND>, MORE, done);
+    if (st) return st;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(S::THREADS);
