@@ -9,7 +9,8 @@ are float32.
 
 ``Fp8Matrix`` holds rows in the order the kernels want them: ``fp8_quantize`` makes one from rows or a matrix, or from a stack
 of experts' matrices; ``fp8_gate_up`` from the two matrices of a gated feed-forward, whose rows then alternate.  A matrix's
-first product waits for what runs ahead of it, later ones may read the matrix before that has ended: it is made once and kept.
+first product (captured, it stays so) waits for what runs ahead of it, later ones may read the matrix before that has ended: it is
+made once and kept.
 
 The functions launch on the current stream, like all of this package; they wait for nothing and keep nothing.
 """
