@@ -8,11 +8,13 @@ finite is NaN as a whole, and so is what is computed from it.  Both sides of a p
 are float32.
 
 ``Fp8Matrix`` holds rows in the order the kernels want them: ``fp8_quantize`` makes one from rows or a matrix, or from a stack
-of experts' matrices; ``fp8_gate_up`` from the two matrices of a gated feed-forward, whose rows then alternate.  A matrix's
-first product (captured, it stays so) waits for what runs ahead of it, later ones may read the matrix before that has ended: it is
-made once and kept.
+of experts' matrices; ``fp8_gate_up`` from the two matrices of a gated feed-forward, whose rows then alternate.  A matrix is made
+once and kept, on the stream that is current when the object is made.  Its products wait for what runs ahead of them until one has
+been launched on that stream (captured ones count for nothing and, captured before that, stay so); from then on they may read
+the matrix before what runs ahead of them has ended.
 
-The functions launch on the current stream, like all of this package; they wait for nothing and keep nothing.
+The functions launch on the current stream, like all of this package, and wait for nothing.  All that is kept from call to call is
+whether a matrix has had that product.
 """
 from __future__ import annotations
 
@@ -64,7 +66,7 @@ class Fp8Matrix:
     partner alternate, so that a product has half as many results as there are rows.  It is not to be changed once it is in
     use.  ``data`` holds ``values``, uint8 [rows of all experts, columns rounded up to 16], an expert's matrix beginning on a
     multiple of 128 rows, and behind them ``scales``, uint8 [rows / 128, columns / 512, 512]."""
-    __slots__ = ("data", "shape", "gated", "rows", "cols", "outputs", "group_rows", "total", "device", "index", "packed", "fresh")
+    __slots__ = ("data", "shape", "gated", "rows", "cols", "outputs", "group_rows", "total", "device", "index", "packed", "stream", "fresh")
 
     def __init__(self, data: torch.Tensor, shape: tuple, gated: bool = False):
         self.data, self.shape, self.gated = data, shape, gated
@@ -76,7 +78,9 @@ class Fp8Matrix:
         self.total = rows if len(shape) == 2 else shape[0] * self.group_rows
         self.device = data.device
         self.index = data.get_device()
-        # until its first product, which does not read it ahead of what runs before
+        # What makes it ends on this stream without a fence, so a product right behind that, with another stream's product already
+        # launched or none, must not read ahead.  Other streams reach the matrix through an event, which is behind its stores.
+        self.stream = _raw_stream(self.index) if self.index >= 0 else 0
         self.fresh = True
         at, ld = data.data_ptr(), (cols + 15) & -16
         self.packed = (at, at + ((self.total * ld + 511) & -512), ld)
@@ -306,9 +310,7 @@ def _pack(how: tuple, x, at: int, M: int, w: Fp8Matrix, y: tuple, out: int, act:
     """A product's struct.  ``x``: (values, scales, stride) of rows in 8 bits, or (numbers, 0, stride, type) of rows that are
     rounded on the way, into the scratch at ``at`` if not by the product itself."""
     K = w.cols
-    fused, raw, fresh = 0, _THERE, 0
-    if w.fresh:
-        w.fresh, fresh = False, 1
+    fused, raw = 0, _THERE
     if len(x) == 4:
         if how[2]:
             fused = _FUSED[x[3]]
@@ -318,7 +320,14 @@ def _pack(how: tuple, x, at: int, M: int, w: Fp8Matrix, y: tuple, out: int, act:
             x = (at, at + ((M * ld + 511) & -512), ld)
     wv, ws, ldw = w.packed
     return _PRODUCT.pack(x[0], x[1], wv, ws, y[0], y[1], stream, x[2], ldw, y[2], M, w.outputs, K, 1 if w.gated else 0, act, out, fused, how[1], limit,
-                         *_NO_EXPERTS, *raw, fresh)
+                         *_NO_EXPERTS, *raw, 1 if w.fresh else 0)
+
+
+def _launched(stream: int, *matrices: Fp8Matrix) -> None:
+    """Products with these matrices have been launched on ``stream``: there the matrices are complete for what comes next."""
+    for w in matrices:
+        if w.fresh and stream == w.stream and not torch.cuda.is_current_stream_capturing():
+            w.fresh = False
 
 
 def linear_fp8(x, w: Fp8Matrix, out: torch.Tensor, activation: str = "none", limit: float = 0.0) -> None:
@@ -341,11 +350,14 @@ def linear_fp8(x, w: Fp8Matrix, out: torch.Tensor, activation: str = "none", lim
             at = held.data_ptr()
             add_launches(1)
         x = (x.data_ptr(), 0, x.stride(0), x.dtype)
-    packed = _pack(how, x, at, M, w, (out.data_ptr(), 0, out.stride(0)), _OUT[out.dtype], act, limit, _raw_stream(device))
+    stream = _raw_stream(device)
+    packed = _pack(how, x, at, M, w, (out.data_ptr(), 0, out.stride(0)), _OUT[out.dtype], act, limit, stream)
     if how[0]:
         _call("fp8_stream", "brolm_fp8_stream", packed, "linear_fp8")
     else:
         _call("fp8_gemm", "brolm_fp8_gemm", packed, "linear_fp8")
+    if w.fresh:
+        _launched(stream, w)
 
 
 def feedforward_fp8(x, gate_up: Fp8Matrix, down: Fp8Matrix, out: torch.Tensor, activation: str = "gelu_tanh", limit: float = 0.0) -> None:
@@ -382,6 +394,8 @@ def feedforward_fp8(x, gate_up: Fp8Matrix, down: Fp8Matrix, out: torch.Tensor, a
     launch = lambda streamed: _launcher("fp8_stream", "brolm_fp8_stream") if streamed else _launcher("fp8_gemm", "brolm_fp8_gemm")
     _check(f(a, launch(first[0]), b, launch(second[0])), "feedforward_fp8")
     add_launches(1 + (1 if x8 else 0) + (1 if floats and h8 else 0))
+    if gate_up.fresh or down.fresh:
+        _launched(stream, gate_up, down)
 
 
 # --- routed experts -----------------------------------------------------------

@@ -1,0 +1,110 @@
+"""When a product may read its matrix ahead of what runs before it, and what a matrix keeps, on the CPU: the launchers are replaced."""
+import pytest
+import torch
+
+from brolm_b200 import kernels
+from brolm_b200.kernels import fp8
+
+MAKER, OTHER = 11, 22          # two streams
+
+
+class Launches:
+    """Stands for the device: which stream is current, whether it is capturing, and the products' structs as they were launched."""
+
+    def __init__(self, monkeypatch):
+        self.stream, self.capturing, self.fails, self.products = MAKER, False, False, []
+        monkeypatch.setattr(fp8, "_raw_stream", lambda device: self.stream)
+        monkeypatch.setattr(fp8, "_device", lambda: 0)
+        monkeypatch.setattr(fp8, "device_sms", lambda device: 148)
+        monkeypatch.setattr(fp8, "_checked", lambda *args: None)
+        monkeypatch.setattr(fp8, "add_launches", lambda n: None)
+        monkeypatch.setattr(fp8, "_launcher", lambda lib, name: 1)
+        monkeypatch.setattr(fp8, "_call", lambda lib, name, packed, what: self.launch(packed))
+        monkeypatch.setitem(fp8._functions, "brolm_fp8_two", lambda a, first, b, second: self.launch(a, b))
+        monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: self.capturing)
+
+    def launch(self, *products):
+        if self.fails:
+            raise kernels.KernelError("refused")
+        self.products += products
+        return 0
+
+    def waits(self):
+        """Of the products launched since the last look: whether each waits before it reads its matrix."""
+        said = [bool(fp8._PRODUCT.unpack(p)[-1]) for p in self.products]
+        self.products = []
+        return said
+
+
+@pytest.fixture
+def device(monkeypatch):
+    return Launches(monkeypatch)
+
+
+def matrix(rows, cols, gated=False):
+    m = fp8._empty((rows, cols), "cpu", gated)
+    m.index, m.stream = 0, MAKER
+    return m
+
+
+def product(w):
+    kernels.linear_fp8(matrix(3, w.cols), w, torch.zeros(3, w.outputs))
+
+
+def test_the_first_product_waits_and_later_ones_do_not(device):
+    w = matrix(64, 256)
+    product(w)
+    product(w)
+    assert device.waits() == [True, False]
+
+
+def test_a_product_on_another_stream_leaves_the_matrix_new_for_the_one_that_made_it(device):
+    w = matrix(64, 256)
+    device.stream = OTHER
+    product(w)
+    device.stream = MAKER
+    product(w)
+    device.stream = OTHER
+    product(w)
+    assert device.waits() == [True, True, False]
+
+
+def test_a_captured_product_leaves_the_matrix_new(device):
+    w = matrix(64, 256)
+    device.capturing = True
+    product(w)
+    product(w)
+    device.capturing = False
+    product(w)
+    product(w)
+    assert device.waits() == [True, True, True, False]
+
+
+def test_a_refused_launch_leaves_the_matrix_new(device):
+    w, up, down = matrix(64, 256), matrix(2 * 128, 256, True), matrix(64, 128)
+    device.fails = True
+    with pytest.raises(kernels.KernelError):
+        product(w)
+    with pytest.raises(kernels.KernelError):
+        kernels.feedforward_fp8(matrix(3, 256), up, down, torch.zeros(3, 64), "silu")
+    device.fails = False
+    product(w)
+    kernels.feedforward_fp8(matrix(3, 256), up, down, torch.zeros(3, 64), "silu")
+    kernels.feedforward_fp8(matrix(3, 256), up, down, torch.zeros(3, 64), "silu")
+    assert device.waits() == [True, True, True, False, False]
+
+
+def test_what_a_product_says_of_its_matrix_is_what_it_found(device):
+    """Two threads with a new matrix: the second packs before the first has launched."""
+    w = matrix(64, 256)
+    seen = []
+    launch = device.launch
+
+    def between(*products):
+        if not seen:
+            seen.append(w.fresh)
+            product(w)                                   # (the other thread's whole call)
+        return launch(*products)
+    device.launch = between
+    product(w)
+    assert seen == [True] and device.waits() == [True, True]
