@@ -350,7 +350,10 @@ __global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS, 2) fp8_stream_kerne
         give_up[0] = aligned ? 0 : 1;
         give_up[1] = 0;
         give_up[2] = tc::g_stall_code;
-        if (!aligned) atomicCAS(&g_fp8_stream_error, 0, 13);
+        if (!aligned) {
+            atomicCAS(&g_fp8_stream_error, 0, 13);
+            pdl_wait();                                        // (no loader will: a block does not end ahead of the kernel before)
+        }
         mbar_init_fence();
     }
     if (ROUND) for (int i = threadIdx.x; i < MOST; i += S::THREADS) most_of[i] = 0;
@@ -426,7 +429,10 @@ __global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS, 2) fp8_stream_kerne
                     more = item < g.items && find(item, rt, group, row0, tile);
                 }
             }
-            pdl_trigger();                               // the stream is asked for: the next kernel may move in
+            // The stream is asked for: the next kernel may move in.  One thread's word stands for the block's, so no other
+            // thread gives it: this one has waited, and what the next kernel reads ahead of its own wait (an experts' list, a
+            // matrix that is not new) is there by then.
+            pdl_trigger();
             if (*give_up) {
                 for (int j = max(0, it - stages); j < it; ++j) drain_on(full0 + 8 * (j % stages), (j / stages) & 1, give_up, 4);
             }
@@ -553,7 +559,6 @@ __global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS, 2) fp8_stream_kerne
             }
         }
     }
-    pdl_trigger();
     fence_before_sync();
     if (team) {
         __syncwarp();

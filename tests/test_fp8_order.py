@@ -1,9 +1,12 @@
 """When a product may read its matrix ahead of what runs before it, and what a matrix keeps, on the CPU: the launchers are replaced."""
+import os
+
 import pytest
 import torch
 
 from brolm_b200 import kernels
 from brolm_b200.kernels import fp8
+from brolm_b200.kernels.build import CSRC
 
 MAKER, OTHER = 11, 22          # two streams
 
@@ -108,3 +111,18 @@ def test_what_a_product_says_of_its_matrix_is_what_it_found(device):
     device.launch = between
     product(w)
     assert seen == [True] and device.waits() == [True, True]
+
+
+@pytest.mark.parametrize("source", ["fp8_stream.cu", "fp8_gemm.cu"])
+def test_the_thread_that_lets_the_next_kernel_begin_has_waited(source):
+    """One thread's trigger stands for its block.  The products have one, the loader's, and the loader waits on every way to it
+    (in the stream on one of two: ahead of its first loads, or behind those of the matrix)."""
+    with open(os.path.join(CSRC, source)) as f:
+        kernel = f.read().split("__global__", 1)[1].split("\n}\n", 1)[0]
+    assert kernel.count("pdl_trigger()") == 1
+    loader = kernel[kernel.index("if (warp == 0) {"):kernel.index("} else if (warp == 1) {")]
+    ahead = loader[:loader.index("pdl_trigger()")]
+    if source == "fp8_stream.cu":
+        assert "if (!ahead) pdl_wait();" in ahead and ahead[ahead.index("if (ahead) {"):].count("pdl_wait();") == 1
+    else:
+        assert "\n            pdl_wait();\n" in ahead                 # (at the loader's own level: on every way)
