@@ -85,6 +85,9 @@ class Fp8Matrix:
         at, ld = data.data_ptr(), (cols + 15) & -16
         self.packed = (at, at + ((self.total * ld + 511) & -512), ld)
 
+    def __reduce__(self):
+        return Fp8Matrix, (self.data, self.shape, self.gated)      # a copy has addresses of its own
+
     @property
     def values(self) -> torch.Tensor:
         return self.data[:self.total * self.packed[2]].view(self.total, self.packed[2])

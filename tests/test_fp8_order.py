@@ -1,5 +1,7 @@
 """When a product may read its matrix ahead of what runs before it, and what a matrix keeps, on the CPU: the launchers are replaced."""
+import copy
 import os
+import pickle
 
 import pytest
 import torch
@@ -126,3 +128,23 @@ def test_the_thread_that_lets_the_next_kernel_begin_has_waited(source):
         assert "if (!ahead) pdl_wait();" in ahead and ahead[ahead.index("if (ahead) {"):].count("pdl_wait();") == 1
     else:
         assert "\n            pdl_wait();\n" in ahead                 # (at the loader's own level: on every way)
+
+
+@pytest.mark.parametrize("how", [copy.deepcopy, copy.copy, lambda m: pickle.loads(pickle.dumps(m))])
+def test_a_copy_of_a_matrix_lies_where_its_own_data_does(how):
+    """A copied model's products read the copy's memory, not that of a matrix which may be gone."""
+    for m in (fp8._empty((300, 1000), "cpu"), fp8._empty((5, 200, 130), "cpu"), fp8._empty((64, 40), "cpu", True)):
+        m.data.copy_(torch.arange(m.data.numel()) % 251)
+        c = how(m)
+        assert (c.shape, c.gated, c.rows, c.cols, c.outputs, c.total) == (m.shape, m.gated, m.rows, m.cols, m.outputs, m.total)
+        assert torch.equal(c.data, m.data) and c.fresh
+        assert c.packed[0] == c.data.data_ptr() == c.values.data_ptr() and c.packed[1] == c.scales.data_ptr() and c.packed[2] == m.packed[2]
+
+
+def test_a_matrix_copied_with_what_holds_it():
+    class Part:
+        pass
+    p = Part()
+    p.w = fp8._empty((300, 1000), "cpu")
+    q = copy.deepcopy(p)
+    assert q.w is not p.w and q.w.packed[0] == q.w.data.data_ptr() != p.w.packed[0]
