@@ -69,13 +69,18 @@ class Fp8Matrix:
     __slots__ = ("data", "shape", "gated", "rows", "cols", "outputs", "group_rows", "total", "device", "index", "packed", "stream", "fresh")
 
     def __init__(self, data: torch.Tensor, shape: tuple, gated: bool = False):
-        self.data, self.shape, self.gated = data, shape, gated
+        if len(shape) not in (2, 3) or shape[0] < 0 or shape[-2] < 0 or shape[-1] <= 0 or (gated and shape[-2] % 2):
+            raise KernelError(f"Fp8Matrix: {tuple(shape)} is no shape of rows or of experts' matrices" + (" with gate and partner in turn" if gated else ""))
+        self.data, self.shape, self.gated = data, tuple(shape), gated
         self.rows, self.cols = rows, cols = shape[-2], shape[-1]
         # how many results a row's product with this matrix has
         self.outputs = rows >> 1 if gated else rows
         # rows that an expert's matrix takes, and all of them
         self.group_rows = rows if len(shape) == 2 else (rows + 127) & -128
         self.total = rows if len(shape) == 2 else shape[0] * self.group_rows
+        if data.dtype != torch.uint8 or data.dim() != 1 or not data.is_contiguous() or data.numel() < _bytes(self.total, cols, self.total):
+            raise KernelError(f"Fp8Matrix: a matrix of shape {tuple(shape)} is {_bytes(self.total, cols, self.total)} bytes (uint8, one dimension, packed), "
+                              f"not {tuple(data.shape)} of {data.dtype}")
         self.device = data.device
         self.index = data.get_device()
         # What makes it ends on this stream without a fence, so a product right behind that, with another stream's product already

@@ -148,3 +148,17 @@ def test_a_matrix_copied_with_what_holds_it():
     p.w = fp8._empty((300, 1000), "cpu")
     q = copy.deepcopy(p)
     assert q.w is not p.w and q.w.packed[0] == q.w.data.data_ptr() != p.w.packed[0]
+
+
+@pytest.mark.parametrize("data", [torch.zeros(63 * 256 + 512, dtype=torch.uint8), torch.zeros(64 * 256 + 511, dtype=torch.uint8), torch.zeros(64 * 256 + 512),
+                                  torch.zeros(2 * (64 * 256 + 512), dtype=torch.uint8)[::2], torch.zeros(2, 64 * 256 + 512, dtype=torch.uint8)])
+def test_a_matrix_of_too_little_or_other_data_is_refused(data):
+    """64 rows of 256 columns: 64 * 256 bytes of values and 512 of scales."""
+    with pytest.raises(kernels.KernelError, match="Fp8Matrix"):
+        kernels.Fp8Matrix(data, (64, 256))
+
+
+@pytest.mark.parametrize("shape, gated", [((64,), False), ((2, 2, 2, 2), False), ((64, 0), False), ((63, 256), True), ((-1, 256), False)])
+def test_a_matrix_of_no_such_shape_is_refused(shape, gated):
+    with pytest.raises(kernels.KernelError, match="Fp8Matrix"):
+        kernels.Fp8Matrix(torch.zeros(1 << 16, dtype=torch.uint8), shape, gated)
