@@ -167,7 +167,7 @@ def fp8_quantize(x: torch.Tensor) -> Fp8Matrix:
 
 def fp8_gate_up(gate: torch.Tensor, up: torch.Tensor) -> Fp8Matrix:
     """The two matrices of a gated feed-forward, or of a stack of experts, in 8 bits, their rows one after the other in turn."""
-    if gate.shape != up.shape or gate.dtype != up.dtype or gate.device != up.device:
+    if gate.dim() not in (2, 3) or gate.shape != up.shape or gate.dtype != up.dtype or gate.device != up.device:
         raise KernelError(f"fp8_gate_up: two matrices of a kind are wanted, not {tuple(gate.shape)} {gate.dtype} and {tuple(up.shape)} {up.dtype}")
     m = fp8_quantize(torch.stack((gate, up), dim=-2).flatten(-3, -2))
     return Fp8Matrix(m.data, m.shape, True)

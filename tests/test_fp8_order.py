@@ -162,3 +162,8 @@ def test_a_matrix_of_too_little_or_other_data_is_refused(data):
 def test_a_matrix_of_no_such_shape_is_refused(shape, gated):
     with pytest.raises(kernels.KernelError, match="Fp8Matrix"):
         kernels.Fp8Matrix(torch.zeros(1 << 16, dtype=torch.uint8), shape, gated)
+
+
+def test_gate_and_partner_are_matrices():
+    with pytest.raises(kernels.KernelError, match="fp8_gate_up"):
+        kernels.fp8_gate_up(torch.zeros(64), torch.zeros(64))
