@@ -75,7 +75,7 @@ register_part("feedforward", "gated", GatedFeedForward)
 class DenseFeedForward(Part):
     """down(act(up(x) + b_up)) + b_down: one hidden layer, no gate, biases optional.  ``activation``: "relu2"
     (the square of relu), "gelu_tanh", "silu" or "none".  The products' float32 sums take bias and activation
-    in one row-wise pass."""
+    in one row-wise pass.  With matrices in 8-bit floating point what lies between is rounded once, from floats."""
 
     kind = "feedforward"
     graph_safe = True
@@ -101,8 +101,13 @@ class DenseFeedForward(Part):
 
     def forward(self, x: torch.Tensor, ctx) -> torch.Tensor:
         """x (tokens, hidden) -> (tokens, hidden) float32 (or partial sums when there is no bias to add)."""
+        fp8 = isinstance(self.w_up, kernels.Fp8Matrix)
+        if fp8 and self.b_up is None and self.activation in kernels.EXPERT_ACTS:
+            y = torch.empty((x.shape[0], self.hidden), dtype=torch.float32, device=x.device)
+            kernels.feedforward_fp8(x, self.w_up, self.w_down, y, self.activation)
+            return y
         up = linear(x, self.w_up, out_dtype=torch.float32, parts_ok=True)
-        act = torch.empty((x.shape[0], self.inter), dtype=ctx.dtype, device=x.device)
+        act = torch.empty((x.shape[0], self.inter), dtype=torch.float32 if fp8 else ctx.dtype, device=x.device)
         kernels.bias_act(up, self.b_up, self.activation, act)
         y = linear(act, self.w_down, out_dtype=torch.float32, parts_ok=True)
         if self.b_down is None:
