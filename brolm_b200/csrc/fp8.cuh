@@ -128,6 +128,7 @@ struct ProductCall {             // brolm_fp8_stream, brolm_fp8_gemm and, with t
     const void* raw;
     long long ld_raw;
     int raw_dtype;
+    int piece;                   // (stream) blocks of K that a float result is summed over before the sum goes to registers; 0: all
     int fresh;                   // (dense) W may be what the kernel before writes: it is not read before that has ended
 };
 static inline int round_first(const ProductCall* c) {

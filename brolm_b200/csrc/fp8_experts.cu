@@ -394,7 +394,7 @@ BROLM_API int brolm_fp8_experts(const ExpertsCall* c) {
     p.x = h.values; p.x_scales = h.scales; p.ldx = h.ldv; p.w = c->down; p.w_scales = c->down_scales; p.ldw = c->down_ld;
     p.y = c->pairs; p.y_scales = nullptr; p.ldy = c->N; p.out = 1; p.N = c->N; p.K = c->inter; p.epilogue = 0; p.act = 0; p.limit = 0.0f;
     // (the first product has waited before it lets this one begin, and so has the list been written)
-    p.scale = nullptr; p.group_rows = c->down_rows; p.down = 1; p.listed = 1;
+    p.scale = nullptr; p.group_rows = c->down_rows; p.down = 1; p.listed = 1; p.piece = c->piece;
     st = c->product(&p);
     if (st || !c->out) return st;
     const dim3 grid(T, (c->N + 4 * THREADS - 1) / (4 * THREADS)), block(THREADS);

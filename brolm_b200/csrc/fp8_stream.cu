@@ -13,6 +13,10 @@
 //             commits
 //   warps 2-5 an accumulator's lane is a row of W, its column a row of X: epilogue, Y[row of X][row of W]
 //
+// The tensor core cuts off where an fma rounds, so the sums of long slices drift (all terms positive, 18,432 along K: 1.1e-5 of the
+// result).  Float results of more than `piece` blocks of K are summed in pieces of that many, which the epilogue adds in registers, as
+// in tiles (PIECES; kernels of their own, for the registers): 1.3e-6.  Results in fewer bits are one piece.
+//
 // Dense: X has up to 128 rows.  Where W has fewer tiles of 128 rows than the device has SMs, K is cut into slices that are the
 // blocks of a cluster; their float sums are added in the order of the slices through the cluster's shared memory.
 // Experts: a list made on the device names for every tile of rows of X the expert whose matrix it meets, its first row and
@@ -53,6 +57,7 @@ struct StreamArgs {
     uint8_t* y_scales;       // (ROUND)
     int y_quads, last;       // last: the last tile of W, of which row_tiles counts pairs where two blocks are a team
     int per;                 // blocks of K of a slice (dense; the cluster's rank is the slice)
+    int piece;               // (PIECES) blocks of K that go into an accumulator
     const void* x;           // rows that are no 8-bit numbers yet (FUSED), elements apart
     long ldx;
     int x_wide, K;
@@ -167,9 +172,14 @@ constexpr int MOST = 2 * 8 * 32;         // rows' largest magnitudes: two rooms 
 
 // FUSED: 0 the rows are 8-bit numbers in memory; 1, 2: they are bfloat16, float numbers, and every block rounds what it needs.
 // ROUND: results are 8-bit rows (a kernel of its own: as a branch it cost the others 0.4 to 0.8 us a launch).
-template <int BT, int FUSED>
+// PIECES: a float result of many blocks of K is summed in pieces, which the epilogue adds: no slower (64 rows 18,432 x 18,432 61.1 us
+// for 61.4, 100 rows 4,608 x 36,864 in slices of 42 blocks 34.4 for 34.9) as long as its code is short: with each of a thread's sums
+// stored by the other forms' code 100 rows took 94 us for 68.
+template <int BT, int FUSED, bool PIECES>
 struct Shape {
-    static constexpr int THREADS = FUSED ? 320 : 192;                   // (eight warps that round, of which four have an epilogue)
+    // warps with an epilogue: 128 sums a thread are more registers than two blocks an SM leave it, so there eight warps have 64 each
+    static constexpr int LEAVING = PIECES && BT == 128 ? 8 : 4;
+    static constexpr int THREADS = FUSED || LEAVING == 8 ? 320 : 192;   // (FUSED: eight warps that round, of which four have an epilogue)
     static constexpr int X_BYTES = BT * BK;
     static constexpr int STAGE_BYTES = FUSED ? W_BYTES : W_BYTES + X_BYTES;      // multiples of 1024
     // accumulators and two pairs of scales in at most half of tensor memory, so that an SM holds two blocks
@@ -304,10 +314,10 @@ __device__ __forceinline__ bool rounded_results(const StreamArgs& g, uint32_t ac
     return true;
 }
 
-template <int BT, int EPI, bool EXPERTS, int FUSED, bool ROUND>
-__global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS, 2) fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w,
+template <int BT, int EPI, bool EXPERTS, int FUSED, bool ROUND, bool PIECES>
+__global__ void __launch_bounds__(Shape<BT, FUSED, PIECES>::THREADS, 2) fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w,
                                                              const __grid_constant__ CUtensorMap map_x, StreamArgs g) {
-    using S = Shape<BT, FUSED>;
+    using S = Shape<BT, FUSED, PIECES>;
     constexpr int ACCS = S::ACCS;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* base = smem_raw;
@@ -342,7 +352,7 @@ __global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS, 2) fp8_stream_kerne
         }
         for (int s = 0; s < 2; ++s) {
             mbar_init(acc_full0 + 8 * s, 1);
-            mbar_init(acc_empty0 + 8 * s, 4);
+            mbar_init(acc_empty0 + 8 * s, S::LEAVING);
         }
         mbar_init(x_ready, 8);
         mbar_init(ended, 1);
@@ -444,35 +454,38 @@ __global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS, 2) fp8_stream_kerne
             int s = 0, phase = 0, local = 0, set = 0;
             bool ok = true;
             int rt, group, row0, tile;
-            for (int item = first; item < g.items && lo < hi && ok; item += step, ++local) {
+            for (int item = first; item < g.items && lo < hi && ok; item += step) {
                 if (!find(item, rt, group, row0, tile)) break;
-                const int as = local % ACCS;
-                ok = wait_on(acc_empty0 + 8 * as, ((local / ACCS) & 1) ^ 1, give_up, 5);
-                if (FUSED && ok && local == 0) ok = wait_on(x_ready, 0, give_up, 6);
-                if (!ok) break;
-                fence_after_sync();
-                const uint32_t acc = tmem + as * BT;
                 uint32_t sfw = 0, sfx = 0;
-                for (int kb = lo; kb < hi; ++kb) {
-                    ok = kb > lo ? wait_one(full0 + 8 * s, phase, give_up, 2) : wait_on(full0 + 8 * s, phase, give_up, 2);
+                for (int from = lo, to; from < hi && ok; from = to, ++local) {
+                    to = PIECES ? min(hi, from + g.piece) : hi;
+                    const int as = local % ACCS;
+                    ok = wait_on(acc_empty0 + 8 * as, ((local / ACCS) & 1) ^ 1, give_up, 5);
+                    if (FUSED && ok && local == 0) ok = wait_on(x_ready, 0, give_up, 6);
                     if (!ok) break;
                     fence_after_sync();
-                    if ((kb & 3) == 0 || kb == lo) {
-                        sfw = tmem + ACCS * BT + 8 * set;
-                        sfx = sfw + 4;
-                        set ^= 1;
-                        scales_to_tmem(sfw, desc_scales(scale0 + s * S::SCALES));
-                        scales_to_tmem(sfx, desc_scales(FUSED ? smem_u32(x_scales) + ((kb >> 2) - (lo >> 2)) * SF_TILE : scale0 + s * S::SCALES + SF_TILE));
-                    }
-                    const uint32_t idk = with_block(id, kb & 3, kb & 3);
-                    const uint64_t a = desc_kmajor(stage0 + s * S::STAGE_BYTES);
-                    const uint64_t b = desc_kmajor(FUSED ? smem_u32(x_blocks) + (kb - lo) * S::X_BYTES : stage0 + s * S::STAGE_BYTES + W_BYTES);
+                    const uint32_t acc = tmem + as * BT;
+                    for (int kb = from; kb < to; ++kb) {
+                        ok = kb > lo ? wait_one(full0 + 8 * s, phase, give_up, 2) : wait_on(full0 + 8 * s, phase, give_up, 2);
+                        if (!ok) break;
+                        fence_after_sync();
+                        if ((kb & 3) == 0 || kb == lo) {
+                            sfw = tmem + ACCS * BT + 8 * set;
+                            sfx = sfw + 4;
+                            set ^= 1;
+                            scales_to_tmem(sfw, desc_scales(scale0 + s * S::SCALES));
+                            scales_to_tmem(sfx, desc_scales(FUSED ? smem_u32(x_scales) + ((kb >> 2) - (lo >> 2)) * SF_TILE : scale0 + s * S::SCALES + SF_TILE));
+                        }
+                        const uint32_t idk = with_block(id, kb & 3, kb & 3);
+                        const uint64_t a = desc_kmajor(stage0 + s * S::STAGE_BYTES);
+                        const uint64_t b = desc_kmajor(FUSED ? smem_u32(x_blocks) + (kb - lo) * S::X_BYTES : stage0 + s * S::STAGE_BYTES + W_BYTES);
 #pragma unroll
-                    for (int k = 0; k < BK / 32; ++k) umma_mx(acc, a + 2 * k, b + 2 * k, idk, sfw, sfx, (kb > lo) | (k > 0));
-                    umma_commit(empty0 + 8 * s);
-                    if (++s == stages) { s = 0; phase ^= 1; }
+                        for (int k = 0; k < BK / 32; ++k) umma_mx(acc, a + 2 * k, b + 2 * k, idk, sfw, sfx, (kb > from) | (k > 0));
+                        umma_commit(empty0 + 8 * s);
+                        if (++s == stages) { s = 0; phase ^= 1; }
+                    }
+                    if (ok) umma_commit(acc_full0 + 8 * as);
                 }
-                if (ok) umma_commit(acc_full0 + 8 * as);
             }
             if (!ok) {                                      // products in flight end before their operands go
                 umma_commit(ended);
@@ -494,35 +507,16 @@ __global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS, 2) fp8_stream_kerne
         __syncwarp();
         if (team && warp < 6) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
         int local = 0, turn = 0, rt, group, row0, tile;
-        for (int item = first; item < g.items && lo < hi && warp < 6; item += step, ++local) {
+        for (int item = first; item < g.items && lo < hi && warp < 2 + S::LEAVING; item += step) {
             if (!find(item, rt, group, row0, tile)) break;
-            const int as = local % ACCS;
-            const bool ready = !*give_up && wait_on(acc_full0 + 8 * as, (local / ACCS) & 1, give_up, 3);
-            if (!__all_sync(0xffffffffu, ready)) break;
-            fence_after_sync();
-            const uint32_t acc = tmem + as * BT + ((uint32_t)(quarter * 32) << 16);
             const int rows = EXPERTS ? min(BT, g.offsets[group + 1] - row0) : g.M;
-            if constexpr (ROUND) {
-                if (!rounded_results<EPI, EXPERTS, BT>(g, acc, acc_empty0 + 8 * as, rows, row0, tile, rt, side, quarter, lane, most_of, joined, turn, give_up)) break;
-                continue;
-            }
             const int wide = (rows + 15) & ~15;
-            for (int c = 0; c < wide; c += 16) {
-                uint32_t v[16];
-                tmem_ld16(acc + c, v);
-                tmem_wait_ld();
-                if (c + 16 >= wide) {                           // all of this accumulator that is wanted is in registers
-                    fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(acc_empty0 + 8 * as);
-                }
-                float o[16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) o[i] = __uint_as_float(v[i]);
+            // sixteen rows of X, from row c on, of this lane's row of W: the epilogue
+            auto leave = [&](int c, float (&o)[16]) {
                 if (slices > 1) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) sums[(c + i) * BR + lrow] = o[i];
-                    continue;
+                    return;
                 }
                 if (EXPERTS && g.scale) {
 #pragma unroll
@@ -542,7 +536,12 @@ __global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS, 2) fp8_stream_kerne
 #pragma unroll
                     for (int i = 0; i < 16; ++i) o[i] = act_of(o[i], g.act);
                 }
-                if (col < g.N) {
+                if (PIECES && !EXPERTS) {                       // (floats; short code, of which there are up to eight copies)
+                    float* to = reinterpret_cast<float*>(g.y) + (c + first_row) * g.ldy + col;
+                    const int left = col < g.N ? rows - c - first_row : 0;
+#pragma unroll
+                    for (int i = 0; i < (EPI == EPI_GATED ? 8 : 16); ++i, to += row_step * g.ldy) if (i * row_step < left) *to = o[i];
+                } else if (col < g.N) {
 #pragma unroll
                     for (int i = 0; i < (EPI == EPI_GATED ? 8 : 16); ++i) {
                         const int r = c + first_row + i * row_step;
@@ -555,6 +554,57 @@ __global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS, 2) fp8_stream_kerne
                             put(g, at * g.ldy + col, o[i]);
                         }
                     }
+                }
+            };
+            constexpr int EACH = BT * 4 / S::LEAVING;           // rows of X of a warp (PIECES)
+            const int c0 = S::LEAVING == 8 && warp >= 6 ? EACH : 0;
+            float sum[PIECES ? EACH : 16];                      // PIECES: of the accumulators that have been, in their order
+#pragma unroll
+            for (int i = 0; i < (PIECES ? EACH : 0); ++i) sum[i] = 0.0f;
+            bool there = true;
+            for (int from = lo; from < hi; from = PIECES ? from + g.piece : hi, ++local) {
+                const int as = local % ACCS;
+                const bool ready = !*give_up && wait_on(acc_full0 + 8 * as, (local / ACCS) & 1, give_up, 3);
+                there = __all_sync(0xffffffffu, ready);
+                if (!there) break;
+                fence_after_sync();
+                const uint32_t acc = tmem + as * BT + ((uint32_t)(quarter * 32) << 16);
+                if constexpr (ROUND) {
+                    there = rounded_results<EPI, EXPERTS, BT>(g, acc, acc_empty0 + 8 * as, rows, row0, tile, rt, side, quarter, lane, most_of, joined, turn, give_up);
+                    continue;
+                }
+                auto take = [&](int c, float* o) {
+                    uint32_t v[16];
+                    tmem_ld16(acc + c, v);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[i] = PIECES ? o[i] + __uint_as_float(v[i]) : __uint_as_float(v[i]);
+                };
+                auto taken = [&]() {                            // all of this accumulator that is wanted is in registers
+                    fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(acc_empty0 + 8 * as);
+                };
+                if constexpr (PIECES) {
+#pragma unroll
+                    for (int c = 0; c < EACH; c += 16) if (c0 + c < wide) take(c0 + c, sum + c);
+                    taken();
+                } else {
+                    for (int c = 0; c < wide; c += 16) {
+                        take(c, sum);
+                        if (c + 16 >= wide) taken();
+                        leave(c, sum);
+                    }
+                }
+            }
+            if (!there) break;
+            if constexpr (PIECES) {
+#pragma unroll
+                for (int c = 0; c < EACH; c += 16) {
+                    float o[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[i] = sum[c + i];
+                    if (c0 + c < wide) leave(c0 + c, o);
                 }
             }
         }
@@ -614,9 +664,9 @@ __global__ void __launch_bounds__(Shape<BT, FUSED>::THREADS, 2) fp8_stream_kerne
     if (warp == 1) tmem_dealloc(tmem, S::TMEM_COLS);
 }
 
-template <int BT, int EPI, bool EXPERTS, int FUSED, bool ROUND>
+template <int BT, int EPI, bool EXPERTS, int FUSED, bool ROUND, bool PIECES>
 int launch(const CUtensorMap& mw, const CUtensorMap& mx, StreamArgs g, int slices, cudaStream_t stream) {
-    using S = Shape<BT, FUSED>;
+    using S = Shape<BT, FUSED, PIECES>;
     const int sms = device_sms();
     const bool split = slices > 1;
     const int members = split ? slices : ROUND && EPI == EPI_GATED ? 2 : 1;
@@ -634,7 +684,7 @@ int launch(const CUtensorMap& mw, const CUtensorMap& mx, StreamArgs g, int slice
     if (smem > room || (split && (size_t)stages * S::STAGE_BYTES < (size_t)BT * BR * 4)) return BROLM_ERR_TOO_LARGE;
     g.stages = stages;
     static OncePerDevice done;
-    const int st = allow_shared_memory(fp8_stream_kernel<BT, EPI, EXPERTS, FUSED, ROUND>, MORE, done);
+    const int st = allow_shared_memory(fp8_stream_kernel<BT, EPI, EXPERTS, FUSED, ROUND, PIECES>, MORE, done);
     if (st) return st;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
@@ -649,31 +699,33 @@ int launch(const CUtensorMap& mw, const CUtensorMap& mx, StreamArgs g, int slice
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = EXPERTS && members == 1 ? 1 : 2;
-    return (int)cudaLaunchKernelEx(&cfg, fp8_stream_kernel<BT, EPI, EXPERTS, FUSED, ROUND>, mw, mx, g);
+    return (int)cudaLaunchKernelEx(&cfg, fp8_stream_kernel<BT, EPI, EXPERTS, FUSED, ROUND, PIECES>, mw, mx, g);
 }
 
-template <int EPI, bool EXPERTS, bool ROUND>
+template <int EPI, bool EXPERTS, bool ROUND, bool PIECES>
 int dispatch(const CUtensorMap& mw, const CUtensorMap& mx, const StreamArgs& g, int bt, int slices, int fused, cudaStream_t stream) {
-    if constexpr (!EXPERTS) {
-        if (fused == 1) return launch<16, EPI, false, 1, ROUND>(mw, mx, g, slices, stream);
-        if (fused == 2) return launch<16, EPI, false, 2, ROUND>(mw, mx, g, slices, stream);
+    if constexpr (!EXPERTS && !PIECES) {
+        if (fused == 1) return launch<16, EPI, false, 1, ROUND, false>(mw, mx, g, slices, stream);
+        if (fused == 2) return launch<16, EPI, false, 2, ROUND, false>(mw, mx, g, slices, stream);
     }
-    if (bt == 16) return launch<16, EPI, EXPERTS, 0, ROUND>(mw, mx, g, slices, stream);
-    if (bt == 32) return launch<32, EPI, EXPERTS, 0, ROUND>(mw, mx, g, slices, stream);
+    if (bt == 16) return launch<16, EPI, EXPERTS, 0, ROUND, PIECES>(mw, mx, g, slices, stream);
+    if (bt == 32) return launch<32, EPI, EXPERTS, 0, ROUND, PIECES>(mw, mx, g, slices, stream);
     if constexpr (!EXPERTS) {
-        if (bt == 64) return launch<64, EPI, false, 0, ROUND>(mw, mx, g, slices, stream);
-        if constexpr (!ROUND) return launch<128, EPI, false, 0, false>(mw, mx, g, slices, stream);
+        if (bt == 64) return launch<64, EPI, false, 0, ROUND, PIECES>(mw, mx, g, slices, stream);
+        if constexpr (!ROUND) return launch<128, EPI, false, 0, false, PIECES>(mw, mx, g, slices, stream);
     }
     return BROLM_ERR_BAD_SIZE;
 }
+template <int EPI, bool EXPERTS>
+int dispatch(const CUtensorMap& mw, const CUtensorMap& mx, const StreamArgs& g, int bt, int slices, int fused, int out, cudaStream_t stream) {
+    if (out == 2) return dispatch<EPI, EXPERTS, true, false>(mw, mx, g, bt, slices, fused, stream);
+    if (out == 1 && g.piece > 0 && g.per > g.piece) return dispatch<EPI, EXPERTS, false, true>(mw, mx, g, bt, slices, fused, stream);
+    return dispatch<EPI, EXPERTS, false, false>(mw, mx, g, bt, slices, fused, stream);
+}
 template <bool EXPERTS>
 int dispatch(const CUtensorMap& mw, const CUtensorMap& mx, const StreamArgs& g, int bt, int slices, int fused, int epilogue, int out, cudaStream_t stream) {
-    if (epilogue == EPI_GATED) {
-        if (out == 2) return dispatch<EPI_GATED, EXPERTS, true>(mw, mx, g, bt, slices, fused, stream);
-        return dispatch<EPI_GATED, EXPERTS, false>(mw, mx, g, bt, slices, fused, stream);
-    }
-    if (out == 2) return dispatch<EPI_STORE, EXPERTS, true>(mw, mx, g, bt, slices, fused, stream);
-    return dispatch<EPI_STORE, EXPERTS, false>(mw, mx, g, bt, slices, fused, stream);
+    if (epilogue == EPI_GATED) return dispatch<EPI_GATED, EXPERTS>(mw, mx, g, bt, slices, fused, out, stream);
+    return dispatch<EPI_STORE, EXPERTS>(mw, mx, g, bt, slices, fused, out, stream);
 }
 
 }  // namespace
@@ -700,7 +752,7 @@ BROLM_API int brolm_fp8_stream(const fp8::ProductCall* c) {
     StreamArgs g = {};
     g.y = c->y; g.ldy = (long)c->ldy; g.M = M; g.N = N; g.out_f32 = c->out == 1; g.act = c->act; g.limit = c->limit;
     g.y_wide = ((uintptr_t)c->y & 15) == 0 && c->ldy % 4 == 0;
-    g.nkb = blocks_of(K); g.quads = quads_of(K);
+    g.nkb = blocks_of(K); g.quads = quads_of(K); g.piece = c->fused ? 0 : c->piece;
     g.w_scales = (const uint8_t*)c->w_scales; g.x_scales = (const uint8_t*)c->x_scales;
     g.last = (int)((w_rows + BR - 1) / BR - 1);
     if (c->out == 2) { g.y_scales = (uint8_t*)c->y_scales; g.y_quads = quads_of(N); }

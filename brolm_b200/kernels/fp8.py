@@ -40,7 +40,7 @@ _raw_stream, _device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDev
 # struct, packed here as C lays it out, and the checks of a call's arguments are one expression; which of them failed is found
 # out only then.
 _ROWS = struct.Struct("@4P3q5i")
-_PRODUCT = struct.Struct("@7P3q8ifi5P7i2Pqii")
+_PRODUCT = struct.Struct("@7P3q8ifi5P7i2Pqiii")
 _EXPERTS = struct.Struct("@13P5q14if")
 _NORM = struct.Struct("@7Pq3i4f")
 _functions: dict = {}
@@ -226,7 +226,7 @@ def residual_rmsnorm_fp8(h: torch.Tensor, y: torch.Tensor, post_weight: Optional
 STREAM_ROWS = 128        # up to as many rows W is streamed; more are tiles of 256 x 256
 FUSED_ROWS = 16          # up to as many rows the stream of W can round the rows itself ...
 _FUSED_BLOCKS = 24       # ... where a block keeps no more than as many blocks of K of them
-_PIECE = 32              # blocks of K that a float32 result is summed over before the sum goes to registers
+_PIECE = 32              # blocks of K that a float32 result is summed over, in tiles and streams, before the sum goes to registers
 _ACTS = {(gated, name): code for gated, table in ((True, ACTIVATIONS), (False, EXPERT_ACTS)) for name, code in table.items()}
 
 
@@ -315,9 +315,9 @@ def _rounded(M: int, K: int, w_rows: int, out: int, words: int, sms: int) -> tup
 _rounded = functools.lru_cache(maxsize=4096)(_rounded)
 
 
-def _pack(how: tuple, x, at: int, M: int, w: Fp8Matrix, y: tuple, out: int, act: int, limit: float, stream: int) -> bytes:
+def _pack(how: tuple, x, at: int, M: int, w: Fp8Matrix, y: tuple, out: int, act: int, limit: float, stream: int, piece: int) -> bytes:
     """A product's struct.  ``x``: (values, scales, stride) of rows in 8 bits, or (numbers, 0, stride, type) of rows that are
-    rounded on the way, into the scratch at ``at`` if not by the product itself."""
+    rounded on the way, into the scratch at ``at`` if not by the product itself.  ``piece``: of a float result that stays one."""
     K = w.cols
     fused, raw = 0, _THERE
     if len(x) == 4:
@@ -329,7 +329,7 @@ def _pack(how: tuple, x, at: int, M: int, w: Fp8Matrix, y: tuple, out: int, act:
             x = (at, at + ((M * ld + 511) & -512), ld)
     wv, ws, ldw = w.packed
     return _PRODUCT.pack(x[0], x[1], wv, ws, y[0], y[1], stream, x[2], ldw, y[2], M, w.outputs, K, 1 if w.gated else 0, act, out, fused, how[1], limit,
-                         *_NO_EXPERTS, *raw, 1 if w.fresh else 0)
+                         *_NO_EXPERTS, *raw, piece, 1 if w.fresh else 0)
 
 
 def _launched(stream: int, *matrices: Fp8Matrix) -> None:
@@ -360,7 +360,7 @@ def linear_fp8(x, w: Fp8Matrix, out: torch.Tensor, activation: str = "none", lim
             add_launches(1)
         x = (x.data_ptr(), 0, x.stride(0), x.dtype)
     stream = _raw_stream(device)
-    packed = _pack(how, x, at, M, w, (out.data_ptr(), 0, out.stride(0)), _OUT[out.dtype], act, limit, stream)
+    packed = _pack(how, x, at, M, w, (out.data_ptr(), 0, out.stride(0)), _OUT[out.dtype], act, limit, stream, _PIECE)
     if how[0]:
         _call("fp8_stream", "brolm_fp8_stream", packed, "linear_fp8")
     else:
@@ -395,8 +395,8 @@ def feedforward_fp8(x, gate_up: Fp8Matrix, down: Fp8Matrix, out: torch.Tensor, a
     ld = (inter + 15) & -16
     between = (at + x8, at + x8 + ((M * ld + 511) & -512), ld)
     stream = _raw_stream(device)
-    a = _pack(first, x, at, M, gate_up, (at + x8 + h8, 0, inter) if floats else between, 1 if floats else 2, act, limit, stream)
-    b = _pack(second, (at + x8 + h8, 0, inter, _F32) if floats else between, at + x8, M, down, (out.data_ptr(), 0, out.stride(0)), _OUT[out.dtype], 0, 0.0, stream)
+    a = _pack(first, x, at, M, gate_up, (at + x8 + h8, 0, inter) if floats else between, 1 if floats else 2, act, limit, stream, 0)
+    b = _pack(second, (at + x8 + h8, 0, inter, _F32) if floats else between, at + x8, M, down, (out.data_ptr(), 0, out.stride(0)), _OUT[out.dtype], 0, 0.0, stream, _PIECE)
     f = _functions.get("brolm_fp8_two")
     if f is None:
         f = _functions["brolm_fp8_two"] = _fn("fp8_rows", "brolm_fp8_two", [c_char_p, c_void_p, c_char_p, c_void_p])
