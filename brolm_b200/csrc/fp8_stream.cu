@@ -439,9 +439,9 @@ __global__ void __launch_bounds__(Shape<BT, FUSED, PIECES>::THREADS, 2) fp8_stre
                     more = item < g.items && find(item, rt, group, row0, tile);
                 }
             }
-            // The stream is asked for: the next kernel may move in.  One thread's word stands for the block's, so no other
-            // thread gives it: this one has waited, and what the next kernel reads ahead of its own wait (an experts' list, a
-            // matrix that is not new) is there by then.
+            // The stream is asked for: the next kernel may move in.  One thread's word stands for the block's, so none gives it
+            // that has not waited, as this one has: what the next kernel reads ahead of its own wait (an experts' list, a matrix
+            // that is not new) is there by then.
             pdl_trigger();
             if (*give_up) {
                 for (int j = max(0, it - stages); j < it; ++j) drain_on(full0 + 8 * (j % stages), (j / stages) & 1, give_up, 4);
@@ -503,6 +503,9 @@ __global__ void __launch_bounds__(Shape<BT, FUSED, PIECES>::THREADS, 2) fp8_stre
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(x_ready);
+            // (these four warps have waited, too, and have nothing else to do: the next kernel's stream begins sooner.  A product of
+            // one row, 2,304 x 9,216, 7.9 -> 7.15 us, of eight 8.6 -> 8.1.)
+            if (warp >= 6) pdl_trigger();
         }
         __syncwarp();
         if (team && warp < 6) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");

@@ -117,14 +117,19 @@ def test_what_a_product_says_of_its_matrix_is_what_it_found(device):
 
 @pytest.mark.parametrize("source", ["fp8_stream.cu", "fp8_gemm.cu"])
 def test_the_thread_that_lets_the_next_kernel_begin_has_waited(source):
-    """One thread's trigger stands for its block.  The products have one, the loader's, and the loader waits on every way to it
-    (in the stream on one of two: ahead of its first loads, or behind those of the matrix)."""
+    """One thread's trigger stands for its block.  The products have the loader's, and the loader waits on every way to it (in the
+    stream on one of two: ahead of its first loads, or behind those of the matrix); the stream also has that of the warps that round
+    rows, all of whose threads wait before they read one."""
     with open(os.path.join(CSRC, source)) as f:
         kernel = f.read().split("__global__", 1)[1].split("\n}\n", 1)[0]
-    assert kernel.count("pdl_trigger()") == 1
+    assert kernel.count("pdl_trigger()") == (2 if source == "fp8_stream.cu" else 1)
     loader = kernel[kernel.index("if (warp == 0) {"):kernel.index("} else if (warp == 1) {")]
     ahead = loader[:loader.index("pdl_trigger()")]
     if source == "fp8_stream.cu":
+        others = kernel[kernel.index("const int quarter = warp & 3;"):]
+        rounding = others[:others.index("pdl_trigger()")]
+        assert "\n        if (EXPERTS || FUSED) pdl_wait();\n        if (FUSED) {\n" in rounding and rounding.rindex("if (FUSED) {") < rounding.rindex("round_rows<")
+        assert "\n        }\n" not in rounding[rounding.index("if (FUSED) {"):]        # the trigger is in that branch
         assert "if (!ahead) pdl_wait();" in ahead and ahead[ahead.index("if (ahead) {"):].count("pdl_wait();") == 1
     else:
         assert "\n            pdl_wait();\n" in ahead                 # (at the loader's own level: on every way)
