@@ -34,6 +34,7 @@ _CODES = {_F32: 0, _BF16: 1}
 _OUT = {_BF16: 0, _F32: 1}
 _FUSED = {_BF16: 1, _F32: 2}
 _NO_CPU = "brolm_b200 kernels run on CUDA tensors only; there is no CPU path"
+_new_matrix = object.__new__
 _raw_stream, _device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 # A product of few rows is a few microseconds on the device, so what the host does for it counts: the launchers take one
@@ -69,26 +70,32 @@ class Fp8Matrix:
     __slots__ = ("data", "shape", "gated", "rows", "cols", "outputs", "group_rows", "total", "device", "index", "packed", "stream", "fresh")
 
     def __init__(self, data: torch.Tensor, shape: tuple, gated: bool = False):
+        shape = tuple(shape)
         if len(shape) not in (2, 3) or shape[0] < 0 or shape[-2] < 0 or shape[-1] <= 0 or (gated and shape[-2] % 2):
-            raise KernelError(f"Fp8Matrix: {tuple(shape)} is no shape of rows or of experts' matrices" + (" with gate and partner in turn" if gated else ""))
-        self.data, self.shape, self.gated = data, tuple(shape), gated
+            raise KernelError(f"Fp8Matrix: {shape} is no shape of rows or of experts' matrices" + (" with gate and partner in turn" if gated else ""))
+        rows = shape[0] if len(shape) == 2 else shape[0] * _round_up(shape[1], 128)
+        need = _bytes(rows, shape[-1], rows)
+        if data.dtype != torch.uint8 or data.dim() != 1 or not data.is_contiguous() or data.numel() < need:
+            raise KernelError(f"Fp8Matrix: a matrix of shape {shape} is {need} bytes (uint8, one dimension, packed), not {tuple(data.shape)} of {data.dtype}")
+        self._lay(data, shape, gated)
+
+    def _lay(self, data: torch.Tensor, shape: tuple, gated: bool) -> "Fp8Matrix":
+        self.data, self.shape, self.gated = data, shape, gated
         self.rows, self.cols = rows, cols = shape[-2], shape[-1]
         # how many results a row's product with this matrix has
         self.outputs = rows >> 1 if gated else rows
         # rows that an expert's matrix takes, and all of them
         self.group_rows = rows if len(shape) == 2 else (rows + 127) & -128
         self.total = rows if len(shape) == 2 else shape[0] * self.group_rows
-        if data.dtype != torch.uint8 or data.dim() != 1 or not data.is_contiguous() or data.numel() < _bytes(self.total, cols, self.total):
-            raise KernelError(f"Fp8Matrix: a matrix of shape {tuple(shape)} is {_bytes(self.total, cols, self.total)} bytes (uint8, one dimension, packed), "
-                              f"not {tuple(data.shape)} of {data.dtype}")
         self.device = data.device
-        self.index = data.get_device()
+        self.index = index = data.get_device()
         # What makes it ends on this stream without a fence, so a product right behind that, with another stream's product already
         # launched or none, must not read ahead.  Other streams reach the matrix through an event, which is behind its stores.
-        self.stream = _raw_stream(self.index) if self.index >= 0 else 0
+        self.stream = _raw_stream(index) if index >= 0 else 0
         self.fresh = True
         at, ld = data.data_ptr(), (cols + 15) & -16
         self.packed = (at, at + ((self.total * ld + 511) & -512), ld)
+        return self
 
     def __reduce__(self):
         return Fp8Matrix, (self.data, self.shape, self.gated)      # a copy has addresses of its own
@@ -125,7 +132,8 @@ def _bytes(rows: int, cols: int, scale_rows: int) -> int:
 
 def _empty(shape: tuple, device, gated: bool = False) -> Fp8Matrix:
     rows = shape[0] if len(shape) == 2 else shape[0] * _round_up(shape[1], 128)
-    return Fp8Matrix(torch.empty(_bytes(rows, shape[-1], rows), dtype=torch.uint8, device=device), shape, gated)
+    # (what the constructor asks holds here; asking costs the host 0.5 us)
+    return _new_matrix(Fp8Matrix)._lay(torch.empty(_bytes(rows, shape[-1], rows), dtype=torch.uint8, device=device), shape, gated)
 
 
 def _refuse(what: str, t: torch.Tensor, name: str, dim: int = 2) -> None:
