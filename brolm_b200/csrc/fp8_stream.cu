@@ -40,7 +40,7 @@ using namespace fp8;
 constexpr int BR = 128, BK = 128;
 constexpr int W_BYTES = BR * BK;
 constexpr int MAX_STAGES = 12;
-constexpr int FUSED_BLOCKS = 24;       // 48 KB of the rows, five stages beside them
+constexpr int FUSED_BLOCKS = 16;       // 32 KB of the rows, four stages beside them (six where no more than half of the SMs get a block)
 
 enum : int { EPI_STORE = 0, EPI_GATED = 1 };
 

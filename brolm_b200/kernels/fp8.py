@@ -233,7 +233,7 @@ def residual_rmsnorm_fp8(h: torch.Tensor, y: torch.Tensor, post_weight: Optional
 # --- products ----------------------------------------------------------------
 STREAM_ROWS = 128        # up to as many rows W is streamed; more are tiles of 256 x 256
 FUSED_ROWS = 16          # up to as many rows the stream of W can round the rows itself ...
-_FUSED_BLOCKS = 24       # ... where a block keeps no more than as many blocks of K of them
+_FUSED_BLOCKS = 16       # ... where a block keeps no more than as many blocks of K of them
 _PIECE = 32              # blocks of K that a float32 result is summed over, in tiles and streams, before the sum goes to registers
 _ACTS = {(gated, name): code for gated, table in ((True, ACTIVATIONS), (False, EXPERT_ACTS)) for name, code in table.items()}
 
@@ -254,8 +254,10 @@ def fp8_slices(tiles: int, nkb: int, sms: int) -> int:
 def fp8_fused(rows: int, nkb: int, slices: int, words: int) -> bool:
     """Whether the stream of W rounds the rows itself: every block those of its slice, four blocks of K of a row (``words`` words
     of sixteen bytes a lane: 2 for bfloat16, 4 for float32) a warp, eight warps with eight such words each in one round.  A
-    launch less, and every block's time: 8 bfloat16 rows 2,304 x 9,216 (slices of nine blocks) 8.8 us fused and 9.8 not, float32
-    rows 10.2 and 8.6, 18,432 x 2,304 (all eighteen) 13.4 and 12.9."""
+    launch less, and every block's time, whose ring the rows leave fewer stages.  Fused / apart in a captured loop, bfloat16 rows:
+    2,304 x 9,216 (slices of 9 blocks) 1 row 6.9 / 8.5 us, 8 rows 8.4 / 8.7; 5,000 x 11,000 (15) 4 rows 12.3 / 13.0; 18,432 x 2,048
+    (16) 1 row 10.1 / 10.5, 4 rows 10.7 / 10.6; x 2,304 (18) 11.1 / 10.8 and 11.9 / 10.8; x 2,944 (23) 13.9 / 12.6 and 14.8 / 12.7.
+    From Python, 1 row: 7.3 / 11.8 with 9 blocks, 11.1 / 11.8 with 18, 14.0 / 13.0 with 23."""
     per = (nkb + slices - 1) // slices
     return rows <= FUSED_ROWS and per <= _FUSED_BLOCKS and rows * ((per + 6) // 4) * words <= 64
 
