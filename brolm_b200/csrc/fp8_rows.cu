@@ -25,19 +25,20 @@ struct RowsArgs {
 // The row of the matrix that row r of x is.
 __device__ __forceinline__ long place_of(const RowsArgs& g, long r) { return g.group == g.group_pad ? r : r / g.group * g.group_pad + r % g.group; }
 
-// A warp has four blocks of a row at a time.  8,192 x 4,608 bfloat16 numbers take 24.8 us, 4.6 TB/s where a copy of them runs at
-// 5.5; two or four rows at a time (26.8, 28.6 us) or the next one's numbers asked for ahead (24.8 to 26.1) gained nothing.
+// A warp has four blocks of a row at a time.  8,192 x 4,608 bfloat16 numbers take 21.8 us, 5.2 TB/s where a copy of them runs at
+// 6.0; two or four rows at a time (26.8, 28.6 us where one took 24.8) or the next one's numbers asked for ahead (24.8 to 26.1) gained
+// nothing.
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(THREADS) quantize_kernel(RowsArgs g) {
     const int lane = threadIdx.x & 31;
     const long items = g.rows * g.quads;
     pdl_wait();
     // Products read a matrix that is not new before they wait for the kernel before them.  A kernel that writes a matrix lets
-    // nothing begin before its blocks have ended, and the matrix's first product waits for it like any reader (a fence here
-    // instead took 4 of 26 us); one that writes rows that a product waits for lets it begin at once.
+    // nothing begin before its blocks have ended, and products wait for it like any reader until one has been launched on its
+    // stream (a fence here instead took 4 of 26 us); one that writes rows that a product waits for lets it begin at once.
     if (g.early) pdl_trigger();
     for (long item = (long)blockIdx.x * WARPS + (threadIdx.x >> 5); item < items; item += (long)gridDim.x * WARPS) {
-        const long row = items <= 0xffffffffl ? (long)((uint32_t)item / (uint32_t)g.quads) : item / g.quads;    // (a long division is 70 instructions)
+        const long row = items <= 0xffffffffl ? (long)((uint32_t)item / (uint32_t)g.quads) : item / g.quads;    // (a division of 32 bits is much shorter)
         const int quad = (int)(item - row * g.quads), c = quad * 512 + lane * 16;
         const T* x = (const T*)g.x + row * g.ldx;
         Piece<T, WIDE> piece;

@@ -734,12 +734,12 @@ int dispatch(const CUtensorMap& mw, const CUtensorMap& mx, const StreamArgs& g, 
 }  // namespace
 
 // Y [M, N] = X W^T (epilogue 0, act 0 or the square of relu) or the gated activation of W's neighbouring rows (epilogue 1: W
-// has 2 N rows); out 0: bfloat16, 1: float, 2 (cut 1, M <= 64): 8 bits, ldy bytes between rows, a multiple of 16, for experts scales as
+// has 2 N rows); out 0: bfloat16, 1: float, summed in pieces of `piece` blocks of K (0: in one), 2 (cut 1, M <= 64): 8 bits, ldy bytes between rows, a multiple of 16, for experts scales as
 // x_scales has them.  X and W as brolm_fp8_quantize leaves them.
 // Dense (experts 0): M <= 128; K is cut into `cut` slices (1 to 8), none of which is empty.  fused 1, 2: X are bfloat16, float
 // numbers (ldx elements between rows, x_scales unused), M <= 16, and a slice has at most FUSED_BLOCKS blocks of 128 of K.
 // Experts: M pairs' rows in the order of their experts, W the experts' matrices, group_rows (a multiple of 128) rows each.  The
-// list (expert, first row) of tiles of `rows` (16 or 32) rows and what it stands on come from brolm_fp8_group; x_scales
+// list (expert, first row) of tiles of `rows` (16 or 32) rows and what it stands on come from brolm_fp8_experts; x_scales
 // has a tile of 128 rows for every tile of the list.  Y [M, N], or with `down` float [top, tokens, N]; `scale` (or null): a
 // number for every pair that multiplies its sums before the activation.
 BROLM_API int brolm_fp8_stream(const fp8::ProductCall* c) {
