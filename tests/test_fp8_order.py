@@ -122,17 +122,19 @@ def test_the_thread_that_lets_the_next_kernel_begin_has_waited(source):
     rows, all of whose threads wait before they read one."""
     with open(os.path.join(CSRC, source)) as f:
         kernel = f.read().split("__global__", 1)[1].split("\n}\n", 1)[0]
-    assert kernel.count("pdl_trigger()") == (2 if source == "fp8_stream.cu" else 1)
-    loader = kernel[kernel.index("if (warp == 0) {"):kernel.index("} else if (warp == 1) {")]
-    ahead = loader[:loader.index("pdl_trigger()")]
-    if source == "fp8_stream.cu":
-        others = kernel[kernel.index("const int quarter = warp & 3;"):]
-        rounding = others[:others.index("pdl_trigger()")]
-        assert "\n        if (EXPERTS || FUSED) pdl_wait();\n        if (FUSED) {\n" in rounding and rounding.rindex("if (FUSED) {") < rounding.rindex("round_rows<")
-        assert "\n        }\n" not in rounding[rounding.index("if (FUSED) {"):]        # the trigger is in that branch
-        assert "if (!ahead) pdl_wait();" in ahead and ahead[ahead.index("if (ahead) {"):].count("pdl_wait();") == 1
-    else:
-        assert "\n            pdl_wait();\n" in ahead                 # (at the loader's own level: on every way)
+    loader, rest = kernel[kernel.index("if (warp == 0) {"):].split("} else if (warp == 1) {", 1)
+    ahead = loader[:loader.rindex("pdl_trigger()")]
+    if source == "fp8_gemm.cu":
+        assert kernel.count("pdl_trigger()") == 1 and "\n            pdl_wait();\n" in ahead        # (at the loader's own level: on every way)
+        return
+    assert kernel.count("pdl_trigger()") == 3
+    wait = "auto wait = [&]() {\n                pdl_wait();\n                if (AT_ONCE) pdl_trigger();\n            };\n"
+    ways = ahead.split(wait)
+    assert len(ways) == 2 and "pdl_trigger()" not in ways[0] + ways[1]
+    assert ways[1].startswith("            if (!ahead) wait();\n") and ways[1][ways[1].index("if (ahead) {"):].count("\n                wait();\n") == 1
+    rounding = rest[rest.index("const int quarter = warp & 3;"):rest.index("pdl_trigger()")]
+    assert "\n        if (EXPERTS || FUSED) pdl_wait();\n        if (FUSED) {\n" in rounding
+    assert "\n        }\n" not in rounding[rounding.index("if (FUSED) {"):]        # the trigger is in that branch
 
 
 @pytest.mark.parametrize("how", [copy.deepcopy, copy.copy, lambda m: pickle.loads(pickle.dumps(m))])
